@@ -21,7 +21,7 @@ extern "C" {
 #endif
 
 /* element types */
-enum { VQ_F16 = 0, VQ_BF16 = 1, VQ_F32 = 2, VQ_U8 = 3, VQ_I32 = 4, VQ_U32 = 5 };
+enum { VQ_F16 = 0, VQ_BF16 = 1, VQ_F32 = 2, VQ_U8 = 3, VQ_I32 = 4, VQ_U32 = 5, VQ_I64 = 6, VQ_F64 = 7 };
 
 /* status codes */
 enum {
@@ -538,6 +538,33 @@ typedef struct vq_index_attend_args {
 } vq_index_attend_args;
 size_t vq_vecinfer_attend_indices_workspace(const vq_index_attend_args *a);
 int vq_vecinfer_attend_indices(const vq_index_attend_args *a);
+
+/* ---- rotary positions ------------------------------------------------------ */
+
+enum { VQ_ROTARY_HALF = 0 /* pairs (i, i + dims/2) */, VQ_ROTARY_INTERLEAVED = 1 /* pairs (2i, 2i + 1) */ };
+
+/* Queries and keys of S consecutive slots of B sequences turned by their positions, in one launch: channel pair i of a row at
+ * position p by the angle p * inv_freq[i] (formed in double), times attention_factor; channels dims .. D - 1 pass through.
+ * x[0] / x[1]: queries and keys (heads[w] == 0: none), [B, heads[w], S, D] with element strides x_strides[w] = {batch, head,
+ * token} and contiguous channels; out[w] likewise, either the very rows of x[w] (same address and strides) or apart from
+ * every input and from the other output.  inv_freq: device, dims / 2 angular frequencies, VQ_F64 or VQ_F32.  The position
+ * of row (b, s) is offset + positions[b * pos_stride_b + s * pos_stride_s] (positions device, VQ_I32 or VQ_I64, or NULL: 0)
+ * + s where add_index is set.  inverse: turns back (the transposed map times attention_factor).  The calls a host model makes of
+ * its rotary embedding in front of update_and_fetch; no counterpart in the reference, whose caches take keys already turned
+ * (veloxquant_mlx/cache/kivi_cache.py:230-262). */
+typedef struct vq_rotary_args {
+    const void *x[2];
+    void *out[2];
+    int64_t heads[2];
+    int64_t x_strides[2][3], out_strides[2][3];
+    int64_t B, S, D, dims;
+    const void *inv_freq;
+    const void *positions;
+    int64_t pos_stride_b, pos_stride_s, offset;
+    int32_t dtype, freq_dtype, pos_dtype, add_index, layout, inverse;
+    float attention_factor;
+} vq_rotary_args;
+int vq_rotary(const vq_rotary_args *args, void *stream);
 
 /* ---- SKVQ clipped group quantisation ------------------------------------- */
 

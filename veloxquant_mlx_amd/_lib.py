@@ -14,7 +14,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("VELOXQUANT_HIP_LIB", os.path.join(_HERE, "libveloxquant_hip.so"))
 
 # element tags (include/veloxquant_hip.h)
-VQ_F16, VQ_BF16, VQ_F32, VQ_U8, VQ_I32, VQ_U32 = 0, 1, 2, 3, 4, 5
+VQ_F16, VQ_BF16, VQ_F32, VQ_U8, VQ_I32, VQ_U32, VQ_I64, VQ_F64 = 0, 1, 2, 3, 4, 5, 6, 7
 VQ_AXIS_TOKEN, VQ_AXIS_CHANNEL = 0, 1
 VQ_V_CHANNEL_PACKED, VQ_V_TOKEN_PACKED = 0, 1
 VQ_ERR_INVALID, VQ_ERR_UNSUPPORTED, VQ_ERR_WORKSPACE, VQ_ERR_HIP = -1, -2, -3, -4
@@ -108,6 +108,20 @@ class KiviAppendArgs(C.Structure):
     ]
 
 
+class RotaryArgs(C.Structure):
+    """Mirror of ``vq_rotary_args``."""
+
+    _fields_ = [
+        ("x", vp * 2), ("out", vp * 2), ("heads", i64 * 2),
+        ("x_strides", i64 * 3 * 2), ("out_strides", i64 * 3 * 2),
+        ("B", i64), ("S", i64), ("D", i64), ("dims", i64),
+        ("inv_freq", vp), ("positions", vp),
+        ("pos_stride_b", i64), ("pos_stride_s", i64), ("offset", i64),
+        ("dtype", i32), ("freq_dtype", i32), ("pos_dtype", i32), ("add_index", i32), ("layout", i32), ("inverse", i32),
+        ("attention_factor", f32),
+    ]
+
+
 _SIGNATURES = {
     "vq_abi_version": (i32, []),
     "vq_last_error": (i32, [C.c_char_p, sz]),
@@ -149,6 +163,7 @@ _SIGNATURES = {
     "vq_kivi_attend_ext": (i32, [C.POINTER(AttendArgs), C.POINTER(AttendExt)]),
     "vq_kivi_attend_static": (i32, [C.POINTER(AttendArgs)]),
     "vq_kivi_prefill_tiles": (i32, [C.POINTER(AttendArgs), i64, i64]),
+    "vq_rotary": (i32, [C.POINTER(RotaryArgs), vp]),
     "vq_vecinfer_attend_workspace": (sz, [C.POINTER(LutAttendArgs)]),
     "vq_vecinfer_attend": (i32, [C.POINTER(LutAttendArgs)]),
     "vq_vecinfer_attend_indices_workspace": (sz, [C.POINTER(IndexAttendArgs)]),

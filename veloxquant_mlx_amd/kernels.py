@@ -16,7 +16,7 @@ import torch
 from torch.autograd import forward_ad as _forward_ad
 
 from . import _lib
-from ._lib import (VQ_AXIS_CHANNEL, VQ_AXIS_TOKEN, VQ_BF16, VQ_F16, VQ_F32, VQ_I32, VQ_U8,
+from ._lib import (VQ_AXIS_CHANNEL, VQ_AXIS_TOKEN, VQ_BF16, VQ_F16, VQ_F32, VQ_F64, VQ_I32, VQ_I64, VQ_U8,
                    VQ_V_CHANNEL_PACKED, VQ_V_TOKEN_PACKED, AttendArgs, IndexAttendArgs, LutAttendArgs)
 
 _FLOAT_TAG = {torch.float16: VQ_F16, torch.bfloat16: VQ_BF16, torch.float32: VQ_F32}
@@ -54,6 +54,17 @@ def _need_gpu(name: str, *tensors: torch.Tensor) -> None:
         if not t.is_cuda:
             raise RuntimeError(f"{name}: tensors must live on a ROCm device (got {t.device}); "
                                "there is no CPU path")
+
+
+def _launch_on(device: torch.device, call) -> None:
+    """Run a library call with ``device`` as the current one (a launch goes to the current device, whose default stream has
+    the same handle on every device) and raise what it returns."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        rc = call()
+    else:
+        with torch.cuda.device(device):
+            rc = call()
+    _lib.check(rc)
 
 
 def _ftag(name: str, t: torch.Tensor) -> int:
@@ -1438,7 +1449,110 @@ __all__ = [
     "kv_tail_append", "kivi_cache_append", "attend_fixed_order",
     "kivi_packed_attend", "scalar_fused_decode_attend", "scalar_fused_decode_attend_batched",
     "scalar_predecoded_attend", "flash_prefill_attend",
+    "rotary_embed",
 ]
+
+
+# ---------------------------------------------------------------------------
+# rotary positions
+# ---------------------------------------------------------------------------
+
+def _extent(t: torch.Tensor) -> tuple[int, int]:
+    """First and one past the last byte of the elements a (non-empty) tensor spans."""
+    lo = t.data_ptr()
+    return lo, lo + (sum((n - 1) * st for n, st in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
+def _same_rows(a: torch.Tensor, b: torch.Tensor) -> bool:
+    return a.data_ptr() == b.data_ptr() and all(x == y or n < 2 for x, y, n in zip(a.stride(), b.stride(), a.shape))
+
+
+def rotary_embed(q: torch.Tensor, k: torch.Tensor | None = None, *, inv_freq: torch.Tensor, offset: int | torch.Tensor = 0,
+                 positions: torch.Tensor | None = None, traditional: bool = False, attention_factor: float = 1.0,
+                 inverse: bool = False, out: torch.Tensor | None = None, k_out: torch.Tensor | None = None):
+    """Rotary positions: channel pair ``i`` of a row at position ``p`` turned by ``p * inv_freq[i]`` and scaled by
+    ``attention_factor``, queries and keys in one launch.  Returns ``q'`` or ``(q', k')``.
+
+    ``q [B,Hq,S,D]`` and ``k [B,Hk,S,D]`` (float16, bfloat16 or float32, one dtype) may be views of any strides, a
+    transposed projection for one; channels must be adjacent, or they are copied first.  ``inv_freq``: ``dims / 2`` angular
+    frequencies, float64 or float32 on the device; channels past ``dims = 2 * len(inv_freq)`` pass through.  Pairs are
+    ``(i, i + dims/2)``, with ``traditional`` ``(2i, 2i + 1)``.  Positions: row ``s`` of sequence ``b`` is at ``offset + s``
+    (an int, or an int32 / int64 tensor ``[B]`` or of one element on the device), or at ``positions[b, s]`` (int32 / int64,
+    ``[S]``, ``[B,S]`` or ``[1,S]``, on the device; then ``offset`` is an int that is added).  Angles are formed in
+    float64, so far positions keep theirs.  ``out`` / ``k_out`` receive the rows (any strides over adjacent channels; the input
+    itself, to turn in place, or memory apart from both inputs and the other output: rows of a cache, for one); new tensors
+    are contiguous.  ``inverse=True`` turns back; times ``attention_factor`` that is the transposed map, the gradient of the
+    forward call (this package's functions record none)."""
+    name = "rotary_embed"
+    given = [(q, out, "q")] if k is None else [(q, out, "q"), (k, k_out, "k")]
+    if k is None and k_out is not None:
+        raise ValueError(f"{name}: k_out without k")
+    for t, _, what in given:
+        if t.ndim != 4:
+            raise ValueError(f"{name}: {what} must be [B, H, S, D], got {tuple(t.shape)}")
+    _need_gpu(name, *(t for t, _, _ in given), inv_freq)
+    B, _, S, D = q.shape
+    tag = _ftag(name, q)
+    if k is not None and (k.dtype != q.dtype or k.device != q.device or (k.shape[0], *k.shape[2:]) != (B, S, D)):
+        raise ValueError(f"{name}: k must be [{B}, H, {S}, {D}] in {q.dtype} on {q.device}, got {tuple(k.shape)} in {k.dtype} on {k.device}")
+    if inv_freq.ndim != 1 or inv_freq.dtype not in (torch.float64, torch.float32) or inv_freq.device != q.device:
+        raise ValueError(f"{name}: inv_freq must be float64 or float32 [dims / 2] on {q.device}")
+    dims = 2 * inv_freq.numel()
+    if not 2 <= dims <= D:
+        raise ValueError(f"{name}: {inv_freq.numel()} frequencies turn {dims} channels of {D}")
+    inv_freq = inv_freq.contiguous()
+    a = _lib.RotaryArgs()
+    a.B, a.S, a.D, a.dims, a.dtype = B, S, D, dims, tag
+    a.inv_freq, a.freq_dtype = inv_freq.data_ptr(), VQ_F64 if inv_freq.dtype == torch.float64 else VQ_F32
+    a.layout, a.inverse, a.attention_factor = int(bool(traditional)), int(bool(inverse)), float(attention_factor)
+    at = positions if positions is not None else offset if isinstance(offset, torch.Tensor) else None
+    if positions is not None and isinstance(offset, torch.Tensor):
+        raise ValueError(f"{name}: with positions, offset is an int")
+    if at is not None:
+        if at.dtype not in (torch.int32, torch.int64) or at.device != q.device:
+            raise ValueError(f"{name}: positions and offsets must be int32 or int64 on {q.device}, got {at.dtype} on {at.device}")
+        a.pos_dtype = VQ_I64 if at.dtype == torch.int64 else VQ_I32
+        if positions is None:
+            if at.numel() != 1 and tuple(at.shape) != (B,):
+                raise ValueError(f"{name}: offset must have one entry or be [{B}], got {tuple(at.shape)}")
+            a.pos_stride_b, a.pos_stride_s, a.add_index = (0 if at.numel() == 1 else at.stride(0)), 0, 1
+        else:
+            shape = (1,) * (2 - at.ndim) + tuple(at.shape)
+            if at.ndim not in (1, 2) or shape[0] not in (1, B) or shape[1] != S:
+                raise ValueError(f"{name}: positions must be [{S}] or [{B}, {S}], got {tuple(at.shape)}")
+            a.pos_stride_b, a.pos_stride_s = (0 if shape[0] == 1 else at.stride(0)), at.stride(-1)
+            a.offset = int(offset)
+        a.positions = at.data_ptr()
+    else:
+        a.offset, a.add_index = int(offset), 1
+    rows, results = [], []
+    for t, o, what in given:
+        if t.stride(3) != 1 and D > 1:
+            t = t.contiguous()
+        if o is None:
+            o = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+        elif o.shape != t.shape or o.dtype != t.dtype or o.device != t.device or (D > 1 and o.stride(3) != 1):
+            raise ValueError(f"{name}: the output for {what} must be {tuple(t.shape)} in {t.dtype} on {t.device} with adjacent channels")
+        elif any(n > 1 and st == 0 for n, st in zip(o.shape, o.stride())):
+            raise ValueError(f"{name}: rows of the output for {what} share memory")
+        rows.append(t)
+        results.append(o)
+    if all(t.numel() == 0 for t in rows):
+        return results[0] if k is None else tuple(results)
+    live = [i for i, t in enumerate(rows) if t.numel()]
+    in_place = [i in live and _same_rows(rows[i], results[i]) for i in range(len(rows))]
+    for i in live:
+        lo, hi = _extent(results[i])
+        for j in live:
+            others = [] if in_place[i] and (i == j or in_place[j]) else [rows[j]] + ([results[j]] if i != j else [])
+            if any(lo < e and s < hi for s, e in map(_extent, others)):
+                raise ValueError(f"{name}: the output for {given[i][2]} overlaps other rows of the call (it may only be its input itself)")
+    for i in live:
+        a.x[i], a.out[i], a.heads[i] = rows[i].data_ptr(), results[i].data_ptr(), rows[i].shape[1]
+        for d in range(3):
+            a.x_strides[i][d], a.out_strides[i][d] = rows[i].stride(d), results[i].stride(d)
+    _launch_on(q.device, lambda: _lib.load().vq_rotary(a, _stream(q)))
+    return results[0] if k is None else tuple(results)
 
 
 # ---------------------------------------------------------------------------
