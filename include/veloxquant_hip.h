@@ -539,6 +539,58 @@ typedef struct vq_index_attend_args {
 size_t vq_vecinfer_attend_indices_workspace(const vq_index_attend_args *a);
 int vq_vecinfer_attend_indices(const vq_index_attend_args *a);
 
+/* ---- attention over a shared prefix, differential attention ------------------- */
+
+/* Keys and values of a batch: n_packed quantised slots as vq_kivi_quant_pack lays them out (buffers of cap_tokens tokens per
+ * (sequence, kv head)), then n_tail plain rows, element (b, h, t, d) of the plain keys at k_tail + b k_strides[0] +
+ * h k_strides[1] + t k_strides[2] + d, of the values likewise.  A packed slot stands for the fp16 number code * scale + zero
+ * (the form in which the reference's cache holds it, veloxquant_mlx/cache/kivi_cache.py:198-201). */
+typedef struct vq_kv_store {
+    const void *k_packed, *k_scale, *k_zero, *v_packed, *v_scale, *v_zero;
+    int64_t n_packed, cap_tokens;
+    const void *k_tail, *v_tail;
+    int64_t n_tail;
+    int64_t k_strides[3], v_strides[3];
+} vq_kv_store;
+
+typedef struct vq_store_attend_args {
+    /* queries / output: [B, Hq, Sq, D] contiguous, dtype VQ_F16 / VQ_BF16 / VQ_F32; D <= 256 */
+    const void *q;
+    void *out;
+    int64_t B, Hq, Hkv, Sq, D;
+    vq_kv_store prefix;   /* one sequence, seen by all (vq_differential_attend: no slots) */
+    vq_kv_store own;      /* B sequences, each behind the prefix; no slots is allowed beside a prefix */
+    /* Optional: live slots of every own store, int64 [B] on the device: sequence b sees its first min(seq_lens[b],
+     * n_packed + n_tail), its queries align to the end of those. */
+    const int64_t *seq_lens;
+    /* vq_differential_attend: the second map's weight, float [Hq] (lam_stride 1) or one value (0), on the device; optional
+     * weight [D] of the norm of every head's output (norm_dtype VQ_F32 / VQ_F16 / VQ_BF16) */
+    const float *lam;
+    int64_t lam_stride;
+    const void *norm_weight;
+    void *workspace;      /* vq_..._workspace(args) bytes, 16-byte aligned; 0: may be NULL */
+    size_t workspace_bytes;
+    void *stream;
+    int64_t sliding_window;   /* > 0: a query sees only that many last slots up to its own position */
+    int32_t dtype, tail_dtype, norm_dtype;
+    int32_t pack_bits, group, meta_dtype, v_layout;   /* of both stores' packed slots */
+    int32_t causal;
+    float scale, norm_eps, gain;
+} vq_store_attend_args;
+
+/* softmax(scale q k^T) v of every sequence's queries over [prefix | its own slots], GQA by repeat-interleave, queries aligned to
+ * the end.  The prefix is read once for the whole batch: its keys and values meet the query rows of all sequences that
+ * share a kv head as one matrix product; each sequence's own slots meet its own rows, and the parts are merged.  No
+ * counterpart in the reference (a batch over one prompt holds the prompt once a sequence there). */
+size_t vq_shared_prefix_attend_workspace(const vq_store_attend_args *a);
+int vq_shared_prefix_attend(const vq_store_attend_args *a);
+
+/* (softmax(scale q1 k1^T) - lam softmax(scale q2 k2^T)) v with q1, k1 the first and q2, k2 the second D / 2 channels of the
+ * rows, v of D channels; then gain * o, or with a norm_weight gain * norm_weight * o / sqrt(mean(o^2) + norm_eps) over a
+ * head's channels.  Both maps' scores and sums are formed in one pass over the slots.  No counterpart in the reference. */
+size_t vq_differential_attend_workspace(const vq_store_attend_args *a);
+int vq_differential_attend(const vq_store_attend_args *a);
+
 /* ---- rotary positions ------------------------------------------------------ */
 
 enum { VQ_ROTARY_HALF = 0 /* pairs (i, i + dims/2) */, VQ_ROTARY_INTERLEAVED = 1 /* pairs (2i, 2i + 1) */ };

@@ -1,0 +1,183 @@
+"""``shared_prefix_attend`` against attention over the concatenated slots in 64 bits."""
+
+import math
+
+import pytest
+import torch
+
+from tests._gpu import gpu, require_gpu
+from tests._spans import attend, close, seen, store
+from veloxquant_mlx_amd import kernels as K
+
+pytestmark = gpu
+F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+
+
+def _weights_rounding(dtype, packed):
+    """Weights are rounded to the type of the products: fp16 over packed slots, else that of the rows; float32 rows: not at all."""
+    return 0.0 if dtype == F32 else torch.finfo(F16 if packed else dtype).eps / 2
+
+
+def _case(B, Hq, Hkv, D, prefix, own, Sq=1, *, bits=4, group=32, v_layout="token", dtype=F16, meta=F16, causal=True, lens=None, window=0,
+          spare=40, view=False, seed=0):
+    kw = dict(bits=bits, group=group, v_layout=v_layout, dtype=dtype, meta=meta, spare=spare, view=view)
+    p, pk, pv = store(1, Hkv, *prefix, D, seed=seed + 1, **kw)
+    o, ok, ov = store(B, Hkv, *own, D, seed=seed + 2, **kw)
+    q = torch.randn((B, Hq, Sq, D), generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda").to(dtype)
+    scale = 1 / math.sqrt(D)
+    lens = None if lens is None else torch.tensor(lens, device="cuda")
+    got = K.shared_prefix_attend(q, p, **o, scale=scale, causal=causal, seq_lens=lens, sliding_window=window)
+    mask = seen(B, Sq, pk.shape[2], ok.shape[2], lens, causal, window)
+    want, far = attend(q, torch.cat([pk.expand(B, -1, -1, -1), ok], 2), torch.cat([pv.expand(B, -1, -1, -1), ov], 2), mask, scale,
+                       _weights_rounding(dtype, prefix[0] + own[0] > 0))
+    assert got.shape == q.shape and got.dtype == q.dtype
+    close(got, want, far)
+    return q, p, o, got
+
+
+@pytest.mark.parametrize("bits,group", [(2, 32), (4, 32), (4, 64), (2, 128)])
+@pytest.mark.parametrize("B,Hq,Hkv,D,prefix,own", [
+    (1, 1, 1, 128, (128, 0), (0, 1)), (3, 8, 2, 128, (256, 7), (0, 33)), (5, 12, 4, 256, (640, 60), (128, 130)), (2, 14, 2, 64, (384, 1), (128, 5)),
+    (7, 32, 8, 128, (1152, 129), (256, 64)), (2, 4, 4, 128, (128, 0), (128, 0)), (33, 7, 1, 128, (128, 63), (0, 2))])
+def test_packed(B, Hq, Hkv, D, prefix, own, bits, group):
+    require_gpu()
+    if group > D:
+        pytest.skip("value groups are at most a head")
+    _case(B, Hq, Hkv, D, prefix, own, bits=bits, group=group)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("B,Hq,Hkv,D,n,own,Sq", [
+    (1, 2, 1, 128, 1, 1, 1), (4, 8, 2, 64, 65, 31, 1), (2, 9, 3, 128, 257, 100, 5), (3, 12, 4, 256, 500, 64, 3), (2, 6, 3, 80, 70, 9, 2),
+    (6, 40, 10, 128, 1000, 1, 1), (130, 4, 1, 64, 97, 3, 1), (2, 4, 2, 128, 300, 200, 200), (1, 64, 1, 128, 130, 40, 7)])
+def test_plain_rows(dtype, B, Hq, Hkv, D, n, own, Sq):
+    require_gpu()
+    _case(B, Hq, Hkv, D, (0, n), (0, own), Sq, dtype=dtype, view=True)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(bits=3, group=32, v_layout="channel"), dict(bits=8, group=32), dict(bits=1, group=32), dict(bits=4, v_layout="channel"),
+    dict(bits=4, meta=F32), dict(bits=4, group=16), dict(bits=4, dtype=F32), dict(bits=4, dtype=BF16), dict(bits=2, dtype=BF16, group=64)])
+def test_other_stores(kw):
+    require_gpu()
+    _case(3, 8, 2, 128, (256, 9), (128, 20), 2, **kw)
+
+
+@pytest.mark.parametrize("dtype,prefix,own", [(F16, (256, 10), (64, 50)), (BF16, (0, 300), (0, 114)), (F32, (64, 9), (32, 40))])
+@pytest.mark.parametrize("causal,window,lens,Sq", [
+    (False, 0, None, 4), (True, 0, [114, 1, 57], 1), (True, 0, [114, 3, 57], 4), (True, 0, [0, 114, 64], 1), (True, 0, [2, 0, 63], 6),
+    (False, 0, [0, 114, 65], 3), (True, 50, None, 4), (True, 200, [114, 1, 60], 2), (False, 100, [114, 20, 60], 2), (True, 1, [0, 5, 114], 1),
+    (True, 0, [-3, 500, 114], 1)])
+def test_masks(dtype, prefix, own, causal, window, lens, Sq):
+    require_gpu()
+    if dtype == F32:
+        lens = None if lens is None else [min(n, 72) for n in lens]
+    _case(3, 8, 2, 128, prefix, own, Sq, dtype=dtype, causal=causal, window=window, lens=lens)
+
+
+def test_without_own_slots_or_without_a_prefix():
+    require_gpu()
+    _case(3, 8, 2, 128, (256, 9), (0, 0), causal=False)
+    _case(3, 8, 2, 128, (0, 0), (128, 9), 3)
+    _case(2, 8, 2, 128, (0, 0), (0, 40), lens=[0, 40])       # a sequence that sees nothing: zero
+    q, p, o, got = _case(2, 8, 2, 128, (0, 0), (0, 40), lens=[0, 40], seed=5)
+    assert bool((got[0] == 0).all())
+
+
+def test_far_scores_and_equal_ones():
+    """Rows whose scores lie hundreds apart, and rows of equal scores."""
+    require_gpu()
+    B, H, D, n = 2, 4, 128, 400
+    q = torch.randn((B, H, 1, D), device="cuda").half() * 30
+    k, v = torch.randn((1, H, n, D), device="cuda").half() * 5, torch.randn((1, H, n, D), device="cuda").half()
+    ok, ov = torch.randn((B, H, 50, D), device="cuda").half(), torch.randn((B, H, 50, D), device="cuda").half()
+    got = K.shared_prefix_attend(q, dict(k_tail=k, v_tail=v, n_tail=n), k_tail=ok, v_tail=ov, n_tail=50, scale=1.0)
+    mask = torch.ones((B, 1, n + 50), dtype=torch.bool, device="cuda")
+    kk, vv = torch.cat([k.expand(B, -1, -1, -1), ok], 2).double(), torch.cat([v.expand(B, -1, -1, -1), ov], 2).double()
+    close(got, *attend(q, kk, vv, mask, 1.0, 2.0 ** -11))
+    got = K.shared_prefix_attend(q * 0, dict(k_tail=k, v_tail=v, n_tail=n), k_tail=ok, v_tail=ov, n_tail=50, scale=1.0)
+    close(got, *attend(q * 0, kk, vv, mask, 1.0, 2.0 ** -11))
+
+
+def test_agrees_with_the_cache_held_per_sequence():
+    """The same slots, the prefix copied into every sequence, through the framework's own decode attention."""
+    require_gpu()
+    B, Hq, Hkv, D, nq = 4, 32, 8, 128, 512
+    q, p, o, got = _case(B, Hq, Hkv, D, (nq, 0), (128, 40), spare=0)
+    axis = dict(k_packed=2, k_scale=2, k_zero=2, v_packed=2, v_scale=3, v_zero=3)
+    both = {n: torch.cat([p[n].expand(B, -1, -1, -1), o[n]], ax).contiguous() for n, ax in axis.items()}
+    ref = K.kivi_packed_attend(q, **both, n_packed=nq + 128, bits=4, group_size=32, v_layout="token", k_tail=o["k_tail"], v_tail=o["v_tail"],
+                               n_tail=40, scale=1 / math.sqrt(D))
+    assert float((got.float() - ref.float()).abs().max()) <= 2e-3 * max(1.0, float(ref.abs().max()))
+
+
+def test_streams_graphs_and_out():
+    require_gpu()
+    B, Hq, Hkv, D = 6, 32, 8, 128
+    q, p, o, got = _case(B, Hq, Hkv, D, (512, 20), (128, 40))
+    call = dict(scale=1 / math.sqrt(D), causal=True)
+    out = torch.empty_like(q)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        K.shared_prefix_attend(q, p, **o, **call, out=out)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(out, got)
+    # two graphs captured one after the other and replayed at once share no scratch, nor does an eager call between
+    lens = torch.full((B,), 168, device="cuda")
+    outs = [torch.empty_like(q), torch.empty_like(q)]
+    graphs = []
+    for i in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            K.shared_prefix_attend(q if i == 0 else -q, p, **o, **call, seq_lens=lens, out=outs[i])
+        graphs.append(g)
+    for n in (168, 5, 130, 0):
+        lens.fill_(n)
+        torch.cuda.synchronize()
+        for t in outs:
+            t.zero_()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            graphs[1].replay()
+        graphs[0].replay()
+        eager = K.shared_prefix_attend(q, p, **o, **call, seq_lens=lens)
+        torch.cuda.current_stream().wait_stream(side)
+        assert torch.equal(outs[0], eager)
+        assert torch.equal(outs[1], K.shared_prefix_attend(-q, p, **o, **call, seq_lens=lens))
+        torch.cuda.synchronize()
+
+
+def test_rows_of_sequences_do_not_depend_on_each_other():
+    require_gpu()
+    q, p, o, got = _case(9, 8, 2, 128, (512, 3), (128, 17))
+    flip = {n: (t.flip(0) if isinstance(t, torch.Tensor) else t) for n, t in o.items()}
+    again = K.shared_prefix_attend(q.flip(0), p, **flip, scale=1 / math.sqrt(128), causal=True)
+    assert torch.equal(again.flip(0), got)
+
+
+def test_refusals():
+    require_gpu()
+    q, p, o, _ = _case(2, 8, 2, 128, (256, 9), (128, 20))
+    ok = dict(scale=0.1)
+    bf = {n: (t.to(BF16) if n in ("k_tail", "v_tail") else t) for n, t in o.items()}
+    for args, what in [
+            ((q[0], p, o), "4D"), ((q.double(), p, o), "dtype"), ((q[..., :64], p, o), "channels"), ((q[:, :3], p, o), "kv heads"),
+            ((q[:1], p, o), "batch"), ((q, {**p, "k_scale": None}, o), "must be given"), ((q, {**p, "group_size": 64}, o), "do not fit"),
+            ((q, {**p, "n_packed": 9999}, o), "do not fit"), ((q, p, {**o, "n_tail": 9999}), "does not fit"), ((q, p, {**o, "v_layout": "x"}), "v_layout"),
+            ((q, p, bf), "differ in plain rows"), ((q, {**p, "k_zero": p["k_zero"].float()}, o), "share one dtype"),
+            ((q, o, o), "batch"), ((q, p, {**o, "v_tail": o["v_tail"][:, :1]}), "alike"), ((q, p, {**o, "k_packed": o["k_packed"].cpu()}), "must live"),
+            ((q, {}, {}), "no key/value slots"), ((q, p, {**o, "n_tail": -1}), "negative")]:
+        with pytest.raises(ValueError, match=what):
+            K.shared_prefix_attend(args[0], args[1], **args[2], **ok)
+    p2 = store(1, 2, 256, 9, 128, bits=2)[0]
+    with pytest.raises(ValueError, match="differ in bits"):
+        K.shared_prefix_attend(q, p2, **o, **ok)
+    for extra, what in [(dict(seq_lens=torch.ones(3, dtype=torch.int64, device="cuda")), "seq_lens"), (dict(seq_lens=torch.ones(2, device="cuda")), "seq_lens"),
+                        (dict(out=q[:, :, :, ::2]), "out must"), (dict(out=torch.empty_like(q, dtype=F32)), "out must"), (dict(sliding_window=-1), "window")]:
+        with pytest.raises(ValueError, match=what):
+            K.shared_prefix_attend(q, p, **o, **{**ok, **extra})
+    long = torch.zeros((2, 8, 500, 128), dtype=F16, device="cuda")
+    with pytest.raises(ValueError, match="exceeds"):
+        K.shared_prefix_attend(long, p, **o, **ok, causal=True)
+    assert K.shared_prefix_attend(q[:, :, :0], p, **o, **ok).shape == (2, 8, 0, 128)

@@ -121,3 +121,19 @@ def test_entry_point_checks_rows():
     assert lib.vq_rotary(None, None) == _lib.VQ_ERR_INVALID
     for empty in (dict(B=0), dict(S=0)):
         assert lib.vq_rotary(_args(**empty), None) == 0
+
+
+@pytest.mark.parametrize("struct,mirror", [("vq_rotary_args", _lib.RotaryArgs), ("vq_kv_store", _lib.KVStore), ("vq_store_attend_args", _lib.StoreAttendArgs)])
+def test_structures_match_the_header(struct, mirror):
+    import os
+    import re
+    text = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "veloxquant_hip.h")).read()
+    body = text[text.index(f"typedef struct {struct} {{"):text.index(f"}} {struct};")]
+    body = re.sub(r"/\*.*?\*/", "", body, flags=re.S)
+    names = []
+    for decl in body.split(";"):
+        for part in decl.split("{")[-1].strip().split(","):
+            part = re.sub(r"\[.*?\]", "", part).strip()
+            if part:
+                names.append(re.findall(r"[A-Za-z_][A-Za-z0-9_]*", part)[-1])
+    assert names == [f[0] for f in mirror._fields_]

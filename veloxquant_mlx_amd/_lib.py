@@ -108,6 +108,35 @@ class KiviAppendArgs(C.Structure):
     ]
 
 
+class KVStore(C.Structure):
+    """Mirror of ``vq_kv_store``."""
+
+    _fields_ = [
+        ("k_packed", vp), ("k_scale", vp), ("k_zero", vp), ("v_packed", vp), ("v_scale", vp), ("v_zero", vp),
+        ("n_packed", i64), ("cap_tokens", i64),
+        ("k_tail", vp), ("v_tail", vp), ("n_tail", i64),
+        ("k_strides", i64 * 3), ("v_strides", i64 * 3),
+    ]
+
+
+class StoreAttendArgs(C.Structure):
+    """Mirror of ``vq_store_attend_args``."""
+
+    _fields_ = [
+        ("q", vp), ("out", vp),
+        ("B", i64), ("Hq", i64), ("Hkv", i64), ("Sq", i64), ("D", i64),
+        ("prefix", KVStore), ("own", KVStore),
+        ("seq_lens", vp),
+        ("lam", vp), ("lam_stride", i64), ("norm_weight", vp),
+        ("workspace", vp), ("workspace_bytes", sz), ("stream", vp),
+        ("sliding_window", i64),
+        ("dtype", i32), ("tail_dtype", i32), ("norm_dtype", i32),
+        ("pack_bits", i32), ("group", i32), ("meta_dtype", i32), ("v_layout", i32),
+        ("causal", i32),
+        ("scale", f32), ("norm_eps", f32), ("gain", f32),
+    ]
+
+
 class RotaryArgs(C.Structure):
     """Mirror of ``vq_rotary_args``."""
 
@@ -120,6 +149,14 @@ class RotaryArgs(C.Structure):
         ("dtype", i32), ("freq_dtype", i32), ("pos_dtype", i32), ("add_index", i32), ("layout", i32), ("inverse", i32),
         ("attention_factor", f32),
     ]
+
+
+# Argument blocks packed by ``struct`` in one go, as ATTEND_PACK: x, out, heads, x_strides, out_strides, ...
+STORE_PACK = "PPPPPPqqPPqqqqqqq"   # a KVStore
+STORE_ATTEND_PACK = struct.Struct("@PPqqqqq" + 2 * STORE_PACK + "PPqPPNPqiiiiiiiifff0q")
+assert STORE_ATTEND_PACK.size == C.sizeof(StoreAttendArgs)
+ROTARY_PACK = struct.Struct("@PPPPqqqqqqqqqqqqqqqqqqPPqqqiiiiiif0q")
+assert ROTARY_PACK.size == C.sizeof(RotaryArgs)
 
 
 _SIGNATURES = {
@@ -163,6 +200,10 @@ _SIGNATURES = {
     "vq_kivi_attend_ext": (i32, [C.POINTER(AttendArgs), C.POINTER(AttendExt)]),
     "vq_kivi_attend_static": (i32, [C.POINTER(AttendArgs)]),
     "vq_kivi_prefill_tiles": (i32, [C.POINTER(AttendArgs), i64, i64]),
+    "vq_shared_prefix_attend_workspace": (sz, [C.POINTER(StoreAttendArgs)]),
+    "vq_shared_prefix_attend": (i32, [C.POINTER(StoreAttendArgs)]),
+    "vq_differential_attend_workspace": (sz, [C.POINTER(StoreAttendArgs)]),
+    "vq_differential_attend": (i32, [C.POINTER(StoreAttendArgs)]),
     "vq_rotary": (i32, [C.POINTER(RotaryArgs), vp]),
     "vq_vecinfer_attend_workspace": (sz, [C.POINTER(LutAttendArgs)]),
     "vq_vecinfer_attend": (i32, [C.POINTER(LutAttendArgs)]),
@@ -191,6 +232,10 @@ def load():
             # the same entry points over a packed argument block (ATTEND_PACK), and its extension or None
             lib.attend_packed = C.CFUNCTYPE(i32, C.c_char_p, C.c_char_p)(("vq_kivi_attend_ext", lib))
             lib.attend_packed_workspace = C.CFUNCTYPE(sz, C.c_char_p, C.c_char_p)(("vq_kivi_attend_workspace_ext", lib))
+            lib.store_attend_packed, lib.store_attend_packed_workspace = (
+                {maps: C.CFUNCTYPE(res, C.c_char_p)((f"vq_{name}_attend{tail}", lib)) for maps, name in ((1, "shared_prefix"), (2, "differential"))}
+                for res, tail in ((i32, ""), (sz, "_workspace")))
+            lib.rotary_packed = C.CFUNCTYPE(i32, C.c_char_p, vp)(("vq_rotary", lib))
             _lib = lib
             return _lib
         except (OSError, AttributeError) as e:  # missing file or symbol

@@ -1449,8 +1449,195 @@ __all__ = [
     "kv_tail_append", "kivi_cache_append", "attend_fixed_order",
     "kivi_packed_attend", "scalar_fused_decode_attend", "scalar_fused_decode_attend_batched",
     "scalar_predecoded_attend", "flash_prefill_attend",
-    "rotary_embed",
+    "rotary_embed", "shared_prefix_attend", "differential_attend",
 ]
+
+
+# ---------------------------------------------------------------------------
+# attention over a shared prefix, differential attention
+# ---------------------------------------------------------------------------
+
+_NO_STORE = (0,) * 17
+
+
+def _store_fields(name, which, device, batch, k_packed=None, k_scale=None, k_zero=None, v_packed=None, v_scale=None, v_zero=None,
+                  n_packed=0, bits=4, group_size=32, v_layout="channel", k_tail=None, v_tail=None, n_tail=0):
+    """A store's fields of the argument block; ``(fields, Hkv, D, packed, tail dtype, keep)`` with ``packed`` = (bits, group,
+    meta tag, layout) or None and ``keep`` what has to live until the launch."""
+    n_packed, n_tail = int(n_packed or 0), int(n_tail or 0)
+    if n_packed < 0 or n_tail < 0:
+        raise ValueError(f"{name}: negative token count ({which})")
+    heads = channels = packed = tail = None
+    keep = []
+    fields = [0, 0, 0, 0, 0, 0, 0, 0]
+    if n_packed:
+        arrays = (k_packed, k_scale, k_zero, v_packed, v_scale, v_zero)
+        for t in arrays:
+            if t is None or not t.is_contiguous() or t.ndim != 4:
+                raise ValueError(f"{name}: packed tensors ({which}) must be given, 4D and contiguous")
+            if t.device != device:
+                raise ValueError(f"{name}: packed tensors ({which}) must live on {device}, got {t.device}")
+        bits, g = int(bits), int(group_size)
+        if not 1 <= bits <= 8 or g < 1 or v_layout not in _V_LAYOUT:
+            raise ValueError(f"{name}: bits={bits}, group_size={g}, v_layout={v_layout!r} ({which})")
+        meta = k_scale.dtype
+        if meta not in (torch.float16, torch.float32) or any(t.dtype != meta for t in (k_zero, v_scale, v_zero)):
+            raise ValueError(f"{name}: scale/zero ({which}) must share one dtype, float16 or float32")
+        if k_packed.element_size() != 4 or v_packed.element_size() != 4:
+            raise ValueError(f"{name}: packed codes ({which}) must be 32-bit words")
+        per = 32 // bits
+        B, heads, cap, W = k_packed.shape
+        channels = k_scale.shape[3]
+        GV = -(-channels // g)
+        k_meta = (B, heads, -(-cap // g), channels)
+        if v_layout == "token":
+            want = ((B, heads, cap // per, channels), (B, heads, GV, cap))
+        else:
+            want = ((B, heads, cap, W), (B, heads, cap, GV))
+        if (B != batch or W != -(-channels // per) or cap < n_packed or (v_layout == "token" and cap % per)
+                or k_scale.shape != k_meta or k_zero.shape != k_meta or v_packed.shape != want[0]
+                or v_scale.shape != want[1] or v_zero.shape != want[1]):
+            raise ValueError(f"{name}: packed tensors ({which}) {[tuple(t.shape) for t in arrays]} do not fit a batch of {batch}, {n_packed} tokens, "
+                             f"{bits} bits, groups of {g}, values packed by {v_layout}")
+        packed = (bits, g, VQ_F16 if meta == torch.float16 else VQ_F32, _V_LAYOUT[v_layout])
+        fields = [*(t.data_ptr() for t in arrays), n_packed, cap]
+    if n_tail:
+        if k_tail is None or v_tail is None:
+            raise ValueError(f"{name}: n_tail > 0 needs k_tail and v_tail ({which})")
+        if k_tail.ndim != 4 or k_tail.shape != v_tail.shape or k_tail.dtype != v_tail.dtype or k_tail.dtype not in _FLOAT_TAG:
+            raise ValueError(f"{name}: k_tail and v_tail ({which}) must be alike, [B, H, n, D] float16, bfloat16 or float32, got "
+                             f"{tuple(k_tail.shape)} {k_tail.dtype} and {tuple(v_tail.shape)} {v_tail.dtype}")
+        if k_tail.device != device or v_tail.device != device:
+            raise ValueError(f"{name}: k_tail and v_tail ({which}) must live on {device}, got {k_tail.device} and {v_tail.device}")
+        B, H, room, D = k_tail.shape
+        if B != batch or room < n_tail or (heads is not None and (H != heads or D != channels)):
+            raise ValueError(f"{name}: tail ({which}) {tuple(k_tail.shape)} does not fit a batch of {batch}, {n_tail} tokens"
+                             + ("" if heads is None else f", {heads} heads of {channels} channels"))
+        heads, channels, tail = H, D, k_tail.dtype
+        if D > 1 and (k_tail.stride(3) != 1 or v_tail.stride(3) != 1):
+            k_tail, v_tail = k_tail[:, :, :n_tail].contiguous(), v_tail[:, :, :n_tail].contiguous()
+            keep = [k_tail, v_tail]
+        fields += [k_tail.data_ptr(), v_tail.data_ptr(), n_tail, *k_tail.stride()[:3], *v_tail.stride()[:3]]
+    else:
+        fields += [0] * 9
+    return fields, heads, channels, packed, tail, keep
+
+
+def _store_attend(name, maps, q, prefix, own, scale, causal, seq_lens, sliding_window, out, lam=None, norm_weight=None, norm_eps=0.0,
+                  gain=1.0):
+    if q.ndim != 4:
+        raise ValueError(f"{name}: q must be 4D, got {tuple(q.shape)}")
+    if not q.is_cuda:
+        _need_gpu(name, q)
+    device, dtype = q.device, q.dtype
+    tag = _ftag(name, q)
+    B, Hq, Sq, D = q.shape
+    if out is None:
+        out = torch.empty(q.shape, dtype=dtype, device=device)
+    elif out.shape != q.shape or out.dtype != dtype or out.device != device or not out.is_contiguous():
+        raise ValueError(f"{name}: out must be a contiguous {tuple(q.shape)} tensor in {dtype} on {device}")
+    own_f, heads, channels, packed, tail, keep = _store_fields(name, "own", device, B, **own)
+    prefix_f = _NO_STORE
+    if prefix is not None:
+        prefix_f, h2, c2, packed2, tail2, keep2 = _store_fields(name, "prefix", device, 1, **prefix)
+        for mine, other, what in ((heads, h2, "kv heads"), (channels, c2, "channels"), (packed, packed2, "bits, groups and layout"),
+                                  (tail, tail2, "plain rows' dtype")):
+            if mine is not None and other is not None and mine != other:
+                raise ValueError(f"{name}: the prefix and the sequences' own slots differ in {what}")
+        heads, channels, packed, tail = heads or h2, channels or c2, packed or packed2, tail or tail2
+        keep += keep2
+    if heads is None:
+        raise ValueError(f"{name}: no key/value slots to attend to")
+    if channels != D or Hq % heads:
+        raise ValueError(f"{name}: q {tuple(q.shape)} over {heads} kv heads of {channels} channels")
+    if q.numel() == 0:
+        return out
+    if not q.is_contiguous():
+        q = q.contiguous()
+    lens = 0
+    if seq_lens is not None:
+        if seq_lens.shape != (B,) or seq_lens.dtype != torch.int64 or seq_lens.device != device or not seq_lens.is_contiguous():
+            raise ValueError(f"{name}: seq_lens must be a contiguous int64 [{B}] tensor on {device}")
+        lens = seq_lens.data_ptr()
+    lam_p = lam_stride = weight = weight_tag = 0
+    if maps == 2:
+        if not isinstance(lam, torch.Tensor):
+            lam = torch.full((1,), float(lam), dtype=torch.float32, device=device)
+        elif lam.dtype != torch.float32 or lam.device != device or (lam.numel() != 1 and lam.shape != (Hq,)) or not lam.is_contiguous():
+            raise ValueError(f"{name}: lam must be a number or a contiguous float32 tensor of one value or [{Hq}] on {device}")
+        lam_p, lam_stride = lam.data_ptr(), 1 if lam.numel() > 1 else 0
+        if norm_weight is not None:
+            if norm_weight.shape != (D,) or norm_weight.device != device or not norm_weight.is_contiguous():
+                raise ValueError(f"{name}: norm_weight must be a contiguous [{D}] tensor on {device}")
+            weight, weight_tag = norm_weight.data_ptr(), _ftag(name, norm_weight)
+    bits, group, meta, layout = packed or (8, 1, 0, 0)
+    lib = _lib.load()
+    stream = _stream_of(device)
+    call, room = lib.store_attend_packed[maps], lib.store_attend_packed_workspace[maps]
+
+    def block(ws):
+        return _lib.STORE_ATTEND_PACK.pack(
+            q.data_ptr(), out.data_ptr(), B, Hq, heads, Sq, D, *prefix_f, *own_f, lens, lam_p, lam_stride, weight,
+            0 if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), stream, sliding_window or 0, tag,
+            tag if tail is None else _FLOAT_TAG[tail], weight_tag, bits, group, meta, layout, 1 if causal else 0, scale, norm_eps, gain)
+
+    def launch():
+        if torch.cuda.is_current_stream_capturing():
+            # a graph's scratch is its own: two graphs captured on one stream may run at once, and the scratch kept for the
+            # stream is given back when a larger one replaces it
+            need = room(block(None))
+            return call(block(torch.empty(need, dtype=torch.uint8, device=device) if need else None))
+        rc = call(block(_workspace(device, 0, stream)))
+        if rc == _lib.VQ_ERR_WORKSPACE:
+            rc = call(block(_workspace(device, room(block(None)), stream)))
+        return rc
+
+    try:
+        _launch_on(device, launch)
+    except (_lib.struct.error, OverflowError) as e:
+        raise ValueError(f"{name}: {e}") from None
+    return out
+
+
+def shared_prefix_attend(q: torch.Tensor, prefix: dict, *, k_packed=None, k_scale=None, k_zero=None, v_packed=None, v_scale=None,
+                         v_zero=None, n_packed: int = 0, bits: int = 4, group_size: int = 32, v_layout: str = "channel", k_tail=None,
+                         v_tail=None, n_tail: int = 0, scale: float = 1.0, causal: bool = False, seq_lens: torch.Tensor | None = None,
+                         sliding_window: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
+    """softmax(q k^T * scale) v for a batch whose sequences share a prefix: sequence ``b`` attends over ``[prefix | its own
+    slots]``, and the prefix is read once for all of them.
+
+    q ``[B,Hq,Sq,D]`` (``D`` up to 256); ``prefix``: the cache arguments of :func:`kivi_packed_attend` (``k_packed`` .. ``n_tail``) for a batch
+    of one; the same arguments of this call are the sequences' own slots, for a batch of ``B`` (``n_packed = n_tail = 0``: none yet).
+    Packed slots of both have one bit width, group size, value layout and scale type; plain rows (``k_tail``, ``v_tail``) one
+    type, any strides over adjacent channels.  A packed slot counts as the fp16 number ``code * scale + zero``.  GQA by
+    repeat-interleave.  Queries align to the end of a sequence; ``causal`` hides the slots behind a query's own position.
+    ``seq_lens`` (int64 ``[B]`` on the device): live own slots of every sequence (right-padded rows past them are never
+    read; with fewer than ``Sq`` the first queries stand inside the prefix).  ``sliding_window > 0``: a query sees only that many last
+    slots up to its own position.  Scores and sums are float32; fp16 / bf16 rows meet as matrix products of that type
+    (weights rounded to it; fp16 over packed slots).  A row that sees nothing is zero.  A value that is not finite makes every row NaN
+    whose block holds its slot, seen or not, as in the plain product."""
+    own = dict(k_packed=k_packed, k_scale=k_scale, k_zero=k_zero, v_packed=v_packed, v_scale=v_scale, v_zero=v_zero, n_packed=n_packed,
+               bits=bits, group_size=group_size, v_layout=v_layout, k_tail=k_tail, v_tail=v_tail, n_tail=n_tail)
+    return _store_attend("shared_prefix_attend", 1, q, prefix, own, scale, causal, seq_lens, sliding_window, out)
+
+
+def differential_attend(q: torch.Tensor, lam: torch.Tensor | float, *, k_packed=None, k_scale=None, k_zero=None, v_packed=None,
+                        v_scale=None, v_zero=None, n_packed: int = 0, bits: int = 4, group_size: int = 32, v_layout: str = "channel",
+                        k_tail=None, v_tail=None, n_tail: int = 0, scale: float = 1.0, causal: bool = False,
+                        seq_lens: torch.Tensor | None = None, sliding_window: int = 0, norm_weight: torch.Tensor | None = None,
+                        norm_eps: float = 1e-5, gain: float = 1.0, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Differential attention, ``(softmax(q1 k1^T * scale) - lam * softmax(q2 k2^T * scale)) v``: a head's ``D`` channels (even, up to
+    256) hold both halves, ``q1, k1`` the first ``D / 2`` and ``q2, k2`` the others; values have ``D`` channels.  ``scale`` is usually
+    ``(D / 2) ** -0.5``.
+
+    q ``[B,Hq,Sq,D]``; slots, masks and lengths as for :func:`shared_prefix_attend` (own slots only; plain keys and values are
+    ``k_tail`` / ``v_tail``).  ``lam``: float32 ``[Hq]`` or of one value on the device, or a number.  The result is scaled by ``gain``; with
+    ``norm_weight`` (``[D]``) every head's output is first divided by ``sqrt(mean(o^2) + norm_eps)`` and multiplied by it, which is the
+    layer's head norm (``gain = 1 - lambda_init``).  Both maps' weights and sums are formed in one pass over the slots."""
+    own = dict(k_packed=k_packed, k_scale=k_scale, k_zero=k_zero, v_packed=v_packed, v_scale=v_scale, v_zero=v_zero, n_packed=n_packed,
+               bits=bits, group_size=group_size, v_layout=v_layout, k_tail=k_tail, v_tail=v_tail, n_tail=n_tail)
+    return _store_attend("differential_attend", 2, q, None, own, scale, causal, seq_lens, sliding_window, out, lam, norm_weight, norm_eps,
+                         gain)
 
 
 # ---------------------------------------------------------------------------
@@ -1484,75 +1671,88 @@ def rotary_embed(q: torch.Tensor, k: torch.Tensor | None = None, *, inv_freq: to
     are contiguous.  ``inverse=True`` turns back; times ``attention_factor`` that is the transposed map, the gradient of the
     forward call (this package's functions record none)."""
     name = "rotary_embed"
-    given = [(q, out, "q")] if k is None else [(q, out, "q"), (k, k_out, "k")]
+    if q.ndim != 4 or (k is not None and k.ndim != 4):
+        raise ValueError(f"{name}: q and k must be [B, H, S, D], got {tuple(q.shape)}" + ("" if k is None else f" and {tuple(k.shape)}"))
     if k is None and k_out is not None:
         raise ValueError(f"{name}: k_out without k")
-    for t, _, what in given:
-        if t.ndim != 4:
-            raise ValueError(f"{name}: {what} must be [B, H, S, D], got {tuple(t.shape)}")
-    _need_gpu(name, *(t for t, _, _ in given), inv_freq)
-    B, _, S, D = q.shape
+    device, dtype = q.device, q.dtype
+    if not (q.is_cuda and inv_freq.is_cuda and (k is None or k.is_cuda)):
+        _need_gpu(name, q, inv_freq, *(() if k is None else (k,)))
+    B, Hq, S, D = q.shape
     tag = _ftag(name, q)
-    if k is not None and (k.dtype != q.dtype or k.device != q.device or (k.shape[0], *k.shape[2:]) != (B, S, D)):
-        raise ValueError(f"{name}: k must be [{B}, H, {S}, {D}] in {q.dtype} on {q.device}, got {tuple(k.shape)} in {k.dtype} on {k.device}")
-    if inv_freq.ndim != 1 or inv_freq.dtype not in (torch.float64, torch.float32) or inv_freq.device != q.device:
-        raise ValueError(f"{name}: inv_freq must be float64 or float32 [dims / 2] on {q.device}")
-    dims = 2 * inv_freq.numel()
+    if k is not None and (k.dtype != dtype or k.device != device or k.shape[0] != B or k.shape[2] != S or k.shape[3] != D):
+        raise ValueError(f"{name}: k must be [{B}, H, {S}, {D}] in {dtype} on {device}, got {tuple(k.shape)} in {k.dtype} on {k.device}")
+    if inv_freq.ndim != 1 or inv_freq.dtype not in (torch.float64, torch.float32) or inv_freq.device != device:
+        raise ValueError(f"{name}: inv_freq must be float64 or float32 [dims / 2] on {device}")
+    dims = 2 * inv_freq.shape[0]
     if not 2 <= dims <= D:
-        raise ValueError(f"{name}: {inv_freq.numel()} frequencies turn {dims} channels of {D}")
+        raise ValueError(f"{name}: {dims // 2} frequencies turn {dims} channels of {D}")
     inv_freq = inv_freq.contiguous()
-    a = _lib.RotaryArgs()
-    a.B, a.S, a.D, a.dims, a.dtype = B, S, D, dims, tag
-    a.inv_freq, a.freq_dtype = inv_freq.data_ptr(), VQ_F64 if inv_freq.dtype == torch.float64 else VQ_F32
-    a.layout, a.inverse, a.attention_factor = int(bool(traditional)), int(bool(inverse)), float(attention_factor)
-    at = positions if positions is not None else offset if isinstance(offset, torch.Tensor) else None
-    if positions is not None and isinstance(offset, torch.Tensor):
-        raise ValueError(f"{name}: with positions, offset is an int")
-    if at is not None:
-        if at.dtype not in (torch.int32, torch.int64) or at.device != q.device:
-            raise ValueError(f"{name}: positions and offsets must be int32 or int64 on {q.device}, got {at.dtype} on {at.device}")
-        a.pos_dtype = VQ_I64 if at.dtype == torch.int64 else VQ_I32
-        if positions is None:
-            if at.numel() != 1 and tuple(at.shape) != (B,):
-                raise ValueError(f"{name}: offset must have one entry or be [{B}], got {tuple(at.shape)}")
-            a.pos_stride_b, a.pos_stride_s, a.add_index = (0 if at.numel() == 1 else at.stride(0)), 0, 1
-        else:
-            shape = (1,) * (2 - at.ndim) + tuple(at.shape)
-            if at.ndim not in (1, 2) or shape[0] not in (1, B) or shape[1] != S:
-                raise ValueError(f"{name}: positions must be [{S}] or [{B}, {S}], got {tuple(at.shape)}")
-            a.pos_stride_b, a.pos_stride_s = (0 if shape[0] == 1 else at.stride(0)), at.stride(-1)
-            a.offset = int(offset)
-        a.positions = at.data_ptr()
+    at, at_b, at_s, first, add_index = None, 0, 0, 0, 1
+    if positions is not None:
+        if isinstance(offset, torch.Tensor):
+            raise ValueError(f"{name}: with positions, offset is an int")
+        at, first, add_index = positions, int(offset), 0
+        many = at.shape[0] if at.ndim == 2 else 1
+        if at.ndim not in (1, 2) or many not in (1, B) or at.shape[-1] != S:
+            raise ValueError(f"{name}: positions must be [{S}] or [{B}, {S}], got {tuple(at.shape)}")
+        at_b, at_s = (at.stride(0) if many > 1 else 0), at.stride(-1)
+    elif isinstance(offset, torch.Tensor):
+        at = offset
+        if at.numel() != 1 and at.shape != (B,):
+            raise ValueError(f"{name}: offset must have one entry or be [{B}], got {tuple(at.shape)}")
+        at_b = at.stride(0) if at.numel() > 1 else 0
     else:
-        a.offset, a.add_index = int(offset), 1
-    rows, results = [], []
-    for t, o, what in given:
+        first = int(offset)
+    if at is not None and (at.dtype not in (torch.int32, torch.int64) or at.device != device):
+        raise ValueError(f"{name}: positions and offsets must be int32 or int64 on {device}, got {at.dtype} on {at.device}")
+
+    def rows_of(t, o, what):
+        """The rows as the library takes them and their output, new or checked."""
         if t.stride(3) != 1 and D > 1:
             t = t.contiguous()
         if o is None:
-            o = torch.empty(t.shape, dtype=t.dtype, device=t.device)
-        elif o.shape != t.shape or o.dtype != t.dtype or o.device != t.device or (D > 1 and o.stride(3) != 1):
-            raise ValueError(f"{name}: the output for {what} must be {tuple(t.shape)} in {t.dtype} on {t.device} with adjacent channels")
+            o = torch.empty(t.shape, dtype=dtype, device=device)
+        elif o.shape != t.shape or o.dtype != dtype or o.device != device or (D > 1 and o.stride(3) != 1):
+            raise ValueError(f"{name}: the output for {what} must be {tuple(t.shape)} in {dtype} on {device} with adjacent channels")
         elif any(n > 1 and st == 0 for n, st in zip(o.shape, o.stride())):
             raise ValueError(f"{name}: rows of the output for {what} share memory")
-        rows.append(t)
-        results.append(o)
-    if all(t.numel() == 0 for t in rows):
-        return results[0] if k is None else tuple(results)
-    live = [i for i, t in enumerate(rows) if t.numel()]
-    in_place = [i in live and _same_rows(rows[i], results[i]) for i in range(len(rows))]
-    for i in live:
-        lo, hi = _extent(results[i])
-        for j in live:
-            others = [] if in_place[i] and (i == j or in_place[j]) else [rows[j]] + ([results[j]] if i != j else [])
-            if any(lo < e and s < hi for s, e in map(_extent, others)):
-                raise ValueError(f"{name}: the output for {given[i][2]} overlaps other rows of the call (it may only be its input itself)")
-    for i in live:
-        a.x[i], a.out[i], a.heads[i] = rows[i].data_ptr(), results[i].data_ptr(), rows[i].shape[1]
-        for d in range(3):
-            a.x_strides[i][d], a.out_strides[i][d] = rows[i].stride(d), results[i].stride(d)
-    _launch_on(q.device, lambda: _lib.load().vq_rotary(a, _stream(q)))
-    return results[0] if k is None else tuple(results)
+        return t, o
+
+    fresh = out is None and k_out is None
+    q, out = rows_of(q, out, "q")
+    result = out
+    Hk, kb, kh, ks, ob, oh, os_, kp, kop = 0, 0, 0, 0, 0, 0, 0, 0, 0
+    if k is not None:
+        k, k_out = rows_of(k, k_out, "k")
+        result = (out, k_out)
+        Hk, kp, kop = k.shape[1], k.data_ptr(), k_out.data_ptr()
+        kb, kh, ks, _ = k.stride()
+        ob, oh, os_, _ = k_out.stride()
+    if B == 0 or S == 0 or Hq + Hk == 0:
+        return result
+    if not fresh:   # (new outputs overlap nothing)
+        live = [p for p in ((q, out, "q"), (k, k_out, "k")) if p[0] is not None and p[0].numel()]
+        still = [_same_rows(t, o) for t, o, _ in live]
+        for i, (t, o, what) in enumerate(live):
+            lo, hi = _extent(o)
+            for j, (u, p, _) in enumerate(live):
+                others = [] if still[i] and (i == j or still[j]) else [u] if i == j else [u, p]
+                if any(lo < e and s < hi for s, e in map(_extent, others)):
+                    raise ValueError(f"{name}: the output for {what} overlaps other rows of the call (it may only be its input itself)")
+    lib = _lib.load()
+    qb, qh, qs, _ = q.stride()
+    pb, ph, ps, _ = out.stride()
+    try:
+        args = _lib.ROTARY_PACK.pack(
+            q.data_ptr(), kp, out.data_ptr(), kop, Hq, Hk, qb, qh, qs, kb, kh, ks, pb, ph, ps, ob, oh, os_, B, S, D, dims,
+            inv_freq.data_ptr(), 0 if at is None else at.data_ptr(), at_b, at_s, first, tag, VQ_F64 if inv_freq.dtype == torch.float64 else VQ_F32,
+            VQ_I64 if at is None or at.dtype == torch.int64 else VQ_I32, add_index, 1 if traditional else 0, 1 if inverse else 0,
+            attention_factor)
+    except (_lib.struct.error, OverflowError) as e:
+        raise ValueError(f"{name}: {e}") from None
+    _launch_on(device, lambda: lib.rotary_packed(args, _stream_of(device)))
+    return result
 
 
 # ---------------------------------------------------------------------------
