@@ -205,8 +205,9 @@ int check_call(const char *fn, const vq_store_attend_args *args, int maps) {
     const int64_t slots = span_prefix_slots(a) + a.own.n_packed + a.own.n_tail;
     VQ_REQUIRE(slots >= 1, VQ_ERR_INVALID, "%s: no key/value slots to attend to", fn);
     VQ_REQUIRE(slots < (INT64_C(1) << 30) && a.Sq < (INT64_C(1) << 30), VQ_ERR_UNSUPPORTED, "%s: more than 2^30 slots or queries a sequence", fn);
-    VQ_REQUIRE(a.B < (INT64_C(1) << 30) && a.Hq < (INT64_C(1) << 20) && a.B * a.Hq < (INT64_C(1) << 31) && a.B * a.Hq * a.Sq < (INT64_C(1) << 31), VQ_ERR_UNSUPPORTED,
-               "%s: 2^31 or more query rows", fn);
+    // (a wave a row in the merge, 2^32 threads a launch at most)
+    VQ_REQUIRE(a.B < (INT64_C(1) << 26) && a.Hq < (INT64_C(1) << 26) && a.B * a.Hq < (INT64_C(1) << 26) && a.B * a.Hq * a.Sq < (INT64_C(1) << 26),
+               VQ_ERR_UNSUPPORTED, "%s: 2^26 or more query rows", fn);
     VQ_REQUIRE(!a.causal || a.Sq <= slots, VQ_ERR_INVALID, "%s: S_q=%lld exceeds the %lld slots; queries align to their end", fn, (long long)a.Sq, (long long)slots);
     VQ_REQUIRE(a.sliding_window >= 0, VQ_ERR_INVALID, "%s: negative sliding window", fn);
     VQ_REQUIRE(a.q != nullptr && a.out != nullptr, VQ_ERR_INVALID, "%s: null q or out", fn);
@@ -268,8 +269,7 @@ template <int MAPS> int attend(const char *fn, const vq_store_attend_args *args)
     if (mfma) {
         if (int rc = launch_span_mfma(c, MAPS)) return rc;
     } else {
-        const int64_t waves = rows * c.nparts;
-        VQ_REQUIRE(cdiv(waves, 4) < (INT64_C(1) << 24) * 4, VQ_ERR_UNSUPPORTED, "%s: too many query rows for this head size or type", fn);
+        const int64_t waves = rows * c.nparts;   // (at most 8192, or one a row)
         span_any_kernel<MAPS><<<(unsigned)cdiv(waves, 4), 256, 0, st>>>(c);
         VQ_HIP_CHECK_LAUNCH(fn);
     }
