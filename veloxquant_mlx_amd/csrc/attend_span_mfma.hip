@@ -32,9 +32,11 @@ void span_mfma_plan(SpanCall &c, int maps) {
     const vq_store_attend_args &a = c.a;
     const int64_t r1 = a.Hq / a.Hkv * a.Sq, all = a.B * r1, prefix = units_of(a.prefix), own = units_of(a.own);
     c.apart = prefix > 0 && a.B > 1 && r1 < 128;
-    auto tiling = [](int64_t rows, int &wt, int &tiles) {
-        wt = rows <= 64 ? 2 : 1;
-        tiles = (int)cdiv(rows, 128 / wt);
+    // four waves of 32 rows and one map each; where rows fill half of them, two share rows and halve the units
+    const int most = 128 / maps;
+    auto tiling = [&](int64_t rows, int &wt, int &tiles) {
+        wt = rows <= most / 2 ? 2 : 1;
+        tiles = (int)cdiv(rows, most / wt);
     };
     tiling(all, c.pwt, c.ptiles);
     tiling(r1, c.owt, c.otiles);
@@ -47,7 +49,6 @@ void span_mfma_plan(SpanCall &c, int maps) {
     c.psplits = c.apart ? (int)cdiv(prefix, run) : 0;
     c.osplits = walk > 0 ? (int)cdiv(walk, run) : 0;
     c.nparts = c.psplits * c.pwt + c.osplits * c.owt;
-    (void)maps;
 }
 
 int launch_span_mfma(const SpanCall &c, int maps) {

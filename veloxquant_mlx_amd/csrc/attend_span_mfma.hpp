@@ -91,7 +91,7 @@ void span_mfma_kernel(SpanCall c) {
     extern __shared__ __align__(16) char lds[];
     using M = SpanMma<T>;
     using Tile = SpanTile<BITS, D>;
-    constexpr int KS = D / 16, DT = D / 32, CH = D / 8;   // channel steps of a score, channel tiles, 16-byte pieces a row
+    constexpr int KS = D / MAPS / 16, DT = D / 32, CH = D / 8;   // channel steps of a score, channel tiles, 16-byte pieces a row
     const vq_store_attend_args &a = c.a;
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -115,7 +115,9 @@ void span_mfma_kernel(SpanCall c) {
         splits = c.osplits; split = id % splits; tile = c.otiles - 1 - id / splits;
         wt = c.owt; rows = r1; part = (c.apart ? c.psplits * c.pwt : 0) + split * wt;
     }
-    const int rt = 128 / wt, rg = wt == 1 ? wave : wave & 1, th = wt == 1 ? 0 : wave >> 1;
+    // the waves: one map each, 32 rows each; the waves that are left over share rows, each with its half of every unit
+    const int map = MAPS == 2 ? wave & 1 : 0, rest = MAPS == 2 ? wave >> 1 : wave, groups = 4 / MAPS / wt;
+    const int rt = 32 * groups, rg = rest % groups, th = rest / groups;
     part += th;
 
     // ---- this lane's query row: positions outermost, so that a tile covers few of them
@@ -186,7 +188,7 @@ void span_mfma_kernel(SpanCall c) {
     const float c2 = __builtin_fabsf(a.scale) * LOG2E;
     u32x4 q[KS];
     {
-        const u16 *src = (const u16 *)a.q + qrow * D + 8 * h;
+        const u16 *src = (const u16 *)a.q + qrow * D + map * (D / MAPS) + 8 * h;
         const u32 sign = a.scale < 0.f ? 0x80008000u : 0u;   // the softmax takes the maximum of the scores themselves
         const bool q_bf16 = a.dtype == VQ_BF16;
 #pragma unroll
@@ -304,66 +306,51 @@ void span_mfma_kernel(SpanCall c) {
     };
 
     // ---- state of the lane's row
-    f32x16 O[MAPS][DT];
-    float m_run[MAPS], l_run[MAPS];
+    f32x16 O[DT];
+    float m_run = -INFINITY, l_run = 0.f;
 #pragma unroll
-    for (int w = 0; w < MAPS; ++w) {
-        m_run[w] = -INFINITY; l_run[w] = 0.f;
+    for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) O[w][dt][r] = 0.f;
-    }
+        for (int r = 0; r < 16; ++r) O[dt][r] = 0.f;
 
     auto work = [&](const Unit &u, int buf, int half) {   // 32 slots of the unit
         const char *kd = lds + buf * Tile::BUF, *vd = kd + Tile::KEYS;
         const int place = u.place + 32 * half;
         if (place >= any_hi || place + 32 <= any_lo || 32 * half >= u.live - u.t0) return;
-        u32 P[MAPS][8];
-        f32x16 S[MAPS];
+        f32x16 S;
 #pragma unroll
-        for (int w = 0; w < MAPS; ++w) {
+        for (int r = 0; r < 16; ++r) S[r] = 0.f;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) S[w][r] = 0.f;
-#pragma unroll
-            for (int ks = w * KS / MAPS; ks < (w + 1) * KS / MAPS; ++ks) {
-                const u32x4 k = *(const u32x4 *)(kd + (32 * half + n) * D * 2 + sp_kpiece<D>(n, 2 * ks + h) * 16);
-                S[w] = M::mma(k, q[ks], S[w]);
-            }
-        }
+        for (int ks = 0; ks < KS; ++ks)
+            S = M::mma(*(const u32x4 *)(kd + (32 * half + n) * D * 2 + sp_kpiece<D>(n, 2 * (map * KS + ks) + h) * 16), q[ks], S);
         const int live_end = u.place + u.live - u.t0;   // slot past the span's live tokens
         if (place + 32 > (all_hi < live_end ? all_hi : live_end) || place < all_lo) {
             const int hi = (lane_hi < live_end ? lane_hi : live_end) - place - 4 * h, lo = lane_lo - place - 4 * h;
 #pragma unroll
-            for (int w = 0; w < MAPS; ++w)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int t = 8 * (r / 4) + r % 4;
-                    if (t >= hi || t < lo) S[w][r] = -INFINITY;
-                }
+            for (int r = 0; r < 16; ++r) {
+                const int t = 8 * (r / 4) + r % 4;
+                if (t >= hi || t < lo) S[r] = -INFINITY;
+            }
         }
+        float mx = fmaxf(S[0], S[1]);
 #pragma unroll
-        for (int w = 0; w < MAPS; ++w) {
-            float mx = fmaxf(S[w][0], S[w][1]);
+        for (int r = 2; r < 16; ++r) mx = fmaxf(mx, S[r]);
+        if (__any(mx * cc > m_run + RESCALE_SLACK)) {
+            const float top = fmaxf(mx, __shfl_xor(mx, 32)) * cc, m = fmaxf(m_run, top);
+            const float alpha = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - m);
+            m_run = m;
+            l_run *= alpha;
 #pragma unroll
-            for (int r = 2; r < 16; ++r) mx = fmaxf(mx, S[w][r]);
-            if (__any(mx * cc > m_run[w] + RESCALE_SLACK)) {
-                const float top = fmaxf(mx, __shfl_xor(mx, 32)) * cc, m = fmaxf(m_run[w], top);
-                const float alpha = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run[w] - m);
-                m_run[w] = m;
-                l_run[w] *= alpha;
+            for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt)
+                for (int r = 0; r < 16; ++r) O[dt][r] *= alpha;
+        }
+        const float nm = m_run == -INFINITY ? 0.f : -m_run;
+        u32 P[8];
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) O[w][dt][r] *= alpha;
-            }
-            const float nm = m_run[w] == -INFINITY ? 0.f : -m_run[w];
-#pragma unroll
-            for (int r = 0; r < 8; ++r) {
-                P[w][r] = M::pack(__builtin_amdgcn_exp2f(__builtin_fmaf(S[w][2 * r], cc, nm)),
-                                  __builtin_amdgcn_exp2f(__builtin_fmaf(S[w][2 * r + 1], cc, nm)));
-                l_run[w] = M::add_pair(P[w][r], l_run[w]);
-            }
+        for (int r = 0; r < 8; ++r) {
+            P[r] = M::pack(__builtin_amdgcn_exp2f(__builtin_fmaf(S[2 * r], cc, nm)), __builtin_amdgcn_exp2f(__builtin_fmaf(S[2 * r + 1], cc, nm)));
+            l_run = M::add_pair(P[r], l_run);
         }
         const bool transposed = BITS && !(u.s & 1);
 #pragma unroll
@@ -381,12 +368,11 @@ void span_mfma_kernel(SpanCall c) {
                     const uint2 v1 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((L *)(uintptr_t)lds_addr(row + 8 * D * 2)));
                     v = u32x4{v0.x, v0.y, v1.x, v1.y};
                 }
-#pragma unroll
-                for (int w = 0; w < MAPS; ++w)
-                    O[w][dt] = M::mma(v, u32x4{P[w][4 * s], P[w][4 * s + 1], P[w][4 * s + 2], P[w][4 * s + 3]}, O[w][dt]);
+                O[dt] = M::mma(v, u32x4{P[4 * s], P[4 * s + 1], P[4 * s + 2], P[4 * s + 3]}, O[dt]);
             }
         }
     };
+    const int half0 = wt == 1 ? 0 : th, half1 = wt == 1 ? 2 : th + 1;
 
     if (w0 < w1) {
         Words wd;
@@ -404,12 +390,8 @@ void span_mfma_kernel(SpanCall c) {
                 fetch(next, buf ^ 1, wd);
             }
             if (wave_works) {
-                if (wt == 1) {
-                    work(u, buf, 0);
-                    work(u, buf, 1);
-                } else {
-                    work(u, buf, th);
-                }
+#pragma unroll 1
+                for (int half = half0; half < half1; ++half) work(u, buf, half);
             }
             if (more) {
                 store_unit(next, buf ^ 1, wd);
@@ -421,40 +403,56 @@ void span_mfma_kernel(SpanCall c) {
     }
 
     // ---- results
-    if (j >= rows) return;
-    float l[MAPS];
-#pragma unroll
-    for (int w = 0; w < MAPS; ++w) l[w] = l_run[w] + __shfl_xor(l_run[w], 32);   // (both halves of a row are here together)
+    float l = l_run + __shfl_xor(l_run, 32);   // both halves of a row
     if (c.nparts > 1) {
-        const int64_t rec = (qrow * c.nparts + part) * MAPS;
+        if (j >= rows) return;
+        const int64_t rec = (qrow * c.nparts + part) * MAPS + map;
+        if (h == 0) *(float2 *)(c.ml + rec * 2) = make_float2(m_run, l);
+        float *dst = c.sums + rec * D + 4 * h;
 #pragma unroll
-        for (int w = 0; w < MAPS; ++w) {
-            if (h == 0) *(float2 *)(c.ml + (rec + w) * 2) = make_float2(m_run[w], l[w]);
-            float *dst = c.sums + (rec + w) * D + 4 * h;
+        for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                for (int r = 0; r < 16; r += 4)
-                    *(float4 *)(dst + 32 * dt + 2 * r) = make_float4(O[w][dt][r], O[w][dt][r + 1], O[w][dt][r + 2], O[w][dt][r + 3]);
-        }
+            for (int r = 0; r < 16; r += 4) *(float4 *)(dst + 32 * dt + 2 * r) = make_float4(O[dt][r], O[dt][r + 1], O[dt][r + 2], O[dt][r + 3]);
         return;
     }
-    float by[MAPS];
-    by[0] = l[0] > 0.f || l[0] != l[0] ? 1.f / l[0] : 0.f;
-    if (MAPS == 2) by[MAPS - 1] = l[MAPS - 1] > 0.f || l[MAPS - 1] != l[MAPS - 1] ? -span_lam(a, hkv * G + rem % G) / l[MAPS - 1] : 0.f;
-    float sq = 0.f;
+    float by = l > 0.f || l != l ? 1.f / l : 0.f, gain = 1.f, sq = 0.f;
+    if (MAPS == 2 && map == 1) by *= -span_lam(a, hkv * G + rem % G);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            float o = O[0][dt][r] * by[0];
-            if (MAPS == 2) o = __builtin_fmaf(O[MAPS - 1][dt][r], by[MAPS - 1], o);
-            O[0][dt][r] = o;
-            sq = __builtin_fmaf(o, o, sq);
+        for (int r = 0; r < 16; ++r) O[dt][r] *= by;
+    bool norm = false;
+    if (MAPS == 2) {
+        // the second map's wave hands its rows over in LDS, a channel tile's quarter of 4 floats a lane at a time
+        static_assert(Tile::LDS >= 2 * D * 32 * 4 || MAPS == 1, "room for the rows of both row groups");
+        float4 *room = (float4 *)lds + rg * (D / 8) * 64 + lane;
+        lds_barrier();
+        if (map == 1) {
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) room[(4 * dt + r) * 64] = make_float4(O[dt][4 * r], O[dt][4 * r + 1], O[dt][4 * r + 2], O[dt][4 * r + 3]);
         }
-    const bool norm = MAPS == 2 && a.norm_weight != nullptr;
-    float gain = MAPS == 2 ? a.gain : 1.f;
-    if (norm) gain /= sqrtf((sq + __shfl_xor(sq, 32)) * (1.f / D) + a.norm_eps);
+        lds_barrier();
+        if (map == 1) return;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float4 x = room[(4 * dt + r) * 64];
+                O[dt][4 * r] += x.x; O[dt][4 * r + 1] += x.y; O[dt][4 * r + 2] += x.z; O[dt][4 * r + 3] += x.w;
+            }
+        gain = a.gain;
+        norm = a.norm_weight != nullptr;
+        if (norm) {
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) sq = __builtin_fmaf(O[dt][r], O[dt][r], sq);
+            gain /= sqrtf((sq + __shfl_xor(sq, 32)) * (1.f / D) + a.norm_eps);
+        }
+    }
+    if (j >= rows) return;
     u16 *dst = (u16 *)a.out + qrow * D + 4 * h;
     const bool out_bf16 = a.dtype == VQ_BF16;
 #pragma unroll
@@ -464,7 +462,7 @@ void span_mfma_kernel(SpanCall c) {
             float o[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                o[e] = O[0][dt][r + e] * gain;
+                o[e] = O[dt][r + e] * gain;
                 if (norm) o[e] *= span_ld(a.norm_weight, a.norm_dtype, 32 * dt + 2 * r + 4 * h + e);
             }
             const uint2 x = out_bf16 ? make_uint2(SpanMma<bf16_t>::pack(o[0], o[1]), SpanMma<bf16_t>::pack(o[2], o[3]))
