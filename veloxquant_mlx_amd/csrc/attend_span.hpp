@@ -16,7 +16,7 @@ struct SpanCall {
     int nparts;            // parts a row
     int psplits, osplits;  // runs of the prefix / of a sequence's own slots (MFMA: see attend_span_mfma.hpp)
     int ptiles, otiles;    // row tiles of the prefix / of a sequence
-    int pwt, owt;          // waves that share a row, each with its part of every unit
+    int pwt, owt;          // waves that share a row (1 or 2), each with its half of every unit
     int apart;             // 1: prefix and own slots belong to different blocks; 0: the blocks of a row walk both
     float *sums;           // [rows][nparts][maps][D]
     float *ml;             // [rows][nparts][maps][2]

@@ -26,29 +26,29 @@ bool span_mfma_supported(const vq_store_attend_args &a) {
            packed_slots_fit(a, a.own);
 }
 
-static int64_t units_of(const vq_kv_store &s) { return cdiv(s.n_packed, SP_UNIT) + cdiv(s.n_tail, SP_UNIT); }
-
 void span_mfma_plan(SpanCall &c, int maps) {
     const vq_store_attend_args &a = c.a;
+    const int64_t unit = a.D == 256 ? 32 : 64;
+    auto units_of = [&](const vq_kv_store &s) { return cdiv(s.n_packed, unit) + cdiv(s.n_tail, unit); };
     const int64_t r1 = a.Hq / a.Hkv * a.Sq, all = a.B * r1, prefix = units_of(a.prefix), own = units_of(a.own);
-    c.apart = prefix > 0 && a.B > 1 && r1 < 128;
-    // four waves of 32 rows and one map each; where rows fill half of them, two share rows and halve the units
-    const int most = 128 / maps;
+    const int most = 32 * SP_WAVES / maps;   // rows of a block
+    // the prefix in blocks of its own where a sequence's rows fill half a block or less
+    c.apart = prefix > 0 && a.B > 1 && r1 <= most / 2;
     auto tiling = [&](int64_t rows, int &wt, int &tiles) {
-        wt = rows <= most / 2 ? 2 : 1;
+        wt = a.D != 256 && rows <= most / 2 ? 2 : 1;
         tiles = (int)cdiv(rows, most / wt);
     };
     tiling(all, c.pwt, c.ptiles);
     tiling(r1, c.owt, c.otiles);
-    // one round of blocks, two a CU (one with heads of 256 channels), of equal runs
-    const int64_t round = a.D == 256 ? 256 : 512;
+    // one round of blocks of equal runs, one block a CU; sequences that differ in length even out over four rounds
+    const int64_t round = a.seq_lens != nullptr ? 1024 : 256;
     const int64_t walk = c.apart ? own : prefix + own;
     const int64_t work = (c.apart ? a.Hkv * c.ptiles * prefix : 0) + a.B * a.Hkv * c.otiles * walk;
     int64_t run = cdiv(work, round);
-    if (run < 2) run = 2;
+    if (run < 4) run = 4;
     c.psplits = c.apart ? (int)cdiv(prefix, run) : 0;
     c.osplits = walk > 0 ? (int)cdiv(walk, run) : 0;
-    c.nparts = c.psplits * c.pwt + c.osplits * c.owt;
+    c.nparts = c.psplits + c.osplits;
 }
 
 int launch_span_mfma(const SpanCall &c, int maps) {

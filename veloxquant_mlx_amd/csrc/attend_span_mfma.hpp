@@ -1,11 +1,13 @@
 // Attention over spans of slots on the matrix units (gfx950, wave64): one kernel for the shared prefix, for a sequence's own slots
 // and for both maps of differential attention.
 //
-// A block of four waves walks units of 64 slots of one kv head.  A unit's keys and values are staged in LDS once for the
-// block, double-buffered: plain rows by asynchronous copies, packed slots through registers, reconstructed to fp16 (one packed
-// fused multiply-add for two codes: exactly fp16(code * scale + zero)).  Each wave holds 32 query rows; the rows are those of all
-// sequences that share the kv head (prefix), or of one sequence (own slots) -- 128 a block, or 64 rows with two waves on
-// each 32, one for either half of every unit.
+// A block of eight waves walks units of 64 slots (32 with heads of 256 channels) of one kv head.  A unit's keys and values are staged
+// in LDS once for the block.  Plain rows are copied there asynchronously, three units ahead.  Packed slots come as words, scales and
+// zeros into a ring of such units, seven ahead, and are reconstructed to fp16 a unit ahead of the products (one packed fused
+// multiply-add for two codes: exactly fp16(code * scale + zero)); four waves reconstruct before their products and four after, so
+// that each SIMD, which holds one of either, keeps its vector and its matrix unit busy at once.  A wave holds 32 query rows of one
+// map.  The rows of a block are those of all sequences that share the kv head (prefix), or of one sequence (own slots); where
+// they fill half of the waves or less, two waves share rows, each with its half of every unit, and add up in LDS at the end.
 //
 // v_mfma_f32_32x32x16 with n = lane % 32, h = lane / 32: A[i = n][k = 8 h + j], B[k = 8 h + j][n], j = 0..7, and
 // D[i = 8 (r / 4) + 4 h + r % 4][n] in register r = 0..15.  Scores are formed transposed, S^T = K Q^T: a lane then holds sixteen slots of
@@ -19,6 +21,7 @@
 // times a run; weights are rounded to the operand type, and their sum is that of the rounded ones.
 #pragma once
 #include <atomic>
+#include <type_traits>
 
 #include "attend_span.hpp"
 
@@ -29,9 +32,7 @@ typedef __bf16 bf16x2v __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8v __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-constexpr int SP_UNIT = 64;         // slots a unit
-constexpr int SP_THREADS = 256;
-constexpr int SP_VROW = 2 * SP_UNIT + 16;   // bytes of a channel's row of transposed values (144: conflict-free b128 access)
+constexpr int SP_WAVES = 8, SP_THREADS = 64 * SP_WAVES;
 
 template <typename T> struct SpanMma;
 template <> struct SpanMma<f16> {
@@ -78,20 +79,51 @@ __device__ __forceinline__ u32x4 sp_values8(const u32 (&c)[4], uint4 scale, uint
     return o;
 }
 
+// sixteen bytes a lane from any addresses into LDS at lds + 16 * lane (lds_copy16 with 64-bit addresses)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void span_copy16(const void *from, u32 lds) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" :: "v"(from), "s"(uniform(lds)) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
+// bare three-way maximum (fmaxf canonicalises its operands first)
+__device__ __forceinline__ float sp_max3(float x, float y, float z) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
+    return r;
+}
+// a choice between two values (between two places, as `c ? x : y` may become, it would move both to scratch memory)
+template <typename T> __device__ __forceinline__ T sp_pick(bool c, T x, T y) { return c ? x : y; }
+
 template <int BITS, int D> struct SpanTile {
-    static constexpr int KEYS = SP_UNIT * D * 2;
-    static constexpr int VALUES = BITS && D * SP_VROW > KEYS ? D * SP_VROW : KEYS;
+    static constexpr int UNIT = D == 256 ? 32 : 64;      // slots a unit
+    static constexpr int HALVES = UNIT / 32;
+    static constexpr int VROW = 2 * UNIT + 16;           // bytes of a channel's row of transposed values (144, 80: b128 reads free of conflicts)
+    static constexpr int KEYS = UNIT * D * 2;
+    static constexpr int VALUES = BITS && D * VROW > KEYS ? D * VROW : KEYS;
     static constexpr int BUF = KEYS + VALUES;
-    static constexpr int LDS = 2 * BUF;
+    static constexpr int BUFS = BITS ? 2 : 0;            // tiles of packed slots: one at work, one in the making
+    static constexpr int ROW_BUF = 2 * KEYS, ROW_BUFS = 4;   // tiles of plain rows: one at work, three under way
+    // a packed unit as it lies in memory: key words, value words, key scales and zeros a piece of 32 slots, value scales and
+    // zeros a piece of 32 channels
+    static constexpr int KWORDS = UNIT * D * BITS / 8, META = UNIT * D / 8;
+    static constexpr int RAW = 2 * KWORDS + 2 * META;
+    static constexpr int RAWS = BITS ? 8 : 0;
+    static constexpr int PIECES = RAW / 1024;            // copies of 1 KB, dealt to the waves
+    static constexpr int COPIES = (PIECES + SP_WAVES - 1) / SP_WAVES;
+    static constexpr int EXCHANGE = SP_WAVES / 2 * (D / 8 * 64 + 64) * 16;   // the rows of half of the waves, at the end
+    static constexpr int max(int x, int y) { return x > y ? x : y; }
+    static constexpr int LDS = max(max(BUFS * BUF + RAWS * RAW, ROW_BUFS * ROW_BUF), EXCHANGE);
+    static_assert(RAW % 1024 == 0 && LDS <= 160 * 1024 && KEYS % (1024 * SP_WAVES) == 0, "tile sizes");
 };
 
 template <int BITS, typename T, int D, int MAPS>
-__global__ __launch_bounds__(SP_THREADS) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2, D == 256 ? 1 : 2)))
-void span_mfma_kernel(SpanCall c) {
+__global__ __launch_bounds__(SP_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2))) void span_mfma_kernel(SpanCall c) {
     extern __shared__ __align__(16) char lds[];
     using M = SpanMma<T>;
     using Tile = SpanTile<BITS, D>;
-    constexpr int KS = D / MAPS / 16, DT = D / 32, CH = D / 8;   // channel steps of a score, channel tiles, 16-byte pieces a row
+    constexpr int UNIT = Tile::UNIT, KS = D / MAPS / 16, KF = KS < 8 ? KS : 8, DT = D / 32, CH = D / 8;   // channel steps of a score, channel tiles, 16-byte pieces a row
     const vq_store_attend_args &a = c.a;
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -108,17 +140,16 @@ void span_mfma_kernel(SpanCall c) {
     if (shared) {
         id /= Hkv;
         splits = c.psplits; split = id % splits; tile = id / splits;
-        wt = c.pwt; rows = B * r1; part = split * wt;
+        wt = c.pwt; rows = B * r1; part = split;
     } else {
         id = (id - shared_blocks) / Hkv;
         b = id % B; id /= B;
         splits = c.osplits; split = id % splits; tile = c.otiles - 1 - id / splits;
-        wt = c.owt; rows = r1; part = (c.apart ? c.psplits * c.pwt : 0) + split * wt;
+        wt = c.owt; rows = r1; part = (c.apart ? c.psplits : 0) + split;
     }
-    // the waves: one map each, 32 rows each; the waves that are left over share rows, each with its half of every unit
-    const int map = MAPS == 2 ? wave & 1 : 0, rest = MAPS == 2 ? wave >> 1 : wave, groups = 4 / MAPS / wt;
-    const int rt = 32 * groups, rg = rest % groups, th = rest / groups;
-    part += th;
+    // the waves: one map and 32 rows each; wt = 2: two of them share rows, each with its half of every unit
+    const int map = MAPS == 2 ? wave & 1 : 0, rest = wave / MAPS, groups = SP_WAVES / MAPS / wt;
+    const int rt = 32 * groups, rg = wt == 2 ? rest >> 1 : rest, th = wt == 2 ? rest & 1 : 0;
 
     // ---- this lane's query row: positions outermost, so that a tile covers few of them
     const int j0 = tile * rt, j = j0 + 32 * rg + n, jc = j < rows ? j : rows - 1;
@@ -153,36 +184,17 @@ void span_mfma_kernel(SpanCall c) {
     }
     blk_lo = __builtin_amdgcn_readfirstlane(blk_lo); blk_hi = __builtin_amdgcn_readfirstlane(blk_hi);
 
-    // ---- the spans: live slots, place of the first, units that the block's rows see
-    const bool with_prefix = shared || !c.apart, with_own = !shared;
-    int live[4], at[4], first[4], end[4], total = 0;
-    live[0] = with_prefix ? (int)a.prefix.n_packed : 0;
-    live[1] = with_prefix ? (int)a.prefix.n_tail : 0;
-    live[2] = with_own ? (own_live < (int)a.own.n_packed ? own_live : (int)a.own.n_packed) : 0;
-    live[3] = with_own ? own_live - live[2] : 0;
-    at[0] = 0; at[1] = (int)a.prefix.n_packed; at[2] = before; at[3] = before + (int)a.own.n_packed;
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-        const int hi = blk_hi - at[s], lo = blk_lo - at[s];
-        const int seen = hi < 0 ? 0 : hi < live[s] ? hi : live[s];
-        first[s] = lo <= 0 ? 0 : lo / SP_UNIT;
-        const int units = (seen + SP_UNIT - 1) / SP_UNIT - first[s];
-        total += units > 0 ? units : 0;
-        end[s] = total;
-    }
-    const int w0 = (int)((int64_t)total * split / splits), w1 = (int)((int64_t)total * (split + 1) / splits);
-
-    struct Unit { int s, t0, place, live; };   // span, first token in it, its slot, live tokens of the span
-    auto unit = [&](int w) {
-        Unit u;
-        if (w < end[0]) u = {0, w + first[0], at[0], live[0]};
-        else if (w < end[1]) u = {1, w - end[0] + first[1], at[1], live[1]};
-        else if (w < end[2]) u = {2, w - end[1] + first[2], at[2], live[2]};
-        else u = {3, w - end[2] + first[3], at[3], live[3]};
-        u.t0 *= SP_UNIT;
-        u.place += u.t0;
-        return u;
+    // ---- the walk: prefix packed, prefix plain, own packed, own plain slots, in units that the block's rows see; this block's run of them
+    auto units_seen = [&](int place, int live) __attribute__((always_inline)) {
+        const int hi = blk_hi - place, seen = hi < live ? hi : live;
+        const int units = (seen + UNIT - 1) / UNIT - (blk_lo > place ? (blk_lo - place) / UNIT : 0);
+        return seen > 0 && units > 0 ? units : 0;
     };
+    const int np0 = shared || !c.apart ? (int)a.prefix.n_packed : 0, nt0 = shared || !c.apart ? (int)a.prefix.n_tail : 0;
+    const int own = shared ? 0 : own_live, np1 = own < (int)a.own.n_packed ? own : (int)a.own.n_packed, nt1 = own - np1;
+    const int tail0 = (int)a.prefix.n_packed, tail1 = before + (int)a.own.n_packed;   // places of the plain slots
+    const int total = units_seen(0, np0) + units_seen(tail0, nt0) + units_seen(before, np1) + units_seen(tail1, nt1);
+    const int w0 = (int)((int64_t)total * split / splits), w1 = (int)((int64_t)total * (split + 1) / splits);
 
     // ---- queries as the B operand: row n, channels 16 ks + 8 h .. + 7
     const float c2 = __builtin_fabsf(a.scale) * LOG2E;
@@ -204,107 +216,6 @@ void span_mfma_kernel(SpanCall c) {
     }
     const float cc = a.scale == 0.f ? 1.f : c2;
 
-    // ---- staging
-    const u32 lds0 = lds_addr(lds);
-    constexpr int COPIES = D / 32;   // copies of 1 KB a wave for a tile
-    struct Words { u32 k[BITS ? D / 32 : 1], v[BITS == 4 ? D / 32 : BITS == 2 ? D / 64 : 1]; };
-    constexpr int KROWS = SP_THREADS / CH;            // key tokens the threads cover at a time
-    constexpr int PER = BITS ? 32 / BITS : 8, KW = D / PER;
-    constexpr int VSTEPS = D / 64;                     // sixteen-token steps of a thread's channel
-    const u32 magic = BITS ? vreg_const(Magic<BITS ? BITS : 4>::bits) : 0u;
-    const int kc = tid % CH, kt = tid / CH;            // packed keys: 8-channel piece, token
-    const int vc = tid % D, vh = tid / D;              // packed values: channel, which of the unit's stretches
-    auto fetch = [&](const Unit &u, int buf, Words &wd) {
-        const vq_kv_store &s = u.s < 2 ? a.prefix : a.own;
-        const int64_t sb = u.s < 2 ? 0 : b;
-        const int last = u.live - 1 - u.t0;            // last live token of the unit, if it is not whole
-        if (BITS && !(u.s & 1)) {
-            const int64_t bh = sb * Hkv + hkv;
-            const u32 *kw = (const u32 *)s.k_packed + (bh * s.cap_tokens + u.t0) * KW;
-            const u32 *vw = (const u32 *)s.v_packed + (bh * (s.cap_tokens / PER) + u.t0 / PER) * D;
-#pragma unroll
-            for (int i = 0; i < D / 32; ++i) {
-                const int t = kt + KROWS * i;
-                wd.k[i] = kw[(t < last ? t : last) * KW + (BITS == 4 ? kc : kc / 2)];
-            }
-            const int lastw = last / PER;
-#pragma unroll
-            for (int i = 0; i < (int)(sizeof(wd.v) / 4); ++i) {
-                const int x = vh * (int)(sizeof(wd.v) / 4) + i;
-                wd.v[i] = vw[(x < lastw ? x : lastw) * D + vc];
-            }
-            return;
-        }
-        if (BITS && a.tail_dtype == VQ_BF16) return;   // (converted on the way: store_unit)
-        const int64_t ks = s.k_strides[2] * 2, vs = s.v_strides[2] * 2;
-        const char *kb = (const char *)s.k_tail + (sb * s.k_strides[0] + hkv * s.k_strides[1]) * 2 + u.t0 * ks;
-        const char *vb = (const char *)s.v_tail + (sb * s.v_strides[0] + hkv * s.v_strides[1]) * 2 + u.t0 * vs;
-#pragma unroll
-        for (int i = 0; i < COPIES; ++i) {
-            const int slot = (wave * COPIES + i) * 64 + lane, t = slot / CH, p = slot % CH;
-            const u32 r = (u32)(t < last ? t : last), dst = lds0 + buf * Tile::BUF + (wave * COPIES + i) * 1024;
-            lds_copy16<0>(kb, r * (u32)ks + sp_kpiece<D>(t, p) * 16, dst);
-            lds_copy16<0>(vb, r * (u32)vs + sp_vpiece<D>(t, p) * 16, dst + Tile::KEYS);
-        }
-    };
-    auto store_unit = [&](const Unit &u, int buf, const Words &wd) {
-        if (!BITS) return;
-        const vq_kv_store &s = u.s < 2 ? a.prefix : a.own;
-        const int64_t sb = u.s < 2 ? 0 : b;
-        const int last = u.live - 1 - u.t0;
-        char *kd = lds + buf * Tile::BUF, *vd = kd + Tile::KEYS;
-        if (u.s & 1) {
-            if (a.tail_dtype != VQ_BF16) return;
-            const u16 *kb = (const u16 *)s.k_tail + sb * s.k_strides[0] + hkv * s.k_strides[1] + u.t0 * s.k_strides[2];
-            const u16 *vb = (const u16 *)s.v_tail + sb * s.v_strides[0] + hkv * s.v_strides[1] + u.t0 * s.v_strides[2];
-            for (int i = 0; i < D / 32; ++i) {
-                const int t = kt + KROWS * i, r = t < last ? t : last;
-                *(f16x8 *)(kd + t * D * 2 + sp_kpiece<D>(t, kc) * 16) = ld_tail8(kb, r * s.k_strides[2] + 8 * kc, true);
-                *(f16x8 *)(vd + t * D * 2 + sp_vpiece<D>(t, kc) * 16) = ld_tail8(vb, r * s.v_strides[2] + 8 * kc, true);
-            }
-            return;
-        }
-        constexpr int BB = BITS ? BITS : 4;
-        const int gshift = __builtin_ctz(a.group);
-        const int64_t bh = sb * Hkv + hkv;
-        const int64_t kg = bh * (s.cap_tokens >> gshift);
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-            // the unit's first and second 32 tokens are one key group or two
-            const int t = kt + KROWS * i, g32 = KROWS * i / 32;
-            const int64_t g = (kg + ((u.t0 + (32 * g32 < last ? 32 * g32 : last)) >> gshift)) * D + 8 * kc;
-            u32 code[4];
-            sp_codes8<BB>(BITS == 2 ? wd.k[i] >> (16 * (kc & 1)) : wd.k[i], magic, code);
-            *(u32x4 *)(kd + t * D * 2 + sp_kpiece<D>(t, kc) * 16) =
-                sp_values8(code, *(const uint4 *)((const f16 *)s.k_scale + g), *(const uint4 *)((const f16 *)s.k_zero + g));
-        }
-        const int64_t vg = (bh * (D >> gshift) + (vc >> gshift)) * s.cap_tokens + u.t0;
-        const bool whole = last >= SP_UNIT - 1;
-#pragma unroll
-        for (int i = 0; i < VSTEPS; ++i) {
-            const int step = vh * VSTEPS + i;
-            u32x4 x[2];
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {   // eight tokens each
-                int t = 16 * step + 8 * k;
-                const int tc = t <= last ? t : last / 8 * 8;   // (past the live tokens: any that are)
-                u32 code[4];
-                sp_codes8<BB>(BITS == 4 ? wd.v[BITS == 4 ? 2 * i + k : 0] : wd.v[BITS == 4 ? 0 : i] >> (16 * k), magic, code);
-                x[k] = sp_values8(code, *(const uint4 *)((const f16 *)s.v_scale + vg + tc), *(const uint4 *)((const f16 *)s.v_zero + vg + tc));
-                if (!whole) {   // a token past the live ones may hold anything: its weight is zero, its value has to be finite
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        if (t + 2 * e > last) x[k][e] = 0u;
-                        else if (t + 2 * e + 1 > last) x[k][e] &= 0xFFFFu;
-                    }
-                }
-            }
-            u32x4 *dst = (u32x4 *)(vd + vc * SP_VROW + step * 32);
-            dst[0] = u32x4{x[0][0], x[0][1], x[1][0], x[1][1]};
-            dst[1] = u32x4{x[0][2], x[0][3], x[1][2], x[1][3]};
-        }
-    };
-
     // ---- state of the lane's row
     f32x16 O[DT];
     float m_run = -INFINITY, l_run = 0.f;
@@ -313,28 +224,64 @@ void span_mfma_kernel(SpanCall c) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) O[dt][r] = 0.f;
 
-    auto work = [&](const Unit &u, int buf, int half) {   // 32 slots of the unit
-        const char *kd = lds + buf * Tile::BUF, *vd = kd + Tile::KEYS;
-        const int place = u.place + 32 * half;
-        if (place >= any_hi || place + 32 <= any_lo || 32 * half >= u.live - u.t0) return;
+    // Where the lane's pieces of the operands lie in a tile: keys of slot n, its piece for channel step ks at key0 ^ 32 ks; row-major values
+    // for the transposing reads, channel tile dt at val0 ^ 64 dt; transposed values of channel n.
+    const u32 lds0 = lds_addr(lds);
+    const u32 key0 = n * D * 2 + sp_kpiece<D>(n, 2 * map * KS + h) * 16;
+    u32 val0;
+    {
+        const int i = lane & 15, t = 4 * h + (i >> 2);
+        val0 = t * D * 2 + sp_vpiece<D>(t, 2 * (lane >> 4 & 1) + ((i & 3) >> 1)) * 16 + (i & 1) * 8;
+    }
+    const u32 col0 = n * Tile::VROW + 16 * h;
+    using L4 = __attribute__((address_space(3))) const u32x4;
+    using LT = __attribute__((address_space(3))) s16x4;
+
+    // 32 slots of a tile at `tile`: the first one's slot, how many live ones the span has from there on
+    auto work = [&](auto transposed, u32 tile, int half, int place, int live) __attribute__((always_inline)) {
+        if (place >= any_hi || place + 32 <= any_lo || live <= 0) return;
         f32x16 S;
 #pragma unroll
         for (int r = 0; r < 16; ++r) S[r] = 0.f;
+        const u32 keys = tile + half * (32 * D * 2);
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-            S = M::mma(*(const u32x4 *)(kd + (32 * half + n) * D * 2 + sp_kpiece<D>(n, 2 * (map * KS + ks) + h) * 16), q[ks], S);
-        const int live_end = u.place + u.live - u.t0;   // slot past the span's live tokens
-        if (place + 32 > (all_hi < live_end ? all_hi : live_end) || place < all_lo) {
-            const int hi = (lane_hi < live_end ? lane_hi : live_end) - place - 4 * h, lo = lane_lo - place - 4 * h;
+        for (int k0 = 0; k0 < KS; k0 += KF) {   // the pieces of eight steps are asked for at once
+            u32x4 k[KF];
+#pragma unroll
+            for (int ks = 0; ks < KF; ++ks) k[ks] = *(L4 *)(uintptr_t)((key0 ^ (32 * (k0 + ks))) + keys);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int ks = 0; ks < KF; ++ks) S = M::mma(k[ks], q[k0 + ks], S);
+        }
+        // the values of the first sixteen slots are on their way while the weights are formed
+        const u32 values = tile + Tile::KEYS + (transposed.value ? half * 64 + col0 : half * (32 * D * 2));
+        auto value = [&](int s, int dt) __attribute__((always_inline)) {
+            if constexpr (transposed.value) {
+                return *(L4 *)(uintptr_t)(values + dt * (32 * Tile::VROW) + s * 32);
+            } else {
+                LT *row = (LT *)(uintptr_t)((val0 ^ (64 * dt)) + values);
+                const uint2 v0 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(row + s * 16 * D / 4));
+                const uint2 v1 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(row + (s * 16 + 8) * D / 4));
+                return u32x4{v0.x, v0.y, v1.x, v1.y};
+            }
+        };
+        u32x4 v[DT];
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) v[dt] = value(0, dt);
+        __builtin_amdgcn_sched_barrier(0);
+        const int end = place + live;
+        if (place + 32 > (all_hi < end ? all_hi : end) || place < all_lo) {
+            const int hi = (lane_hi < end ? lane_hi : end) - place - 4 * h, lo = lane_lo - place - 4 * h;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const int t = 8 * (r / 4) + r % 4;
                 if (t >= hi || t < lo) S[r] = -INFINITY;
             }
         }
-        float mx = fmaxf(S[0], S[1]);
+        float mx = sp_max3(S[0], S[1], S[2]);
 #pragma unroll
-        for (int r = 2; r < 16; ++r) mx = fmaxf(mx, S[r]);
+        for (int r = 3; r < 15; r += 2) mx = sp_max3(mx, S[r], S[r + 1]);
+        mx = sp_max3(mx, S[15], S[15]);
         if (__any(mx * cc > m_run + RESCALE_SLACK)) {
             const float top = fmaxf(mx, __shfl_xor(mx, 32)) * cc, m = fmaxf(m_run, top);
             const float alpha = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - m);
@@ -346,66 +293,287 @@ void span_mfma_kernel(SpanCall c) {
                 for (int r = 0; r < 16; ++r) O[dt][r] *= alpha;
         }
         const float nm = m_run == -INFINITY ? 0.f : -m_run;
-        u32 P[8];
+        u32x4 P[2];
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
-            P[r] = M::pack(__builtin_amdgcn_exp2f(__builtin_fmaf(S[2 * r], cc, nm)), __builtin_amdgcn_exp2f(__builtin_fmaf(S[2 * r + 1], cc, nm)));
-            l_run = M::add_pair(P[r], l_run);
+            const u32 p = M::pack(__builtin_amdgcn_exp2f(__builtin_fmaf(S[2 * r], cc, nm)), __builtin_amdgcn_exp2f(__builtin_fmaf(S[2 * r + 1], cc, nm)));
+            P[r / 4][r % 4] = p;
+            l_run = M::add_pair(p, l_run);
         }
-        const bool transposed = BITS && !(u.s & 1);
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
+        for (int dt = 0; dt < DT; ++dt) {   // (the next sixteen slots' piece is asked for as its place falls free)
+            O[dt] = M::mma(v[dt], P[0], O[dt]);
+            v[dt] = value(1, dt);
+        }
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt) {
-                u32x4 v;
-                if (transposed) {
-                    v = *(const u32x4 *)(vd + (32 * dt + n) * SP_VROW + (2 * half + s) * 32 + 16 * h);
-                } else {
-                    const int i = lane & 15, t = 4 * h + (i >> 2), p = 4 * dt + 2 * (lane >> 4 & 1) + ((i & 3) >> 1);
-                    const char *row = vd + (32 * half + 16 * s + t) * D * 2 + sp_vpiece<D>(t, p) * 16 + (i & 1) * 8;
-                    using L = __attribute__((address_space(3))) s16x4;
-                    const uint2 v0 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((L *)(uintptr_t)lds_addr(row)));
-                    const uint2 v1 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((L *)(uintptr_t)lds_addr(row + 8 * D * 2)));
-                    v = u32x4{v0.x, v0.y, v1.x, v1.y};
+        for (int dt = 0; dt < DT; ++dt) O[dt] = M::mma(v[dt], P[1], O[dt]);
+    };
+    const int half0 = th, half1 = wt == 1 ? Tile::HALVES : th + 1;
+    auto compute = [&](auto transposed, u32 tile, int place, int live) __attribute__((always_inline)) {
+        if (!wave_works) return;
+#pragma unroll 1
+        for (int half = half0; half < half1; ++half) work(transposed, tile, half, place + 32 * half, live - 32 * half);
+    };
+
+    // ---- one span after the other.  A store's fields are read from the argument block where a span begins (`fresh` hides the block's
+    // address from the compiler, which would hold all of them in scalar registers from the start and spill those).
+    using Args = const __attribute__((address_space(4))) SpanCall;
+    using Store = const __attribute__((address_space(4))) vq_kv_store;
+    auto fresh = []() __attribute__((always_inline)) {
+        Args *p = (Args *)__builtin_amdgcn_kernarg_segment_ptr();
+        asm volatile("" : "+s"(p));
+        return p;
+    };
+    // `count` units of plain rows from row t0 on
+    auto walk_rows = [&](int which, int t0, int count, int place, int live) __attribute__((always_inline)) {
+        Args *args = fresh();
+        Store *s = &args->a.prefix + which;
+        const int64_t sb = which ? b : 0;
+        const int64_t ks = s->k_strides[2] * 2, vs = s->v_strides[2] * 2;
+        const char *kb = (const char *)s->k_tail + (sb * s->k_strides[0] + hkv * s->k_strides[1]) * 2 + t0 * ks;
+        const char *vb = (const char *)s->v_tail + (sb * s->v_strides[0] + hkv * s->v_strides[1]) * 2 + t0 * vs;
+        if (BITS && args->a.tail_dtype == VQ_BF16) {   // converted on the way, a unit at a time
+#pragma unroll 1
+            for (int i = 0; i < count; ++i, kb += UNIT * ks, vb += UNIT * vs, place += UNIT, live -= UNIT) {
+                for (int x = tid; x < UNIT * CH; x += SP_THREADS) {
+                    const int t = x / CH, p = x % CH, r = t < live ? t : live - 1;
+                    *(f16x8 *)(lds + t * D * 2 + sp_kpiece<D>(t, p) * 16) = ld_tail8(kb + r * ks, 8 * p, true);
+                    *(f16x8 *)(lds + Tile::KEYS + t * D * 2 + sp_vpiece<D>(t, p) * 16) = ld_tail8(vb + r * vs, 8 * p, true);
                 }
-                O[dt] = M::mma(v, u32x4{P[4 * s], P[4 * s + 1], P[4 * s + 2], P[4 * s + 3]}, O[dt]);
+                lds_barrier();
+                compute(std::false_type{}, lds0, place, live);
+                lds_barrier();
             }
+            return;
+        }
+        constexpr int AHEAD = Tile::ROW_BUFS - 1, N = Tile::KEYS / 1024 / SP_WAVES;   // units asked for ahead; copies a wave for the keys of one
+        u32 koff[N], voff[N];   // of the lane's pieces, in a whole unit
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int slot = (wave * N + i) * 64 + lane, t = slot / CH, p = slot % CH;
+            koff[i] = (u32)t * (u32)ks + sp_kpiece<D>(t, p) * 16;
+            voff[i] = (u32)t * (u32)vs + sp_vpiece<D>(t, p) * 16;
+        }
+        u32 fill = lds0 + wave * N * 1024, tile = lds0;
+        const u32 past = lds0 + Tile::ROW_BUFS * Tile::ROW_BUF;
+        int asked_live = live;
+        auto fetch = [&]() __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                u32 ko = koff[i], vo = voff[i];
+                if (asked_live < UNIT) {   // a row past the live ones repeats the last
+                    const int slot = (wave * N + i) * 64 + lane, t = slot / CH;
+                    const int r = t < asked_live ? t : asked_live - 1;   // (the pieces' order goes by the tile's row)
+                    ko = (u32)r * (u32)ks + sp_kpiece<D>(t, slot % CH) * 16;
+                    vo = (u32)r * (u32)vs + sp_vpiece<D>(t, slot % CH) * 16;
+                }
+                lds_copy16<0>(kb, ko, fill + i * 1024);
+                lds_copy16<0>(vb, vo, fill + i * 1024 + Tile::KEYS);
+            }
+            kb += UNIT * ks;
+            vb += UNIT * vs;
+            asked_live -= UNIT;
+            fill += Tile::ROW_BUF;
+            if (fill >= past) fill -= Tile::ROW_BUFS * Tile::ROW_BUF;
+        };
+#pragma unroll 1
+        for (int i = 0; i < AHEAD && i < count; ++i) fetch();
+#pragma unroll 1
+        for (int i = 0; i < count; ++i, place += UNIT, live -= UNIT) {
+            // the unit is here once the copies of at most AHEAD - 1 later ones are under way; past the barrier every wave has left the
+            // tile before it, the next to be filled
+            if (i + AHEAD <= count) wait_copies<(AHEAD - 1) * 2 * N>();
+            else wait_copies<0>();
+            lds_barrier();
+            if (i + AHEAD < count) fetch();
+            compute(std::false_type{}, tile, place, live);
+            tile += Tile::ROW_BUF;
+            if (tile == past) tile = lds0;
+        }
+        lds_barrier();   // the tiles are free
+    };
+    // `count` units of packed slots from slot t0 on
+    auto walk_packed = [&](auto which, int t0, int count, int place, int live) __attribute__((always_inline)) {   // (a template: plain rows have none)
+        constexpr int BB = BITS ? BITS : 4, PER = 32 / BB, KW = D / PER, RAWS = Tile::RAWS, N = Tile::COPIES;
+        Args *args = fresh();
+        Store *s = &args->a.prefix + which;
+        const int gshift = __builtin_ctz(args->a.group);
+        const int64_t bh = (which ? (int64_t)b : 0) * Hkv + hkv, cap = s->cap_tokens;
+        const char *kw = (const char *)s->k_packed + bh * cap * KW * 4, *vw = (const char *)s->v_packed + bh * (cap / PER) * D * 4;
+        const char *ks = (const char *)s->k_scale + bh * (cap >> gshift) * D * 2, *kz = (const char *)s->k_zero + bh * (cap >> gshift) * D * 2;
+        const char *vs = (const char *)s->v_scale + bh * (D >> gshift) * cap * 2, *vz = (const char *)s->v_zero + bh * (D >> gshift) * cap * 2;
+        // The unit as it lies in memory: a piece of 1 KB a copy, the pieces dealt to the waves (as many copies a wave: spare ones repeat the
+        // last piece).  What lies past the live slots is not read: a lane whose sixteen bytes would start there repeats the last ones before.
+        constexpr int MP = Tile::META / 16, TP = UNIT / 8;   // scales and zeros: [32 slots][which][pieces of channels], then [32 channels][which][pieces of slots]
+        auto piece_of = [&](int i) __attribute__((always_inline)) {
+            const int p = i * SP_WAVES + wave;
+            return p < Tile::PIECES ? p : Tile::PIECES - 1;
+        };
+        auto lane_at = [&](int i, int n_live) __attribute__((always_inline)) -> const char * {   // in the span's first unit
+            const int p = piece_of(i);
+            int off = p * 1024 + lane * 16;
+            if (p < Tile::KWORDS / 1024) {
+                const int last = n_live * KW * 4 - 16;
+                return kw + (off < last ? off : last);
+            }
+            off -= Tile::KWORDS;
+            if (p < 2 * Tile::KWORDS / 1024) {
+                const int last = (n_live + PER - 1) / PER * D * 4 - 16;
+                return vw + (off < last ? off : last);
+            }
+            const int x = (off - Tile::KWORDS) / 16, y = x - MP;
+            if (x < MP) {
+                const int t = 32 * (x / (2 * CH)), tc = t < n_live ? t : n_live - 1;
+                return sp_pick((x / CH & 1) != 0, kz, ks) + (tc >> gshift) * D * 2 + x % CH * 16;
+            }
+            const int t = y % TP * 8, tc = t < n_live ? t : (n_live - 1) / 8 * 8;
+            return sp_pick((y / TP & 1) != 0, vz, vs) + ((y / (2 * TP) * 32 >> gshift) * cap + tc) * 2;
+        };
+        const char *at[N ? N : 1];
+#pragma unroll
+        for (int i = 0; i < N; ++i) at[i] = lane_at(i, UNIT);
+        const u32 raw0 = lds0 + Tile::BUFS * Tile::BUF;
+        int asked = t0, asked_live = live;
+        u32 fill = raw0;
+        auto fetch = [&]() __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int p = piece_of(i);
+                const char *from = at[i];
+                if (asked_live < UNIT) from = lane_at(i, asked_live);
+                if (p < Tile::KWORDS / 1024) from += (int64_t)asked * (KW * 4);
+                else if (p < 2 * Tile::KWORDS / 1024) from += (int64_t)(asked / PER) * (D * 4);
+                else from += p * 1024 + lane * 16 - 2 * Tile::KWORDS < Tile::META ? (int64_t)(asked >> gshift) * (D * 2) : (int64_t)asked * 2;
+                span_copy16(from, fill + p * 1024);
+            }
+            asked += UNIT;
+            asked_live -= UNIT;
+            fill += Tile::RAW;
+            if (fill == raw0 + RAWS * Tile::RAW) fill = raw0;
+        };
+        // a unit from the ring into a tile
+        const u32 magic = vreg_const(Magic<BB>::bits);
+        const int kc = tid % CH, kt = tid / CH;            // keys: 8-channel piece, slot
+        const int vc = tid % D, step = tid / D;            // values: channel, sixteen slots
+        constexpr int KROWS = SP_THREADS / CH;             // slots that the threads cover at a time
+        char *take = lds + Tile::BUFS * Tile::BUF;
+        auto build = [&](u32 buf, int n_live) __attribute__((always_inline)) {
+            char *kd = lds + buf, *vd = kd + Tile::KEYS;
+            const char *raw = take;
+            const uint4 *kmeta = (const uint4 *)(raw + 2 * Tile::KWORDS);
+            const uint4 *vmeta = (const uint4 *)(raw + 2 * Tile::KWORDS + Tile::META);
+#pragma unroll
+            for (int i = 0; i < UNIT / KROWS; ++i) {
+                const int t = kt + KROWS * i;
+                const u32 w = ((const u32 *)raw)[t * KW + (BB == 4 ? kc : kc / 2)];
+                u32 code[4];
+                sp_codes8<BB>(BB == 2 ? w >> (16 * (kc & 1)) : w, magic, code);
+                *(u32x4 *)(kd + t * D * 2 + sp_kpiece<D>(t, kc) * 16) = sp_values8(code, kmeta[t / 32 * 2 * CH + kc], kmeta[(t / 32 * 2 + 1) * CH + kc]);
+            }
+            if (step < UNIT / 16) {
+                const u32 *words = (const u32 *)(raw + Tile::KWORDS) + vc;
+                const uint4 *meta = vmeta + vc / 32 * 2 * TP + 2 * step;
+                u32x4 x[2];
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {   // eight slots each
+                    const u32 w = BB == 4 ? words[(2 * step + k) * D] : words[step * D] >> (16 * k);
+                    u32 code[4];
+                    sp_codes8<BB>(w, magic, code);
+                    x[k] = sp_values8(code, meta[k], meta[TP + k]);
+                }
+                if (n_live < UNIT) {   // a slot past the live ones may hold anything: its weight is zero, its value has to be finite
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int t = 16 * step + 8 * k + 2 * e;
+                            x[k][e] = t >= n_live ? 0u : t + 1 >= n_live ? x[k][e] & 0xFFFFu : x[k][e];
+                        }
+                }
+                u32x4 *dst = (u32x4 *)(vd + vc * Tile::VROW + step * 32);
+                dst[0] = u32x4{x[0][0], x[0][1], x[1][0], x[1][1]};
+                dst[1] = u32x4{x[0][2], x[0][3], x[1][2], x[1][3]};
+            }
+            take += Tile::RAW;
+            if (take == lds + Tile::BUFS * Tile::BUF + RAWS * Tile::RAW) take -= RAWS * Tile::RAW;
+        };
+#pragma unroll 1
+        for (int i = 0; i < RAWS - 1 && i < count; ++i) fetch();
+        if (count >= RAWS - 1) wait_copies<(RAWS - 3) * N>();
+        else wait_copies<0>();
+        lds_barrier();
+        build(0, live);
+        lds_barrier();
+        u32 buf = 0;
+#pragma unroll 1
+        for (int i = 0; i < count; ++i, place += UNIT, live -= UNIT) {
+            // unit i is in its tile, unit i + 1 in the ring; into the slot that unit i - 1 has left
+            const bool more = i + 1 < count, deep = i + RAWS - 1 < count;
+            if (deep) fetch();
+            if (more && wave < SP_WAVES / 2) build(Tile::BUF - buf, live - UNIT);
+            compute(std::true_type{}, lds0 + buf, place, live);
+            if (more && wave >= SP_WAVES / 2) build(Tile::BUF - buf, live - UNIT);
+            if (deep) wait_copies<(RAWS - 3) * N>();   // unit i + 2 is in the ring once at most units i + 3 .. i + RAWS - 1 are under way
+            else wait_copies<0>();
+            lds_barrier();
+            buf = Tile::BUF - buf;
         }
     };
-    const int half0 = wt == 1 ? 0 : th, half1 = wt == 1 ? 2 : th + 1;
-
-    if (w0 < w1) {
-        Words wd;
-        Unit u = unit(w0);
-        fetch(u, 0, wd);
-        store_unit(u, 0, wd);
-        wait_copies<0>();
-        lds_barrier();
-        int buf = 0;
-        for (int w = w0; w < w1; ++w, buf ^= 1) {
-            const bool more = w + 1 < w1;
-            Unit next = u;
-            if (more) {
-                next = unit(w + 1);
-                fetch(next, buf ^ 1, wd);
-            }
-            if (wave_works) {
+    {
+        int skip = w0, left = w1 - w0;
 #pragma unroll 1
-                for (int half = half0; half < half1; ++half) work(u, buf, half);
-            }
-            if (more) {
-                store_unit(next, buf ^ 1, wd);
-                wait_copies<0>();
-                lds_barrier();
-                u = next;
+        for (int which = 0; which < 2 && left > 0; ++which) {
+#pragma unroll
+            for (int plain = 0; plain < 2; ++plain) {
+                const int at = which ? (plain ? +tail1 : +before) : (plain ? +tail0 : 0), live = which ? (plain ? +nt1 : +np1) : (plain ? +nt0 : +np0);
+                const int units = units_seen(at, live);
+                const int mine = units - skip < left ? units - skip : left;
+                if (mine > 0) {
+                    const int t0 = ((blk_lo > at ? (blk_lo - at) / UNIT : 0) + skip) * UNIT;
+                    if (plain) walk_rows(which, t0, mine, at + t0, live - t0);
+                    else if constexpr (BITS != 0) walk_packed(which, t0, mine, at + t0, live - t0);
+                    left -= mine;
+                    skip = 0;
+                } else {
+                    skip -= units;
+                }
             }
         }
     }
 
-    // ---- results
-    float l = l_run + __shfl_xor(l_run, 32);   // both halves of a row
+    // ---- results: the other half's part of the row, then the other map's
+    float l = l_run + __shfl_xor(l_run, 32);   // both lanes of a row
+    float4 *room = (float4 *)lds + (map * groups + rg) * (D / 8 * 64 + 64) + lane;   // 4 floats a lane and quarter of a channel tile; sum and maximum
+    if (wt == 2) {
+        lds_barrier();
+        if (th == 1) {
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) room[(4 * dt + r) * 64] = make_float4(O[dt][4 * r], O[dt][4 * r + 1], O[dt][4 * r + 2], O[dt][4 * r + 3]);
+            room[DT * 4 * 64] = make_float4(m_run, l, 0.f, 0.f);
+        }
+        lds_barrier();
+        if (th == 0) {
+            const float4 ml = room[DT * 4 * 64];
+            const float m = fmaxf(m_run, ml.x);
+            const float f0 = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - m), f1 = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ml.x - m);
+            m_run = m;
+            l = l * f0 + ml.y * f1;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float4 x = room[(4 * dt + r) * 64];
+                    O[dt][4 * r] = O[dt][4 * r] * f0 + x.x * f1;
+                    O[dt][4 * r + 1] = O[dt][4 * r + 1] * f0 + x.y * f1;
+                    O[dt][4 * r + 2] = O[dt][4 * r + 2] * f0 + x.z * f1;
+                    O[dt][4 * r + 3] = O[dt][4 * r + 3] * f0 + x.w * f1;
+                }
+        }
+    }
     if (c.nparts > 1) {
-        if (j >= rows) return;
+        if (th == 1 || j >= rows) return;
         const int64_t rec = (qrow * c.nparts + part) * MAPS + map;
         if (h == 0) *(float2 *)(c.ml + rec * 2) = make_float2(m_run, l);
         float *dst = c.sums + rec * D + 4 * h;
@@ -423,23 +591,21 @@ void span_mfma_kernel(SpanCall c) {
         for (int r = 0; r < 16; ++r) O[dt][r] *= by;
     bool norm = false;
     if (MAPS == 2) {
-        // the second map's wave hands its rows over in LDS, a channel tile's quarter of 4 floats a lane at a time
-        static_assert(Tile::LDS >= 2 * D * 32 * 4 || MAPS == 1, "room for the rows of both row groups");
-        float4 *room = (float4 *)lds + rg * (D / 8) * 64 + lane;
+        float4 *other = (float4 *)lds + rg * (D / 8) * 64 + lane;
         lds_barrier();
-        if (map == 1) {
+        if (map == 1 && th == 0) {
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) room[(4 * dt + r) * 64] = make_float4(O[dt][4 * r], O[dt][4 * r + 1], O[dt][4 * r + 2], O[dt][4 * r + 3]);
+                for (int r = 0; r < 4; ++r) other[(4 * dt + r) * 64] = make_float4(O[dt][4 * r], O[dt][4 * r + 1], O[dt][4 * r + 2], O[dt][4 * r + 3]);
         }
         lds_barrier();
-        if (map == 1) return;
+        if (map == 1 || th == 1) return;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const float4 x = room[(4 * dt + r) * 64];
+                const float4 x = other[(4 * dt + r) * 64];
                 O[dt][4 * r] += x.x; O[dt][4 * r + 1] += x.y; O[dt][4 * r + 2] += x.z; O[dt][4 * r + 3] += x.w;
             }
         gain = a.gain;
@@ -452,7 +618,7 @@ void span_mfma_kernel(SpanCall c) {
             gain /= sqrtf((sq + __shfl_xor(sq, 32)) * (1.f / D) + a.norm_eps);
         }
     }
-    if (j >= rows) return;
+    if (th == 1 || j >= rows) return;
     u16 *dst = (u16 *)a.out + qrow * D + 4 * h;
     const bool out_bf16 = a.dtype == VQ_BF16;
 #pragma unroll
