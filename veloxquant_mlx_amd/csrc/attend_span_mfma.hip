@@ -1,5 +1,5 @@
 // Which calls the matrix-unit kernel takes, how it cuts them, its launch.
-#include "attend_span_mfma.hpp"
+#include "attend_span_few.hpp"
 
 namespace vq {
 
@@ -28,33 +28,45 @@ bool span_mfma_supported(const vq_store_attend_args &a) {
 
 void span_mfma_plan(SpanCall &c, int maps) {
     const vq_store_attend_args &a = c.a;
-    const int64_t unit = a.D == 256 ? 32 : 64;
-    auto units_of = [&](const vq_kv_store &s) { return cdiv(s.n_packed, unit) + cdiv(s.n_tail, unit); };
-    const int64_t r1 = a.Hq / a.Hkv * a.Sq, all = a.B * r1, prefix = units_of(a.prefix), own = units_of(a.own);
-    const int most = 32 * SP_WAVES / maps;   // rows of a block
+    const bool packed = a.prefix.n_packed + a.own.n_packed > 0;
+    const int64_t r1 = a.Hq / a.Hkv * a.Sq, all = a.B * r1;
+    const int most = 32 * SP_WAVES / maps, few = 32 / maps;   // rows of a block of the one kernel, of the other
+    auto units_of = [](const vq_kv_store &s, int64_t unit) { return cdiv(s.n_packed, unit) + cdiv(s.n_tail, unit); };
     // the prefix in blocks of its own where a sequence's rows fill half a block or less
-    c.apart = prefix > 0 && a.B > 1 && r1 <= most / 2;
-    auto tiling = [&](int64_t rows, int &wt, int &tiles) {
-        wt = a.D != 256 && rows <= most / 2 ? 2 : 1;
-        tiles = (int)cdiv(rows, most / wt);
-    };
-    tiling(all, c.pwt, c.ptiles);
-    tiling(r1, c.owt, c.otiles);
-    // one round of blocks of equal runs, one block a CU; sequences that differ in length even out over four rounds
+    const bool prefix_slots = a.prefix.n_packed + a.prefix.n_tail > 0;
+    c.apart = prefix_slots && a.B > 1 && r1 <= most / 2;
+    c.pfew = packed && all <= few;
+    c.ofew = packed && r1 <= few;
+    // One round of blocks of equal runs, one block a CU, each side for itself where they are launches of their own; sequences that differ
+    // in length even out over four rounds.  A run is four units a wave or more for few rows, four units a block else.
     const int64_t round = a.seq_lens != nullptr ? 1024 : 256;
-    const int64_t walk = c.apart ? own : prefix + own;
-    const int64_t work = (c.apart ? a.Hkv * c.ptiles * prefix : 0) + a.B * a.Hkv * c.otiles * walk;
-    int64_t run = cdiv(work, round);
-    if (run < 4) run = 4;
-    c.psplits = c.apart ? (int)cdiv(prefix, run) : 0;
-    c.osplits = walk > 0 ? (int)cdiv(walk, run) : 0;
+    auto side = [&](bool by_few, int64_t rows, int64_t slots32, int64_t slots64, int64_t times, int &wt, int &tiles, int64_t &units, int64_t &least) {
+        wt = !by_few && a.D != 256 && rows <= most / 2 ? 2 : 1;
+        tiles = by_few ? 1 : (int)cdiv(rows, most / wt);
+        units = by_few || a.D == 256 ? slots32 : slots64;
+        least = by_few ? (a.D == 256 ? 16 : 32) : 4;
+        return times * a.Hkv * tiles * units;   // units of all blocks
+    };
+    const int64_t p32 = units_of(a.prefix, 32), p64 = units_of(a.prefix, 64), o32 = units_of(a.own, 32), o64 = units_of(a.own, 64);
+    int64_t pu = 0, ou = 0, pleast, oleast, pwork = 0, owork;
+    if (c.apart) pwork = side(c.pfew, all, p32, p64, 1, c.pwt, c.ptiles, pu, pleast);
+    owork = side(c.ofew, r1, c.apart ? o32 : p32 + o32, c.apart ? o64 : p64 + o64, a.B, c.owt, c.otiles, ou, oleast);
+    const bool together = c.apart && c.pfew == c.ofew;
+    auto cut = [&](int64_t units, int64_t work, int64_t least) {
+        int64_t run = cdiv(together ? pwork + owork : work, round);
+        run = run < least ? least : run;
+        return (int)cdiv(units, run);
+    };
+    c.psplits = c.apart ? cut(pu, pwork, pleast) : 0;
+    c.osplits = cut(ou, owork, oleast);
     c.nparts = c.psplits + c.osplits;
 }
 
 int launch_span_mfma(const SpanCall &c, int maps) {
     const vq_store_attend_args &a = c.a;
-    if (a.prefix.n_packed + a.own.n_packed > 0) return a.pack_bits == 4 ? launch_span_packed4(c, maps) : launch_span_packed2(c, maps);
-    return a.dtype == VQ_F16 ? launch_span_rows_f16(c, maps) : launch_span_rows_bf16(c, maps);
+    if (a.prefix.n_packed + a.own.n_packed == 0) return a.dtype == VQ_F16 ? launch_span_rows_f16(c, maps) : launch_span_rows_bf16(c, maps);
+    if (int rc = a.pack_bits == 4 ? launch_span_packed4(c, maps) : launch_span_packed2(c, maps)) return rc;
+    return a.pack_bits == 4 ? launch_span_few4(c, maps) : launch_span_few2(c, maps);
 }
 
 }  // namespace vq

@@ -87,7 +87,8 @@ __device__ __forceinline__ void span_copy16(const void *from, u32 lds) {
 }
 #pragma clang diagnostic pop
 
-// bare three-way maximum (fmaxf canonicalises its operands first)
+// bare three-way maximum (fmaxf canonicalises its operands first); not the first reader of a matrix product, whose result the
+// compiler does not wait for on behalf of inline assembly
 __device__ __forceinline__ float sp_max3(float x, float y, float z) {
     float r;
     asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
@@ -95,6 +96,28 @@ __device__ __forceinline__ float sp_max3(float x, float y, float z) {
 }
 // a choice between two values (between two places, as `c ? x : y` may become, it would move both to scratch memory)
 template <typename T> __device__ __forceinline__ T sp_pick(bool c, T x, T y) { return c ? x : y; }
+
+__device__ __forceinline__ u32 sp_bf16_to_f16(u32 x) { return as_u(f16x2{(f16)bf16_to_f32((u16)x), (f16)bf16_to_f32((u16)(x >> 16))}); }
+__device__ __forceinline__ u32x4 sp_bf16_to_f16(u32x4 x) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = sp_bf16_to_f16(x[i]);
+    return x;
+}
+// N adjacent words
+template <int N> __device__ __forceinline__ void sp_load_words(const char *p, u32 (&w)[N]) {
+    if constexpr (N == 1) {
+        w[0] = *(const u32 *)p;
+    } else if constexpr (N == 2) {
+        const uint2 x = *(const uint2 *)p;
+        w[0] = x.x; w[1] = x.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            const uint4 x = *(const uint4 *)(p + 4 * i);
+            w[i] = x.x; w[i + 1] = x.y; w[i + 2] = x.z; w[i + 3] = x.w;
+        }
+    }
+}
 
 template <int BITS, int D> struct SpanTile {
     static constexpr int UNIT = D == 256 ? 32 : 64;      // slots a unit
@@ -133,7 +156,7 @@ __global__ __launch_bounds__(SP_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
     // ---- the block: kv head fastest (blocks of one kv head and run, which read the same slots, lie a multiple of the head count
     // apart), under a causal mask the row tiles that see most first
     int id = (int)blockIdx.x;
-    const int shared_blocks = c.apart ? c.psplits * c.ptiles * Hkv : 0;
+    const int shared_blocks = c.apart && !c.pfew ? c.psplits * c.ptiles * Hkv : 0;
     const bool shared = id < shared_blocks;
     int b = 0, split, tile, splits, wt, rows, part;
     const int hkv = shared ? id % Hkv : (id - shared_blocks) % Hkv;
@@ -206,10 +229,7 @@ __global__ __launch_bounds__(SP_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             u32x4 x = *(const u32x4 *)(src + 16 * ks);
-            if (sizeof(T) == 2 && BITS != 0 && q_bf16) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) x[i] = as_u(f16x2{(f16)bf16_to_f32((u16)x[i]), (f16)bf16_to_f32((u16)(x[i] >> 16))});
-            }
+            if (BITS != 0 && q_bf16) x = sp_bf16_to_f16(x);
 #pragma unroll
             for (int i = 0; i < 4; ++i) q[ks][i] = a.scale == 0.f ? 0u : x[i] ^ sign;
         }
@@ -278,10 +298,9 @@ __global__ __launch_bounds__(SP_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
                 if (t >= hi || t < lo) S[r] = -INFINITY;
             }
         }
-        float mx = sp_max3(S[0], S[1], S[2]);
+        float mx = fmaxf(S[0], S[1]);   // (first: the compiler waits for the products only before instructions of its own)
 #pragma unroll
-        for (int r = 3; r < 15; r += 2) mx = sp_max3(mx, S[r], S[r + 1]);
-        mx = sp_max3(mx, S[15], S[15]);
+        for (int r = 2; r < 16; r += 2) mx = sp_max3(mx, S[r], S[r + 1]);
         if (__any(mx * cc > m_run + RESCALE_SLACK)) {
             const float top = fmaxf(mx, __shfl_xor(mx, 32)) * cc, m = fmaxf(m_run, top);
             const float alpha = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - m);
@@ -637,20 +656,26 @@ __global__ __launch_bounds__(SP_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
         }
 }
 
+// More than 64 KB of block-shared memory has to be allowed per kernel and device, once (a second setter repeats the same call).
+inline int span_allow_lds(const void *kernel, int bytes, std::atomic<bool> *allowed) {
+    if (bytes <= 64 * 1024) return VQ_OK;
+    int dev = 0;
+    (void)hipGetDevice(&dev);
+    if (dev >= 0 && dev < 64 && allowed[dev].load(std::memory_order_acquire)) return VQ_OK;
+    const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    VQ_REQUIRE(e == hipSuccess, VQ_ERR_HIP, "attention over spans: %d bytes of block-shared memory: %s", bytes, hipGetErrorString(e));
+    if (dev >= 0 && dev < 64) allowed[dev].store(true, std::memory_order_release);
+    return VQ_OK;
+}
+
 template <int BITS, typename T, int D, int MAPS> int launch_span_mfma_as(const SpanCall &c) {
     constexpr int bytes = SpanTile<BITS, D>::LDS;
     const auto kernel = span_mfma_kernel<BITS, T, D, MAPS>;
-    if (bytes > 64 * 1024) {   // has to be allowed per kernel and device, once; a second setter repeats the same call
-        static std::atomic<bool> allowed[64] = {};
-        int dev = 0;
-        (void)hipGetDevice(&dev);
-        if (dev < 0 || dev >= 64 || !allowed[dev].load(std::memory_order_acquire)) {
-            (void)hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-            if (dev >= 0 && dev < 64) allowed[dev].store(true, std::memory_order_release);
-        }
-    }
-    const int64_t blocks = (c.apart ? (int64_t)c.psplits * c.ptiles * c.a.Hkv : 0) + c.a.B * c.a.Hkv * c.otiles * c.osplits;
-    VQ_REQUIRE(blocks < (INT64_C(1) << 24), VQ_ERR_UNSUPPORTED, "attention over spans: too many sequences and heads for one launch");
+    static std::atomic<bool> allowed[64] = {};
+    if (int rc = span_allow_lds((const void *)kernel, bytes, allowed)) return rc;
+    const int64_t blocks = (c.apart && !c.pfew ? (int64_t)c.psplits * c.ptiles * c.a.Hkv : 0) + (c.ofew ? 0 : c.a.B * c.a.Hkv * c.otiles * c.osplits);
+    if (blocks == 0) return VQ_OK;
+    VQ_REQUIRE(blocks < (INT64_C(1) << 23), VQ_ERR_UNSUPPORTED, "attention over spans: too many sequences and heads for one launch");
     kernel<<<(unsigned)blocks, SP_THREADS, bytes, (hipStream_t)c.a.stream>>>(c);
     VQ_HIP_CHECK_LAUNCH("attention over spans");
     return VQ_OK;
