@@ -23,7 +23,7 @@ def _args(**kw):
     (dict(B=0), "bad sizes"), (dict(Hq=7), "multiple of H_kv"), (dict(D=300), "must be <= 256"), (dict(dtype=_lib.VQ_U8), "q/out dtype"),
     (dict(own__n_tail=0), "no key/value slots"), (dict(own__n_tail=-1), "negative token count"), (dict(own__k_tail=None), "null tail pointer"),
     (dict(tail_dtype=_lib.VQ_I32), "tail dtype"), (dict(own__n_packed=64), "null packed pointer"), (dict(sliding_window=-1), "sliding window"),
-    (dict(causal=1, Sq=301), "exceeds"), (dict(q=None), "null q"), (dict(own__n_tail=1 << 30), "2.30 slots"), (dict(B=1 << 28), "query rows")])
+    (dict(causal=1, Sq=301), "exceeds"), (dict(q=None), "null q"), (dict(own__n_tail=1 << 30), "2.30 slots"), (dict(B=1 << 25), "query rows")])
 @pytest.mark.parametrize("call", ["vq_shared_prefix_attend", "vq_differential_attend"])
 def test_refused(call, kw, what):
     lib = _lib.load()

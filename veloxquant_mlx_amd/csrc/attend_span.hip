@@ -111,64 +111,95 @@ template <int MAPS> __global__ __launch_bounds__(256) void span_any_kernel(SpanC
     }
 }
 
-// One wave a row: the parts' sums at their common maximum, over the sum of the weights; of two maps the difference, and the
-// head's norm.  A row that sees nothing is zero.
-template <int MAPS> __global__ __launch_bounds__(256) void span_merge_kernel(SpanCall c) {
+// The parts' sums at their common maximum, over the sum of the weights; of two maps the difference, and the head's norm.  A row that sees
+// nothing is zero.  Bound by latency: WAVES waves a row, each with every WAVES-th eight parts, whose sums are asked for at once
+// (one wave and one part at a time took 46 us for 840 rows of 68 parts, this 6).
+constexpr int MERGE_AT_ONCE = 8;
+template <int MAPS, int WAVES> __global__ __launch_bounds__(256) void span_merge_kernel(SpanCall c) {
     constexpr int E = SPAN_MAX_D / 64;
+    __shared__ float s_part[4][MAPS][SPAN_MAX_D + 2];
     const vq_store_attend_args &a = c.a;
-    const int lane = threadIdx.x & 63;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= a.B * a.Hq * a.Sq) return;
-    const int64_t D = a.D;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t row = (int64_t)blockIdx.x * (4 / WAVES) + wave / WAVES;
+    if (row >= a.B * a.Hq * a.Sq) return;   // (the whole block where waves share a row)
+    const int D = (int)a.D;
     const float *ml = c.ml + row * c.nparts * MAPS * 2, *sums = c.sums + row * c.nparts * MAPS * D;
-    float o[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = 0.f;
+    float num[MAPS][E], m[MAPS], l[MAPS];
 #pragma unroll
     for (int w = 0; w < MAPS; ++w) {
-        // 64 parts at a time, a lane each: their maxima, weights and the sum of the weights
-        float m = -INFINITY, l = 0.f, num[E];
+        m[w] = -INFINITY; l[w] = 0.f;
 #pragma unroll
-        for (int e = 0; e < E; ++e) num[e] = 0.f;
-        for (int p0 = 0; p0 < c.nparts; p0 += 64) {
-            const bool mine = p0 + lane < c.nparts;
-            const float pm = mine ? ml[((p0 + lane) * MAPS + w) * 2] : -INFINITY;
-            const float pl = mine ? ml[((p0 + lane) * MAPS + w) * 2 + 1] : 0.f;
-            float mn = pm;
+        for (int e = 0; e < E; ++e) num[w][e] = 0.f;
+        for (int p0 = wave % WAVES * MERGE_AT_ONCE; p0 < c.nparts; p0 += WAVES * MERGE_AT_ONCE) {
+            float2 x[MERGE_AT_ONCE];
+            float y[MERGE_AT_ONCE][E];
 #pragma unroll
-            for (int off = 32; off > 0; off >>= 1) mn = fmaxf(mn, __shfl_xor(mn, off));
-            mn = fmaxf(mn, m);
-            if (mn == -INFINITY) continue;
-            const float f = exp2f(m - mn), weight = pm == -INFINITY ? 0.f : exp2f(pm - mn);
-            l = l * f + span_wave_sum(weight * pl);
-            m = mn;
+            for (int p = 0; p < MERGE_AT_ONCE; ++p) {
+                const int at = (p0 + p < c.nparts ? p0 + p : p0) * MAPS + w;
+                x[p] = *(const float2 *)(ml + at * 2);
 #pragma unroll
-            for (int e = 0; e < E; ++e) num[e] *= f;
-            const int n = c.nparts - p0 < 64 ? c.nparts - p0 : 64;
-            for (int p = 0; p < n; ++p) {
-                const float wp = __shfl(weight, p);
-                if (wp == 0.f) continue;   // (a part without a visible slot: its sums are zero or not written)
-                const float *x = sums + ((int64_t)(p0 + p) * MAPS + w) * D;
+                for (int e = 0; e < E; ++e) y[p][e] = lane + 64 * e < D ? sums[(int64_t)at * D + lane + 64 * e] : 0.f;
+            }
+            float mn = m[w];
 #pragma unroll
-                for (int e = 0; e < E; ++e)
-                    if (lane + 64 * e < D) num[e] = __builtin_fmaf(wp, x[lane + 64 * e], num[e]);
+            for (int p = 0; p < MERGE_AT_ONCE; ++p) mn = fmaxf(mn, x[p].x);
+            if (mn == -INFINITY) continue;   // (parts without a visible slot: their sums are not written)
+            const float f = exp2f(m[w] - mn);
+            m[w] = mn;
+            l[w] *= f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) num[w][e] *= f;
+#pragma unroll
+            for (int p = 0; p < MERGE_AT_ONCE; ++p) {
+                if (p0 + p >= c.nparts || x[p].x == -INFINITY) continue;
+                const float by = exp2f(x[p].x - mn);
+                l[w] = __builtin_fmaf(by, x[p].y, l[w]);
+#pragma unroll
+                for (int e = 0; e < E; ++e) num[w][e] = __builtin_fmaf(by, y[p][e], num[w][e]);
             }
         }
-        const float by = l > 0.f || l != l ? (w == 0 ? 1.f : -span_lam(a, row / a.Sq % a.Hq)) / l : 0.f;
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = __builtin_fmaf(num[e], by, o[e]);
     }
-    if (MAPS == 2 && a.norm_weight != nullptr) {
-        float sq = 0.f;
+    if (WAVES > 1) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) sq = __builtin_fmaf(o[e], o[e], sq);
-        const float by = a.gain / sqrtf(span_wave_sum(sq) / (float)D + a.norm_eps);
+        for (int w = 0; w < MAPS; ++w) {
+            if (lane == 0) { s_part[wave][w][0] = m[w]; s_part[wave][w][1] = l[w]; }
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (lane + 64 * e < D) s_part[wave][w][2 + lane + 64 * e] = num[w][e];
+        }
+        __syncthreads();
+        if (wave > 0) return;
+#pragma unroll
+        for (int w = 0; w < MAPS; ++w)
+            for (int v = 1; v < WAVES; ++v) {
+                const float *o = s_part[v][w], mn = fmaxf(m[w], o[0]);
+                if (mn == -INFINITY) continue;
+                const float f = exp2f(m[w] - mn), by = exp2f(o[0] - mn);
+                m[w] = mn;
+                l[w] = l[w] * f + o[1] * by;
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (lane + 64 * e < D) num[w][e] = num[w][e] * f + o[2 + lane + 64 * e] * by;
+            }
+    }
+    float o[E];
+#pragma unroll
+    for (int w = 0; w < MAPS; ++w) {
+        const float by = l[w] > 0.f || l[w] != l[w] ? (w == 0 ? 1.f : -span_lam(a, row / a.Sq % a.Hq)) / l[w] : 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = w == 0 ? num[0][e] * by : __builtin_fmaf(num[w][e], by, o[e]);
+    }
+    if (MAPS == 2) {
+        float gain = a.gain;
+        if (a.norm_weight != nullptr) {
+            float sq = 0.f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) sq = __builtin_fmaf(o[e], o[e], sq);
+            gain /= sqrtf(span_wave_sum(sq) / (float)D + a.norm_eps);
+        }
 #pragma unroll
         for (int e = 0; e < E; ++e)
-            if (lane + 64 * e < D) o[e] *= by * span_ld(a.norm_weight, a.norm_dtype, lane + 64 * e);
-    } else if (MAPS == 2) {
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] *= a.gain;
+            o[e] *= a.norm_weight != nullptr && lane + 64 * e < D ? gain * span_ld(a.norm_weight, a.norm_dtype, lane + 64 * e) : gain;
     }
 #pragma unroll
     for (int e = 0; e < E; ++e)
@@ -205,9 +236,9 @@ int check_call(const char *fn, const vq_store_attend_args *args, int maps) {
     const int64_t slots = span_prefix_slots(a) + a.own.n_packed + a.own.n_tail;
     VQ_REQUIRE(slots >= 1, VQ_ERR_INVALID, "%s: no key/value slots to attend to", fn);
     VQ_REQUIRE(slots < (INT64_C(1) << 30) && a.Sq < (INT64_C(1) << 30), VQ_ERR_UNSUPPORTED, "%s: more than 2^30 slots or queries a sequence", fn);
-    // (a wave a row in the merge, 2^32 threads a launch at most)
-    VQ_REQUIRE(a.B < (INT64_C(1) << 26) && a.Hq < (INT64_C(1) << 26) && a.B * a.Hq < (INT64_C(1) << 26) && a.B * a.Hq * a.Sq < (INT64_C(1) << 26),
-               VQ_ERR_UNSUPPORTED, "%s: 2^26 or more query rows", fn);
+    // (up to a block a row in the merge, 2^32 threads a launch at most)
+    VQ_REQUIRE(a.B < (INT64_C(1) << 24) && a.Hq < (INT64_C(1) << 24) && a.B * a.Hq < (INT64_C(1) << 24) && a.B * a.Hq * a.Sq < (INT64_C(1) << 24),
+               VQ_ERR_UNSUPPORTED, "%s: 2^24 or more query rows", fn);
     VQ_REQUIRE(!a.causal || a.Sq <= slots, VQ_ERR_INVALID, "%s: S_q=%lld exceeds the %lld slots; queries align to their end", fn, (long long)a.Sq, (long long)slots);
     VQ_REQUIRE(a.sliding_window >= 0, VQ_ERR_INVALID, "%s: negative sliding window", fn);
     VQ_REQUIRE(a.q != nullptr && a.out != nullptr, VQ_ERR_INVALID, "%s: null q or out", fn);
@@ -274,7 +305,9 @@ template <int MAPS> int attend(const char *fn, const vq_store_attend_args *args)
         VQ_HIP_CHECK_LAUNCH(fn);
     }
     if (!direct) {
-        span_merge_kernel<MAPS><<<(unsigned)cdiv(rows, 4), 256, 0, st>>>(c);
+        // (a row to a block where its parts are many, or rows too few to fill the chip with a wave each)
+        if (c.nparts > 2 * MERGE_AT_ONCE || (c.nparts > MERGE_AT_ONCE && rows < 4096)) span_merge_kernel<MAPS, 4><<<(unsigned)rows, 256, 0, st>>>(c);
+        else span_merge_kernel<MAPS, 1><<<(unsigned)cdiv(rows, 4), 256, 0, st>>>(c);
         VQ_HIP_CHECK_LAUNCH(fn);
     }
     return VQ_OK;

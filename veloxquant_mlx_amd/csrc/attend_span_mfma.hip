@@ -37,28 +37,28 @@ void span_mfma_plan(SpanCall &c, int maps) {
     c.apart = prefix_slots && a.B > 1 && r1 <= most / 2;
     c.pfew = packed && all <= few;
     c.ofew = packed && r1 <= few;
-    // One round of blocks of equal runs, one block a CU, each side for itself where they are launches of their own; sequences that differ
-    // in length even out over four rounds.  A run is four units a wave or more for few rows, four units a block else.
-    const int64_t round = a.seq_lens != nullptr ? 1024 : 256;
+    // One round of blocks of equal runs, one block a CU, each side for itself where they are launches of their own; own slots of sequences
+    // that differ in length even out over four rounds.  A run is four units a wave or more for few rows, eight units a block else: a block
+    // costs about as much to start and end.
     auto side = [&](bool by_few, int64_t rows, int64_t slots32, int64_t slots64, int64_t times, int &wt, int &tiles, int64_t &units, int64_t &least) {
         wt = !by_few && a.D != 256 && rows <= most / 2 ? 2 : 1;
         tiles = by_few ? 1 : (int)cdiv(rows, most / wt);
         units = by_few || a.D == 256 ? slots32 : slots64;
-        least = by_few ? (a.D == 256 ? 16 : 32) : 4;
+        least = by_few ? (a.D == 256 ? 16 : 32) : a.D == 256 ? 16 : 8;
         return times * a.Hkv * tiles * units;   // units of all blocks
     };
     const int64_t p32 = units_of(a.prefix, 32), p64 = units_of(a.prefix, 64), o32 = units_of(a.own, 32), o64 = units_of(a.own, 64);
-    int64_t pu = 0, ou = 0, pleast, oleast, pwork = 0, owork;
+    int64_t pu = 0, ou = 0, pleast = 1, oleast = 1, pwork = 0;
     if (c.apart) pwork = side(c.pfew, all, p32, p64, 1, c.pwt, c.ptiles, pu, pleast);
-    owork = side(c.ofew, r1, c.apart ? o32 : p32 + o32, c.apart ? o64 : p64 + o64, a.B, c.owt, c.otiles, ou, oleast);
+    const int64_t owork = side(c.ofew, r1, c.apart ? o32 : p32 + o32, c.apart ? o64 : p64 + o64, a.B, c.owt, c.otiles, ou, oleast);
     const bool together = c.apart && c.pfew == c.ofew;
-    auto cut = [&](int64_t units, int64_t work, int64_t least) {
-        int64_t run = cdiv(together ? pwork + owork : work, round);
+    auto cut = [&](int64_t units, int64_t work, int64_t least, int64_t blocks) {
+        int64_t run = cdiv(together ? pwork + owork : work, blocks);
         run = run < least ? least : run;
         return (int)cdiv(units, run);
     };
-    c.psplits = c.apart ? cut(pu, pwork, pleast) : 0;
-    c.osplits = cut(ou, owork, oleast);
+    c.psplits = c.apart ? cut(pu, pwork, pleast, 256) : 0;
+    c.osplits = cut(ou, owork, oleast, a.seq_lens != nullptr ? 1024 : 256);
     c.nparts = c.psplits + c.osplits;
 }
 
