@@ -37,7 +37,7 @@ void span_mfma_plan(SpanCall &c, int maps) {
     c.apart = prefix_slots && a.B > 1 && r1 <= most / 2;
     c.pfew = packed && all <= few;
     c.ofew = packed && r1 <= few;
-    // One round of blocks of equal runs, one block a CU, each side for itself where they are launches of their own; own slots of sequences
+    // One round of blocks of equal runs, two blocks a CU (one of few rows or heads of 256 channels), each side for itself where they are launches of their own; own slots of sequences
     // that differ in length even out over four rounds.  A run is four units a wave or more for few rows, eight units a block else: a block
     // costs about as much to start and end.
     auto side = [&](bool by_few, int64_t rows, int64_t slots32, int64_t slots64, int64_t times, int &wt, int &tiles, int64_t &units, int64_t &least) {
@@ -57,8 +57,9 @@ void span_mfma_plan(SpanCall &c, int maps) {
         run = run < least ? least : run;
         return (int)cdiv(units, run);
     };
-    c.psplits = c.apart ? cut(pu, pwork, pleast, 256) : 0;
-    c.osplits = cut(ou, owork, oleast, a.seq_lens != nullptr ? 1024 : 256);
+    auto round = [&](bool by_few) { return by_few ? 256 : 512; };   // blocks that run at once
+    c.psplits = c.apart ? cut(pu, pwork, pleast, round(c.pfew)) : 0;
+    c.osplits = cut(ou, owork, oleast, round(c.ofew) * (a.seq_lens != nullptr ? 4 : 1));
     c.nparts = c.psplits + c.osplits;
 }
 

@@ -1,13 +1,18 @@
 // Attention over spans of slots on the matrix units (gfx950, wave64): one kernel for the shared prefix, for a sequence's own slots
 // and for both maps of differential attention.
 //
-// A block of eight waves walks units of 64 slots (32 with heads of 256 channels) of one kv head.  A unit's keys and values are staged
-// in LDS once for the block.  Plain rows are copied there asynchronously, three units ahead.  Packed slots come as words, scales and
-// zeros into a ring of such units, seven ahead, and are reconstructed to fp16 a unit ahead of the products (one packed fused
-// multiply-add for two codes: exactly fp16(code * scale + zero)); four waves reconstruct before their products and four after, so
-// that each SIMD, which holds one of either, keeps its vector and its matrix unit busy at once.  A wave holds 32 query rows of one
-// map.  The rows of a block are those of all sequences that share the kv head (prefix), or of one sequence (own slots); where
-// they fill half of the waves or less, two waves share rows, each with its half of every unit, and add up in LDS at the end.
+// A block of four waves walks units of 64 slots (32 with heads of 256 channels) of one kv head, two blocks a CU (one).  A unit's keys and
+// values are staged in LDS once for the block.  Plain rows are copied there asynchronously, a unit or more ahead.  Packed slots come as
+// words, scales and zeros into a ring of such units, copied ahead, and are reconstructed to fp16 between the products (one packed fused
+// multiply-add for two codes: exactly fp16(code * scale + zero)).  A wave holds 32 query rows of one map.  The rows of a block are those of
+// all sequences that share the kv head (prefix), or of one sequence (own slots); where they fill half of the waves or less, two waves
+// share rows, each with its half of every unit, and add up in LDS at the end.
+//
+// Bound by what a SIMD has to do one after the other for a unit of 32 rows: 32 products of 32 cycles at 128 channels, ~200 vector
+// instructions of the softmax, ~120 of reconstruction.  Two blocks a CU, which no barrier ties together, overlap one's vector work, copies
+// and start with the other's products.  (Eight waves in one block took longer: in step at every barrier, a unit of 64 slots of two maps
+// took 3700 cycles, and with half of the waves a phase behind the other half 2700, where the products alone take 1540; and every block
+// starts and ends alone on its CU, 10 us.)
 //
 // v_mfma_f32_32x32x16 with n = lane % 32, h = lane / 32: A[i = n][k = 8 h + j], B[k = 8 h + j][n], j = 0..7, and
 // D[i = 8 (r / 4) + 4 h + r % 4][n] in register r = 0..15.  Scores are formed transposed, S^T = K Q^T: a lane then holds sixteen slots of
@@ -32,7 +37,7 @@ typedef __bf16 bf16x2v __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8v __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-constexpr int SP_WAVES = 8, SP_THREADS = 64 * SP_WAVES;
+constexpr int SP_WAVES = 4, SP_THREADS = 64 * SP_WAVES;
 
 template <typename T> struct SpanMma;
 template <> struct SpanMma<f16> {
@@ -126,27 +131,30 @@ template <int BITS, int D> struct SpanTile {
     static constexpr int KEYS = UNIT * D * 2;
     static constexpr int VALUES = BITS && D * VROW > KEYS ? D * VROW : KEYS;
     static constexpr int BUF = KEYS + VALUES;
-    static constexpr int BUFS = BITS ? 2 : 0;            // tiles of packed slots: one at work, one in the making
-    static constexpr int ROW_BUF = 2 * KEYS, ROW_BUFS = 4;   // tiles of plain rows: one at work, three under way
+    static constexpr int MOST = 80 * 1024;   // block-shared memory of a block
+    static constexpr int ROW_BUF = 2 * KEYS, ROW_BUFS = MOST / ROW_BUF < 4 ? MOST / ROW_BUF : 4;   // tiles of plain rows: one at work, the others under way
     // a packed unit as it lies in memory: key words, value words, key scales and zeros a piece of 32 slots, value scales and
     // zeros a piece of 32 channels
     static constexpr int KWORDS = UNIT * D * BITS / 8, META = UNIT * D / 8;
     static constexpr int RAW = 2 * KWORDS + 2 * META;
-    static constexpr int RAWS = BITS ? 8 : 0;
+    static constexpr int RAWS = BITS ? (MOST - BUF) / RAW < 6 ? (MOST - BUF) / RAW : 6 : 0;   // beside the one tile
     static constexpr int PIECES = RAW / 1024;            // copies of 1 KB, dealt to the waves
     static constexpr int COPIES = (PIECES + SP_WAVES - 1) / SP_WAVES;
     static constexpr int EXCHANGE = SP_WAVES / 2 * (D / 8 * 64 + 64) * 16;   // the rows of half of the waves, at the end
     static constexpr int max(int x, int y) { return x > y ? x : y; }
-    static constexpr int LDS = max(max(BUFS * BUF + RAWS * RAW, ROW_BUFS * ROW_BUF), EXCHANGE);
-    static_assert(RAW % 1024 == 0 && LDS <= 160 * 1024 && KEYS % (1024 * SP_WAVES) == 0, "tile sizes");
+    static constexpr int LDS = max(max(BITS ? BUF + RAWS * RAW : 0, ROW_BUFS * ROW_BUF), EXCHANGE);
+    static_assert(LDS <= MOST && ROW_BUFS >= 2 && (BITS == 0 || RAWS >= 3) && RAW % 1024 == 0 && KEYS % (1024 * SP_WAVES) == 0, "tile sizes");
 };
 
-template <int BITS, typename T, int D, int MAPS>
-__global__ __launch_bounds__(SP_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2))) void span_mfma_kernel(SpanCall c) {
+// blocks of the prefix, in front of those of the sequences' own slots
+__host__ __device__ __forceinline__ int span_shared_blocks(const SpanCall &c) { return c.apart && !c.pfew ? c.psplits * c.ptiles * (int)c.a.Hkv : 0; }
+
+// One block.  WT = 2: two waves share rows, each with its half of every unit.
+template <int BITS, typename T, int D, int MAPS, int WT> __device__ __forceinline__ void span_mfma_block(const SpanCall &c) {
     extern __shared__ __align__(16) char lds[];
     using M = SpanMma<T>;
     using Tile = SpanTile<BITS, D>;
-    constexpr int UNIT = Tile::UNIT, KS = D / MAPS / 16, KF = KS < 8 ? KS : 8, DT = D / 32, CH = D / 8;   // channel steps of a score, channel tiles, 16-byte pieces a row
+    constexpr int UNIT = Tile::UNIT, KS = D / MAPS / 16, DT = D / 32, CH = D / 8;   // channel steps of a score, channel tiles, 16-byte pieces a row
     const vq_store_attend_args &a = c.a;
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -156,23 +164,23 @@ __global__ __launch_bounds__(SP_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
     // ---- the block: kv head fastest (blocks of one kv head and run, which read the same slots, lie a multiple of the head count
     // apart), under a causal mask the row tiles that see most first
     int id = (int)blockIdx.x;
-    const int shared_blocks = c.apart && !c.pfew ? c.psplits * c.ptiles * Hkv : 0;
+    const int shared_blocks = span_shared_blocks(c);
     const bool shared = id < shared_blocks;
-    int b = 0, split, tile, splits, wt, rows, part;
+    int b = 0, split, tile, splits, rows, part;
     const int hkv = shared ? id % Hkv : (id - shared_blocks) % Hkv;
     if (shared) {
         id /= Hkv;
         splits = c.psplits; split = id % splits; tile = id / splits;
-        wt = c.pwt; rows = B * r1; part = split;
+        rows = B * r1; part = split;
     } else {
         id = (id - shared_blocks) / Hkv;
         b = id % B; id /= B;
         splits = c.osplits; split = id % splits; tile = c.otiles - 1 - id / splits;
-        wt = c.owt; rows = r1; part = (c.apart ? c.psplits : 0) + split;
+        rows = r1; part = (c.apart ? c.psplits : 0) + split;
     }
-    // the waves: one map and 32 rows each; wt = 2: two of them share rows, each with its half of every unit
-    const int map = MAPS == 2 ? wave & 1 : 0, rest = wave / MAPS, groups = SP_WAVES / MAPS / wt;
-    const int rt = 32 * groups, rg = wt == 2 ? rest >> 1 : rest, th = wt == 2 ? rest & 1 : 0;
+    // the waves: one map and 32 rows each
+    constexpr int groups = SP_WAVES / MAPS / WT, rt = 32 * groups, X = WT == 2 ? 1 : Tile::HALVES;   // ... and X stretches of 32 slots of a unit
+    const int map = MAPS == 2 ? wave & 1 : 0, rest = wave / MAPS, rg = WT == 2 ? rest >> 1 : rest, th = WT == 2 ? rest & 1 : 0;
 
     // ---- this lane's query row: positions outermost, so that a tile covers few of them
     const int j0 = tile * rt, j = j0 + 32 * rg + n, jc = j < rows ? j : rows - 1;
@@ -257,52 +265,50 @@ __global__ __launch_bounds__(SP_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
     using L4 = __attribute__((address_space(3))) const u32x4;
     using LT = __attribute__((address_space(3))) s16x4;
 
-    // 32 slots of a tile at `tile`: the first one's slot, how many live ones the span has from there on
-    auto work = [&](auto transposed, u32 tile, int half, int place, int live) __attribute__((always_inline)) {
-        if (place >= any_hi || place + 32 <= any_lo || live <= 0) return;
-        f32x16 S;
+    f32x16 S[X];
+    u32x4 P[X][2];
+    // Operands are asked for four products ahead, as written: left to itself the scheduler reads each right before its product and waits.
+    constexpr int AHEAD = 4;
+    auto scores = [&](u32 tile) __attribute__((always_inline)) {
+        constexpr int N = X * KS;
+        auto key = [&](int i) __attribute__((always_inline)) { return *(L4 *)(uintptr_t)((key0 ^ (32 * (i % KS))) + tile + i / KS * (32 * D * 2)); };
+        u32x4 k[AHEAD];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) S[r] = 0.f;
-        const u32 keys = tile + half * (32 * D * 2);
+        for (int i = 0; i < AHEAD && i < N; ++i) k[i] = key(i);
 #pragma unroll
-        for (int k0 = 0; k0 < KS; k0 += KF) {   // the pieces of eight steps are asked for at once
-            u32x4 k[KF];
+        for (int x = 0; x < X; ++x)
 #pragma unroll
-            for (int ks = 0; ks < KF; ++ks) k[ks] = *(L4 *)(uintptr_t)((key0 ^ (32 * (k0 + ks))) + keys);
+            for (int r = 0; r < 16; ++r) S[x][r] = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            S[i / KS] = M::mma(k[i % AHEAD], q[i % KS], S[i / KS]);
+            if (i + AHEAD < N) k[i % AHEAD] = key(i + AHEAD);
             __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int ks = 0; ks < KF; ++ks) S = M::mma(k[ks], q[k0 + ks], S);
         }
-        // the values of the first sixteen slots are on their way while the weights are formed
-        const u32 values = tile + Tile::KEYS + (transposed.value ? half * 64 + col0 : half * (32 * D * 2));
-        auto value = [&](int s, int dt) __attribute__((always_inline)) {
-            if constexpr (transposed.value) {
-                return *(L4 *)(uintptr_t)(values + dt * (32 * Tile::VROW) + s * 32);
-            } else {
-                LT *row = (LT *)(uintptr_t)((val0 ^ (64 * dt)) + values);
-                const uint2 v0 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(row + s * 16 * D / 4));
-                const uint2 v1 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(row + (s * 16 + 8) * D / 4));
-                return u32x4{v0.x, v0.y, v1.x, v1.y};
-            }
-        };
-        u32x4 v[DT];
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) v[dt] = value(0, dt);
-        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto weights = [&](int place, int live) __attribute__((always_inline)) {
         const int end = place + live;
-        if (place + 32 > (all_hi < end ? all_hi : end) || place < all_lo) {
+        if (place + 32 * X > (all_hi < end ? all_hi : end) || place < all_lo) {
             const int hi = (lane_hi < end ? lane_hi : end) - place - 4 * h, lo = lane_lo - place - 4 * h;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int t = 8 * (r / 4) + r % 4;
-                if (t >= hi || t < lo) S[r] = -INFINITY;
-            }
-        }
-        float mx = fmaxf(S[0], S[1]);   // (first: the compiler waits for the products only before instructions of its own)
+            for (int x = 0; x < X; ++x)
 #pragma unroll
-        for (int r = 2; r < 16; r += 2) mx = sp_max3(mx, S[r], S[r + 1]);
-        if (__any(mx * cc > m_run + RESCALE_SLACK)) {
-            const float top = fmaxf(mx, __shfl_xor(mx, 32)) * cc, m = fmaxf(m_run, top);
+                for (int r = 0; r < 16; ++r) {
+                    const int t = 32 * x + 8 * (r / 4) + r % 4;
+                    if (t >= hi || t < lo) S[x][r] = -INFINITY;
+                }
+        }
+        // (the first reader of the products is the compiler's own, which waits for them: it does not on behalf of inline assembly)
+        float mx[X];
+#pragma unroll
+        for (int x = 0; x < X; ++x) {
+            const float m0 = fmaxf(S[x][0], S[x][1]);
+            mx[x] = sp_max3(sp_max3(sp_max3(m0, S[x][2], S[x][3]), sp_max3(m0, S[x][4], S[x][5]), sp_max3(m0, S[x][6], S[x][7])), sp_max3(m0, S[x][8], S[x][9]),
+                            sp_max3(sp_max3(m0, S[x][10], S[x][11]), sp_max3(m0, S[x][12], S[x][13]), sp_max3(m0, S[x][14], S[x][15])));
+        }
+        const float most = X == 2 ? fmaxf(mx[0], mx[X - 1]) : mx[0];
+        if (__any(most * cc > m_run + RESCALE_SLACK)) {
+            const float top = fmaxf(most, __shfl_xor(most, 32)) * cc, m = fmaxf(m_run, top);
             const float alpha = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - m);
             m_run = m;
             l_run *= alpha;
@@ -312,26 +318,47 @@ __global__ __launch_bounds__(SP_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
                 for (int r = 0; r < 16; ++r) O[dt][r] *= alpha;
         }
         const float nm = m_run == -INFINITY ? 0.f : -m_run;
-        u32x4 P[2];
+        float l2[2] = {0.f, 0.f};   // (short chains)
 #pragma unroll
-        for (int r = 0; r < 8; ++r) {
-            const u32 p = M::pack(__builtin_amdgcn_exp2f(__builtin_fmaf(S[2 * r], cc, nm)), __builtin_amdgcn_exp2f(__builtin_fmaf(S[2 * r + 1], cc, nm)));
-            P[r / 4][r % 4] = p;
-            l_run = M::add_pair(p, l_run);
-        }
+        for (int x = 0; x < X; ++x)
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {   // (the next sixteen slots' piece is asked for as its place falls free)
-            O[dt] = M::mma(v[dt], P[0], O[dt]);
-            v[dt] = value(1, dt);
-        }
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) O[dt] = M::mma(v[dt], P[1], O[dt]);
+            for (int r = 0; r < 8; ++r) {
+                const u32 p = M::pack(__builtin_amdgcn_exp2f(__builtin_fmaf(S[x][2 * r], cc, nm)), __builtin_amdgcn_exp2f(__builtin_fmaf(S[x][2 * r + 1], cc, nm)));
+                P[x][r / 4][r % 4] = p;
+                l2[r & 1] = M::add_pair(p, l2[r & 1]);
+            }
+        l_run += l2[0] + l2[1];
     };
-    const int half0 = th, half1 = wt == 1 ? Tile::HALVES : th + 1;
+    auto sums = [&](auto transposed, u32 tile) __attribute__((always_inline)) {
+        constexpr int N = 2 * X * DT;
+        const u32 values = tile + Tile::KEYS + (transposed.value ? col0 : 0u);
+        auto value = [&](int i) __attribute__((always_inline)) {   // of channel tile i % DT, the step's slots 16 (i / DT) .. + 15
+            const int s = i / DT, dt = i % DT;
+            if constexpr (transposed.value) {
+                return *(L4 *)(uintptr_t)(values + dt * (32 * Tile::VROW) + s * 32);
+            } else {
+                LT *row = (LT *)(uintptr_t)((val0 ^ (64 * dt)) + values);
+                const uint2 v0 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(row + s * 16 * D / 4));
+                const uint2 v1 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(row + (s * 16 + 8) * D / 4));
+                return u32x4{v0.x, v0.y, v1.x, v1.y};
+            }
+        };
+        u32x4 v[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD && i < N; ++i) v[i] = value(i);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            O[i % DT] = M::mma(v[i % AHEAD], P[i / DT / 2][i / DT % 2], O[i % DT]);
+            if (i + AHEAD < N) v[i % AHEAD] = value(i + AHEAD);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    // (units that none of the wave's rows sees are left out whole: a unit's stretches are not tested one by one)
     auto compute = [&](auto transposed, u32 tile, int place, int live) __attribute__((always_inline)) {
-        if (!wave_works) return;
-#pragma unroll 1
-        for (int half = half0; half < half1; ++half) work(transposed, tile, half, place + 32 * half, live - 32 * half);
+        if (!wave_works || place >= any_hi || place + UNIT <= any_lo) return;
+        scores(tile + th * (32 * D * 2));
+        weights(place + 32 * th, live - 32 * th);
+        sums(transposed, tile + (transposed.value ? th * 64 : th * (32 * D * 2)));
     };
 
     // ---- one span after the other.  A store's fields are read from the argument block where a span begins (`fresh` hides the block's
@@ -351,21 +378,8 @@ __global__ __launch_bounds__(SP_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
         const int64_t ks = s->k_strides[2] * 2, vs = s->v_strides[2] * 2;
         const char *kb = (const char *)s->k_tail + (sb * s->k_strides[0] + hkv * s->k_strides[1]) * 2 + t0 * ks;
         const char *vb = (const char *)s->v_tail + (sb * s->v_strides[0] + hkv * s->v_strides[1]) * 2 + t0 * vs;
-        if (BITS && args->a.tail_dtype == VQ_BF16) {   // converted on the way, a unit at a time
-#pragma unroll 1
-            for (int i = 0; i < count; ++i, kb += UNIT * ks, vb += UNIT * vs, place += UNIT, live -= UNIT) {
-                for (int x = tid; x < UNIT * CH; x += SP_THREADS) {
-                    const int t = x / CH, p = x % CH, r = t < live ? t : live - 1;
-                    *(f16x8 *)(lds + t * D * 2 + sp_kpiece<D>(t, p) * 16) = ld_tail8(kb + r * ks, 8 * p, true);
-                    *(f16x8 *)(lds + Tile::KEYS + t * D * 2 + sp_vpiece<D>(t, p) * 16) = ld_tail8(vb + r * vs, 8 * p, true);
-                }
-                lds_barrier();
-                compute(std::false_type{}, lds0, place, live);
-                lds_barrier();
-            }
-            return;
-        }
-        constexpr int AHEAD = Tile::ROW_BUFS - 1, N = Tile::KEYS / 1024 / SP_WAVES;   // units asked for ahead; copies a wave for the keys of one
+        const bool convert = BITS != 0 && args->a.tail_dtype == VQ_BF16;   // (a unit at a time, not copied ahead)
+        constexpr int R = Tile::ROW_BUFS, N = Tile::KEYS / 1024 / SP_WAVES;   // copies a wave for the keys of a unit
         u32 koff[N], voff[N];   // of the lane's pieces, in a whole unit
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -373,40 +387,56 @@ __global__ __launch_bounds__(SP_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
             koff[i] = (u32)t * (u32)ks + sp_kpiece<D>(t, p) * 16;
             voff[i] = (u32)t * (u32)vs + sp_vpiece<D>(t, p) * 16;
         }
-        u32 fill = lds0 + wave * N * 1024, tile = lds0;
-        const u32 past = lds0 + Tile::ROW_BUFS * Tile::ROW_BUF;
-        int asked_live = live;
+        const u32 past = lds0 + R * Tile::ROW_BUF;
+        u32 fill = lds0 + wave * N * 1024;   // where the next unit's copies go
+        int asked_live = live, asked = 0;
         auto fetch = [&]() __attribute__((always_inline)) {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 u32 ko = koff[i], vo = voff[i];
-                if (asked_live < UNIT) {   // a row past the live ones repeats the last
-                    const int slot = (wave * N + i) * 64 + lane, t = slot / CH;
-                    const int r = t < asked_live ? t : asked_live - 1;   // (the pieces' order goes by the tile's row)
-                    ko = (u32)r * (u32)ks + sp_kpiece<D>(t, slot % CH) * 16;
-                    vo = (u32)r * (u32)vs + sp_vpiece<D>(t, slot % CH) * 16;
+                if (asked_live < UNIT) {   // a row past the live ones repeats the last (the pieces' order goes by the tile's row)
+                    int slot = (wave * N + i) * 64 + lane;
+                    asm volatile("" : "+v"(slot));   // (not to be worked out ahead, and held, for all units)
+                    const int t = slot / CH, p = slot % CH;
+                    const u32 r = (u32)(t < asked_live ? t : asked_live - 1);
+                    ko = r * (u32)ks + sp_kpiece<D>(t, p) * 16;
+                    vo = r * (u32)vs + sp_vpiece<D>(t, p) * 16;
                 }
                 lds_copy16<0>(kb, ko, fill + i * 1024);
                 lds_copy16<0>(vb, vo, fill + i * 1024 + Tile::KEYS);
             }
             kb += UNIT * ks;
             vb += UNIT * vs;
+            ++asked;
             asked_live -= UNIT;
             fill += Tile::ROW_BUF;
-            if (fill >= past) fill -= Tile::ROW_BUFS * Tile::ROW_BUF;
+            if (fill >= past) fill -= R * Tile::ROW_BUF;
         };
 #pragma unroll 1
-        for (int i = 0; i < AHEAD && i < count; ++i) fetch();
+        for (int i = 0; i < R - 1 && i < count && !convert; ++i) fetch();
+        u32 tile = lds0;
 #pragma unroll 1
         for (int i = 0; i < count; ++i, place += UNIT, live -= UNIT) {
-            // the unit is here once the copies of at most AHEAD - 1 later ones are under way; past the barrier every wave has left the
-            // tile before it, the next to be filled
-            if (i + AHEAD <= count) wait_copies<(AHEAD - 1) * 2 * N>();
+            // the unit is here once the copies of at most R - 2 later ones are under way; past the barrier every wave has left the tile
+            // before it, the next to be filled
+            if (i + R - 1 <= count) wait_copies<(R - 2) * 2 * N>();
             else wait_copies<0>();
             lds_barrier();
-            if (i + AHEAD < count) fetch();
+            if (convert) {
+#pragma unroll 1
+                for (int x = tid; x < UNIT * CH; x += SP_THREADS) {
+                    const int t = x / CH, p = x % CH, r = t < live ? t : live - 1;
+                    *(f16x8 *)(lds + t * D * 2 + sp_kpiece<D>(t, p) * 16) = ld_tail8(kb + r * ks, 8 * p, true);
+                    *(f16x8 *)(lds + Tile::KEYS + t * D * 2 + sp_vpiece<D>(t, p) * 16) = ld_tail8(vb + r * vs, 8 * p, true);
+                }
+                kb += UNIT * ks;
+                vb += UNIT * vs;
+                lds_barrier();
+            } else if (asked < count) {
+                fetch();
+            }
             compute(std::false_type{}, tile, place, live);
-            tile += Tile::ROW_BUF;
+            if (!convert) tile += Tile::ROW_BUF;
             if (tile == past) tile = lds0;
         }
         lds_barrier();   // the tiles are free
@@ -431,6 +461,7 @@ __global__ __launch_bounds__(SP_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
         auto lane_at = [&](int i, int n_live) __attribute__((always_inline)) -> const char * {   // in the span's first unit
             const int p = piece_of(i);
             int off = p * 1024 + lane * 16;
+            asm volatile("" : "+v"(off));   // (not to be worked out ahead, and held, for all units)
             if (p < Tile::KWORDS / 1024) {
                 const int last = n_live * KW * 4 - 16;
                 return kw + (off < last ? off : last);
@@ -451,7 +482,7 @@ __global__ __launch_bounds__(SP_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
         const char *at[N ? N : 1];
 #pragma unroll
         for (int i = 0; i < N; ++i) at[i] = lane_at(i, UNIT);
-        const u32 raw0 = lds0 + Tile::BUFS * Tile::BUF;
+        const u32 raw0 = lds0 + Tile::BUF;
         int asked = t0, asked_live = live;
         u32 fill = raw0;
         auto fetch = [&]() __attribute__((always_inline)) {
@@ -472,25 +503,30 @@ __global__ __launch_bounds__(SP_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
         };
         // a unit from the ring into a tile
         const u32 magic = vreg_const(Magic<BB>::bits);
-        const int kc = tid % CH, kt = tid / CH;            // keys: 8-channel piece, slot
-        const int vc = tid % D, step = tid / D;            // values: channel, sixteen slots
         constexpr int KROWS = SP_THREADS / CH;             // slots that the threads cover at a time
-        char *take = lds + Tile::BUFS * Tile::BUF;
-        auto build = [&](u32 buf, int n_live) __attribute__((always_inline)) {
-            char *kd = lds + buf, *vd = kd + Tile::KEYS;
-            const char *raw = take;
-            const uint4 *kmeta = (const uint4 *)(raw + 2 * Tile::KWORDS);
-            const uint4 *vmeta = (const uint4 *)(raw + 2 * Tile::KWORDS + Tile::META);
+        constexpr int VSTEPS = UNIT * D / 16 / SP_THREADS; // sixteen slots each, of a thread's channel
+        const char *take = lds + Tile::BUF;
+        auto make = [&](int n_live) __attribute__((always_inline)) {
+            char *kd = lds, *vd = lds + Tile::KEYS;
+            int id = tid;
+            asm volatile("" : "+v"(id));   // (addresses are not to be worked out ahead, and held, for all units)
+            const int kc = id % CH, kt = id / CH;   // keys: 8-channel piece, slot
+            const int vc = id % D, vh = id / D;     // values: channel, which of the unit's stretches
+            const uint4 *kmeta = (const uint4 *)(take + 2 * Tile::KWORDS);
+            const uint4 *vmeta = (const uint4 *)(take + 2 * Tile::KWORDS + Tile::META);
 #pragma unroll
             for (int i = 0; i < UNIT / KROWS; ++i) {
                 const int t = kt + KROWS * i;
-                const u32 w = ((const u32 *)raw)[t * KW + (BB == 4 ? kc : kc / 2)];
+                const u32 w = ((const u32 *)take)[t * KW + (BB == 4 ? kc : kc / 2)];
                 u32 code[4];
                 sp_codes8<BB>(BB == 2 ? w >> (16 * (kc & 1)) : w, magic, code);
                 *(u32x4 *)(kd + t * D * 2 + sp_kpiece<D>(t, kc) * 16) = sp_values8(code, kmeta[t / 32 * 2 * CH + kc], kmeta[(t / 32 * 2 + 1) * CH + kc]);
+                __builtin_amdgcn_sched_barrier(0);
             }
-            if (step < UNIT / 16) {
-                const u32 *words = (const u32 *)(raw + Tile::KWORDS) + vc;
+            const u32 *words = (const u32 *)(take + Tile::KWORDS) + vc;
+#pragma unroll
+            for (int i = 0; i < VSTEPS; ++i) {
+                const int step = vh * VSTEPS + i;
                 const uint4 *meta = vmeta + vc / 32 * 2 * TP + 2 * step;
                 u32x4 x[2];
 #pragma unroll
@@ -512,31 +548,25 @@ __global__ __launch_bounds__(SP_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
                 u32x4 *dst = (u32x4 *)(vd + vc * Tile::VROW + step * 32);
                 dst[0] = u32x4{x[0][0], x[0][1], x[1][0], x[1][1]};
                 dst[1] = u32x4{x[0][2], x[0][3], x[1][2], x[1][3]};
+                __builtin_amdgcn_sched_barrier(0);
             }
             take += Tile::RAW;
-            if (take == lds + Tile::BUFS * Tile::BUF + RAWS * Tile::RAW) take -= RAWS * Tile::RAW;
+            if (take == lds + Tile::BUF + RAWS * Tile::RAW) take -= RAWS * Tile::RAW;
         };
 #pragma unroll 1
-        for (int i = 0; i < RAWS - 1 && i < count; ++i) fetch();
-        if (count >= RAWS - 1) wait_copies<(RAWS - 3) * N>();
-        else wait_copies<0>();
-        lds_barrier();
-        build(0, live);
-        lds_barrier();
-        u32 buf = 0;
+        for (int i = 0; i < RAWS && i < count; ++i) fetch();
 #pragma unroll 1
         for (int i = 0; i < count; ++i, place += UNIT, live -= UNIT) {
-            // unit i is in its tile, unit i + 1 in the ring; into the slot that unit i - 1 has left
-            const bool more = i + 1 < count, deep = i + RAWS - 1 < count;
-            if (deep) fetch();
-            if (more && wave < SP_WAVES / 2) build(Tile::BUF - buf, live - UNIT);
-            compute(std::true_type{}, lds0 + buf, place, live);
-            if (more && wave >= SP_WAVES / 2) build(Tile::BUF - buf, live - UNIT);
-            if (deep) wait_copies<(RAWS - 3) * N>();   // unit i + 2 is in the ring once at most units i + 3 .. i + RAWS - 1 are under way
+            // unit i is in the ring once at most the RAWS - 1 units behind it are under way; past the barrier every wave has left the tile
+            if (i + RAWS <= count) wait_copies<(RAWS - 1) * N>();
             else wait_copies<0>();
             lds_barrier();
-            buf = Tile::BUF - buf;
+            make(live);
+            lds_barrier();
+            if (i + RAWS < count) fetch();   // into the slot that unit i has left
+            compute(std::true_type{}, lds0, place, live);
         }
+        lds_barrier();
     };
     {
         int skip = w0, left = w1 - w0;
@@ -563,7 +593,7 @@ __global__ __launch_bounds__(SP_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
     // ---- results: the other half's part of the row, then the other map's
     float l = l_run + __shfl_xor(l_run, 32);   // both lanes of a row
     float4 *room = (float4 *)lds + (map * groups + rg) * (D / 8 * 64 + 64) + lane;   // 4 floats a lane and quarter of a channel tile; sum and maximum
-    if (wt == 2) {
+    if (WT == 2) {
         lds_barrier();
         if (th == 1) {
 #pragma unroll
@@ -654,6 +684,12 @@ __global__ __launch_bounds__(SP_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
                                      : make_uint2(SpanMma<f16>::pack(o[0], o[1]), SpanMma<f16>::pack(o[2], o[3]));
             *(uint2 *)(dst + 32 * dt + 2 * r) = x;
         }
+}
+
+template <int BITS, typename T, int D, int MAPS>
+__global__ __launch_bounds__(SP_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2))) void span_mfma_kernel(SpanCall c) {
+    if (D != 256 && ((int)blockIdx.x < span_shared_blocks(c) ? c.pwt : c.owt) == 2) span_mfma_block<BITS, T, D, MAPS, D == 256 ? 1 : 2>(c);
+    else span_mfma_block<BITS, T, D, MAPS, 1>(c);
 }
 
 // More than 64 KB of block-shared memory has to be allowed per kernel and device, once (a second setter repeats the same call).
