@@ -18,8 +18,9 @@
 
 namespace vq {
 
-template <int BITS, int D> struct SpanFew {
-    static constexpr int WAVES = D == 256 ? 4 : 8, THREADS = 64 * WAVES, UNIT = 32;
+// Four waves a block, two blocks a CU (one with heads of 256 channels).  Eight waves for rows of few slots, which they walk without parts.
+template <int BITS, int D, int WAVES_> struct SpanFew {
+    static constexpr int WAVES = WAVES_, THREADS = 64 * WAVES, UNIT = 32;
     static constexpr int PER = 32 / BITS, KROW = D * BITS / 8, WORDS = UNIT * KROW;   // bytes of a slot's key words, of a unit's key (value) words
     static constexpr int META = 4 * D;                     // bytes of a unit's key (value) scales and zeros
     static constexpr int RAW = 2 * WORDS + 2 * META;
@@ -30,11 +31,11 @@ template <int BITS, int D> struct SpanFew {
     static_assert(RING >= 3 && LDS <= 160 * 1024, "room for a unit at work and two under way");
 };
 
-template <int BITS, int D, int MAPS>
-__global__ __launch_bounds__((SpanFew<BITS, D>::THREADS)) __attribute__((amdgpu_waves_per_eu(SpanFew<BITS, D>::WAVES / 4, SpanFew<BITS, D>::WAVES / 4)))
+template <int BITS, int D, int MAPS, int WAVES>
+__global__ __launch_bounds__((64 * WAVES)) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2, D == 256 ? 1 : 2)))
 void span_few_kernel(SpanCall c) {
     extern __shared__ __align__(16) char lds[];
-    using F = SpanFew<BITS, D>;
+    using F = SpanFew<BITS, D, WAVES>;
     using M = SpanMma<f16>;
     constexpr int KS = D / 16, DT = D / 32, CH = D / 8, UNIT = F::UNIT, PER = F::PER;
     const vq_store_attend_args &a = c.a;
@@ -214,7 +215,7 @@ void span_few_kernel(SpanCall c) {
             fill += F::RAW;
             if (fill == room + RING * F::RAW) fill = room;
         };
-        const u32 magic = vreg_const(Magic<BITS>::bits);
+        const SpanMagic<BITS> magic;
         const char *take = room_p;
         auto step = [&]() __attribute__((always_inline)) {
             // scores
@@ -238,7 +239,7 @@ void span_few_kernel(SpanCall c) {
                 for (int e = 0; e < PERP; ++e) {
                     const int k = p * PERP + e;
                     u32 code[4];
-                    sp_codes8<BITS>(BITS == 4 ? w[e % 4] : w[e / 2] >> (16 * (e & 1)), magic, code);
+                    sp_codes8<BITS>(BITS == 4 ? w[e % 4] : w[e / 2], magic, code, 2 * (e & 1));
                     S = M::mma(sp_values8(code, kmeta[k], kmeta[CH + k]), q[k], S);
                 }
             }
@@ -442,17 +443,23 @@ void span_few_kernel(SpanCall c) {
     }
 }
 
-template <int BITS, int D, int MAPS> int launch_span_few_as(const SpanCall &c) {
-    constexpr int bytes = SpanFew<BITS, D>::LDS;
-    const auto kernel = span_few_kernel<BITS, D, MAPS>;
+template <int BITS, int D, int MAPS, int WAVES> int launch_span_few_of(const SpanCall &c) {
+    constexpr int bytes = SpanFew<BITS, D, WAVES>::LDS;
+    const auto kernel = span_few_kernel<BITS, D, MAPS, WAVES>;
     static std::atomic<bool> allowed[64] = {};
     if (int rc = span_allow_lds((const void *)kernel, bytes, allowed)) return rc;
     const int64_t blocks = (c.apart && c.pfew ? (int64_t)c.psplits * c.a.Hkv : 0) + (c.ofew ? c.a.B * c.a.Hkv * c.osplits : 0);
     if (blocks == 0) return VQ_OK;
     VQ_REQUIRE(blocks < (INT64_C(1) << 23), VQ_ERR_UNSUPPORTED, "attention over spans: too many sequences and heads for one launch");
-    kernel<<<(unsigned)blocks, SpanFew<BITS, D>::THREADS, bytes, (hipStream_t)c.a.stream>>>(c);
+    kernel<<<(unsigned)blocks, 64 * WAVES, bytes, (hipStream_t)c.a.stream>>>(c);
     VQ_HIP_CHECK_LAUNCH("attention over spans");
     return VQ_OK;
+}
+template <int BITS, int D, int MAPS> int launch_span_few_as(const SpanCall &c) {
+    if constexpr (D != 256) {
+        if (c.owaves == 8) return launch_span_few_of<BITS, D, MAPS, 8>(c);
+    }
+    return launch_span_few_of<BITS, D, MAPS, 4>(c);
 }
 
 int launch_span_few2(const SpanCall &c, int maps);

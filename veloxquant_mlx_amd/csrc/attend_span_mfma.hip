@@ -44,7 +44,7 @@ void span_mfma_plan(SpanCall &c, int maps) {
         wt = !by_few && a.D != 256 && rows <= most / 2 ? 2 : 1;
         tiles = by_few ? 1 : (int)cdiv(rows, most / wt);
         units = by_few || a.D == 256 ? slots32 : slots64;
-        least = by_few ? (a.D == 256 ? 16 : 32) : a.D == 256 ? 16 : 8;
+        least = by_few ? 16 : a.D == 256 ? 16 : 8;
         return times * a.Hkv * tiles * units;   // units of all blocks
     };
     const int64_t p32 = units_of(a.prefix, 32), p64 = units_of(a.prefix, 64), o32 = units_of(a.own, 32), o64 = units_of(a.own, 64);
@@ -57,9 +57,16 @@ void span_mfma_plan(SpanCall &c, int maps) {
         run = run < least ? least : run;
         return (int)cdiv(units, run);
     };
-    auto round = [&](bool by_few) { return by_few ? 256 : 512; };   // blocks that run at once
+    auto round = [&](bool by_few) { return by_few && a.D == 256 ? 256 : 512; };   // blocks that run at once
     c.psplits = c.apart ? cut(pu, pwork, pleast, round(c.pfew)) : 0;
     c.osplits = cut(ou, owork, oleast, round(c.ofew) * (a.seq_lens != nullptr ? 4 : 1));
+    // Rows of few slots: a block of eight waves walks them without parts where four would leave five units a wave (16 us, and 17 of two
+    // parts and their merge).
+    c.owaves = 4;
+    if (c.ofew && !c.apart && c.osplits > 1 && ou <= 40 && a.D != 256) {
+        c.owaves = 8;
+        c.osplits = 1;
+    }
     c.nparts = c.psplits + c.osplits;
 }
 

@@ -64,17 +64,27 @@ template <> struct SpanMma<bf16_t> {
 template <int D> __device__ __forceinline__ int sp_kpiece(int t, int c) { return c ^ (t & (D >= 128 ? 15 : 7)); }
 template <int D> __device__ __forceinline__ int sp_vpiece(int t, int c) { return c ^ (D >= 128 ? (t & 3) << 2 : (t >> 1 & 1) << 2); }
 
-// Eight codes of a packed word (4 bits: the word; 2 bits: its lower half) as fp16, in order.
-template <int BITS> __device__ __forceinline__ void sp_codes8(u32 w, u32 magic, u32 (&c)[4]) {
-    const u32x4 r = __builtin_bit_cast(u32x4, unpack8<BITS>(w, magic));
-    if (BITS == 4) {   // pairs (0,4) (1,5) (2,6) (3,7)
-        c[0] = pair_lo(r[0], r[1]); c[1] = pair_lo(r[2], r[3]); c[2] = pair_hi(r[0], r[1]); c[3] = pair_hi(r[2], r[3]);
-    } else {           // pairs (0,8) (1,9) (2,10) (3,11), and of the word eight bits on (4,12) ...
-        const u32x4 s = __builtin_bit_cast(u32x4, unpack8<BITS>(w >> 8, magic));
-        c[0] = pair_lo(r[0], r[1]); c[1] = pair_lo(r[2], r[3]); c[2] = pair_lo(s[0], s[1]); c[3] = pair_lo(s[2], s[3]);
-    }
+// Eight codes of a packed word (4 bits: the word; 2 bits: its bytes `first` and `first` + 1) as fp16, in order.  A byte is set in both
+// halves of a register and the codes are taken where they stand, adjacent ones one in each half, as the low mantissa bits of a number
+// whose unit is the place: bits 0 and up of 1024, bits 2 and up of 256, bits 4 and up of 64, bits 6 and up of 16.
+template <int BITS> struct SpanMagic {
+    u32 even = vreg_const(BITS == 4 ? 0x54006400u : 0x5C006400u), odd = vreg_const(0x4C005400u);
+};
+template <int BITS> __device__ __forceinline__ void sp_codes8(u32 w, const SpanMagic<BITS> &magic, u32 (&c)[4], int first = 0) {
+    if constexpr (BITS == 4) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) c[i] = as_u(as_h2(c[i]) + as_h2(Magic<BITS>::neg_off_pair));
+        for (int i = 0; i < 4; ++i) {
+            const u32 x = __builtin_amdgcn_perm(0u, w, 0x00010001u * i);
+            c[i] = as_u(as_h2((x & 0x00F0000Fu) | magic.even) + f16x2{(f16)-1024.f, (f16)-64.f});
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const u32 x = __builtin_amdgcn_perm(0u, w, 0x00010001u * (first + i));
+            c[2 * i] = as_u(as_h2((x & 0x000C0003u) | magic.even) + f16x2{(f16)-1024.f, (f16)-256.f});
+            c[2 * i + 1] = as_u(as_h2((x & 0x00C00030u) | magic.odd) + f16x2{(f16)-64.f, (f16)-16.f});
+        }
+    }
 }
 __device__ __forceinline__ u32x4 sp_values8(const u32 (&c)[4], uint4 scale, uint4 zero) {
     const u32 s[4] = {scale.x, scale.y, scale.z, scale.w}, z[4] = {zero.x, zero.y, zero.z, zero.w};
@@ -502,7 +512,7 @@ template <int BITS, typename T, int D, int MAPS, int WT> __device__ __forceinlin
             if (fill == raw0 + RAWS * Tile::RAW) fill = raw0;
         };
         // a unit from the ring into a tile
-        const u32 magic = vreg_const(Magic<BB>::bits);
+        const SpanMagic<BB> magic;
         constexpr int KROWS = SP_THREADS / CH;             // slots that the threads cover at a time
         constexpr int VSTEPS = UNIT * D / 16 / SP_THREADS; // sixteen slots each, of a thread's channel
         const char *take = lds + Tile::BUF;
@@ -531,9 +541,9 @@ template <int BITS, typename T, int D, int MAPS, int WT> __device__ __forceinlin
                 u32x4 x[2];
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {   // eight slots each
-                    const u32 w = BB == 4 ? words[(2 * step + k) * D] : words[step * D] >> (16 * k);
+                    const u32 w = words[(BB == 4 ? 2 * step + k : step) * D];
                     u32 code[4];
-                    sp_codes8<BB>(w, magic, code);
+                    sp_codes8<BB>(w, magic, code, 2 * k);
                     x[k] = sp_values8(code, meta[k], meta[TP + k]);
                 }
                 if (n_live < UNIT) {   // a slot past the live ones may hold anything: its weight is zero, its value has to be finite
