@@ -143,6 +143,8 @@ template <int MAPS, int WAVES> __global__ __launch_bounds__(256) void span_merge
             float mn = m[w];
 #pragma unroll
             for (int p = 0; p < MERGE_AT_ONCE; ++p) mn = fmaxf(mn, x[p].x);
+#pragma unroll
+            for (int p = 0; p < MERGE_AT_ONCE; ++p) l[w] = x[p].y != x[p].y ? x[p].y : l[w];   // (a row of NaN has no maximum)
             if (mn == -INFINITY) continue;   // (parts without a visible slot: their sums are not written)
             const float f = exp2f(m[w] - mn);
             m[w] = mn;
@@ -173,6 +175,7 @@ template <int MAPS, int WAVES> __global__ __launch_bounds__(256) void span_merge
         for (int w = 0; w < MAPS; ++w)
             for (int v = 1; v < WAVES; ++v) {
                 const float *o = s_part[v][w], mn = fmaxf(m[w], o[0]);
+                if (o[1] != o[1]) l[w] = o[1];
                 if (mn == -INFINITY) continue;
                 const float f = exp2f(m[w] - mn), by = exp2f(o[0] - mn);
                 m[w] = mn;

@@ -31,9 +31,7 @@ template <int BITS, int D, int WAVES_> struct SpanFew {
     static_assert(RING >= 3 && LDS <= 160 * 1024, "room for a unit at work and two under way");
 };
 
-template <int BITS, int D, int MAPS, int WAVES>
-__global__ __launch_bounds__((64 * WAVES)) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2, D == 256 ? 1 : 2)))
-void span_few_kernel(SpanCall c) {
+template <int BITS, int D, int MAPS, int WAVES> __device__ __forceinline__ void span_few_block(const SpanCall &c, int id) {
     extern __shared__ __align__(16) char lds[];
     using F = SpanFew<BITS, D, WAVES>;
     using M = SpanMma<f16>;
@@ -45,7 +43,6 @@ void span_few_kernel(SpanCall c) {
     const int before = (int)span_prefix_slots(a);
 
     // ---- the block: the prefix under the rows of all sequences, or a sequence's slots under its rows; kv head fastest
-    int id = (int)blockIdx.x;
     const int shared_blocks = c.apart && c.pfew ? c.psplits * Hkv : 0;
     const bool shared = id < shared_blocks;
     if (!shared) id -= shared_blocks;
@@ -94,6 +91,13 @@ void span_few_kernel(SpanCall c) {
     const int tail0 = (int)a.prefix.n_packed, tail1 = before + (int)a.own.n_packed;
     const int total = units_seen(0, np0) + units_seen(tail0, nt0) + units_seen(before, np1) + units_seen(tail1, nt1);
     const int w0 = (int)((int64_t)total * split / splits), w1 = (int)((int64_t)total * (split + 1) / splits);
+    if (w0 == w1 && c.nparts > 1) {   // (uniform) nothing: sums are not written
+        if (tid < rows * MAPS) {
+            int x, y;
+            *(float2 *)(c.ml + ((row_of(tid / MAPS, x, y) * c.nparts + part) * MAPS + tid % MAPS) * 2) = make_float2(-INFINITY, 0.f);
+        }
+        return;
+    }
 
     // ---- queries as the B operand of the scores
     u32x4 q[KS];
@@ -443,6 +447,31 @@ void span_few_kernel(SpanCall c) {
     }
 }
 
+template <int BITS, int D, int MAPS, int WAVES>
+__global__ __launch_bounds__((64 * WAVES)) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2, D == 256 ? 1 : 2))) void span_few_kernel(SpanCall c) {
+    span_few_block<BITS, D, MAPS, WAVES>(c, (int)blockIdx.x);
+}
+
+// Blocks of a prefix in tiles and behind them blocks of own slots, which share the CUs with them (in two launches 184 us for 128 sequences of
+// 1k slots on a prefix of 32k, together 171; the kinds in turn 226, as a CU then holds two of one kind).
+template <int BITS, int D> __global__ __launch_bounds__(SP_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2))) void span_both_kernel(SpanCall c) {
+    const int id = (int)blockIdx.x, tiles = span_shared_blocks(c);
+    if (id < tiles) span_mfma_block<BITS, f16, D, 1>(c, id);
+    else span_few_block<BITS, D, 1, 4>(c, id - tiles);
+}
+
+template <int BITS, int D> int launch_span_both_as(const SpanCall &c) {
+    constexpr int bytes = SpanTile<BITS, D>::LDS > SpanFew<BITS, D, 4>::LDS ? SpanTile<BITS, D>::LDS : SpanFew<BITS, D, 4>::LDS;
+    const auto kernel = span_both_kernel<BITS, D>;
+    static std::atomic<bool> allowed[64] = {};
+    if (int rc = span_allow_lds((const void *)kernel, bytes, allowed)) return rc;
+    const int64_t tiles = (int64_t)c.psplits * c.ptiles * c.a.Hkv, few = c.a.B * c.a.Hkv * c.osplits, blocks = tiles + few;
+    VQ_REQUIRE(blocks < (INT64_C(1) << 23), VQ_ERR_UNSUPPORTED, "attention over spans: too many sequences and heads for one launch");
+    kernel<<<(unsigned)blocks, SP_THREADS, bytes, (hipStream_t)c.a.stream>>>(c);
+    VQ_HIP_CHECK_LAUNCH("attention over spans");
+    return VQ_OK;
+}
+
 template <int BITS, int D, int MAPS, int WAVES> int launch_span_few_of(const SpanCall &c) {
     constexpr int bytes = SpanFew<BITS, D, WAVES>::LDS;
     const auto kernel = span_few_kernel<BITS, D, MAPS, WAVES>;
@@ -464,6 +493,8 @@ template <int BITS, int D, int MAPS> int launch_span_few_as(const SpanCall &c) {
 
 int launch_span_few2(const SpanCall &c, int maps);
 int launch_span_few4(const SpanCall &c, int maps);
+int launch_span_both2(const SpanCall &c);
+int launch_span_both4(const SpanCall &c);
 
 #define VQ_SPAN_FEW_LAUNCHER(NAME, BITS)                                                                                \
     namespace vq {                                                                                                      \

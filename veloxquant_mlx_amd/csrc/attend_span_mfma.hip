@@ -16,6 +16,9 @@ static bool packed_slots_fit(const vq_store_attend_args &a, const vq_kv_store &s
     return (all & 15) == 0 && s.cap_tokens % a.group == 0 && s.cap_tokens % (32 / a.pack_bits) == 0;
 }
 
+// a prefix in tiles and own slots of few rows in one launch (heads of 256 channels have other waves a CU for each)
+static bool span_both(const SpanCall &c) { return c.apart && !c.pfew && c.ofew && c.a.D != 256; }
+
 bool span_mfma_supported(const vq_store_attend_args &a) {
     if ((a.D != 64 && a.D != 128 && a.D != 256) || a.dtype == VQ_F32 || (((uintptr_t)a.q | (uintptr_t)a.out) & 15) != 0) return false;
     if (!plain_rows_fit(a.prefix) || !plain_rows_fit(a.own)) return false;
@@ -37,9 +40,9 @@ void span_mfma_plan(SpanCall &c, int maps) {
     c.apart = prefix_slots && a.B > 1 && r1 <= most / 2;
     c.pfew = packed && all <= few;
     c.ofew = packed && r1 <= few;
-    // One round of blocks of equal runs, two blocks a CU (one of few rows or heads of 256 channels), each side for itself where they are launches of their own; own slots of sequences
-    // that differ in length even out over four rounds.  A run is four units a wave or more for few rows, eight units a block else: a block
-    // costs about as much to start and end.
+    // One round of blocks of equal runs, two blocks a CU (one of few rows of 256 channels, or of tiles beside few rows), each side for itself
+    // where they differ; own slots of sequences that differ in length even out over four rounds.  A run is four units a wave or more for few
+    // rows, eight units a block else: a block costs about as much to start and end.
     auto side = [&](bool by_few, int64_t rows, int64_t slots32, int64_t slots64, int64_t times, int &wt, int &tiles, int64_t &units, int64_t &least) {
         wt = !by_few && a.D != 256 && rows <= most / 2 ? 2 : 1;
         tiles = by_few ? 1 : (int)cdiv(rows, most / wt);
@@ -58,7 +61,9 @@ void span_mfma_plan(SpanCall &c, int maps) {
         return (int)cdiv(units, run);
     };
     auto round = [&](bool by_few) { return by_few && a.D == 256 ? 256 : 512; };   // blocks that run at once
-    c.psplits = c.apart ? cut(pu, pwork, pleast, round(c.pfew)) : 0;
+    // (tiles beside few rows: one a CU where the few rows' work can fill the other half -- 43 us and 47 of two a CU for 21 sequences of 0.6k slots
+    // on 16k -- and two where not, 136 us and 150 for 128 of 80 slots on 32k)
+    c.psplits = c.apart ? cut(pu, pwork, pleast, span_both(c) && pwork <= owork ? 256 : round(c.pfew)) : 0;
     c.osplits = cut(ou, owork, oleast, round(c.ofew) * (a.seq_lens != nullptr ? 4 : 1));
     // Rows of few slots: a block of eight waves walks them without parts where four would leave five units a wave (16 us, and 17 of two
     // parts and their merge).
@@ -73,6 +78,7 @@ void span_mfma_plan(SpanCall &c, int maps) {
 int launch_span_mfma(const SpanCall &c, int maps) {
     const vq_store_attend_args &a = c.a;
     if (a.prefix.n_packed + a.own.n_packed == 0) return a.dtype == VQ_F16 ? launch_span_rows_f16(c, maps) : launch_span_rows_bf16(c, maps);
+    if (span_both(c)) return a.pack_bits == 4 ? launch_span_both4(c) : launch_span_both2(c);
     if (int rc = a.pack_bits == 4 ? launch_span_packed4(c, maps) : launch_span_packed2(c, maps)) return rc;
     return a.pack_bits == 4 ? launch_span_few4(c, maps) : launch_span_few2(c, maps);
 }

@@ -160,7 +160,7 @@ template <int BITS, int D> struct SpanTile {
 __host__ __device__ __forceinline__ int span_shared_blocks(const SpanCall &c) { return c.apart && !c.pfew ? c.psplits * c.ptiles * (int)c.a.Hkv : 0; }
 
 // One block.  WT = 2: two waves share rows, each with its half of every unit.
-template <int BITS, typename T, int D, int MAPS, int WT> __device__ __forceinline__ void span_mfma_block(const SpanCall &c) {
+template <int BITS, typename T, int D, int MAPS, int WT> __device__ __forceinline__ void span_mfma_block(const SpanCall &c, int id) {
     extern __shared__ __align__(16) char lds[];
     using M = SpanMma<T>;
     using Tile = SpanTile<BITS, D>;
@@ -173,7 +173,6 @@ template <int BITS, typename T, int D, int MAPS, int WT> __device__ __forceinlin
 
     // ---- the block: kv head fastest (blocks of one kv head and run, which read the same slots, lie a multiple of the head count
     // apart), under a causal mask the row tiles that see most first
-    int id = (int)blockIdx.x;
     const int shared_blocks = span_shared_blocks(c);
     const bool shared = id < shared_blocks;
     int b = 0, split, tile, splits, rows, part;
@@ -236,6 +235,10 @@ template <int BITS, typename T, int D, int MAPS, int WT> __device__ __forceinlin
     const int tail0 = (int)a.prefix.n_packed, tail1 = before + (int)a.own.n_packed;   // places of the plain slots
     const int total = units_seen(0, np0) + units_seen(tail0, nt0) + units_seen(before, np1) + units_seen(tail1, nt1);
     const int w0 = (int)((int64_t)total * split / splits), w1 = (int)((int64_t)total * (split + 1) / splits);
+    if (w0 == w1 && c.nparts > 1) {   // (uniform) nothing: sums are not written
+        if (th == 0 && h == 0 && j < rows) *(float2 *)(c.ml + ((qrow * c.nparts + part) * MAPS + map) * 2) = make_float2(-INFINITY, 0.f);
+        return;
+    }
 
     // ---- queries as the B operand: row n, channels 16 ks + 8 h .. + 7
     const float c2 = __builtin_fabsf(a.scale) * LOG2E;
@@ -696,10 +699,14 @@ template <int BITS, typename T, int D, int MAPS, int WT> __device__ __forceinlin
         }
 }
 
+template <int BITS, typename T, int D, int MAPS> __device__ __forceinline__ void span_mfma_block(const SpanCall &c, int id) {
+    if (D != 256 && (id < span_shared_blocks(c) ? c.pwt : c.owt) == 2) span_mfma_block<BITS, T, D, MAPS, D == 256 ? 1 : 2>(c, id);
+    else span_mfma_block<BITS, T, D, MAPS, 1>(c, id);
+}
+
 template <int BITS, typename T, int D, int MAPS>
 __global__ __launch_bounds__(SP_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2))) void span_mfma_kernel(SpanCall c) {
-    if (D != 256 && ((int)blockIdx.x < span_shared_blocks(c) ? c.pwt : c.owt) == 2) span_mfma_block<BITS, T, D, MAPS, D == 256 ? 1 : 2>(c);
-    else span_mfma_block<BITS, T, D, MAPS, 1>(c);
+    span_mfma_block<BITS, T, D, MAPS>(c, (int)blockIdx.x);
 }
 
 // More than 64 KB of block-shared memory has to be allowed per kernel and device, once (a second setter repeats the same call).
