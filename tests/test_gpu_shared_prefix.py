@@ -56,6 +56,33 @@ def test_plain_rows(dtype, B, Hq, Hkv, D, n, own, Sq):
 
 
 @pytest.mark.parametrize("kw", [
+    dict(B=40, Hq=8, Hkv=2, D=128, prefix=(1024, 70), own=(256, 33), bits=4), dict(B=40, Hq=8, Hkv=2, D=64, prefix=(640, 3), own=(128, 1), bits=2),
+    dict(B=24, Hq=12, Hkv=3, D=128, prefix=(2048, 0), own=(512, 9), bits=4, group=64, lens=[(b * 97) % 522 for b in range(24)]),
+    dict(B=70, Hq=4, Hkv=4, D=128, prefix=(384, 5), own=(128, 20), bits=2, window=150), dict(B=20, Hq=6, Hkv=2, D=256, prefix=(512, 40), own=(128, 9)),
+    dict(B=9, Hq=16, Hkv=2, D=128, prefix=(512, 1), own=(128, 30), Sq=5, dtype=BF16), dict(B=33, Hq=2, Hkv=2, D=128, prefix=(0, 90), own=(128, 30)),
+    dict(B=3, Hq=16, Hkv=2, D=128, prefix=(4096, 0), own=(0, 140), Sq=7, group=128)])
+def test_prefixes_of_many_rows(kw):
+    """The prefix under the rows of all sequences, next to own slots under few rows, with lengths and windows that leave runs empty."""
+    require_gpu()
+    _case(**kw)
+
+
+@pytest.mark.parametrize("prefix,own,B", [((0, 90), (0, 40), 2), ((1024, 70), (256, 33), 40), ((4096, 0), (128, 3), 2), ((512, 0), (0, 9), 2)])
+def test_a_query_of_nan_is_nan_and_alone(prefix, own, B):
+    """Its row, however the slots are cut, and no other."""
+    require_gpu()
+    p, _, _ = store(1, 2, *prefix, 128, seed=1)
+    o, _, _ = store(B, 2, *own, 128, seed=2)
+    q = torch.randn((B, 8, 1, 128), generator=torch.Generator(device="cuda").manual_seed(0), device="cuda").half()
+    clean = K.shared_prefix_attend(q, p, **o, scale=0.1)
+    q[1, 3, 0, 5] = float("nan")
+    got = K.shared_prefix_attend(q, p, **o, scale=0.1)
+    assert bool(got[1, 3].isnan().all())
+    got[1, 3] = clean[1, 3]
+    assert torch.equal(got, clean)
+
+
+@pytest.mark.parametrize("kw", [
     dict(bits=3, group=32, v_layout="channel"), dict(bits=8, group=32), dict(bits=1, group=32), dict(bits=4, v_layout="channel"),
     dict(bits=4, meta=F32), dict(bits=4, group=16), dict(bits=4, dtype=F32), dict(bits=4, dtype=BF16), dict(bits=2, dtype=BF16, group=64)])
 def test_other_stores(kw):

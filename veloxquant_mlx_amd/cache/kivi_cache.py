@@ -83,6 +83,16 @@ def own_half_of_paired_output(o: torch.Tensor, n_kv_heads: int) -> torch.Tensor:
     return res.view(*lead, H * R, Sq, D)
 
 
+def batch_lengths(name: str, lengths, q: torch.Tensor) -> torch.Tensor:
+    """Live tokens of every sequence of ``q``'s batch, as the kernels take them: int64 ``[B]`` on its device."""
+    n = lengths
+    if not (isinstance(n, torch.Tensor) and n.dtype == torch.int64 and n.ndim == 1 and n.device == q.device and n.is_contiguous()):
+        n = torch.as_tensor(lengths, device=q.device).to(torch.int64).reshape(-1).contiguous()
+    if n.numel() != q.shape[0]:
+        raise ValueError(f"{name}: lengths has {n.numel()} entries for a batch of {q.shape[0]}")
+    return n
+
+
 class KIVIKVCache(FP16KVCache):
     """KV cache with KIVI asymmetric group quantisation.
 
@@ -96,6 +106,7 @@ class KIVIKVCache(FP16KVCache):
 
     def __init__(self, config: Any) -> None:
         super().__init__()
+        self._config = config
         self._head_dim = int(config.head_dim)
         b = config.bit_width_inlier
         if isinstance(b, list):
@@ -464,6 +475,49 @@ class KIVIKVCache(FP16KVCache):
         return self._attend(q, scale, causal=causal, sliding_window=sliding_window, fixed_order=fixed_order, lengths=lengths,
                             num_splits=num_splits)
 
+    def fused_differential_sdpa(self, q: torch.Tensor, lam: torch.Tensor | float, scale: float, *, causal: bool = True,
+                                sliding_window: int = 0, lengths: torch.Tensor | None = None, norm_weight: torch.Tensor | None = None,
+                                norm_eps: float = 1e-5, gain: float = 1.0) -> torch.Tensor:
+        """Differential attention of ``q [B,H_q,S_q,D]`` over the cache (``(softmax(q1 k1^T * scale) - lam * softmax(q2 k2^T * scale)) v``, the
+        two halves of a head's channels; :func:`veloxquant_mlx_amd.kernels.differential_attend`), masks and ``lengths`` as for
+        :meth:`fused_sdpa`.  ``lam``: a number, or float32 of one value or ``[H_q]`` on the device; ``norm_weight``, ``norm_eps`` and
+        ``gain``: the layer's head norm.  Heads of 64 channels need ``kivi_pair_heads=False`` in memory-bound mode: a pair of heads
+        kept side by side has no halves of its own."""
+        name = f"{type(self).__name__}.fused_differential_sdpa"
+        if not self._fused_enabled:
+            raise RuntimeError(f"{name} called but fused_sdpa was not enabled via KVCacheConfig.fused_sdpa=True.")
+        if self.offset == 0:
+            raise RuntimeError(f"{name} called before any tokens were cached via update_and_fetch.")
+        if self._pair:
+            raise ValueError(f"{name}: heads of 64 channels are kept in pairs; set kivi_pair_heads=False")
+        if self._extra_attend_args():
+            raise ValueError(f"{name}: a cache with rows kept outside its packed store is not taken")
+        if lengths is not None:
+            lengths = batch_lengths(name, lengths, q)
+        if q.shape[2] == 1:
+            self._drop_tiles()
+        return K.differential_attend(q, lam, **self._store_args(), scale=float(scale), causal=bool(causal), seq_lens=lengths,
+                                     sliding_window=int(sliding_window or 0), norm_weight=norm_weight, norm_eps=float(norm_eps),
+                                     gain=float(gain))
+
+    def share(self):
+        """A :class:`~veloxquant_mlx_amd.cache.SharedPrefixKIVICache`: these tokens (a batch of one, memory-bound mode), copied, as the prefix
+        that the sequences of a batch share."""
+        from .shared_prefix_cache import SharedPrefixKIVICache
+        return SharedPrefixKIVICache(self)
+
+    def _store_args(self) -> dict:
+        """The cache's slots as the kernels' arguments, a deferred token stored."""
+        self._store_pending()
+        nq, n_tail = self._n_quantized, self.offset - self._n_quantized
+        if self._memory_bound:
+            tk, tv = self._tail_k, self._tail_v
+        elif n_tail:
+            tk, tv = self.keys[:, :, nq:], self.values[:, :, nq:]
+        return dict(k_packed=self._kp, k_scale=self._ks, k_zero=self._kz, v_packed=self._vp, v_scale=self._vs, v_zero=self._vz, n_packed=nq,
+                    bits=self._field, group_size=self._group_size, v_layout=self._v_layout, k_tail=tk if n_tail else None,
+                    v_tail=tv if n_tail else None, n_tail=n_tail)
+
     def _attends_in_one_launch(self) -> bool:
         """Whether a decode step over heads of 128 channels, or of 64 kept in pairs, takes the matrix-unit decode launch (its gate
         on the cache's side)."""
@@ -480,12 +534,7 @@ class KIVIKVCache(FP16KVCache):
             self._store_pending()
         extra = self._extra_attend_args()
         if lengths is not None:
-            n = lengths
-            if not (isinstance(n, torch.Tensor) and n.dtype == torch.int64 and n.ndim == 1 and n.device == q.device and n.is_contiguous()):
-                n = torch.as_tensor(lengths, device=q.device).to(torch.int64).reshape(-1).contiguous()
-            if n.numel() != q.shape[0]:
-                raise ValueError(f"KIVIKVCache.fused_sdpa: lengths has {n.numel()} entries for a batch of {q.shape[0]}")
-            lengths = n
+            lengths = batch_lengths("KIVIKVCache.fused_sdpa", lengths, q)
         if step and q.ndim == 4 and self._memory_bound and nq > 0 and n_tail > 0 and not extra:
             k_new, v_new = self._pending if self._pending is not None else (None, None)
             out = K.kivi_decode_attend(q, self._kp, self._ks, self._kz, self._vp, self._vs, self._vz, nq, self._field, self._group_size,

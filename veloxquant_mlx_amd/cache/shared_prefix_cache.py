@@ -1,0 +1,119 @@
+"""KIVI cache of a batch of sequences behind a prefix that they share.
+
+Many sequences that start with the same tokens (a system prompt, a document asked about more than once, samples of one prompt) hold
+those tokens once: the prefix, packed, for a batch of one, and behind it every sequence's own tokens in a memory-bound
+:class:`KIVIKVCache`.  Attention reads the prefix once for all of them (:func:`veloxquant_mlx_amd.kernels.shared_prefix_attend`)::
+
+    cache.update_and_fetch(k, v)           # the prompt, a batch of one
+    shared = cache.share()
+    shared.update_and_fetch(k, v)          # [B, H, S, D]: the next tokens of B sequences
+    out = shared.fused_sdpa(q, scale)
+
+Positions go on behind the prefix: ``offset`` counts its tokens.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from .. import kernels as K
+from .kivi_cache import KIVIKVCache, batch_lengths, own_half_of_paired_output, pad_queries_for_paired_heads
+
+
+class SharedPrefixKIVICache:
+    """``[prefix | own tokens]`` of every sequence of a batch; :meth:`KIVIKVCache.share` makes one.
+
+    The prefix is a copy of the cache's tokens at that time and does not change any more; several objects may stand on one
+    (:meth:`branch`).  A cache of its own in every other respect: ``update_and_fetch``, ``fused_sdpa``, ``trim`` (of the own tokens),
+    ``offset``, ``nbytes``."""
+
+    _memory_bound = True   # attention goes through fused_sdpa; update_and_fetch returns placeholders
+
+    def __init__(self, cache: KIVIKVCache) -> None:
+        if type(cache) is not KIVIKVCache or not cache._memory_bound:
+            raise ValueError("SharedPrefixKIVICache: the prefix must be a KIVIKVCache with fused_sdpa_memory_bound=True")
+        if cache.offset == 0 or cache._shape_bhd[0] != 1:
+            raise ValueError(f"SharedPrefixKIVICache: the prefix must hold tokens of a batch of one, got {cache.offset} tokens of a batch "
+                             f"of {cache._shape_bhd[0]}")
+        prefix = KIVIKVCache(cache._config)
+        prefix._max_ctx = None   # (no room for more tokens)
+        prefix.state = cache.state
+        prefix._kv_heads = cache._kv_heads
+        self._join(prefix)
+
+    def _join(self, prefix: KIVIKVCache) -> None:
+        self._prefix = prefix
+        self._prefix_args = prefix._store_args()
+        self._kv_heads = abs(prefix._kv_heads) if prefix._pair else prefix._shape_bhd[1]
+        self._head_dim = prefix._shape_bhd[2] // (2 if prefix._pair else 1)
+        self._own = KIVIKVCache(prefix._config)
+        self._own._launch_stores = False   # (no launch of this cache stores a token that was held back)
+
+    def branch(self) -> "SharedPrefixKIVICache":
+        """Another batch on the same prefix, without tokens of its own yet."""
+        other = object.__new__(SharedPrefixKIVICache)
+        other._join(self._prefix)
+        return other
+
+    @property
+    def prefix_length(self) -> int:
+        return self._prefix.offset
+
+    @property
+    def offset(self) -> int:
+        """Tokens of a sequence, the prefix included: the position of the next one."""
+        return self._prefix.offset + self._own.offset
+
+    def size(self) -> int:
+        return self.offset
+
+    def empty(self) -> bool:
+        return False
+
+    def update_and_fetch(self, keys: torch.Tensor, values: torch.Tensor):
+        """Append ``[B,H,S,D]`` keys and values to the sequences' own tokens, quantised as they age as in any
+        :class:`KIVIKVCache`; returns zero-stride placeholders of the whole length."""
+        dtype = self._prefix._tail_k.dtype if self._prefix_args["n_tail"] else keys.dtype
+        if keys.ndim != 4 or keys.shape[1] != self._kv_heads or keys.shape[3] != self._head_dim or keys.dtype != dtype or values.dtype != dtype:
+            raise ValueError(f"SharedPrefixKIVICache.update_and_fetch: keys and values must be [B, {self._kv_heads}, S, {self._head_dim}] {dtype} "
+                             f"as the prefix is, got {tuple(keys.shape)} {keys.dtype} and {tuple(values.shape)} {values.dtype}")
+        if self._own.offset and keys.shape[0] != self._own._shape_bhd[0]:
+            raise ValueError(f"SharedPrefixKIVICache.update_and_fetch: {keys.shape[0]} sequences, this cache holds {self._own._shape_bhd[0]}")
+        z = self._own.update_and_fetch(keys, values)[0]
+        z = z[:, :, :1].expand(keys.shape[0], self._kv_heads, self.offset, self._head_dim)
+        return z, z
+
+    def fused_sdpa(self, q: torch.Tensor, scale: float, *, causal: bool = True, sliding_window: int = 0,
+                   lengths: torch.Tensor | None = None) -> torch.Tensor:
+        """Attention of ``q [B,H_q,S_q,D]`` over prefix and own tokens, queries aligned to the end, under the masks of
+        :meth:`KIVIKVCache.fused_sdpa`.  ``lengths`` (int ``[B]``, on the device or the host) gives every sequence of a right-padded
+        batch its number of live tokens, the prefix included (and so no fewer than those).  The same bits from run to run."""
+        name = "SharedPrefixKIVICache.fused_sdpa"
+        if lengths is not None:
+            if not (isinstance(lengths, torch.Tensor) and lengths.is_cuda) and min(torch.as_tensor(lengths).reshape(-1).tolist(), default=0) < self.prefix_length:
+                raise ValueError(f"{name}: lengths count the prefix of {self.prefix_length} tokens")
+            lengths = batch_lengths(name, lengths, q) - self.prefix_length
+        pair = self._prefix._pair
+        if pair:
+            if q.ndim != 4 or q.shape[3] != self._head_dim or q.shape[1] % self._kv_heads:
+                raise ValueError(f"{name}: q {tuple(q.shape)} over {self._kv_heads} kv heads of {self._head_dim} channels")
+            q = pad_queries_for_paired_heads(q, self._kv_heads)
+        own = self._own._store_args() if self._own.offset else {}
+        out = K.shared_prefix_attend(q, self._prefix_args, **own, scale=float(scale), causal=bool(causal), seq_lens=lengths,
+                                     sliding_window=int(sliding_window or 0))
+        return own_half_of_paired_output(out, self._kv_heads) if pair else out
+
+    def is_trimmable(self) -> bool:
+        return True
+
+    def trim(self, n: int) -> int:
+        """Drop the last ``n`` own tokens of every sequence; the prefix stays."""
+        return self._own.trim(n)
+
+    @property
+    def nbytes(self) -> int:
+        """Bytes of the own tokens and, once, of the prefix."""
+        return self._prefix.nbytes + self._own.nbytes
+
+
+__all__ = ["SharedPrefixKIVICache"]
