@@ -284,7 +284,8 @@ template <int BITS, typename T, int D, int MAPS, int WT> __device__ __forceinlin
     constexpr int AHEAD = 4;
     auto scores = [&](u32 tile) __attribute__((always_inline)) {
         constexpr int N = X * KS;
-        auto key = [&](int i) __attribute__((always_inline)) { return *(L4 *)(uintptr_t)((key0 ^ (32 * (i % KS))) + tile + i / KS * (32 * D * 2)); };
+        // (the stretches in turn: a product waits 52 cycles for the one it adds to, and takes 32)
+        auto key = [&](int i) __attribute__((always_inline)) { return *(L4 *)(uintptr_t)((key0 ^ (32 * (i / X))) + tile + i % X * (32 * D * 2)); };
         u32x4 k[AHEAD];
 #pragma unroll
         for (int i = 0; i < AHEAD && i < N; ++i) k[i] = key(i);
@@ -294,7 +295,7 @@ template <int BITS, typename T, int D, int MAPS, int WT> __device__ __forceinlin
             for (int r = 0; r < 16; ++r) S[x][r] = 0.f;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            S[i / KS] = M::mma(k[i % AHEAD], q[i % KS], S[i / KS]);
+            S[i % X] = M::mma(k[i % AHEAD], q[i / X], S[i % X]);
             if (i + AHEAD < N) k[i % AHEAD] = key(i + AHEAD);
             __builtin_amdgcn_sched_barrier(0);
         }
