@@ -150,8 +150,8 @@ template <int BITS, int D> struct SpanTile {
     static constexpr int RAWS = BITS ? (MOST - BUF) / RAW < 6 ? (MOST - BUF) / RAW : 6 : 0;   // beside the one tile
     static constexpr int PIECES = RAW / 1024;            // copies of 1 KB, dealt to the waves
     static constexpr int COPIES = (PIECES + SP_WAVES - 1) / SP_WAVES;
-    static constexpr int EXCHANGE = SP_WAVES / 2 * (D / 8 * 64 + 64) * 16;   // the rows of half of the waves, at the end
     static constexpr int max(int x, int y) { return x > y ? x : y; }
+    static constexpr int EXCHANGE = max(SP_WAVES / 2 * (D / 8 * 64 + 64) * 16, SP_WAVES * 32 * (D < 128 ? 4 * D + 16 : 528));   // rows at the end, of half of the waves or by 128 channels
     static constexpr int LDS = max(max(BITS ? BUF + RAWS * RAW : 0, ROW_BUFS * ROW_BUF), EXCHANGE);
     static_assert(LDS <= MOST && ROW_BUFS >= 2 && (BITS == 0 || RAWS >= 3) && RAW % 1024 == 0 && KEYS % (1024 * SP_WAVES) == 0, "tile sizes");
 };
@@ -635,27 +635,47 @@ template <int BITS, typename T, int D, int MAPS, int WT> __device__ __forceinlin
                 }
         }
     }
+    // The wave's rows go out through its own room in LDS, where a row is contiguous: lanes n held a row each, of which a store would write
+    // eight or sixteen bytes (so written, the end of a block took 7000 cycles at 128 channels and 25000 at 256, now XX and XX).
+    constexpr int CB = D < 128 ? D : 128, LR = CB / 4, RS = CB * 4 + 16;   // channels at a time, lanes a row, bytes of a row
+    auto rows_out = [&](char *mine, auto put) __attribute__((always_inline)) {
+#pragma unroll
+        for (int c0 = 0; c0 < D; c0 += CB) {
+#pragma unroll
+            for (int dt = 0; dt < CB / 32; ++dt)
+#pragma unroll
+                for (int r = 0; r < 16; r += 4) {
+                    const f32x16 &o = O[c0 / 32 + dt];
+                    *(float4 *)(mine + n * RS + (32 * dt + 2 * r + 4 * h) * 4) = make_float4(o[r], o[r + 1], o[r + 2], o[r + 3]);
+                }
+            asm volatile("" ::: "memory");   // (a wave's LDS accesses are in order; these are other lanes')
+#pragma unroll 4
+            for (int x = lane / LR; x < 32; x += 64 / LR)
+                put(x, c0 + lane % LR * 4, *(const float4 *)(mine + x * RS + lane % LR * 16));
+            asm volatile("" ::: "memory");
+        }
+    };
+    const int first = j0 + 32 * rg;
     if (c.nparts > 1) {
-        if (th == 1 || j >= rows) return;
-        const int64_t rec = (qrow * c.nparts + part) * MAPS + map;
-        if (h == 0) *(float2 *)(c.ml + rec * 2) = make_float2(m_run, l);
-        float *dst = c.sums + rec * D + 4 * h;
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-            for (int r = 0; r < 16; r += 4) *(float4 *)(dst + 32 * dt + 2 * r) = make_float4(O[dt][r], O[dt][r + 1], O[dt][r + 2], O[dt][r + 3]);
+        if (WT != 2) lds_barrier();   // (all waves have left the tiles)
+        if (th == 1) return;
+        if (h == 0 && j < rows) *(float2 *)(c.ml + ((qrow * c.nparts + part) * MAPS + map) * 2) = make_float2(m_run, l);
+        rows_out(lds + (WT == 2 ? (map * groups + rg) * (D / 8 * 64 + 64) * 16 : wave * 32 * RS), [&](int x, int ch, float4 v) __attribute__((always_inline)) {
+            const int64_t at = ((int64_t)__shfl((int)qrow, x) * c.nparts + part) * MAPS + map;
+            if (first + x < rows) *(float4 *)(c.sums + at * D + ch) = v;
+        });
         return;
     }
-    float by = l > 0.f || l != l ? 1.f / l : 0.f, gain = 1.f, sq = 0.f;
+    float by = l > 0.f || l != l ? 1.f / l : 0.f;
     if (MAPS == 2 && map == 1) by *= -span_lam(a, hkv * G + rem % G);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
         for (int r = 0; r < 16; ++r) O[dt][r] *= by;
+    float4 *other = (float4 *)lds + rg * (D / 8 * 64 + 64) + lane;   // (room for rows_out, too)
     bool norm = false;
+    lds_barrier();
     if (MAPS == 2) {
-        float4 *other = (float4 *)lds + rg * (D / 8) * 64 + lane;
-        lds_barrier();
         if (map == 1 && th == 0) {
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt)
@@ -671,33 +691,39 @@ template <int BITS, typename T, int D, int MAPS, int WT> __device__ __forceinlin
                 const float4 x = other[(4 * dt + r) * 64];
                 O[dt][4 * r] += x.x; O[dt][4 * r + 1] += x.y; O[dt][4 * r + 2] += x.z; O[dt][4 * r + 3] += x.w;
             }
-        gain = a.gain;
+        float gain = a.gain;
         norm = a.norm_weight != nullptr;
         if (norm) {
+            float sq = 0.f;
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) sq = __builtin_fmaf(O[dt][r], O[dt][r], sq);
             gain /= sqrtf((sq + __shfl_xor(sq, 32)) * (1.f / D) + a.norm_eps);
         }
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) O[dt][r] *= gain;
     }
-    if (th == 1 || j >= rows) return;
-    u16 *dst = (u16 *)a.out + qrow * D + 4 * h;
+    if (th == 1) return;
     const bool out_bf16 = a.dtype == VQ_BF16;
+    float4 weight[D / CB];
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-            float o[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                o[e] = O[dt][r + e] * gain;
-                if (norm) o[e] *= span_ld(a.norm_weight, a.norm_dtype, 32 * dt + 2 * r + 4 * h + e);
-            }
-            const uint2 x = out_bf16 ? make_uint2(SpanMma<bf16_t>::pack(o[0], o[1]), SpanMma<bf16_t>::pack(o[2], o[3]))
-                                     : make_uint2(SpanMma<f16>::pack(o[0], o[1]), SpanMma<f16>::pack(o[2], o[3]));
-            *(uint2 *)(dst + 32 * dt + 2 * r) = x;
-        }
+    for (int i = 0; i < D / CB; ++i) {
+        const int ch = i * CB + lane % LR * 4;
+        weight[i] = norm ? make_float4(span_ld(a.norm_weight, a.norm_dtype, ch), span_ld(a.norm_weight, a.norm_dtype, ch + 1), span_ld(a.norm_weight, a.norm_dtype, ch + 2),
+                                       span_ld(a.norm_weight, a.norm_dtype, ch + 3))
+                         : make_float4(1.f, 1.f, 1.f, 1.f);
+    }
+    rows_out(MAPS == 2 ? (char *)(other - lane) : lds + rg * 32 * RS, [&](int x, int ch, float4 v) __attribute__((always_inline)) {
+        const int64_t row = __shfl((int)qrow, x);
+        const float4 w = weight[D > CB ? ch / CB : 0];
+        v = make_float4(v.x * w.x, v.y * w.y, v.z * w.z, v.w * w.w);
+        if (first + x < rows)
+            *(uint2 *)((u16 *)a.out + row * D + ch) = out_bf16 ? make_uint2(SpanMma<bf16_t>::pack(v.x, v.y), SpanMma<bf16_t>::pack(v.z, v.w))
+                                                               : make_uint2(SpanMma<f16>::pack(v.x, v.y), SpanMma<f16>::pack(v.z, v.w));
+    });
 }
 
 template <int BITS, typename T, int D, int MAPS> __device__ __forceinline__ void span_mfma_block(const SpanCall &c, int id) {
