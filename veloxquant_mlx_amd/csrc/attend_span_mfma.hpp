@@ -638,7 +638,9 @@ template <int BITS, typename T, int D, int MAPS, int WT> __device__ __forceinlin
     // The wave's rows go out through its own room in LDS, where a row is contiguous: lanes n held a row each, of which a store would write
     // eight or sixteen bytes (so written, the end of a block took 7000 cycles at 128 channels and 25000 at 256, now XX and XX).
     constexpr int CB = D < 128 ? D : 128, LR = CB / 4, RS = CB * 4 + 16;   // channels at a time, lanes a row, bytes of a row
-    auto rows_out = [&](char *mine, auto put) __attribute__((always_inline)) {
+    const int first = j0 + 32 * rg;
+    auto rows_out = [&](char *mine, float times, auto begin, auto put) __attribute__((always_inline)) {
+        constexpr int AT_ONCE = D == 256 ? 4 : 8;
 #pragma unroll
         for (int c0 = 0; c0 < D; c0 += CB) {
 #pragma unroll
@@ -646,32 +648,40 @@ template <int BITS, typename T, int D, int MAPS, int WT> __device__ __forceinlin
 #pragma unroll
                 for (int r = 0; r < 16; r += 4) {
                     const f32x16 &o = O[c0 / 32 + dt];
-                    *(float4 *)(mine + n * RS + (32 * dt + 2 * r + 4 * h) * 4) = make_float4(o[r], o[r + 1], o[r + 2], o[r + 3]);
+                    *(float4 *)(mine + n * RS + (32 * dt + 2 * r + 4 * h) * 4) = make_float4(o[r] * times, o[r + 1] * times, o[r + 2] * times, o[r + 3] * times);
                 }
             asm volatile("" ::: "memory");   // (a wave's LDS accesses are in order; these are other lanes')
-#pragma unroll 4
-            for (int x = lane / LR; x < 32; x += 64 / LR)
-                put(x, c0 + lane % LR * 4, *(const float4 *)(mine + x * RS + lane % LR * 16));
+            const int ch = c0 + lane % LR * 4;
+            const float4 f = begin(ch);
+#pragma unroll 1
+            for (int x0 = lane / LR; x0 < 32; x0 += AT_ONCE * 64 / LR) {
+                int row[AT_ONCE];
+                float4 v[AT_ONCE];
+#pragma unroll
+                for (int i = 0; i < AT_ONCE; ++i) {
+                    const int x = x0 + i * 64 / LR;
+                    row[i] = __shfl((int)qrow, x);   // (fewer than 2^24 rows)
+                    v[i] = *(const float4 *)(mine + x * RS + lane % LR * 16);
+                }
+#pragma unroll
+                for (int i = 0; i < AT_ONCE; ++i)
+                    if (first + x0 + i * 64 / LR < rows) put(row[i], ch, v[i], f);
+            }
             asm volatile("" ::: "memory");
         }
     };
-    const int first = j0 + 32 * rg;
     if (c.nparts > 1) {
         if (WT != 2) lds_barrier();   // (all waves have left the tiles)
         if (th == 1) return;
         if (h == 0 && j < rows) *(float2 *)(c.ml + ((qrow * c.nparts + part) * MAPS + map) * 2) = make_float2(m_run, l);
-        rows_out(lds + (WT == 2 ? (map * groups + rg) * (D / 8 * 64 + 64) * 16 : wave * 32 * RS), [&](int x, int ch, float4 v) __attribute__((always_inline)) {
-            const int64_t at = ((int64_t)__shfl((int)qrow, x) * c.nparts + part) * MAPS + map;
-            if (first + x < rows) *(float4 *)(c.sums + at * D + ch) = v;
-        });
+        rows_out(lds + (WT == 2 ? (map * groups + rg) * (D / 8 * 64 + 64) * 16 : wave * 32 * RS), 1.f, [](int) { return make_float4(1.f, 1.f, 1.f, 1.f); },
+                 [&](int row, int ch, float4 v, float4) __attribute__((always_inline)) {
+                     *(float4 *)(c.sums + (((int64_t)row * c.nparts + part) * MAPS + map) * D + ch) = v;
+                 });
         return;
     }
     float by = l > 0.f || l != l ? 1.f / l : 0.f;
     if (MAPS == 2 && map == 1) by *= -span_lam(a, hkv * G + rem % G);
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) O[dt][r] *= by;
     float4 *other = (float4 *)lds + rg * (D / 8 * 64 + 64) + lane;   // (room for rows_out, too)
     bool norm = false;
     lds_barrier();
@@ -680,18 +690,21 @@ template <int BITS, typename T, int D, int MAPS, int WT> __device__ __forceinlin
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) other[(4 * dt + r) * 64] = make_float4(O[dt][4 * r], O[dt][4 * r + 1], O[dt][4 * r + 2], O[dt][4 * r + 3]);
+                for (int r = 0; r < 4; ++r) other[(4 * dt + r) * 64] = make_float4(O[dt][4 * r] * by, O[dt][4 * r + 1] * by, O[dt][4 * r + 2] * by, O[dt][4 * r + 3] * by);
         }
         lds_barrier();
         if (map == 1 || th == 1) return;
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
+        for (int dt = 0; dt < DT; ++dt) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const float4 x = other[(4 * dt + r) * 64];
-                O[dt][4 * r] += x.x; O[dt][4 * r + 1] += x.y; O[dt][4 * r + 2] += x.z; O[dt][4 * r + 3] += x.w;
+                O[dt][4 * r] = __builtin_fmaf(O[dt][4 * r], by, x.x); O[dt][4 * r + 1] = __builtin_fmaf(O[dt][4 * r + 1], by, x.y);
+                O[dt][4 * r + 2] = __builtin_fmaf(O[dt][4 * r + 2], by, x.z); O[dt][4 * r + 3] = __builtin_fmaf(O[dt][4 * r + 3], by, x.w);
             }
-        float gain = a.gain;
+            __builtin_amdgcn_sched_barrier(0);   // (all of them at once do not fit beside the sums)
+        }
+        by = a.gain;
         norm = a.norm_weight != nullptr;
         if (norm) {
             float sq = 0.f;
@@ -699,31 +712,22 @@ template <int BITS, typename T, int D, int MAPS, int WT> __device__ __forceinlin
             for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) sq = __builtin_fmaf(O[dt][r], O[dt][r], sq);
-            gain /= sqrtf((sq + __shfl_xor(sq, 32)) * (1.f / D) + a.norm_eps);
+            by /= sqrtf((sq + __shfl_xor(sq, 32)) * (1.f / D) + a.norm_eps);
         }
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) O[dt][r] *= gain;
     }
     if (th == 1) return;
-    const bool out_bf16 = a.dtype == VQ_BF16;
-    float4 weight[D / CB];
-#pragma unroll
-    for (int i = 0; i < D / CB; ++i) {
-        const int ch = i * CB + lane % LR * 4;
-        weight[i] = norm ? make_float4(span_ld(a.norm_weight, a.norm_dtype, ch), span_ld(a.norm_weight, a.norm_dtype, ch + 1), span_ld(a.norm_weight, a.norm_dtype, ch + 2),
-                                       span_ld(a.norm_weight, a.norm_dtype, ch + 3))
-                         : make_float4(1.f, 1.f, 1.f, 1.f);
-    }
-    rows_out(MAPS == 2 ? (char *)(other - lane) : lds + rg * 32 * RS, [&](int x, int ch, float4 v) __attribute__((always_inline)) {
-        const int64_t row = __shfl((int)qrow, x);
-        const float4 w = weight[D > CB ? ch / CB : 0];
-        v = make_float4(v.x * w.x, v.y * w.y, v.z * w.z, v.w * w.w);
-        if (first + x < rows)
-            *(uint2 *)((u16 *)a.out + row * D + ch) = out_bf16 ? make_uint2(SpanMma<bf16_t>::pack(v.x, v.y), SpanMma<bf16_t>::pack(v.z, v.w))
-                                                               : make_uint2(SpanMma<f16>::pack(v.x, v.y), SpanMma<f16>::pack(v.z, v.w));
-    });
+    const bool out_bf16 = BITS == 0 ? std::is_same_v<T, bf16_t> : a.dtype == VQ_BF16;
+    rows_out(MAPS == 2 ? (char *)(other - lane) : lds + rg * 32 * RS, by,
+             [&](int ch) __attribute__((always_inline)) {
+                 if (!norm) return make_float4(1.f, 1.f, 1.f, 1.f);
+                 return make_float4(span_ld(a.norm_weight, a.norm_dtype, ch), span_ld(a.norm_weight, a.norm_dtype, ch + 1),
+                                    span_ld(a.norm_weight, a.norm_dtype, ch + 2), span_ld(a.norm_weight, a.norm_dtype, ch + 3));
+             },
+             [&](int row, int ch, float4 v, float4 w) __attribute__((always_inline)) {
+                 v = make_float4(v.x * w.x, v.y * w.y, v.z * w.z, v.w * w.w);
+                 *(uint2 *)((u16 *)a.out + (int64_t)row * D + ch) = out_bf16 ? make_uint2(SpanMma<bf16_t>::pack(v.x, v.y), SpanMma<bf16_t>::pack(v.z, v.w))
+                                                                            : make_uint2(SpanMma<f16>::pack(v.x, v.y), SpanMma<f16>::pack(v.z, v.w));
+             });
 }
 
 template <int BITS, typename T, int D, int MAPS> __device__ __forceinline__ void span_mfma_block(const SpanCall &c, int id) {
