@@ -282,7 +282,8 @@ template <int BITS, typename T, int D, int MAPS, int WT> __device__ __forceinlin
     u32x4 P[X][2];
     // Operands are asked for four products ahead, as written: left to itself the scheduler reads each right before its product and waits.
     constexpr int AHEAD = 4;
-    auto scores = [&](u32 tile) __attribute__((always_inline)) {
+    // (`aside`: copies of a later unit that are asked for in between, keys' beside the products, values' beside the exponentials)
+    auto scores = [&](u32 tile, auto &aside) __attribute__((always_inline)) {
         constexpr int N = X * KS;
         // (the stretches in turn: a product waits 52 cycles for the one it adds to, and takes 32)
         auto key = [&](int i) __attribute__((always_inline)) { return *(L4 *)(uintptr_t)((key0 ^ (32 * (i / X))) + tile + i % X * (32 * D * 2)); };
@@ -297,10 +298,11 @@ template <int BITS, typename T, int D, int MAPS, int WT> __device__ __forceinlin
         for (int i = 0; i < N; ++i) {
             S[i % X] = M::mma(k[i % AHEAD], q[i / X], S[i % X]);
             if (i + AHEAD < N) k[i % AHEAD] = key(i + AHEAD);
+            aside.keys(i);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    auto weights = [&](int place, int live) __attribute__((always_inline)) {
+    auto weights = [&](int place, int live, auto &aside) __attribute__((always_inline)) {
         const int end = place + live;
         if (place + 32 * X > (all_hi < end ? all_hi : end) || place < all_lo) {
             const int hi = (lane_hi < end ? lane_hi : end) - place - 4 * h, lo = lane_lo - place - 4 * h;
@@ -340,6 +342,7 @@ template <int BITS, typename T, int D, int MAPS, int WT> __device__ __forceinlin
                 const u32 p = M::pack(__builtin_amdgcn_exp2f(__builtin_fmaf(S[x][2 * r], cc, nm)), __builtin_amdgcn_exp2f(__builtin_fmaf(S[x][2 * r + 1], cc, nm)));
                 P[x][r / 4][r % 4] = p;
                 l2[r & 1] = M::add_pair(p, l2[r & 1]);
+                if (r & 1) aside.values(4 * x + r / 2);
             }
         l_run += l2[0] + l2[1];
     };
@@ -368,11 +371,19 @@ template <int BITS, typename T, int D, int MAPS, int WT> __device__ __forceinlin
         }
     };
     // (units that none of the wave's rows sees are left out whole: a unit's stretches are not tested one by one)
-    auto compute = [&](auto transposed, u32 tile, int place, int live) __attribute__((always_inline)) {
-        if (!wave_works || place >= any_hi || place + UNIT <= any_lo) return;
-        scores(tile + th * (32 * D * 2));
-        weights(place + 32 * th, live - 32 * th);
+    auto compute = [&](auto transposed, u32 tile, int place, int live, auto &&aside) __attribute__((always_inline)) {
+        if (!wave_works || place >= any_hi || place + UNIT <= any_lo) {
+            aside.all();
+            return;
+        }
+        scores(tile + th * (32 * D * 2), aside);
+        weights(place + 32 * th, live - 32 * th, aside);
         sums(transposed, tile + (transposed.value ? th * 64 : th * (32 * D * 2)));
+    };
+    struct Nothing {
+        __device__ __forceinline__ void keys(int) {}
+        __device__ __forceinline__ void values(int) {}
+        __device__ __forceinline__ void all() {}
     };
 
     // ---- one span after the other.  A store's fields are read from the argument block where a span begins (`fresh` hides the block's
@@ -402,57 +413,81 @@ template <int BITS, typename T, int D, int MAPS, int WT> __device__ __forceinlin
             voff[i] = (u32)t * (u32)vs + sp_vpiece<D>(t, p) * 16;
         }
         const u32 past = lds0 + R * Tile::ROW_BUF;
+        static_assert(X * KS >= N && 4 * X >= N, "as many copies as places to ask for them");
         u32 fill = lds0 + wave * N * 1024;   // where the next unit's copies go
-        int asked_live = live, asked = 0;
-        auto fetch = [&]() __attribute__((always_inline)) {
+        int asked = 0, asked_live = live;    // that unit
+        auto cut_short = [&]() __attribute__((always_inline)) {   // a row past the live ones repeats the last (the pieces' order goes by the tile's row)
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                u32 ko = koff[i], vo = voff[i];
-                if (asked_live < UNIT) {   // a row past the live ones repeats the last (the pieces' order goes by the tile's row)
-                    int slot = (wave * N + i) * 64 + lane;
-                    asm volatile("" : "+v"(slot));   // (not to be worked out ahead, and held, for all units)
-                    const int t = slot / CH, p = slot % CH;
-                    const u32 r = (u32)(t < asked_live ? t : asked_live - 1);
-                    ko = r * (u32)ks + sp_kpiece<D>(t, p) * 16;
-                    vo = r * (u32)vs + sp_vpiece<D>(t, p) * 16;
-                }
-                lds_copy16<0>(kb, ko, fill + i * 1024);
-                lds_copy16<0>(vb, vo, fill + i * 1024 + Tile::KEYS);
+                int slot = (wave * N + i) * 64 + lane;
+                asm volatile("" : "+v"(slot));   // (not to be worked out ahead, and held, for all units)
+                const int t = slot / CH, p = slot % CH;
+                const u32 r = (u32)(t < asked_live ? t : asked_live - 1);
+                koff[i] = r * (u32)ks + sp_kpiece<D>(t, p) * 16;
+                voff[i] = r * (u32)vs + sp_vpiece<D>(t, p) * 16;
             }
-            kb += UNIT * ks;
-            vb += UNIT * vs;
-            ++asked;
-            asked_live -= UNIT;
+        };
+        if (asked_live < UNIT) cut_short();
+        auto next = [&]() __attribute__((always_inline)) {   // (behind the last unit: that one again, which nobody reads)
+            if (asked + 1 < count) {
+                kb += UNIT * ks;
+                vb += UNIT * vs;
+                ++asked;
+                asked_live -= UNIT;
+                if (asked_live < UNIT) cut_short();
+            }
             fill += Tile::ROW_BUF;
             if (fill >= past) fill -= R * Tile::ROW_BUF;
         };
+        struct Copies {
+            const char *kb, *vb;
+            const u32 (&koff)[N], (&voff)[N];
+            u32 to;
+            __device__ __forceinline__ void keys(int i) const { if (i < N) lds_copy16<0>(kb, koff[i < N ? i : 0], to + i * 1024); }
+            __device__ __forceinline__ void values(int i) const { if (i < N) lds_copy16<0>(vb, voff[i < N ? i : 0], to + i * 1024 + Tile::KEYS); }
+            __device__ __forceinline__ void all() const {
+#pragma unroll
+                for (int i = 0; i < N; ++i) { keys(i); values(i); }
+            }
+        };
 #pragma unroll 1
-        for (int i = 0; i < R - 1 && i < count && !convert; ++i) fetch();
+        for (int i = 0; i < R - 1 && !convert; ++i) {
+            Copies{kb, vb, koff, voff, fill}.all();
+            next();
+        }
         u32 tile = lds0;
 #pragma unroll 1
         for (int i = 0; i < count; ++i, place += UNIT, live -= UNIT) {
             // the unit is here once the copies of at most R - 2 later ones are under way; past the barrier every wave has left the tile
             // before it, the next to be filled
-            if (i + R - 1 <= count) wait_copies<(R - 2) * 2 * N>();
-            else wait_copies<0>();
+            wait_copies<(R - 2) * 2 * N>();
             lds_barrier();
-            if (convert) {
+            if constexpr (BITS == 0) {
+                // (asked for at once behind the barrier, the waves' copies hold each other up for 500 cycles)
+                const Copies copies{kb, vb, koff, voff, fill};
+                compute(std::false_type{}, tile, place, live, copies);
+                next();
+            } else {
+                if (convert) {   // (a unit at a time)
 #pragma unroll 1
-                for (int x = tid; x < UNIT * CH; x += SP_THREADS) {
-                    const int t = x / CH, p = x % CH, r = t < live ? t : live - 1;
-                    *(f16x8 *)(lds + t * D * 2 + sp_kpiece<D>(t, p) * 16) = ld_tail8(kb + r * ks, 8 * p, true);
-                    *(f16x8 *)(lds + Tile::KEYS + t * D * 2 + sp_vpiece<D>(t, p) * 16) = ld_tail8(vb + r * vs, 8 * p, true);
+                    for (int x = tid; x < UNIT * CH; x += SP_THREADS) {
+                        const int t = x / CH, p = x % CH, r = t < live ? t : live - 1;
+                        *(f16x8 *)(lds + t * D * 2 + sp_kpiece<D>(t, p) * 16) = ld_tail8(kb + r * ks, 8 * p, true);
+                        *(f16x8 *)(lds + Tile::KEYS + t * D * 2 + sp_vpiece<D>(t, p) * 16) = ld_tail8(vb + r * vs, 8 * p, true);
+                    }
+                    kb += UNIT * ks;
+                    vb += UNIT * vs;
+                    lds_barrier();
+                } else {
+                    Copies{kb, vb, koff, voff, fill}.all();
+                    next();
                 }
-                kb += UNIT * ks;
-                vb += UNIT * vs;
-                lds_barrier();
-            } else if (asked < count) {
-                fetch();
+                compute(std::false_type{}, tile, place, live, Nothing{});
             }
-            compute(std::false_type{}, tile, place, live);
             if (!convert) tile += Tile::ROW_BUF;
             if (tile == past) tile = lds0;
         }
+        wait_copies<0>();
         lds_barrier();   // the tiles are free
     };
     // `count` units of packed slots from slot t0 on
@@ -578,7 +613,7 @@ template <int BITS, typename T, int D, int MAPS, int WT> __device__ __forceinlin
             make(live);
             lds_barrier();
             if (i + RAWS < count) fetch();   // into the slot that unit i has left
-            compute(std::true_type{}, lds0, place, live);
+            compute(std::true_type{}, lds0, place, live, Nothing{});
         }
         lds_barrier();
     };
