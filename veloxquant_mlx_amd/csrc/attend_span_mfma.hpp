@@ -670,12 +670,37 @@ template <int BITS, typename T, int D, int MAPS, int WT> __device__ __forceinlin
                 }
         }
     }
-    // The wave's rows go out through its own room in LDS, where a row is contiguous: lanes n held a row each, of which a store would write
-    // eight or sixteen bytes (so written, the end of a block took 7000 cycles at 128 channels and 25000 at 256, now XX and XX).
-    constexpr int CB = D < 128 ? D : 128, LR = CB / 4, RS = CB * 4 + 16;   // channels at a time, lanes a row, bytes of a row
+    // The wave's rows go out through its own room in LDS, where a row of W channels is contiguous: lanes n hold a row each, of which a store
+    // would write eight or sixteen bytes (so written, three prompts of 1001 with heads of 256 channels took 95 us, so 50).
     const int first = j0 + 32 * rg;
-    auto rows_out = [&](char *mine, float times, auto begin, auto put) __attribute__((always_inline)) {
-        constexpr int AT_ONCE = D == 256 ? 4 : 8;
+    auto place_of = [&](auto width, char *mine, int dt, int r) __attribute__((always_inline)) {   // the lane's channels 32 dt + 2 r + 4 h .. + 3
+        return (float4 *)(mine + n * (width.value * 4 + 16) + (32 * dt + 2 * r + 4 * h) * 4);
+    };
+    // put(row, its factor, channel, four values) for every row and channel c0 .. c0 + W - 1
+    auto rows_out = [&](auto width, const char *mine, int c0, float factor, auto put) __attribute__((always_inline)) {
+        constexpr int LANES = width.value / 4, AT_ONCE = 4;   // of a row
+        asm volatile("" ::: "memory");   // (a wave's LDS accesses are in order; these are other lanes')
+#pragma unroll 1
+        for (int x0 = lane / LANES; x0 < 32; x0 += AT_ONCE * 64 / LANES) {
+            int row[AT_ONCE];
+            float f[AT_ONCE];
+            float4 v[AT_ONCE];
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i) {
+                const int x = x0 + i * 64 / LANES;
+                row[i] = __shfl((int)qrow, x);   // (fewer than 2^24 rows)
+                f[i] = __shfl(factor, x);
+                v[i] = *(const float4 *)(mine + x * (width.value * 4 + 16) + lane % LANES * 16);
+            }
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i)
+                if (first + x0 + i * 64 / LANES < rows) put(row[i], f[i], c0 + lane % LANES * 4, v[i]);
+        }
+        asm volatile("" ::: "memory");
+    };
+    constexpr int CB = D < 128 ? D : 128;   // channels at a time, of waves that all have rows to write
+    using Block = std::integral_constant<int, CB>;
+    auto blocks_out = [&](char *mine, float factor, auto put) __attribute__((always_inline)) {
 #pragma unroll
         for (int c0 = 0; c0 < D; c0 += CB) {
 #pragma unroll
@@ -683,86 +708,70 @@ template <int BITS, typename T, int D, int MAPS, int WT> __device__ __forceinlin
 #pragma unroll
                 for (int r = 0; r < 16; r += 4) {
                     const f32x16 &o = O[c0 / 32 + dt];
-                    *(float4 *)(mine + n * RS + (32 * dt + 2 * r + 4 * h) * 4) = make_float4(o[r] * times, o[r + 1] * times, o[r + 2] * times, o[r + 3] * times);
+                    *place_of(Block{}, mine, dt, r) = make_float4(o[r], o[r + 1], o[r + 2], o[r + 3]);
                 }
-            asm volatile("" ::: "memory");   // (a wave's LDS accesses are in order; these are other lanes')
-            const int ch = c0 + lane % LR * 4;
-            const float4 f = begin(ch);
-#pragma unroll 1
-            for (int x0 = lane / LR; x0 < 32; x0 += AT_ONCE * 64 / LR) {
-                int row[AT_ONCE];
-                float4 v[AT_ONCE];
-#pragma unroll
-                for (int i = 0; i < AT_ONCE; ++i) {
-                    const int x = x0 + i * 64 / LR;
-                    row[i] = __shfl((int)qrow, x);   // (fewer than 2^24 rows)
-                    v[i] = *(const float4 *)(mine + x * RS + lane % LR * 16);
-                }
-#pragma unroll
-                for (int i = 0; i < AT_ONCE; ++i)
-                    if (first + x0 + i * 64 / LR < rows) put(row[i], ch, v[i], f);
-            }
-            asm volatile("" ::: "memory");
+            rows_out(Block{}, mine, c0, factor, put);
         }
     };
+    const bool out_bf16 = BITS == 0 ? std::is_same_v<T, bf16_t> : a.dtype == VQ_BF16;
+    auto store = [&](int row, int ch, float4 v) __attribute__((always_inline)) {
+        *(uint2 *)((u16 *)a.out + (int64_t)row * D + ch) = out_bf16 ? make_uint2(SpanMma<bf16_t>::pack(v.x, v.y), SpanMma<bf16_t>::pack(v.z, v.w))
+                                                                   : make_uint2(SpanMma<f16>::pack(v.x, v.y), SpanMma<f16>::pack(v.z, v.w));
+    };
+    if (WT != 2) lds_barrier();   // (all waves have left the tiles)
     if (c.nparts > 1) {
-        if (WT != 2) lds_barrier();   // (all waves have left the tiles)
         if (th == 1) return;
         if (h == 0 && j < rows) *(float2 *)(c.ml + ((qrow * c.nparts + part) * MAPS + map) * 2) = make_float2(m_run, l);
-        rows_out(lds + (WT == 2 ? (map * groups + rg) * (D / 8 * 64 + 64) * 16 : wave * 32 * RS), 1.f, [](int) { return make_float4(1.f, 1.f, 1.f, 1.f); },
-                 [&](int row, int ch, float4 v, float4) __attribute__((always_inline)) {
-                     *(float4 *)(c.sums + (((int64_t)row * c.nparts + part) * MAPS + map) * D + ch) = v;
-                 });
+        blocks_out(lds + (WT == 2 ? (map * groups + rg) * (D / 8 * 64 + 64) * 16 : wave * 32 * (CB * 4 + 16)), 1.f,
+                   [&](int row, float, int ch, float4 v) __attribute__((always_inline)) {
+                       *(float4 *)(c.sums + (((int64_t)row * c.nparts + part) * MAPS + map) * D + ch) = v;
+                   });
         return;
     }
     float by = l > 0.f || l != l ? 1.f / l : 0.f;
-    if (MAPS == 2 && map == 1) by *= -span_lam(a, hkv * G + rem % G);
-    float4 *other = (float4 *)lds + rg * (D / 8 * 64 + 64) + lane;   // (room for rows_out, too)
-    bool norm = false;
-    lds_barrier();
-    if (MAPS == 2) {
+    if constexpr (MAPS == 1) {
+        if (WT == 2) lds_barrier();   // (another wave's room)
+        if (th == 1) return;
+        blocks_out(lds + rg * 32 * (CB * 4 + 16), by, [&](int row, float f, int ch, float4 v) __attribute__((always_inline)) {
+            store(row, ch, make_float4(v.x * f, v.y * f, v.z * f, v.w * f));
+        });
+    } else {
+        // the second map's rows, then the difference in their place
+        using Row = std::integral_constant<int, D>;
+        char *room = lds + rg * (D / 8 * 64 + 64) * 16;
+        if (WT == 2) lds_barrier();
         if (map == 1 && th == 0) {
+            by *= -span_lam(a, hkv * G + rem % G);
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) other[(4 * dt + r) * 64] = make_float4(O[dt][4 * r] * by, O[dt][4 * r + 1] * by, O[dt][4 * r + 2] * by, O[dt][4 * r + 3] * by);
+                for (int r = 0; r < 16; r += 4) *place_of(Row{}, room, dt, r) = make_float4(O[dt][r] * by, O[dt][r + 1] * by, O[dt][r + 2] * by, O[dt][r + 3] * by);
         }
         lds_barrier();
         if (map == 1 || th == 1) return;
+        float sq = 0.f;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const float4 x = other[(4 * dt + r) * 64];
-                O[dt][4 * r] = __builtin_fmaf(O[dt][4 * r], by, x.x); O[dt][4 * r + 1] = __builtin_fmaf(O[dt][4 * r + 1], by, x.y);
-                O[dt][4 * r + 2] = __builtin_fmaf(O[dt][4 * r + 2], by, x.z); O[dt][4 * r + 3] = __builtin_fmaf(O[dt][4 * r + 3], by, x.w);
+            for (int r = 0; r < 16; r += 4) {
+                float4 *at = place_of(Row{}, room, dt, r), x = *at;
+                x = make_float4(__builtin_fmaf(O[dt][r], by, x.x), __builtin_fmaf(O[dt][r + 1], by, x.y), __builtin_fmaf(O[dt][r + 2], by, x.z), __builtin_fmaf(O[dt][r + 3], by, x.w));
+                sq = __builtin_fmaf(x.x, x.x, sq); sq = __builtin_fmaf(x.y, x.y, sq); sq = __builtin_fmaf(x.z, x.z, sq); sq = __builtin_fmaf(x.w, x.w, sq);
+                *at = x;
             }
-            __builtin_amdgcn_sched_barrier(0);   // (all of them at once do not fit beside the sums)
         }
-        by = a.gain;
-        norm = a.norm_weight != nullptr;
-        if (norm) {
-            float sq = 0.f;
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) sq = __builtin_fmaf(O[dt][r], O[dt][r], sq);
-            by /= sqrtf((sq + __shfl_xor(sq, 32)) * (1.f / D) + a.norm_eps);
+        float gain = a.gain;
+        float4 weight = make_float4(1.f, 1.f, 1.f, 1.f);   // of the lane's channels
+        if (a.norm_weight != nullptr) {
+            gain /= sqrtf((sq + __shfl_xor(sq, 32)) * (1.f / D) + a.norm_eps);
+            const int ch = lane % (D / 4) * 4;
+            weight = make_float4(span_ld(a.norm_weight, a.norm_dtype, ch), span_ld(a.norm_weight, a.norm_dtype, ch + 1),
+                                 span_ld(a.norm_weight, a.norm_dtype, ch + 2), span_ld(a.norm_weight, a.norm_dtype, ch + 3));
         }
+        rows_out(Row{}, room, 0, gain, [&](int row, float f, int ch, float4 v) __attribute__((always_inline)) {
+            store(row, ch, make_float4(v.x * f * weight.x, v.y * f * weight.y, v.z * f * weight.z, v.w * f * weight.w));
+        });
     }
-    if (th == 1) return;
-    const bool out_bf16 = BITS == 0 ? std::is_same_v<T, bf16_t> : a.dtype == VQ_BF16;
-    rows_out(MAPS == 2 ? (char *)(other - lane) : lds + rg * 32 * RS, by,
-             [&](int ch) __attribute__((always_inline)) {
-                 if (!norm) return make_float4(1.f, 1.f, 1.f, 1.f);
-                 return make_float4(span_ld(a.norm_weight, a.norm_dtype, ch), span_ld(a.norm_weight, a.norm_dtype, ch + 1),
-                                    span_ld(a.norm_weight, a.norm_dtype, ch + 2), span_ld(a.norm_weight, a.norm_dtype, ch + 3));
-             },
-             [&](int row, int ch, float4 v, float4 w) __attribute__((always_inline)) {
-                 v = make_float4(v.x * w.x, v.y * w.y, v.z * w.z, v.w * w.w);
-                 *(uint2 *)((u16 *)a.out + (int64_t)row * D + ch) = out_bf16 ? make_uint2(SpanMma<bf16_t>::pack(v.x, v.y), SpanMma<bf16_t>::pack(v.z, v.w))
-                                                                            : make_uint2(SpanMma<f16>::pack(v.x, v.y), SpanMma<f16>::pack(v.z, v.w));
-             });
 }
 
 template <int BITS, typename T, int D, int MAPS> __device__ __forceinline__ void span_mfma_block(const SpanCall &c, int id) {
