@@ -56,10 +56,13 @@ def _need_gpu(name: str, *tensors: torch.Tensor) -> None:
                                "there is no CPU path")
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)   # (a tensor of the device is there: it is set up)
+
+
 def _launch_on(device: torch.device, call) -> None:
     """Run a library call with ``device`` as the current one (a launch goes to the current device, whose default stream has
     the same handle on every device) and raise what it returns."""
-    if device.index is None or device.index == torch.cuda.current_device():
+    if device.index is None or device.index == _current_device():
         rc = call()
     else:
         with torch.cuda.device(device):
@@ -1460,6 +1463,10 @@ __all__ = [
 _NO_STORE = (0,) * 17
 
 
+_META_DTYPES = frozenset((torch.float16, torch.float32))
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
+
+
 def _store_fields(name, which, device, batch, k_packed=None, k_scale=None, k_zero=None, v_packed=None, v_scale=None, v_zero=None,
                   n_packed=0, bits=4, group_size=32, v_layout="channel", k_tail=None, v_tail=None, n_tail=0):
     """A store's fields of the argument block; ``(fields, Hkv, D, packed, tail dtype, keep)`` with ``packed`` = (bits, group,
@@ -1473,7 +1480,7 @@ def _store_fields(name, which, device, batch, k_packed=None, k_scale=None, k_zer
     if n_packed:
         arrays = (k_packed, k_scale, k_zero, v_packed, v_scale, v_zero)
         for t in arrays:
-            if t is None or not t.is_contiguous() or t.ndim != 4:
+            if t is None or t.ndim != 4 or not t.is_contiguous():
                 raise ValueError(f"{name}: packed tensors ({which}) must be given, 4D and contiguous")
             if t.device != device:
                 raise ValueError(f"{name}: packed tensors ({which}) must live on {device}, got {t.device}")
@@ -1481,43 +1488,48 @@ def _store_fields(name, which, device, batch, k_packed=None, k_scale=None, k_zer
         if not 1 <= bits <= 8 or g < 1 or v_layout not in _V_LAYOUT:
             raise ValueError(f"{name}: bits={bits}, group_size={g}, v_layout={v_layout!r} ({which})")
         meta = k_scale.dtype
-        if meta not in (torch.float16, torch.float32) or any(t.dtype != meta for t in (k_zero, v_scale, v_zero)):
+        if meta not in _META_DTYPES or k_zero.dtype != meta or v_scale.dtype != meta or v_zero.dtype != meta:
             raise ValueError(f"{name}: scale/zero ({which}) must share one dtype, float16 or float32")
-        if k_packed.element_size() != 4 or v_packed.element_size() != 4:
+        if k_packed.itemsize != 4 or v_packed.itemsize != 4:
             raise ValueError(f"{name}: packed codes ({which}) must be 32-bit words")
         per = 32 // bits
         B, heads, cap, W = k_packed.shape
-        channels = k_scale.shape[3]
+        k_meta, v_meta = k_scale.shape, v_scale.shape
+        channels = k_meta[3]
         GV = -(-channels // g)
-        k_meta = (B, heads, -(-cap // g), channels)
         if v_layout == "token":
             want = ((B, heads, cap // per, channels), (B, heads, GV, cap))
         else:
             want = ((B, heads, cap, W), (B, heads, cap, GV))
         if (B != batch or W != -(-channels // per) or cap < n_packed or (v_layout == "token" and cap % per)
-                or k_scale.shape != k_meta or k_zero.shape != k_meta or v_packed.shape != want[0]
-                or v_scale.shape != want[1] or v_zero.shape != want[1]):
+                or k_meta != (B, heads, -(-cap // g), channels) or k_zero.shape != k_meta or v_packed.shape != want[0]
+                or v_meta != want[1] or v_zero.shape != v_meta):
             raise ValueError(f"{name}: packed tensors ({which}) {[tuple(t.shape) for t in arrays]} do not fit a batch of {batch}, {n_packed} tokens, "
                              f"{bits} bits, groups of {g}, values packed by {v_layout}")
         packed = (bits, g, VQ_F16 if meta == torch.float16 else VQ_F32, _V_LAYOUT[v_layout])
-        fields = [*(t.data_ptr() for t in arrays), n_packed, cap]
+        fields = [k_packed.data_ptr(), k_scale.data_ptr(), k_zero.data_ptr(), v_packed.data_ptr(), v_scale.data_ptr(), v_zero.data_ptr(),
+                  n_packed, cap]
     if n_tail:
         if k_tail is None or v_tail is None:
             raise ValueError(f"{name}: n_tail > 0 needs k_tail and v_tail ({which})")
-        if k_tail.ndim != 4 or k_tail.shape != v_tail.shape or k_tail.dtype != v_tail.dtype or k_tail.dtype not in _FLOAT_TAG:
+        shape, dtype = k_tail.shape, k_tail.dtype
+        if len(shape) != 4 or shape != v_tail.shape or dtype != v_tail.dtype or dtype not in _FLOAT_TAG:
             raise ValueError(f"{name}: k_tail and v_tail ({which}) must be alike, [B, H, n, D] float16, bfloat16 or float32, got "
-                             f"{tuple(k_tail.shape)} {k_tail.dtype} and {tuple(v_tail.shape)} {v_tail.dtype}")
+                             f"{tuple(shape)} {dtype} and {tuple(v_tail.shape)} {v_tail.dtype}")
         if k_tail.device != device or v_tail.device != device:
             raise ValueError(f"{name}: k_tail and v_tail ({which}) must live on {device}, got {k_tail.device} and {v_tail.device}")
-        B, H, room, D = k_tail.shape
+        B, H, room, D = shape
         if B != batch or room < n_tail or (heads is not None and (H != heads or D != channels)):
-            raise ValueError(f"{name}: tail ({which}) {tuple(k_tail.shape)} does not fit a batch of {batch}, {n_tail} tokens"
+            raise ValueError(f"{name}: tail ({which}) {tuple(shape)} does not fit a batch of {batch}, {n_tail} tokens"
                              + ("" if heads is None else f", {heads} heads of {channels} channels"))
-        heads, channels, tail = H, D, k_tail.dtype
-        if D > 1 and (k_tail.stride(3) != 1 or v_tail.stride(3) != 1):
+        heads, channels, tail = H, D, dtype
+        kb, kh, kr, k1 = k_tail.stride()
+        vb, vh, vr, v1 = v_tail.stride()
+        if D > 1 and (k1 != 1 or v1 != 1):
             k_tail, v_tail = k_tail[:, :, :n_tail].contiguous(), v_tail[:, :, :n_tail].contiguous()
             keep = [k_tail, v_tail]
-        fields += [k_tail.data_ptr(), v_tail.data_ptr(), n_tail, *k_tail.stride()[:3], *v_tail.stride()[:3]]
+            (kb, kh, kr, _), (vb, vh, vr, _) = k_tail.stride(), v_tail.stride()
+        fields += [k_tail.data_ptr(), v_tail.data_ptr(), n_tail, kb, kh, kr, vb, vh, vr]
     else:
         fields += [0] * 9
     return fields, heads, channels, packed, tail, keep
@@ -1533,7 +1545,7 @@ def _store_attend(name, maps, q, prefix, own, scale, causal, seq_lens, sliding_w
     tag = _ftag(name, q)
     B, Hq, Sq, D = q.shape
     if out is None:
-        out = torch.empty(q.shape, dtype=dtype, device=device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != q.shape or out.dtype != dtype or out.device != device or not out.is_contiguous():
         raise ValueError(f"{name}: out must be a contiguous {tuple(q.shape)} tensor in {dtype} on {device}")
     own_f, heads, channels, packed, tail, keep = _store_fields(name, "own", device, B, **own)
@@ -1582,7 +1594,7 @@ def _store_attend(name, maps, q, prefix, own, scale, causal, seq_lens, sliding_w
             tag if tail is None else _FLOAT_TAG[tail], weight_tag, bits, group, meta, layout, 1 if causal else 0, scale, norm_eps, gain)
 
     def launch():
-        if torch.cuda.is_current_stream_capturing():
+        if _capturing():
             # a graph's scratch is its own: two graphs captured on one stream may run at once, and the scratch kept for the
             # stream is given back when a larger one replaces it
             need = room(block(None))
@@ -1712,7 +1724,7 @@ def rotary_embed(q: torch.Tensor, k: torch.Tensor | None = None, *, inv_freq: to
         if t.stride(3) != 1 and D > 1:
             t = t.contiguous()
         if o is None:
-            o = torch.empty(t.shape, dtype=dtype, device=device)
+            o = torch.empty_like(t, memory_format=torch.contiguous_format)
         elif o.shape != t.shape or o.dtype != dtype or o.device != device or (D > 1 and o.stride(3) != 1):
             raise ValueError(f"{name}: the output for {what} must be {tuple(t.shape)} in {dtype} on {device} with adjacent channels")
         elif any(n > 1 and st == 0 for n, st in zip(o.shape, o.stride())):
