@@ -42,12 +42,13 @@ void span_mfma_plan(SpanCall &c, int maps) {
     c.ofew = packed && r1 <= few;
     // One round of blocks of equal runs, two blocks a CU (one of few rows of 256 channels, or of tiles beside few rows), each side for itself
     // where they differ; own slots of sequences that differ in length even out over four rounds.  A run is four units a wave or more for few
-    // rows, eight units a block else: a block costs about as much to start and end.
+    // rows, six units a block else, which a block costs to start and end (12 sequences of five rows on 4k plain slots: 25.8 us with four, 23.9
+    // with six, 25.2 with eight).
     auto side = [&](bool by_few, int64_t rows, int64_t slots32, int64_t slots64, int64_t times, int &wt, int &tiles, int64_t &units, int64_t &least) {
         wt = !by_few && a.D != 256 && rows <= most / 2 ? 2 : 1;
         tiles = by_few ? 1 : (int)cdiv(rows, most / wt);
         units = by_few || a.D == 256 ? slots32 : slots64;
-        least = by_few ? 16 : a.D == 256 ? 16 : 8;
+        least = by_few ? 16 : a.D == 256 ? 12 : 6;
         return times * a.Hkv * tiles * units;   // units of all blocks
     };
     const int64_t p32 = units_of(a.prefix, 32), p64 = units_of(a.prefix, 64), o32 = units_of(a.own, 32), o64 = units_of(a.own, 64);

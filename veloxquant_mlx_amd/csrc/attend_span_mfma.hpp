@@ -1,18 +1,20 @@
 // Attention over spans of slots on the matrix units (gfx950, wave64): one kernel for the shared prefix, for a sequence's own slots
 // and for both maps of differential attention.
 //
-// A block of four waves walks units of 64 slots (32 with heads of 256 channels) of one kv head, two blocks a CU (one).  A unit's keys and
+// A block of four waves walks units of 64 slots (32 with heads of 256 channels) of one kv head, two blocks a CU.  A unit's keys and
 // values are staged in LDS once for the block.  Plain rows are copied there asynchronously, a unit or more ahead.  Packed slots come as
 // words, scales and zeros into a ring of such units, copied ahead, and are reconstructed to fp16 between the products (one packed fused
 // multiply-add for two codes: exactly fp16(code * scale + zero)).  A wave holds 32 query rows of one map.  The rows of a block are those of
 // all sequences that share the kv head (prefix), or of one sequence (own slots); where they fill half of the waves or less, two waves
 // share rows, each with its half of every unit, and add up in LDS at the end.
 //
-// Bound by what a SIMD has to do one after the other for a unit of 32 rows: 32 products of 32 cycles at 128 channels, ~200 vector
-// instructions of the softmax, ~120 of reconstruction.  Two blocks a CU, which no barrier ties together, overlap one's vector work, copies
-// and start with the other's products.  (Eight waves in one block took longer: in step at every barrier, a unit of 64 slots of two maps
-// took 3700 cycles, and with half of the waves a phase behind the other half 2700, where the products alone take 1540; and every block
-// starts and ends alone on its CU, 10 us.)
+// Bound by what a SIMD's two waves do one after the other.  For a unit of 64 slots and 32 rows, two maps of 128 channels, a wave spends 770
+// cycles in 24 products and ~950 in the softmax (32 exponentials of 16 cycles, ~130 other instructions); measured: 2550 cycles a unit while
+// the other wave takes 3100, 1.87 GHz, 227 us for 32 heads over 4096 tokens (910 TFLOP/s of products).  Two blocks a CU, which no barrier
+// ties together, overlap one's vector work, copies, start (5000 cycles, integer divisions) and end with the other's products.  What was
+// slower: eight waves in one block, 3700 cycles a unit in step at every barrier, 2700 with half of the waves a phase behind the other half, as
+// every block then starts and ends alone on its CU; 64 rows a wave, which halves the LDS reads, 268 us to 261; a causal order
+// that pairs long tiles with short ones on a CU, 99 us to 96 for heads of 256 channels.
 //
 // v_mfma_f32_32x32x16 with n = lane % 32, h = lane / 32: A[i = n][k = 8 h + j], B[k = 8 h + j][n], j = 0..7, and
 // D[i = 8 (r / 4) + 4 h + r % 4][n] in register r = 0..15.  Scores are formed transposed, S^T = K Q^T: a lane then holds sixteen slots of
