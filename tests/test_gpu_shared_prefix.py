@@ -126,6 +126,65 @@ def test_far_scores_and_equal_ones():
     close(got, *attend(q * 0, kk, vv, mask, 1.0, 2.0 ** -11))
 
 
+@pytest.mark.parametrize("packed,dtype,G", [(True, F16, 1), (True, F16, 40), (False, F16, 1), (False, F16, 40), (False, BF16, 1)])
+def test_many_small_weights_count(packed, dtype, G):
+    """One slot takes the maximum, 2^13 others weigh 2^-25.3 of it each, and are what the result is made of.  A weight of fp16 is off by at
+    most half a step, 2^-11 of itself or 2^-32 of the largest.  (Enough sequences and heads that a row's slots are not cut into runs, of
+    which each would have a maximum of its own.)"""
+    require_gpu()
+    B, H, D, n = 64, 8, 64, 1 << 13
+    k, v = torch.zeros((B, H, n, D), dtype=dtype, device="cuda"), torch.ones((B, H, n, D), dtype=dtype, device="cuda")
+    k[:, :, 70, 0], v[:, :, 70] = 1.0, 0.0
+    scale = 25.3 * math.log(2.0) / 8
+    q = torch.zeros((B, H * G, 1, D), dtype=dtype, device="cuda")
+    q[..., 0] = 8.0
+    peak = 1.0
+    if packed:
+        kq, vq = K.kivi_quant_pack(k, -2, 32, 4, meta_dtype=F16), K.kivi_quant_pack(v, -1, 32, 4, meta_dtype=F16, v_layout="token")
+        own = dict(k_packed=kq[0], k_scale=kq[1], k_zero=kq[2], v_packed=vq[0], v_scale=vq[1], v_zero=vq[2], n_packed=n, bits=4, group_size=32, v_layout="token")
+        peak = float((15 * kq[1][0, 0, 70 // 32, 0].double()).half())
+    else:
+        own = dict(k_tail=k, v_tail=v, n_tail=n)
+    got = K.shared_prefix_attend(q, dict(n_tail=0), **own, scale=scale)
+    small = math.exp(-8.0 * peak * scale)
+    want = (n - 1) * small / (1 + (n - 1) * small)
+    u = torch.finfo(dtype).eps / 2
+    far = want * (2 * u + 16 * 2.0 ** -18) + (0 if dtype == BF16 else n * 2.0 ** -32) + u * want + torch.finfo(dtype).smallest_normal * u
+    assert float((got.double() - want).abs().max()) <= far
+
+
+@pytest.mark.parametrize("Sq", [1, 40])
+@pytest.mark.parametrize("packed", [True, False])
+def test_offsets_past_32_bits(packed, Sq):
+    """The second kv head's slots lie more than 4 GiB behind the first's; a window over the last ones, behind which little is read."""
+    require_gpu()
+    Hq, Hkv, D, window, last = 4, 2, 128, 300, 1024
+    p, k, v = store(1, Hkv, *((last, 0) if packed else (0, last)), D, bits=4, group=64, seed=5)
+    room = 70_000_000 // 64 * 64 if packed else 17_000_000
+    if packed:
+        for name, axis, per in (("k_packed", 2, 1), ("k_scale", 2, 64), ("k_zero", 2, 64), ("v_packed", 2, 8), ("v_scale", 3, 1), ("v_zero", 3, 1)):
+            shape = list(p[name].shape)
+            shape[axis] = room // per
+            big = torch.empty(shape, dtype=p[name].dtype, device="cuda")
+            big.narrow(axis, (room - last) // per, last // per).copy_(p[name])
+            p[name] = big
+        p["n_packed"] = room
+        assert p["k_packed"][:, :1].numel() * 4 > 1 << 32
+    else:
+        for name in ("k_tail", "v_tail"):
+            big = torch.empty((1, Hkv, room, D), dtype=F16, device="cuda")
+            big[:, :, -last:] = p[name]
+            p[name] = big
+        p["n_tail"] = room
+        assert p["k_tail"][:, :1].numel() * 2 > 1 << 32
+    o, ok, ov = store(2, Hkv, 0, 50, D, seed=6)
+    q = torch.randn((2, Hq, Sq, D), generator=torch.Generator(device="cuda").manual_seed(0), device="cuda").half()
+    got = K.shared_prefix_attend(q, p, **{**o, "bits": 4, "group_size": 64}, scale=0.1, causal=True, sliding_window=window)
+    ks, vs = (torch.cat([x.expand(2, -1, -1, -1), y], 2) for x, y in ((k, ok), (v, ov)))
+    want, far = attend(q, ks, vs, seen(2, Sq, last, 50, None, True, window), 0.1, torch.finfo(F16).eps / 2)
+    close(got, want, far)
+
+
 def test_agrees_with_the_cache_held_per_sequence():
     """The same slots, the prefix copied into every sequence, through the framework's own decode attention."""
     require_gpu()

@@ -146,7 +146,7 @@ template <int BITS, int D, int MAPS, int WAVES> __device__ __forceinline__ void 
 #pragma unroll
                 for (int r = 0; r < 16; ++r) O[dt][r] *= alpha;
         }
-        const float nm = m_run == -INFINITY ? 0.f : -m_run;
+        const float nm = m_run == -INFINITY ? 0.f : SP_LIFT - m_run;
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
             const u32 p = M::pack(__builtin_amdgcn_exp2f(__builtin_fmaf(S[2 * r], cc, nm)), __builtin_amdgcn_exp2f(__builtin_fmaf(S[2 * r + 1], cc, nm)));

@@ -41,6 +41,10 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 constexpr int SP_WAVES = 4, SP_THREADS = 64 * SP_WAVES;
 
+// Weights of fp16 are formed as 2^SP_LIFT exp2(s - m), at most 2^15 with m followed within 2^8: fp16 then tells a weight of 2^-32 of the
+// largest from zero (2^-25 without), of which a long context may hold as many as count.  Sums and the weights' sum carry the factor alike.
+constexpr float SP_LIFT = 7.f;
+
 template <typename T> struct SpanMma;
 template <> struct SpanMma<f16> {
     static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
@@ -335,7 +339,7 @@ template <int BITS, typename T, int D, int MAPS, int WT> __device__ __forceinlin
 #pragma unroll
                 for (int r = 0; r < 16; ++r) O[dt][r] *= alpha;
         }
-        const float nm = m_run == -INFINITY ? 0.f : -m_run;
+        const float nm = m_run == -INFINITY ? 0.f : std::is_same_v<T, f16> ? SP_LIFT - m_run : -m_run;
         float l2[2] = {0.f, 0.f};   // (short chains)
 #pragma unroll
         for (int x = 0; x < X; ++x)
