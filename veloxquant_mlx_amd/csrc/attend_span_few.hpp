@@ -90,7 +90,8 @@ template <int BITS, int D, int MAPS, int WAVES> __device__ __forceinline__ void 
     const int own = shared ? 0 : own_live, np1 = own < (int)a.own.n_packed ? own : (int)a.own.n_packed, nt1 = own - np1;
     const int tail0 = (int)a.prefix.n_packed, tail1 = before + (int)a.own.n_packed;
     const int total = units_seen(0, np0) + units_seen(tail0, nt0) + units_seen(before, np1) + units_seen(tail1, nt1);
-    const int w0 = (int)((int64_t)total * split / splits), w1 = (int)((int64_t)total * (split + 1) / splits);
+    const int run = total / splits, longer = total % splits;   // (the first runs a unit longer)
+    const int w0 = split * run + (split < longer ? split : longer), w1 = w0 + run + (split < longer ? 1 : 0);
     if (w0 == w1 && c.nparts > 1) {   // (uniform) nothing: sums are not written
         if (tid < rows * MAPS) {
             int x, y;

@@ -240,7 +240,8 @@ template <int BITS, typename T, int D, int MAPS, int WT> __device__ __forceinlin
     const int own = shared ? 0 : own_live, np1 = own < (int)a.own.n_packed ? own : (int)a.own.n_packed, nt1 = own - np1;
     const int tail0 = (int)a.prefix.n_packed, tail1 = before + (int)a.own.n_packed;   // places of the plain slots
     const int total = units_seen(0, np0) + units_seen(tail0, nt0) + units_seen(before, np1) + units_seen(tail1, nt1);
-    const int w0 = (int)((int64_t)total * split / splits), w1 = (int)((int64_t)total * (split + 1) / splits);
+    const int run = total / splits, longer = total % splits;   // (the first runs a unit longer)
+    const int w0 = split * run + (split < longer ? split : longer), w1 = w0 + run + (split < longer ? 1 : 0);
     if (w0 == w1 && c.nparts > 1) {   // (uniform) nothing: sums are not written
         if (th == 0 && h == 0 && j < rows) *(float2 *)(c.ml + ((qrow * c.nparts + part) * MAPS + map) * 2) = make_float2(-INFINITY, 0.f);
         return;
