@@ -258,7 +258,17 @@ template <int BITS, int D, int MAPS, int WAVES> __device__ __forceinline__ void 
                 // scales and zeros of slots 16 s + 4 h .. + 3 and 16 s + 8 + 4 h .. + 3
                 const uint2 s0 = *(const uint2 *)(vmeta + 32 * s), s1 = *(const uint2 *)(vmeta + 32 * s + 16);
                 const uint2 z0 = *(const uint2 *)(vmeta + F::META / 2 + 32 * s), z1 = *(const uint2 *)(vmeta + F::META / 2 + 32 * s + 16);
-                const uint4 sc = make_uint4(s0.x, s0.y, s1.x, s1.y), ze = make_uint4(z0.x, z0.y, z1.x, z1.y);
+                uint4 sc = make_uint4(s0.x, s0.y, s1.x, s1.y), ze = make_uint4(z0.x, z0.y, z1.x, z1.y);
+                if (live < UNIT) {   // a slot past the live ones may hold anything: its weight is zero, its value has to be finite
+                    u32 m[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int t = 16 * s + 4 * h + 2 * (e & 1) + 8 * (e >> 1);
+                        m[e] = t >= live ? 0u : t + 1 >= live ? 0xFFFFu : ~0u;
+                    }
+                    sc = make_uint4(sc.x & m[0], sc.y & m[1], sc.z & m[2], sc.w & m[3]);
+                    ze = make_uint4(ze.x & m[0], ze.y & m[1], ze.z & m[2], ze.w & m[3]);
+                }
                 u32 lo[DT], hi[DT];   // the words of the sixteen slots (4 bits: of eight each)
                 sp_load_words<DT>(vw_p + ((BITS == 4 ? 2 * s : s) * D + DT * n) * 4, lo);
                 if constexpr (BITS == 4) sp_load_words<DT>(vw_p + ((2 * s + 1) * D + DT * n) * 4, hi);
@@ -269,14 +279,7 @@ template <int BITS, int D, int MAPS, int WAVES> __device__ __forceinline__ void 
                                             : __builtin_amdgcn_perm(0u, lo[dt], h ? 0x0C0C0301u : 0x0C0C0200u);
                     u32 code[4];
                     sp_codes8<BITS>(w, magic, code);
-                    u32x4 v = sp_values8(code, sc, ze);
-                    if (live < UNIT) {   // a slot past the live ones may hold anything: its weight is zero, its value has to be finite
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int t = 16 * s + 4 * h + 2 * (e & 1) + 8 * (e >> 1);
-                            v[e] = t >= live ? 0u : t + 1 >= live ? v[e] & 0xFFFFu : v[e];
-                        }
-                    }
+                    const u32x4 v = sp_values8(code, sc, ze);
                     O[dt] = M::mma(v, P[s], O[dt]);
                 }
             }
