@@ -35,9 +35,13 @@ void span_mfma_plan(SpanCall &c, int maps) {
     const int64_t r1 = a.Hq / a.Hkv * a.Sq, all = a.B * r1;
     const int most = 32 * SP_WAVES / maps, few = 32 / maps;   // rows of a block of the one kernel, of the other
     auto units_of = [](const vq_kv_store &s, int64_t unit) { return cdiv(s.n_packed, unit) + cdiv(s.n_tail, unit); };
-    // the prefix in blocks of its own where a sequence's rows fill half a block or less
+    // The prefix in blocks of its own where a sequence's rows fill half a block or less; not where prefix and own slots are few enough for one
+    // block a row tile and no parts (8 sequences of 33 slots on 700 packed: 11.7 us, and 13.4 apart; 32 of them 12.5 and 22.7; 12 of five rows and
+    // 60 slots on 200 plain: 11.5 and 15.4).
     const bool prefix_slots = a.prefix.n_packed + a.prefix.n_tail > 0;
-    c.apart = prefix_slots && a.B > 1 && r1 <= most / 2;
+    const bool brief = packed ? r1 <= few && a.D != 256 && units_of(a.prefix, 32) + units_of(a.own, 32) <= 40 && a.B * a.Hkv <= 256
+                              : a.D != 256 && units_of(a.prefix, 64) + units_of(a.own, 64) <= 8 && a.B * a.Hkv <= 512;
+    c.apart = prefix_slots && a.B > 1 && r1 <= most / 2 && !brief;
     c.pfew = packed && all <= few;
     c.ofew = packed && r1 <= few;
     // One round of blocks of equal runs, two blocks a CU (one of few rows of 256 channels, or of tiles beside few rows), each side for itself
@@ -73,6 +77,7 @@ void span_mfma_plan(SpanCall &c, int maps) {
         c.owaves = 8;
         c.osplits = 1;
     }
+    if (brief && !packed && !c.apart) c.osplits = 1;
     c.nparts = c.psplits + c.osplits;
 }
 
