@@ -55,6 +55,13 @@ def test_plain_rows(dtype, B, Hq, Hkv, D, n, own, Sq):
     _case(B, Hq, Hkv, D, (0, n), (0, own), Sq, dtype=dtype, view=True)
 
 
+def test_float32_scales_near_zero():
+    """code * scale + zero of float32 scales is formed with one rounding to float32: a difference of near-equal numbers, seen alone through a
+    window of one slot, is the fp16 number nearest to it."""
+    require_gpu()
+    _case(1, 6, 2, 200, (2192, 700), (48, 65), 130, group=16, v_layout="channel", dtype=BF16, meta=F32, window=1, spare=0, view=True, seed=253)
+
+
 @pytest.mark.parametrize("kw", [
     dict(B=40, Hq=8, Hkv=2, D=128, prefix=(1024, 70), own=(256, 33), bits=4), dict(B=40, Hq=8, Hkv=2, D=64, prefix=(640, 3), own=(128, 1), bits=2),
     dict(B=24, Hq=12, Hkv=3, D=128, prefix=(2048, 0), own=(512, 9), bits=4, group=64, lens=[(b * 97) % 522 for b in range(24)]),

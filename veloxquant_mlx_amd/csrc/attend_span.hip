@@ -16,7 +16,7 @@ struct SpanPacked {
     int64_t D, W, GV, GK;
     __device__ __forceinline__ float fp16_of(uint32_t word, int slot, const void *scale, const void *zero, int64_t at) const {
         const float code = (float)((word >> (slot * bits)) & mask);
-        return (float)(f16)__fadd_rn(__fmul_rn(code, span_ld(scale, meta, at)), span_ld(zero, meta, at));
+        return (float)(f16)__builtin_fmaf(code, span_ld(scale, meta, at), span_ld(zero, meta, at));
     }
     __device__ __forceinline__ float key(int64_t bh, int64_t t, int64_t d) const {
         const uint32_t w = ((const uint32_t *)s->k_packed)[(bh * s->cap_tokens + t) * W + d / per];
