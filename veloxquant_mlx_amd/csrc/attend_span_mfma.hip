@@ -44,18 +44,22 @@ void span_mfma_plan(SpanCall &c, int maps) {
     c.apart = prefix_slots && a.B > 1 && r1 <= most / 2 && !brief;
     c.pfew = packed && all <= few;
     c.ofew = packed && r1 <= few;
+    const int64_t p32 = units_of(a.prefix, 32), p64 = units_of(a.prefix, 64), o32 = units_of(a.own, 32), o64 = units_of(a.own, 64);
+    // Two waves share rows where those fill half a block, and over plain rows where blocks of as many rows as fit would leave half of the chip empty
+    // (two maps, 8 heads over 500 tokens: 13.8 us, and 16.4; 8 sequences of five rows and 200 slots on 2000: 16.5 and 18.0).
+    auto blocks_of = [&](int64_t rows, int64_t units, int64_t times) { return times * a.Hkv * cdiv(rows, most) * cdiv(units, 6); };
+    const bool roomy = !packed && (c.apart ? blocks_of(all, p64, 1) + blocks_of(r1, o64, a.B) : blocks_of(r1, p64 + o64, a.B)) <= 256;
     // One round of blocks of equal runs, two blocks a CU (one of few rows of 256 channels, or of tiles beside few rows), each side for itself
     // where they differ; own slots of sequences that differ in length even out over four rounds.  A run is four units a wave or more for few
     // rows, six units a block else, which a block costs to start and end (12 sequences of five rows on 4k plain slots: 25.8 us with four, 23.9
     // with six, 25.2 with eight).
     auto side = [&](bool by_few, int64_t rows, int64_t slots32, int64_t slots64, int64_t times, int &wt, int &tiles, int64_t &units, int64_t &least) {
-        wt = !by_few && a.D != 256 && rows <= most / 2 ? 2 : 1;
-        tiles = by_few ? 1 : (int)cdiv(rows, most / wt);
         units = by_few || a.D == 256 ? slots32 : slots64;
         least = by_few ? 16 : a.D == 256 ? 12 : 6;
+        wt = !by_few && a.D != 256 && (rows <= most / 2 || roomy) ? 2 : 1;
+        tiles = by_few ? 1 : (int)cdiv(rows, most / wt);
         return times * a.Hkv * tiles * units;   // units of all blocks
     };
-    const int64_t p32 = units_of(a.prefix, 32), p64 = units_of(a.prefix, 64), o32 = units_of(a.own, 32), o64 = units_of(a.own, 64);
     int64_t pu = 0, ou = 0, pleast = 1, oleast = 1, pwork = 0;
     if (c.apart) pwork = side(c.pfew, all, p32, p64, 1, c.pwt, c.ptiles, pu, pleast);
     const int64_t owork = side(c.ofew, r1, c.apart ? o32 : p32 + o32, c.apart ? o64 : p64 + o64, a.B, c.owt, c.otiles, ou, oleast);
