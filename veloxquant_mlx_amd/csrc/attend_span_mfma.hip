@@ -74,6 +74,12 @@ void span_mfma_plan(SpanCall &c, int maps) {
     // on 16k -- and two where not, 136 us and 150 for 128 of 80 slots on 32k)
     c.psplits = c.apart ? cut(pu, pwork, pleast, span_both(c) && pwork <= owork ? 256 : round(c.pfew)) : 0;
     c.osplits = cut(ou, owork, oleast, round(c.ofew) * (a.seq_lens != nullptr ? 4 : 1));
+    // Parts are written and read again, at ~4 TB/s, and merged in a launch of ~6 us: rows of tiles stay whole where the units saved, ~1.4 us each, are
+    // worth less (two maps, 16 heads over 1000 tokens: 24.5 us whole, and 40.7 in two parts).
+    if (!c.apart && !c.ofew && c.osplits > 1) {
+        const double traffic = (double)a.B * a.Hq * a.Sq * maps * a.D * 8 * c.osplits / 4e6;
+        if (1.4 * (double)(ou - cdiv(ou, c.osplits)) < 6 + traffic) c.osplits = 1;
+    }
     // Rows of few slots: a block of eight waves walks them without parts where four would leave five units a wave (16 us, and 17 of two
     // parts and their merge).
     c.owaves = 4;
