@@ -102,6 +102,10 @@ def test_a_prompt_shared_by_sequences(kw):
     step(shared, 5, 1)
     assert other.offset == prompt + 4 and shared.offset == prompt + 57
     assert shared.trim(1000) == 57 and shared.offset == prompt
+    step(shared, 5, 40)
+    step(shared, 5, 1)
+    assert shared.trim(39) == 39 and shared.offset == prompt + 2 and shared._own._n_quantized == 0
+    step(shared, 5, 1)
 
 
 def test_one_sequence_is_a_cache():

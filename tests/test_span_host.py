@@ -74,3 +74,23 @@ def test_host_tensors_are_refused():
     for call in (lambda: K.shared_prefix_attend(q, {}, k_tail=q, v_tail=q, n_tail=1), lambda: K.differential_attend(q, 0.5, k_tail=q, v_tail=q, n_tail=1)):
         with pytest.raises(RuntimeError, match="no CPU path"):
             call()
+
+
+def _cache(**kw):
+    from veloxquant_mlx_amd.cache import KVCacheConfig, KVCacheFactory
+    return KVCacheFactory.create(KVCacheConfig(**{**dict(method="kivi", head_dim=128, bit_width_inlier=4, fused_sdpa=True), **kw}))
+
+
+def test_caches_that_cannot_be_shared():
+    for kw, what in ((dict(fused_sdpa_memory_bound=True), "batch of one"), (dict(), "memory_bound"), (dict(fused_sdpa=False), "memory_bound"),
+                     (dict(method="kivi_sink", fused_sdpa_memory_bound=True), "must be a KIVIKVCache")):
+        with pytest.raises(ValueError, match=what):
+            _cache(**kw).share()
+
+
+def test_differential_attention_needs_a_packed_cache_with_tokens():
+    q = torch.zeros((1, 4, 1, 128), dtype=torch.float16)
+    with pytest.raises(RuntimeError, match="not enabled"):
+        _cache(fused_sdpa=False).fused_differential_sdpa(q, 0.1, 0.1)
+    with pytest.raises(RuntimeError, match="before any tokens"):
+        _cache().fused_differential_sdpa(q, 0.1, 0.1)
