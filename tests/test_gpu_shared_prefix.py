@@ -55,6 +55,44 @@ def test_plain_rows(dtype, B, Hq, Hkv, D, n, own, Sq):
     _case(B, Hq, Hkv, D, (0, n), (0, own), Sq, dtype=dtype, view=True)
 
 
+@pytest.mark.parametrize("kw", [
+    dict(Hq=8, D=128, own=(512, 70), bits=4), dict(Hq=8, D=64, own=(256, 33), bits=2), dict(Hq=4, D=256, own=(256, 40)), dict(Hq=40, D=128, own=(512, 40), Sq=3),
+    dict(Hq=8, D=128, own=(0, 200), dtype=BF16), dict(Hq=8, D=128, own=(0, 200), dtype=BF16, Sq=70), dict(Hq=8, D=80, own=(256, 33)),
+    dict(Hq=8, D=128, own=(128, 50), dtype=BF16), dict(Hq=8, D=128, own=(128, 50), v_layout="channel")])
+@pytest.mark.parametrize("prefix", [(0, 0), (1536, 20)])
+def test_nothing_behind_a_sequence_counts(kw, prefix):
+    """Rows, scales and zeros behind a sequence's length may be NaN: the same bits, both operators."""
+    require_gpu()
+    kw = dict(bits=4, group=32, v_layout="token", dtype=F16, Sq=1) | kw
+    Hq, D, own, Sq, dtype, Hkv = kw.pop("Hq"), kw.pop("D"), kw.pop("own"), kw.pop("Sq"), kw["dtype"], 2
+    lens = [0, 1, 31, 32, 33, own[0], own[0] + 1, sum(own) - 1, sum(own), 100]
+    B = len(lens)
+    if D % kw["group"]:
+        kw["group"] = 16
+    o, _, _ = store(B, Hkv, *own, D, seed=2, **kw)
+    p = store(1, Hkv, *prefix, D, seed=1, **kw)[0] if sum(prefix) else None
+    q = torch.randn((B, Hq, Sq, D), generator=torch.Generator(device="cuda").manual_seed(0), device="cuda").to(dtype)
+    dead = {n: t.clone() if isinstance(t, torch.Tensor) else t for n, t in o.items()}
+    for b, n in enumerate(lens):
+        tail = max(0, n - own[0])
+        if own[1]:
+            dead["k_tail"][b, :, tail:], dead["v_tail"][b, :, tail:] = float("nan"), float("nan")
+        if own[0]:
+            group = -(-n // kw["group"])
+            for name in ("k_scale", "k_zero"):
+                dead[name][b, :, group:] = float("nan")
+            for name in ("v_scale", "v_zero"):
+                (dead[name][b, ..., n:] if kw["v_layout"] == "token" else dead[name][b, :, n:]).fill_(float("nan"))
+    at = torch.tensor(lens, device="cuda")
+    for causal in (False, True):
+        call = dict(scale=0.1, causal=causal, seq_lens=at)
+        if p is not None:
+            one, two = (K.shared_prefix_attend(q, p, **x, **call) for x in (o, dead))
+        else:
+            one, two = (K.differential_attend(q, 0.4, **x, **call) for x in (o, dead))
+        assert bool(one.isfinite().all()) and torch.equal(one, two)
+
+
 def test_float32_scales_near_zero():
     """code * scale + zero of float32 scales is formed with one rounding to float32: a difference of near-equal numbers, seen alone through a
     window of one slot, is the fp16 number nearest to it."""
