@@ -383,9 +383,14 @@ template <int BITS, typename T, int D, int MAPS, int WT> __device__ __forceinlin
             aside.all();
             return;
         }
+        // (a wave at its products goes before one at its softmax: 1 to 2 % but for few units a block)
+        __builtin_amdgcn_s_setprio(1);
         scores(tile + th * (32 * D * 2), aside);
+        __builtin_amdgcn_s_setprio(0);
         weights(place + 32 * th, live - 32 * th, aside);
+        __builtin_amdgcn_s_setprio(1);
         sums(transposed, tile + (transposed.value ? th * 64 : th * (32 * D * 2)));
+        __builtin_amdgcn_s_setprio(0);
     };
     struct Nothing {
         __device__ __forceinline__ void keys(int) {}
