@@ -43,7 +43,7 @@ constexpr int SP_WAVES = 4, SP_THREADS = 64 * SP_WAVES;
 
 // Weights of fp16 are formed as 2^SP_LIFT exp2(s - m), at most 2^15 with m followed within 2^8: fp16 then tells a weight of 2^-32 of the
 // largest from zero (2^-25 without), of which a long context may hold as many as count.  Sums and the weights' sum carry the factor alike.
-constexpr float SP_LIFT = 7.f;
+constexpr float SP_LIFT = 7.f, SP_MOST = 32768.f;
 
 template <typename T> struct SpanMma;
 template <> struct SpanMma<f16> {
@@ -289,6 +289,11 @@ template <int BITS, typename T, int D, int MAPS, int WT> __device__ __forceinlin
     u32x4 P[X][2];
     // Operands are asked for four products ahead, as written: left to itself the scheduler reads each right before its product and waits.
     constexpr int AHEAD = 4;
+    struct Nothing {
+        __device__ __forceinline__ void keys(int) {}
+        __device__ __forceinline__ void values(int) {}
+        __device__ __forceinline__ void all() {}
+    };
     // (`aside`: copies of a later unit that are asked for in between, keys' beside the products, values' beside the exponentials)
     auto scores = [&](u32 tile, auto &aside) __attribute__((always_inline)) {
         constexpr int N = X * KS;
@@ -321,17 +326,37 @@ template <int BITS, typename T, int D, int MAPS, int WT> __device__ __forceinlin
                     if (t >= hi || t < lo) S[x][r] = -INFINITY;
                 }
         }
+        // The weights at the reference maximum as it is.  Only where a lane's sum of them passes what fp16 holds, or a row has no reference yet,
+        // the maximum is looked for and they are formed again: a few times a run.
         // (the first reader of the products is the compiler's own, which waits for them: it does not on behalf of inline assembly)
-        float mx[X];
+        float l2[2], nm;   // (short chains)
+        auto form = [&](auto &aside) __attribute__((always_inline)) {
+            nm = m_run == -INFINITY ? 0.f : std::is_same_v<T, f16> ? SP_LIFT - m_run : -m_run;
+            l2[0] = l2[1] = 0.f;
 #pragma unroll
-        for (int x = 0; x < X; ++x) {
-            const float m0 = fmaxf(S[x][0], S[x][1]);
-            mx[x] = sp_max3(sp_max3(sp_max3(m0, S[x][2], S[x][3]), sp_max3(m0, S[x][4], S[x][5]), sp_max3(m0, S[x][6], S[x][7])), sp_max3(m0, S[x][8], S[x][9]),
-                            sp_max3(sp_max3(m0, S[x][10], S[x][11]), sp_max3(m0, S[x][12], S[x][13]), sp_max3(m0, S[x][14], S[x][15])));
-        }
-        const float most = X == 2 ? fmaxf(mx[0], mx[X - 1]) : mx[0];
-        if (__any(most * cc > m_run + RESCALE_SLACK)) {
-            const float top = fmaxf(most, __shfl_xor(most, 32)) * cc, m = fmaxf(m_run, top);
+            for (int x = 0; x < X; ++x)
+#pragma unroll
+                for (int r = 0; r < 8; ++r) {
+                    const u32 p = M::pack(__builtin_amdgcn_exp2f(__builtin_fmaf(S[x][2 * r], cc, nm)), __builtin_amdgcn_exp2f(__builtin_fmaf(S[x][2 * r + 1], cc, nm)));
+                    P[x][r / 4][r % 4] = p;
+                    l2[r & 1] = M::add_pair(p, l2[r & 1]);
+                    if (r & 1) aside.values(4 * x + r / 2);
+                }
+        };
+        form(aside);
+        const bool late = l2[0] + l2[1] > SP_MOST || m_run == -INFINITY;
+        if (__any(late)) {   // (for the rows that need it: a row's bits do not depend on the wave's others)
+            const int other = __shfl_xor(late ? 1 : 0, 32);   // (by all lanes)
+            const bool needed = late || other != 0;
+            float mx[X];
+#pragma unroll
+            for (int x = 0; x < X; ++x) {
+                const float m0 = fmaxf(S[x][0], S[x][1]);
+                mx[x] = sp_max3(sp_max3(sp_max3(m0, S[x][2], S[x][3]), sp_max3(m0, S[x][4], S[x][5]), sp_max3(m0, S[x][6], S[x][7])), sp_max3(m0, S[x][8], S[x][9]),
+                                sp_max3(sp_max3(m0, S[x][10], S[x][11]), sp_max3(m0, S[x][12], S[x][13]), sp_max3(m0, S[x][14], S[x][15])));
+            }
+            const float most = X == 2 ? fmaxf(mx[0], mx[X - 1]) : mx[0];
+            const float top = fmaxf(most, __shfl_xor(most, 32)) * cc, m = needed ? fmaxf(m_run, top) : m_run;
             const float alpha = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - m);
             m_run = m;
             l_run *= alpha;
@@ -339,18 +364,9 @@ template <int BITS, typename T, int D, int MAPS, int WT> __device__ __forceinlin
             for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) O[dt][r] *= alpha;
+            Nothing nothing;
+            form(nothing);
         }
-        const float nm = m_run == -INFINITY ? 0.f : std::is_same_v<T, f16> ? SP_LIFT - m_run : -m_run;
-        float l2[2] = {0.f, 0.f};   // (short chains)
-#pragma unroll
-        for (int x = 0; x < X; ++x)
-#pragma unroll
-            for (int r = 0; r < 8; ++r) {
-                const u32 p = M::pack(__builtin_amdgcn_exp2f(__builtin_fmaf(S[x][2 * r], cc, nm)), __builtin_amdgcn_exp2f(__builtin_fmaf(S[x][2 * r + 1], cc, nm)));
-                P[x][r / 4][r % 4] = p;
-                l2[r & 1] = M::add_pair(p, l2[r & 1]);
-                if (r & 1) aside.values(4 * x + r / 2);
-            }
         l_run += l2[0] + l2[1];
     };
     auto sums = [&](auto transposed, u32 tile) __attribute__((always_inline)) {
@@ -391,11 +407,6 @@ template <int BITS, typename T, int D, int MAPS, int WT> __device__ __forceinlin
         __builtin_amdgcn_s_setprio(1);
         sums(transposed, tile + (transposed.value ? th * 64 : th * (32 * D * 2)));
         __builtin_amdgcn_s_setprio(0);
-    };
-    struct Nothing {
-        __device__ __forceinline__ void keys(int) {}
-        __device__ __forceinline__ void values(int) {}
-        __device__ __forceinline__ void all() {}
     };
 
     // ---- one span after the other.  A store's fields are read from the argument block where a span begins (`fresh` hides the block's
