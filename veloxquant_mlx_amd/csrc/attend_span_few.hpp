@@ -134,11 +134,27 @@ template <int BITS, int D, int MAPS, int WAVES> __device__ __forceinline__ void 
                 if (t >= hi || t < lo) S[r] = -INFINITY;
             }
         }
-        float mx = fmaxf(S[0], S[1]);   // (first: the compiler waits for the products only before instructions of its own)
+        // (as in attend_span_mfma.hpp: the maximum only where the weights' sum asks for it)
+        float l2[2], nm;
+        auto form = [&]() __attribute__((always_inline)) {
+            nm = m_run == -INFINITY ? 0.f : SP_LIFT - m_run;
+            l2[0] = l2[1] = 0.f;
 #pragma unroll
-        for (int r = 2; r < 16; r += 2) mx = sp_max3(mx, S[r], S[r + 1]);
-        if (__any(mx * cc > m_run + RESCALE_SLACK)) {
-            const float top = fmaxf(mx, __shfl_xor(mx, 32)) * cc, m = fmaxf(m_run, top);
+            for (int r = 0; r < 8; ++r) {
+                const u32 p = M::pack(__builtin_amdgcn_exp2f(__builtin_fmaf(S[2 * r], cc, nm)), __builtin_amdgcn_exp2f(__builtin_fmaf(S[2 * r + 1], cc, nm)));
+                P[r / 4][r % 4] = p;
+                l2[r & 1] = M::add_pair(p, l2[r & 1]);
+            }
+        };
+        form();
+        const bool late = l2[0] + l2[1] > SP_MOST || m_run == -INFINITY;
+        if (__any(late)) {
+            const int other = __shfl_xor(late ? 1 : 0, 32);   // (by all lanes)
+            const bool needed = late || other != 0;
+            float mx = fmaxf(S[0], S[1]);
+#pragma unroll
+            for (int r = 2; r < 16; r += 2) mx = sp_max3(mx, S[r], S[r + 1]);
+            const float top = fmaxf(mx, __shfl_xor(mx, 32)) * cc, m = needed ? fmaxf(m_run, top) : m_run;
             const float alpha = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - m);
             m_run = m;
             l_run *= alpha;
@@ -146,14 +162,9 @@ template <int BITS, int D, int MAPS, int WAVES> __device__ __forceinline__ void 
             for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) O[dt][r] *= alpha;
+            form();
         }
-        const float nm = m_run == -INFINITY ? 0.f : SP_LIFT - m_run;
-#pragma unroll
-        for (int r = 0; r < 8; ++r) {
-            const u32 p = M::pack(__builtin_amdgcn_exp2f(__builtin_fmaf(S[2 * r], cc, nm)), __builtin_amdgcn_exp2f(__builtin_fmaf(S[2 * r + 1], cc, nm)));
-            P[r / 4][r % 4] = p;
-            l_run = M::add_pair(p, l_run);
-        }
+        l_run += l2[0] + l2[1];
     };
 
     const u32 room = lds_addr(lds) + wave * F::ROOM;   // this wave's
