@@ -9,8 +9,8 @@
 // share rows, each with its half of every unit, and add up in LDS at the end.
 //
 // Bound by what a SIMD's two waves do one after the other.  For a unit of 64 slots and 32 rows, two maps of 128 channels, a wave spends 770
-// cycles in 24 products and ~950 in the softmax (32 exponentials of 16 cycles, ~130 other instructions); measured: 2550 cycles a unit while
-// the other wave takes 3100, 1.87 GHz, 227 us for 32 heads over 4096 tokens (910 TFLOP/s of products).  Two blocks a CU, which no barrier
+// cycles in 24 products and ~900 in the softmax (32 exponentials of 16 cycles, ~110 other instructions); measured: 2550 cycles a unit while
+// the other wave takes 3100, 1.87 GHz, 225 to 233 us for 32 heads over 4096 tokens (900 TFLOP/s of products).  Two blocks a CU, which no barrier
 // ties together, overlap one's vector work, copies, start (5000 cycles, integer divisions) and end with the other's products.  What was
 // slower: eight waves in one block, 3700 cycles a unit in step at every barrier, 2700 with half of the waves a phase behind the other half, as
 // every block then starts and ends alone on its CU; 64 rows a wave, which halves the LDS reads, 268 us to 261; a causal order
@@ -24,8 +24,8 @@
 // sixteen columns, lane i gets column i), from packed ones by storing them transposed in that very order.  Sums, maxima
 // and accumulators stay in the lane of their row.
 //
-// The softmax keeps a reference maximum that follows the true one lazily (within 8 powers of two), so accumulators are rescaled a few
-// times a run; weights are rounded to the operand type, and their sum is that of the rounded ones.
+// The softmax keeps a reference maximum that follows the true one only where a lane's sum of weights passes 2^15, so accumulators are rescaled
+// a few times a run and most units look for no maximum; weights are rounded to the operand type, and their sum is that of the rounded ones.
 #pragma once
 #include <atomic>
 #include <type_traits>
@@ -41,7 +41,7 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 constexpr int SP_WAVES = 4, SP_THREADS = 64 * SP_WAVES;
 
-// Weights of fp16 are formed as 2^SP_LIFT exp2(s - m), at most 2^15 with m followed within 2^8: fp16 then tells a weight of 2^-32 of the
+// Weights of fp16 are formed as 2^SP_LIFT exp2(s - m), at most SP_MOST: fp16 then tells a weight of 2^-32 of the
 // largest from zero (2^-25 without), of which a long context may hold as many as count.  Sums and the weights' sum carry the factor alike.
 constexpr float SP_LIFT = 7.f, SP_MOST = 32768.f;
 
