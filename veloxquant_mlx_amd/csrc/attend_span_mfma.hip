@@ -55,7 +55,7 @@ void span_mfma_plan(SpanCall &c, int maps) {
     // with six, 25.2 with eight).
     auto side = [&](bool by_few, int64_t rows, int64_t slots32, int64_t slots64, int64_t times, int &wt, int &tiles, int64_t &units, int64_t &least) {
         units = by_few || a.D == 256 ? slots32 : slots64;
-        least = by_few ? 16 : a.D == 256 ? 12 : 6;
+        least = by_few ? 16 : 6;
         wt = !by_few && a.D != 256 && (rows <= most / 2 || roomy) ? 2 : 1;
         tiles = by_few ? 1 : (int)cdiv(rows, most / wt);
         return times * a.Hkv * tiles * units;   // units of all blocks
