@@ -17,7 +17,7 @@ struct SpanCall {
     int psplits, osplits;  // runs of the prefix / of a sequence's own slots (MFMA: see attend_span_mfma.hpp)
     int ptiles, otiles;    // row tiles of the prefix / of a sequence
     int pwt, owt;          // waves that share a row (1 or 2), each with its half of every unit
-    int pfew, ofew;        // 1: that side by the kernel for few rows (attend_span_few.hpp), one tile of rows
+    int pfew, ofew;        // 1: that side by the kernel for few rows (attend_span_few.hpp)
     int owaves;            // waves of a block of that kernel: 4, or 8 (own slots and prefix together, one part)
     int apart;             // 1: prefix and own slots belong to different blocks; 0: the blocks of a row walk both
     float *sums;           // [rows][nparts][maps][D]

@@ -1,4 +1,4 @@
-// Attention over spans of packed slots for few query rows: up to 32 rows of one kv head, or 16 with two maps (gfx950, wave64).
+// Attention over spans of packed slots for few query rows: tiles of up to 32 rows of one kv head, or 16 with two maps (gfx950, wave64).
 //
 // Bound by the bytes of the slots and by reconstructing them, so no wave waits for another: every wave walks its own units of 32 slots,
 // every WAVES-th of the block's run, from its own ring in LDS that asynchronous copies fill RING - 1 units ahead, and reconstructs
@@ -43,20 +43,22 @@ template <int BITS, int D, int MAPS, int WAVES> __device__ __forceinline__ void 
     const int before = (int)span_prefix_slots(a);
 
     // ---- the block: the prefix under the rows of all sequences, or a sequence's slots under its rows; kv head fastest
-    const int shared_blocks = c.apart && c.pfew ? c.psplits * Hkv : 0;
+    const int shared_blocks = c.apart && c.pfew ? c.psplits * c.ptiles * Hkv : 0;
     const bool shared = id < shared_blocks;
     if (!shared) id -= shared_blocks;
     const int hkv = id % Hkv;
     id /= Hkv;
     const int b = shared ? 0 : id % (int)a.B;
     if (!shared) id /= (int)a.B;
-    const int split = id, splits = shared ? c.psplits : c.osplits, part = shared || !c.apart ? split : c.psplits + split;
+    const int splits = shared ? c.psplits : c.osplits, split = id % splits, part = shared || !c.apart ? split : c.psplits + split;
     const int rows = shared ? (int)a.B * r1 : r1;
 
     // ---- this lane's query row: positions outermost
     constexpr int ROWS = 32 / MAPS;
-    const int map = MAPS == 2 ? n >> 4 : 0, j = n % ROWS, jc = j < rows ? j : rows - 1;
+    const int j0 = id / splits * ROWS, here = rows - j0 < ROWS ? rows - j0 : ROWS;   // the block's tile of rows
+    const int map = MAPS == 2 ? n >> 4 : 0, j = n % ROWS, jc = j < here ? j : here - 1;
     auto row_of = [&](int x, int &jb, int &pos) __attribute__((always_inline)) {   // flattened [B, Hq, Sq] row of tile row x
+        x += j0;
         const int rem = shared ? x % r1 : x;
         jb = shared ? x / r1 : b;
         pos = rem / G;
@@ -93,7 +95,7 @@ template <int BITS, int D, int MAPS, int WAVES> __device__ __forceinline__ void 
     const int run = total / splits, longer = total % splits;   // (the first runs a unit longer)
     const int w0 = split * run + (split < longer ? split : longer), w1 = w0 + run + (split < longer ? 1 : 0);
     if (w0 == w1 && c.nparts > 1) {   // (uniform) nothing: sums are not written
-        if (tid < rows * MAPS) {
+        if (tid < here * MAPS) {
             int x, y;
             *(float2 *)(c.ml + ((row_of(tid / MAPS, x, y) * c.nparts + part) * MAPS + tid % MAPS) * 2) = make_float2(-INFINITY, 0.f);
         }
@@ -407,7 +409,7 @@ template <int BITS, int D, int MAPS, int WAVES> __device__ __forceinline__ void 
     lds_barrier();
     const int ch = tid & 31;
 #pragma unroll 1
-    for (int x = tid >> 5; x < ROWS && x < rows; x += F::THREADS / 32) {
+    for (int x = tid >> 5; x < here; x += F::THREADS / 32) {
         int jb2, pos2;
         const int64_t row = row_of(x, jb2, pos2);
         float o[DT];
@@ -437,7 +439,7 @@ template <int BITS, int D, int MAPS, int WAVES> __device__ __forceinline__ void 
 #pragma unroll
                 for (int dt = 0; dt < DT; dt += 2) *(float2 *)(dst + dt) = make_float2(num[dt], num[dt + 1]);
             }
-            const float by = den > 0.f || den != den ? (w == 0 ? 1.f : -span_lam(a, hkv * G + (shared ? x % r1 : x) % G)) / den : 0.f;
+            const float by = den > 0.f || den != den ? (w == 0 ? 1.f : -span_lam(a, hkv * G + (shared ? (j0 + x) % r1 : j0 + x) % G)) / den : 0.f;
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) o[dt] = __builtin_fmaf(num[dt], by, o[dt]);
         }
@@ -480,7 +482,7 @@ template <int BITS, int D> int launch_span_both_as(const SpanCall &c) {
     const auto kernel = span_both_kernel<BITS, D>;
     static std::atomic<bool> allowed[64] = {};
     if (int rc = span_allow_lds((const void *)kernel, bytes, allowed)) return rc;
-    const int64_t tiles = (int64_t)c.psplits * c.ptiles * c.a.Hkv, few = c.a.B * c.a.Hkv * c.osplits, blocks = tiles + few;
+    const int64_t tiles = (int64_t)c.psplits * c.ptiles * c.a.Hkv, few = c.a.B * c.a.Hkv * c.osplits * c.otiles, blocks = tiles + few;
     VQ_REQUIRE(blocks < (INT64_C(1) << 23), VQ_ERR_UNSUPPORTED, "attention over spans: too many sequences and heads for one launch");
     kernel<<<(unsigned)blocks, SP_THREADS, bytes, (hipStream_t)c.a.stream>>>(c);
     VQ_HIP_CHECK_LAUNCH("attention over spans");
@@ -492,7 +494,7 @@ template <int BITS, int D, int MAPS, int WAVES> int launch_span_few_of(const Spa
     const auto kernel = span_few_kernel<BITS, D, MAPS, WAVES>;
     static std::atomic<bool> allowed[64] = {};
     if (int rc = span_allow_lds((const void *)kernel, bytes, allowed)) return rc;
-    const int64_t blocks = (c.apart && c.pfew ? (int64_t)c.psplits * c.a.Hkv : 0) + (c.ofew ? c.a.B * c.a.Hkv * c.osplits : 0);
+    const int64_t blocks = (c.apart && c.pfew ? (int64_t)c.psplits * c.ptiles * c.a.Hkv : 0) + (c.ofew ? c.a.B * c.a.Hkv * c.osplits * c.otiles : 0);
     if (blocks == 0) return VQ_OK;
     VQ_REQUIRE(blocks < (INT64_C(1) << 23), VQ_ERR_UNSUPPORTED, "attention over spans: too many sequences and heads for one launch");
     kernel<<<(unsigned)blocks, 64 * WAVES, bytes, (hipStream_t)c.a.stream>>>(c);

@@ -42,8 +42,10 @@ void span_mfma_plan(SpanCall &c, int maps) {
     const bool brief = packed ? r1 <= few && a.D != 256 && units_of(a.prefix, 32) + units_of(a.own, 32) <= 40 && a.B * a.Hkv <= 256
                               : a.D != 256 && units_of(a.prefix, 64) + units_of(a.own, 64) <= 8 && a.B * a.Hkv <= 512;
     c.apart = prefix_slots && a.B > 1 && r1 <= most / 2 && !brief;
-    c.pfew = packed && all <= few;
-    c.ofew = packed && r1 <= few;
+    // few rows: one tile of the kernel for them; two with heads of 256 channels, of which the other kernel would leave half of its waves idle
+    const int most_few = a.D == 256 ? 2 * few : few;
+    c.pfew = packed && all <= most_few;
+    c.ofew = packed && r1 <= most_few;
     const int64_t p32 = units_of(a.prefix, 32), p64 = units_of(a.prefix, 64), o32 = units_of(a.own, 32), o64 = units_of(a.own, 64);
     // Two waves share rows where those fill half a block, and over plain rows where blocks of as many rows as fit would leave half of the chip empty
     // (two maps, 8 heads over 500 tokens: 13.8 us, and 16.4; 8 sequences of five rows and 200 slots on 2000: 16.5 and 18.0).
@@ -57,7 +59,7 @@ void span_mfma_plan(SpanCall &c, int maps) {
         units = by_few || a.D == 256 ? slots32 : slots64;
         least = by_few ? 16 : 6;
         wt = !by_few && a.D != 256 && (rows <= most / 2 || roomy) ? 2 : 1;
-        tiles = by_few ? 1 : (int)cdiv(rows, most / wt);
+        tiles = (int)cdiv(rows, by_few ? few : most / wt);
         return times * a.Hkv * tiles * units;   // units of all blocks
     };
     int64_t pu = 0, ou = 0, pleast = 1, oleast = 1, pwork = 0;
