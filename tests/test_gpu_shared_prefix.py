@@ -105,7 +105,8 @@ def test_float32_scales_near_zero():
     dict(B=24, Hq=12, Hkv=3, D=128, prefix=(2048, 0), own=(512, 9), bits=4, group=64, lens=[(b * 97) % 522 for b in range(24)]),
     dict(B=70, Hq=4, Hkv=4, D=128, prefix=(384, 5), own=(128, 20), bits=2, window=150), dict(B=20, Hq=6, Hkv=2, D=256, prefix=(512, 40), own=(128, 9)),
     dict(B=9, Hq=16, Hkv=2, D=128, prefix=(512, 1), own=(128, 30), Sq=5, dtype=BF16), dict(B=33, Hq=2, Hkv=2, D=128, prefix=(0, 90), own=(128, 30)),
-    dict(B=3, Hq=16, Hkv=2, D=128, prefix=(4096, 0), own=(0, 140), Sq=7, group=128)])
+    dict(B=3, Hq=16, Hkv=2, D=128, prefix=(4096, 0), own=(0, 140), Sq=7, group=128), dict(B=30, Hq=9, Hkv=3, D=128, prefix=(1536, 20), own=(256, 9)),
+    dict(B=61, Hq=8, Hkv=2, D=256, prefix=(1280, 5), own=(128, 40), bits=2), dict(B=9, Hq=8, Hkv=2, D=64, prefix=(1280, 0), own=(640, 33), Sq=9, window=700)])
 def test_prefixes_of_many_rows(kw):
     """The prefix under the rows of all sequences, next to own slots under few rows, with lengths and windows that leave runs empty."""
     require_gpu()

@@ -42,11 +42,14 @@ void span_mfma_plan(SpanCall &c, int maps) {
     const bool brief = packed ? r1 <= few && a.D != 256 && units_of(a.prefix, 32) + units_of(a.own, 32) <= 40 && a.B * a.Hkv <= 256
                               : a.D != 256 && units_of(a.prefix, 64) + units_of(a.own, 64) <= 8 && a.B * a.Hkv <= 512;
     c.apart = prefix_slots && a.B > 1 && r1 <= most / 2 && !brief;
-    // few rows: one tile of the kernel for them; two with heads of 256 channels, of which the other kernel would leave half of its waves idle
-    const int most_few = a.D == 256 ? 2 * few : few;
-    c.pfew = packed && all <= most_few;
-    c.ofew = packed && r1 <= most_few;
     const int64_t p32 = units_of(a.prefix, 32), p64 = units_of(a.prefix, 64), o32 = units_of(a.own, 32), o64 = units_of(a.own, 64);
+    // Few rows by the kernel for them, in so many tiles: each reads and reconstructs the slots again, as the other kernel's blocks do, but no wave
+    // waits for another, and none of them idles at heads of 256 channels, where the other's waves share no rows.  A prefix: 64 rows over 16k slots
+    // 27.8 us, and 33.1 by the other kernel, 126 rows of 256 channels 64 and 78; 128 rows of 128 channels 44.7 and 41.1.  Own slots, two maps and 80
+    // rows over 8k 32 us and 37, but 155 and 148 for 16 sequences of 16k; next to a prefix in tiles 66 and 71 for 16 sequences of 36 rows, 46 and 41
+    // for four.
+    c.pfew = packed && all <= (a.D == 256 ? 8 : 3) * few;
+    c.ofew = packed && (r1 <= few || (r1 <= 2 * few && 2 * a.B * a.Hkv * o32 <= 65536 && (!c.apart || c.pfew || a.B * a.Hkv >= 64)));
     // Two waves share rows where those fill half a block, and over plain rows where blocks of as many rows as fit would leave half of the chip empty
     // (two maps, 8 heads over 500 tokens: 13.8 us, and 16.4; 8 sequences of five rows and 200 slots on 2000: 16.5 and 18.0).
     auto blocks_of = [&](int64_t rows, int64_t units, int64_t times) { return times * a.Hkv * cdiv(rows, most) * cdiv(units, 6); };
