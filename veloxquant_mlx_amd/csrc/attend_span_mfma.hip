@@ -76,7 +76,7 @@ void span_mfma_plan(SpanCall &c, int maps) {
     };
     auto round = [&](bool by_few) { return by_few && a.D == 256 ? 256 : 512; };   // blocks that run at once
     // (tiles beside few rows: one a CU where the few rows' work can fill the other half -- 43 us and 47 of two a CU for 21 sequences of 0.6k slots
-    // on 16k -- and two where not, 136 us and 150 for 128 of 80 slots on 32k)
+    // on 16k, as tiles -- and two where not, 136 us and 150 for 128 of 80 slots on 32k)
     c.psplits = c.apart ? cut(pu, pwork, pleast, span_both(c) && pwork <= owork ? 256 : round(c.pfew)) : 0;
     c.osplits = cut(ou, owork, oleast, round(c.ofew) * (a.seq_lens != nullptr ? 4 : 1));
     // Parts are written and read again, at ~4 TB/s, and merged in a launch of ~6 us: rows of tiles stay whole where the units saved, ~1.4 us each, are
