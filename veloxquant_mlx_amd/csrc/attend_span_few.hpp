@@ -261,10 +261,18 @@ template <int BITS, int D, int MAPS, int WAVES> __device__ __forceinline__ void 
                     S = M::mma(sp_values8(code, kmeta[k], kmeta[CH + k]), q[k], S);
                 }
             }
+            // (the values' words are asked for ahead of the softmax)
+            const char *vw_p = take + F::WORDS;
+            u32 lo[2][DT], hi[2][DT];   // of sixteen slots (4 bits: of eight each)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                sp_load_words<DT>(vw_p + ((BITS == 4 ? 2 * s : s) * D + DT * n) * 4, lo[s]);
+                if constexpr (BITS == 4) sp_load_words<DT>(vw_p + ((2 * s + 1) * D + DT * n) * 4, hi[s]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
             u32x4 P[2];
             softmax(S, place, live, P);
             // sums: channels DT n + dt
-            const char *vw_p = take + F::WORDS;
             const char *vmeta = take + 2 * F::WORDS + F::META + (DT * n / 32) * 64 + 8 * h;
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
@@ -282,14 +290,11 @@ template <int BITS, int D, int MAPS, int WAVES> __device__ __forceinline__ void 
                     sc = make_uint4(sc.x & m[0], sc.y & m[1], sc.z & m[2], sc.w & m[3]);
                     ze = make_uint4(ze.x & m[0], ze.y & m[1], ze.z & m[2], ze.w & m[3]);
                 }
-                u32 lo[DT], hi[DT];   // the words of the sixteen slots (4 bits: of eight each)
-                sp_load_words<DT>(vw_p + ((BITS == 4 ? 2 * s : s) * D + DT * n) * 4, lo);
-                if constexpr (BITS == 4) sp_load_words<DT>(vw_p + ((2 * s + 1) * D + DT * n) * 4, hi);
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) {
                     // 4 bits: this half's sixteen bits of either word; 2 bits: bytes h and 2 + h of the one
-                    const u32 w = BITS == 4 ? __builtin_amdgcn_perm(hi[dt], lo[dt], h ? 0x07060302u : 0x05040100u)
-                                            : __builtin_amdgcn_perm(0u, lo[dt], h ? 0x0C0C0301u : 0x0C0C0200u);
+                    const u32 w = BITS == 4 ? __builtin_amdgcn_perm(hi[s][dt], lo[s][dt], h ? 0x07060302u : 0x05040100u)
+                                            : __builtin_amdgcn_perm(0u, lo[s][dt], h ? 0x0C0C0301u : 0x0C0C0200u);
                     u32 code[4];
                     sp_codes8<BITS>(w, magic, code);
                     const u32x4 v = sp_values8(code, sc, ze);
