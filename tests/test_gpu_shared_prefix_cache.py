@@ -127,6 +127,24 @@ def test_one_sequence_is_a_cache():
     assert float((one.float() - other.float()).abs().max()) <= 2e-3 * max(1.0, float(one.abs().max()))
 
 
+def test_the_context_limit_counts_the_prefix():
+    require_gpu()
+    cache = _cache(128, fused_sdpa_max_ctx=512)
+    k = torch.randn((1, 2, 300, 128), device="cuda").half()
+    cache.update_and_fetch(k, k)
+    shared = cache.share()
+    rows = lambda n: torch.randn((3, 2, n, 128), device="cuda").half()
+    x = rows(200)
+    shared.update_and_fetch(x, x)
+    assert shared.offset == 500 and shared._own._packed_cap == 224     # 212 left, in whole groups
+    q = torch.randn((3, 4, 1, 128), device="cuda").half()
+    before = shared.fused_sdpa(q, 0.1)
+    with pytest.raises(RuntimeError, match="fused_sdpa_max_ctx"):
+        x = rows(100)
+        shared.update_and_fetch(x, x)
+    assert shared.offset == 500 and torch.equal(shared.fused_sdpa(q, 0.1), before)
+
+
 def test_shared_refusals():
     require_gpu()
     k = torch.zeros((2, 2, 5, 128), dtype=F16, device="cuda")

@@ -25,7 +25,8 @@ class SharedPrefixKIVICache:
 
     The prefix is a copy of the cache's tokens at that time and does not change any more; several objects may stand on one
     (:meth:`branch`).  A cache of its own in every other respect: ``update_and_fetch``, ``fused_sdpa``, ``trim`` (of the own tokens),
-    ``offset``, ``nbytes``."""
+    ``offset``, ``nbytes``.  ``fused_sdpa_max_ctx`` bounds prefix and own tokens together (the own packed store is sized by what
+    the prefix leaves)."""
 
     _memory_bound = True   # attention goes through fused_sdpa; update_and_fetch returns placeholders
 
@@ -48,6 +49,8 @@ class SharedPrefixKIVICache:
         self._head_dim = prefix._shape_bhd[2] // (2 if prefix._pair else 1)
         self._own = KIVIKVCache(prefix._config)
         self._own._launch_stores = False   # (no launch of this cache stores a token that was held back)
+        if self._own._max_ctx is not None:   # of the whole context
+            self._own._max_ctx = max(0, self._own._max_ctx - prefix.offset)
 
     def branch(self) -> "SharedPrefixKIVICache":
         """Another batch on the same prefix, without tokens of its own yet."""
