@@ -214,6 +214,21 @@ class KIVIKVCache(FP16KVCache):
         return (aged // self._group_size) * self._group_size
 
     # ------------------------------------------------------------------ packed store
+    def _fit_buffers(self, B: int, H: int, D: int, keys: torch.Tensor) -> None:
+        """Memory-bound mode's buffers have one batch, head count and head size, and the kernels that write them take their
+        addresses.  A cache without tokens lets go of buffers that are not for ``keys``; one with tokens refuses them."""
+        t = self._tail_k if self._tail_k is not None else self._ks
+        if t is None or (t.shape[0] == B and t.shape[1] == H and t.shape[3] == D and t.device == keys.device
+                         and (self.offset > 0 or t is self._ks or t.dtype == keys.dtype)):
+            return
+        if self.offset > 0:
+            raise ValueError(f"{type(self).__name__}.update_and_fetch: rows of {B} sequences, {H} heads and {D} channels on {keys.device}; this cache "
+                             f"holds {t.shape[0]} sequences, {t.shape[1]} heads and {t.shape[3]} channels on {t.device}")
+        self._kp = self._ks = self._kz = self._vp = self._vs = self._vz = None
+        self._packed_cap = 0
+        self._tail_k = self._tail_v = self._tail_spare = None
+        self._drop_tiles()
+
     def _ensure_packed_capacity(self, B: int, H: int, D: int, needed: int, device) -> None:
         if self._max_ctx is not None and needed > self._max_ctx:
             raise RuntimeError(f"KIVIKVCache: context length {needed} exceeded fused_sdpa_max_ctx={self._max_ctx}. "
@@ -289,12 +304,17 @@ class KIVIKVCache(FP16KVCache):
                 if D != 64 or not same:
                     raise ValueError(f"KIVIKVCache.update_and_fetch: this cache pairs {abs(self._kv_heads)} kv heads of 64 channels, "
                                      f"got {tuple(keys.shape)}")
+                shape = (B, (H + 1) // 2, 2 * D)
+                if self.offset == 0 or shape != self._shape_bhd:
+                    self._fit_buffers(*shape, keys)
                 self._kv_heads = H
-                self._shape_bhd = (B, (H + 1) // 2, 2 * D)
+                self._shape_bhd = shape
                 if not self._defer_token(keys, values):
                     self._update_memory_bound(pair_heads(keys), pair_heads(values))
                 z = self._zero_scalar.expand(B, H, self.offset, D)
                 return z, z
+            if self.offset == 0 or (B, H, D) != self._shape_bhd:
+                self._fit_buffers(B, H, D, keys)
             self._shape_bhd = (B, H, D)
             return self._update_memory_bound(keys, values)
         self._shape_bhd = (B, H, D)

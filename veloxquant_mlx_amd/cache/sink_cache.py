@@ -117,6 +117,8 @@ class SinkProtectedKVCache(KIVIKVCache):
     # ------------------------------------------------------------------ protocol
     def update_and_fetch(self, keys: torch.Tensor, values: torch.Tensor):
         B, H, S, D = keys.shape
+        if self._memory_bound and (self.offset == 0 or (B, H, D) != self._shape_bhd):
+            self._fit_buffers(B, H, D, keys)
         self._shape_bhd = (B, H, D)
         if self._n_sink:
             token_norm = torch.linalg.vector_norm(keys.float(), dim=-1).mean(dim=1)      # [B, S]
@@ -162,6 +164,13 @@ class SinkProtectedKVCache(KIVIKVCache):
         self._tokens_seen += S
 
     # ------------------------------------------------------------------ packed modes
+    def _fit_buffers(self, B: int, H: int, D: int, keys: torch.Tensor) -> None:
+        super()._fit_buffers(B, H, D, keys)
+        if self._tail_k is None and self._kp is None:   # nothing is kept: neither are protected rows
+            self._side_k = self._side_v = self._side_pos_dev = None
+            self._side_pos = []
+            self._top = _TopNorms(self._n_sink)
+
     def _pack_block(self, k_blk: torch.Tensor, v_blk: torch.Tensor, lo: int) -> None:
         B, H, n, D = k_blk.shape
         protected = self._top.inside(lo, lo + n)[:B] if self._n_sink else None

@@ -593,15 +593,29 @@ def kivi_cache_append(k_new: torch.Tensor, v_new: torch.Tensor, k_tail: torch.Te
     (k_packed, k_scale, k_zero, v_packed, v_scale, v_zero)`` at token ``dst_tok0`` and the
     rest moves to the front of ``spare = (k_spare, v_spare)``.  The steps of
     ``KIVIKVCache.update_and_fetch`` (veloxquant_mlx/cache/kivi_cache.py:206-262) on packed
-    buffers.  The caller owns the shapes: all tensors share a device, the new tokens and the
-    four tails one dtype, every buffer is contiguous except ``k_new`` / ``v_new``, whose
-    channels are.  ``args`` may carry a ``KiviAppendArgs`` from a previous call to refill."""
+    buffers.  All buffers are for the new tokens' batch, heads and channels.  The caller sees to the rest: all
+    tensors share a device, the new tokens and the four tails one dtype, every buffer is contiguous except ``k_new`` /
+    ``v_new``, whose channels are.  ``args`` may carry a ``KiviAppendArgs`` from a previous call to refill."""
     name = "kivi_cache_append"
-    _need_gpu(name, k_new)
     a = _lib.KiviAppendArgs() if args is None else args
     B, H, S, D = k_new.shape
     if v_new.shape != k_new.shape or k_tail.shape != v_tail.shape or k_tail.ndim != 4:
         raise ValueError(f"{name}: keys/values must be [B,H,S,D] and the tails [B,H,cap,D]")
+    if k_tail.shape[0] != B or k_tail.shape[1] != H or k_tail.shape[3] != D:
+        raise ValueError(f"{name}: tails {tuple(k_tail.shape)} do not fit new tokens {tuple(k_new.shape)}")
+    if n_flush:
+        per, cap = 32 // bits, packed[0].shape[2]
+        W, GV = -(-D // per), -(-D // group_size)
+        k_meta = (B, H, -(-cap // group_size), D)
+        v_want = ((cap // per, D), (GV, cap)) if v_layout == "token" else ((cap, W), (cap, GV))
+        want = ((B, H, cap, W), k_meta, k_meta, (B, H, *v_want[0]), (B, H, *v_want[1]), (B, H, *v_want[1]))
+        if any(t.shape != shape for t, shape in zip(packed, want)):
+            raise ValueError(f"{name}: packed store {[tuple(t.shape) for t in packed]} does not fit new tokens {tuple(k_new.shape)} at {bits} "
+                             f"bits, groups of {group_size}, values packed by {v_layout}")
+        room = spare[0].shape
+        if room != spare[1].shape or len(room) != 4 or room[0] != B or room[1] != H or room[3] != D:
+            raise ValueError(f"{name}: spare tails {tuple(room)} and {tuple(spare[1].shape)} do not fit new tokens {tuple(k_new.shape)}")
+    _need_gpu(name, k_new)
     if not (k_new.dtype == v_new.dtype == k_tail.dtype == v_tail.dtype):
         raise ValueError(f"{name}: new tokens and tails must share one dtype")
     a.k_new, a.v_new = k_new.data_ptr(), v_new.data_ptr()
@@ -621,8 +635,6 @@ def kivi_cache_append(k_new: torch.Tensor, v_new: torch.Tensor, k_tail: torch.Te
         a.v_packed, a.v_scale, a.v_zero = vp_.data_ptr(), vsc.data_ptr(), vz.data_ptr()
         a.meta_dtype = VQ_F16 if ksc.dtype == torch.float16 else VQ_F32
         a.cap_tokens, a.dst_tok0 = kp.shape[2], dst_tok0
-        if v_layout == "token" and vp_.shape[2] * per != kp.shape[2]:
-            raise ValueError(f"{name}: key and value stores differ in capacity")
         a.group, a.levels, a.eps, a.pack_bits, a.v_layout = group_size, levels, eps, bits, _V_LAYOUT[v_layout]
         a.k_spare, a.v_spare, a.spare_cap = spare[0].data_ptr(), spare[1].data_ptr(), spare[0].shape[2]
     _lib.check(_lib.load().vq_kivi_cache_append(C.byref(a), _stream(k_new)))
