@@ -271,9 +271,10 @@ SpanCall cut(const vq_store_attend_args &a, int maps) {
     return c;
 }
 
+// (the sums take whole 16 bytes, so that the pairs (m, l) behind them, read and written whole, are aligned with odd heads too)
 int64_t scratch_floats(const SpanCall &c, int maps, int64_t &sums) {
     const int64_t recs = c.a.B * c.a.Hq * c.a.Sq * c.nparts * maps;
-    sums = recs * c.a.D;
+    sums = cdiv(recs * c.a.D, 4) * 4;
     return sums + recs * 2;
 }
 
