@@ -1674,6 +1674,22 @@ def _extent(t: torch.Tensor) -> tuple[int, int]:
     return lo, lo + (sum((n - 1) * st for n, st in zip(t.shape, t.stride())) + 1) * t.element_size()
 
 
+def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two (non-empty) strided tensors certainly share no byte: their extents lie apart, or do so modulo one of their strides (views
+    of one projection, whose rows alternate: modulo a token's stride each is one stretch)."""
+    (a0, a1), (b0, b1) = _extent(a), _extent(b)
+    if a1 <= b0 or b1 <= a0:
+        return True
+    sides = [[(n, st * t.element_size()) for n, st in zip(t.shape, t.stride()) if n > 1 and st > 0] for t in (a, b)]
+    for m in {st for side in sides for _, st in side}:
+        # a dimension whose stride is a multiple of m stays where it is, the others take up a stretch
+        wide = [t.element_size() + sum((n - 1) * st for n, st in side if st % m) for t, side in zip((a, b), sides)]
+        off = (b0 - a0) % m
+        if wide[0] <= off and off + wide[1] <= m:
+            return True
+    return False
+
+
 def _same_rows(a: torch.Tensor, b: torch.Tensor) -> bool:
     return a.data_ptr() == b.data_ptr() and all(x == y or n < 2 for x, y, n in zip(a.stride(), b.stride(), a.shape))
 
@@ -1756,14 +1772,14 @@ def rotary_embed(q: torch.Tensor, k: torch.Tensor | None = None, *, inv_freq: to
     if B == 0 or S == 0 or Hq + Hk == 0:
         return result
     if not fresh:   # (new outputs overlap nothing)
-        live = [p for p in ((q, out, "q"), (k, k_out, "k")) if p[0] is not None and p[0].numel()]
-        still = [_same_rows(t, o) for t, o, _ in live]
-        for i, (t, o, what) in enumerate(live):
-            lo, hi = _extent(o)
-            for j, (u, p, _) in enumerate(live):
-                others = [] if still[i] and (i == j or still[j]) else [u] if i == j else [u, p]
-                if any(lo < e and s < hi for s, e in map(_extent, others)):
-                    raise ValueError(f"{name}: the output for {what} overlaps other rows of the call (it may only be its input itself)")
+        has_q, has_k = q.numel() > 0, k is not None and k.numel() > 0
+        q_still, k_still = has_q and _same_rows(q, out), has_k and _same_rows(k, k_out)
+        # an output and whatever it is not: its own rows unless turned in place, the other side's rows and output
+        both = has_q and has_k
+        for meets, what, o, t in ((has_q and not q_still, "q", out, q), (has_k and not k_still, "k", k_out, k), (both, "q", out, k_out),
+                                  (both and not k_still, "q", out, k), (both and not q_still, "k", k_out, q)):
+            if meets and not _apart(o, t):
+                raise ValueError(f"{name}: the output for {what} overlaps other rows of the call (it may only be its input itself)")
     lib = _lib.load()
     qb, qh, qs, _ = q.stride()
     pb, ph, ps, _ = out.stride()
