@@ -101,3 +101,17 @@ def test_outputs_that_meet_other_rows_are_refused(calls):
         with pytest.raises(ValueError, match="overlaps"):
             K.rotary_embed(**args, inv_freq=f)
     assert not calls
+
+
+def test_outputs_whose_rows_share_memory_are_refused(calls):
+    f, buf = torch.ones(8), torch.zeros(8192)
+    x = torch.zeros((2, 3, 5, 16))
+    for strides in ((240, 80, 8, 1), (240, 80, 15, 1), (240, 0, 16, 1), (240, 79, 16, 1), (239, 80, 16, 1), (80, 80, 16, 1)):
+        with pytest.raises(ValueError, match="share memory"):
+            K.rotary_embed(x, inv_freq=f, out=buf.as_strided(x.shape, strides))
+        with pytest.raises(ValueError, match="share memory"):
+            K.rotary_embed(x, x.clone(), inv_freq=f, k_out=buf.as_strided(x.shape, strides))
+    for strides in ((240, 80, 16, 1), (16, 32, 96, 1), (48, 16, 96, 1), (1000, 17, 60, 1), (16, 160, 32, 1)):
+        K.rotary_embed(x, inv_freq=f, out=buf.as_strided(x.shape, strides))
+    K.rotary_embed(x[:1, :1], inv_freq=f, out=buf.as_strided((1, 1, 5, 16), (0, 0, 16, 1)))   # strides that nothing walks
+    assert len(calls) == 6

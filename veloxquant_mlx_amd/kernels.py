@@ -1690,6 +1690,16 @@ def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
     return False
 
 
+def _rows_apart(t: torch.Tensor) -> bool:
+    """Whether every element of a strided tensor has a place of its own: each stride passes all that the smaller ones reach."""
+    reach = 1
+    for st, n in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n > 1):
+        if st < reach:
+            return False
+        reach += (n - 1) * st
+    return True
+
+
 def _same_rows(a: torch.Tensor, b: torch.Tensor) -> bool:
     return a.data_ptr() == b.data_ptr() and all(x == y or n < 2 for x, y, n in zip(a.stride(), b.stride(), a.shape))
 
@@ -1755,7 +1765,7 @@ def rotary_embed(q: torch.Tensor, k: torch.Tensor | None = None, *, inv_freq: to
             o = torch.empty_like(t, memory_format=torch.contiguous_format)
         elif o.shape != t.shape or o.dtype != dtype or o.device != device or (D > 1 and o.stride(3) != 1):
             raise ValueError(f"{name}: the output for {what} must be {tuple(t.shape)} in {dtype} on {device} with adjacent channels")
-        elif any(n > 1 and st == 0 for n, st in zip(o.shape, o.stride())):
+        elif not _rows_apart(o):
             raise ValueError(f"{name}: rows of the output for {what} share memory")
         return t, o
 
