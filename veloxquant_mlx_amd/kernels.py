@@ -1568,11 +1568,12 @@ def _store_attend(name, maps, q, prefix, own, scale, causal, seq_lens, sliding_w
                                   (tail, tail2, "plain rows' dtype")):
             if mine is not None and other is not None and mine != other:
                 raise ValueError(f"{name}: the prefix and the sequences' own slots differ in {what}")
-        heads, channels, packed, tail = heads or h2, channels or c2, packed or packed2, tail or tail2
+        heads, channels = (h2, c2) if heads is None else (heads, channels)
+        packed, tail = packed or packed2, tail or tail2
         keep += keep2
     if heads is None:
         raise ValueError(f"{name}: no key/value slots to attend to")
-    if channels != D or Hq % heads:
+    if not heads or channels != D or Hq % heads:
         raise ValueError(f"{name}: q {tuple(q.shape)} over {heads} kv heads of {channels} channels")
     if q.numel() == 0:
         return out
