@@ -148,3 +148,20 @@ def test_the_append_refuses_buffers_of_other_rows():
             call(tails(), 32, packed(), spare)
     with pytest.raises(RuntimeError, match="no CPU path"):   # (buffers that fit)
         call(tails(), 32, packed(), tails())
+
+
+def test_a_shared_cache_refuses_values_unlike_the_keys(writes):
+    """Before anything is counted: the cache goes on as it was."""
+    cache = _cache()
+    cache.state = (_rows(1, 2, 9, 128), _rows(1, 2, 9, 128))
+    shared = cache.share()
+    good = _rows(3, 2, 5, 128)
+    shared.update_and_fetch(good, good)
+    for S in (5, 1):
+        k = _rows(3, 2, S, 128)
+        for v in (_rows(3, 2, S + 1, 128), _rows(1, 2, S, 128), _rows(3, 1, S, 128), _rows(3, 2, S, 64), k[0], k.bfloat16()):
+            with pytest.raises(ValueError, match="as the prefix is"):
+                shared.update_and_fetch(k, v)
+    assert shared.offset == 14 and len(writes) == 1
+    shared.update_and_fetch(good, good)
+    assert shared.offset == 19

@@ -77,7 +77,8 @@ class SharedPrefixKIVICache:
         """Append ``[B,H,S,D]`` keys and values to the sequences' own tokens, quantised as they age as in any
         :class:`KIVIKVCache`; returns zero-stride placeholders of the whole length."""
         dtype = self._prefix._tail_k.dtype if self._prefix_args["n_tail"] else keys.dtype
-        if keys.ndim != 4 or keys.shape[1] != self._kv_heads or keys.shape[3] != self._head_dim or keys.dtype != dtype or values.dtype != dtype:
+        if (keys.ndim != 4 or keys.shape[1] != self._kv_heads or keys.shape[3] != self._head_dim or values.shape != keys.shape
+                or keys.dtype != dtype or values.dtype != dtype):
             raise ValueError(f"SharedPrefixKIVICache.update_and_fetch: keys and values must be [B, {self._kv_heads}, S, {self._head_dim}] {dtype} "
                              f"as the prefix is, got {tuple(keys.shape)} {keys.dtype} and {tuple(values.shape)} {values.dtype}")
         if self._own.offset and keys.shape[0] != self._own._shape_bhd[0]:
