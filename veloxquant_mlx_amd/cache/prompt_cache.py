@@ -20,7 +20,11 @@ _FORMAT = "veloxquant-prompt-cache-1"
 
 
 def save_prompt_cache(path: str, caches: Sequence, metadata: dict | None = None) -> None:
-    """Write ``[c.state for c in caches]`` and their ``meta_state`` to ``path``."""
+    """Write ``[c.state for c in caches]`` and their ``meta_state`` to ``path``.  Sequences behind a shared prefix are not
+    saved (the cache that the prefix was shared from is, and is shared again)."""
+    for i, c in enumerate(caches):
+        if not hasattr(c, "state"):
+            raise ValueError(f"save_prompt_cache: layer {i} is a {type(c).__name__}, which has no state to save")
     tensors: dict[str, torch.Tensor] = {}
     layers = []
     for i, c in enumerate(caches):

@@ -25,8 +25,8 @@ class SharedPrefixKIVICache:
 
     The prefix is a copy of the cache's tokens at that time and does not change any more; several objects may stand on one
     (:meth:`branch`).  A cache of its own in every other respect: ``update_and_fetch``, ``fused_sdpa``, ``trim`` (of the own tokens),
-    ``offset``, ``nbytes``.  ``fused_sdpa_max_ctx`` bounds prefix and own tokens together (the own packed store is sized by what
-    the prefix leaves)."""
+    ``offset``, ``nbytes``; but no ``state``: a prompt-cache file holds the cache that was shared.  ``fused_sdpa_max_ctx`` bounds
+    prefix and own tokens together (the own packed store is sized by what the prefix leaves)."""
 
     _memory_bound = True   # attention goes through fused_sdpa; update_and_fetch returns placeholders
 
