@@ -118,7 +118,9 @@ __device__ __forceinline__ float sp_max3(float x, float y, float z) {
 // a choice between two values (between two places, as `c ? x : y` may become, it would move both to scratch memory)
 template <typename T> __device__ __forceinline__ T sp_pick(bool c, T x, T y) { return c ? x : y; }
 
-__device__ __forceinline__ u32 sp_bf16_to_f16(u32 x) { return as_u(f16x2{(f16)bf16_to_f32((u16)x), (f16)bf16_to_f32((u16)(x >> 16))}); }
+// bf16 as fp16, two at a time: magnitudes above 65504 as 65504, what is not finite as it is
+__device__ __forceinline__ f16 sp_fp16_of(float v) { return (f16)(__builtin_fabsf(v) < INFINITY ? __builtin_amdgcn_fmed3f(v, -65504.f, 65504.f) : v); }
+__device__ __forceinline__ u32 sp_bf16_to_f16(u32 x) { return as_u(f16x2{sp_fp16_of(bf16_to_f32((u16)x)), sp_fp16_of(bf16_to_f32((u16)(x >> 16)))}); }
 __device__ __forceinline__ u32x4 sp_bf16_to_f16(u32x4 x) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[i] = sp_bf16_to_f16(x[i]);
@@ -495,8 +497,8 @@ template <int BITS, typename T, int D, int MAPS, int WT> __device__ __forceinlin
 #pragma unroll 1
                     for (int x = tid; x < UNIT * CH; x += SP_THREADS) {
                         const int t = x / CH, p = x % CH, r = t < live ? t : live - 1;
-                        *(f16x8 *)(lds + t * D * 2 + sp_kpiece<D>(t, p) * 16) = ld_tail8(kb + r * ks, 8 * p, true);
-                        *(f16x8 *)(lds + Tile::KEYS + t * D * 2 + sp_vpiece<D>(t, p) * 16) = ld_tail8(vb + r * vs, 8 * p, true);
+                        *(u32x4 *)(lds + t * D * 2 + sp_kpiece<D>(t, p) * 16) = sp_bf16_to_f16(*(const u32x4 *)(kb + r * ks + 16 * p));
+                        *(u32x4 *)(lds + Tile::KEYS + t * D * 2 + sp_vpiece<D>(t, p) * 16) = sp_bf16_to_f16(*(const u32x4 *)(vb + r * vs + 16 * p));
                     }
                     kb += UNIT * ks;
                     vb += UNIT * vs;
