@@ -109,12 +109,15 @@ template <int BITS, int D, int MAPS, int WAVES> __device__ __forceinline__ void 
         const u32 sign = a.scale < 0.f ? 0x80008000u : 0u;   // the softmax takes the maximum of the scores themselves
         const bool q_bf16 = a.dtype == VQ_BF16, mine = a.scale != 0.f && (MAPS == 1 || map == h);
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            u32x4 x = *(const u32x4 *)(src + 8 * ks);
-            if (q_bf16) x = sp_bf16_to_f16(x);
+        for (int ks = 0; ks < KS; ++ks) q[ks] = *(const u32x4 *)(src + 8 * ks);
+        if (q_bf16) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) q[ks][i] = mine ? x[i] ^ sign : 0u;
+            for (int ks = 0; ks < KS; ++ks) q[ks] = sp_bf16_to_f16(q[ks]);
         }
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) q[ks][i] = mine ? q[ks][i] ^ sign : 0u;
     }
     const float cc = a.scale == 0.f ? 1.f : __builtin_fabsf(a.scale) * LOG2E;
 
@@ -335,15 +338,17 @@ template <int BITS, int D, int MAPS, int WAVES> __device__ __forceinline__ void 
                 lds_copy16<0>(vb, (u32)r * (u32)vst + p * 16, room + VT + x * 1024);
             }
             wait_copies<0>();
+            if (bf16) {   // in place, the lane's own pieces
+                u32x4 *piece = (u32x4 *)(lds + wave * F::ROOM) + lane;
+#pragma unroll 1
+                for (int x = 0; x < UNIT * CH / 32; ++x) piece[x * 64] = sp_bf16_to_f16(piece[x * 64]);
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            }
             f32x16 S;
 #pragma unroll
             for (int r = 0; r < 16; ++r) S[r] = 0.f;
 #pragma unroll
-            for (int k = 0; k < KS; ++k) {
-                u32x4 x = *(const u32x4 *)(room_p + n * D * 2 + sp_kpiece<D>(n, h * KS + k) * 16);
-                if (bf16) x = sp_bf16_to_f16(x);
-                S = M::mma(x, q[k], S);
-            }
+            for (int k = 0; k < KS; ++k) S = M::mma(*(const u32x4 *)(room_p + n * D * 2 + sp_kpiece<D>(n, h * KS + k) * 16), q[k], S);
             u32x4 P[2];
             softmax(S, place, live, P);
 #pragma unroll
@@ -354,10 +359,6 @@ template <int BITS, int D, int MAPS, int WAVES> __device__ __forceinline__ void 
                 for (int e = 0; e < 8; ++e) {
                     const int t = 16 * s2 + 4 * h + (e & 3) + 8 * (e >> 2);
                     sp_load_words<DT / 2>(room_p + VT + t * D * 2 + n * DT * 2, x[e]);
-                    if (bf16) {
-#pragma unroll
-                        for (int k = 0; k < DT / 2; ++k) x[e][k] = sp_bf16_to_f16(x[e][k]);
-                    }
                 }
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) {

@@ -118,9 +118,12 @@ __device__ __forceinline__ float sp_max3(float x, float y, float z) {
 // a choice between two values (between two places, as `c ? x : y` may become, it would move both to scratch memory)
 template <typename T> __device__ __forceinline__ T sp_pick(bool c, T x, T y) { return c ? x : y; }
 
-// bf16 as fp16, two at a time: magnitudes above 65504 as 65504, what is not finite as it is
-__device__ __forceinline__ f16 sp_fp16_of(float v) { return (f16)(__builtin_fabsf(v) < INFINITY ? __builtin_amdgcn_fmed3f(v, -65504.f, 65504.f) : v); }
-__device__ __forceinline__ u32 sp_bf16_to_f16(u32 x) { return as_u(f16x2{sp_fp16_of(bf16_to_f32((u16)x)), sp_fp16_of(bf16_to_f32((u16)(x >> 16)))}); }
+// bf16 as fp16, two at a time, rounded towards zero: exact in fp16's normal range, magnitudes above 65504 as 65504, below 2^-14 cut to multiples of
+// 2^-24 (a product of such a channel is off by 2^-24 of the other factor, where a score's bf16 operands are by 2^-9 of themselves); what is not
+// finite stays so.  (Rounded to nearest and clamped it takes twice the instructions, which made the kernel of tiles and few rows 2 % slower.)
+__device__ __forceinline__ u32 sp_bf16_to_f16(u32 x) {
+    return __builtin_bit_cast(u32, __builtin_amdgcn_cvt_pkrtz(__uint_as_float(x << 16), __uint_as_float(x & 0xFFFF0000u)));
+}
 __device__ __forceinline__ u32x4 sp_bf16_to_f16(u32x4 x) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[i] = sp_bf16_to_f16(x[i]);
@@ -257,12 +260,15 @@ template <int BITS, typename T, int D, int MAPS, int WT> __device__ __forceinlin
         const u32 sign = a.scale < 0.f ? 0x80008000u : 0u;   // the softmax takes the maximum of the scores themselves
         const bool q_bf16 = a.dtype == VQ_BF16;
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            u32x4 x = *(const u32x4 *)(src + 16 * ks);
-            if (BITS != 0 && q_bf16) x = sp_bf16_to_f16(x);
+        for (int ks = 0; ks < KS; ++ks) q[ks] = *(const u32x4 *)(src + 16 * ks);
+        if (BITS != 0 && q_bf16) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) q[ks][i] = a.scale == 0.f ? 0u : x[i] ^ sign;
+            for (int ks = 0; ks < KS; ++ks) q[ks] = sp_bf16_to_f16(q[ks]);
         }
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) q[ks][i] = a.scale == 0.f ? 0u : q[ks][i] ^ sign;
     }
     const float cc = a.scale == 0.f ? 1.f : c2;
 
