@@ -579,15 +579,22 @@ typedef struct vq_store_attend_args {
 } vq_store_attend_args;
 
 /* softmax(scale q k^T) v of every sequence's queries over [prefix | its own slots], GQA by repeat-interleave, queries aligned to
- * the end.  The prefix is read once for the whole batch: its keys and values meet the query rows of all sequences that
- * share a kv head as one matrix product; each sequence's own slots meet its own rows, and the parts are merged.  No
- * counterpart in the reference (a batch over one prompt holds the prompt once a sequence there). */
+ * the end.  The prefix is held once for the whole batch.  Where the matrix units take the call (D of 64, 128 or 256, rows
+ * of 16 bits, 2- or 4-bit slots in groups of 32, 64 or 128 with fp16 scales and token-packed values) and a sequence has up to
+ * 64 rows a kv head (queries times query heads), the prefix meets the rows of all sequences as one matrix product, read
+ * once a tile of them (128 rows, or 32 where they are few), each sequence's own slots meet its own rows, and the parts are
+ * merged.  Longer chunks, and calls so short that they need no parts, walk [prefix | own slots] a sequence; other sizes,
+ * types and layouts a query row, in float32, which is an order of magnitude slower.  Over packed slots the matrix units
+ * work in fp16: bf16 queries and plain rows count as fp16 numbers there, magnitudes above 65504 as 65504.  out may be q;
+ * else it lies apart from every input.  No counterpart in the reference (a batch over one prompt holds the prompt once a
+ * sequence there). */
 size_t vq_shared_prefix_attend_workspace(const vq_store_attend_args *a);
 int vq_shared_prefix_attend(const vq_store_attend_args *a);
 
 /* (softmax(scale q1 k1^T) - lam softmax(scale q2 k2^T)) v with q1, k1 the first and q2, k2 the second D / 2 channels of the
  * rows, v of D channels; then gain * o, or with a norm_weight gain * norm_weight * o / sqrt(mean(o^2) + norm_eps) over a
- * head's channels.  Both maps' scores and sums are formed in one pass over the slots.  No counterpart in the reference. */
+ * head's channels.  Both maps' scores and sums are formed in one pass over the slots; kernels, types and out as for
+ * vq_shared_prefix_attend.  No counterpart in the reference. */
 size_t vq_differential_attend_workspace(const vq_store_attend_args *a);
 int vq_differential_attend(const vq_store_attend_args *a);
 
@@ -598,8 +605,9 @@ enum { VQ_ROTARY_HALF = 0 /* pairs (i, i + dims/2) */, VQ_ROTARY_INTERLEAVED = 1
 /* Queries and keys of S consecutive slots of B sequences turned by their positions, in one launch: channel pair i of a row at
  * position p by the angle p * inv_freq[i] (formed in double), times attention_factor; channels dims .. D - 1 pass through.
  * x[0] / x[1]: queries and keys (heads[w] == 0: none), [B, heads[w], S, D] with element strides x_strides[w] = {batch, head,
- * token} and contiguous channels; out[w] likewise, either the very rows of x[w] (same address and strides) or apart from
- * every input and from the other output.  inv_freq: device, dims / 2 angular frequencies, VQ_F64 or VQ_F32.  The position
+ * token} and contiguous channels; out[w] likewise, its rows apart from each other, and either the very rows of x[w] (same
+ * address and strides) or sharing no byte with an input's; never with the other output's or the other input's rows (rows
+ * that lie between each other, as views of one projection do, share none).  inv_freq: device, dims / 2 angular frequencies, VQ_F64 or VQ_F32.  The position
  * of row (b, s) is offset + positions[b * pos_stride_b + s * pos_stride_s] (positions device, VQ_I32 or VQ_I64, or NULL: 0)
  * + s where add_index is set.  inverse: turns back (the transposed map times attention_factor).  The calls a host model makes of
  * its rotary embedding in front of update_and_fetch; no counterpart in the reference, whose caches take keys already turned

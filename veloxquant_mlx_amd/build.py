@@ -32,7 +32,9 @@ def sources() -> list[str]:
 
 # Kernels that account for their own global-to-LDS copies with the outstanding-load counter: a
 # register spilled to scratch memory would be reloaded with a vector load the accounting does
-# not know, so these sources must compile without scratch.
+# not know, so these sources must compile without scratch.  (Such loads make a counted wait longer, never too short: accesses to
+# memory leave the counter in the order they were issued.  The tiles of attend_span_mfma.hpp with heads of 256 channels, whose
+# accumulators and queries fill the registers, are built with 23 to 59 spilled ones and lose overlap by it, no copy.)
 NO_SCRATCH = ("attend_mfma_packed_",)
 
 

@@ -2,7 +2,8 @@
 
 Many sequences that start with the same tokens (a system prompt, a document asked about more than once, samples of one prompt) hold
 those tokens once: the prefix, packed, for a batch of one, and behind it every sequence's own tokens in a memory-bound
-:class:`KIVIKVCache`.  Attention reads the prefix once for all of them (:func:`veloxquant_mlx_amd.kernels.shared_prefix_attend`)::
+:class:`KIVIKVCache`.  Attention of few tokens a sequence reads the prefix for all of them together
+(:func:`veloxquant_mlx_amd.kernels.shared_prefix_attend`, which names the stores it does so for; longer chunks read it a sequence)::
 
     cache.update_and_fetch(k, v)           # the prompt, a batch of one
     shared = cache.share()

@@ -475,8 +475,8 @@ __global__ __launch_bounds__((64 * WAVES)) __attribute__((amdgpu_waves_per_eu(D 
     span_few_block<BITS, D, MAPS, WAVES>(c, (int)blockIdx.x);
 }
 
-// Blocks of a prefix in tiles and behind them blocks of own slots, which share the CUs with them (in two launches 184 us for 128 sequences of
-// 1k slots on a prefix of 32k, together 171; the kinds in turn 226, as a CU then holds two of one kind).
+// Blocks of a prefix in tiles and behind them blocks of own slots, which share the CUs with them (128 sequences of 1k slots on a prefix of 32k:
+// 184 us in two launches, 161 together; with the kinds in turn a CU held two of one kind, 55 us more than behind each other).
 template <int BITS, int D> __global__ __launch_bounds__(SP_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2))) void span_both_kernel(SpanCall c) {
     const int id = (int)blockIdx.x, tiles = span_shared_blocks(c);
     if (id < tiles) span_mfma_block<BITS, f16, D, 1>(c, id);

@@ -1629,7 +1629,7 @@ def shared_prefix_attend(q: torch.Tensor, prefix: dict, *, k_packed=None, k_scal
                          v_tail=None, n_tail: int = 0, scale: float = 1.0, causal: bool = False, seq_lens: torch.Tensor | None = None,
                          sliding_window: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
     """softmax(q k^T * scale) v for a batch whose sequences share a prefix: sequence ``b`` attends over ``[prefix | its own
-    slots]``, and the prefix is read once for all of them.
+    slots]``, and the prefix is held once for all of them.
 
     q ``[B,Hq,Sq,D]`` (``D`` up to 256); ``prefix``: the cache arguments of :func:`kivi_packed_attend` (``k_packed`` .. ``n_tail``) for a batch
     of one; the same arguments of this call are the sequences' own slots, for a batch of ``B`` (``n_packed = n_tail = 0``: none yet).
@@ -1639,8 +1639,14 @@ def shared_prefix_attend(q: torch.Tensor, prefix: dict, *, k_packed=None, k_scal
     ``seq_lens`` (int64 ``[B]`` on the device): live own slots of every sequence (right-padded rows past them are never
     read; with fewer than ``Sq`` the first queries stand inside the prefix).  ``sliding_window > 0``: a query sees only that many last
     slots up to its own position.  Scores and sums are float32; fp16 / bf16 rows meet as matrix products of that type
-    (weights rounded to it; fp16 over packed slots).  A row that sees nothing is zero.  A value that is not finite makes every row NaN
-    whose block holds its slot, seen or not, as in the plain product."""
+    (weights rounded to it; fp16 over packed slots, where bf16 queries and plain rows count as fp16 numbers, magnitudes above 65504 as
+    65504).  A row that sees nothing is zero.  A value that is not finite makes every row NaN whose block holds its slot, seen or not, as
+    in the plain product.  ``out`` (contiguous, as ``q``) may be ``q`` itself; else it lies apart from every input.
+
+    With heads of 64, 128 or 256 channels, 16-bit rows and 2- or 4-bit slots (groups of 32, 64 or 128, float16 scales, values packed by
+    token) and up to 64 rows a sequence and kv head (``Sq * Hq / Hkv``) the prefix meets the rows of all sequences together, read once a
+    tile of 128 of them (32 where they are few).  Longer chunks walk it a sequence and tile; other stores and types a query row, an
+    order of magnitude slower."""
     own = dict(k_packed=k_packed, k_scale=k_scale, k_zero=k_zero, v_packed=v_packed, v_scale=v_scale, v_zero=v_zero, n_packed=n_packed,
                bits=bits, group_size=group_size, v_layout=v_layout, k_tail=k_tail, v_tail=v_tail, n_tail=n_tail)
     return _store_attend("shared_prefix_attend", 1, q, prefix, own, scale, causal, seq_lens, sliding_window, out)
@@ -1658,7 +1664,7 @@ def differential_attend(q: torch.Tensor, lam: torch.Tensor | float, *, k_packed=
     q ``[B,Hq,Sq,D]``; slots, masks and lengths as for :func:`shared_prefix_attend` (own slots only; plain keys and values are
     ``k_tail`` / ``v_tail``).  ``lam``: float32 ``[Hq]`` or of one value on the device, or a number.  The result is scaled by ``gain``; with
     ``norm_weight`` (``[D]``) every head's output is first divided by ``sqrt(mean(o^2) + norm_eps)`` and multiplied by it, which is the
-    layer's head norm (``gain = 1 - lambda_init``).  Both maps' weights and sums are formed in one pass over the slots."""
+    layer's head norm (``gain = 1 - lambda_init``).  Both maps' weights and sums are formed in one pass over the slots.  ``out`` may be ``q``."""
     own = dict(k_packed=k_packed, k_scale=k_scale, k_zero=k_zero, v_packed=v_packed, v_scale=v_scale, v_zero=v_zero, n_packed=n_packed,
                bits=bits, group_size=group_size, v_layout=v_layout, k_tail=k_tail, v_tail=v_tail, n_tail=n_tail)
     return _store_attend("differential_attend", 2, q, None, own, scale, causal, seq_lens, sliding_window, out, lam, norm_weight, norm_eps,
@@ -1718,8 +1724,8 @@ def rotary_embed(q: torch.Tensor, k: torch.Tensor | None = None, *, inv_freq: to
     (an int, or an int32 / int64 tensor ``[B]`` or of one element on the device), or at ``positions[b, s]`` (int32 / int64,
     ``[S]``, ``[B,S]`` or ``[1,S]``, on the device; then ``offset`` is an int that is added).  Angles are formed in
     float64, so far positions keep theirs.  ``out`` / ``k_out`` receive the rows (any strides over adjacent channels; the input
-    itself, to turn in place, or memory apart from both inputs and the other output: rows of a cache, for one); new tensors
-    are contiguous.  ``inverse=True`` turns back; times ``attention_factor`` that is the transposed map, the gradient of the
+    itself, to turn in place, or rows that share no memory with each other, with both inputs and the other output: those of a
+    cache, or others of the same projection); new tensors are contiguous.  ``inverse=True`` turns back; times ``attention_factor`` that is the transposed map, the gradient of the
     forward call (this package's functions record none)."""
     name = "rotary_embed"
     if q.ndim != 4 or (k is not None and k.ndim != 4):
