@@ -1682,19 +1682,35 @@ def _extent(t: torch.Tensor) -> tuple[int, int]:
 
 
 def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether two (non-empty) strided tensors certainly share no byte: their extents lie apart, or do so modulo one of their strides (views
+    """Whether two (non-empty) strided 4D tensors certainly share no byte: their extents lie apart, or do so modulo one of their strides (views
     of one projection, whose rows alternate: modulo a token's stride each is one stretch)."""
     (a0, a1), (b0, b1) = _extent(a), _extent(b)
     if a1 <= b0 or b1 <= a0:
         return True
-    sides = [[(n, st * t.element_size()) for n, st in zip(t.shape, t.stride()) if n > 1 and st > 0] for t in (a, b)]
-    for m in {st for side in sides for _, st in side}:
-        # a dimension whose stride is a multiple of m stays where it is, the others take up a stretch
-        wide = [t.element_size() + sum((n - 1) * st for n, st in side if st % m) for t, side in zip((a, b), sides)]
-        off = (b0 - a0) % m
-        if wide[0] <= off and off + wide[1] <= m:
-            return True
+    ea, eb = a.element_size(), b.element_size()
+    off = b0 - a0
+    tried = {0}
+    for t, e in ((a, ea), (b, eb)):
+        shape, strides = t.shape, t.stride()
+        for d in (2, 0, 1, 3):   # (tokens and sequences first: of views of one projection these tell)
+            m = strides[d] * e
+            if shape[d] < 2 or m in tried:
+                continue
+            tried.add(m)
+            at = off % m
+            if _stretch(a, ea, m) <= at and at + _stretch(b, eb, m) <= m:
+                return True
     return False
+
+
+def _stretch(t: torch.Tensor, size: int, m: int) -> int:
+    """Bytes that a tensor's rows span modulo ``m``: a dimension whose stride is a multiple of it stays where it is."""
+    reach = size
+    for n, st in zip(t.shape, t.stride()):
+        st *= size
+        if st % m:
+            reach += (n - 1) * st
+    return reach
 
 
 def _rows_apart(t: torch.Tensor) -> bool:
