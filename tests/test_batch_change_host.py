@@ -165,3 +165,14 @@ def test_a_shared_cache_refuses_values_unlike_the_keys(writes):
     assert shared.offset == 14 and len(writes) == 1
     shared.update_and_fetch(good, good)
     assert shared.offset == 19
+
+
+def test_no_tokens_are_appended_to_a_shared_cache(writes):
+    """A chunk of length zero, before any own token and behind some."""
+    cache = _cache()
+    cache.state = (_rows(1, 2, 9, 128), _rows(1, 2, 9, 128))
+    shared = cache.share()
+    none, some = _rows(3, 2, 0, 128), _rows(3, 2, 5, 128)
+    for x, n in ((none, 0), (some, 5), (none, 5), (some, 10)):
+        k, v = shared.update_and_fetch(x, x)
+        assert k.shape == v.shape == (3, 2, 9 + n, 128) and shared.offset == 9 + n

@@ -84,8 +84,8 @@ class SharedPrefixKIVICache:
                              f"as the prefix is, got {tuple(keys.shape)} {keys.dtype} and {tuple(values.shape)} {values.dtype}")
         if self._own.offset and keys.shape[0] != self._own._shape_bhd[0]:
             raise ValueError(f"SharedPrefixKIVICache.update_and_fetch: {keys.shape[0]} sequences, this cache holds {self._own._shape_bhd[0]}")
-        z = self._own.update_and_fetch(keys, values)[0]
-        z = z[:, :, :1].expand(keys.shape[0], self._kv_heads, self.offset, self._head_dim)
+        self._own.update_and_fetch(keys, values)
+        z = self._own._zero_scalar.expand(keys.shape[0], self._kv_heads, self.offset, self._head_dim)
         return z, z
 
     def fused_sdpa(self, q: torch.Tensor, scale: float, *, causal: bool = True, sliding_window: int = 0,
