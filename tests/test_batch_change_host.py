@@ -176,3 +176,17 @@ def test_no_tokens_are_appended_to_a_shared_cache(writes):
     for x, n in ((none, 0), (some, 5), (none, 5), (some, 10)):
         k, v = shared.update_and_fetch(x, x)
         assert k.shape == v.shape == (3, 2, 9 + n, 128) and shared.offset == 9 + n
+
+
+def test_a_restored_prefix_of_paired_heads_takes_its_keys(writes):
+    """Restored without its meta_state it holds 5 or 6 heads; keys of neither leave it as it is."""
+    cache = _cache(head_dim=64)
+    cache.state = (_rows(1, 3, 9, 128), _rows(1, 3, 9, 128))      # three pairs
+    for H in (5, 6):
+        shared = cache.share()
+        for bad in (10, 4, 12, 3):
+            with pytest.raises(ValueError, match="as the prefix is"):
+                shared.update_and_fetch(_rows(2, bad, 1, 64), _rows(2, bad, 1, 64))
+        assert shared.update_and_fetch(_rows(2, H, 4, 64), _rows(2, H, 4, 64))[0].shape == (2, H, 13, 64)
+        with pytest.raises(ValueError, match="as the prefix is"):
+            shared.update_and_fetch(_rows(2, 11 - H, 1, 64), _rows(2, 11 - H, 1, 64))

@@ -74,10 +74,18 @@ class SharedPrefixKIVICache:
     def empty(self) -> bool:
         return False
 
+    def _heads_under(self, heads: int) -> int:
+        """The kv head count under ``heads`` of keys or queries.  A prefix restored without its ``meta_state`` shows pairs of heads, not whether
+        the last one is whole: one head less where the heads do not divide over an even count, as in :class:`KIVIKVCache`."""
+        H = self._kv_heads
+        return H - 1 if self._prefix._kv_heads < 0 and H % 2 == 0 and H > 2 and heads % H and heads % (H - 1) == 0 else H
+
     def update_and_fetch(self, keys: torch.Tensor, values: torch.Tensor):
         """Append ``[B,H,S,D]`` keys and values to the sequences' own tokens, quantised as they age as in any
         :class:`KIVIKVCache`; returns zero-stride placeholders of the whole length."""
         dtype = self._prefix._tail_k.dtype if self._prefix_args["n_tail"] else keys.dtype
+        if keys.ndim == 4 and self._own.offset == 0 and keys.shape[1] == self._heads_under(keys.shape[1]):
+            self._kv_heads = keys.shape[1]
         if (keys.ndim != 4 or keys.shape[1] != self._kv_heads or keys.shape[3] != self._head_dim or values.shape != keys.shape
                 or keys.dtype != dtype or values.dtype != dtype):
             raise ValueError(f"SharedPrefixKIVICache.update_and_fetch: keys and values must be [B, {self._kv_heads}, S, {self._head_dim}] {dtype} "
@@ -98,15 +106,17 @@ class SharedPrefixKIVICache:
             if not (isinstance(lengths, torch.Tensor) and lengths.is_cuda) and min(torch.as_tensor(lengths).reshape(-1).tolist(), default=0) < self.prefix_length:
                 raise ValueError(f"{name}: lengths count the prefix of {self.prefix_length} tokens")
             lengths = batch_lengths(name, lengths, q) - self.prefix_length
-        pair = self._prefix._pair
+        pair, H = self._prefix._pair, self._kv_heads
         if pair:
-            if q.ndim != 4 or q.shape[3] != self._head_dim or q.shape[1] % self._kv_heads:
-                raise ValueError(f"{name}: q {tuple(q.shape)} over {self._kv_heads} kv heads of {self._head_dim} channels")
-            q = pad_queries_for_paired_heads(q, self._kv_heads)
+            if q.ndim == 4 and self._own.offset == 0:
+                H = self._heads_under(q.shape[1])
+            if q.ndim != 4 or q.shape[3] != self._head_dim or q.shape[1] % H:
+                raise ValueError(f"{name}: q {tuple(q.shape)} over {H} kv heads of {self._head_dim} channels")
+            q = pad_queries_for_paired_heads(q, H)
         own = self._own._store_args() if self._own.offset else {}
         out = K.shared_prefix_attend(q, self._prefix_args, **own, scale=float(scale), causal=bool(causal), seq_lens=lengths,
                                      sliding_window=int(sliding_window or 0))
-        return own_half_of_paired_output(out, self._kv_heads) if pair else out
+        return own_half_of_paired_output(out, H) if pair else out
 
     def is_trimmable(self) -> bool:
         return True
