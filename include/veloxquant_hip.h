@@ -598,6 +598,45 @@ int vq_shared_prefix_attend(const vq_store_attend_args *a);
 size_t vq_differential_attend_workspace(const vq_store_attend_args *a);
 int vq_differential_attend(const vq_store_attend_args *a);
 
+/* ---- attention over chosen blocks of a packed store ---------------------------- */
+
+/* The blocks of block_tokens packed slots (a multiple of the group) that the queries of a tile attend to, by a bound on their scores: a
+ * key group's keys lie between zero and zero + levels * scale in every channel, so sum_c max(q_c zero_c, q_c (zero_c + levels
+ * scale_c)) bounds its products with a query; a block's score is the largest bound over its groups, the query heads of the kv head
+ * and the queries of the tile (query_block consecutive ones choose together, the last tile fewer), of the groups that a query sees.
+ * Query i of Sq stands at slot n - Sq + i of the sequence's n live slots (n_packed + n_tail, or seq_lens); causal hides the slots
+ * behind it.  Of the blocks that the tile's last query sees all are chosen if they are `count` at most; else the first `first`, the
+ * last `recent` and the best of the others.  Scores are formed in 64 bits, equal ones go to the lower block, NaN above all.  out:
+ * int32 [B, Hkv, tiles, count], ascending, -1 behind the chosen where fewer are visible.  No counterpart in the reference. */
+typedef struct vq_block_select_args {
+    const void *q;                     /* [B, Hq, Sq, D] contiguous, dtype; D <= 256 */
+    const void *k_scale, *k_zero;      /* [B, Hkv, ceil(cap_tokens / group), D], meta_dtype VQ_F16 / VQ_F32 */
+    int32_t *out;
+    int64_t B, Hq, Hkv, Sq, D;
+    int64_t n_packed, cap_tokens, n_tail;
+    int64_t block_tokens, query_block, count, first, recent;
+    const int64_t *seq_lens;           /* optional, int64 [B] on the device */
+    void *workspace;                   /* vq_block_select_workspace(args) bytes, 16-byte aligned; 0: may be NULL */
+    size_t workspace_bytes;
+    void *stream;
+    int32_t dtype, meta_dtype, group, levels, causal;
+} vq_block_select_args;
+size_t vq_block_select_workspace(const vq_block_select_args *a);
+int vq_block_select(const vq_block_select_args *a);
+
+/* softmax(scale q k^T) v of every query over the slots of the blocks that its tile's list names and over all plain rows (the tail) of
+ * its sequence, causal as in vq_shared_prefix_attend.  store: its own slots only, no prefix, no window.  blocks: int32 [B, Hkv, tiles,
+ * count] on the device, tiles = ceil(Sq / query_block), entries in any order: entry e names the packed slots e * block_tokens ..
+ * (e + 1) * block_tokens - 1; what is below zero or past the live slots is nothing, an entry named twice counts twice.  Numbers, types and
+ * out as for vq_shared_prefix_attend.  No counterpart in the reference. */
+typedef struct vq_block_attend_args {
+    vq_store_attend_args store;
+    const int32_t *blocks;
+    int64_t count, block_tokens, query_block;
+} vq_block_attend_args;
+size_t vq_block_attend_workspace(const vq_block_attend_args *a);
+int vq_block_attend(const vq_block_attend_args *a);
+
 /* ---- rotary positions ------------------------------------------------------ */
 
 enum { VQ_ROTARY_HALF = 0 /* pairs (i, i + dims/2) */, VQ_ROTARY_INTERLEAVED = 1 /* pairs (2i, 2i + 1) */ };
@@ -625,6 +664,18 @@ typedef struct vq_rotary_args {
     float attention_factor;
 } vq_rotary_args;
 int vq_rotary(const vq_rotary_args *args, void *stream);
+
+/* The same behind the norm of every head's row: x_c w_c / sqrt(mean(x^2) + eps) over its D channels, then the turn (channels past dims
+ * pass through normed).  weight[w]: device, [D] (weight_stride 0) or a row a head (weight_stride the elements between them), weight_dtype
+ * VQ_F16 / VQ_BF16 / VQ_F32, or NULL for ones.  Squares, sum and turn in float32, one rounding at the end; not inverse. */
+typedef struct vq_norm_rotary_args {
+    vq_rotary_args rotary;
+    const void *weight[2];
+    int64_t weight_stride[2];
+    int32_t weight_dtype;
+    float eps;
+} vq_norm_rotary_args;
+int vq_norm_rotary(const vq_norm_rotary_args *args, void *stream);
 
 /* ---- SKVQ clipped group quantisation ------------------------------------- */
 

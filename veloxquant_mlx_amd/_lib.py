@@ -151,12 +151,43 @@ class RotaryArgs(C.Structure):
     ]
 
 
+class NormRotaryArgs(C.Structure):
+    """Mirror of ``vq_norm_rotary_args``."""
+
+    _fields_ = [("rotary", RotaryArgs), ("weight", vp * 2), ("weight_stride", i64 * 2), ("weight_dtype", i32), ("eps", f32)]
+
+
+class BlockSelectArgs(C.Structure):
+    """Mirror of ``vq_block_select_args``."""
+
+    _fields_ = [
+        ("q", vp), ("k_scale", vp), ("k_zero", vp), ("out", vp),
+        ("B", i64), ("Hq", i64), ("Hkv", i64), ("Sq", i64), ("D", i64),
+        ("n_packed", i64), ("cap_tokens", i64), ("n_tail", i64),
+        ("block_tokens", i64), ("query_block", i64), ("count", i64), ("first", i64), ("recent", i64),
+        ("seq_lens", vp), ("workspace", vp), ("workspace_bytes", sz), ("stream", vp),
+        ("dtype", i32), ("meta_dtype", i32), ("group", i32), ("levels", i32), ("causal", i32),
+    ]
+
+
+class BlockAttendArgs(C.Structure):
+    """Mirror of ``vq_block_attend_args``."""
+
+    _fields_ = [("store", StoreAttendArgs), ("blocks", vp), ("count", i64), ("block_tokens", i64), ("query_block", i64)]
+
+
 # Argument blocks packed by ``struct`` in one go, as ATTEND_PACK: x, out, heads, x_strides, out_strides, ...
 STORE_PACK = "PPPPPPqqPPqqqqqqq"   # a KVStore
 STORE_ATTEND_PACK = struct.Struct("@PPqqqqq" + 2 * STORE_PACK + "PPqPPNPqiiiiiiiifff0q")
 assert STORE_ATTEND_PACK.size == C.sizeof(StoreAttendArgs)
 ROTARY_PACK = struct.Struct("@PPPPqqqqqqqqqqqqqqqqqqPPqqqiiiiiif0q")
 assert ROTARY_PACK.size == C.sizeof(RotaryArgs)
+NORM_PACK = struct.Struct("@PPqqif")   # behind a ROTARY_PACK
+assert ROTARY_PACK.size + NORM_PACK.size == C.sizeof(NormRotaryArgs)
+BLOCK_SELECT_PACK = struct.Struct("@PPPPqqqqqqqqqqqqqPPNPiiiii0q")
+assert BLOCK_SELECT_PACK.size == C.sizeof(BlockSelectArgs)
+BLOCK_LISTS_PACK = struct.Struct("@Pqqq")   # behind a STORE_ATTEND_PACK
+assert STORE_ATTEND_PACK.size + BLOCK_LISTS_PACK.size == C.sizeof(BlockAttendArgs)
 
 
 _SIGNATURES = {
@@ -204,7 +235,12 @@ _SIGNATURES = {
     "vq_shared_prefix_attend": (i32, [C.POINTER(StoreAttendArgs)]),
     "vq_differential_attend_workspace": (sz, [C.POINTER(StoreAttendArgs)]),
     "vq_differential_attend": (i32, [C.POINTER(StoreAttendArgs)]),
+    "vq_block_select_workspace": (sz, [C.POINTER(BlockSelectArgs)]),
+    "vq_block_select": (i32, [C.POINTER(BlockSelectArgs)]),
+    "vq_block_attend_workspace": (sz, [C.POINTER(BlockAttendArgs)]),
+    "vq_block_attend": (i32, [C.POINTER(BlockAttendArgs)]),
     "vq_rotary": (i32, [C.POINTER(RotaryArgs), vp]),
+    "vq_norm_rotary": (i32, [C.POINTER(NormRotaryArgs), vp]),
     "vq_vecinfer_attend_workspace": (sz, [C.POINTER(LutAttendArgs)]),
     "vq_vecinfer_attend": (i32, [C.POINTER(LutAttendArgs)]),
     "vq_vecinfer_attend_indices_workspace": (sz, [C.POINTER(IndexAttendArgs)]),
@@ -233,9 +269,12 @@ def load():
             lib.attend_packed = C.CFUNCTYPE(i32, C.c_char_p, C.c_char_p)(("vq_kivi_attend_ext", lib))
             lib.attend_packed_workspace = C.CFUNCTYPE(sz, C.c_char_p, C.c_char_p)(("vq_kivi_attend_workspace_ext", lib))
             lib.store_attend_packed, lib.store_attend_packed_workspace = (
-                {maps: C.CFUNCTYPE(res, C.c_char_p)((f"vq_{name}_attend{tail}", lib)) for maps, name in ((1, "shared_prefix"), (2, "differential"))}
+                {maps: C.CFUNCTYPE(res, C.c_char_p)((f"vq_{name}_attend{tail}", lib)) for maps, name in ((1, "shared_prefix"), (2, "differential"), (0, "block"))}
                 for res, tail in ((i32, ""), (sz, "_workspace")))
+            lib.block_select_packed = C.CFUNCTYPE(i32, C.c_char_p)(("vq_block_select", lib))
+            lib.block_select_packed_workspace = C.CFUNCTYPE(sz, C.c_char_p)(("vq_block_select_workspace", lib))
             lib.rotary_packed = C.CFUNCTYPE(i32, C.c_char_p, vp)(("vq_rotary", lib))
+            lib.norm_rotary_packed = C.CFUNCTYPE(i32, C.c_char_p, vp)(("vq_norm_rotary", lib))
             _lib = lib
             return _lib
         except (OSError, AttributeError) as e:  # missing file or symbol

@@ -520,6 +520,54 @@ class KIVIKVCache(FP16KVCache):
                                      sliding_window=int(sliding_window or 0), norm_weight=norm_weight, norm_eps=float(norm_eps),
                                      gain=float(gain))
 
+    def _sparse_ready(self, name: str) -> None:
+        if not self._fused_enabled:
+            raise RuntimeError(f"{name} called but fused_sdpa was not enabled via KVCacheConfig.fused_sdpa=True.")
+        if self.offset == 0:
+            raise RuntimeError(f"{name} called before any tokens were cached via update_and_fetch.")
+        if self._pair:
+            raise ValueError(f"{name}: heads of 64 channels are kept in pairs; set kivi_pair_heads=False")
+        if self._extra_attend_args():
+            raise ValueError(f"{name}: a cache with rows kept outside its packed store is not taken")
+
+    def select_blocks(self, q: torch.Tensor, n_select: int, *, block_size: int | None = None, query_block: int = 1, first: int = 1,
+                      recent: int = 1, causal: bool = True, lengths: torch.Tensor | None = None) -> torch.Tensor:
+        """The ``n_select`` blocks of ``block_size`` packed tokens (a multiple of the group size, the default) that ``q [B,H_q,S_q,D]`` should
+        attend to (:func:`veloxquant_mlx_amd.kernels.select_blocks`): the first ``first``, the last ``recent`` and those whose scale and
+        zero bound the largest scores, per kv head and tile of ``query_block`` queries.  int32 ``[B, H, tiles, n_select]``."""
+        name = f"{type(self).__name__}.select_blocks"
+        self._sparse_ready(name)
+        nq = self._n_quantized
+        if nq == 0:
+            B, H, _ = self._shape_bhd
+            return torch.full((B, H, -(-q.shape[2] // int(query_block)), int(n_select)), -1, dtype=torch.int32, device=q.device)
+        if lengths is not None:
+            lengths = batch_lengths(name, lengths, q)
+        return K.select_blocks(q, self._ks, self._kz, n_select, levels=self._levels, group_size=self._group_size, n_packed=nq,
+                               n_tail=self.offset - nq, block_size=block_size, query_block=query_block, first=first, recent=recent,
+                               causal=bool(causal), seq_lens=lengths)
+
+    def fused_sparse_sdpa(self, q: torch.Tensor, scale: float, n_select: int = 0, *, blocks: torch.Tensor | None = None,
+                          block_size: int | None = None, query_block: int = 1, first: int = 1, recent: int = 1, causal: bool = True,
+                          lengths: torch.Tensor | None = None) -> torch.Tensor:
+        """Attention of ``q [B,H_q,S_q,D]`` over ``n_select`` blocks of the packed tokens, chosen as by :meth:`select_blocks` or given in
+        ``blocks``, and over all newer tokens (:func:`veloxquant_mlx_amd.kernels.block_sparse_attend`); masks and ``lengths`` as for
+        :meth:`fused_sdpa`.  Heads of 64 channels need ``kivi_pair_heads=False`` in memory-bound mode."""
+        name = f"{type(self).__name__}.fused_sparse_sdpa"
+        self._sparse_ready(name)
+        if lengths is not None:
+            lengths = batch_lengths(name, lengths, q)
+        if q.shape[2] == 1:
+            self._drop_tiles()
+        store = self._store_args()
+        if blocks is None:
+            if n_select < 1:
+                raise ValueError(f"{name}: n_select={n_select} must be at least 1, or blocks given")
+            blocks = self.select_blocks(q, n_select, block_size=block_size, query_block=query_block, first=first, recent=recent, causal=causal,
+                                        lengths=lengths)
+        return K.block_sparse_attend(q, blocks, **store, block_size=self._group_size if block_size is None else block_size, query_block=query_block,
+                                     scale=float(scale), causal=bool(causal), seq_lens=lengths)
+
     def share(self):
         """A :class:`~veloxquant_mlx_amd.cache.SharedPrefixKIVICache`: these tokens (a batch of one, memory-bound mode), copied, as the prefix
         that the sequences of a batch share."""

@@ -1,0 +1,144 @@
+// Attention over chosen blocks of a packed store and over all of its plain rows.
+//
+// Row (b, h, i) of a query sees, of the packed slots, those of the blocks that its tile's list names (tile i / query_block of its kv
+// head), each entry's slots e block .. (e + 1) block - 1 as far as they are live and not behind the query; entries below zero or past
+// the store name nothing, an entry that is named twice counts twice.  Behind them come the plain rows (the tail), up to the query's own
+// place.  o = sum p v / sum p, p = exp(scale q k - max) over what it sees; a row that sees nothing is zero.
+#include "attend_blocks.hpp"
+
+namespace vq {
+
+namespace {
+
+// Any head size up to 256, type, bit width, layout and strides, in float32 on the vector units: a wave takes a query row over a run
+// of its list's entries and a run of its tail, lanes along the channels.
+__global__ __launch_bounds__(256) void blocks_any_kernel(BlockCall c) {
+    constexpr int E = SPAN_MAX_D / 64;
+    const vq_store_attend_args &a = c.s.a;
+    const int lane = threadIdx.x & 63;
+    const int64_t wid = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (wid >= a.B * a.Hq * a.Sq * c.s.nparts) return;   // whole waves leave together
+    const int64_t row = wid / c.s.nparts, part = wid % c.s.nparts;
+    const int64_t pos = row % a.Sq, h = row / a.Sq % a.Hq, b = row / (a.Sq * a.Hq);
+    const int64_t hkv = h / (a.Hq / a.Hkv), D = a.D, bh = b * a.Hkv + hkv;
+    int64_t lo, hi;
+    span_visible(a, span_own_live(a, b), pos, lo, hi);
+    const float scale = a.scale * LOG2E;
+    const int32_t *list = c.blocks + (bh * c.tiles + pos / c.query_block) * c.count;
+
+    float q[E], acc[E], m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const int64_t d = lane + 64 * e;
+        q[e] = d < D ? span_ld(a.q, a.dtype, row * D + d) : 0.f;
+        acc[e] = 0.f;
+    }
+    const SpanPacked p = SpanPacked::of(a, a.own);
+    auto take = [&](int64_t t) {
+        float v[E], dot = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int64_t d = lane + 64 * e;
+            v[e] = 0.f;
+            if (d >= D) continue;
+            float k;
+            if (t < a.own.n_packed) {
+                k = p.key(bh, t, d);
+                v[e] = p.value(bh, t, d);
+            } else {
+                const int64_t r = t - a.own.n_packed;
+                k = span_ld(a.own.k_tail, a.tail_dtype, b * a.own.k_strides[0] + hkv * a.own.k_strides[1] + r * a.own.k_strides[2] + d);
+                v[e] = span_ld(a.own.v_tail, a.tail_dtype, b * a.own.v_strides[0] + hkv * a.own.v_strides[1] + r * a.own.v_strides[2] + d);
+            }
+            dot = __builtin_fmaf(q[e], k, dot);
+        }
+        const float x = span_wave_sum(dot) * scale, mn = fmaxf(m, x);
+        const float keep = mn == -INFINITY ? 1.f : exp2f(m - mn), y = mn == -INFINITY && x == x ? 0.f : exp2f(x - mn);
+        l = l * keep + y;
+        m = mn;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = __builtin_fmaf(y, v[e], acc[e] * keep);
+    };
+    const int64_t packed = hi < a.own.n_packed ? hi : a.own.n_packed;
+    for (int64_t i = c.count * part / c.s.nparts; i < c.count * (part + 1) / c.s.nparts; ++i) {
+        const int64_t t0 = (int64_t)list[i] * c.block_tokens;
+        if (t0 < 0) continue;
+        const int64_t t1 = t0 + c.block_tokens < packed ? t0 + c.block_tokens : packed;
+        for (int64_t t = t0; t < t1; ++t) take(t);
+    }
+    const int64_t n = hi > a.own.n_packed ? hi - a.own.n_packed : 0;
+    for (int64_t t = n * part / c.s.nparts; t < n * (part + 1) / c.s.nparts; ++t) take(a.own.n_packed + t);
+    const int64_t rec = row * c.s.nparts + part;
+    if (lane == 0) { c.s.ml[rec * 2] = m; c.s.ml[rec * 2 + 1] = l; }
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+        if (lane + 64 * e < D) c.s.sums[rec * D + lane + 64 * e] = acc[e];
+}
+
+int check_blocks(const char *fn, const vq_block_attend_args *args) {
+    VQ_REQUIRE(args != nullptr, VQ_ERR_INVALID, "%s: null argument block", fn);
+    const vq_store_attend_args &a = args->store;
+    if (int rc = span_check_call(fn, &a, 1)) return rc;
+    VQ_REQUIRE(span_prefix_slots(a) == 0, VQ_ERR_INVALID, "%s: takes no shared prefix", fn);
+    VQ_REQUIRE(a.sliding_window == 0, VQ_ERR_INVALID, "%s: takes no sliding window", fn);
+    VQ_REQUIRE(args->block_tokens >= 1 && args->block_tokens < (INT64_C(1) << 30), VQ_ERR_INVALID, "%s: bad block size", fn);
+    VQ_REQUIRE(args->query_block >= 1 && args->query_block < (INT64_C(1) << 30), VQ_ERR_INVALID, "%s: query_block must be at least 1", fn);
+    VQ_REQUIRE(args->count >= 0 && args->count < (INT64_C(1) << 30), VQ_ERR_INVALID, "%s: bad list length", fn);
+    VQ_REQUIRE(args->count == 0 || args->blocks != nullptr, VQ_ERR_INVALID, "%s: null blocks", fn);
+    return VQ_OK;
+}
+
+BlockCall cut_blocks(const vq_block_attend_args &args) {
+    BlockCall c = {};
+    c.s.a = args.store;
+    c.blocks = args.blocks;
+    c.count = args.count;
+    c.block_tokens = args.block_tokens;
+    c.query_block = args.query_block;
+    const vq_store_attend_args &a = c.s.a;
+    c.tiles = cdiv(a.Sq, c.query_block);
+    if (a.own.n_packed == 0) { c.s.a.pack_bits = 8; c.s.a.group = 1; c.count = 0; }   // fields that no packed slot reads
+    // as many waves as fill the chip eight deep, runs of 64 slots or more
+    const int64_t rows = a.B * a.Hq * a.Sq;
+    double slots = (double)c.count * (double)c.block_tokens;
+    slots = (slots < (double)a.own.n_packed ? slots : (double)a.own.n_packed) + (double)a.own.n_tail;
+    int64_t parts = 8192 / rows;
+    if ((double)parts > slots / 64.) parts = (int64_t)(slots / 64.);
+    c.s.nparts = (int)(parts < 1 ? 1 : parts);
+    return c;
+}
+
+// (the sums take whole 16 bytes, so that the pairs behind them are aligned with odd heads too)
+int64_t block_floats(const BlockCall &c, int64_t &sums) {
+    const int64_t recs = c.s.a.B * c.s.a.Hq * c.s.a.Sq * c.s.nparts;
+    sums = cdiv(recs * c.s.a.D, 4) * 4;
+    return sums + recs * 2;
+}
+
+}  // namespace
+
+}  // namespace vq
+
+extern "C" size_t vq_block_attend_workspace(const vq_block_attend_args *args) {
+    using namespace vq;
+    if (check_blocks("vq_block_attend", args) != VQ_OK) return 0;
+    int64_t sums;
+    return (size_t)block_floats(cut_blocks(*args), sums) * 4;
+}
+
+extern "C" int vq_block_attend(const vq_block_attend_args *args) {
+    using namespace vq;
+    const char *fn = "vq_block_attend";
+    if (int rc = check_blocks(fn, args)) return rc;
+    BlockCall c = cut_blocks(*args);
+    const vq_store_attend_args &a = c.s.a;
+    int64_t sums;
+    const size_t need = (size_t)block_floats(c, sums) * 4;
+    VQ_REQUIRE(a.workspace != nullptr && a.workspace_bytes >= need && ((uintptr_t)a.workspace & 15) == 0, VQ_ERR_WORKSPACE,
+               "%s: workspace of %zu bytes required, 16-byte aligned", fn, need);
+    c.s.sums = (float *)a.workspace;
+    c.s.ml = c.s.sums + sums;
+    blocks_any_kernel<<<(unsigned)cdiv(a.B * a.Hq * a.Sq * c.s.nparts, 4), 256, 0, (hipStream_t)a.stream>>>(c);
+    VQ_HIP_CHECK_LAUNCH(fn);
+    return launch_span_merge1(fn, c.s);
+}

@@ -1,0 +1,14 @@
+// A call of attention over chosen blocks of a packed store (attend_blocks.hip) and how it is cut: the store, parts and scratch of
+// attention over spans (attend_span.hpp; one map, no prefix, no window), and the lists of blocks.
+#pragma once
+#include "attend_span.hpp"
+
+namespace vq {
+
+struct BlockCall {
+    SpanCall s;
+    const int32_t *blocks;   // [B][Hkv][tiles][count]
+    int64_t tiles, count, block_tokens, query_block;
+};
+
+}  // namespace vq

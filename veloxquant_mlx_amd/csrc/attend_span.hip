@@ -6,32 +6,6 @@ namespace vq {
 
 namespace {
 
-constexpr int SPAN_MAX_D = 256;
-
-// One element of a packed store's key or value as the fp16 number it stands for.
-struct SpanPacked {
-    const vq_kv_store *s;
-    int bits, per, group, meta, v_layout;
-    uint32_t mask;
-    int64_t D, W, GV, GK;
-    __device__ __forceinline__ float fp16_of(uint32_t word, int slot, const void *scale, const void *zero, int64_t at) const {
-        const float code = (float)((word >> (slot * bits)) & mask);
-        return (float)(f16)__builtin_fmaf(code, span_ld(scale, meta, at), span_ld(zero, meta, at));
-    }
-    __device__ __forceinline__ float key(int64_t bh, int64_t t, int64_t d) const {
-        const uint32_t w = ((const uint32_t *)s->k_packed)[(bh * s->cap_tokens + t) * W + d / per];
-        return fp16_of(w, (int)(d % per), s->k_scale, s->k_zero, (bh * GK + t / group) * D + d);
-    }
-    __device__ __forceinline__ float value(int64_t bh, int64_t t, int64_t d) const {
-        if (v_layout == VQ_V_CHANNEL_PACKED) {
-            const uint32_t w = ((const uint32_t *)s->v_packed)[(bh * s->cap_tokens + t) * W + d / per];
-            return fp16_of(w, (int)(d % per), s->v_scale, s->v_zero, (bh * s->cap_tokens + t) * GV + d / group);
-        }
-        const uint32_t w = ((const uint32_t *)s->v_packed)[(bh * (s->cap_tokens / per) + t / per) * D + d];
-        return fp16_of(w, (int)(t % per), s->v_scale, s->v_zero, (bh * GV + d / group) * s->cap_tokens + t);
-    }
-};
-
 // Any head size up to 256, type, bit width, layout and strides, in float32 on the vector units: a wave takes a query row over
 // a run of its slots, lanes along the channels.  For the shapes that the matrix-unit kernel does not take (float32 rows,
 // head sizes other than 64, 128 and 256, fields of 1, 3 and 5 to 8 bits, groups of 16, channel-packed values, float32 scale and zero).
@@ -69,10 +43,7 @@ template <int MAPS> __global__ __launch_bounds__(256) void span_any_kernel(SpanC
         const bool shared = g < before;
         const vq_kv_store &s = shared ? a.prefix : a.own;
         const int64_t t = shared ? g : g - before, sb = shared ? 0 : b;
-        const int per = 32 / a.pack_bits;
-        auto up = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
-        const SpanPacked p = {&s, a.pack_bits, per, a.group, a.meta_dtype, a.v_layout, (1u << a.pack_bits) - 1u, D, up(D, per),
-                              up(D, a.group), up(s.cap_tokens, a.group)};
+        const SpanPacked p = SpanPacked::of(a, s);
         float v[E], dot[MAPS];
 #pragma unroll
         for (int w = 0; w < MAPS; ++w) dot[w] = 0.f;
@@ -230,7 +201,9 @@ int check_store(const char *fn, const char *which, const vq_store_attend_args &a
     return VQ_OK;
 }
 
-int check_call(const char *fn, const vq_store_attend_args *args, int maps) {
+}  // namespace
+
+int span_check_call(const char *fn, const vq_store_attend_args *args, int maps) {
     VQ_REQUIRE(args != nullptr, VQ_ERR_INVALID, "%s: null argument block", fn);
     const vq_store_attend_args &a = *args;
     VQ_REQUIRE(a.B >= 1 && a.Hq >= 1 && a.Hkv >= 1 && a.Sq >= 1 && a.D >= 1, VQ_ERR_INVALID, "%s: bad sizes", fn);
@@ -257,6 +230,8 @@ int check_call(const char *fn, const vq_store_attend_args *args, int maps) {
     return VQ_OK;
 }
 
+namespace {
+
 SpanCall cut(const vq_store_attend_args &a, int maps) {
     SpanCall c = {};
     c.a = a;
@@ -282,15 +257,26 @@ int64_t scratch_floats(const SpanCall &c, int maps, int64_t &sums) {
 }
 
 size_t workspace(const char *fn, const vq_store_attend_args *args, int maps) {
-    if (check_call(fn, args, maps) != VQ_OK) return 0;
+    if (span_check_call(fn, args, maps) != VQ_OK) return 0;
     const SpanCall c = cut(*args, maps);
     if (c.nparts == 1 && span_mfma_supported(c.a)) return 0;
     int64_t sums;
     return (size_t)scratch_floats(c, maps, sums) * 4;
 }
 
+template <int MAPS> int launch_merge(const char *fn, const SpanCall &c) {
+    const int64_t rows = c.a.B * c.a.Hq * c.a.Sq;
+    hipStream_t st = (hipStream_t)c.a.stream;
+    // (a row to a block where its parts are many, or rows too few to fill the chip with a wave each: 512 rows of 16 parts and two maps 9.8 us, a
+    // wave each 11.1; 1920 rows of 11 parts 7.0, a wave each 5.2)
+    if (c.nparts > 2 * MERGE_AT_ONCE || (c.nparts > MERGE_AT_ONCE && rows < 1024)) span_merge_kernel<MAPS, 4><<<(unsigned)rows, 256, 0, st>>>(c);
+    else span_merge_kernel<MAPS, 1><<<(unsigned)cdiv(rows, 4), 256, 0, st>>>(c);
+    VQ_HIP_CHECK_LAUNCH(fn);
+    return VQ_OK;
+}
+
 template <int MAPS> int attend(const char *fn, const vq_store_attend_args *args) {
-    if (int rc = check_call(fn, args, MAPS)) return rc;
+    if (int rc = span_check_call(fn, args, MAPS)) return rc;
     SpanCall c = cut(*args, MAPS);
     const vq_store_attend_args &a = c.a;
     const bool mfma = span_mfma_supported(a), direct = mfma && c.nparts == 1;
@@ -311,17 +297,13 @@ template <int MAPS> int attend(const char *fn, const vq_store_attend_args *args)
         span_any_kernel<MAPS><<<(unsigned)cdiv(waves, 4), 256, 0, st>>>(c);
         VQ_HIP_CHECK_LAUNCH(fn);
     }
-    if (!direct) {
-        // (a row to a block where its parts are many, or rows too few to fill the chip with a wave each: 512 rows of 16 parts and two maps 9.8 us, a
-        // wave each 11.1; 1920 rows of 11 parts 7.0, a wave each 5.2)
-        if (c.nparts > 2 * MERGE_AT_ONCE || (c.nparts > MERGE_AT_ONCE && rows < 1024)) span_merge_kernel<MAPS, 4><<<(unsigned)rows, 256, 0, st>>>(c);
-        else span_merge_kernel<MAPS, 1><<<(unsigned)cdiv(rows, 4), 256, 0, st>>>(c);
-        VQ_HIP_CHECK_LAUNCH(fn);
-    }
+    if (!direct) return launch_merge<MAPS>(fn, c);
     return VQ_OK;
 }
 
 }  // namespace
+
+int launch_span_merge1(const char *fn, const SpanCall &c) { return launch_merge<1>(fn, c); }
 
 }  // namespace vq
 

@@ -9,6 +9,8 @@
 
 namespace vq {
 
+constexpr int SPAN_MAX_D = 256;
+
 // A call and how it is cut.  Every kernel writes partials -- per (query row, part, map) the sums of exp2(s - m) v over its
 // slots, and (m, the sum of exp2(s - m)), m in log2 units -- unless there is one part a row, where it writes the output.
 struct SpanCall {
@@ -53,6 +55,40 @@ __device__ __forceinline__ float span_wave_sum(float v) {
     return v;
 }
 __device__ __forceinline__ float span_lam(const vq_store_attend_args &a, int64_t h) { return a.lam[h * a.lam_stride]; }
+
+// One element of a packed store's key or value as the fp16 number it stands for.
+struct SpanPacked {
+    const vq_kv_store *s;
+    int bits, per, group, meta, v_layout;
+    uint32_t mask;
+    int64_t D, W, GV, GK;
+    __device__ __forceinline__ float fp16_of(uint32_t word, int slot, const void *scale, const void *zero, int64_t at) const {
+        const float code = (float)((word >> (slot * bits)) & mask);
+        return (float)(f16)__builtin_fmaf(code, span_ld(scale, meta, at), span_ld(zero, meta, at));
+    }
+    __device__ __forceinline__ float key(int64_t bh, int64_t t, int64_t d) const {
+        const uint32_t w = ((const uint32_t *)s->k_packed)[(bh * s->cap_tokens + t) * W + d / per];
+        return fp16_of(w, (int)(d % per), s->k_scale, s->k_zero, (bh * GK + t / group) * D + d);
+    }
+    __device__ __forceinline__ float value(int64_t bh, int64_t t, int64_t d) const {
+        if (v_layout == VQ_V_CHANNEL_PACKED) {
+            const uint32_t w = ((const uint32_t *)s->v_packed)[(bh * s->cap_tokens + t) * W + d / per];
+            return fp16_of(w, (int)(d % per), s->v_scale, s->v_zero, (bh * s->cap_tokens + t) * GV + d / group);
+        }
+        const uint32_t w = ((const uint32_t *)s->v_packed)[(bh * (s->cap_tokens / per) + t / per) * D + d];
+        return fp16_of(w, (int)(t % per), s->v_scale, s->v_zero, (bh * GV + d / group) * s->cap_tokens + t);
+    }
+    static __device__ __forceinline__ SpanPacked of(const vq_store_attend_args &a, const vq_kv_store &s) {
+        const int per = 32 / a.pack_bits;
+        auto up = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
+        return {&s, a.pack_bits, per, a.group, a.meta_dtype, a.v_layout, (1u << a.pack_bits) - 1u, a.D, up(a.D, per), up(a.D, a.group),
+                up(s.cap_tokens, a.group)};
+    }
+};
+
+// the checks of a call, the merge of the parts of rows of one map (attend_span.hip)
+int span_check_call(const char *fn, const vq_store_attend_args *args, int maps);
+int launch_span_merge1(const char *fn, const SpanCall &c);
 
 // whether the matrix-unit kernel takes the call, its cut, its launch (attend_span_mfma.hip)
 bool span_mfma_supported(const vq_store_attend_args &a);

@@ -76,6 +76,8 @@ template <> struct Elem<float> {
         default: return vq::fail(VQ_ERR_INVALID, "unsupported float dtype tag %d", (int)(tag)); \
     }
 
+int check_rotary(const char *fn, const vq_rotary_args &a);   // (rotary.hip) the checks of a call that turns rows
+
 static inline bool is_float_tag(int t) { return t == VQ_F16 || t == VQ_BF16 || t == VQ_F32; }
 static inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 

@@ -146,31 +146,41 @@ template <typename T> int launch_rotary(const vq_rotary_args &a, hipStream_t st)
 
 }  // namespace vq
 
-extern "C" int vq_rotary(const vq_rotary_args *args, void *stream) {
-    using namespace vq;
-    VQ_REQUIRE(args != nullptr, VQ_ERR_INVALID, "vq_rotary: no arguments");
-    const vq_rotary_args &a = *args;
-    VQ_REQUIRE(is_float_tag(a.dtype), VQ_ERR_INVALID, "vq_rotary: unsupported dtype tag %d", a.dtype);
-    VQ_REQUIRE(a.B >= 0 && a.S >= 0 && a.D >= 1 && a.heads[0] >= 0 && a.heads[1] >= 0, VQ_ERR_INVALID, "vq_rotary: bad sizes");
+namespace vq {
+
+int check_rotary(const char *fn, const vq_rotary_args &a) {
+    VQ_REQUIRE(is_float_tag(a.dtype), VQ_ERR_INVALID, "%s: unsupported dtype tag %d", fn, a.dtype);
+    VQ_REQUIRE(a.B >= 0 && a.S >= 0 && a.D >= 1 && a.heads[0] >= 0 && a.heads[1] >= 0, VQ_ERR_INVALID, "%s: bad sizes", fn);
     VQ_REQUIRE(a.dims >= 2 && a.dims % 2 == 0 && a.dims <= a.D, VQ_ERR_INVALID,
-               "vq_rotary: dims=%lld must be even, at least 2 and at most the head size %lld", (long long)a.dims, (long long)a.D);
-    VQ_REQUIRE(a.layout == VQ_ROTARY_HALF || a.layout == VQ_ROTARY_INTERLEAVED, VQ_ERR_INVALID, "vq_rotary: unknown layout %d", a.layout);
-    VQ_REQUIRE(a.freq_dtype == VQ_F64 || a.freq_dtype == VQ_F32, VQ_ERR_INVALID, "vq_rotary: frequencies must be float64 or float32");
+               "%s: dims=%lld must be even, at least 2 and at most the head size %lld", fn, (long long)a.dims, (long long)a.D);
+    VQ_REQUIRE(a.layout == VQ_ROTARY_HALF || a.layout == VQ_ROTARY_INTERLEAVED, VQ_ERR_INVALID, "%s: unknown layout %d", fn, a.layout);
+    VQ_REQUIRE(a.freq_dtype == VQ_F64 || a.freq_dtype == VQ_F32, VQ_ERR_INVALID, "%s: frequencies must be float64 or float32", fn);
     VQ_REQUIRE(a.positions == nullptr || a.pos_dtype == VQ_I32 || a.pos_dtype == VQ_I64, VQ_ERR_INVALID,
-               "vq_rotary: positions must be int32 or int64");
+               "%s: positions must be int32 or int64", fn);
     const int64_t heads = a.heads[0] + a.heads[1];
     VQ_REQUIRE(heads <= 65535 && a.D <= 65536 && a.S < (INT64_C(1) << 31), VQ_ERR_UNSUPPORTED,
-               "vq_rotary: at most 65535 heads, 65536 channels and 2^31 - 1 positions a sequence");
+               "%s: at most 65535 heads, 65536 channels and 2^31 - 1 positions a sequence", fn);
     if (a.B == 0 || a.S == 0 || heads == 0) return VQ_OK;
-    VQ_REQUIRE(a.B < (INT64_C(1) << 31), VQ_ERR_UNSUPPORTED, "vq_rotary: too many rows for one launch");
-    VQ_REQUIRE(a.inv_freq != nullptr, VQ_ERR_INVALID, "vq_rotary: frequencies must be given");
+    VQ_REQUIRE(a.B < (INT64_C(1) << 31), VQ_ERR_UNSUPPORTED, "%s: too many rows for one launch", fn);
+    VQ_REQUIRE(a.inv_freq != nullptr, VQ_ERR_INVALID, "%s: frequencies must be given", fn);
     for (int w = 0; w < 2; ++w)
-        VQ_REQUIRE(a.heads[w] == 0 || (a.x[w] != nullptr && a.out[w] != nullptr), VQ_ERR_INVALID, "vq_rotary: rows and outputs must be given");
+        VQ_REQUIRE(a.heads[w] == 0 || (a.x[w] != nullptr && a.out[w] != nullptr), VQ_ERR_INVALID, "%s: rows and outputs must be given", fn);
     const int64_t sizes[2][3] = {{a.B, a.heads[0], a.S}, {a.B, a.heads[1], a.S}};
     for (int w = 0; w < 2; ++w)
         for (int d = 0; d < 3; ++d)
             VQ_REQUIRE(a.heads[w] == 0 || a.x[w] != a.out[w] || sizes[w][d] < 2 || a.x_strides[w][d] == a.out_strides[w][d], VQ_ERR_INVALID,
-                       "vq_rotary: rows turned in place keep their strides");
+                       "%s: rows turned in place keep their strides", fn);
+    return VQ_OK;
+}
+
+}  // namespace vq
+
+extern "C" int vq_rotary(const vq_rotary_args *args, void *stream) {
+    using namespace vq;
+    VQ_REQUIRE(args != nullptr, VQ_ERR_INVALID, "vq_rotary: no arguments");
+    const vq_rotary_args &a = *args;
+    if (int rc = check_rotary("vq_rotary", a)) return rc;
+    if (a.B == 0 || a.S == 0 || a.heads[0] + a.heads[1] == 0) return VQ_OK;
     VQ_DISPATCH_FLOAT(a.dtype, T, return launch_rotary<T>(a, (hipStream_t)stream));
     return VQ_OK;
 }

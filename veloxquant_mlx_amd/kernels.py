@@ -1464,7 +1464,7 @@ __all__ = [
     "kv_tail_append", "kivi_cache_append", "attend_fixed_order",
     "kivi_packed_attend", "scalar_fused_decode_attend", "scalar_fused_decode_attend_batched",
     "scalar_predecoded_attend", "flash_prefill_attend",
-    "rotary_embed", "shared_prefix_attend", "differential_attend",
+    "rotary_embed", "norm_rotary_embed", "shared_prefix_attend", "differential_attend", "select_blocks", "block_sparse_attend",
 ]
 
 
@@ -1547,8 +1547,21 @@ def _store_fields(name, which, device, batch, k_packed=None, k_scale=None, k_zer
     return fields, heads, channels, packed, tail, keep
 
 
+def _scratch_call(device, stream, call, room, block):
+    """Run ``call(block(workspace))`` with the stream's scratch, or with one of its own that a graph under capture keeps."""
+    if _capturing():
+        # a graph's scratch is its own: two graphs captured on one stream may run at once, and the scratch kept for the
+        # stream is given back when a larger one replaces it
+        need = room(block(None))
+        return call(block(torch.empty(need, dtype=torch.uint8, device=device) if need else None))
+    rc = call(block(_workspace(device, 0, stream)))
+    if rc == _lib.VQ_ERR_WORKSPACE:
+        rc = call(block(_workspace(device, room(block(None)), stream)))
+    return rc
+
+
 def _store_attend(name, maps, q, prefix, own, scale, causal, seq_lens, sliding_window, out, lam=None, norm_weight=None, norm_eps=0.0,
-                  gain=1.0):
+                  gain=1.0, lists=None):
     if q.ndim != 4:
         raise ValueError(f"{name}: q must be 4D, got {tuple(q.shape)}")
     if not q.is_cuda:
@@ -1596,6 +1609,19 @@ def _store_attend(name, maps, q, prefix, own, scale, causal, seq_lens, sliding_w
                 raise ValueError(f"{name}: norm_weight must be a contiguous [{D}] tensor on {device}")
             weight, weight_tag = norm_weight.data_ptr(), _ftag(name, norm_weight)
     bits, group, meta, layout = packed or (8, 1, 0, 0)
+    more = b""
+    if lists is not None:
+        blocks, block_size, query_block = lists
+        if block_size < 1 or query_block < 1:
+            raise ValueError(f"{name}: block_size={block_size} and query_block={query_block} must be at least 1")
+        want = (B, heads, -(-Sq // query_block))
+        if blocks.ndim != 4 or blocks.shape[:3] != want or blocks.dtype != torch.int32 or blocks.device != device or not blocks.is_contiguous():
+            raise ValueError(f"{name}: blocks must be a contiguous int32 [{want[0]}, {want[1]}, {want[2]}, n] tensor on {device}, got {tuple(blocks.shape)} "
+                             f"in {blocks.dtype} on {blocks.device}")
+        try:
+            more = _lib.BLOCK_LISTS_PACK.pack(blocks.data_ptr(), blocks.shape[3], block_size, query_block)
+        except (_lib.struct.error, OverflowError) as e:
+            raise ValueError(f"{name}: {e}") from None
     lib = _lib.load()
     stream = _stream_of(device)
     call, room = lib.store_attend_packed[maps], lib.store_attend_packed_workspace[maps]
@@ -1604,21 +1630,10 @@ def _store_attend(name, maps, q, prefix, own, scale, causal, seq_lens, sliding_w
         return _lib.STORE_ATTEND_PACK.pack(
             q.data_ptr(), out.data_ptr(), B, Hq, heads, Sq, D, *prefix_f, *own_f, lens, lam_p, lam_stride, weight,
             0 if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), stream, sliding_window or 0, tag,
-            tag if tail is None else _FLOAT_TAG[tail], weight_tag, bits, group, meta, layout, 1 if causal else 0, scale, norm_eps, gain)
-
-    def launch():
-        if _capturing():
-            # a graph's scratch is its own: two graphs captured on one stream may run at once, and the scratch kept for the
-            # stream is given back when a larger one replaces it
-            need = room(block(None))
-            return call(block(torch.empty(need, dtype=torch.uint8, device=device) if need else None))
-        rc = call(block(_workspace(device, 0, stream)))
-        if rc == _lib.VQ_ERR_WORKSPACE:
-            rc = call(block(_workspace(device, room(block(None)), stream)))
-        return rc
+            tag if tail is None else _FLOAT_TAG[tail], weight_tag, bits, group, meta, layout, 1 if causal else 0, scale, norm_eps, gain) + more
 
     try:
-        _launch_on(device, launch)
+        _launch_on(device, lambda: _scratch_call(device, stream, call, room, block))
     except (_lib.struct.error, OverflowError) as e:
         raise ValueError(f"{name}: {e}") from None
     return out
@@ -1669,6 +1684,100 @@ def differential_attend(q: torch.Tensor, lam: torch.Tensor | float, *, k_packed=
                bits=bits, group_size=group_size, v_layout=v_layout, k_tail=k_tail, v_tail=v_tail, n_tail=n_tail)
     return _store_attend("differential_attend", 2, q, None, own, scale, causal, seq_lens, sliding_window, out, lam, norm_weight, norm_eps,
                          gain)
+
+
+# ---------------------------------------------------------------------------
+# attention over chosen blocks
+# ---------------------------------------------------------------------------
+
+def select_blocks(q: torch.Tensor, k_scale: torch.Tensor, k_zero: torch.Tensor, n_select: int, *, levels: int, group_size: int, n_packed: int,
+                  n_tail: int = 0, block_size: int | None = None, query_block: int = 1, first: int = 0, recent: int = 0,
+                  causal: bool = False, seq_lens: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """The ``n_select`` blocks of a packed store's slots that every query (or tile of queries) attends to with
+    :func:`block_sparse_attend`: int32 ``[B, Hkv, tiles, n_select]``, ascending, -1 at the end where fewer are visible.
+
+    A block holds ``block_size`` slots, a multiple of ``group_size`` (default: one group).  Its score bounds what any of its keys can score: a
+    group's keys lie between ``zero`` and ``zero + levels * scale`` in every channel (``levels`` the top code), so ``sum_c max(q_c zero_c,
+    q_c (zero_c + levels scale_c))`` is at least every ``q k`` of the group; the block's is the largest over its groups, over the query heads of
+    the kv head and over the ``query_block`` consecutive queries of the tile, which choose together (the last tile may hold fewer).  ``k_scale``,
+    ``k_zero [B,Hkv,cap/group,D]`` (float16 or float32) are the store's own, so choosing reads no key.
+
+    q ``[B,Hq,Sq,D]`` (``D`` up to 256).  ``n_packed`` and ``n_tail``: slots of the store and plain rows behind them; with ``seq_lens``
+    (int64 ``[B]`` on the device) a sequence has only that many live ones of both.  Queries align to the end of a sequence; ``causal`` hides
+    the slots behind a query's own position, and a block is visible if its first slot is.  If the tile's last query sees ``n_select``
+    blocks or fewer, those are all chosen; else the first ``first``, the last ``recent`` and the best of the others.  Scores are formed in
+    64 bits, so the choice does not depend on the order of a sum; of equal ones the lower block is taken, NaN counts above all."""
+    name = "select_blocks"
+    if q.ndim != 4 or k_scale.ndim != 4:
+        raise ValueError(f"{name}: q must be [B, Hq, Sq, D] and k_scale [B, Hkv, groups, D], got {tuple(q.shape)} and {tuple(k_scale.shape)}")
+    if not q.is_cuda:
+        _need_gpu(name, q)
+    device = q.device
+    B, Hq, Sq, D = q.shape
+    tag = _ftag(name, q)
+    heads, groups = k_scale.shape[1], k_scale.shape[2]
+    group_size, n_packed, n_tail, n_select = int(group_size), int(n_packed), int(n_tail), int(n_select)
+    block_size = group_size if block_size is None else int(block_size)
+    query_block, first, recent = int(query_block), int(first), int(recent)
+    if k_scale.shape != (B, heads, groups, D) or k_zero.shape != k_scale.shape or k_zero.dtype != k_scale.dtype or k_scale.dtype not in _META_DTYPES:
+        raise ValueError(f"{name}: k_scale and k_zero must be alike, [{B}, Hkv, groups, {D}] float16 or float32, got {tuple(k_scale.shape)} "
+                         f"{k_scale.dtype} and {tuple(k_zero.shape)} {k_zero.dtype}")
+    if k_scale.device != device or k_zero.device != device or not k_scale.is_contiguous() or not k_zero.is_contiguous():
+        raise ValueError(f"{name}: k_scale and k_zero must be contiguous on {device}")
+    if not heads or Hq % heads:
+        raise ValueError(f"{name}: {Hq} query heads over {heads} kv heads")
+    if group_size < 1 or block_size < 1 or block_size % group_size or query_block < 1 or n_select < 1:
+        raise ValueError(f"{name}: blocks of {block_size} in groups of {group_size}, {n_select} of them for {query_block} queries")
+    if first < 0 or recent < 0 or first + recent > n_select:
+        raise ValueError(f"{name}: {first} first and {recent} recent blocks of {n_select}")
+    if n_packed < 0 or n_tail < 0 or n_packed > groups * group_size:
+        raise ValueError(f"{name}: {n_packed} packed slots in {groups} groups of {group_size}, {n_tail} behind them")
+    shape = (B, heads, -(-Sq // query_block), n_select)
+    if out is None:
+        out = torch.empty(shape, dtype=torch.int32, device=device)
+    elif out.shape != shape or out.dtype != torch.int32 or out.device != device or not out.is_contiguous():
+        raise ValueError(f"{name}: out must be a contiguous int32 {shape} tensor on {device}")
+    lens = 0
+    if seq_lens is not None:
+        if seq_lens.shape != (B,) or seq_lens.dtype != torch.int64 or seq_lens.device != device or not seq_lens.is_contiguous():
+            raise ValueError(f"{name}: seq_lens must be a contiguous int64 [{B}] tensor on {device}")
+        lens = seq_lens.data_ptr()
+    if out.numel() == 0:
+        return out
+    if not q.is_contiguous():
+        q = q.contiguous()
+    lib = _lib.load()
+    stream = _stream_of(device)
+
+    def block(ws):
+        return _lib.BLOCK_SELECT_PACK.pack(
+            q.data_ptr(), k_scale.data_ptr(), k_zero.data_ptr(), out.data_ptr(), B, Hq, heads, Sq, D, n_packed, groups * group_size, n_tail, block_size,
+            query_block, n_select, first, recent, lens, 0 if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), stream, tag,
+            _FLOAT_TAG[k_scale.dtype], group_size, levels, 1 if causal else 0)
+
+    try:
+        _launch_on(device, lambda: _scratch_call(device, stream, lib.block_select_packed, lib.block_select_packed_workspace, block))
+    except (_lib.struct.error, OverflowError) as e:
+        raise ValueError(f"{name}: {e}") from None
+    return out
+
+
+def block_sparse_attend(q: torch.Tensor, blocks: torch.Tensor, *, block_size: int, query_block: int = 1, k_packed=None, k_scale=None,
+                        k_zero=None, v_packed=None, v_scale=None, v_zero=None, n_packed: int = 0, bits: int = 4, group_size: int = 32,
+                        v_layout: str = "channel", k_tail=None, v_tail=None, n_tail: int = 0, scale: float = 1.0, causal: bool = False,
+                        seq_lens: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """softmax(q k^T * scale) v over chosen blocks of the packed slots and over the whole tail.
+
+    q ``[B,Hq,Sq,D]`` (``D`` up to 256); the store's arguments, ``scale``, ``causal``, ``seq_lens`` and ``out`` as for
+    :func:`shared_prefix_attend` (own slots only).  ``blocks``: int32 ``[B, Hkv, ceil(Sq / query_block), n]`` on the device, as
+    :func:`select_blocks` gives them: queries ``t * query_block`` and the next ``query_block - 1`` see, of the packed slots, those of the blocks of
+    list ``t`` of their kv head (entry ``e``: slots ``e * block_size`` .. ``(e + 1) * block_size - 1``), as far as these are live and, with
+    ``causal``, not behind the query.  Entries may come in any order; one below zero or past the live slots names nothing, one that is
+    named twice counts twice.  The plain rows of the tail are all seen, up to the query's own.  Slots that no list names are not read.  A
+    row that sees nothing is zero.  Numbers as for :func:`shared_prefix_attend`."""
+    own = dict(k_packed=k_packed, k_scale=k_scale, k_zero=k_zero, v_packed=v_packed, v_scale=v_scale, v_zero=v_zero, n_packed=n_packed,
+               bits=bits, group_size=group_size, v_layout=v_layout, k_tail=k_tail, v_tail=v_tail, n_tail=n_tail)
+    return _store_attend("block_sparse_attend", 0, q, None, own, scale, causal, seq_lens, 0, out, lists=(blocks, int(block_size), int(query_block)))
 
 
 # ---------------------------------------------------------------------------
@@ -1743,7 +1852,44 @@ def rotary_embed(q: torch.Tensor, k: torch.Tensor | None = None, *, inv_freq: to
     itself, to turn in place, or rows that share no memory with each other, with both inputs and the other output: those of a
     cache, or others of the same projection); new tensors are contiguous.  ``inverse=True`` turns back; times ``attention_factor`` that is the transposed map, the gradient of the
     forward call (this package's functions record none)."""
-    name = "rotary_embed"
+    return _rotary_rows("rotary_embed", q, k, inv_freq, offset, positions, traditional, attention_factor, inverse, out, k_out)
+
+
+def norm_rotary_embed(q: torch.Tensor, k: torch.Tensor | None = None, *, q_weight: torch.Tensor | None = None,
+                      k_weight: torch.Tensor | None = None, norm_eps: float = 1e-6, inv_freq: torch.Tensor, offset: int | torch.Tensor = 0,
+                      positions: torch.Tensor | None = None, traditional: bool = False, attention_factor: float = 1.0,
+                      out: torch.Tensor | None = None, k_out: torch.Tensor | None = None):
+    """Norm of every head's row and rotary positions, of queries and keys in one launch: ``y = x / sqrt(mean(x^2) + norm_eps) * weight`` over
+    the ``D`` channels of a head, then the turn of :func:`rotary_embed` (channels past ``dims`` pass through normed and are not scaled by
+    ``attention_factor``).  Returns ``q'`` or ``(q', k')``.
+
+    ``q_weight``, ``k_weight``: ``[D]``, or a row a head (``[Hq, D]``, ``[Hk, D]``), float16, bfloat16 or float32, both of one dtype; None: ones.
+    Squares, their sum, the norm and the turn are float32, with one rounding at the end.  The other arguments, strides and outputs as for
+    :func:`rotary_embed`."""
+    name = "norm_rotary_embed"
+    eps = float(norm_eps)
+    if not 0 <= eps < float("inf"):
+        raise ValueError(f"{name}: norm_eps={norm_eps} must be a number from 0 on")
+    at, strides, tag, keep = [0, 0], [0, 0], 0, []
+    for i, (w, x, what) in enumerate(((q_weight, q, "q"), (k_weight, k, "k"))):
+        if w is None:
+            continue
+        if x is None:
+            raise ValueError(f"{name}: k_weight without k")
+        if x.ndim != 4 or w.device != x.device or (w.shape != x.shape[3:] and w.shape != (x.shape[1], x.shape[3])):
+            raise ValueError(f"{name}: the weight for {what} must be [D] or [H, D] of its {tuple(x.shape)} on {x.device}, got {tuple(w.shape)} on {w.device}")
+        if keep and w.dtype != keep[0].dtype:
+            raise ValueError(f"{name}: q_weight and k_weight must be of one dtype, got {keep[0].dtype} and {w.dtype}")
+        tag = _ftag(name, w)
+        w = w.contiguous()
+        keep.append(w)
+        at[i], strides[i] = w.data_ptr(), x.shape[3] if w.ndim == 2 else 0
+    return _rotary_rows(name, q, k, inv_freq, offset, positions, traditional, attention_factor, False, out, k_out,
+                        _lib.NORM_PACK.pack(*at, *strides, tag, eps), keep)
+
+
+def _rotary_rows(name, q, k, inv_freq, offset, positions, traditional, attention_factor, inverse, out, k_out, norm=None, keep=()):
+    """``norm``: the packed fields of the norm in front of the turn, or None; ``keep``: tensors that they point into."""
     if q.ndim != 4 or (k is not None and k.ndim != 4):
         raise ValueError(f"{name}: q and k must be [B, H, S, D], got {tuple(q.shape)}" + ("" if k is None else f" and {tuple(k.shape)}"))
     if k is None and k_out is not None:
@@ -1824,7 +1970,10 @@ def rotary_embed(q: torch.Tensor, k: torch.Tensor | None = None, *, inv_freq: to
             attention_factor)
     except (_lib.struct.error, OverflowError) as e:
         raise ValueError(f"{name}: {e}") from None
-    _launch_on(device, lambda: lib.rotary_packed(args, _stream_of(device)))
+    if norm is None:
+        _launch_on(device, lambda: lib.rotary_packed(args, _stream_of(device)))
+    else:
+        _launch_on(device, lambda: lib.norm_rotary_packed(args + norm, _stream_of(device)))
     return result
 
 

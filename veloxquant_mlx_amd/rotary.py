@@ -7,6 +7,8 @@ scaled context) and turns queries and keys in one launch (:func:`veloxquant_mlx_
     q, k = rope(q, k, offset=cache.offset)
     cache.update_and_fetch(k, v)
     out = cache.fused_sdpa(q, scale)
+
+Models that norm queries and keys a head do both in one launch: ``rope.normed(q, k, q_weight=.., k_weight=.., offset=..)``.
 """
 
 from __future__ import annotations
@@ -112,6 +114,15 @@ class RotaryPositions:
         factor = 1 / self.attention_factor if inverse else self.attention_factor
         return K.rotary_embed(q, k, inv_freq=self.inv_freq, offset=offset, positions=positions, traditional=self.traditional,
                               attention_factor=factor, inverse=inverse, out=out, k_out=k_out)
+
+    def normed(self, q: torch.Tensor, k: torch.Tensor | None = None, *, q_weight: torch.Tensor | None = None,
+               k_weight: torch.Tensor | None = None, norm_eps: float = 1e-6, offset: int | torch.Tensor = 0,
+               positions: torch.Tensor | None = None, out: torch.Tensor | None = None, k_out: torch.Tensor | None = None):
+        """The same behind the norm of every head's row, for models that norm queries and keys a head: one launch for both
+        (:func:`~veloxquant_mlx_amd.kernels.norm_rotary_embed`)."""
+        return K.norm_rotary_embed(q, k, q_weight=q_weight, k_weight=k_weight, norm_eps=norm_eps, inv_freq=self.inv_freq, offset=offset,
+                                   positions=positions, traditional=self.traditional, attention_factor=self.attention_factor, out=out,
+                                   k_out=k_out)
 
 
 __all__ = ["RotaryPositions", "rotary_frequencies"]
