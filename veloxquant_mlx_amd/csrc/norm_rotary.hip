@@ -77,10 +77,205 @@ template <typename T> __global__ __launch_bounds__(256) void norm_rotary_any_ker
     for (int64_t d = a.dims + lane; d < a.D; d += 64) Elem<T>::st(out + d, normed(d));
 }
 
-template <typename T> int launch_norm_rotary(const vq_norm_rotary_args &c, hipStream_t st) {
-    const vq_rotary_args &a = c.rotary;
-    const int64_t rows = a.B * (a.heads[0] + a.heads[1]) * a.S;
-    norm_rotary_any_kernel<T><<<(unsigned)cdiv(rows, 4), 256, 0, st>>>(c);
+constexpr int NR_THREADS = 256;
+constexpr int NR_FLIGHT = 4;              // rows a lane has in flight
+constexpr int64_t NR_FILL = 256 * 1024;   // threads that fill the chip: 16 waves a CU
+
+struct NormRotaryCall {
+    vq_norm_rotary_args n;
+    int lanes_log2;         // lanes of a row, of which the first `units` hold channels and the first `rot_units` of those turn
+    int units, rot_units;
+    int heads_per_thread;
+    float by_d;             // 1 / D
+    int wide_weight;        // 1: weights of the element type, read in whole pieces
+};
+
+template <typename T, int N> struct alignas(sizeof(T) * N) NormPiece { T v[N]; };
+__device__ __forceinline__ void nr_st(f16 *p, float v) { *p = (f16)v; }
+__device__ __forceinline__ void nr_st(bf16_t *p, float v) { p->bits = __builtin_bit_cast(u16, (__bf16)v); }   // (one instruction for two)
+__device__ __forceinline__ void nr_st(float *p, float v) { *p = v; }
+
+// Rows in whole pieces of 16 bytes.  The lanes of a row hold two pieces each, in the half layout a piece and the one that its channels pair with,
+// so the row is read once: the squares meet in log2(lanes) shuffles, norm and turn are applied to what the lane holds.  A lane keeps the sines
+// and cosines of its pairs at one position and walks over heads, queries then keys; norm weight and turn are one factor a term
+// (w_0 cos, w_1 sin, w_1 cos, w_0 sin), formed once for all heads that share a weight row, and the first rows are asked for ahead of the angles.
+template <typename T, int N, bool HALF> __global__ __launch_bounds__(NR_THREADS) void norm_rotary_kernel(NormRotaryCall c) {
+    const vq_rotary_args &a = c.n.rotary;
+    const int u = threadIdx.x & ((1 << c.lanes_log2) - 1);
+    const int64_t tok = (int64_t)blockIdx.x * (NR_THREADS >> c.lanes_log2) + (threadIdx.x >> c.lanes_log2);
+    if (tok >= a.B * a.S) return;   // (the lanes of a row leave together)
+    const int64_t b = tok / a.S, s = tok - b * a.S;
+    const int D = (int)a.D, dims = (int)a.dims;
+    // the lane's two pieces: the channel of each, which of them are there, which turn
+    int c0, c1;
+    bool turn0, turn1;
+    if (HALF) {
+        turn0 = turn1 = u < c.rot_units;
+        c0 = turn0 ? u * N : dims + 2 * (u - c.rot_units) * N;
+        c1 = turn0 ? c0 + dims / 2 : c0 + N;
+    } else {
+        c0 = 2 * u * N;
+        c1 = c0 + N;
+        turn0 = c0 < dims;
+        turn1 = c1 < dims;
+    }
+    const bool has0 = u < c.units, has1 = has0 && c1 < D;
+    if (!has1) c1 = 0;
+    if (!has0) c0 = 0;
+    using P = NormPiece<T, N>;
+    const int Hq = (int)a.heads[0], heads = Hq + (int)a.heads[1];
+    const int first = (int)blockIdx.y * c.heads_per_thread, end = first + c.heads_per_thread < heads ? first + c.heads_per_thread : heads;
+    P x0[NR_FLIGHT], x1[NR_FLIGHT];
+    // rows h .. of the heads up to `to`, all queries or all keys
+    auto load = [&](int h, int to) __attribute__((always_inline)) {
+        const int w = h >= Hq;
+        const T *from = (const T *)a.x[w] + b * a.x_strides[w][0] + s * a.x_strides[w][2];
+#pragma unroll
+        for (int k = 0; k < NR_FLIGHT; ++k) {
+            const T *row = from + (int64_t)((h + k < to ? h + k : h) - (w ? Hq : 0)) * a.x_strides[w][1];   // (missing rows: the first again)
+            x0[k] = *(const P *)(row + c0);
+            x1[k] = *(const P *)(row + c1);
+        }
+    };
+    auto upto = [&](int h) __attribute__((always_inline)) { const int last = h < Hq && Hq < end ? Hq : end; return h + NR_FLIGHT < last ? h + NR_FLIGHT : last; };
+    int h = first, to = upto(h);
+    load(h, to);
+    // sines and cosines: half layout of pair j, (c0 + j, c1 + j); interleaved of pairs j of the first piece, then of the second
+    float cs[N], sn[N];
+    if (turn0) {
+        const double place = (double)nr_position(a, b, s) * 0.15915494309189533577;   // turns per radian
+        const int i0 = u * N;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            cs[j] = 1.f;
+            sn[j] = 0.f;
+            if (HALF || j < N / 2 || turn1) nr_angle(a, place, i0 + j, cs[j], sn[j]);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) { cs[j] = 1.f; sn[j] = 0.f; }
+    }
+    // factors of a value by its own channel (A, C) and of its partner (B, E)
+    float A[N], B[N], C[N], E[N];
+    auto factors = [&](int w, int head) __attribute__((always_inline)) {
+        float w0[N], w1[N];
+        const int64_t at = (int64_t)head * c.n.weight_stride[w];
+        if (c.n.weight[w] == nullptr) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) w0[j] = w1[j] = 1.f;
+        } else if (c.wide_weight) {
+            const P y0 = *(const P *)((const T *)c.n.weight[w] + at + c0), y1 = *(const P *)((const T *)c.n.weight[w] + at + c1);
+#pragma unroll
+            for (int j = 0; j < N; ++j) { w0[j] = Elem<T>::ld(&y0.v[j]); w1[j] = Elem<T>::ld(&y1.v[j]); }
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                w0[j] = nr_ld(c.n.weight[w], c.n.weight_dtype, at + c0 + j);
+                w1[j] = nr_ld(c.n.weight[w], c.n.weight_dtype, at + c1 + j);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            if (HALF) {
+                A[j] = cs[j] * w0[j]; B[j] = sn[j] * w1[j];
+                C[j] = cs[j] * w1[j]; E[j] = sn[j] * w0[j];
+            } else {   // pair j / 2 of either piece
+                A[j] = cs[j / 2] * w0[j]; C[j] = cs[N / 2 + j / 2] * w1[j];
+                B[j] = sn[j / 2] * w0[j ^ 1]; E[j] = sn[N / 2 + j / 2] * w1[j ^ 1];
+            }
+        }
+    };
+    int weighted = -1;   // which factors are held: of the queries or of the keys
+#pragma unroll 1
+    for (;;) {
+        const int w = h >= Hq;
+        const bool own = c.n.weight_stride[w] != 0 && c.n.weight[w] != nullptr;
+        if (weighted != w && !own) factors(w, 0);
+        weighted = own ? -1 : w;
+        T *out = (T *)a.out[w] + b * a.out_strides[w][0] + s * a.out_strides[w][2];
+        float sum[NR_FLIGHT];
+#pragma unroll
+        for (int k = 0; k < NR_FLIGHT; ++k) {
+            float p0 = 0.f, p1 = 0.f;
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const float v0 = Elem<T>::ld(&x0[k].v[j]), v1 = Elem<T>::ld(&x1[k].v[j]);
+                p0 = __builtin_fmaf(v0, v0, p0);
+                p1 = __builtin_fmaf(v1, v1, p1);
+            }
+            sum[k] = (has0 ? p0 : 0.f) + (has1 ? p1 : 0.f);
+        }
+        for (int off = 1; off < 1 << c.lanes_log2; off <<= 1)
+#pragma unroll
+            for (int k = 0; k < NR_FLIGHT; ++k) sum[k] += __shfl_xor(sum[k], off);
+#pragma unroll
+        for (int k = 0; k < NR_FLIGHT; ++k) {
+            if (h + k >= to) break;
+            const int head = h + k - (w ? Hq : 0);
+            if (own) factors(w, head);
+            const float r = nr_rsqrt(__builtin_fmaf(sum[k], c.by_d, c.n.eps));
+            P y0, y1;
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const float v0 = Elem<T>::ld(&x0[k].v[j]) * r, v1 = Elem<T>::ld(&x1[k].v[j]) * r;
+                if (HALF) {
+                    nr_st(&y0.v[j], turn0 ? __builtin_fmaf(v0, A[j], -(v1 * B[j])) : v0 * A[j]);
+                    nr_st(&y1.v[j], turn0 ? __builtin_fmaf(v1, C[j], v0 * E[j]) : v1 * C[j]);
+                } else {
+                    const float o0 = Elem<T>::ld(&x0[k].v[j ^ 1]) * r, o1 = Elem<T>::ld(&x1[k].v[j ^ 1]) * r;
+                    nr_st(&y0.v[j], turn0 ? __builtin_fmaf(v0, A[j], j & 1 ? o0 * B[j] : -(o0 * B[j])) : v0 * A[j]);
+                    nr_st(&y1.v[j], turn1 ? __builtin_fmaf(v1, C[j], j & 1 ? o1 * E[j] : -(o1 * E[j])) : v1 * C[j]);
+                }
+            }
+            T *row = out + (int64_t)head * a.out_strides[w][1];
+            if (has0) *(P *)(row + c0) = y0;
+            if (has1) *(P *)(row + c1) = y1;
+        }
+        h = to;
+        if (h >= end) break;
+        to = upto(h);
+        load(h, to);
+    }
+}
+
+template <typename T> int launch_norm_rotary(const vq_norm_rotary_args &n, hipStream_t st) {
+    constexpr int N = 16 / (int)sizeof(T);
+    const vq_rotary_args &a = n.rotary;
+    const bool half = a.layout == VQ_ROTARY_HALF;
+    const int heads = (int)(a.heads[0] + a.heads[1]);
+    NormRotaryCall c;
+    c.n = n;
+    // 16-byte pieces where every row of every tensor is aligned for them, no pair is cut and a wave's lanes hold the row
+    const int64_t pieces = a.D / N;
+    c.rot_units = (int)(half ? a.dims / 2 / N : 0);
+    c.units = (int)(half ? c.rot_units + cdiv(pieces - 2 * c.rot_units, 2) : cdiv(pieces, 2));
+    bool wide = a.D % N == 0 && (half ? a.dims / 2 : a.dims) % N == 0 && pieces <= 128;
+    bool wide_weight = true;
+    for (int w = 0; w < 2; ++w) {
+        if (a.heads[w] == 0) continue;
+        wide = wide && (((uintptr_t)a.x[w] | (uintptr_t)a.out[w]) & 15) == 0;
+        for (int d = 0; d < 3; ++d) wide = wide && a.x_strides[w][d] % N == 0 && a.out_strides[w][d] % N == 0;
+        if (n.weight[w] != nullptr) wide_weight = wide_weight && n.weight_dtype == a.dtype && ((uintptr_t)n.weight[w] & 15) == 0 && n.weight_stride[w] % N == 0;
+    }
+    const int64_t tokens = a.B * a.S;
+    if (wide) {
+        c.wide_weight = wide_weight;
+        c.by_d = 1.f / (float)a.D;
+        c.lanes_log2 = 0;
+        while (1 << c.lanes_log2 < c.units) ++c.lanes_log2;
+        const int64_t threads = tokens << c.lanes_log2;
+        VQ_REQUIRE(threads < (INT64_C(1) << 32) - NR_THREADS, VQ_ERR_UNSUPPORTED, "vq_norm_rotary: too many rows for one launch");
+        c.heads_per_thread = heads;
+        while (c.heads_per_thread > 1 && threads * cdiv(heads, c.heads_per_thread) < NR_FILL)
+            c.heads_per_thread = c.heads_per_thread > NR_FLIGHT ? (int)cdiv(cdiv(c.heads_per_thread, 2), NR_FLIGHT) * NR_FLIGHT : c.heads_per_thread / 2;
+        const dim3 grid((unsigned)cdiv(threads, NR_THREADS), (unsigned)cdiv(heads, c.heads_per_thread));
+        if (half) norm_rotary_kernel<T, N, true><<<grid, NR_THREADS, 0, st>>>(c);
+        else norm_rotary_kernel<T, N, false><<<grid, NR_THREADS, 0, st>>>(c);
+        VQ_HIP_CHECK_LAUNCH("vq_norm_rotary");
+        return VQ_OK;
+    }
+    const int64_t rows = tokens * heads;
+    norm_rotary_any_kernel<T><<<(unsigned)cdiv(rows, 4), 256, 0, st>>>(n);
     VQ_HIP_CHECK_LAUNCH("vq_norm_rotary");
     return VQ_OK;
 }
