@@ -99,7 +99,9 @@ __device__ __forceinline__ void nr_st(float *p, float v) { *p = v; }
 // so the row is read once: the squares meet in log2(lanes) shuffles, norm and turn are applied to what the lane holds.  A lane keeps the sines
 // and cosines of its pairs at one position and walks over heads, queries then keys; norm weight and turn are one factor a term
 // (w_0 cos, w_1 sin, w_1 cos, w_0 sin), formed once for all heads that share a weight row, and the first rows are asked for ahead of the angles.
-template <typename T, int N, bool HALF> __global__ __launch_bounds__(NR_THREADS) void norm_rotary_kernel(NormRotaryCall c) {
+//
+// OWN: a weight row a head; its pieces are asked for with the row's, in place of the factors.
+template <typename T, int N, bool HALF, bool OWN> __global__ __launch_bounds__(NR_THREADS) void norm_rotary_kernel(NormRotaryCall c) {
     const vq_rotary_args &a = c.n.rotary;
     const int u = threadIdx.x & ((1 << c.lanes_log2) - 1);
     const int64_t tok = (int64_t)blockIdx.x * (NR_THREADS >> c.lanes_log2) + (threadIdx.x >> c.lanes_log2);
@@ -125,16 +127,22 @@ template <typename T, int N, bool HALF> __global__ __launch_bounds__(NR_THREADS)
     using P = NormPiece<T, N>;
     const int Hq = (int)a.heads[0], heads = Hq + (int)a.heads[1];
     const int first = (int)blockIdx.y * c.heads_per_thread, end = first + c.heads_per_thread < heads ? first + c.heads_per_thread : heads;
-    P x0[NR_FLIGHT], x1[NR_FLIGHT];
+    P x0[NR_FLIGHT], x1[NR_FLIGHT], w0[NR_FLIGHT], w1[NR_FLIGHT];
     // rows h .. of the heads up to `to`, all queries or all keys
     auto load = [&](int h, int to) __attribute__((always_inline)) {
         const int w = h >= Hq;
         const T *from = (const T *)a.x[w] + b * a.x_strides[w][0] + s * a.x_strides[w][2];
 #pragma unroll
         for (int k = 0; k < NR_FLIGHT; ++k) {
-            const T *row = from + (int64_t)((h + k < to ? h + k : h) - (w ? Hq : 0)) * a.x_strides[w][1];   // (missing rows: the first again)
+            const int64_t head = (h + k < to ? h + k : h) - (w ? Hq : 0);   // (missing rows: the first again)
+            const T *row = from + head * a.x_strides[w][1];
             x0[k] = *(const P *)(row + c0);
             x1[k] = *(const P *)(row + c1);
+            if (OWN) {
+                const T *weight = (const T *)c.n.weight[w] + head * c.n.weight_stride[w];
+                w0[k] = *(const P *)(weight + c0);
+                w1[k] = *(const P *)(weight + c1);
+            }
         }
     };
     auto upto = [&](int h) __attribute__((always_inline)) { const int last = h < Hq && Hq < end ? Hq : end; return h + NR_FLIGHT < last ? h + NR_FLIGHT : last; };
@@ -157,31 +165,30 @@ template <typename T, int N, bool HALF> __global__ __launch_bounds__(NR_THREADS)
     }
     // factors of a value by its own channel (A, C) and of its partner (B, E)
     float A[N], B[N], C[N], E[N];
-    auto factors = [&](int w, int head) __attribute__((always_inline)) {
-        float w0[N], w1[N];
-        const int64_t at = (int64_t)head * c.n.weight_stride[w];
+    auto factors = [&](int w) __attribute__((always_inline)) {
+        float f0[N], f1[N];
         if (c.n.weight[w] == nullptr) {
 #pragma unroll
-            for (int j = 0; j < N; ++j) w0[j] = w1[j] = 1.f;
+            for (int j = 0; j < N; ++j) f0[j] = f1[j] = 1.f;
         } else if (c.wide_weight) {
-            const P y0 = *(const P *)((const T *)c.n.weight[w] + at + c0), y1 = *(const P *)((const T *)c.n.weight[w] + at + c1);
+            const P y0 = *(const P *)((const T *)c.n.weight[w] + c0), y1 = *(const P *)((const T *)c.n.weight[w] + c1);
 #pragma unroll
-            for (int j = 0; j < N; ++j) { w0[j] = Elem<T>::ld(&y0.v[j]); w1[j] = Elem<T>::ld(&y1.v[j]); }
+            for (int j = 0; j < N; ++j) { f0[j] = Elem<T>::ld(&y0.v[j]); f1[j] = Elem<T>::ld(&y1.v[j]); }
         } else {
 #pragma unroll
             for (int j = 0; j < N; ++j) {
-                w0[j] = nr_ld(c.n.weight[w], c.n.weight_dtype, at + c0 + j);
-                w1[j] = nr_ld(c.n.weight[w], c.n.weight_dtype, at + c1 + j);
+                f0[j] = nr_ld(c.n.weight[w], c.n.weight_dtype, c0 + j);
+                f1[j] = nr_ld(c.n.weight[w], c.n.weight_dtype, c1 + j);
             }
         }
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             if (HALF) {
-                A[j] = cs[j] * w0[j]; B[j] = sn[j] * w1[j];
-                C[j] = cs[j] * w1[j]; E[j] = sn[j] * w0[j];
+                A[j] = cs[j] * f0[j]; B[j] = sn[j] * f1[j];
+                C[j] = cs[j] * f1[j]; E[j] = sn[j] * f0[j];
             } else {   // pair j / 2 of either piece
-                A[j] = cs[j / 2] * w0[j]; C[j] = cs[N / 2 + j / 2] * w1[j];
-                B[j] = sn[j / 2] * w0[j ^ 1]; E[j] = sn[N / 2 + j / 2] * w1[j ^ 1];
+                A[j] = cs[j / 2] * f0[j]; C[j] = cs[N / 2 + j / 2] * f1[j];
+                B[j] = sn[j / 2] * f0[j ^ 1]; E[j] = sn[N / 2 + j / 2] * f1[j ^ 1];
             }
         }
     };
@@ -189,9 +196,8 @@ template <typename T, int N, bool HALF> __global__ __launch_bounds__(NR_THREADS)
 #pragma unroll 1
     for (;;) {
         const int w = h >= Hq;
-        const bool own = c.n.weight_stride[w] != 0 && c.n.weight[w] != nullptr;
-        if (weighted != w && !own) factors(w, 0);
-        weighted = own ? -1 : w;
+        if (!OWN && weighted != w) factors(w);
+        weighted = w;
         T *out = (T *)a.out[w] + b * a.out_strides[w][0] + s * a.out_strides[w][2];
         float sum[NR_FLIGHT];
 #pragma unroll
@@ -211,23 +217,24 @@ template <typename T, int N, bool HALF> __global__ __launch_bounds__(NR_THREADS)
 #pragma unroll
         for (int k = 0; k < NR_FLIGHT; ++k) {
             if (h + k >= to) break;
-            const int head = h + k - (w ? Hq : 0);
-            if (own) factors(w, head);
             const float r = nr_rsqrt(__builtin_fmaf(sum[k], c.by_d, c.n.eps));
             P y0, y1;
+            float v0[N], v1[N];
 #pragma unroll
             for (int j = 0; j < N; ++j) {
-                const float v0 = Elem<T>::ld(&x0[k].v[j]) * r, v1 = Elem<T>::ld(&x1[k].v[j]) * r;
-                if (HALF) {
-                    nr_st(&y0.v[j], turn0 ? __builtin_fmaf(v0, A[j], -(v1 * B[j])) : v0 * A[j]);
-                    nr_st(&y1.v[j], turn0 ? __builtin_fmaf(v1, C[j], v0 * E[j]) : v1 * C[j]);
-                } else {
-                    const float o0 = Elem<T>::ld(&x0[k].v[j ^ 1]) * r, o1 = Elem<T>::ld(&x1[k].v[j ^ 1]) * r;
-                    nr_st(&y0.v[j], turn0 ? __builtin_fmaf(v0, A[j], j & 1 ? o0 * B[j] : -(o0 * B[j])) : v0 * A[j]);
-                    nr_st(&y1.v[j], turn1 ? __builtin_fmaf(v1, C[j], j & 1 ? o1 * E[j] : -(o1 * E[j])) : v1 * C[j]);
-                }
+                v0[j] = Elem<T>::ld(&x0[k].v[j]) * r;
+                v1[j] = Elem<T>::ld(&x1[k].v[j]) * r;
+                if (OWN) { v0[j] *= Elem<T>::ld(&w0[k].v[j]); v1[j] *= Elem<T>::ld(&w1[k].v[j]); }
             }
-            T *row = out + (int64_t)head * a.out_strides[w][1];
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const int p = HALF ? j : j / 2, p1 = HALF ? j : N / 2 + j / 2;   // the pairs of channels j of either piece
+                const float fa = OWN ? cs[p] : A[j], fb = OWN ? sn[p] : B[j], fc = OWN ? cs[p1] : C[j], fe = OWN ? sn[p1] : E[j];
+                const float o0 = HALF ? v1[j] : v0[j ^ 1], o1 = HALF ? v0[j] : v1[j ^ 1];
+                nr_st(&y0.v[j], turn0 ? __builtin_fmaf(v0[j], fa, !HALF && j & 1 ? o0 * fb : -(o0 * fb)) : OWN ? v0[j] : v0[j] * fa);
+                nr_st(&y1.v[j], turn1 ? __builtin_fmaf(v1[j], fc, HALF || j & 1 ? o1 * fe : -(o1 * fe)) : OWN ? v1[j] : v1[j] * fc);
+            }
+            T *row = out + (int64_t)(h + k - (w ? Hq : 0)) * a.out_strides[w][1];
             if (has0) *(P *)(row + c0) = y0;
             if (has1) *(P *)(row + c1) = y1;
         }
@@ -250,15 +257,17 @@ template <typename T> int launch_norm_rotary(const vq_norm_rotary_args &n, hipSt
     c.rot_units = (int)(half ? a.dims / 2 / N : 0);
     c.units = (int)(half ? c.rot_units + cdiv(pieces - 2 * c.rot_units, 2) : cdiv(pieces, 2));
     bool wide = a.D % N == 0 && (half ? a.dims / 2 : a.dims) % N == 0 && pieces <= 128;
-    bool wide_weight = true;
+    // OWN: both (those that are there) have a row a head, in whole pieces of the element type; one of the two alone, another type: a wave a row
+    bool wide_weight = true, own = false, shared = false;
     for (int w = 0; w < 2; ++w) {
         if (a.heads[w] == 0) continue;
         wide = wide && (((uintptr_t)a.x[w] | (uintptr_t)a.out[w]) & 15) == 0;
         for (int d = 0; d < 3; ++d) wide = wide && a.x_strides[w][d] % N == 0 && a.out_strides[w][d] % N == 0;
+        (n.weight[w] != nullptr && n.weight_stride[w] != 0 ? own : shared) = true;
         if (n.weight[w] != nullptr) wide_weight = wide_weight && n.weight_dtype == a.dtype && ((uintptr_t)n.weight[w] & 15) == 0 && n.weight_stride[w] % N == 0;
     }
     const int64_t tokens = a.B * a.S;
-    if (wide) {
+    if (wide && !(own && (shared || !wide_weight))) {
         c.wide_weight = wide_weight;
         c.by_d = 1.f / (float)a.D;
         c.lanes_log2 = 0;
@@ -269,8 +278,10 @@ template <typename T> int launch_norm_rotary(const vq_norm_rotary_args &n, hipSt
         while (c.heads_per_thread > 1 && threads * cdiv(heads, c.heads_per_thread) < NR_FILL)
             c.heads_per_thread = c.heads_per_thread > NR_FLIGHT ? (int)cdiv(cdiv(c.heads_per_thread, 2), NR_FLIGHT) * NR_FLIGHT : c.heads_per_thread / 2;
         const dim3 grid((unsigned)cdiv(threads, NR_THREADS), (unsigned)cdiv(heads, c.heads_per_thread));
-        if (half) norm_rotary_kernel<T, N, true><<<grid, NR_THREADS, 0, st>>>(c);
-        else norm_rotary_kernel<T, N, false><<<grid, NR_THREADS, 0, st>>>(c);
+        if (own && half) norm_rotary_kernel<T, N, true, true><<<grid, NR_THREADS, 0, st>>>(c);
+        else if (own) norm_rotary_kernel<T, N, false, true><<<grid, NR_THREADS, 0, st>>>(c);
+        else if (half) norm_rotary_kernel<T, N, true, false><<<grid, NR_THREADS, 0, st>>>(c);
+        else norm_rotary_kernel<T, N, false, false><<<grid, NR_THREADS, 0, st>>>(c);
         VQ_HIP_CHECK_LAUNCH("vq_norm_rotary");
         return VQ_OK;
     }
