@@ -95,8 +95,8 @@ __device__ __forceinline__ void nr_st(f16 *p, float v) { *p = (f16)v; }
 __device__ __forceinline__ void nr_st(bf16_t *p, float v) { p->bits = __builtin_bit_cast(u16, (__bf16)v); }   // (one instruction for two)
 __device__ __forceinline__ void nr_st(float *p, float v) { *p = v; }
 
-// Rows in whole pieces of 16 bytes.  The lanes of a row hold two pieces each, in the half layout a piece and the one that its channels pair with,
-// so the row is read once: the squares meet in log2(lanes) shuffles, norm and turn are applied to what the lane holds.  A lane keeps the sines
+// Rows in whole pieces of 16 bytes.  The lanes of a row hold two pieces each, in the half layout a piece and the one that its channels pair with
+// (else half a row apart, so that a load of the lanes is one stretch), so the row is read once: the squares meet in log2(lanes) shuffles, norm and turn are applied to what the lane holds.  A lane keeps the sines
 // and cosines of its pairs at one position and walks over heads, queries then keys; norm weight and turn are one factor a term
 // (w_0 cos, w_1 sin, w_1 cos, w_0 sin), formed once for all heads that share a weight row, and the first rows are asked for ahead of the angles.
 //
@@ -113,11 +113,11 @@ template <typename T, int N, bool HALF, bool OWN> __global__ __launch_bounds__(N
     bool turn0, turn1;
     if (HALF) {
         turn0 = turn1 = u < c.rot_units;
-        c0 = turn0 ? u * N : dims + 2 * (u - c.rot_units) * N;
-        c1 = turn0 ? c0 + dims / 2 : c0 + N;
+        c0 = turn0 ? u * N : dims + (u - c.rot_units) * N;
+        c1 = turn0 ? c0 + dims / 2 : c0 + (c.units - c.rot_units) * N;
     } else {
-        c0 = 2 * u * N;
-        c1 = c0 + N;
+        c0 = u * N;
+        c1 = c0 + c.units * N;
         turn0 = c0 < dims;
         turn1 = c1 < dims;
     }
@@ -152,12 +152,13 @@ template <typename T, int N, bool HALF, bool OWN> __global__ __launch_bounds__(N
     float cs[N], sn[N];
     if (turn0) {
         const double place = (double)nr_position(a, b, s) * 0.15915494309189533577;   // turns per radian
-        const int i0 = u * N;
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             cs[j] = 1.f;
             sn[j] = 0.f;
-            if (HALF || j < N / 2 || turn1) nr_angle(a, place, i0 + j, cs[j], sn[j]);
+            if (HALF) nr_angle(a, place, c0 + j, cs[j], sn[j]);
+            else if (j < N / 2) nr_angle(a, place, c0 / 2 + j, cs[j], sn[j]);
+            else if (turn1) nr_angle(a, place, c1 / 2 + j - N / 2, cs[j], sn[j]);
         }
     } else {
 #pragma unroll
