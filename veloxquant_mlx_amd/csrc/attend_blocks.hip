@@ -88,6 +88,31 @@ int check_blocks(const char *fn, const vq_block_attend_args *args) {
     return VQ_OK;
 }
 
+// The matrix-unit kernel takes what it takes of attention over spans, where blocks are whole units of 32 slots: tiles of 32 rows of a kv head's
+// query heads at the positions of one list, each over the list's units, in as many runs as fill the chip.
+bool plan_few(BlockCall &c) {
+    const vq_store_attend_args &a = c.s.a;
+    if (a.own.n_packed == 0 || c.block_tokens % 32 != 0 || !span_mfma_supported(a)) return false;
+    const int64_t all = cdiv(a.own.n_packed, 32), sub = c.block_tokens / 32 < all ? c.block_tokens / 32 : all;
+    const int64_t qb = c.query_block < a.Sq ? c.query_block : a.Sq, row_tiles = cdiv(a.Hq / a.Hkv * qb, 32);
+    if (c.count * sub >= (1 << 24)) return false;
+    const int64_t units = c.count * sub + cdiv(a.own.n_tail, 32), items = a.B * a.Hkv * c.tiles * row_tiles;
+    // One round of blocks of equal runs, two blocks a CU (one with heads of 256 channels), four units a wave or more
+    int64_t run = cdiv(items * units, a.D == 256 ? 256 : 512);
+    if (run < 16) run = 16;
+    if (run > BLOCK_UNITS) run = BLOCK_UNITS;
+    const int64_t splits = units > 0 ? cdiv(units, run) : 1;
+    if (items * splits >= (1 << 22)) return false;
+    c.s.apart = c.s.pfew = 0;
+    c.s.ofew = 1;
+    c.s.owaves = 4;
+    c.s.osplits = c.s.nparts = (int)splits;
+    c.lists = {c.blocks, (int)c.tiles, (int)c.count, (int)c.block_tokens, (int)qb, (int)cdiv(a.own.n_packed, c.block_tokens), (int)sub, (int)(c.count * sub),
+               (int)units, (int)row_tiles};
+    c.few = 1;
+    return true;
+}
+
 BlockCall cut_blocks(const vq_block_attend_args &args) {
     BlockCall c = {};
     c.s.a = args.store;
@@ -98,6 +123,7 @@ BlockCall cut_blocks(const vq_block_attend_args &args) {
     const vq_store_attend_args &a = c.s.a;
     c.tiles = cdiv(a.Sq, c.query_block);
     if (a.own.n_packed == 0) { c.s.a.pack_bits = 8; c.s.a.group = 1; c.count = 0; }   // fields that no packed slot reads
+    if (plan_few(c)) return c;
     // as many waves as fill the chip eight deep, runs of 64 slots or more
     const int64_t rows = a.B * a.Hq * a.Sq;
     double slots = (double)c.count * (double)c.block_tokens;
@@ -106,6 +132,12 @@ BlockCall cut_blocks(const vq_block_attend_args &args) {
     if ((double)parts > slots / 64.) parts = (int64_t)(slots / 64.);
     c.s.nparts = (int)(parts < 1 ? 1 : parts);
     return c;
+}
+
+int64_t block_floats(const BlockCall &c, int64_t &sums);
+size_t block_bytes(const BlockCall &c) {
+    int64_t sums;
+    return c.few && c.s.nparts == 1 ? 0 : (size_t)block_floats(c, sums) * 4;
 }
 
 // (the sums take whole 16 bytes, so that the pairs behind them are aligned with odd heads too)
@@ -122,8 +154,7 @@ int64_t block_floats(const BlockCall &c, int64_t &sums) {
 extern "C" size_t vq_block_attend_workspace(const vq_block_attend_args *args) {
     using namespace vq;
     if (check_blocks("vq_block_attend", args) != VQ_OK) return 0;
-    int64_t sums;
-    return (size_t)block_floats(cut_blocks(*args), sums) * 4;
+    return block_bytes(cut_blocks(*args));
 }
 
 extern "C" int vq_block_attend(const vq_block_attend_args *args) {
@@ -132,12 +163,19 @@ extern "C" int vq_block_attend(const vq_block_attend_args *args) {
     if (int rc = check_blocks(fn, args)) return rc;
     BlockCall c = cut_blocks(*args);
     const vq_store_attend_args &a = c.s.a;
-    int64_t sums;
-    const size_t need = (size_t)block_floats(c, sums) * 4;
-    VQ_REQUIRE(a.workspace != nullptr && a.workspace_bytes >= need && ((uintptr_t)a.workspace & 15) == 0, VQ_ERR_WORKSPACE,
+    const size_t need = block_bytes(c);
+    VQ_REQUIRE(need == 0 || (a.workspace != nullptr && a.workspace_bytes >= need && ((uintptr_t)a.workspace & 15) == 0), VQ_ERR_WORKSPACE,
                "%s: workspace of %zu bytes required, 16-byte aligned", fn, need);
-    c.s.sums = (float *)a.workspace;
-    c.s.ml = c.s.sums + sums;
+    if (need > 0) {
+        int64_t sums;
+        (void)block_floats(c, sums);
+        c.s.sums = (float *)a.workspace;
+        c.s.ml = c.s.sums + sums;
+    }
+    if (c.few) {
+        if (int rc = a.pack_bits == 4 ? launch_blocks_few4(c.s, c.lists) : launch_blocks_few2(c.s, c.lists)) return rc;
+        return need > 0 ? launch_span_merge1(fn, c.s) : VQ_OK;
+    }
     blocks_any_kernel<<<(unsigned)cdiv(a.B * a.Hq * a.Sq * c.s.nparts, 4), 256, 0, (hipStream_t)a.stream>>>(c);
     VQ_HIP_CHECK_LAUNCH(fn);
     return launch_span_merge1(fn, c.s);

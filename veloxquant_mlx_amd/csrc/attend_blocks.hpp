@@ -9,6 +9,11 @@ struct BlockCall {
     SpanCall s;
     const int32_t *blocks;   // [B][Hkv][tiles][count]
     int64_t tiles, count, block_tokens, query_block;
+    int few;                 // 1: by the matrix-unit kernel for few rows (attend_span_few.hpp), with
+    BlockLists lists;
 };
+
+int launch_blocks_few2(const SpanCall &c, const BlockLists &l);
+int launch_blocks_few4(const SpanCall &c, const BlockLists &l);
 
 }  // namespace vq

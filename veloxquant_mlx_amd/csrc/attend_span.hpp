@@ -26,6 +26,18 @@ struct SpanCall {
     float *ml;             // [rows][nparts][maps][2]
 };
 
+// Lists of blocks of packed slots (attend_blocks.hip), one a tile of queries of a kv head, in units of 32 slots for the kernel for few rows: a
+// list's unit v is unit v % sub of its entry v / sub, then come the tail's.
+struct BlockLists {
+    const int32_t *blocks;          // [B][Hkv][tiles][count]
+    int tiles, count;               // lists a kv head, entries a list
+    int block_tokens, query_block;
+    int total;                      // blocks of the store
+    int sub, packed_units, units;   // units of an entry, of a list, and with the tail
+    int row_tiles;                  // tiles of rows of a tile of queries
+};
+constexpr int BLOCK_UNITS = 1024;   // units of a list that a block of threads walks, at most
+
 __device__ __forceinline__ int64_t span_own_live(const vq_store_attend_args &a, int64_t b) {
     const int64_t room = a.own.n_packed + a.own.n_tail;
     if (a.seq_lens == nullptr) return room;

@@ -31,7 +31,9 @@ template <int BITS, int D, int WAVES_> struct SpanFew {
     static_assert(RING >= 3 && LDS <= 160 * 1024, "room for a unit at work and two under way");
 };
 
-template <int BITS, int D, int MAPS, int WAVES> __device__ __forceinline__ void span_few_block(const SpanCall &c, int id) {
+// LISTS: the packed slots of the blocks that the row's list names, in place of all (one map, no prefix, no window).
+template <int BITS, int D, int MAPS, int WAVES, bool LISTS = false>
+__device__ __forceinline__ void span_few_block(const SpanCall &c, int id, const BlockLists &bl = {}) {
     extern __shared__ __align__(16) char lds[];
     using F = SpanFew<BITS, D, WAVES>;
     using M = SpanMma<f16>;
@@ -51,17 +53,17 @@ template <int BITS, int D, int MAPS, int WAVES> __device__ __forceinline__ void 
     const int b = shared ? 0 : id % (int)a.B;
     if (!shared) id /= (int)a.B;
     const int splits = shared ? c.psplits : c.osplits, split = id % splits, part = shared || !c.apart ? split : c.psplits + split;
-    const int rows = shared ? (int)a.B * r1 : r1;
-
     // ---- this lane's query row: positions outermost
     constexpr int ROWS = 32 / MAPS;
-    const int j0 = id / splits * ROWS, here = rows - j0 < ROWS ? rows - j0 : ROWS;   // the block's tile of rows
+    const int tile = LISTS ? id / splits / bl.row_tiles : 0, pos0 = LISTS ? tile * bl.query_block : 0;   // the tile of queries, its first
+    const int rows = LISTS ? G * (Sq - pos0 < bl.query_block ? Sq - pos0 : bl.query_block) : shared ? (int)a.B * r1 : r1;
+    const int j0 = (LISTS ? id / splits % bl.row_tiles : id / splits) * ROWS, here = rows - j0 < ROWS ? rows - j0 : ROWS;   // the block's tile of rows
     const int map = MAPS == 2 ? n >> 4 : 0, j = n % ROWS, jc = j < here ? j : here - 1;
     auto row_of = [&](int x, int &jb, int &pos) __attribute__((always_inline)) {   // flattened [B, Hq, Sq] row of tile row x
         x += j0;
         const int rem = shared ? x % r1 : x;
         jb = shared ? x / r1 : b;
-        pos = rem / G;
+        pos = pos0 + rem / G;
         return ((int64_t)jb * a.Hq + hkv * G + rem % G) * Sq + pos;
     };
     int jb, pos;
@@ -91,10 +93,45 @@ template <int BITS, int D, int MAPS, int WAVES> __device__ __forceinline__ void 
     const int np0 = shared || !c.apart ? (int)a.prefix.n_packed : 0, nt0 = shared || !c.apart ? (int)a.prefix.n_tail : 0;
     const int own = shared ? 0 : own_live, np1 = own < (int)a.own.n_packed ? own : (int)a.own.n_packed, nt1 = own - np1;
     const int tail0 = (int)a.prefix.n_packed, tail1 = before + (int)a.own.n_packed;
-    const int total = units_seen(0, np0) + units_seen(tail0, nt0) + units_seen(before, np1) + units_seen(tail1, nt1);
+    const int total = LISTS ? bl.units : units_seen(0, np0) + units_seen(tail0, nt0) + units_seen(before, np1) + units_seen(tail1, nt1);
     const int run = total / splits, longer = total % splits;   // (the first runs a unit longer)
     const int w0 = split * run + (split < longer ? split : longer), w1 = w0 + run + (split < longer ? 1 : 0);
-    if (w0 == w1 && c.nparts > 1) {   // (uniform) nothing: sums are not written
+    // ---- lists: the run's units of packed slots that some row sees, in order; then its units of the tail, from tail_u on
+    int *const listed = (int *)(lds + F::LDS);
+    int n_listed = 0, tail_u = 0, tail_units = 0;
+    if constexpr (LISTS) {
+        const int32_t *list = bl.blocks + (((int64_t)b * Hkv + hkv) * bl.tiles + tile) * bl.count;
+        const int limit = any_hi < np1 ? any_hi : np1, last = w1 < bl.packed_units ? w1 : bl.packed_units;
+        int *const taken = listed + BLOCK_UNITS;   // by each wave
+#pragma unroll 1
+        for (int v0 = w0; v0 < last; v0 += F::THREADS) {
+            const int v = v0 + tid;
+            int t0 = -1;
+            if (v < last) {
+                const int e = list[v / bl.sub];
+                if (e >= 0 && e < bl.total) t0 = e * bl.block_tokens + v % bl.sub * UNIT;
+            }
+            const bool take = t0 >= 0 && t0 < limit;
+            const uint64_t m = __ballot(take);
+            if (lane == 0) taken[wave] = __popcll(m);
+            lds_barrier();
+            int at = n_listed + __popcll(m & ((UINT64_C(1) << lane) - 1));
+#pragma unroll
+            for (int w = 0; w < F::WAVES; ++w) {
+                const int x = taken[w];
+                at += w < wave ? x : 0;
+                n_listed += x;
+            }
+            if (take) listed[at] = t0;
+            lds_barrier();
+        }
+        n_listed = __builtin_amdgcn_readfirstlane(n_listed);
+        tail_u = w0 > bl.packed_units ? w0 - bl.packed_units : 0;
+        const int seen = (any_hi < own_live ? any_hi : own_live) - tail1, most = (seen + UNIT - 1) / UNIT;
+        const int end = w1 - bl.packed_units < most ? w1 - bl.packed_units : most;
+        tail_units = end > tail_u ? end - tail_u : 0;
+    }
+    if ((LISTS ? n_listed + tail_units == 0 : w0 == w1) && c.nparts > 1) {   // (uniform) nothing: sums are not written
         if (tid < here * MAPS) {
             int x, y;
             *(float2 *)(c.ml + ((row_of(tid / MAPS, x, y) * c.nparts + part) * MAPS + tid % MAPS) * 2) = make_float2(-INFINITY, 0.f);
@@ -219,8 +256,14 @@ template <int BITS, int D, int MAPS, int WAVES> __device__ __forceinline__ void 
 #pragma unroll
         for (int i = 0; i < N; ++i) at[i] = lane_at(i, UNIT);
         int asked = t0, asked_live = live;
+        [[maybe_unused]] int next = 0;   // (lists)
         u32 fill = room;
         auto fetch = [&]() __attribute__((always_inline)) {
+            if constexpr (LISTS) {
+                asked = __builtin_amdgcn_readfirstlane(listed[wave + next * F::WAVES]);
+                asked_live = live - asked;
+                ++next;
+            }
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 const char *from = at[i];
@@ -231,14 +274,16 @@ template <int BITS, int D, int MAPS, int WAVES> __device__ __forceinline__ void 
                 from += off < F::WORDS ? key : off < 2 * F::WORDS ? value : off < 2 * F::WORDS + F::META ? kmeta : vmeta;
                 if (i * 1024 + 1024 <= F::RAW || lane * 16 < F::RAW - i * 1024) span_copy16(from, fill + i * 1024);
             }
-            asked += STEP;
-            asked_live -= STEP;
+            if constexpr (!LISTS) {
+                asked += STEP;
+                asked_live -= STEP;
+            }
             fill += F::RAW;
             if (fill == room + RING * F::RAW) fill = room;
         };
         const SpanMagic<BITS> magic;
         const char *take = room_p;
-        auto step = [&]() __attribute__((always_inline)) {
+        auto step = [&](int place, int live) __attribute__((always_inline)) {
             // scores
             f32x16 S;
 #pragma unroll
@@ -310,12 +355,17 @@ template <int BITS, int D, int MAPS, int WAVES> __device__ __forceinline__ void 
 #pragma unroll 1
         for (int i = 0; i < RING - 1 && i < count; ++i) fetch();
 #pragma unroll 1
-        for (int i = 0; i < count; ++i, place += STEP, live -= STEP) {
+        for (int i = 0; i < count; ++i, place += LISTS ? 0 : STEP, live -= LISTS ? 0 : STEP) {
             // this unit is here once at most the later ones' copies are under way; the slot that the unit before it has left is filled
             if (i + RING - 1 <= count) wait_copies<(RING - 2) * N>();
             else wait_copies<0>();
             if (i + RING - 1 < count) fetch();
-            step();
+            if constexpr (LISTS) {
+                const int t = __builtin_amdgcn_readfirstlane(listed[wave + i * F::WAVES]);
+                step(t, live - t);
+            } else {
+                step(place, live);
+            }
             // (the slot's reads are over before a copy may land in it)
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
@@ -371,7 +421,11 @@ template <int BITS, int D, int MAPS, int WAVES> __device__ __forceinline__ void 
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (the room's reads are over)
         }
     };
-    {
+    if constexpr (LISTS) {
+        if (wave < n_listed) walk_packed(1, 0, (n_listed - wave + F::WAVES - 1) / F::WAVES, 0, np1);
+        const int turn = (wave + F::WAVES - n_listed % F::WAVES) % F::WAVES, t0 = (tail_u + turn) * UNIT;
+        if (turn < tail_units) walk_rows(1, t0, (tail_units - turn + F::WAVES - 1) / F::WAVES, tail1 + t0, nt1 - t0);
+    } else {
         int skip = w0, left = w1 - w0, turn = wave;   // the wave's first unit of what is left
 #pragma unroll 1
         for (int which = 0; which < 2 && left > 0; ++which) {
@@ -518,6 +572,28 @@ int launch_span_few2(const SpanCall &c, int maps);
 int launch_span_few4(const SpanCall &c, int maps);
 int launch_span_both2(const SpanCall &c);
 int launch_span_both4(const SpanCall &c);
+
+// ---- lists of blocks
+constexpr int BLOCK_LDS = (BLOCK_UNITS + 8) * 4;   // their units, and a number a wave
+template <int BITS, int D, int WAVES>
+__global__ __launch_bounds__((64 * WAVES)) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2, D == 256 ? 1 : 2))) void blocks_few_kernel(SpanCall c, BlockLists bl) {
+    span_few_block<BITS, D, 1, WAVES, true>(c, (int)blockIdx.x, bl);
+}
+template <int BITS, int D, int WAVES> int launch_blocks_few_of(const SpanCall &c, const BlockLists &bl) {
+    constexpr int bytes = SpanFew<BITS, D, WAVES>::LDS + BLOCK_LDS;
+    static_assert(bytes <= 160 * 1024, "units beside the rooms");
+    const auto kernel = blocks_few_kernel<BITS, D, WAVES>;
+    static std::atomic<bool> allowed[64] = {};
+    if (int rc = span_allow_lds((const void *)kernel, bytes, allowed)) return rc;
+    kernel<<<(unsigned)(c.a.B * c.a.Hkv * c.osplits * bl.tiles * bl.row_tiles), 64 * WAVES, bytes, (hipStream_t)c.a.stream>>>(c, bl);
+    VQ_HIP_CHECK_LAUNCH("attention over blocks");
+    return VQ_OK;
+}
+template <int BITS> int launch_blocks_few_as(const SpanCall &c, const BlockLists &bl) {
+    if (c.a.D == 256) return launch_blocks_few_of<BITS, 256, 4>(c, bl);
+    if (c.a.D == 64) return c.owaves == 8 ? launch_blocks_few_of<BITS, 64, 8>(c, bl) : launch_blocks_few_of<BITS, 64, 4>(c, bl);
+    return c.owaves == 8 ? launch_blocks_few_of<BITS, 128, 8>(c, bl) : launch_blocks_few_of<BITS, 128, 4>(c, bl);
+}
 
 #define VQ_SPAN_FEW_LAUNCHER(NAME, BITS)                                                                                \
     namespace vq {                                                                                                      \
