@@ -128,6 +128,7 @@ def test_select_asks_for_a_workspace():
     assert lib.vq_block_select(_select(workspace=4096, workspace_bytes=need - 1)) == _lib.VQ_ERR_WORKSPACE
     assert lib.vq_block_select(_select(workspace=4097, workspace_bytes=need)) == _lib.VQ_ERR_WORKSPACE
     assert lib.vq_block_select_workspace(_select(count=10)) == 0      # every block is chosen
+    assert lib.vq_block_select_workspace(_select(n_packed=0)) == 0
 
 
 def test_select_blocks_refuses():

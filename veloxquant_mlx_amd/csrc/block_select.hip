@@ -9,6 +9,8 @@
 //
 // The chosen ones come out in ascending order, -1 behind them where fewer are visible: the first `first` and the last `recent` visible
 // blocks always, the others by score.
+#include <atomic>
+
 #include "common.hpp"
 
 namespace vq {
@@ -18,7 +20,16 @@ namespace {
 struct SelectCall {
     vq_block_select_args a;
     int64_t tiles, total;   // tiles of queries a sequence, blocks of the store
-    double *scores;         // [B][Hkv][tiles][total]
+    int64_t items;          // B Hkv tiles
+    double *scores;         // [items][total], of 64 bits (or room for them)
+    // the filter on the matrix units:
+    int mma;                // 1: it takes the call
+    int64_t query_block;    // (at most Sq)
+    int row_tiles;          // of 32 rows an item
+    int64_t groups;         // of the packed slots
+    int runs, run_units;    // waves a row tile, units of 32 groups of each
+    float *approx;          // [items][row_tiles][groups]
+    float *bounds;          // [items][row_tiles][runs]
 };
 
 __device__ __forceinline__ float sel_ld(const void *p, int tag, int64_t i) {
@@ -69,77 +80,463 @@ __global__ __launch_bounds__(256) void block_score_kernel(SelectCall c) {
     if (lane == 0) c.scores[id] = best;
 }
 
-// A block of threads a tile: the least score among the chosen by a radix select over the scores' bits, then the chosen in order.
-constexpr int PICK_THREADS = 256;
+// ---- the matrix units as a filter
+
+typedef uint32_t u32;
+typedef u32 u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ f16x2 as_h2(u32 x) { return __builtin_bit_cast(f16x2, x); }
+__device__ __forceinline__ u32 positive(u32 x) { return __builtin_bit_cast(u32, __builtin_elementwise_max(as_h2(x), f16x2{(f16)0.f, (f16)0.f})); }
+__device__ __forceinline__ u32 max_bits(u32 x, u32 y) {   // of two magnitudes each
+    return __builtin_bit_cast(u32, __builtin_elementwise_max(__builtin_bit_cast(u16x2, x), __builtin_bit_cast(u16x2, y)));
+}
+__device__ __forceinline__ f32x16 mma(u32x4 x, u32x4 y, f32x16 acc) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, y), acc, 0, 0, 0);
+}
+
+// Bounds of 32 rows (the query heads of a kv head at the queries of a tile) and 32 groups a step, in float32:
+//
+//   sum_c max(q z, q (z + L s)) = q . z + L (q+ . s+ + q- . s-),   x+ = max(x, 0), x- = max(-x, 0)
+//
+// products of fp16 numbers with v_mfma_f32_32x32x16 (the last one only where a scale is negative; lane n = lane % 32, h = lane / 32: row or group n,
+// channels 16 ks + 8 h ..).  A wave keeps its rows' queries, walks a run of units of 32 groups and writes each group's largest bound over its rows.
+// bf16 queries become fp16 numbers by a power of two that puts a row tile's largest near 2^15.  Float32 sums of D terms are off by less than
+// (D + 8) 2^-22 sum |q| (|z| + L |s|): with the largest sum of |q| and the largest |z| and |s| the wave also writes a bound of that sum, so the
+// choice knows how far to trust the scores.  Bound by the bytes of the scales and zeros for one query a sequence.
+template <int D, bool BF16> __global__ __launch_bounds__(256) void block_bound_kernel(SelectCall c) {
+    constexpr int KS = D / 16;
+    const vq_block_select_args &a = c.a;
+    const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
+    int64_t id = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (id >= c.items * c.row_tiles * c.runs) return;
+    const int run = (int)(id % c.runs);
+    const int64_t tile_row = id / c.runs;   // (item, row tile)
+    const int rt = (int)(tile_row % c.row_tiles);
+    const int64_t item = tile_row / c.row_tiles;
+    const int tile = (int)(item % c.tiles), hkv = (int)(item / c.tiles % a.Hkv), b = (int)(item / c.tiles / a.Hkv);
+    const int G = (int)(a.Hq / a.Hkv), g = a.group;
+    const int pos0 = tile * (int)c.query_block, last = (int)sel_last(a, tile), rows = (last - pos0 + 1) * G;
+    const int live = (int)sel_end(a, b, last), groups = (live + g - 1) / g;   // that some row sees
+    const int u0 = run * c.run_units * 32, u1 = u0 + c.run_units * 32 < groups ? u0 + c.run_units * 32 : groups;
+    float *const bound = c.bounds + id;
+    if (u0 >= u1) {
+        if (lane == 0) *bound = 0.f;
+        return;
+    }
+    auto row_at = [&](int x) __attribute__((always_inline)) { x += rt * 32; return x < rows ? x : rows - 1; };
+    u32x4 q[KS];
+    {
+        const int x = row_at(n);
+        const u16 *src = (const u16 *)a.q + (((int64_t)b * a.Hq + hkv * G + x % G) * a.Sq + pos0 + x / G) * D + 8 * h;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) q[k] = *(const u32x4 *)(src + 16 * k);
+    }
+    float unscale = 1.f;
+    if constexpr (BF16) {
+        u32 top = 0;
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top = max_bits(top, q[k][i] & 0x7FFF7FFFu);
+        top = top >> 16 > (top & 0xFFFFu) ? top >> 16 : top & 0xFFFFu;
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) { const u32 o = __shfl_xor(top, off); top = o > top ? o : top; }
+        // 2^(141 - e) with e the largest's exponent field: below 2^15; what is not finite stays so
+        const int e = (int)(top >> 7), up = e == 0 || e == 255 ? 0 : 141 - e;
+        const int up1 = up / 2, up2 = up - up1;   // (either factor is a normal number)
+        const float f1 = __uint_as_float((u32)(127 + up1) << 23), f2 = __uint_as_float((u32)(127 + up2) << 23);
+        unscale = __uint_as_float((u32)(127 - up1) << 23);
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float x = __uint_as_float(q[k][i] << 16) * f1 * f2, y = __uint_as_float(q[k][i] & 0xFFFF0000u) * f1 * f2;
+                q[k][i] = __builtin_bit_cast(u32, f16x2{(f16)x, (f16)y});
+            }
+        unscale *= __uint_as_float((u32)(127 - up2) << 23);
+    }
+    const float levels = (float)a.levels;
+    float size = 0.f;   // the largest row's sum of magnitudes
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) size += __builtin_fabsf((float)as_h2(q[k][i])[0]) + __builtin_fabsf((float)as_h2(q[k][i])[1]);
+    size += __shfl_xor(size, 32);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) { const float o = __shfl_xor(size, off); size = o > size || o != o ? o : size; }
+
+    const int64_t stride = (a.cap_tokens + g - 1) / g, bh = (int64_t)b * a.Hkv + hkv;
+    const int seen = (int)sel_end(a, b, pos0);   // by every query
+    float *const out = c.approx + tile_row * c.groups;
+    u32 top_z = 0, top_s = 0;
+#pragma unroll 1
+    for (int u = u0; u < u1; u += 32) {
+        const int at = u + n < u1 ? u + n : u1 - 1;
+        const u16 *zero = (const u16 *)a.k_zero + (bh * stride + at) * D + 8 * h, *scale = (const u16 *)a.k_scale + (bh * stride + at) * D + 8 * h;
+        u32x4 z[KS], s[KS];
+#pragma unroll
+        for (int k = 0; k < KS; ++k) { z[k] = *(const u32x4 *)(zero + 16 * k); s[k] = *(const u32x4 *)(scale + 16 * k); }
+        f32x16 S, W;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) S[r] = W[r] = 0.f;
+        u32 sign = 0;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            S = mma(q[k], z[k], S);
+            u32x4 p;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                sign |= s[k][i];
+                top_z = max_bits(top_z, z[k][i] & 0x7FFF7FFFu);
+                top_s = max_bits(top_s, s[k][i] & 0x7FFF7FFFu);
+                p[i] = positive(q[k][i]);
+            }
+            W = mma(p, s[k], W);
+        }
+        if (__any((sign & 0x80008000u) != 0)) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) W[r] = 0.f;
+#pragma unroll 1
+            for (int m = 0; m < 2; ++m) {
+                const u32 flip = m ? 0x80008000u : 0u;
+#pragma unroll
+                for (int k = 0; k < KS; ++k) {
+                    u32x4 p, y;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) { p[i] = positive(q[k][i] ^ flip); y[i] = positive(s[k][i] ^ flip); }
+                    W = mma(p, y, W);
+                }
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) S[r] = __builtin_fmaf(levels, W[r], S[r]);
+        if ((u + 31) * (int64_t)g >= seen) {   // groups that some queries do not see (in 64 bits: the last ones may lie past the store)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int x = row_at(8 * (r / 4) + 4 * h + r % 4);
+                if (at * g >= (int)sel_end(a, b, pos0 + x / G)) S[r] = -INFINITY;
+            }
+        }
+        float best = S[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) best = fmaxf(best, S[r]);
+        best = fmaxf(best, __shfl_xor(best, 32)) * unscale;
+        if (h == 0 && u + n < u1) out[u + n] = best;
+    }
+    top_z = max_bits(top_z, __builtin_amdgcn_alignbyte(top_z, top_z, 2));
+    top_s = max_bits(top_s, __builtin_amdgcn_alignbyte(top_s, top_s, 2));
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) { top_z = max_bits(top_z, __shfl_xor(top_z, off)); top_s = max_bits(top_s, __shfl_xor(top_s, off)); }
+    const float mz = (float)__builtin_bit_cast(f16, (u16)top_z), ms = (float)__builtin_bit_cast(f16, (u16)top_s);
+    if (lane == 0) *bound = size * (mz + levels * ms) * unscale;   // (not finite where a query, scale or zero is not)
+}
+
+// ---- the choice
+
 __device__ __forceinline__ uint64_t pick_key(double s) {   // ascending with the score, NaN above all
     if (s != s) return ~UINT64_C(0);
     const uint64_t u = (uint64_t)__double_as_longlong(s + 0.);
     return u >> 63 ? ~u : u | (UINT64_C(1) << 63);
 }
-__global__ __launch_bounds__(PICK_THREADS) void block_pick_kernel(SelectCall c) {
-    const vq_block_select_args &a = c.a;
-    __shared__ uint32_t hist[256];
-    __shared__ uint32_t waves[2][PICK_THREADS / 64];
-    __shared__ uint64_t s_key;
-    __shared__ int64_t s_left;
+__device__ __forceinline__ uint64_t max_key(uint64_t x, uint64_t y) { return x > y ? x : y; }
+__device__ __forceinline__ double shfl_add(double s, int off) { return s + __shfl_xor(s, off); }
+
+// The key of block j's score in 64 bits, by a wave: 64 / R lanes a row (R the rows, up to the next power of two), eight channels at a time.
+__device__ __forceinline__ uint64_t exact_key(const vq_block_select_args &a, int64_t b, int64_t hkv, int64_t tile, int64_t j) {
+    const int lane = threadIdx.x & 63, G = (int)(a.Hq / a.Hkv), D = (int)a.D, g = a.group;
+    const int pos0 = (int)(tile * a.query_block), rows = ((int)sel_last(a, tile) - pos0 + 1) * G;
+    int many = 1;
+    while (many < rows && many < 64) many <<= 1;
+    const int parts = 64 / many, part = lane % parts;
+    const int64_t groups = (a.cap_tokens + g - 1) / g;
+    uint64_t best = 0;
+    for (int r0 = 0; r0 < rows; r0 += many) {
+        const int r = r0 + lane / parts, x = r < rows ? r : rows - 1;
+        const int64_t end = sel_end(a, b, pos0 + x / G);
+        const u16 *q = (const u16 *)a.q + ((b * a.Hq + hkv * G + x % G) * a.Sq + pos0 + x / G) * D;
+        for (int64_t t = j * a.block_tokens; t < (j + 1) * a.block_tokens && t < a.n_packed; t += g) {
+            const int64_t at = ((b * a.Hkv + hkv) * groups + t / g) * D;
+            double s = 0.;
+            for (int d = part * 8; d < D; d += parts * 8) {
+                const u32x4 x4 = *(const u32x4 *)(q + d), z4 = *(const u32x4 *)((const u16 *)a.k_zero + at + d), s4 = *(const u32x4 *)((const u16 *)a.k_scale + at + d);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const u16 xb = (u16)(x4[i / 2] >> (16 * (i & 1)));
+                    const double y = a.dtype == VQ_BF16 ? (double)bf16_to_f32(xb) : (double)(float)__builtin_bit_cast(f16, xb);
+                    const double z = (double)(float)as_h2(z4[i / 2])[i & 1], r1 = y * (double)(float)as_h2(s4[i / 2])[i & 1] * a.levels;
+                    s += y * z + (r1 > 0. || r1 != r1 ? r1 : 0.);
+                }
+            }
+            for (int off = 1; off < parts; off <<= 1) s = shfl_add(s, off);
+            if (t < end) best = max_key(best, pick_key(s));
+        }
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) best = max_key(best, __shfl_xor((unsigned long long)best, off));
+    return best;
+}
+
+constexpr int PICK_THREADS = 256, PICK_WAVES = PICK_THREADS / 64;
+constexpr int PICK_MOST = 16384;   // blocks whose scores are held in LDS
+constexpr int PICK_LIST = 512;     // blocks that are told apart in 64 bits there
+
+// Sum over the threads below this one, and the total (`waves`: a number a wave, in LDS; a barrier before its next use).
+__device__ __forceinline__ u32 block_before(bool mine, u32 &total, u32 *waves) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint64_t m = __ballot(mine);
+    __syncthreads();
+    if (lane == 0) waves[wave] = (u32)__popcll(m);
+    __syncthreads();
+    u32 before = (u32)__popcll(m & ((UINT64_C(1) << lane) - 1));
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < PICK_WAVES; ++w) {
+        const u32 x = waves[w];
+        before += w < wave ? x : 0;
+        total += x;
+    }
+    return before;
+}
+
+// `left` becomes how many are to be taken of the bin it returns, counted from the highest bin down; hist[256] is read by its threads
+// (a barrier after the last count).  Suffix sums: of the bins above within the wave, then of the waves above.
+__device__ __forceinline__ int pick_bin(const u32 *hist, u32 &left, u32 *found) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int64_t row = blockIdx.x, tile = row % c.tiles, b = row / c.tiles / a.Hkv;
-    const int64_t V = (sel_end(a, b, sel_last(a, tile)) + a.block_tokens - 1) / a.block_tokens;
-    int32_t *out = a.out + row * a.count;
+    const u32 mine = hist[tid];
+    u32 sum = mine;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) { const u32 o = __shfl_down(sum, off); sum += lane + off < 64 ? o : 0; }
+    if (lane == 0) found[2 + wave] = sum;
+    __syncthreads();
+    u32 above = sum - mine;
+#pragma unroll
+    for (int w = 1; w < PICK_WAVES; ++w) above += w > wave ? found[2 + w] : 0;
+    if (above < left && above + mine >= left) { found[0] = (u32)tid; found[1] = left - above; }
+    __syncthreads();
+    left = found[1];
+    return (int)found[0];
+}
+
+// A block of threads a tile.  STORED: scores of 64 bits lie in memory, their float32 roundings are the approximate ones; else those of the matrix units.
+//
+// The kth best is looked for among the approximate scores by bins between the smallest and the largest, again inside its bin while
+// that holds many.  With scores off by e at most, those above the bin's largest + 2 e are among the chosen, those below its smallest - 2 e are
+// not; the few between are told apart by their scores in 64 bits.  Where these are more than PICK_LIST (equal scores, values that are not
+// finite, which make e so) all of them are, by a radix select over the bits.
+template <bool STORED> __global__ __launch_bounds__(PICK_THREADS) void block_pick_kernel(SelectCall c) {
+    const vq_block_select_args &a = c.a;
+    extern __shared__ float keys[];   // of the blocks [lo, hi)
+    __shared__ u32 hist[256], waves[PICK_WAVES], found[2 + PICK_WAVES];
+    __shared__ float low[PICK_WAVES], high[PICK_WAVES], off_by[PICK_WAVES];
+    __shared__ int list[PICK_LIST];
+    __shared__ uint64_t exact[PICK_LIST];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int64_t item = blockIdx.x, tile = item % c.tiles, hkv = item / c.tiles % a.Hkv, b = item / c.tiles / a.Hkv;
+    const int64_t end = sel_end(a, b, sel_last(a, tile)), V = (end + a.block_tokens - 1) / a.block_tokens;
+    int32_t *out = a.out + item * a.count;
     if (V <= a.count) {
         for (int64_t i = tid; i < a.count; i += PICK_THREADS) out[i] = i < V ? (int32_t)i : -1;
         return;
     }
-    const double *score = c.scores + row * c.total;
-    const int64_t lo = a.first, hi = V - a.recent, want = a.count - a.first - a.recent;   // of [lo, hi)
+    const int lo = (int)a.first, hi = (int)(V - a.recent), n = hi - lo;
+    const u32 want = (u32)(a.count - a.first - a.recent);   // of [lo, hi), which holds more
     for (int64_t i = tid; i < a.first; i += PICK_THREADS) out[i] = (int32_t)i;
     for (int64_t i = tid; i < a.recent; i += PICK_THREADS) out[a.count - a.recent + i] = (int32_t)(hi + i);
     if (want == 0) return;
+    double *const score = c.scores + item * c.total;
+
+    // ---- approximate scores, their range and how far they may be off
+    float least = INFINITY, most = -INFINITY, e = 0.f;
+    bool odd = false;   // something is not finite
+    for (int j = tid; j < n; j += PICK_THREADS) {
+        float x = -INFINITY;
+        if (STORED) {
+            x = (float)score[lo + j];
+        } else {
+            const int g = a.group, per = (int)(a.block_tokens / g), u0 = (lo + j) * per, seen = (int)((end + g - 1) / g), u1 = u0 + per < seen ? u0 + per : seen;
+            for (int rt = 0; rt < c.row_tiles; ++rt)
+                for (int u = u0; u < u1; ++u) {
+                    const float y = c.approx[(item * c.row_tiles + rt) * c.groups + u];
+                    x = fmaxf(x, y);
+                }
+        }
+        keys[j] = x;
+        odd = odd || !(__builtin_fabsf(x) < INFINITY);
+        least = fminf(least, x);
+        most = fmaxf(most, x);
+    }
+    if (STORED) {
+        e = fmaxf(__builtin_fabsf(least), __builtin_fabsf(most)) * 0x1p-23f;
+    } else {
+        for (int i = tid; i < c.row_tiles * c.runs; i += PICK_THREADS) {
+            const float y = c.bounds[item * c.row_tiles * c.runs + i];
+            odd = odd || !(y < INFINITY);
+            e = fmaxf(e, y);
+        }
+        e *= (float)(a.D + 8) * 0x1p-22f;
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+        least = fminf(least, __shfl_xor(least, off));
+        most = fmaxf(most, __shfl_xor(most, off));
+        e = fmaxf(e, __shfl_xor(e, off));
+    }
+    if (__any(odd)) e = INFINITY;
+    if (lane == 0) { low[wave] = least; high[wave] = most; off_by[wave] = e; }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < PICK_WAVES; ++w) { least = fminf(least, low[w]); most = fmaxf(most, high[w]); e = fmaxf(e, off_by[w]); }
+    e = 2.f * e + 0x1p-100f;   // of two scores' difference, also where products are too small for float32
+
+    // ---- the bin of the kth best
+    u32 left = want, among = (u32)n;
+    float from = least, to = most;
+    if (e < INFINITY) {
+        for (int pass = 0; pass < 4 && among > 8 && to - from > e; ++pass) {
+            const float by = 255.f / (to - from);   // (bin 255: the largest alone)
+            hist[tid] = 0;
+            __syncthreads();
+            for (int j = tid; j < n; j += PICK_THREADS) {
+                const float x = keys[j];
+                if (x >= from && x <= to) atomicAdd(&hist[(int)((x - from) * by) & 255], 1u);
+            }
+            __syncthreads();
+            const int bin = pick_bin(hist, left, found);
+            among = hist[bin];
+            float l = INFINITY, m = -INFINITY;
+            for (int j = tid; j < n; j += PICK_THREADS) {
+                const float x = keys[j];
+                if (x >= from && x <= to && ((int)((x - from) * by) & 255) == bin) { l = fminf(l, x); m = fmaxf(m, x); }
+            }
+#pragma unroll
+            for (int off = 32; off > 0; off >>= 1) { l = fminf(l, __shfl_xor(l, off)); m = fmaxf(m, __shfl_xor(m, off)); }
+            __syncthreads();
+            if (lane == 0) { low[wave] = l; high[wave] = m; }
+            __syncthreads();
+            from = low[0]; to = high[0];
+#pragma unroll
+            for (int w = 1; w < PICK_WAVES; ++w) { from = fminf(from, low[w]); to = fmaxf(to, high[w]); }
+        }
+    }
+    const float over = e < INFINITY ? to + e : INFINITY, under = e < INFINITY ? from - e : -INFINITY;
+
+    // ---- those between
+    u32 sure = 0, doubt = 0;
+    __syncthreads();
+    for (int j0 = 0; j0 < n; j0 += PICK_THREADS) {
+        const float x = j0 + tid < n ? keys[j0 + tid] : -INFINITY;
+        const bool here = j0 + tid < n, in = here && x > over, maybe = here && !in && !(x < under);
+        u32 some;
+        const u32 at = block_before(maybe, some, waves);
+        if (maybe && doubt + at < PICK_LIST) list[doubt + at] = j0 + tid;
+        doubt += some;
+        (void)block_before(in, some, waves);
+        sure += some;
+    }
+    const u32 need = want - sure;   // of the doubtful
+    __syncthreads();
+    if (doubt > PICK_LIST) {
+        // all of them by their bits; the sure ones as the highest
+        for (int j = wave; j < n; j += PICK_WAVES) {
+            const float x = keys[j];
+            uint64_t k;
+            if (x > over) k = ~UINT64_C(0);
+            else if (x < under) k = 0;
+            else k = STORED ? pick_key(score[lo + j]) : exact_key(a, b, hkv, tile, lo + j);
+            if (lane == 0) ((uint64_t *)score)[lo + j] = k;
+        }
+        __threadfence_block();
+        __syncthreads();
+        const uint64_t *all = (const uint64_t *)score + lo;
+        uint64_t key = 0;
+        left = want;
+        for (int shift = 56; shift >= 0; shift -= 8) {
+            hist[tid] = 0;
+            __syncthreads();
+            for (int j = tid; j < n; j += PICK_THREADS)
+                if (shift == 56 || (all[j] ^ key) >> (shift + 8) == 0) atomicAdd(&hist[all[j] >> shift & 255], 1u);
+            __syncthreads();
+            key |= (uint64_t)pick_bin(hist, left, found) << shift;
+            __syncthreads();
+        }
+        u32 equal = 0;
+        for (int j0 = 0; j0 < n; j0 += PICK_THREADS) {
+            const int j = j0 + tid;
+            u32 some;
+            const u32 rank = equal + block_before(j < n && all[j] == key, some, waves);
+            equal += some;
+            if (j < n) keys[j] = all[j] > key || (all[j] == key && rank < left) ? INFINITY : -INFINITY;
+        }
+    } else if (doubt > need) {
+        for (u32 i = wave; i < doubt; i += PICK_WAVES) {
+            const uint64_t k = STORED ? pick_key(score[lo + list[i]]) : exact_key(a, b, hkv, tile, lo + list[i]);
+            if (lane == 0) exact[i] = k;
+        }
+        __syncthreads();
+        for (u32 i = tid; i < doubt; i += PICK_THREADS) {
+            const uint64_t k = exact[i];
+            u32 better = 0;   // (the list ascends: of equal scores the lower block comes first)
+            for (u32 o = 0; o < doubt; ++o) better += exact[o] > k || (exact[o] == k && o < i) ? 1 : 0;
+            keys[list[i]] = better < need ? INFINITY : -INFINITY;
+        }
+    } else {
+        for (u32 i = tid; i < doubt; i += PICK_THREADS) keys[list[i]] = INFINITY;
+    }
+    __syncthreads();
+    // ---- in order
+    u32 done = 0;
+    for (int j0 = 0; j0 < n; j0 += PICK_THREADS) {
+        const bool take = j0 + tid < n && (keys[j0 + tid] == INFINITY || keys[j0 + tid] > over);
+        u32 some;
+        const u32 at = done + block_before(take, some, waves);
+        if (take) out[lo + at] = lo + j0 + tid;
+        done += some;
+    }
+}
+
+// The same over any number of blocks, their scores of 64 bits in memory throughout.
+__global__ __launch_bounds__(PICK_THREADS) void block_pick_any_kernel(SelectCall c) {
+    const vq_block_select_args &a = c.a;
+    __shared__ u32 hist[256], waves[PICK_WAVES], found[2 + PICK_WAVES];
+    const int tid = threadIdx.x;
+    const int64_t item = blockIdx.x, tile = item % c.tiles, b = item / c.tiles / a.Hkv;
+    const int64_t V = (sel_end(a, b, sel_last(a, tile)) + a.block_tokens - 1) / a.block_tokens;
+    int32_t *out = a.out + item * a.count;
+    if (V <= a.count) {
+        for (int64_t i = tid; i < a.count; i += PICK_THREADS) out[i] = i < V ? (int32_t)i : -1;
+        return;
+    }
+    const double *score = c.scores + item * c.total;
+    const int lo = (int)a.first, hi = (int)(V - a.recent);
+    u32 left = (u32)(a.count - a.first - a.recent);
+    for (int64_t i = tid; i < a.first; i += PICK_THREADS) out[i] = (int32_t)i;
+    for (int64_t i = tid; i < a.recent; i += PICK_THREADS) out[a.count - a.recent + i] = (int32_t)(hi + i);
+    if (left == 0) return;
     uint64_t key = 0;
-    int64_t left = want;   // how many of those that share the key's upper bits
     for (int shift = 56; shift >= 0; shift -= 8) {
         hist[tid] = 0;
         __syncthreads();
-        for (int64_t j = lo + tid; j < hi; j += PICK_THREADS) {
+        for (int j = lo + tid; j < hi; j += PICK_THREADS) {
             const uint64_t k = pick_key(score[j]);
             if (shift == 56 || (k ^ key) >> (shift + 8) == 0) atomicAdd(&hist[k >> shift & 255], 1u);
         }
         __syncthreads();
-        if (tid == 0) {
-            int64_t above = 0;
-            int digit = 255;
-            while (digit > 0 && above + hist[digit] < left) above += hist[digit--];
-            s_key = key | (uint64_t)digit << shift;
-            s_left = left - above;
-        }
+        key |= (uint64_t)pick_bin(hist, left, found) << shift;
         __syncthreads();
-        key = s_key;
-        left = s_left;
     }
-    // those above the key, and the first `left` of those that equal it
-    int64_t done = 0, equal = 0;
-    for (int64_t j0 = lo; j0 < hi; j0 += PICK_THREADS) {
-        const int64_t j = j0 + tid;
+    u32 done = 0, equal = 0;
+    for (int j0 = lo; j0 < hi; j0 += PICK_THREADS) {
+        const int j = j0 + tid;
         const uint64_t k = j < hi ? pick_key(score[j]) : 0;
-        const bool eq = j < hi && k == key, gt = j < hi && k > key;
-        const uint64_t e = __ballot(eq), below = (UINT64_C(1) << lane) - 1;
-        if (lane == 0) waves[0][wave] = (uint32_t)__popcll(e);
-        __syncthreads();
-        int64_t rank = equal + __popcll(e & below);
-        for (int w = 0; w < PICK_THREADS / 64; ++w) {
-            if (w < wave) rank += waves[0][w];
-            equal += waves[0][w];
-        }
-        const bool take = gt || (eq && rank < left);
-        const uint64_t m = __ballot(take);
-        if (lane == 0) waves[1][wave] = (uint32_t)__popcll(m);
-        __syncthreads();
-        int64_t at = done + __popcll(m & below);
-        for (int w = 0; w < PICK_THREADS / 64; ++w) {
-            if (w < wave) at += waves[1][w];
-            done += waves[1][w];
-        }
-        if (take) out[lo + at] = (int32_t)j;
+        u32 some;
+        const u32 rank = equal + block_before(j < hi && k == key, some, waves);
+        equal += some;
+        const bool take = j < hi && (k > key || (k == key && rank < left));
+        const u32 at = done + block_before(take, some, waves);
+        if (take) out[lo + at] = j;
+        done += some;
     }
 }
 
@@ -175,9 +572,56 @@ SelectCall cut_select(const vq_block_select_args &a) {
     c.a = a;
     c.tiles = cdiv(a.Sq, a.query_block);
     c.total = cdiv(a.n_packed, a.block_tokens);
+    c.items = a.B * a.Hkv * c.tiles;
+    c.query_block = a.query_block < a.Sq ? a.query_block : a.Sq;
+    c.groups = cdiv(a.n_packed, a.group);
+    c.row_tiles = (int)cdiv(a.Hq / a.Hkv * c.query_block, 32);
+    if (c.total <= a.count) return c;   // every visible block is chosen: no scores
+    c.mma = (a.D == 64 || a.D == 128 || a.D == 256) && a.dtype != VQ_F32 && a.meta_dtype == VQ_F16 && c.total <= PICK_MOST &&
+            (((uintptr_t)a.q | (uintptr_t)a.k_scale | (uintptr_t)a.k_zero) & 15) == 0;
+    if (c.mma) {
+        // a unit a wave until sixteen waves a CU have work
+        const int64_t units = cdiv(c.groups, 32), waves = c.items * c.row_tiles * units;
+        c.run_units = (int)cdiv(waves, 4096);
+        if (c.run_units > units) c.run_units = (int)units;
+        c.runs = (int)cdiv(units, c.run_units);
+        // (the products and the grid of a call of this size are left to the vector units)
+        if ((double)c.items * c.row_tiles * (double)c.groups >= 67108864.) c.mma = 0;
+    }
     return c;
 }
-size_t select_bytes(const SelectCall &c) { return c.total <= c.a.count ? 0 : (size_t)(c.a.B * c.a.Hkv * c.tiles * c.total) * 8; }
+struct SelectRoom { size_t scores, approx, bounds, all; };
+SelectRoom select_room(const SelectCall &c) {
+    SelectRoom r = {};
+    if (c.total <= c.a.count) return r;
+    auto whole = [](size_t n) { return (n + 15) / 16 * 16; };
+    r.approx = whole((size_t)(c.items * c.total) * 8);
+    r.bounds = r.all = r.approx;
+    if (c.mma) {
+        r.bounds = r.approx + whole((size_t)(c.items * c.row_tiles * c.groups) * 4);
+        r.all = r.bounds + whole((size_t)(c.items * c.row_tiles * c.runs) * 4);
+    }
+    return r;
+}
+
+// (the scores of up to PICK_MOST blocks and the tables beside them pass the 64 KB that a block has unasked)
+template <bool STORED> int allow_lds(const char *fn, size_t bytes) {
+    if (bytes <= 48 * 1024) return VQ_OK;
+    static std::atomic<bool> allowed[64] = {};
+    int dev = 0;
+    (void)hipGetDevice(&dev);
+    if (dev >= 0 && dev < 64 && allowed[dev].load(std::memory_order_acquire)) return VQ_OK;
+    const hipError_t e = hipFuncSetAttribute((const void *)block_pick_kernel<STORED>, hipFuncAttributeMaxDynamicSharedMemorySize, PICK_MOST * 4);
+    VQ_REQUIRE(e == hipSuccess, VQ_ERR_HIP, "%s: %d bytes of block-shared memory: %s", fn, PICK_MOST * 4, hipGetErrorString(e));
+    if (dev >= 0 && dev < 64) allowed[dev].store(true, std::memory_order_release);
+    return VQ_OK;
+}
+
+template <int D> void launch_bounds(const SelectCall &c, hipStream_t st) {
+    const unsigned blocks = (unsigned)cdiv(c.items * c.row_tiles * c.runs, 4);
+    if (c.a.dtype == VQ_BF16) block_bound_kernel<D, true><<<blocks, 256, 0, st>>>(c);
+    else block_bound_kernel<D, false><<<blocks, 256, 0, st>>>(c);
+}
 
 }  // namespace
 
@@ -186,7 +630,7 @@ size_t select_bytes(const SelectCall &c) { return c.total <= c.a.count ? 0 : (si
 extern "C" size_t vq_block_select_workspace(const vq_block_select_args *args) {
     using namespace vq;
     if (check_select("vq_block_select", args) != VQ_OK) return 0;
-    return select_bytes(cut_select(*args));
+    return select_room(cut_select(*args)).all;
 }
 
 extern "C" int vq_block_select(const vq_block_select_args *args) {
@@ -195,17 +639,30 @@ extern "C" int vq_block_select(const vq_block_select_args *args) {
     if (int rc = check_select(fn, args)) return rc;
     SelectCall c = cut_select(*args);
     const vq_block_select_args &a = c.a;
-    const size_t need = select_bytes(c);
-    VQ_REQUIRE(need == 0 || (a.workspace != nullptr && a.workspace_bytes >= need && ((uintptr_t)a.workspace & 15) == 0), VQ_ERR_WORKSPACE,
-               "%s: workspace of %zu bytes required, 16-byte aligned", fn, need);
-    c.scores = (double *)a.workspace;
+    const SelectRoom room = select_room(c);
+    VQ_REQUIRE(room.all == 0 || (a.workspace != nullptr && a.workspace_bytes >= room.all && ((uintptr_t)a.workspace & 15) == 0), VQ_ERR_WORKSPACE,
+               "%s: workspace of %zu bytes required, 16-byte aligned", fn, room.all);
     hipStream_t st = (hipStream_t)a.stream;
-    const int64_t rows = a.B * a.Hkv * c.tiles;
-    if (need > 0) {
-        block_score_kernel<<<(unsigned)cdiv(rows * c.total, 4), 256, 0, st>>>(c);
+    const size_t lds = room.all > 0 && c.total <= PICK_MOST ? (size_t)c.total * 4 : 0;   // (no scores: every block is chosen)
+    if (room.all > 0) {
+        c.scores = (double *)a.workspace;
+        c.approx = (float *)((char *)a.workspace + room.approx);
+        c.bounds = (float *)((char *)a.workspace + room.bounds);
+        if (!c.mma) block_score_kernel<<<(unsigned)cdiv(c.items * c.total, 4), 256, 0, st>>>(c);
+        else if (a.D == 64) launch_bounds<64>(c, st);
+        else if (a.D == 128) launch_bounds<128>(c, st);
+        else launch_bounds<256>(c, st);
         VQ_HIP_CHECK_LAUNCH(fn);
     }
-    block_pick_kernel<<<(unsigned)rows, PICK_THREADS, 0, st>>>(c);
+    if (c.total > PICK_MOST) {
+        block_pick_any_kernel<<<(unsigned)c.items, PICK_THREADS, 0, st>>>(c);
+    } else if (c.mma) {
+        if (int rc = allow_lds<false>(fn, lds)) return rc;
+        block_pick_kernel<false><<<(unsigned)c.items, PICK_THREADS, lds, st>>>(c);
+    } else {
+        if (int rc = allow_lds<true>(fn, lds)) return rc;
+        block_pick_kernel<true><<<(unsigned)c.items, PICK_THREADS, lds, st>>>(c);
+    }
     VQ_HIP_CHECK_LAUNCH(fn);
     return VQ_OK;
 }
