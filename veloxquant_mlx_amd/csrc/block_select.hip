@@ -26,7 +26,7 @@ struct SelectCall {
     int mma;                // 1: it takes the call
     int64_t query_block;    // (at most Sq)
     int row_tiles;          // of 32 rows an item
-    int64_t groups;         // of the packed slots
+    int64_t groups, stride; // of the packed slots, of the store
     int runs, run_units;    // waves a row tile, units of 32 groups of each
     float *approx;          // [items][row_tiles][groups]
     float *bounds;          // [items][row_tiles][runs]
@@ -38,18 +38,21 @@ __device__ __forceinline__ float sel_ld(const void *p, int tag, int64_t i) {
     return ((const float *)p)[i];
 }
 
-// slots [0, end) of the packed ones that query i of sequence b sees
-__device__ __forceinline__ int64_t sel_end(const vq_block_select_args &a, int64_t b, int64_t i) {
-    const int64_t room = a.n_packed + a.n_tail;
-    int64_t live = a.seq_lens == nullptr ? room : a.seq_lens[b];
-    live = live < 0 ? 0 : live < room ? live : room;
-    int64_t end = a.causal ? live - a.Sq + i + 1 : live;
+// slots [0, end) of the packed ones that query i of sequence b sees (slots and queries: below 2^30)
+__device__ __forceinline__ int sel_end(const vq_block_select_args &a, int b, int i) {
+    const int packed = (int)a.n_packed, room = packed + (int)a.n_tail;
+    int live = room;
+    if (a.seq_lens != nullptr) {
+        const int64_t n = a.seq_lens[b];
+        live = n < 0 ? 0 : n < room ? (int)n : room;
+    }
+    int end = a.causal ? live - (int)a.Sq + i + 1 : live;
     end = end < live ? end : live;
-    return end < 0 ? 0 : end < a.n_packed ? end : a.n_packed;
+    return end < 0 ? 0 : end < packed ? end : packed;
 }
-__device__ __forceinline__ int64_t sel_last(const vq_block_select_args &a, int64_t tile) {
-    const int64_t last = (tile + 1) * a.query_block;
-    return (last < a.Sq ? last : a.Sq) - 1;
+__device__ __forceinline__ int sel_last(const vq_block_select_args &a, int tile) {
+    const int64_t last = (tile + INT64_C(1)) * a.query_block;
+    return (int)(last < a.Sq ? last : a.Sq) - 1;
 }
 
 // A wave a (tile, block): lanes along the channels.
@@ -59,11 +62,11 @@ __global__ __launch_bounds__(256) void block_score_kernel(SelectCall c) {
     const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (id >= a.B * a.Hkv * c.tiles * c.total) return;
     const int64_t j = id % c.total, tile = id / c.total % c.tiles, bh = id / (c.total * c.tiles), hkv = bh % a.Hkv, b = bh / a.Hkv;
-    const int64_t G = a.Hq / a.Hkv, i1 = sel_last(a, tile), groups = (a.cap_tokens + a.group - 1) / a.group;
+    const int64_t G = a.Hq / a.Hkv, i1 = sel_last(a, (int)tile), groups = (a.cap_tokens + a.group - 1) / a.group;
     double best = -INFINITY;
     for (int64_t t = j * a.block_tokens; t < (j + 1) * a.block_tokens; t += a.group)
         for (int64_t i = tile * a.query_block; i <= i1; ++i) {
-            if (t >= sel_end(a, b, i)) continue;
+            if (t >= sel_end(a, (int)b, (int)i)) continue;
             for (int64_t g = 0; g < G; ++g) {
                 double s = 0.;
                 for (int64_t d = lane; d < a.D; d += 64) {
@@ -105,18 +108,19 @@ __device__ __forceinline__ f32x16 mma(u32x4 x, u32x4 y, f32x16 acc) {
 // bf16 queries become fp16 numbers by a power of two that puts a row tile's largest near 2^15.  Float32 sums of D terms are off by less than
 // (D + 8) 2^-22 sum |q| (|z| + L |s|): with the largest sum of |q| and the largest |z| and |s| the wave also writes a bound of that sum, so the
 // choice knows how far to trust the scores.  Bound by the bytes of the scales and zeros for one query a sequence.
-template <int D, bool BF16> __global__ __launch_bounds__(256) void block_bound_kernel(SelectCall c) {
+template <int D, bool BF16> __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void block_bound_kernel(SelectCall c) {
     constexpr int KS = D / 16;
+    constexpr bool AHEAD = D <= 128;   // room for the next unit's scales and zeros beside this one's
     const vq_block_select_args &a = c.a;
     const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
-    int64_t id = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (id >= c.items * c.row_tiles * c.runs) return;
-    const int run = (int)(id % c.runs);
-    const int64_t tile_row = id / c.runs;   // (item, row tile)
-    const int rt = (int)(tile_row % c.row_tiles);
-    const int64_t item = tile_row / c.row_tiles;
-    const int tile = (int)(item % c.tiles), hkv = (int)(item / c.tiles % a.Hkv), b = (int)(item / c.tiles / a.Hkv);
-    const int G = (int)(a.Hq / a.Hkv), g = a.group;
+    const u32 id = blockIdx.x * 4 + (u32)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (id >= (u32)c.items * (u32)c.row_tiles * (u32)c.runs) return;
+    const int run = (int)(id % (u32)c.runs);
+    const u32 tile_row = id / (u32)c.runs;   // (item, row tile)
+    const int rt = (int)(tile_row % (u32)c.row_tiles);
+    const u32 item = tile_row / (u32)c.row_tiles, bh = item / (u32)c.tiles;
+    const int tile = (int)(item % (u32)c.tiles), hkv = (int)(bh % (u32)a.Hkv), b = (int)(bh / (u32)a.Hkv);
+    const int G = (int)a.Hq / (int)a.Hkv, g = a.group;
     const int pos0 = tile * (int)c.query_block, last = (int)sel_last(a, tile), rows = (last - pos0 + 1) * G;
     const int live = (int)sel_end(a, b, last), groups = (live + g - 1) / g;   // that some row sees
     const int u0 = run * c.run_units * 32, u1 = u0 + c.run_units * 32 < groups ? u0 + c.run_units * 32 : groups;
@@ -125,6 +129,14 @@ template <int D, bool BF16> __global__ __launch_bounds__(256) void block_bound_k
         if (lane == 0) *bound = 0.f;
         return;
     }
+    struct Unit { u32x4 z[KS], s[KS]; };
+    const int64_t first = (int64_t)bh * c.stride * D + 8 * h;
+    const u16 *const zeros = (const u16 *)a.k_zero + first, *const scales = (const u16 *)a.k_scale + first;
+    auto load = [&](int u, Unit &x) __attribute__((always_inline)) {
+        const int64_t at = (int64_t)(u + n < u1 ? u + n : u1 - 1) * D;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) { x.z[k] = *(const u32x4 *)(zeros + at + 16 * k); x.s[k] = *(const u32x4 *)(scales + at + 16 * k); }
+    };
     auto row_at = [&](int x) __attribute__((always_inline)) { x += rt * 32; return x < rows ? x : rows - 1; };
     u32x4 q[KS];
     {
@@ -133,6 +145,8 @@ template <int D, bool BF16> __global__ __launch_bounds__(256) void block_bound_k
 #pragma unroll
         for (int k = 0; k < KS; ++k) q[k] = *(const u32x4 *)(src + 16 * k);
     }
+    Unit ahead;
+    load(u0, ahead);
     float unscale = 1.f;
     if constexpr (BF16) {
         u32 top = 0;
@@ -167,33 +181,26 @@ template <int D, bool BF16> __global__ __launch_bounds__(256) void block_bound_k
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) { const float o = __shfl_xor(size, off); size = o > size || o != o ? o : size; }
 
-    const int64_t stride = (a.cap_tokens + g - 1) / g, bh = (int64_t)b * a.Hkv + hkv;
     const int seen = (int)sel_end(a, b, pos0);   // by every query
-    float *const out = c.approx + tile_row * c.groups;
+    float *const out = c.approx + (int64_t)tile_row * c.groups;
     u32 top_z = 0, top_s = 0;
-#pragma unroll 1
-    for (int u = u0; u < u1; u += 32) {
-        const int at = u + n < u1 ? u + n : u1 - 1;
-        const u16 *zero = (const u16 *)a.k_zero + (bh * stride + at) * D + 8 * h, *scale = (const u16 *)a.k_scale + (bh * stride + at) * D + 8 * h;
-        u32x4 z[KS], s[KS];
-#pragma unroll
-        for (int k = 0; k < KS; ++k) { z[k] = *(const u32x4 *)(zero + 16 * k); s[k] = *(const u32x4 *)(scale + 16 * k); }
+    auto step = [&](int u, const Unit &x) __attribute__((always_inline)) {
         f32x16 S, W;
 #pragma unroll
         for (int r = 0; r < 16; ++r) S[r] = W[r] = 0.f;
         u32 sign = 0;
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
-            S = mma(q[k], z[k], S);
+            S = mma(q[k], x.z[k], S);
             u32x4 p;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                sign |= s[k][i];
-                top_z = max_bits(top_z, z[k][i] & 0x7FFF7FFFu);
-                top_s = max_bits(top_s, s[k][i] & 0x7FFF7FFFu);
+                sign |= x.s[k][i];
+                top_z = max_bits(top_z, x.z[k][i] & 0x7FFF7FFFu);
+                top_s = max_bits(top_s, x.s[k][i] & 0x7FFF7FFFu);
                 p[i] = positive(q[k][i]);
             }
-            W = mma(p, s[k], W);
+            W = mma(p, x.s[k], W);
         }
         if (__any((sign & 0x80008000u) != 0)) {
 #pragma unroll
@@ -205,7 +212,7 @@ template <int D, bool BF16> __global__ __launch_bounds__(256) void block_bound_k
                 for (int k = 0; k < KS; ++k) {
                     u32x4 p, y;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) { p[i] = positive(q[k][i] ^ flip); y[i] = positive(s[k][i] ^ flip); }
+                    for (int i = 0; i < 4; ++i) { p[i] = positive(q[k][i] ^ flip); y[i] = positive(x.s[k][i] ^ flip); }
                     W = mma(p, y, W);
                 }
             }
@@ -213,10 +220,11 @@ template <int D, bool BF16> __global__ __launch_bounds__(256) void block_bound_k
 #pragma unroll
         for (int r = 0; r < 16; ++r) S[r] = __builtin_fmaf(levels, W[r], S[r]);
         if ((u + 31) * (int64_t)g >= seen) {   // groups that some queries do not see (in 64 bits: the last ones may lie past the store)
+            const int at = u + n < u1 ? u + n : u1 - 1;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const int x = row_at(8 * (r / 4) + 4 * h + r % 4);
-                if (at * g >= (int)sel_end(a, b, pos0 + x / G)) S[r] = -INFINITY;
+                const int x2 = row_at(8 * (r / 4) + 4 * h + r % 4);
+                if (at * g >= (int)sel_end(a, b, pos0 + x2 / G)) S[r] = -INFINITY;
             }
         }
         float best = S[0];
@@ -224,6 +232,17 @@ template <int D, bool BF16> __global__ __launch_bounds__(256) void block_bound_k
         for (int r = 1; r < 16; ++r) best = fmaxf(best, S[r]);
         best = fmaxf(best, __shfl_xor(best, 32)) * unscale;
         if (h == 0 && u + n < u1) out[u + n] = best;
+    };
+#pragma unroll 1
+    for (int u = u0; u < u1; u += 32) {
+        if constexpr (AHEAD) {
+            const Unit x = ahead;
+            if (u + 32 < u1) load(u + 32, ahead);
+            step(u, x);
+        } else {
+            step(u, ahead);
+            if (u + 32 < u1) load(u + 32, ahead);
+        }
     }
     top_z = max_bits(top_z, __builtin_amdgcn_alignbyte(top_z, top_z, 2));
     top_s = max_bits(top_s, __builtin_amdgcn_alignbyte(top_s, top_s, 2));
@@ -244,20 +263,19 @@ __device__ __forceinline__ uint64_t max_key(uint64_t x, uint64_t y) { return x >
 __device__ __forceinline__ double shfl_add(double s, int off) { return s + __shfl_xor(s, off); }
 
 // The key of block j's score in 64 bits, by a wave: 64 / R lanes a row (R the rows, up to the next power of two), eight channels at a time.
-__device__ __forceinline__ uint64_t exact_key(const vq_block_select_args &a, int64_t b, int64_t hkv, int64_t tile, int64_t j) {
-    const int lane = threadIdx.x & 63, G = (int)(a.Hq / a.Hkv), D = (int)a.D, g = a.group;
-    const int pos0 = (int)(tile * a.query_block), rows = ((int)sel_last(a, tile) - pos0 + 1) * G;
+__device__ __forceinline__ uint64_t exact_key(const SelectCall &c, int b, int hkv, int tile, int j) {
+    const vq_block_select_args &a = c.a;
+    const int lane = threadIdx.x & 63, G = (int)a.Hq / (int)a.Hkv, D = (int)a.D, g = a.group, per = (int)a.block_tokens / g;
+    const int pos0 = tile * (int)c.query_block, rows = (sel_last(a, tile) - pos0 + 1) * G;
     int many = 1;
     while (many < rows && many < 64) many <<= 1;
     const int parts = 64 / many, part = lane % parts;
-    const int64_t groups = (a.cap_tokens + g - 1) / g;
     uint64_t best = 0;
     for (int r0 = 0; r0 < rows; r0 += many) {
-        const int r = r0 + lane / parts, x = r < rows ? r : rows - 1;
-        const int64_t end = sel_end(a, b, pos0 + x / G);
-        const u16 *q = (const u16 *)a.q + ((b * a.Hq + hkv * G + x % G) * a.Sq + pos0 + x / G) * D;
-        for (int64_t t = j * a.block_tokens; t < (j + 1) * a.block_tokens && t < a.n_packed; t += g) {
-            const int64_t at = ((b * a.Hkv + hkv) * groups + t / g) * D;
+        const int r = r0 + lane / parts, x = r < rows ? r : rows - 1, end = sel_end(a, b, pos0 + x / G);
+        const u16 *q = (const u16 *)a.q + (((int64_t)b * a.Hq + hkv * G + x % G) * a.Sq + pos0 + x / G) * D;
+        for (int u = j * per; u < (j + 1) * per && u < (int)c.groups; ++u) {
+            const int64_t at = (((int64_t)b * a.Hkv + hkv) * c.stride + u) * D;
             double s = 0.;
             for (int d = part * 8; d < D; d += parts * 8) {
                 const u32x4 x4 = *(const u32x4 *)(q + d), z4 = *(const u32x4 *)((const u16 *)a.k_zero + at + d), s4 = *(const u32x4 *)((const u16 *)a.k_scale + at + d);
@@ -270,7 +288,7 @@ __device__ __forceinline__ uint64_t exact_key(const vq_block_select_args &a, int
                 }
             }
             for (int off = 1; off < parts; off <<= 1) s = shfl_add(s, off);
-            if (t < end) best = max_key(best, pick_key(s));
+            if (u * g < end) best = max_key(best, pick_key(s));
         }
     }
 #pragma unroll
@@ -278,12 +296,11 @@ __device__ __forceinline__ uint64_t exact_key(const vq_block_select_args &a, int
     return best;
 }
 
-constexpr int PICK_THREADS = 256, PICK_WAVES = PICK_THREADS / 64;
 constexpr int PICK_MOST = 16384;   // blocks whose scores are held in LDS
 constexpr int PICK_LIST = 512;     // blocks that are told apart in 64 bits there
 
 // Sum over the threads below this one, and the total (`waves`: a number a wave, in LDS; a barrier before its next use).
-__device__ __forceinline__ u32 block_before(bool mine, u32 &total, u32 *waves) {
+template <int WAVES> __device__ __forceinline__ u32 block_before(bool mine, u32 &total, u32 *waves) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const uint64_t m = __ballot(mine);
     __syncthreads();
@@ -292,7 +309,7 @@ __device__ __forceinline__ u32 block_before(bool mine, u32 &total, u32 *waves) {
     u32 before = (u32)__popcll(m & ((UINT64_C(1) << lane) - 1));
     total = 0;
 #pragma unroll
-    for (int w = 0; w < PICK_WAVES; ++w) {
+    for (int w = 0; w < WAVES; ++w) {
         const u32 x = waves[w];
         before += w < wave ? x : 0;
         total += x;
@@ -304,16 +321,16 @@ __device__ __forceinline__ u32 block_before(bool mine, u32 &total, u32 *waves) {
 // (a barrier after the last count).  Suffix sums: of the bins above within the wave, then of the waves above.
 __device__ __forceinline__ int pick_bin(const u32 *hist, u32 &left, u32 *found) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const u32 mine = hist[tid];
+    const u32 mine = tid < 256 ? hist[tid] : 0;
     u32 sum = mine;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) { const u32 o = __shfl_down(sum, off); sum += lane + off < 64 ? o : 0; }
-    if (lane == 0) found[2 + wave] = sum;
+    if (lane == 0 && wave < 4) found[2 + wave] = sum;
     __syncthreads();
     u32 above = sum - mine;
 #pragma unroll
-    for (int w = 1; w < PICK_WAVES; ++w) above += w > wave ? found[2 + w] : 0;
-    if (above < left && above + mine >= left) { found[0] = (u32)tid; found[1] = left - above; }
+    for (int w = 1; w < 4; ++w) above += w > wave ? found[2 + w] : 0;
+    if (tid < 256 && above < left && above + mine >= left) { found[0] = (u32)tid; found[1] = left - above; }
     __syncthreads();
     left = found[1];
     return (int)found[0];
@@ -325,37 +342,41 @@ __device__ __forceinline__ int pick_bin(const u32 *hist, u32 &left, u32 *found) 
 // that holds many.  With scores off by e at most, those above the bin's largest + 2 e are among the chosen, those below its smallest - 2 e are
 // not; the few between are told apart by their scores in 64 bits.  Where these are more than PICK_LIST (equal scores, values that are not
 // finite, which make e so) all of them are, by a radix select over the bits.
-template <bool STORED> __global__ __launch_bounds__(PICK_THREADS) void block_pick_kernel(SelectCall c) {
+template <bool STORED, int THREADS> __global__ __launch_bounds__(THREADS) void block_pick_kernel(SelectCall c) {
+    constexpr int WAVES = THREADS / 64;
     const vq_block_select_args &a = c.a;
     extern __shared__ float keys[];   // of the blocks [lo, hi)
-    __shared__ u32 hist[256], waves[PICK_WAVES], found[2 + PICK_WAVES];
-    __shared__ float low[PICK_WAVES], high[PICK_WAVES], off_by[PICK_WAVES];
+    __shared__ u32 hist[256], waves[WAVES], found[6];
+    __shared__ float low[WAVES], high[WAVES], off_by[WAVES];
     __shared__ int list[PICK_LIST];
     __shared__ uint64_t exact[PICK_LIST];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int64_t item = blockIdx.x, tile = item % c.tiles, hkv = item / c.tiles % a.Hkv, b = item / c.tiles / a.Hkv;
-    const int64_t end = sel_end(a, b, sel_last(a, tile)), V = (end + a.block_tokens - 1) / a.block_tokens;
+    const u32 bh = blockIdx.x / (u32)c.tiles;
+    const int64_t item = blockIdx.x;
+    const int tile = (int)(blockIdx.x % (u32)c.tiles), hkv = (int)(bh % (u32)a.Hkv), b = (int)(bh / (u32)a.Hkv);
+    const int end = sel_end(a, b, sel_last(a, tile)), V = (int)((u32)(end + (int)a.block_tokens - 1) / (u32)a.block_tokens);
     int32_t *out = a.out + item * a.count;
     if (V <= a.count) {
-        for (int64_t i = tid; i < a.count; i += PICK_THREADS) out[i] = i < V ? (int32_t)i : -1;
+        for (int64_t i = tid; i < a.count; i += THREADS) out[i] = i < V ? (int32_t)i : -1;
         return;
     }
-    const int lo = (int)a.first, hi = (int)(V - a.recent), n = hi - lo;
+    const int lo = (int)a.first, hi = V - (int)a.recent, n = hi - lo;
     const u32 want = (u32)(a.count - a.first - a.recent);   // of [lo, hi), which holds more
-    for (int64_t i = tid; i < a.first; i += PICK_THREADS) out[i] = (int32_t)i;
-    for (int64_t i = tid; i < a.recent; i += PICK_THREADS) out[a.count - a.recent + i] = (int32_t)(hi + i);
+    for (int64_t i = tid; i < a.first; i += THREADS) out[i] = (int32_t)i;
+    for (int64_t i = tid; i < a.recent; i += THREADS) out[a.count - a.recent + i] = (int32_t)(hi + i);
     if (want == 0) return;
     double *const score = c.scores + item * c.total;
 
     // ---- approximate scores, their range and how far they may be off
     float least = INFINITY, most = -INFINITY, e = 0.f;
+    const int per = (int)a.block_tokens / a.group, seen = (end + a.group - 1) / a.group;   // groups of a block, groups that some row sees
     bool odd = false;   // something is not finite
-    for (int j = tid; j < n; j += PICK_THREADS) {
+    for (int j = tid; j < n; j += THREADS) {
         float x = -INFINITY;
         if (STORED) {
             x = (float)score[lo + j];
         } else {
-            const int g = a.group, per = (int)(a.block_tokens / g), u0 = (lo + j) * per, seen = (int)((end + g - 1) / g), u1 = u0 + per < seen ? u0 + per : seen;
+            const int u0 = (lo + j) * per, u1 = u0 + per < seen ? u0 + per : seen;
             for (int rt = 0; rt < c.row_tiles; ++rt)
                 for (int u = u0; u < u1; ++u) {
                     const float y = c.approx[(item * c.row_tiles + rt) * c.groups + u];
@@ -370,7 +391,7 @@ template <bool STORED> __global__ __launch_bounds__(PICK_THREADS) void block_pic
     if (STORED) {
         e = fmaxf(__builtin_fabsf(least), __builtin_fabsf(most)) * 0x1p-23f;
     } else {
-        for (int i = tid; i < c.row_tiles * c.runs; i += PICK_THREADS) {
+        for (int i = tid; i < c.row_tiles * c.runs; i += THREADS) {
             const float y = c.bounds[item * c.row_tiles * c.runs + i];
             odd = odd || !(y < INFINITY);
             e = fmaxf(e, y);
@@ -387,7 +408,7 @@ template <bool STORED> __global__ __launch_bounds__(PICK_THREADS) void block_pic
     if (lane == 0) { low[wave] = least; high[wave] = most; off_by[wave] = e; }
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < PICK_WAVES; ++w) { least = fminf(least, low[w]); most = fmaxf(most, high[w]); e = fmaxf(e, off_by[w]); }
+    for (int w = 0; w < WAVES; ++w) { least = fminf(least, low[w]); most = fmaxf(most, high[w]); e = fmaxf(e, off_by[w]); }
     e = 2.f * e + 0x1p-100f;   // of two scores' difference, also where products are too small for float32
 
     // ---- the bin of the kth best
@@ -396,9 +417,9 @@ template <bool STORED> __global__ __launch_bounds__(PICK_THREADS) void block_pic
     if (e < INFINITY) {
         for (int pass = 0; pass < 4 && among > 8 && to - from > e; ++pass) {
             const float by = 255.f / (to - from);   // (bin 255: the largest alone)
-            hist[tid] = 0;
+            if (tid < 256) hist[tid] = 0;
             __syncthreads();
-            for (int j = tid; j < n; j += PICK_THREADS) {
+            for (int j = tid; j < n; j += THREADS) {
                 const float x = keys[j];
                 if (x >= from && x <= to) atomicAdd(&hist[(int)((x - from) * by) & 255], 1u);
             }
@@ -406,7 +427,7 @@ template <bool STORED> __global__ __launch_bounds__(PICK_THREADS) void block_pic
             const int bin = pick_bin(hist, left, found);
             among = hist[bin];
             float l = INFINITY, m = -INFINITY;
-            for (int j = tid; j < n; j += PICK_THREADS) {
+            for (int j = tid; j < n; j += THREADS) {
                 const float x = keys[j];
                 if (x >= from && x <= to && ((int)((x - from) * by) & 255) == bin) { l = fminf(l, x); m = fmaxf(m, x); }
             }
@@ -417,7 +438,7 @@ template <bool STORED> __global__ __launch_bounds__(PICK_THREADS) void block_pic
             __syncthreads();
             from = low[0]; to = high[0];
 #pragma unroll
-            for (int w = 1; w < PICK_WAVES; ++w) { from = fminf(from, low[w]); to = fmaxf(to, high[w]); }
+            for (int w = 1; w < WAVES; ++w) { from = fminf(from, low[w]); to = fmaxf(to, high[w]); }
         }
     }
     const float over = e < INFINITY ? to + e : INFINITY, under = e < INFINITY ? from - e : -INFINITY;
@@ -425,26 +446,26 @@ template <bool STORED> __global__ __launch_bounds__(PICK_THREADS) void block_pic
     // ---- those between
     u32 sure = 0, doubt = 0;
     __syncthreads();
-    for (int j0 = 0; j0 < n; j0 += PICK_THREADS) {
+    for (int j0 = 0; j0 < n; j0 += THREADS) {
         const float x = j0 + tid < n ? keys[j0 + tid] : -INFINITY;
         const bool here = j0 + tid < n, in = here && x > over, maybe = here && !in && !(x < under);
         u32 some;
-        const u32 at = block_before(maybe, some, waves);
+        const u32 at = block_before<WAVES>(maybe, some, waves);
         if (maybe && doubt + at < PICK_LIST) list[doubt + at] = j0 + tid;
         doubt += some;
-        (void)block_before(in, some, waves);
+        (void)block_before<WAVES>(in, some, waves);
         sure += some;
     }
     const u32 need = want - sure;   // of the doubtful
     __syncthreads();
     if (doubt > PICK_LIST) {
         // all of them by their bits; the sure ones as the highest
-        for (int j = wave; j < n; j += PICK_WAVES) {
+        for (int j = wave; j < n; j += WAVES) {
             const float x = keys[j];
             uint64_t k;
             if (x > over) k = ~UINT64_C(0);
             else if (x < under) k = 0;
-            else k = STORED ? pick_key(score[lo + j]) : exact_key(a, b, hkv, tile, lo + j);
+            else k = STORED ? pick_key(score[lo + j]) : exact_key(c, b, hkv, tile, lo + j);
             if (lane == 0) ((uint64_t *)score)[lo + j] = k;
         }
         __threadfence_block();
@@ -453,72 +474,74 @@ template <bool STORED> __global__ __launch_bounds__(PICK_THREADS) void block_pic
         uint64_t key = 0;
         left = want;
         for (int shift = 56; shift >= 0; shift -= 8) {
-            hist[tid] = 0;
+            if (tid < 256) hist[tid] = 0;
             __syncthreads();
-            for (int j = tid; j < n; j += PICK_THREADS)
+            for (int j = tid; j < n; j += THREADS)
                 if (shift == 56 || (all[j] ^ key) >> (shift + 8) == 0) atomicAdd(&hist[all[j] >> shift & 255], 1u);
             __syncthreads();
             key |= (uint64_t)pick_bin(hist, left, found) << shift;
             __syncthreads();
         }
         u32 equal = 0;
-        for (int j0 = 0; j0 < n; j0 += PICK_THREADS) {
+        for (int j0 = 0; j0 < n; j0 += THREADS) {
             const int j = j0 + tid;
             u32 some;
-            const u32 rank = equal + block_before(j < n && all[j] == key, some, waves);
+            const u32 rank = equal + block_before<WAVES>(j < n && all[j] == key, some, waves);
             equal += some;
             if (j < n) keys[j] = all[j] > key || (all[j] == key && rank < left) ? INFINITY : -INFINITY;
         }
     } else if (doubt > need) {
-        for (u32 i = wave; i < doubt; i += PICK_WAVES) {
-            const uint64_t k = STORED ? pick_key(score[lo + list[i]]) : exact_key(a, b, hkv, tile, lo + list[i]);
+        for (u32 i = wave; i < doubt; i += WAVES) {
+            const uint64_t k = STORED ? pick_key(score[lo + list[i]]) : exact_key(c, b, hkv, tile, lo + list[i]);
             if (lane == 0) exact[i] = k;
         }
         __syncthreads();
-        for (u32 i = tid; i < doubt; i += PICK_THREADS) {
+        for (u32 i = tid; i < doubt; i += THREADS) {
             const uint64_t k = exact[i];
             u32 better = 0;   // (the list ascends: of equal scores the lower block comes first)
             for (u32 o = 0; o < doubt; ++o) better += exact[o] > k || (exact[o] == k && o < i) ? 1 : 0;
             keys[list[i]] = better < need ? INFINITY : -INFINITY;
         }
     } else {
-        for (u32 i = tid; i < doubt; i += PICK_THREADS) keys[list[i]] = INFINITY;
+        for (u32 i = tid; i < doubt; i += THREADS) keys[list[i]] = INFINITY;
     }
     __syncthreads();
     // ---- in order
     u32 done = 0;
-    for (int j0 = 0; j0 < n; j0 += PICK_THREADS) {
+    for (int j0 = 0; j0 < n; j0 += THREADS) {
         const bool take = j0 + tid < n && (keys[j0 + tid] == INFINITY || keys[j0 + tid] > over);
         u32 some;
-        const u32 at = done + block_before(take, some, waves);
+        const u32 at = done + block_before<WAVES>(take, some, waves);
         if (take) out[lo + at] = lo + j0 + tid;
         done += some;
     }
 }
 
+constexpr int ANY_THREADS = 256;
+
 // The same over any number of blocks, their scores of 64 bits in memory throughout.
-__global__ __launch_bounds__(PICK_THREADS) void block_pick_any_kernel(SelectCall c) {
+__global__ __launch_bounds__(ANY_THREADS) void block_pick_any_kernel(SelectCall c) {
     const vq_block_select_args &a = c.a;
-    __shared__ u32 hist[256], waves[PICK_WAVES], found[2 + PICK_WAVES];
+    __shared__ u32 hist[256], waves[ANY_THREADS / 64], found[6];
     const int tid = threadIdx.x;
     const int64_t item = blockIdx.x, tile = item % c.tiles, b = item / c.tiles / a.Hkv;
-    const int64_t V = (sel_end(a, b, sel_last(a, tile)) + a.block_tokens - 1) / a.block_tokens;
+    const int64_t V = (sel_end(a, (int)b, sel_last(a, (int)tile)) + a.block_tokens - 1) / a.block_tokens;
     int32_t *out = a.out + item * a.count;
     if (V <= a.count) {
-        for (int64_t i = tid; i < a.count; i += PICK_THREADS) out[i] = i < V ? (int32_t)i : -1;
+        for (int64_t i = tid; i < a.count; i += ANY_THREADS) out[i] = i < V ? (int32_t)i : -1;
         return;
     }
     const double *score = c.scores + item * c.total;
     const int lo = (int)a.first, hi = (int)(V - a.recent);
     u32 left = (u32)(a.count - a.first - a.recent);
-    for (int64_t i = tid; i < a.first; i += PICK_THREADS) out[i] = (int32_t)i;
-    for (int64_t i = tid; i < a.recent; i += PICK_THREADS) out[a.count - a.recent + i] = (int32_t)(hi + i);
+    for (int64_t i = tid; i < a.first; i += ANY_THREADS) out[i] = (int32_t)i;
+    for (int64_t i = tid; i < a.recent; i += ANY_THREADS) out[a.count - a.recent + i] = (int32_t)(hi + i);
     if (left == 0) return;
     uint64_t key = 0;
     for (int shift = 56; shift >= 0; shift -= 8) {
         hist[tid] = 0;
         __syncthreads();
-        for (int j = lo + tid; j < hi; j += PICK_THREADS) {
+        for (int j = lo + tid; j < hi; j += ANY_THREADS) {
             const uint64_t k = pick_key(score[j]);
             if (shift == 56 || (k ^ key) >> (shift + 8) == 0) atomicAdd(&hist[k >> shift & 255], 1u);
         }
@@ -527,14 +550,14 @@ __global__ __launch_bounds__(PICK_THREADS) void block_pick_any_kernel(SelectCall
         __syncthreads();
     }
     u32 done = 0, equal = 0;
-    for (int j0 = lo; j0 < hi; j0 += PICK_THREADS) {
+    for (int j0 = lo; j0 < hi; j0 += ANY_THREADS) {
         const int j = j0 + tid;
         const uint64_t k = j < hi ? pick_key(score[j]) : 0;
         u32 some;
-        const u32 rank = equal + block_before(j < hi && k == key, some, waves);
+        const u32 rank = equal + block_before<ANY_THREADS / 64>(j < hi && k == key, some, waves);
         equal += some;
         const bool take = j < hi && (k > key || (k == key && rank < left));
-        const u32 at = done + block_before(take, some, waves);
+        const u32 at = done + block_before<ANY_THREADS / 64>(take, some, waves);
         if (take) out[lo + at] = j;
         done += some;
     }
@@ -575,14 +598,15 @@ SelectCall cut_select(const vq_block_select_args &a) {
     c.items = a.B * a.Hkv * c.tiles;
     c.query_block = a.query_block < a.Sq ? a.query_block : a.Sq;
     c.groups = cdiv(a.n_packed, a.group);
+    c.stride = cdiv(a.cap_tokens, a.group);
     c.row_tiles = (int)cdiv(a.Hq / a.Hkv * c.query_block, 32);
     if (c.total <= a.count) return c;   // every visible block is chosen: no scores
     c.mma = (a.D == 64 || a.D == 128 || a.D == 256) && a.dtype != VQ_F32 && a.meta_dtype == VQ_F16 && c.total <= PICK_MOST &&
             (((uintptr_t)a.q | (uintptr_t)a.k_scale | (uintptr_t)a.k_zero) & 15) == 0;
     if (c.mma) {
-        // a unit a wave until sixteen waves a CU have work
+        // a unit a wave until the eight waves that a CU holds have work
         const int64_t units = cdiv(c.groups, 32), waves = c.items * c.row_tiles * units;
-        c.run_units = (int)cdiv(waves, 4096);
+        c.run_units = (int)cdiv(waves, 2048);
         if (c.run_units > units) c.run_units = (int)units;
         c.runs = (int)cdiv(units, c.run_units);
         // (the products and the grid of a call of this size are left to the vector units)
@@ -605,16 +629,23 @@ SelectRoom select_room(const SelectCall &c) {
 }
 
 // (the scores of up to PICK_MOST blocks and the tables beside them pass the 64 KB that a block has unasked)
-template <bool STORED> int allow_lds(const char *fn, size_t bytes) {
-    if (bytes <= 48 * 1024) return VQ_OK;
-    static std::atomic<bool> allowed[64] = {};
-    int dev = 0;
-    (void)hipGetDevice(&dev);
-    if (dev >= 0 && dev < 64 && allowed[dev].load(std::memory_order_acquire)) return VQ_OK;
-    const hipError_t e = hipFuncSetAttribute((const void *)block_pick_kernel<STORED>, hipFuncAttributeMaxDynamicSharedMemorySize, PICK_MOST * 4);
-    VQ_REQUIRE(e == hipSuccess, VQ_ERR_HIP, "%s: %d bytes of block-shared memory: %s", fn, PICK_MOST * 4, hipGetErrorString(e));
-    if (dev >= 0 && dev < 64) allowed[dev].store(true, std::memory_order_release);
+template <bool STORED, int THREADS> int launch_pick_of(const char *fn, const SelectCall &c, size_t bytes, hipStream_t st) {
+    const auto kernel = block_pick_kernel<STORED, THREADS>;
+    if (bytes > 48 * 1024) {
+        static std::atomic<bool> allowed[64] = {};
+        int dev = 0;
+        (void)hipGetDevice(&dev);
+        if (dev < 0 || dev >= 64 || !allowed[dev].load(std::memory_order_acquire)) {
+            const hipError_t e = hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, PICK_MOST * 4);
+            VQ_REQUIRE(e == hipSuccess, VQ_ERR_HIP, "%s: %d bytes of block-shared memory: %s", fn, PICK_MOST * 4, hipGetErrorString(e));
+            if (dev >= 0 && dev < 64) allowed[dev].store(true, std::memory_order_release);
+        }
+    }
+    kernel<<<(unsigned)c.items, THREADS, bytes, st>>>(c);
     return VQ_OK;
+}
+template <bool STORED> int launch_pick(const char *fn, const SelectCall &c, size_t bytes, hipStream_t st) {
+    return c.total > 256 ? launch_pick_of<STORED, 1024>(fn, c, bytes, st) : launch_pick_of<STORED, 256>(fn, c, bytes, st);
 }
 
 template <int D> void launch_bounds(const SelectCall &c, hipStream_t st) {
@@ -655,13 +686,9 @@ extern "C" int vq_block_select(const vq_block_select_args *args) {
         VQ_HIP_CHECK_LAUNCH(fn);
     }
     if (c.total > PICK_MOST) {
-        block_pick_any_kernel<<<(unsigned)c.items, PICK_THREADS, 0, st>>>(c);
-    } else if (c.mma) {
-        if (int rc = allow_lds<false>(fn, lds)) return rc;
-        block_pick_kernel<false><<<(unsigned)c.items, PICK_THREADS, lds, st>>>(c);
-    } else {
-        if (int rc = allow_lds<true>(fn, lds)) return rc;
-        block_pick_kernel<true><<<(unsigned)c.items, PICK_THREADS, lds, st>>>(c);
+        block_pick_any_kernel<<<(unsigned)c.items, ANY_THREADS, 0, st>>>(c);
+    } else if (int rc = c.mma ? launch_pick<false>(fn, c, lds, st) : launch_pick<true>(fn, c, lds, st)) {
+        return rc;
     }
     VQ_HIP_CHECK_LAUNCH(fn);
     return VQ_OK;
