@@ -24,6 +24,7 @@ struct SelectCall {
     double *scores;         // [items][total], of 64 bits (or room for them)
     // the filter on the matrix units:
     int mma;                // 1: it takes the call
+    int one;                // 1: in one launch, a block an item
     int64_t query_block;    // (at most Sq)
     int row_tiles;          // of 32 rows an item
     int64_t groups, stride; // of the packed slots, of the store
@@ -38,14 +39,15 @@ __device__ __forceinline__ float sel_ld(const void *p, int tag, int64_t i) {
     return ((const float *)p)[i];
 }
 
-// slots [0, end) of the packed ones that query i of sequence b sees (slots and queries: below 2^30)
-__device__ __forceinline__ int sel_end(const vq_block_select_args &a, int b, int i) {
-    const int packed = (int)a.n_packed, room = packed + (int)a.n_tail;
-    int live = room;
-    if (a.seq_lens != nullptr) {
-        const int64_t n = a.seq_lens[b];
-        live = n < 0 ? 0 : n < room ? (int)n : room;
-    }
+// Live slots of a sequence, and of the packed ones those [0, end) that its query i sees (slots and queries: below 2^30).
+__device__ __forceinline__ int sel_live(const vq_block_select_args &a, int b) {
+    const int room = (int)a.n_packed + (int)a.n_tail;
+    if (a.seq_lens == nullptr) return room;
+    const int64_t n = a.seq_lens[b];
+    return n < 0 ? 0 : n < room ? (int)n : room;
+}
+__device__ __forceinline__ int sel_end(const vq_block_select_args &a, int live, int i) {
+    const int packed = (int)a.n_packed;
     int end = a.causal ? live - (int)a.Sq + i + 1 : live;
     end = end < live ? end : live;
     return end < 0 ? 0 : end < packed ? end : packed;
@@ -63,10 +65,11 @@ __global__ __launch_bounds__(256) void block_score_kernel(SelectCall c) {
     if (id >= a.B * a.Hkv * c.tiles * c.total) return;
     const int64_t j = id % c.total, tile = id / c.total % c.tiles, bh = id / (c.total * c.tiles), hkv = bh % a.Hkv, b = bh / a.Hkv;
     const int64_t G = a.Hq / a.Hkv, i1 = sel_last(a, (int)tile), groups = (a.cap_tokens + a.group - 1) / a.group;
+    const int live = sel_live(a, (int)b);
     double best = -INFINITY;
     for (int64_t t = j * a.block_tokens; t < (j + 1) * a.block_tokens; t += a.group)
         for (int64_t i = tile * a.query_block; i <= i1; ++i) {
-            if (t >= sel_end(a, (int)b, (int)i)) continue;
+            if (t >= sel_end(a, live, (int)i)) continue;
             for (int64_t g = 0; g < G; ++g) {
                 double s = 0.;
                 for (int64_t d = lane; d < a.D; d += 64) {
@@ -108,29 +111,16 @@ __device__ __forceinline__ f32x16 mma(u32x4 x, u32x4 y, f32x16 acc) {
 // bf16 queries become fp16 numbers by a power of two that puts a row tile's largest near 2^15.  Float32 sums of D terms are off by less than
 // (D + 8) 2^-22 sum |q| (|z| + L |s|): with the largest sum of |q| and the largest |z| and |s| the wave also writes a bound of that sum, so the
 // choice knows how far to trust the scores.  Bound by the bytes of the scales and zeros for one query a sequence.
-template <int D, bool BF16> __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void block_bound_kernel(SelectCall c) {
+// One wave's run: units u0, u0 + step, .. of 32 groups below u1 (in groups; u0 < u1), each group's score to out; returns the bound of
+// sum |q| (|z| + L |s|) (the same in every lane; not finite where a query, scale or zero is not).
+template <int D, bool BF16>
+__device__ __forceinline__ float bound_units(const SelectCall &c, int b, int hkv, int tile, int rt, int live, int u0, int u1, int stride, float *out) {
     constexpr int KS = D / 16;
-    constexpr bool AHEAD = D <= 128;   // room for the next unit's scales and zeros beside this one's
     const vq_block_select_args &a = c.a;
-    const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
-    const u32 id = blockIdx.x * 4 + (u32)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (id >= (u32)c.items * (u32)c.row_tiles * (u32)c.runs) return;
-    const int run = (int)(id % (u32)c.runs);
-    const u32 tile_row = id / (u32)c.runs;   // (item, row tile)
-    const int rt = (int)(tile_row % (u32)c.row_tiles);
-    const u32 item = tile_row / (u32)c.row_tiles, bh = item / (u32)c.tiles;
-    const int tile = (int)(item % (u32)c.tiles), hkv = (int)(bh % (u32)a.Hkv), b = (int)(bh / (u32)a.Hkv);
-    const int G = (int)a.Hq / (int)a.Hkv, g = a.group;
-    const int pos0 = tile * (int)c.query_block, last = (int)sel_last(a, tile), rows = (last - pos0 + 1) * G;
-    const int live = (int)sel_end(a, b, last), groups = (live + g - 1) / g;   // that some row sees
-    const int u0 = run * c.run_units * 32, u1 = u0 + c.run_units * 32 < groups ? u0 + c.run_units * 32 : groups;
-    float *const bound = c.bounds + id;
-    if (u0 >= u1) {
-        if (lane == 0) *bound = 0.f;
-        return;
-    }
+    const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5, G = (int)a.Hq / (int)a.Hkv, g = a.group;
+    const int pos0 = tile * (int)c.query_block, rows = (sel_last(a, tile) - pos0 + 1) * G;
     struct Unit { u32x4 z[KS], s[KS]; };
-    const int64_t first = (int64_t)bh * c.stride * D + 8 * h;
+    const int64_t first = ((int64_t)b * a.Hkv + hkv) * c.stride * D + 8 * h;
     const u16 *const zeros = (const u16 *)a.k_zero + first, *const scales = (const u16 *)a.k_scale + first;
     auto load = [&](int u, Unit &x) __attribute__((always_inline)) {
         const int64_t at = (int64_t)(u + n < u1 ? u + n : u1 - 1) * D;
@@ -181,10 +171,13 @@ template <int D, bool BF16> __global__ __launch_bounds__(256) __attribute__((amd
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) { const float o = __shfl_xor(size, off); size = o > size || o != o ? o : size; }
 
-    const int seen = (int)sel_end(a, b, pos0);   // by every query
-    float *const out = c.approx + (int64_t)tile_row * c.groups;
+    const int seen = sel_end(a, live, pos0);   // by every query
     u32 top_z = 0, top_s = 0;
     auto step = [&](int u, const Unit &x) __attribute__((always_inline)) {
+        // (what is formed of the queries is formed anew in every step: held across them it would push other registers to scratch memory, whose reloads
+        // wait for the unit that is under way)
+#pragma unroll
+        for (int k = 0; k < KS; ++k) asm volatile("" : "+v"(q[k]));
         f32x16 S, W;
 #pragma unroll
         for (int r = 0; r < 16; ++r) S[r] = W[r] = 0.f;
@@ -224,7 +217,7 @@ template <int D, bool BF16> __global__ __launch_bounds__(256) __attribute__((amd
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const int x2 = row_at(8 * (r / 4) + 4 * h + r % 4);
-                if (at * g >= (int)sel_end(a, b, pos0 + x2 / G)) S[r] = -INFINITY;
+                if (at * g >= sel_end(a, live, pos0 + x2 / G)) S[r] = -INFINITY;
             }
         }
         float best = S[0];
@@ -234,14 +227,14 @@ template <int D, bool BF16> __global__ __launch_bounds__(256) __attribute__((amd
         if (h == 0 && u + n < u1) out[u + n] = best;
     };
 #pragma unroll 1
-    for (int u = u0; u < u1; u += 32) {
-        if constexpr (AHEAD) {
+    for (int u = u0; u < u1; u += stride) {
+        if constexpr (D <= 128) {   // (the next unit's scales and zeros fit beside this one's)
             const Unit x = ahead;
-            if (u + 32 < u1) load(u + 32, ahead);
+            if (u + stride < u1) load(u + stride, ahead);
             step(u, x);
         } else {
             step(u, ahead);
-            if (u + 32 < u1) load(u + 32, ahead);
+            if (u + stride < u1) load(u + stride, ahead);
         }
     }
     top_z = max_bits(top_z, __builtin_amdgcn_alignbyte(top_z, top_z, 2));
@@ -249,7 +242,23 @@ template <int D, bool BF16> __global__ __launch_bounds__(256) __attribute__((amd
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) { top_z = max_bits(top_z, __shfl_xor(top_z, off)); top_s = max_bits(top_s, __shfl_xor(top_s, off)); }
     const float mz = (float)__builtin_bit_cast(f16, (u16)top_z), ms = (float)__builtin_bit_cast(f16, (u16)top_s);
-    if (lane == 0) *bound = size * (mz + levels * ms) * unscale;   // (not finite where a query, scale or zero is not)
+    return size * (mz + levels * ms) * unscale;
+}
+
+// Items of many rows, and few of many groups: a wave a run of units, scores and bounds to memory.
+template <int D, bool BF16> __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2, D == 256 ? 1 : 2))) void block_bound_kernel(SelectCall c) {
+    const vq_block_select_args &a = c.a;
+    const u32 id = blockIdx.x * 4 + (u32)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (id >= (u32)c.items * (u32)c.row_tiles * (u32)c.runs) return;
+    const int run = (int)(id % (u32)c.runs);
+    const u32 tile_row = id / (u32)c.runs;   // (item, row tile)
+    const u32 item = tile_row / (u32)c.row_tiles, bh = item / (u32)c.tiles;
+    const int tile = (int)(item % (u32)c.tiles), hkv = (int)(bh % (u32)a.Hkv), b = (int)(bh / (u32)a.Hkv), live = sel_live(a, b);
+    const int groups = (sel_end(a, live, sel_last(a, tile)) + a.group - 1) / a.group;   // that some row sees
+    const int u0 = run * c.run_units * 32, u1 = u0 + c.run_units * 32 < groups ? u0 + c.run_units * 32 : groups;
+    float bound = 0.f;
+    if (u0 < u1) bound = bound_units<D, BF16>(c, b, hkv, tile, (int)(tile_row % (u32)c.row_tiles), live, u0, u1, 32, c.approx + (int64_t)tile_row * c.groups);
+    if ((threadIdx.x & 63) == 0) c.bounds[id] = bound;
 }
 
 // ---- the choice
@@ -263,7 +272,8 @@ __device__ __forceinline__ uint64_t max_key(uint64_t x, uint64_t y) { return x >
 __device__ __forceinline__ double shfl_add(double s, int off) { return s + __shfl_xor(s, off); }
 
 // The key of block j's score in 64 bits, by a wave: 64 / R lanes a row (R the rows, up to the next power of two), eight channels at a time.
-__device__ __forceinline__ uint64_t exact_key(const SelectCall &c, int b, int hkv, int tile, int j) {
+__device__ __forceinline__ uint64_t exact_key(const SelectCall &c, int b, int hkv, int tile, int live, int j) {
+    constexpr int AHEAD = 4;   // steps of the channels whose loads are under way at once
     const vq_block_select_args &a = c.a;
     const int lane = threadIdx.x & 63, G = (int)a.Hq / (int)a.Hkv, D = (int)a.D, g = a.group, per = (int)a.block_tokens / g;
     const int pos0 = tile * (int)c.query_block, rows = (sel_last(a, tile) - pos0 + 1) * G;
@@ -272,19 +282,31 @@ __device__ __forceinline__ uint64_t exact_key(const SelectCall &c, int b, int hk
     const int parts = 64 / many, part = lane % parts;
     uint64_t best = 0;
     for (int r0 = 0; r0 < rows; r0 += many) {
-        const int r = r0 + lane / parts, x = r < rows ? r : rows - 1, end = sel_end(a, b, pos0 + x / G);
+        const int r = r0 + lane / parts, x = r < rows ? r : rows - 1, end = sel_end(a, live, pos0 + x / G);
         const u16 *q = (const u16 *)a.q + (((int64_t)b * a.Hq + hkv * G + x % G) * a.Sq + pos0 + x / G) * D;
         for (int u = j * per; u < (j + 1) * per && u < (int)c.groups; ++u) {
             const int64_t at = (((int64_t)b * a.Hkv + hkv) * c.stride + u) * D;
             double s = 0.;
-            for (int d = part * 8; d < D; d += parts * 8) {
-                const u32x4 x4 = *(const u32x4 *)(q + d), z4 = *(const u32x4 *)((const u16 *)a.k_zero + at + d), s4 = *(const u32x4 *)((const u16 *)a.k_scale + at + d);
+            for (int d0 = part * 8; d0 < D; d0 += AHEAD * parts * 8) {
+                u32x4 x4[AHEAD], z4[AHEAD], s4[AHEAD];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const u16 xb = (u16)(x4[i / 2] >> (16 * (i & 1)));
-                    const double y = a.dtype == VQ_BF16 ? (double)bf16_to_f32(xb) : (double)(float)__builtin_bit_cast(f16, xb);
-                    const double z = (double)(float)as_h2(z4[i / 2])[i & 1], r1 = y * (double)(float)as_h2(s4[i / 2])[i & 1] * a.levels;
-                    s += y * z + (r1 > 0. || r1 != r1 ? r1 : 0.);
+                for (int k = 0; k < AHEAD; ++k) {
+                    const int d = d0 + k * parts * 8;
+                    if (k > 0 && d >= D) { x4[k] = z4[k] = s4[k] = u32x4{0, 0, 0, 0}; continue; }
+                    x4[k] = *(const u32x4 *)(q + d);
+                    z4[k] = *(const u32x4 *)((const u16 *)a.k_zero + at + d);
+                    s4[k] = *(const u32x4 *)((const u16 *)a.k_scale + at + d);
+                }
+#pragma unroll
+                for (int k = 0; k < AHEAD; ++k) {
+                    if (k > 0 && d0 + k * parts * 8 >= D) break;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const u16 xb = (u16)(x4[k][i / 2] >> (16 * (i & 1)));
+                        const double y = a.dtype == VQ_BF16 ? (double)bf16_to_f32(xb) : (double)(float)__builtin_bit_cast(f16, xb);
+                        const double z = (double)(float)as_h2(z4[k][i / 2])[i & 1], r1 = y * (double)(float)as_h2(s4[k][i / 2])[i & 1] * a.levels;
+                        s += y * z + (r1 > 0. || r1 != r1 ? r1 : 0.);
+                    }
                 }
             }
             for (int off = 1; off < parts; off <<= 1) s = shfl_add(s, off);
@@ -296,20 +318,30 @@ __device__ __forceinline__ uint64_t exact_key(const SelectCall &c, int b, int hk
     return best;
 }
 
+constexpr int PICK_THREADS = 512, PICK_WAVES = PICK_THREADS / 64;
 constexpr int PICK_MOST = 16384;   // blocks whose scores are held in LDS
 constexpr int PICK_LIST = 512;     // blocks that are told apart in 64 bits there
 
-// Sum over the threads below this one, and the total (`waves`: a number a wave, in LDS; a barrier before its next use).
-template <int WAVES> __device__ __forceinline__ u32 block_before(bool mine, u32 &total, u32 *waves) {
+
+struct PickRoom {
+    u32 hist[PICK_THREADS], waves[PICK_WAVES], found[2];
+    float low[PICK_WAVES], high[PICK_WAVES], off_by[PICK_WAVES];
+    int list[PICK_LIST];
+    uint64_t exact[PICK_LIST];
+};
+
+// How many threads below this one say `one` (lower half) and `two` (upper half; counts below 2^16), and in `total` how many in all.  (Two barriers
+// around each use of `waves`.)
+__device__ __forceinline__ u32 block_before(bool one, bool two, u32 &total, u32 *waves) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint64_t m = __ballot(mine);
+    const uint64_t m1 = __ballot(one), m2 = __ballot(two), below = (UINT64_C(1) << lane) - 1;
     __syncthreads();
-    if (lane == 0) waves[wave] = (u32)__popcll(m);
+    if (lane == 0) waves[wave] = (u32)__popcll(m1) | (u32)__popcll(m2) << 16;
     __syncthreads();
-    u32 before = (u32)__popcll(m & ((UINT64_C(1) << lane) - 1));
+    u32 before = (u32)__popcll(m1 & below) | (u32)__popcll(m2 & below) << 16;
     total = 0;
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
+    for (int w = 0; w < PICK_WAVES; ++w) {
         const u32 x = waves[w];
         before += w < wave ? x : 0;
         total += x;
@@ -317,248 +349,270 @@ template <int WAVES> __device__ __forceinline__ u32 block_before(bool mine, u32 
     return before;
 }
 
-// `left` becomes how many are to be taken of the bin it returns, counted from the highest bin down; hist[256] is read by its threads
-// (a barrier after the last count).  Suffix sums: of the bins above within the wave, then of the waves above.
-__device__ __forceinline__ int pick_bin(const u32 *hist, u32 &left, u32 *found) {
+// The bin, a thread each, that holds the `left`-th from the highest bin down; `left` becomes how many of that bin are wanted.  (A barrier
+// lies between the last count and the call.)
+__device__ __forceinline__ int pick_bin(const u32 *hist, u32 &left, u32 *waves, u32 *found) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const u32 mine = tid < 256 ? hist[tid] : 0;
+    const u32 mine = hist[tid];
     u32 sum = mine;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) { const u32 o = __shfl_down(sum, off); sum += lane + off < 64 ? o : 0; }
-    if (lane == 0 && wave < 4) found[2 + wave] = sum;
+    if (lane == 0) waves[wave] = sum;
     __syncthreads();
     u32 above = sum - mine;
 #pragma unroll
-    for (int w = 1; w < 4; ++w) above += w > wave ? found[2 + w] : 0;
-    if (tid < 256 && above < left && above + mine >= left) { found[0] = (u32)tid; found[1] = left - above; }
+    for (int w = 1; w < PICK_WAVES; ++w) above += w > wave ? waves[w] : 0;
+    if (above < left && above + mine >= left) { found[0] = (u32)tid; found[1] = left - above; }
     __syncthreads();
     left = found[1];
     return (int)found[0];
 }
 
-// A block of threads a tile.  STORED: scores of 64 bits lie in memory, their float32 roundings are the approximate ones; else those of the matrix units.
+// The choice of a tile, by a block of threads.  keys: the approximate scores of the blocks [lo, hi) from this thread's blocks on, in LDS; `least`, `most`, `e`: of this
+// thread's, the last one how far a score may be off, infinite where something is not finite.
 //
 // The kth best is looked for among the approximate scores by bins between the smallest and the largest, again inside its bin while
 // that holds many.  With scores off by e at most, those above the bin's largest + 2 e are among the chosen, those below its smallest - 2 e are
-// not; the few between are told apart by their scores in 64 bits.  Where these are more than PICK_LIST (equal scores, values that are not
-// finite, which make e so) all of them are, by a radix select over the bits.
-template <bool STORED, int THREADS> __global__ __launch_bounds__(THREADS) void block_pick_kernel(SelectCall c) {
-    constexpr int WAVES = THREADS / 64;
+// not; the few between are told apart by their scores in 64 bits, a wave each.  Where these are more than PICK_LIST (equal scores, values that are
+// not finite, which make e so) all of them are, by a radix select over the bits.
+// STORED: the scores of 64 bits lie in memory; else they are formed here.
+template <bool STORED>
+__device__ __forceinline__ void pick(const SelectCall &c, PickRoom &room, float *keys, int b, int hkv, int tile, int live, int lo, int n, u32 want, float least, float most,
+                                     float e) {
     const vq_block_select_args &a = c.a;
-    extern __shared__ float keys[];   // of the blocks [lo, hi)
-    __shared__ u32 hist[256], waves[WAVES], found[6];
-    __shared__ float low[WAVES], high[WAVES], off_by[WAVES];
-    __shared__ int list[PICK_LIST];
-    __shared__ uint64_t exact[PICK_LIST];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const u32 bh = blockIdx.x / (u32)c.tiles;
-    const int64_t item = blockIdx.x;
-    const int tile = (int)(blockIdx.x % (u32)c.tiles), hkv = (int)(bh % (u32)a.Hkv), b = (int)(bh / (u32)a.Hkv);
-    const int end = sel_end(a, b, sel_last(a, tile)), V = (int)((u32)(end + (int)a.block_tokens - 1) / (u32)a.block_tokens);
-    int32_t *out = a.out + item * a.count;
-    if (V <= a.count) {
-        for (int64_t i = tid; i < a.count; i += THREADS) out[i] = i < V ? (int32_t)i : -1;
-        return;
-    }
-    const int lo = (int)a.first, hi = V - (int)a.recent, n = hi - lo;
-    const u32 want = (u32)(a.count - a.first - a.recent);   // of [lo, hi), which holds more
-    for (int64_t i = tid; i < a.first; i += THREADS) out[i] = (int32_t)i;
-    for (int64_t i = tid; i < a.recent; i += THREADS) out[a.count - a.recent + i] = (int32_t)(hi + i);
-    if (want == 0) return;
-    double *const score = c.scores + item * c.total;
-
-    // ---- approximate scores, their range and how far they may be off
-    float least = INFINITY, most = -INFINITY, e = 0.f;
-    const int per = (int)a.block_tokens / a.group, seen = (end + a.group - 1) / a.group;   // groups of a block, groups that some row sees
-    bool odd = false;   // something is not finite
-    for (int j = tid; j < n; j += THREADS) {
-        float x = -INFINITY;
-        if (STORED) {
-            x = (float)score[lo + j];
-        } else {
-            const int u0 = (lo + j) * per, u1 = u0 + per < seen ? u0 + per : seen;
-            for (int rt = 0; rt < c.row_tiles; ++rt)
-                for (int u = u0; u < u1; ++u) {
-                    const float y = c.approx[(item * c.row_tiles + rt) * c.groups + u];
-                    x = fmaxf(x, y);
-                }
-        }
-        keys[j] = x;
-        odd = odd || !(__builtin_fabsf(x) < INFINITY);
-        least = fminf(least, x);
-        most = fmaxf(most, x);
-    }
-    if (STORED) {
-        e = fmaxf(__builtin_fabsf(least), __builtin_fabsf(most)) * 0x1p-23f;
-    } else {
-        for (int i = tid; i < c.row_tiles * c.runs; i += THREADS) {
-            const float y = c.bounds[item * c.row_tiles * c.runs + i];
-            odd = odd || !(y < INFINITY);
-            e = fmaxf(e, y);
-        }
-        e *= (float)(a.D + 8) * 0x1p-22f;
-    }
+    int32_t *out = a.out + (int64_t)blockIdx.x * a.count;
+    uint64_t *const score = (uint64_t *)c.scores + (int64_t)blockIdx.x * c.total;   // 64 bits a block
+    auto key_of = [&](int j) __attribute__((always_inline)) {
+        return STORED ? pick_key(__longlong_as_double((int64_t)score[lo + j])) : exact_key(c, b, hkv, tile, live, lo + j);
+    };
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) {
         least = fminf(least, __shfl_xor(least, off));
         most = fmaxf(most, __shfl_xor(most, off));
         e = fmaxf(e, __shfl_xor(e, off));
     }
-    if (__any(odd)) e = INFINITY;
-    if (lane == 0) { low[wave] = least; high[wave] = most; off_by[wave] = e; }
+    if (lane == 0) { room.low[wave] = least; room.high[wave] = most; room.off_by[wave] = e; }
+    room.hist[tid] = 0;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) { least = fminf(least, low[w]); most = fmaxf(most, high[w]); e = fmaxf(e, off_by[w]); }
+    for (int w = 0; w < PICK_WAVES; ++w) { least = fminf(least, room.low[w]); most = fmaxf(most, room.high[w]); e = fmaxf(e, room.off_by[w]); }
     e = 2.f * e + 0x1p-100f;   // of two scores' difference, also where products are too small for float32
 
     // ---- the bin of the kth best
     u32 left = want, among = (u32)n;
     float from = least, to = most;
     if (e < INFINITY) {
-        for (int pass = 0; pass < 4 && among > 8 && to - from > e; ++pass) {
-            const float by = 255.f / (to - from);   // (bin 255: the largest alone)
-            if (tid < 256) hist[tid] = 0;
-            __syncthreads();
-            for (int j = tid; j < n; j += THREADS) {
+#pragma unroll 1
+        for (int pass = 0; pass < 4 && among > PICK_WAVES && to - from > e; ++pass) {
+            const float by = (float)(PICK_THREADS - 1) / (to - from);   // (the last bin: the largest alone)
+            if (pass > 0) {
+                room.hist[tid] = 0;
+                __syncthreads();
+            }
+            for (int j = tid; j < n; j += PICK_THREADS) {
                 const float x = keys[j];
-                if (x >= from && x <= to) atomicAdd(&hist[(int)((x - from) * by) & 255], 1u);
+                if (x >= from && x <= to) atomicAdd(&room.hist[(u32)((x - from) * by) % PICK_THREADS], 1u);
             }
             __syncthreads();
-            const int bin = pick_bin(hist, left, found);
-            among = hist[bin];
+            const u32 bin = (u32)pick_bin(room.hist, left, room.waves, room.found);
+            among = room.hist[bin];
             float l = INFINITY, m = -INFINITY;
-            for (int j = tid; j < n; j += THREADS) {
+            for (int j = tid; j < n; j += PICK_THREADS) {
                 const float x = keys[j];
-                if (x >= from && x <= to && ((int)((x - from) * by) & 255) == bin) { l = fminf(l, x); m = fmaxf(m, x); }
+                if (x >= from && x <= to && (u32)((x - from) * by) % PICK_THREADS == bin) { l = fminf(l, x); m = fmaxf(m, x); }
             }
 #pragma unroll
             for (int off = 32; off > 0; off >>= 1) { l = fminf(l, __shfl_xor(l, off)); m = fmaxf(m, __shfl_xor(m, off)); }
+            if (lane == 0) { room.low[wave] = l; room.high[wave] = m; }
             __syncthreads();
-            if (lane == 0) { low[wave] = l; high[wave] = m; }
-            __syncthreads();
-            from = low[0]; to = high[0];
+            from = room.low[0]; to = room.high[0];
 #pragma unroll
-            for (int w = 1; w < WAVES; ++w) { from = fminf(from, low[w]); to = fmaxf(to, high[w]); }
+            for (int w = 1; w < PICK_WAVES; ++w) { from = fminf(from, room.low[w]); to = fmaxf(to, room.high[w]); }
         }
     }
     const float over = e < INFINITY ? to + e : INFINITY, under = e < INFINITY ? from - e : -INFINITY;
 
     // ---- those between
     u32 sure = 0, doubt = 0;
-    __syncthreads();
-    for (int j0 = 0; j0 < n; j0 += THREADS) {
+    for (int j0 = 0; j0 < n; j0 += PICK_THREADS) {
         const float x = j0 + tid < n ? keys[j0 + tid] : -INFINITY;
         const bool here = j0 + tid < n, in = here && x > over, maybe = here && !in && !(x < under);
         u32 some;
-        const u32 at = block_before<WAVES>(maybe, some, waves);
-        if (maybe && doubt + at < PICK_LIST) list[doubt + at] = j0 + tid;
-        doubt += some;
-        (void)block_before<WAVES>(in, some, waves);
-        sure += some;
+        const u32 at = doubt + (block_before(maybe, in, some, room.waves) & 0xFFFFu);
+        if (maybe && at < PICK_LIST) room.list[at] = j0 + tid;
+        doubt += some & 0xFFFFu;
+        sure += some >> 16;
     }
     const u32 need = want - sure;   // of the doubtful
     __syncthreads();
     if (doubt > PICK_LIST) {
         // all of them by their bits; the sure ones as the highest
-        for (int j = wave; j < n; j += WAVES) {
+        for (int j = wave; j < n; j += PICK_WAVES) {
             const float x = keys[j];
-            uint64_t k;
-            if (x > over) k = ~UINT64_C(0);
-            else if (x < under) k = 0;
-            else k = STORED ? pick_key(score[lo + j]) : exact_key(c, b, hkv, tile, lo + j);
-            if (lane == 0) ((uint64_t *)score)[lo + j] = k;
+            const uint64_t k = x > over ? ~UINT64_C(0) : x < under ? 0 : key_of(j);
+            if (lane == 0) score[lo + j] = k;
         }
         __threadfence_block();
         __syncthreads();
-        const uint64_t *all = (const uint64_t *)score + lo;
+        const uint64_t *all = score + lo;
         uint64_t key = 0;
         left = want;
         for (int shift = 56; shift >= 0; shift -= 8) {
-            if (tid < 256) hist[tid] = 0;
+            room.hist[tid] = 0;
             __syncthreads();
-            for (int j = tid; j < n; j += THREADS)
-                if (shift == 56 || (all[j] ^ key) >> (shift + 8) == 0) atomicAdd(&hist[all[j] >> shift & 255], 1u);
+            for (int j = tid; j < n; j += PICK_THREADS)
+                if (shift == 56 || (all[j] ^ key) >> (shift + 8) == 0) atomicAdd(&room.hist[all[j] >> shift & 255], 1u);
             __syncthreads();
-            key |= (uint64_t)pick_bin(hist, left, found) << shift;
+            key |= (uint64_t)pick_bin(room.hist, left, room.waves, room.found) << shift;
             __syncthreads();
         }
         u32 equal = 0;
-        for (int j0 = 0; j0 < n; j0 += THREADS) {
+        for (int j0 = 0; j0 < n; j0 += PICK_THREADS) {
             const int j = j0 + tid;
             u32 some;
-            const u32 rank = equal + block_before<WAVES>(j < n && all[j] == key, some, waves);
+            const u32 rank = equal + block_before(j < n && all[j] == key, false, some, room.waves);
             equal += some;
             if (j < n) keys[j] = all[j] > key || (all[j] == key && rank < left) ? INFINITY : -INFINITY;
         }
     } else if (doubt > need) {
-        for (u32 i = wave; i < doubt; i += WAVES) {
-            const uint64_t k = STORED ? pick_key(score[lo + list[i]]) : exact_key(c, b, hkv, tile, lo + list[i]);
-            if (lane == 0) exact[i] = k;
+        for (u32 i = wave; i < doubt; i += PICK_WAVES) {
+            const uint64_t k = key_of(room.list[i]);
+            if (lane == 0) room.exact[i] = k;
         }
         __syncthreads();
-        for (u32 i = tid; i < doubt; i += THREADS) {
-            const uint64_t k = exact[i];
+        for (u32 i = tid; i < doubt; i += PICK_THREADS) {
+            const uint64_t k = room.exact[i];
             u32 better = 0;   // (the list ascends: of equal scores the lower block comes first)
-            for (u32 o = 0; o < doubt; ++o) better += exact[o] > k || (exact[o] == k && o < i) ? 1 : 0;
-            keys[list[i]] = better < need ? INFINITY : -INFINITY;
+            for (u32 o = 0; o < doubt; ++o) better += room.exact[o] > k || (room.exact[o] == k && o < i) ? 1 : 0;
+            keys[room.list[i]] = better < need ? INFINITY : -INFINITY;
         }
     } else {
-        for (u32 i = tid; i < doubt; i += THREADS) keys[list[i]] = INFINITY;
+        for (u32 i = tid; i < doubt; i += PICK_THREADS) keys[room.list[i]] = INFINITY;
     }
     __syncthreads();
     // ---- in order
     u32 done = 0;
-    for (int j0 = 0; j0 < n; j0 += THREADS) {
+    for (int j0 = 0; j0 < n; j0 += PICK_THREADS) {
         const bool take = j0 + tid < n && (keys[j0 + tid] == INFINITY || keys[j0 + tid] > over);
         u32 some;
-        const u32 at = done + block_before<WAVES>(take, some, waves);
+        const u32 at = done + block_before(take, false, some, room.waves);
         if (take) out[lo + at] = lo + j0 + tid;
         done += some;
     }
 }
 
-constexpr int ANY_THREADS = 256;
+// A tile's place, what it sees, and the choices that need no score: all of at most `count` visible blocks, and else the first and the recent ones.
+// False: nothing is left to choose.
+struct PickTile { int b, hkv, tile, live, end, lo, n; u32 want; };
+__device__ __forceinline__ bool pick_begin(const SelectCall &c, PickTile &t) {
+    const vq_block_select_args &a = c.a;
+    const u32 bh = blockIdx.x / (u32)c.tiles;
+    t.tile = (int)(blockIdx.x % (u32)c.tiles);
+    t.hkv = (int)(bh % (u32)a.Hkv);
+    t.b = (int)(bh / (u32)a.Hkv);
+    t.live = sel_live(a, t.b);
+    t.end = sel_end(a, t.live, sel_last(a, t.tile));
+    const int V = (int)((u32)(t.end + (int)a.block_tokens - 1) / (u32)a.block_tokens), count = (int)a.count;
+    int32_t *out = a.out + (int64_t)blockIdx.x * count;
+    if (V <= count) {
+        for (int i = threadIdx.x; i < count; i += blockDim.x) out[i] = i < V ? i : -1;
+        return false;
+    }
+    t.lo = (int)a.first;
+    t.n = V - (int)a.recent - t.lo;
+    t.want = (u32)(count - (int)a.first - (int)a.recent);   // of n, which are more
+    for (int i = threadIdx.x; i < t.lo; i += blockDim.x) out[i] = i;
+    for (int i = threadIdx.x; i < (int)a.recent; i += blockDim.x) out[count - (int)a.recent + i] = t.lo + t.n + i;
+    return t.want > 0;
+}
+
+// A thread's blocks' approximate scores from those of their groups (row tile rt's at approx + rt * groups).
+__device__ __forceinline__ void pick_blocks(const SelectCall &c, const PickTile &t, const float *approx, int row_tiles, int groups, float *keys, float &least, float &most, float &e) {
+    const int per = (int)c.a.block_tokens / c.a.group, seen = (t.end + c.a.group - 1) / c.a.group;   // groups of a block, groups that some row sees
+    for (int j = threadIdx.x; j < t.n; j += PICK_THREADS) {
+        const int u0 = (t.lo + j) * per, u1 = u0 + per < seen ? u0 + per : seen;
+        float x = -INFINITY;
+        for (int rt = 0; rt < row_tiles; ++rt)
+            for (int u = u0; u < u1; ++u) x = fmaxf(x, approx[(int64_t)rt * groups + u]);
+        keys[j] = x;
+        if (!(__builtin_fabsf(x) < INFINITY)) e = INFINITY;
+        least = fminf(least, x);
+        most = fmaxf(most, x);
+    }
+}
+__device__ __forceinline__ float pick_error(const SelectCall &c, float bound) { return bound < INFINITY ? bound * ((float)(c.a.D + 8) * 0x1p-22f) : INFINITY; }
+
+template <bool STORED> __global__ __launch_bounds__(PICK_THREADS) void block_pick_kernel(SelectCall c) {
+    extern __shared__ float keys[];
+    __shared__ PickRoom room;
+    PickTile t;
+    if (!pick_begin(c, t)) return;
+    float least = INFINITY, most = -INFINITY, e = 0.f;
+    if (STORED) {
+        for (int j = threadIdx.x; j < t.n; j += PICK_THREADS) {
+            const float x = (float)c.scores[blockIdx.x * c.total + t.lo + j];
+            keys[j] = x;
+            e = __builtin_fabsf(x) < INFINITY ? fmaxf(e, __builtin_fabsf(x) * 0x1p-23f) : INFINITY;
+            least = fminf(least, x);
+            most = fmaxf(most, x);
+        }
+    } else {
+        const int many = c.row_tiles * c.runs;
+        for (int i = threadIdx.x; i < many; i += PICK_THREADS) e = fmaxf(e, pick_error(c, c.bounds[(int64_t)blockIdx.x * many + i]));
+        pick_blocks(c, t, c.approx + (int64_t)blockIdx.x * c.row_tiles * c.groups, c.row_tiles, (int)c.groups, keys, least, most, e);
+    }
+    pick<STORED>(c, room, keys, t.b, t.hkv, t.tile, t.live, t.lo, t.n, t.want, least, most, e);
+}
+
+// Scores and choice of a tile of up to 32 rows in one block, the scores in LDS.
+template <int D, bool BF16>
+__global__ __launch_bounds__(PICK_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2))) void block_choose_kernel(SelectCall c) {
+    extern __shared__ float keys[];   // [total], then the groups' scores
+    __shared__ PickRoom room;
+    PickTile t;
+    if (!pick_begin(c, t)) return;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), per = (int)c.a.block_tokens / c.a.group, seen = (t.end + c.a.group - 1) / c.a.group;
+    const int u0 = t.lo * per, u1 = (t.lo + t.n) * per < seen ? (t.lo + t.n) * per : seen;   // the groups of those to choose from
+    float *const approx = keys + c.total;
+    float least = INFINITY, most = -INFINITY, e = 0.f;
+    if (u0 + wave * 32 < u1) e = pick_error(c, bound_units<D, BF16>(c, t.b, t.hkv, t.tile, 0, t.live, u0 + wave * 32, u1, PICK_WAVES * 32, approx));
+    __syncthreads();
+    pick_blocks(c, t, approx, 1, 0, keys, least, most, e);
+    pick<false>(c, room, keys, t.b, t.hkv, t.tile, t.live, t.lo, t.n, t.want, least, most, e);
+}
 
 // The same over any number of blocks, their scores of 64 bits in memory throughout.
-__global__ __launch_bounds__(ANY_THREADS) void block_pick_any_kernel(SelectCall c) {
-    const vq_block_select_args &a = c.a;
-    __shared__ u32 hist[256], waves[ANY_THREADS / 64], found[6];
+__global__ __launch_bounds__(PICK_THREADS) void block_pick_any_kernel(SelectCall c) {
+    __shared__ u32 hist[PICK_THREADS], waves[PICK_WAVES], found[2];
+    PickTile t;
+    if (!pick_begin(c, t)) return;
     const int tid = threadIdx.x;
-    const int64_t item = blockIdx.x, tile = item % c.tiles, b = item / c.tiles / a.Hkv;
-    const int64_t V = (sel_end(a, (int)b, sel_last(a, (int)tile)) + a.block_tokens - 1) / a.block_tokens;
-    int32_t *out = a.out + item * a.count;
-    if (V <= a.count) {
-        for (int64_t i = tid; i < a.count; i += ANY_THREADS) out[i] = i < V ? (int32_t)i : -1;
-        return;
-    }
-    const double *score = c.scores + item * c.total;
-    const int lo = (int)a.first, hi = (int)(V - a.recent);
-    u32 left = (u32)(a.count - a.first - a.recent);
-    for (int64_t i = tid; i < a.first; i += ANY_THREADS) out[i] = (int32_t)i;
-    for (int64_t i = tid; i < a.recent; i += ANY_THREADS) out[a.count - a.recent + i] = (int32_t)(hi + i);
-    if (left == 0) return;
+    const double *score = c.scores + blockIdx.x * c.total + t.lo;
+    int32_t *out = c.a.out + (int64_t)blockIdx.x * c.a.count + t.lo;
+    u32 left = t.want;
     uint64_t key = 0;
     for (int shift = 56; shift >= 0; shift -= 8) {
         hist[tid] = 0;
         __syncthreads();
-        for (int j = lo + tid; j < hi; j += ANY_THREADS) {
+        for (int j = tid; j < t.n; j += PICK_THREADS) {
             const uint64_t k = pick_key(score[j]);
             if (shift == 56 || (k ^ key) >> (shift + 8) == 0) atomicAdd(&hist[k >> shift & 255], 1u);
         }
         __syncthreads();
-        key |= (uint64_t)pick_bin(hist, left, found) << shift;
+        key |= (uint64_t)pick_bin(hist, left, waves, found) << shift;
         __syncthreads();
     }
     u32 done = 0, equal = 0;
-    for (int j0 = lo; j0 < hi; j0 += ANY_THREADS) {
+    for (int j0 = 0; j0 < t.n; j0 += PICK_THREADS) {
         const int j = j0 + tid;
-        const uint64_t k = j < hi ? pick_key(score[j]) : 0;
+        const uint64_t k = j < t.n ? pick_key(score[j]) : 0;
         u32 some;
-        const u32 rank = equal + block_before<ANY_THREADS / 64>(j < hi && k == key, some, waves);
+        const u32 rank = equal + block_before(j < t.n && k == key, false, some, waves);
         equal += some;
-        const bool take = j < hi && (k > key || (k == key && rank < left));
-        const u32 at = done + block_before<ANY_THREADS / 64>(take, some, waves);
-        if (take) out[lo + at] = j;
+        const bool take = j < t.n && (k > key || (k == key && rank < left));
+        const u32 at = done + block_before(take, false, some, waves);
+        if (take) out[at] = t.lo + j;
         done += some;
     }
 }
@@ -611,6 +665,7 @@ SelectCall cut_select(const vq_block_select_args &a) {
         c.runs = (int)cdiv(units, c.run_units);
         // (the products and the grid of a call of this size are left to the vector units)
         if ((double)c.items * c.row_tiles * (double)c.groups >= 67108864.) c.mma = 0;
+        c.one = c.mma && c.row_tiles == 1 && (c.total + c.groups) * 4 <= PICK_MOST * 4;
     }
     return c;
 }
@@ -621,18 +676,16 @@ SelectRoom select_room(const SelectCall &c) {
     auto whole = [](size_t n) { return (n + 15) / 16 * 16; };
     r.approx = whole((size_t)(c.items * c.total) * 8);
     r.bounds = r.all = r.approx;
-    if (c.mma) {
+    if (c.mma && !c.one) {
         r.bounds = r.approx + whole((size_t)(c.items * c.row_tiles * c.groups) * 4);
         r.all = r.bounds + whole((size_t)(c.items * c.row_tiles * c.runs) * 4);
     }
     return r;
 }
 
-// (the scores of up to PICK_MOST blocks and the tables beside them pass the 64 KB that a block has unasked)
-template <bool STORED, int THREADS> int launch_pick_of(const char *fn, const SelectCall &c, size_t bytes, hipStream_t st) {
-    const auto kernel = block_pick_kernel<STORED, THREADS>;
+// (`bytes` of scores beside the tables may pass the 64 KB that a block has unasked)
+template <typename Kernel> int launch_pick(const char *fn, Kernel kernel, std::atomic<bool> *allowed, const SelectCall &c, size_t bytes, hipStream_t st) {
     if (bytes > 48 * 1024) {
-        static std::atomic<bool> allowed[64] = {};
         int dev = 0;
         (void)hipGetDevice(&dev);
         if (dev < 0 || dev >= 64 || !allowed[dev].load(std::memory_order_acquire)) {
@@ -641,17 +694,19 @@ template <bool STORED, int THREADS> int launch_pick_of(const char *fn, const Sel
             if (dev >= 0 && dev < 64) allowed[dev].store(true, std::memory_order_release);
         }
     }
-    kernel<<<(unsigned)c.items, THREADS, bytes, st>>>(c);
+    kernel<<<(unsigned)c.items, PICK_THREADS, bytes, st>>>(c);
+    VQ_HIP_CHECK_LAUNCH(fn);
     return VQ_OK;
 }
-template <bool STORED> int launch_pick(const char *fn, const SelectCall &c, size_t bytes, hipStream_t st) {
-    return c.total > 256 ? launch_pick_of<STORED, 1024>(fn, c, bytes, st) : launch_pick_of<STORED, 256>(fn, c, bytes, st);
+template <int D, bool BF16> int launch_choice(const char *fn, const SelectCall &c, hipStream_t st) {
+    static std::atomic<bool> allowed[2][64] = {};
+    if (c.one) return launch_pick(fn, block_choose_kernel<D, BF16>, allowed[0], c, (size_t)(c.total + c.groups) * 4, st);
+    block_bound_kernel<D, BF16><<<(unsigned)cdiv(c.items * c.row_tiles * c.runs, 4), 256, 0, st>>>(c);
+    VQ_HIP_CHECK_LAUNCH(fn);
+    return launch_pick(fn, block_pick_kernel<false>, allowed[1], c, (size_t)c.total * 4, st);
 }
-
-template <int D> void launch_bounds(const SelectCall &c, hipStream_t st) {
-    const unsigned blocks = (unsigned)cdiv(c.items * c.row_tiles * c.runs, 4);
-    if (c.a.dtype == VQ_BF16) block_bound_kernel<D, true><<<blocks, 256, 0, st>>>(c);
-    else block_bound_kernel<D, false><<<blocks, 256, 0, st>>>(c);
+template <int D> int launch_choice(const char *fn, const SelectCall &c, hipStream_t st) {
+    return c.a.dtype == VQ_BF16 ? launch_choice<D, true>(fn, c, st) : launch_choice<D, false>(fn, c, st);
 }
 
 }  // namespace
@@ -674,22 +729,20 @@ extern "C" int vq_block_select(const vq_block_select_args *args) {
     VQ_REQUIRE(room.all == 0 || (a.workspace != nullptr && a.workspace_bytes >= room.all && ((uintptr_t)a.workspace & 15) == 0), VQ_ERR_WORKSPACE,
                "%s: workspace of %zu bytes required, 16-byte aligned", fn, room.all);
     hipStream_t st = (hipStream_t)a.stream;
-    const size_t lds = room.all > 0 && c.total <= PICK_MOST ? (size_t)c.total * 4 : 0;   // (no scores: every block is chosen)
     if (room.all > 0) {
         c.scores = (double *)a.workspace;
         c.approx = (float *)((char *)a.workspace + room.approx);
         c.bounds = (float *)((char *)a.workspace + room.bounds);
-        if (!c.mma) block_score_kernel<<<(unsigned)cdiv(c.items * c.total, 4), 256, 0, st>>>(c);
-        else if (a.D == 64) launch_bounds<64>(c, st);
-        else if (a.D == 128) launch_bounds<128>(c, st);
-        else launch_bounds<256>(c, st);
+        if (c.mma) return a.D == 64 ? launch_choice<64>(fn, c, st) : a.D == 128 ? launch_choice<128>(fn, c, st) : launch_choice<256>(fn, c, st);
+        block_score_kernel<<<(unsigned)cdiv(c.items * c.total, 4), 256, 0, st>>>(c);
         VQ_HIP_CHECK_LAUNCH(fn);
+        if (c.total > PICK_MOST) {
+            block_pick_any_kernel<<<(unsigned)c.items, PICK_THREADS, 0, st>>>(c);
+            VQ_HIP_CHECK_LAUNCH(fn);
+            return VQ_OK;
+        }
     }
-    if (c.total > PICK_MOST) {
-        block_pick_any_kernel<<<(unsigned)c.items, ANY_THREADS, 0, st>>>(c);
-    } else if (int rc = c.mma ? launch_pick<false>(fn, c, lds, st) : launch_pick<true>(fn, c, lds, st)) {
-        return rc;
-    }
-    VQ_HIP_CHECK_LAUNCH(fn);
-    return VQ_OK;
+    // (without a workspace: every visible block is chosen)
+    static std::atomic<bool> allowed[64] = {};
+    return launch_pick(fn, block_pick_kernel<true>, allowed, c, room.all > 0 ? (size_t)c.total * 4 : 0, st);
 }
