@@ -98,6 +98,22 @@ __device__ __forceinline__ u32 positive(u32 x) { return __builtin_bit_cast(u32, 
 __device__ __forceinline__ u32 max_bits(u32 x, u32 y) {   // of two magnitudes each
     return __builtin_bit_cast(u32, __builtin_elementwise_max(__builtin_bit_cast(u16x2, x), __builtin_bit_cast(u16x2, y)));
 }
+// of three halves each, NaN where one is: the largest of x, y and -y; of x, y and z; the smallest of x, y and z (none the result of a matrix product)
+__device__ __forceinline__ u32 top_magnitude(u32 x, u32 y) {
+    u32 r;
+    asm("v_pk_maximum3_f16 %0, %1, %2, %2 neg_lo:[0,0,1] neg_hi:[0,0,1]" : "=v"(r) : "v"(x), "v"(y));
+    return r;
+}
+__device__ __forceinline__ u32 top3(u32 x, u32 y, u32 z) {
+    u32 r;
+    asm("v_pk_maximum3_f16 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
+    return r;
+}
+__device__ __forceinline__ u32 low3(u32 x, u32 y, u32 z) {
+    u32 r;
+    asm("v_pk_minimum3_f16 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
+    return r;
+}
 __device__ __forceinline__ f32x16 mma(u32x4 x, u32x4 y, f32x16 acc) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, y), acc, 0, 0, 0);
 }
@@ -181,21 +197,26 @@ __device__ __forceinline__ float bound_units(const SelectCall &c, int b, int hkv
         f32x16 S, W;
 #pragma unroll
         for (int r = 0; r < 16; ++r) S[r] = W[r] = 0.f;
-        u32 sign = 0;
+        u32 low = 0;
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
             S = mma(q[k], x.z[k], S);
             u32x4 p;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                sign |= x.s[k][i];
-                top_z = max_bits(top_z, x.z[k][i] & 0x7FFF7FFFu);
-                top_s = max_bits(top_s, x.s[k][i] & 0x7FFF7FFFu);
+                top_z = top_magnitude(top_z, x.z[k][i]);
                 p[i] = positive(q[k][i]);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+                top_s = top3(top_s, x.s[k][i], x.s[k][i + 1]);
+                low = low3(low, x.s[k][i], x.s[k][i + 1]);
             }
             W = mma(p, x.s[k], W);
         }
-        if (__any((sign & 0x80008000u) != 0)) {
+        if (__any(low != 0)) {   // a scale below zero, or NaN
+            top_s = top_magnitude(top_s, low);
+
 #pragma unroll
             for (int r = 0; r < 16; ++r) W[r] = 0.f;
 #pragma unroll 1
@@ -237,6 +258,9 @@ __device__ __forceinline__ float bound_units(const SelectCall &c, int b, int hkv
             if (u + stride < u1) load(u + stride, ahead);
         }
     }
+    // (magnitudes' bits from here on, NaN's above all others)
+    top_z &= 0x7FFF7FFFu;
+    top_s &= 0x7FFF7FFFu;
     top_z = max_bits(top_z, __builtin_amdgcn_alignbyte(top_z, top_z, 2));
     top_s = max_bits(top_s, __builtin_amdgcn_alignbyte(top_s, top_s, 2));
 #pragma unroll
@@ -271,68 +295,68 @@ __device__ __forceinline__ uint64_t pick_key(double s) {   // ascending with the
 __device__ __forceinline__ uint64_t max_key(uint64_t x, uint64_t y) { return x > y ? x : y; }
 __device__ __forceinline__ double shfl_add(double s, int off) { return s + __shfl_xor(s, off); }
 
-// The key of block j's score in 64 bits, by a wave: 64 / R lanes a row (R the rows, up to the next power of two), eight channels at a time.
-__device__ __forceinline__ uint64_t exact_key(const SelectCall &c, int b, int hkv, int tile, int live, int j) {
-    constexpr int AHEAD = 4;   // steps of the channels whose loads are under way at once
+// The key of group u's score in 64 bits, the largest over the tile's rows, by a wave: 64 / R lanes a row (R the rows, up to the next power of two),
+// eight channels at a time.
+__device__ __forceinline__ uint64_t exact_key(const SelectCall &c, int b, int hkv, int tile, int live, int u) {
+    constexpr int AHEAD = 8;   // steps of the channels whose loads are under way at once
     const vq_block_select_args &a = c.a;
-    const int lane = threadIdx.x & 63, G = (int)a.Hq / (int)a.Hkv, D = (int)a.D, g = a.group, per = (int)a.block_tokens / g;
+    const int lane = threadIdx.x & 63, G = (int)a.Hq / (int)a.Hkv, D = (int)a.D, g = a.group;
     const int pos0 = tile * (int)c.query_block, rows = (sel_last(a, tile) - pos0 + 1) * G;
     int many = 1;
     while (many < rows && many < 64) many <<= 1;
     const int parts = 64 / many, part = lane % parts;
+    const int64_t at = (((int64_t)b * a.Hkv + hkv) * c.stride + u) * D;
+    const u16 *const zero = (const u16 *)a.k_zero + at, *const scale = (const u16 *)a.k_scale + at;
     uint64_t best = 0;
     for (int r0 = 0; r0 < rows; r0 += many) {
         const int r = r0 + lane / parts, x = r < rows ? r : rows - 1, end = sel_end(a, live, pos0 + x / G);
         const u16 *q = (const u16 *)a.q + (((int64_t)b * a.Hq + hkv * G + x % G) * a.Sq + pos0 + x / G) * D;
-        for (int u = j * per; u < (j + 1) * per && u < (int)c.groups; ++u) {
-            const int64_t at = (((int64_t)b * a.Hkv + hkv) * c.stride + u) * D;
-            double s = 0.;
-            for (int d0 = part * 8; d0 < D; d0 += AHEAD * parts * 8) {
-                u32x4 x4[AHEAD], z4[AHEAD], s4[AHEAD];
+        double s = 0.;
+        for (int d0 = part * 8; d0 < D; d0 += AHEAD * parts * 8) {
+            u32x4 x4[AHEAD], z4[AHEAD], s4[AHEAD];
 #pragma unroll
-                for (int k = 0; k < AHEAD; ++k) {
-                    const int d = d0 + k * parts * 8;
-                    if (k > 0 && d >= D) { x4[k] = z4[k] = s4[k] = u32x4{0, 0, 0, 0}; continue; }
-                    x4[k] = *(const u32x4 *)(q + d);
-                    z4[k] = *(const u32x4 *)((const u16 *)a.k_zero + at + d);
-                    s4[k] = *(const u32x4 *)((const u16 *)a.k_scale + at + d);
-                }
+            for (int k = 0; k < AHEAD; ++k) {
+                const int d = d0 + k * parts * 8;
+                if (k > 0 && d >= D) { x4[k] = z4[k] = s4[k] = u32x4{0, 0, 0, 0}; continue; }
+                x4[k] = *(const u32x4 *)(q + d);
+                z4[k] = *(const u32x4 *)(zero + d);
+                s4[k] = *(const u32x4 *)(scale + d);
+            }
 #pragma unroll
-                for (int k = 0; k < AHEAD; ++k) {
-                    if (k > 0 && d0 + k * parts * 8 >= D) break;
+            for (int k = 0; k < AHEAD; ++k) {
+                if (k > 0 && d0 + k * parts * 8 >= D) break;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const u16 xb = (u16)(x4[k][i / 2] >> (16 * (i & 1)));
-                        const double y = a.dtype == VQ_BF16 ? (double)bf16_to_f32(xb) : (double)(float)__builtin_bit_cast(f16, xb);
-                        const double z = (double)(float)as_h2(z4[k][i / 2])[i & 1], r1 = y * (double)(float)as_h2(s4[k][i / 2])[i & 1] * a.levels;
-                        s += y * z + (r1 > 0. || r1 != r1 ? r1 : 0.);
-                    }
+                for (int i = 0; i < 8; ++i) {
+                    const u16 xb = (u16)(x4[k][i / 2] >> (16 * (i & 1)));
+                    const double y = a.dtype == VQ_BF16 ? (double)bf16_to_f32(xb) : (double)(float)__builtin_bit_cast(f16, xb);
+                    const double z = (double)(float)as_h2(z4[k][i / 2])[i & 1], r1 = y * (double)(float)as_h2(s4[k][i / 2])[i & 1] * a.levels;
+                    s += y * z + (r1 > 0. || r1 != r1 ? r1 : 0.);
                 }
             }
-            for (int off = 1; off < parts; off <<= 1) s = shfl_add(s, off);
-            if (u * g < end) best = max_key(best, pick_key(s));
         }
+        for (int off = 1; off < parts; off <<= 1) s = shfl_add(s, off);
+        if (u * g < end) best = max_key(best, pick_key(s));
     }
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) best = max_key(best, __shfl_xor((unsigned long long)best, off));
     return best;
 }
 
-constexpr int PICK_THREADS = 512, PICK_WAVES = PICK_THREADS / 64;
 constexpr int PICK_MOST = 16384;   // blocks whose scores are held in LDS
 constexpr int PICK_LIST = 512;     // blocks that are told apart in 64 bits there
 
 
-struct PickRoom {
-    u32 hist[PICK_THREADS], waves[PICK_WAVES], found[2];
-    float low[PICK_WAVES], high[PICK_WAVES], off_by[PICK_WAVES];
+template <int THREADS> struct PickRoom {
+    static constexpr int WAVES = THREADS / 64;
+    u32 hist[THREADS], waves[WAVES], found[2];
+    float low[WAVES], high[WAVES], off_by[WAVES];
     int list[PICK_LIST];
     uint64_t exact[PICK_LIST];
 };
 
 // How many threads below this one say `one` (lower half) and `two` (upper half; counts below 2^16), and in `total` how many in all.  (Two barriers
 // around each use of `waves`.)
-__device__ __forceinline__ u32 block_before(bool one, bool two, u32 &total, u32 *waves) {
+template <int WAVES> __device__ __forceinline__ u32 block_before(bool one, bool two, u32 &total, u32 *waves) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const uint64_t m1 = __ballot(one), m2 = __ballot(two), below = (UINT64_C(1) << lane) - 1;
     __syncthreads();
@@ -341,7 +365,7 @@ __device__ __forceinline__ u32 block_before(bool one, bool two, u32 &total, u32 
     u32 before = (u32)__popcll(m1 & below) | (u32)__popcll(m2 & below) << 16;
     total = 0;
 #pragma unroll
-    for (int w = 0; w < PICK_WAVES; ++w) {
+    for (int w = 0; w < WAVES; ++w) {
         const u32 x = waves[w];
         before += w < wave ? x : 0;
         total += x;
@@ -351,7 +375,7 @@ __device__ __forceinline__ u32 block_before(bool one, bool two, u32 &total, u32 
 
 // The bin, a thread each, that holds the `left`-th from the highest bin down; `left` becomes how many of that bin are wanted.  (A barrier
 // lies between the last count and the call.)
-__device__ __forceinline__ int pick_bin(const u32 *hist, u32 &left, u32 *waves, u32 *found) {
+template <int WAVES> __device__ __forceinline__ int pick_bin(const u32 *hist, u32 &left, u32 *waves, u32 *found) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const u32 mine = hist[tid];
     u32 sum = mine;
@@ -361,7 +385,7 @@ __device__ __forceinline__ int pick_bin(const u32 *hist, u32 &left, u32 *waves, 
     __syncthreads();
     u32 above = sum - mine;
 #pragma unroll
-    for (int w = 1; w < PICK_WAVES; ++w) above += w > wave ? waves[w] : 0;
+    for (int w = 1; w < WAVES; ++w) above += w > wave ? waves[w] : 0;
     if (above < left && above + mine >= left) { found[0] = (u32)tid; found[1] = left - above; }
     __syncthreads();
     left = found[1];
@@ -376,16 +400,22 @@ __device__ __forceinline__ int pick_bin(const u32 *hist, u32 &left, u32 *waves, 
 // not; the few between are told apart by their scores in 64 bits, a wave each.  Where these are more than PICK_LIST (equal scores, values that are
 // not finite, which make e so) all of them are, by a radix select over the bits.
 // STORED: the scores of 64 bits lie in memory; else they are formed here.
-template <bool STORED>
-__device__ __forceinline__ void pick(const SelectCall &c, PickRoom &room, float *keys, int b, int hkv, int tile, int live, int lo, int n, u32 want, float least, float most,
+template <bool STORED, int THREADS>
+__device__ __forceinline__ void pick(const SelectCall &c, PickRoom<THREADS> &room, float *keys, int b, int hkv, int tile, int live, int lo, int n, u32 want, float least, float most,
                                      float e) {
+    constexpr int WAVES = THREADS / 64;
     const vq_block_select_args &a = c.a;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int32_t *out = a.out + (int64_t)blockIdx.x * a.count;
     uint64_t *const score = (uint64_t *)c.scores + (int64_t)blockIdx.x * c.total;   // 64 bits a block
-    auto key_of = [&](int j) __attribute__((always_inline)) {
-        return STORED ? pick_key(__longlong_as_double((int64_t)score[lo + j])) : exact_key(c, b, hkv, tile, live, lo + j);
+    const int per = (int)a.block_tokens / a.group;   // groups of a block
+    // the key of a group of block j (group i of it), by a wave; 0 behind the last one
+    auto key_of = [&](int j, int i) __attribute__((always_inline)) -> uint64_t {
+        if (STORED) return pick_key(__longlong_as_double((int64_t)score[lo + j]));
+        const int u = (lo + j) * per + i;
+        return u < (int)c.groups ? exact_key(c, b, hkv, tile, live, u) : 0;
     };
+    const int parts = STORED ? 1 : per;
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) {
         least = fminf(least, __shfl_xor(least, off));
@@ -396,7 +426,7 @@ __device__ __forceinline__ void pick(const SelectCall &c, PickRoom &room, float 
     room.hist[tid] = 0;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < PICK_WAVES; ++w) { least = fminf(least, room.low[w]); most = fmaxf(most, room.high[w]); e = fmaxf(e, room.off_by[w]); }
+    for (int w = 0; w < WAVES; ++w) { least = fminf(least, room.low[w]); most = fmaxf(most, room.high[w]); e = fmaxf(e, room.off_by[w]); }
     e = 2.f * e + 0x1p-100f;   // of two scores' difference, also where products are too small for float32
 
     // ---- the bin of the kth best
@@ -404,23 +434,23 @@ __device__ __forceinline__ void pick(const SelectCall &c, PickRoom &room, float 
     float from = least, to = most;
     if (e < INFINITY) {
 #pragma unroll 1
-        for (int pass = 0; pass < 4 && among > PICK_WAVES && to - from > e; ++pass) {
-            const float by = (float)(PICK_THREADS - 1) / (to - from);   // (the last bin: the largest alone)
+        for (int pass = 0; pass < 4 && among > WAVES && to - from > e; ++pass) {
+            const float by = (float)(THREADS - 1) / (to - from);   // (the last bin: the largest alone)
             if (pass > 0) {
                 room.hist[tid] = 0;
                 __syncthreads();
             }
-            for (int j = tid; j < n; j += PICK_THREADS) {
+            for (int j = tid; j < n; j += THREADS) {
                 const float x = keys[j];
-                if (x >= from && x <= to) atomicAdd(&room.hist[(u32)((x - from) * by) % PICK_THREADS], 1u);
+                if (x >= from && x <= to) atomicAdd(&room.hist[(u32)((x - from) * by) % THREADS], 1u);
             }
             __syncthreads();
-            const u32 bin = (u32)pick_bin(room.hist, left, room.waves, room.found);
+            const u32 bin = (u32)pick_bin<WAVES>(room.hist, left, room.waves, room.found);
             among = room.hist[bin];
             float l = INFINITY, m = -INFINITY;
-            for (int j = tid; j < n; j += PICK_THREADS) {
+            for (int j = tid; j < n; j += THREADS) {
                 const float x = keys[j];
-                if (x >= from && x <= to && (u32)((x - from) * by) % PICK_THREADS == bin) { l = fminf(l, x); m = fmaxf(m, x); }
+                if (x >= from && x <= to && (u32)((x - from) * by) % THREADS == bin) { l = fminf(l, x); m = fmaxf(m, x); }
             }
 #pragma unroll
             for (int off = 32; off > 0; off >>= 1) { l = fminf(l, __shfl_xor(l, off)); m = fmaxf(m, __shfl_xor(m, off)); }
@@ -428,18 +458,18 @@ __device__ __forceinline__ void pick(const SelectCall &c, PickRoom &room, float 
             __syncthreads();
             from = room.low[0]; to = room.high[0];
 #pragma unroll
-            for (int w = 1; w < PICK_WAVES; ++w) { from = fminf(from, room.low[w]); to = fmaxf(to, room.high[w]); }
+            for (int w = 1; w < WAVES; ++w) { from = fminf(from, room.low[w]); to = fmaxf(to, room.high[w]); }
         }
     }
     const float over = e < INFINITY ? to + e : INFINITY, under = e < INFINITY ? from - e : -INFINITY;
 
     // ---- those between
     u32 sure = 0, doubt = 0;
-    for (int j0 = 0; j0 < n; j0 += PICK_THREADS) {
+    for (int j0 = 0; j0 < n; j0 += THREADS) {
         const float x = j0 + tid < n ? keys[j0 + tid] : -INFINITY;
         const bool here = j0 + tid < n, in = here && x > over, maybe = here && !in && !(x < under);
         u32 some;
-        const u32 at = doubt + (block_before(maybe, in, some, room.waves) & 0xFFFFu);
+        const u32 at = doubt + (block_before<WAVES>(maybe, in, some, room.waves) & 0xFFFFu);
         if (maybe && at < PICK_LIST) room.list[at] = j0 + tid;
         doubt += some & 0xFFFFu;
         sure += some >> 16;
@@ -448,9 +478,11 @@ __device__ __forceinline__ void pick(const SelectCall &c, PickRoom &room, float 
     __syncthreads();
     if (doubt > PICK_LIST) {
         // all of them by their bits; the sure ones as the highest
-        for (int j = wave; j < n; j += PICK_WAVES) {
+        for (int j = wave; j < n; j += WAVES) {
             const float x = keys[j];
-            const uint64_t k = x > over ? ~UINT64_C(0) : x < under ? 0 : key_of(j);
+            uint64_t k = x > over ? ~UINT64_C(0) : 0;
+            if (!(x > over) && !(x < under))
+                for (int i = 0; i < parts; ++i) k = max_key(k, key_of(j, i));
             if (lane == 0) score[lo + j] = k;
         }
         __threadfence_block();
@@ -461,42 +493,44 @@ __device__ __forceinline__ void pick(const SelectCall &c, PickRoom &room, float 
         for (int shift = 56; shift >= 0; shift -= 8) {
             room.hist[tid] = 0;
             __syncthreads();
-            for (int j = tid; j < n; j += PICK_THREADS)
+            for (int j = tid; j < n; j += THREADS)
                 if (shift == 56 || (all[j] ^ key) >> (shift + 8) == 0) atomicAdd(&room.hist[all[j] >> shift & 255], 1u);
             __syncthreads();
-            key |= (uint64_t)pick_bin(room.hist, left, room.waves, room.found) << shift;
+            key |= (uint64_t)pick_bin<WAVES>(room.hist, left, room.waves, room.found) << shift;
             __syncthreads();
         }
         u32 equal = 0;
-        for (int j0 = 0; j0 < n; j0 += PICK_THREADS) {
+        for (int j0 = 0; j0 < n; j0 += THREADS) {
             const int j = j0 + tid;
             u32 some;
-            const u32 rank = equal + block_before(j < n && all[j] == key, false, some, room.waves);
+            const u32 rank = equal + block_before<WAVES>(j < n && all[j] == key, false, some, room.waves);
             equal += some;
             if (j < n) keys[j] = all[j] > key || (all[j] == key && rank < left) ? INFINITY : -INFINITY;
         }
     } else if (doubt > need) {
-        for (u32 i = wave; i < doubt; i += PICK_WAVES) {
-            const uint64_t k = key_of(room.list[i]);
-            if (lane == 0) room.exact[i] = k;
+        for (u32 i = tid; i < doubt; i += THREADS) room.exact[i] = 0;
+        __syncthreads();
+        for (u32 i = wave; i < doubt * parts; i += WAVES) {
+            const uint64_t k = key_of(room.list[i / parts], i % parts);
+            if (lane == 0) atomicMax((unsigned long long *)&room.exact[i / parts], (unsigned long long)k);
         }
         __syncthreads();
-        for (u32 i = tid; i < doubt; i += PICK_THREADS) {
+        for (u32 i = tid; i < doubt; i += THREADS) {
             const uint64_t k = room.exact[i];
             u32 better = 0;   // (the list ascends: of equal scores the lower block comes first)
             for (u32 o = 0; o < doubt; ++o) better += room.exact[o] > k || (room.exact[o] == k && o < i) ? 1 : 0;
             keys[room.list[i]] = better < need ? INFINITY : -INFINITY;
         }
     } else {
-        for (u32 i = tid; i < doubt; i += PICK_THREADS) keys[room.list[i]] = INFINITY;
+        for (u32 i = tid; i < doubt; i += THREADS) keys[room.list[i]] = INFINITY;
     }
     __syncthreads();
     // ---- in order
     u32 done = 0;
-    for (int j0 = 0; j0 < n; j0 += PICK_THREADS) {
+    for (int j0 = 0; j0 < n; j0 += THREADS) {
         const bool take = j0 + tid < n && (keys[j0 + tid] == INFINITY || keys[j0 + tid] > over);
         u32 some;
-        const u32 at = done + block_before(take, false, some, room.waves);
+        const u32 at = done + block_before<WAVES>(take, false, some, room.waves);
         if (take) out[lo + at] = lo + j0 + tid;
         done += some;
     }
@@ -528,9 +562,9 @@ __device__ __forceinline__ bool pick_begin(const SelectCall &c, PickTile &t) {
 }
 
 // A thread's blocks' approximate scores from those of their groups (row tile rt's at approx + rt * groups).
-__device__ __forceinline__ void pick_blocks(const SelectCall &c, const PickTile &t, const float *approx, int row_tiles, int groups, float *keys, float &least, float &most, float &e) {
+template <int THREADS> __device__ __forceinline__ void pick_blocks(const SelectCall &c, const PickTile &t, const float *approx, int row_tiles, int groups, float *keys, float &least, float &most, float &e) {
     const int per = (int)c.a.block_tokens / c.a.group, seen = (t.end + c.a.group - 1) / c.a.group;   // groups of a block, groups that some row sees
-    for (int j = threadIdx.x; j < t.n; j += PICK_THREADS) {
+    for (int j = threadIdx.x; j < t.n; j += THREADS) {
         const int u0 = (t.lo + j) * per, u1 = u0 + per < seen ? u0 + per : seen;
         float x = -INFINITY;
         for (int rt = 0; rt < row_tiles; ++rt)
@@ -543,14 +577,14 @@ __device__ __forceinline__ void pick_blocks(const SelectCall &c, const PickTile 
 }
 __device__ __forceinline__ float pick_error(const SelectCall &c, float bound) { return bound < INFINITY ? bound * ((float)(c.a.D + 8) * 0x1p-22f) : INFINITY; }
 
-template <bool STORED> __global__ __launch_bounds__(PICK_THREADS) void block_pick_kernel(SelectCall c) {
+template <bool STORED, int THREADS> __global__ __launch_bounds__(THREADS) void block_pick_kernel(SelectCall c) {
     extern __shared__ float keys[];
-    __shared__ PickRoom room;
+    __shared__ PickRoom<THREADS> room;
     PickTile t;
     if (!pick_begin(c, t)) return;
     float least = INFINITY, most = -INFINITY, e = 0.f;
     if (STORED) {
-        for (int j = threadIdx.x; j < t.n; j += PICK_THREADS) {
+        for (int j = threadIdx.x; j < t.n; j += THREADS) {
             const float x = (float)c.scores[blockIdx.x * c.total + t.lo + j];
             keys[j] = x;
             e = __builtin_fabsf(x) < INFINITY ? fmaxf(e, __builtin_fabsf(x) * 0x1p-23f) : INFINITY;
@@ -559,32 +593,34 @@ template <bool STORED> __global__ __launch_bounds__(PICK_THREADS) void block_pic
         }
     } else {
         const int many = c.row_tiles * c.runs;
-        for (int i = threadIdx.x; i < many; i += PICK_THREADS) e = fmaxf(e, pick_error(c, c.bounds[(int64_t)blockIdx.x * many + i]));
-        pick_blocks(c, t, c.approx + (int64_t)blockIdx.x * c.row_tiles * c.groups, c.row_tiles, (int)c.groups, keys, least, most, e);
+        for (int i = threadIdx.x; i < many; i += THREADS) e = fmaxf(e, pick_error(c, c.bounds[(int64_t)blockIdx.x * many + i]));
+        pick_blocks<THREADS>(c, t, c.approx + (int64_t)blockIdx.x * c.row_tiles * c.groups, c.row_tiles, (int)c.groups, keys, least, most, e);
     }
-    pick<STORED>(c, room, keys, t.b, t.hkv, t.tile, t.live, t.lo, t.n, t.want, least, most, e);
+    pick<STORED, THREADS>(c, room, keys, t.b, t.hkv, t.tile, t.live, t.lo, t.n, t.want, least, most, e);
 }
 
 // Scores and choice of a tile of up to 32 rows in one block, the scores in LDS.
-template <int D, bool BF16>
-__global__ __launch_bounds__(PICK_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2))) void block_choose_kernel(SelectCall c) {
+template <int D, bool BF16, int THREADS>
+__global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(2, 2))) void block_choose_kernel(SelectCall c) {
+    constexpr int WAVES = THREADS / 64;
     extern __shared__ float keys[];   // [total], then the groups' scores
-    __shared__ PickRoom room;
+    __shared__ PickRoom<THREADS> room;
     PickTile t;
     if (!pick_begin(c, t)) return;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), per = (int)c.a.block_tokens / c.a.group, seen = (t.end + c.a.group - 1) / c.a.group;
     const int u0 = t.lo * per, u1 = (t.lo + t.n) * per < seen ? (t.lo + t.n) * per : seen;   // the groups of those to choose from
     float *const approx = keys + c.total;
     float least = INFINITY, most = -INFINITY, e = 0.f;
-    if (u0 + wave * 32 < u1) e = pick_error(c, bound_units<D, BF16>(c, t.b, t.hkv, t.tile, 0, t.live, u0 + wave * 32, u1, PICK_WAVES * 32, approx));
+    if (u0 + wave * 32 < u1) e = pick_error(c, bound_units<D, BF16>(c, t.b, t.hkv, t.tile, 0, t.live, u0 + wave * 32, u1, WAVES * 32, approx));
     __syncthreads();
-    pick_blocks(c, t, approx, 1, 0, keys, least, most, e);
-    pick<false>(c, room, keys, t.b, t.hkv, t.tile, t.live, t.lo, t.n, t.want, least, most, e);
+    pick_blocks<THREADS>(c, t, approx, 1, 0, keys, least, most, e);
+    pick<false, THREADS>(c, room, keys, t.b, t.hkv, t.tile, t.live, t.lo, t.n, t.want, least, most, e);
 }
 
 // The same over any number of blocks, their scores of 64 bits in memory throughout.
-__global__ __launch_bounds__(PICK_THREADS) void block_pick_any_kernel(SelectCall c) {
-    __shared__ u32 hist[PICK_THREADS], waves[PICK_WAVES], found[2];
+__global__ __launch_bounds__(256) void block_pick_any_kernel(SelectCall c) {
+    constexpr int THREADS = 256, WAVES = THREADS / 64;
+    __shared__ u32 hist[THREADS], waves[WAVES], found[2];
     PickTile t;
     if (!pick_begin(c, t)) return;
     const int tid = threadIdx.x;
@@ -595,23 +631,23 @@ __global__ __launch_bounds__(PICK_THREADS) void block_pick_any_kernel(SelectCall
     for (int shift = 56; shift >= 0; shift -= 8) {
         hist[tid] = 0;
         __syncthreads();
-        for (int j = tid; j < t.n; j += PICK_THREADS) {
+        for (int j = tid; j < t.n; j += THREADS) {
             const uint64_t k = pick_key(score[j]);
             if (shift == 56 || (k ^ key) >> (shift + 8) == 0) atomicAdd(&hist[k >> shift & 255], 1u);
         }
         __syncthreads();
-        key |= (uint64_t)pick_bin(hist, left, waves, found) << shift;
+        key |= (uint64_t)pick_bin<WAVES>(hist, left, waves, found) << shift;
         __syncthreads();
     }
     u32 done = 0, equal = 0;
-    for (int j0 = 0; j0 < t.n; j0 += PICK_THREADS) {
+    for (int j0 = 0; j0 < t.n; j0 += THREADS) {
         const int j = j0 + tid;
         const uint64_t k = j < t.n ? pick_key(score[j]) : 0;
         u32 some;
-        const u32 rank = equal + block_before(j < t.n && k == key, false, some, waves);
+        const u32 rank = equal + block_before<WAVES>(j < t.n && k == key, false, some, waves);
         equal += some;
         const bool take = j < t.n && (k > key || (k == key && rank < left));
-        const u32 at = done + block_before(take, false, some, waves);
+        const u32 at = done + block_before<WAVES>(take, false, some, waves);
         if (take) out[at] = t.lo + j;
         done += some;
     }
@@ -684,7 +720,7 @@ SelectRoom select_room(const SelectCall &c) {
 }
 
 // (`bytes` of scores beside the tables may pass the 64 KB that a block has unasked)
-template <typename Kernel> int launch_pick(const char *fn, Kernel kernel, std::atomic<bool> *allowed, const SelectCall &c, size_t bytes, hipStream_t st) {
+template <typename Kernel> int launch_pick(const char *fn, Kernel kernel, int threads, std::atomic<bool> *allowed, const SelectCall &c, size_t bytes, hipStream_t st) {
     if (bytes > 48 * 1024) {
         int dev = 0;
         (void)hipGetDevice(&dev);
@@ -694,16 +730,18 @@ template <typename Kernel> int launch_pick(const char *fn, Kernel kernel, std::a
             if (dev >= 0 && dev < 64) allowed[dev].store(true, std::memory_order_release);
         }
     }
-    kernel<<<(unsigned)c.items, PICK_THREADS, bytes, st>>>(c);
+    kernel<<<(unsigned)c.items, threads, bytes, st>>>(c);
     VQ_HIP_CHECK_LAUNCH(fn);
     return VQ_OK;
 }
 template <int D, bool BF16> int launch_choice(const char *fn, const SelectCall &c, hipStream_t st) {
-    static std::atomic<bool> allowed[2][64] = {};
-    if (c.one) return launch_pick(fn, block_choose_kernel<D, BF16>, allowed[0], c, (size_t)(c.total + c.groups) * 4, st);
+    static std::atomic<bool> allowed[3][64] = {};
+    const size_t scores = (size_t)(c.total + c.groups) * 4;
+    if (c.one && c.items <= 256) return launch_pick(fn, block_choose_kernel<D, BF16, 512>, 512, allowed[0], c, scores, st);
+    if (c.one) return launch_pick(fn, block_choose_kernel<D, BF16, 256>, 256, allowed[1], c, scores, st);
     block_bound_kernel<D, BF16><<<(unsigned)cdiv(c.items * c.row_tiles * c.runs, 4), 256, 0, st>>>(c);
     VQ_HIP_CHECK_LAUNCH(fn);
-    return launch_pick(fn, block_pick_kernel<false>, allowed[1], c, (size_t)c.total * 4, st);
+    return launch_pick(fn, block_pick_kernel<false, 512>, 512, allowed[2], c, (size_t)c.total * 4, st);
 }
 template <int D> int launch_choice(const char *fn, const SelectCall &c, hipStream_t st) {
     return c.a.dtype == VQ_BF16 ? launch_choice<D, true>(fn, c, st) : launch_choice<D, false>(fn, c, st);
@@ -737,12 +775,12 @@ extern "C" int vq_block_select(const vq_block_select_args *args) {
         block_score_kernel<<<(unsigned)cdiv(c.items * c.total, 4), 256, 0, st>>>(c);
         VQ_HIP_CHECK_LAUNCH(fn);
         if (c.total > PICK_MOST) {
-            block_pick_any_kernel<<<(unsigned)c.items, PICK_THREADS, 0, st>>>(c);
+            block_pick_any_kernel<<<(unsigned)c.items, 256, 0, st>>>(c);
             VQ_HIP_CHECK_LAUNCH(fn);
             return VQ_OK;
         }
     }
     // (without a workspace: every visible block is chosen)
     static std::atomic<bool> allowed[64] = {};
-    return launch_pick(fn, block_pick_kernel<true>, allowed, c, room.all > 0 ? (size_t)c.total * 4 : 0, st);
+    return launch_pick(fn, block_pick_kernel<true, 512>, 512, allowed, c, room.all > 0 ? (size_t)c.total * 4 : 0, st);
 }
