@@ -9,9 +9,7 @@
 //
 // The chosen ones come out in ascending order, -1 behind them where fewer are visible: the first `first` and the last `recent` visible
 // blocks always, the others by score.
-#include <atomic>
-
-#include "common.hpp"
+#include "attend_span_mfma.hpp"
 
 namespace vq {
 
@@ -88,12 +86,8 @@ __global__ __launch_bounds__(256) void block_score_kernel(SelectCall c) {
 
 // ---- the matrix units as a filter
 
-typedef uint32_t u32;
-typedef u32 u32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 
-__device__ __forceinline__ f16x2 as_h2(u32 x) { return __builtin_bit_cast(f16x2, x); }
 __device__ __forceinline__ u32 positive(u32 x) { return __builtin_bit_cast(u32, __builtin_elementwise_max(as_h2(x), f16x2{(f16)0.f, (f16)0.f})); }
 __device__ __forceinline__ u32 max_bits(u32 x, u32 y) {   // of two magnitudes each
     return __builtin_bit_cast(u32, __builtin_elementwise_max(__builtin_bit_cast(u16x2, x), __builtin_bit_cast(u16x2, y)));
@@ -114,9 +108,6 @@ __device__ __forceinline__ u32 low3(u32 x, u32 y, u32 z) {
     asm("v_pk_minimum3_f16 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
     return r;
 }
-__device__ __forceinline__ f32x16 mma(u32x4 x, u32x4 y, f32x16 acc) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, y), acc, 0, 0, 0);
-}
 
 // Bounds of 32 rows (the query heads of a kv head at the queries of a tile) and 32 groups a step, in float32:
 //
@@ -127,22 +118,37 @@ __device__ __forceinline__ f32x16 mma(u32x4 x, u32x4 y, f32x16 acc) {
 // bf16 queries become fp16 numbers by a power of two that puts a row tile's largest near 2^15.  Float32 sums of D terms are off by less than
 // (D + 8) 2^-22 sum |q| (|z| + L |s|): with the largest sum of |q| and the largest |z| and |s| the wave also writes a bound of that sum, so the
 // choice knows how far to trust the scores.  Bound by the bytes of the scales and zeros for one query a sequence.
-// One wave's run: units u0, u0 + step, .. of 32 groups below u1 (in groups; u0 < u1), each group's score to out; returns the bound of
+// Zeros and scales come asynchronously, in whole stretches of 1 KB, into the wave's ring, the next unit's ahead (as loads of a lane's own operands they touch a
+// cache line in four instructions: 16 sequences at 32k 27 us, this .. us); pieces of a row lie rotated by the row, so that the lanes that read them
+// spread over the banks.
+template <int D> struct BoundRing { static constexpr int HALF = 64 * D, BYTES = 2 * HALF, COPIES = HALF / 1024; };   // a wave's: zeros, scales of 32 groups
+
+// One wave's run: units u0, u0 + stride, .. of 32 groups below u1 (in groups; u0 < u1), each group's score to out; returns the bound of
 // sum |q| (|z| + L |s|) (the same in every lane; not finite where a query, scale or zero is not).
 template <int D, bool BF16>
-__device__ __forceinline__ float bound_units(const SelectCall &c, int b, int hkv, int tile, int rt, int live, int u0, int u1, int stride, float *out) {
-    constexpr int KS = D / 16;
+__device__ __forceinline__ float bound_units(const SelectCall &c, int b, int hkv, int tile, int rt, int live, int u0, int u1, int stride, float *out, char *ring) {
+    constexpr int KS = D / 16, CH = D / 8, N = BoundRing<D>::COPIES;
     const vq_block_select_args &a = c.a;
     const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5, G = (int)a.Hq / (int)a.Hkv, g = a.group;
     const int pos0 = tile * (int)c.query_block, rows = (sel_last(a, tile) - pos0 + 1) * G;
-    struct Unit { u32x4 z[KS], s[KS]; };
-    const int64_t first = ((int64_t)b * a.Hkv + hkv) * c.stride * D + 8 * h;
+    const int64_t first = ((int64_t)b * a.Hkv + hkv) * c.stride * D;
     const u16 *const zeros = (const u16 *)a.k_zero + first, *const scales = (const u16 *)a.k_scale + first;
-    auto load = [&](int u, Unit &x) __attribute__((always_inline)) {
-        const int64_t at = (int64_t)(u + n < u1 ? u + n : u1 - 1) * D;
+    auto copy = [&](const u16 *from, int u, u32 to) __attribute__((always_inline)) {   // (a group past the run's repeats the last)
+        const u16 *base = from + (int64_t)u * D;
 #pragma unroll
-        for (int k = 0; k < KS; ++k) { x.z[k] = *(const u32x4 *)(zeros + at + 16 * k); x.s[k] = *(const u32x4 *)(scales + at + 16 * k); }
+        for (int x = 0; x < N; ++x) {
+            const int t = x * (64 / CH) + lane / CH, row = t < u1 - u ? t : u1 - u - 1;
+            lds_copy16<0>(base, (u32)(row * D * 2 + sp_kpiece<D>(t, lane % CH) * 16), to + x * 1024);
+        }
     };
+    auto read = [&](const char *from, u32x4 (&x)[KS]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int k = 0; k < KS; ++k) x[k] = *(const u32x4 *)(from + n * D * 2 + sp_kpiece<D>(n, 2 * k + h) * 16);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (before a copy may land there)
+    };
+    const u32 zeros_at = lds_addr(ring), scales_at = zeros_at + BoundRing<D>::HALF;
+    copy(zeros, u0, zeros_at);
+    copy(scales, u0, scales_at);
     auto row_at = [&](int x) __attribute__((always_inline)) { x += rt * 32; return x < rows ? x : rows - 1; };
     u32x4 q[KS];
     {
@@ -151,8 +157,6 @@ __device__ __forceinline__ float bound_units(const SelectCall &c, int b, int hkv
 #pragma unroll
         for (int k = 0; k < KS; ++k) q[k] = *(const u32x4 *)(src + 16 * k);
     }
-    Unit ahead;
-    load(u0, ahead);
     float unscale = 1.f;
     if constexpr (BF16) {
         u32 top = 0;
@@ -189,30 +193,41 @@ __device__ __forceinline__ float bound_units(const SelectCall &c, int b, int hkv
 
     const int seen = sel_end(a, live, pos0);   // by every query
     u32 top_z = 0, top_s = 0;
-    auto step = [&](int u, const Unit &x) __attribute__((always_inline)) {
-        // (what is formed of the queries is formed anew in every step: held across them it would push other registers to scratch memory, whose reloads
-        // wait for the unit that is under way)
+#pragma unroll 1
+    for (int u = u0; u < u1; u += stride) {
+        const bool more = u + stride < u1;
+        // (what is formed of the queries is formed anew in every step: held across them it would take the registers of other waves)
 #pragma unroll
         for (int k = 0; k < KS; ++k) asm volatile("" : "+v"(q[k]));
         f32x16 S, W;
 #pragma unroll
         for (int r = 0; r < 16; ++r) S[r] = W[r] = 0.f;
+        u32x4 x[KS];
+        wait_copies<N>();   // the scales' copies may be under way
+        read(ring, x);
+        if (more) copy(zeros, u + stride, zeros_at);
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            S = SpanMma<f16>::mma(q[k], x[k], S);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top_z = top_magnitude(top_z, x[k][i]);
+        }
+        if (more) wait_copies<N>();
+        else wait_copies<0>();
+        read(ring + BoundRing<D>::HALF, x);
+        if (more) copy(scales, u + stride, scales_at);
         u32 low = 0;
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
-            S = mma(q[k], x.z[k], S);
             u32x4 p;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                top_z = top_magnitude(top_z, x.z[k][i]);
-                p[i] = positive(q[k][i]);
-            }
+            for (int i = 0; i < 4; ++i) p[i] = positive(q[k][i]);
 #pragma unroll
             for (int i = 0; i < 4; i += 2) {
-                top_s = top3(top_s, x.s[k][i], x.s[k][i + 1]);
-                low = low3(low, x.s[k][i], x.s[k][i + 1]);
+                top_s = top3(top_s, x[k][i], x[k][i + 1]);
+                low = low3(low, x[k][i], x[k][i + 1]);
             }
-            W = mma(p, x.s[k], W);
+            W = SpanMma<f16>::mma(p, x[k], W);
         }
         if (__any(low != 0)) {   // a scale below zero, or NaN
             top_s = top_magnitude(top_s, low);
@@ -226,8 +241,8 @@ __device__ __forceinline__ float bound_units(const SelectCall &c, int b, int hkv
                 for (int k = 0; k < KS; ++k) {
                     u32x4 p, y;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) { p[i] = positive(q[k][i] ^ flip); y[i] = positive(x.s[k][i] ^ flip); }
-                    W = mma(p, y, W);
+                    for (int i = 0; i < 4; ++i) { p[i] = positive(q[k][i] ^ flip); y[i] = positive(x[k][i] ^ flip); }
+                    W = SpanMma<f16>::mma(p, y, W);
                 }
             }
         }
@@ -246,17 +261,6 @@ __device__ __forceinline__ float bound_units(const SelectCall &c, int b, int hkv
         for (int r = 1; r < 16; ++r) best = fmaxf(best, S[r]);
         best = fmaxf(best, __shfl_xor(best, 32)) * unscale;
         if (h == 0 && u + n < u1) out[u + n] = best;
-    };
-#pragma unroll 1
-    for (int u = u0; u < u1; u += stride) {
-        if constexpr (D <= 128) {   // (the next unit's scales and zeros fit beside this one's)
-            const Unit x = ahead;
-            if (u + stride < u1) load(u + stride, ahead);
-            step(u, x);
-        } else {
-            step(u, ahead);
-            if (u + stride < u1) load(u + stride, ahead);
-        }
     }
     // (magnitudes' bits from here on, NaN's above all others)
     top_z &= 0x7FFF7FFFu;
@@ -270,9 +274,11 @@ __device__ __forceinline__ float bound_units(const SelectCall &c, int b, int hkv
 }
 
 // Items of many rows, and few of many groups: a wave a run of units, scores and bounds to memory.
-template <int D, bool BF16> __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2, D == 256 ? 1 : 2))) void block_bound_kernel(SelectCall c) {
+template <int D, bool BF16> __global__ __launch_bounds__(256) void block_bound_kernel(SelectCall c) {
+    extern __shared__ __align__(16) char rings[];
     const vq_block_select_args &a = c.a;
-    const u32 id = blockIdx.x * 4 + (u32)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const u32 id = blockIdx.x * 4 + (u32)wave;
     if (id >= (u32)c.items * (u32)c.row_tiles * (u32)c.runs) return;
     const int run = (int)(id % (u32)c.runs);
     const u32 tile_row = id / (u32)c.runs;   // (item, row tile)
@@ -281,7 +287,8 @@ template <int D, bool BF16> __global__ __launch_bounds__(256) __attribute__((amd
     const int groups = (sel_end(a, live, sel_last(a, tile)) + a.group - 1) / a.group;   // that some row sees
     const int u0 = run * c.run_units * 32, u1 = u0 + c.run_units * 32 < groups ? u0 + c.run_units * 32 : groups;
     float bound = 0.f;
-    if (u0 < u1) bound = bound_units<D, BF16>(c, b, hkv, tile, (int)(tile_row % (u32)c.row_tiles), live, u0, u1, 32, c.approx + (int64_t)tile_row * c.groups);
+    if (u0 < u1) bound = bound_units<D, BF16>(c, b, hkv, tile, (int)(tile_row % (u32)c.row_tiles), live, u0, u1, 32, c.approx + (int64_t)tile_row * c.groups,
+                                                   rings + wave * BoundRing<D>::BYTES);
     if ((threadIdx.x & 63) == 0) c.bounds[id] = bound;
 }
 
@@ -343,6 +350,7 @@ __device__ __forceinline__ uint64_t exact_key(const SelectCall &c, int b, int hk
 }
 
 constexpr int PICK_MOST = 16384;   // blocks whose scores are held in LDS
+constexpr int ONE_SCORES = 20 * 1024;   // bytes of scores beside the rings of eight waves
 constexpr int PICK_LIST = 512;     // blocks that are told apart in 64 bits there
 
 
@@ -601,9 +609,10 @@ template <bool STORED, int THREADS> __global__ __launch_bounds__(THREADS) void b
 
 // Scores and choice of a tile of up to 32 rows in one block, the scores in LDS.
 template <int D, bool BF16, int THREADS>
-__global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(2, 2))) void block_choose_kernel(SelectCall c) {
+__global__ __launch_bounds__(THREADS) void block_choose_kernel(SelectCall c) {
     constexpr int WAVES = THREADS / 64;
-    extern __shared__ float keys[];   // [total], then the groups' scores
+    extern __shared__ __align__(16) char rings[];   // of the waves, then the scores of the blocks and of the groups
+    float *const keys = (float *)(rings + WAVES * BoundRing<D>::BYTES);
     __shared__ PickRoom<THREADS> room;
     PickTile t;
     if (!pick_begin(c, t)) return;
@@ -611,7 +620,8 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(2, 2)))
     const int u0 = t.lo * per, u1 = (t.lo + t.n) * per < seen ? (t.lo + t.n) * per : seen;   // the groups of those to choose from
     float *const approx = keys + c.total;
     float least = INFINITY, most = -INFINITY, e = 0.f;
-    if (u0 + wave * 32 < u1) e = pick_error(c, bound_units<D, BF16>(c, t.b, t.hkv, t.tile, 0, t.live, u0 + wave * 32, u1, WAVES * 32, approx));
+    if (u0 + wave * 32 < u1) e = pick_error(c, bound_units<D, BF16>(c, t.b, t.hkv, t.tile, 0, t.live, u0 + wave * 32, u1, WAVES * 32, approx,
+                                                                       rings + wave * BoundRing<D>::BYTES));
     __syncthreads();
     pick_blocks<THREADS>(c, t, approx, 1, 0, keys, least, most, e);
     pick<false, THREADS>(c, room, keys, t.b, t.hkv, t.tile, t.live, t.lo, t.n, t.want, least, most, e);
@@ -701,7 +711,7 @@ SelectCall cut_select(const vq_block_select_args &a) {
         c.runs = (int)cdiv(units, c.run_units);
         // (the products and the grid of a call of this size are left to the vector units)
         if ((double)c.items * c.row_tiles * (double)c.groups >= 67108864.) c.mma = 0;
-        c.one = c.mma && c.row_tiles == 1 && (c.total + c.groups) * 4 <= PICK_MOST * 4;
+        c.one = c.mma && c.row_tiles == 1 && (c.total + c.groups) * 4 <= ONE_SCORES;
     }
     return c;
 }
@@ -719,33 +729,43 @@ SelectRoom select_room(const SelectCall &c) {
     return r;
 }
 
-// (`bytes` of scores beside the tables may pass the 64 KB that a block has unasked)
-template <typename Kernel> int launch_pick(const char *fn, Kernel kernel, int threads, std::atomic<bool> *allowed, const SelectCall &c, size_t bytes, hipStream_t st) {
-    if (bytes > 48 * 1024) {
+// `bytes` of block-shared memory, of `most` for other calls
+template <typename Kernel> int launch_of(const char *fn, Kernel kernel, int64_t blocks, int threads, size_t bytes, size_t most, std::atomic<bool> *allowed, const SelectCall &c) {
+    if (bytes > 48 * 1024) {   // (with the tables beside it more than a block has unasked)
         int dev = 0;
         (void)hipGetDevice(&dev);
         if (dev < 0 || dev >= 64 || !allowed[dev].load(std::memory_order_acquire)) {
-            const hipError_t e = hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, PICK_MOST * 4);
-            VQ_REQUIRE(e == hipSuccess, VQ_ERR_HIP, "%s: %d bytes of block-shared memory: %s", fn, PICK_MOST * 4, hipGetErrorString(e));
+            const hipError_t e = hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)most);
+            VQ_REQUIRE(e == hipSuccess, VQ_ERR_HIP, "%s: %zu bytes of block-shared memory: %s", fn, most, hipGetErrorString(e));
             if (dev >= 0 && dev < 64) allowed[dev].store(true, std::memory_order_release);
         }
     }
-    kernel<<<(unsigned)c.items, threads, bytes, st>>>(c);
+    kernel<<<(unsigned)blocks, threads, bytes, (hipStream_t)c.a.stream>>>(c);
     VQ_HIP_CHECK_LAUNCH(fn);
     return VQ_OK;
 }
-template <int D, bool BF16> int launch_choice(const char *fn, const SelectCall &c, hipStream_t st) {
-    static std::atomic<bool> allowed[3][64] = {};
-    const size_t scores = (size_t)(c.total + c.groups) * 4;
-    if (c.one && c.items <= 256) return launch_pick(fn, block_choose_kernel<D, BF16, 512>, 512, allowed[0], c, scores, st);
-    if (c.one) return launch_pick(fn, block_choose_kernel<D, BF16, 256>, 256, allowed[1], c, scores, st);
-    block_bound_kernel<D, BF16><<<(unsigned)cdiv(c.items * c.row_tiles * c.runs, 4), 256, 0, st>>>(c);
-    VQ_HIP_CHECK_LAUNCH(fn);
-    return launch_pick(fn, block_pick_kernel<false, 512>, 512, allowed[2], c, (size_t)c.total * 4, st);
+template <bool STORED> int launch_pick(const char *fn, const SelectCall &c, size_t bytes) {
+    static std::atomic<bool> allowed[64] = {};
+    return launch_of(fn, block_pick_kernel<STORED, 512>, c.items, 512, bytes, PICK_MOST * 4, allowed, c);
 }
-template <int D> int launch_choice(const char *fn, const SelectCall &c, hipStream_t st) {
-    return c.a.dtype == VQ_BF16 ? launch_choice<D, true>(fn, c, st) : launch_choice<D, false>(fn, c, st);
+template <int D, bool BF16, int THREADS> int launch_one(const char *fn, const SelectCall &c) {
+    constexpr size_t rings = THREADS / 64 * BoundRing<D>::BYTES;
+    static std::atomic<bool> allowed[64] = {};
+    return launch_of(fn, block_choose_kernel<D, BF16, THREADS>, c.items, THREADS, rings + (size_t)(c.total + c.groups) * 4, rings + ONE_SCORES, allowed, c);
 }
+template <int D, bool BF16> int launch_choice(const char *fn, const SelectCall &c) {
+    if (c.one) {
+        if constexpr (D < 256) {
+            if (c.items <= 256) return launch_one<D, BF16, 512>(fn, c);
+        }
+        return launch_one<D, BF16, 256>(fn, c);
+    }
+    constexpr size_t rings = 4 * BoundRing<D>::BYTES;
+    static std::atomic<bool> allowed[64] = {};
+    if (int rc = launch_of(fn, block_bound_kernel<D, BF16>, cdiv(c.items * c.row_tiles * c.runs, 4), 256, rings, rings, allowed, c)) return rc;
+    return launch_pick<false>(fn, c, (size_t)c.total * 4);
+}
+template <int D> int launch_choice(const char *fn, const SelectCall &c) { return c.a.dtype == VQ_BF16 ? launch_choice<D, true>(fn, c) : launch_choice<D, false>(fn, c); }
 
 }  // namespace
 
@@ -771,7 +791,7 @@ extern "C" int vq_block_select(const vq_block_select_args *args) {
         c.scores = (double *)a.workspace;
         c.approx = (float *)((char *)a.workspace + room.approx);
         c.bounds = (float *)((char *)a.workspace + room.bounds);
-        if (c.mma) return a.D == 64 ? launch_choice<64>(fn, c, st) : a.D == 128 ? launch_choice<128>(fn, c, st) : launch_choice<256>(fn, c, st);
+        if (c.mma) return a.D == 64 ? launch_choice<64>(fn, c) : a.D == 128 ? launch_choice<128>(fn, c) : launch_choice<256>(fn, c);
         block_score_kernel<<<(unsigned)cdiv(c.items * c.total, 4), 256, 0, st>>>(c);
         VQ_HIP_CHECK_LAUNCH(fn);
         if (c.total > PICK_MOST) {
@@ -781,6 +801,5 @@ extern "C" int vq_block_select(const vq_block_select_args *args) {
         }
     }
     // (without a workspace: every visible block is chosen)
-    static std::atomic<bool> allowed[64] = {};
-    return launch_pick(fn, block_pick_kernel<true, 512>, 512, allowed, c, room.all > 0 ? (size_t)c.total * 4 : 0, st);
+    return launch_pick<true>(fn, c, room.all > 0 ? (size_t)c.total * 4 : 0);
 }
