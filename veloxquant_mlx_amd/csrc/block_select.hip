@@ -92,17 +92,7 @@ __device__ __forceinline__ u32 positive(u32 x) { return __builtin_bit_cast(u32, 
 __device__ __forceinline__ u32 max_bits(u32 x, u32 y) {   // of two magnitudes each
     return __builtin_bit_cast(u32, __builtin_elementwise_max(__builtin_bit_cast(u16x2, x), __builtin_bit_cast(u16x2, y)));
 }
-// of three halves each, NaN where one is: the largest of x, y and -y; of x, y and z; the smallest of x, y and z (none the result of a matrix product)
-__device__ __forceinline__ u32 top_magnitude(u32 x, u32 y) {
-    u32 r;
-    asm("v_pk_maximum3_f16 %0, %1, %2, %2 neg_lo:[0,0,1] neg_hi:[0,0,1]" : "=v"(r) : "v"(x), "v"(y));
-    return r;
-}
-__device__ __forceinline__ u32 top3(u32 x, u32 y, u32 z) {
-    u32 r;
-    asm("v_pk_maximum3_f16 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
-    return r;
-}
+// the smallest of three halves each, NaN where one is (none the result of a matrix product)
 __device__ __forceinline__ u32 low3(u32 x, u32 y, u32 z) {
     u32 r;
     asm("v_pk_minimum3_f16 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
@@ -116,15 +106,15 @@ __device__ __forceinline__ u32 low3(u32 x, u32 y, u32 z) {
 // products of fp16 numbers with v_mfma_f32_32x32x16 (the last one only where a scale is negative; lane n = lane % 32, h = lane / 32: row or group n,
 // channels 16 ks + 8 h ..).  A wave keeps its rows' queries, walks a run of units of 32 groups and writes each group's largest bound over its rows.
 // bf16 queries become fp16 numbers by a power of two that puts a row tile's largest near 2^15.  Float32 sums of D terms are off by less than
-// (D + 8) 2^-22 sum |q| (|z| + L |s|): with the largest sum of |q| and the largest |z| and |s| the wave also writes a bound of that sum, so the
-// choice knows how far to trust the scores.  Bound by the bytes of the scales and zeros for one query a sequence.
+// (D + 8) 2^-22 A, A = sum |q| (|z| + L |s|), which the wave forms too, by a third product: the choice knows how far to trust the scores (with A
+// bounded by the largest sum of |q| times the largest |z| + L |s| it asked 64 bits for 3 to 5 blocks a tile).  Bound by the bytes of the scales and zeros for one query a sequence.
 // Zeros and scales come asynchronously, in whole stretches of 1 KB, into the wave's ring, the next unit's ahead (as loads of a lane's own operands they touch a
 // cache line in four instructions: 16 sequences at 32k 27 us, this .. us); pieces of a row lie rotated by the row, so that the lanes that read them
 // spread over the banks.
 template <int D> struct BoundRing { static constexpr int HALF = 64 * D, BYTES = 2 * HALF, COPIES = HALF / 1024; };   // a wave's: zeros, scales of 32 groups
 
-// One wave's run: units u0, u0 + stride, .. of 32 groups below u1 (in groups; u0 < u1), each group's score to out; returns the bound of
-// sum |q| (|z| + L |s|) (the same in every lane; not finite where a query, scale or zero is not).
+// One wave's run: units u0, u0 + stride, .. of 32 groups below u1 (in groups; u0 < u1), each group's score to out; returns the largest
+// A (the same in every lane; not finite where a query, scale or zero is not).
 template <int D, bool BF16>
 __device__ __forceinline__ float bound_units(const SelectCall &c, int b, int hkv, int tile, int rt, int live, int u0, int u1, int stride, float *out, char *ring) {
     constexpr int KS = D / 16, CH = D / 8, N = BoundRing<D>::COPIES;
@@ -182,27 +172,19 @@ __device__ __forceinline__ float bound_units(const SelectCall &c, int b, int hkv
         unscale *= __uint_as_float((u32)(127 - up2) << 23);
     }
     const float levels = (float)a.levels;
-    float size = 0.f;   // the largest row's sum of magnitudes
-#pragma unroll
-    for (int k = 0; k < KS; ++k)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) size += __builtin_fabsf((float)as_h2(q[k][i])[0]) + __builtin_fabsf((float)as_h2(q[k][i])[1]);
-    size += __shfl_xor(size, 32);
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) { const float o = __shfl_xor(size, off); size = o > size || o != o ? o : size; }
-
+    const u32 levels2 = __builtin_bit_cast(u32, f16x2{(f16)levels, (f16)levels});
     const int seen = sel_end(a, live, pos0);   // by every query
-    u32 top_z = 0, top_s = 0;
+    u32 most = 0;   // bits of the largest sum of |q| (|z| + L |s|), NaN above infinity above all else
 #pragma unroll 1
     for (int u = u0; u < u1; u += stride) {
         const bool more = u + stride < u1;
         // (what is formed of the queries is formed anew in every step: held across them it would take the registers of other waves)
 #pragma unroll
         for (int k = 0; k < KS; ++k) asm volatile("" : "+v"(q[k]));
-        f32x16 S, W;
+        f32x16 S, W, A;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) S[r] = W[r] = 0.f;
-        u32x4 x[KS];
+        for (int r = 0; r < 16; ++r) S[r] = W[r] = A[r] = 0.f;
+        u32x4 x[KS], y[KS];
         wait_copies<N>();   // the scales' copies may be under way
         read(ring, x);
         if (more) copy(zeros, u + stride, zeros_at);
@@ -210,7 +192,7 @@ __device__ __forceinline__ float bound_units(const SelectCall &c, int b, int hkv
         for (int k = 0; k < KS; ++k) {
             S = SpanMma<f16>::mma(q[k], x[k], S);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) top_z = top_magnitude(top_z, x[k][i]);
+            for (int i = 0; i < 4; ++i) y[k][i] = x[k][i] & 0x7FFF7FFFu;
         }
         if (more) wait_copies<N>();
         else wait_copies<0>();
@@ -218,34 +200,45 @@ __device__ __forceinline__ float bound_units(const SelectCall &c, int b, int hkv
         if (more) copy(scales, u + stride, scales_at);
         u32 low = 0;
 #pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) low = low3(low, x[k][i], x[k][i + 1]);
+        const bool negative = __any(low != 0);   // a scale below zero, or NaN
+        // |z| + L |s| as fp16 numbers, off by 2^-11 of themselves
+#pragma unroll
         for (int k = 0; k < KS; ++k) {
             u32x4 p;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) p[i] = positive(q[k][i]);
-#pragma unroll
-            for (int i = 0; i < 4; i += 2) {
-                top_s = top3(top_s, x[k][i], x[k][i + 1]);
-                low = low3(low, x[k][i], x[k][i + 1]);
+            for (int i = 0; i < 4; ++i) {
+                const u32 size = negative ? x[k][i] & 0x7FFF7FFFu : x[k][i];
+                y[k][i] = as_u(__builtin_elementwise_fma(as_h2(size), as_h2(levels2), as_h2(y[k][i])));
+                p[i] = q[k][i] & 0x7FFF7FFFu;
             }
-            W = SpanMma<f16>::mma(p, x[k], W);
+            A = SpanMma<f16>::mma(p, y[k], A);
         }
-        if (__any(low != 0)) {   // a scale below zero, or NaN
-            top_s = top_magnitude(top_s, low);
-
+        if (!negative) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) W[r] = 0.f;
+            for (int k = 0; k < KS; ++k) {
+                u32x4 p;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) p[i] = positive(q[k][i]);
+                W = SpanMma<f16>::mma(p, x[k], W);
+            }
+        } else {
 #pragma unroll 1
             for (int m = 0; m < 2; ++m) {
                 const u32 flip = m ? 0x80008000u : 0u;
 #pragma unroll
                 for (int k = 0; k < KS; ++k) {
-                    u32x4 p, y;
+                    u32x4 p, t;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) { p[i] = positive(q[k][i] ^ flip); y[i] = positive(x[k][i] ^ flip); }
-                    W = SpanMma<f16>::mma(p, y, W);
+                    for (int i = 0; i < 4; ++i) { p[i] = positive(q[k][i] ^ flip); t[i] = positive(x[k][i] ^ flip); }
+                    W = SpanMma<f16>::mma(p, t, W);
                 }
             }
         }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) { const u32 bits = __float_as_uint(A[r]); most = bits > most ? bits : most; }
 #pragma unroll
         for (int r = 0; r < 16; ++r) S[r] = __builtin_fmaf(levels, W[r], S[r]);
         if ((u + 31) * (int64_t)g >= seen) {   // groups that some queries do not see (in 64 bits: the last ones may lie past the store)
@@ -262,15 +255,9 @@ __device__ __forceinline__ float bound_units(const SelectCall &c, int b, int hkv
         best = fmaxf(best, __shfl_xor(best, 32)) * unscale;
         if (h == 0 && u + n < u1) out[u + n] = best;
     }
-    // (magnitudes' bits from here on, NaN's above all others)
-    top_z &= 0x7FFF7FFFu;
-    top_s &= 0x7FFF7FFFu;
-    top_z = max_bits(top_z, __builtin_amdgcn_alignbyte(top_z, top_z, 2));
-    top_s = max_bits(top_s, __builtin_amdgcn_alignbyte(top_s, top_s, 2));
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) { top_z = max_bits(top_z, __shfl_xor(top_z, off)); top_s = max_bits(top_s, __shfl_xor(top_s, off)); }
-    const float mz = (float)__builtin_bit_cast(f16, (u16)top_z), ms = (float)__builtin_bit_cast(f16, (u16)top_s);
-    return size * (mz + levels * ms) * unscale;
+    for (int off = 32; off > 0; off >>= 1) { const u32 o = __shfl_xor(most, off); most = o > most ? o : most; }
+    return __uint_as_float(most) * unscale;
 }
 
 // Items of many rows, and few of many groups: a wave a run of units, scores and bounds to memory.
@@ -404,9 +391,9 @@ template <int WAVES> __device__ __forceinline__ int pick_bin(const u32 *hist, u3
 // thread's, the last one how far a score may be off, infinite where something is not finite.
 //
 // The kth best is looked for among the approximate scores by bins between the smallest and the largest, again inside its bin while
-// that holds many.  With scores off by e at most, those above the bin's largest + 2 e are among the chosen, those below its smallest - 2 e are
-// not; the few between are told apart by their scores in 64 bits, a wave each.  Where these are more than PICK_LIST (equal scores, values that are
-// not finite, which make e so) all of them are, by a radix select over the bits.
+// that holds many, then in the bin's order.  With scores off by e at most, those more than 2 e above it are among the chosen, those more than 2 e
+// below are not; if not all of the few between are wanted, these are told apart by their scores in 64 bits, a wave a group.  Where these are more than
+// PICK_LIST (equal scores, values that are not finite, which make e so) they are by a radix select over the bits.
 // STORED: the scores of 64 bits lie in memory; else they are formed here.
 template <bool STORED, int THREADS>
 __device__ __forceinline__ void pick(const SelectCall &c, PickRoom<THREADS> &room, float *keys, int b, int hkv, int tile, int live, int lo, int n, u32 want, float least, float most,
@@ -442,7 +429,7 @@ __device__ __forceinline__ void pick(const SelectCall &c, PickRoom<THREADS> &roo
     float from = least, to = most;
     if (e < INFINITY) {
 #pragma unroll 1
-        for (int pass = 0; pass < 4 && among > WAVES && to - from > e; ++pass) {
+        for (int pass = 0; pass < 4 && among > 32 && to - from > e; ++pass) {
             const float by = (float)(THREADS - 1) / (to - from);   // (the last bin: the largest alone)
             if (pass > 0) {
                 room.hist[tid] = 0;
@@ -469,23 +456,67 @@ __device__ __forceinline__ void pick(const SelectCall &c, PickRoom<THREADS> &roo
             for (int w = 1; w < WAVES; ++w) { from = fminf(from, room.low[w]); to = fmaxf(to, room.high[w]); }
         }
     }
-    const float over = e < INFINITY ? to + e : INFINITY, under = e < INFINITY ? from - e : -INFINITY;
-
-    // ---- those between
-    u32 sure = 0, doubt = 0;
+    // ---- the list of those that may be the kth best, or are within e of it; t: the kth best's score, where the list is short
+    float over = e < INFINITY ? to + e : INFINITY, under = e < INFINITY ? from - e : -INFINITY;
+    u32 sure = 0, listed = 0;
     for (int j0 = 0; j0 < n; j0 += THREADS) {
         const float x = j0 + tid < n ? keys[j0 + tid] : -INFINITY;
         const bool here = j0 + tid < n, in = here && x > over, maybe = here && !in && !(x < under);
         u32 some;
-        const u32 at = doubt + (block_before<WAVES>(maybe, in, some, room.waves) & 0xFFFFu);
+        const u32 at = listed + (block_before<WAVES>(maybe, in, some, room.waves) & 0xFFFFu);
         if (maybe && at < PICK_LIST) room.list[at] = j0 + tid;
-        doubt += some & 0xFFFFu;
+        listed += some & 0xFFFFu;
         sure += some >> 16;
     }
-    const u32 need = want - sure;   // of the doubtful
+    const u32 need = want - sure;   // of the list
     __syncthreads();
-    if (doubt > PICK_LIST) {
-        // all of them by their bits; the sure ones as the highest
+    if (listed <= 64) {   // every wave the same
+        const int j = room.list[lane < (int)listed ? lane : 0];
+        const float x = lane < (int)listed ? keys[j] : -INFINITY;
+        u32 rank = 0;   // (equal ones in the list's order)
+        for (int o = 0; o < (int)listed; ++o) { const float y = __shfl(x, o); rank += y > x || (y == x && o < lane) ? 1 : 0; }
+        const uint64_t kth = __ballot(lane < (int)listed && rank == need - 1);
+        const float t = __shfl(x, kth != 0 ? __builtin_ctzll(kth) : 0);   // (none among values that are not finite: e is not either)
+        const bool in = lane < (int)listed && x > t + e, maybe = lane < (int)listed && !in && !(x < t - e);
+        const uint64_t m = __ballot(maybe);
+        const u32 doubt = (u32)__popcll(m), wanted = need - (u32)__popcll(__ballot(in));
+        const bool all = doubt == wanted;
+        const u32 mine = (u32)__popcll(m & ((UINT64_C(1) << lane) - 1));   // this lane's place among the doubtful
+        if (wave == 0 && maybe) { room.list[64 + mine] = j; room.exact[mine] = 0; }
+        __syncthreads();   // (every wave has read the list's scores, which the first one replaces)
+        if (!all) {
+            for (u32 i = wave; i < doubt * parts; i += WAVES) {
+                const uint64_t k = key_of(room.list[64 + i / parts], i % parts);
+                if (lane == 0) atomicMax((unsigned long long *)&room.exact[i / parts], (unsigned long long)k);
+            }
+            __syncthreads();
+        }
+        if (wave == 0 && lane < (int)listed) {
+            bool take = in || (maybe && all);
+            if (maybe && !all) {
+                const uint64_t k = room.exact[mine];
+                u32 better = 0;   // (the list ascends: of equal scores the lower block comes first)
+                for (u32 o = 0; o < doubt; ++o) better += room.exact[o] > k || (room.exact[o] == k && o < mine) ? 1 : 0;
+                take = better < wanted;
+            }
+            keys[j] = take ? INFINITY : -INFINITY;
+        }
+    } else if (listed <= PICK_LIST) {
+        for (u32 i = tid; i < listed; i += THREADS) room.exact[i] = 0;
+        __syncthreads();
+        for (u32 i = wave; i < listed * parts; i += WAVES) {
+            const uint64_t k = key_of(room.list[i / parts], i % parts);
+            if (lane == 0) atomicMax((unsigned long long *)&room.exact[i / parts], (unsigned long long)k);
+        }
+        __syncthreads();
+        for (u32 i = tid; i < listed; i += THREADS) {
+            const uint64_t k = room.exact[i];
+            u32 better = 0;
+            for (u32 o = 0; o < listed; ++o) better += room.exact[o] > k || (room.exact[o] == k && o < i) ? 1 : 0;
+            keys[room.list[i]] = better < need ? INFINITY : -INFINITY;
+        }
+    } else {
+        // all of the list by their bits; the sure ones as the highest
         for (int j = wave; j < n; j += WAVES) {
             const float x = keys[j];
             uint64_t k = x > over ? ~UINT64_C(0) : 0;
@@ -515,22 +546,6 @@ __device__ __forceinline__ void pick(const SelectCall &c, PickRoom<THREADS> &roo
             equal += some;
             if (j < n) keys[j] = all[j] > key || (all[j] == key && rank < left) ? INFINITY : -INFINITY;
         }
-    } else if (doubt > need) {
-        for (u32 i = tid; i < doubt; i += THREADS) room.exact[i] = 0;
-        __syncthreads();
-        for (u32 i = wave; i < doubt * parts; i += WAVES) {
-            const uint64_t k = key_of(room.list[i / parts], i % parts);
-            if (lane == 0) atomicMax((unsigned long long *)&room.exact[i / parts], (unsigned long long)k);
-        }
-        __syncthreads();
-        for (u32 i = tid; i < doubt; i += THREADS) {
-            const uint64_t k = room.exact[i];
-            u32 better = 0;   // (the list ascends: of equal scores the lower block comes first)
-            for (u32 o = 0; o < doubt; ++o) better += room.exact[o] > k || (room.exact[o] == k && o < i) ? 1 : 0;
-            keys[room.list[i]] = better < need ? INFINITY : -INFINITY;
-        }
-    } else {
-        for (u32 i = tid; i < doubt; i += THREADS) keys[room.list[i]] = INFINITY;
     }
     __syncthreads();
     // ---- in order
@@ -583,7 +598,7 @@ template <int THREADS> __device__ __forceinline__ void pick_blocks(const SelectC
         most = fmaxf(most, x);
     }
 }
-__device__ __forceinline__ float pick_error(const SelectCall &c, float bound) { return bound < INFINITY ? bound * ((float)(c.a.D + 8) * 0x1p-22f) : INFINITY; }
+__device__ __forceinline__ float pick_error(const SelectCall &c, float bound) { return bound < INFINITY ? bound * ((float)(c.a.D + 9) * 0x1p-22f) : INFINITY; }
 
 template <bool STORED, int THREADS> __global__ __launch_bounds__(THREADS) void block_pick_kernel(SelectCall c) {
     extern __shared__ float keys[];
