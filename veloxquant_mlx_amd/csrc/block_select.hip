@@ -123,12 +123,24 @@ __device__ __forceinline__ float bound_units(const SelectCall &c, int b, int hkv
     const int pos0 = tile * (int)c.query_block, rows = (sel_last(a, tile) - pos0 + 1) * G;
     const int64_t first = ((int64_t)b * a.Hkv + hkv) * c.stride * D;
     const u16 *const zeros = (const u16 *)a.k_zero + first, *const scales = (const u16 *)a.k_scale + first;
-    auto copy = [&](const u16 *from, int u, u32 to) __attribute__((always_inline)) {   // (a group past the run's repeats the last)
-        const u16 *base = from + (int64_t)u * D;
+    constexpr int TURN = D >= 128 ? CH / 4 : 1;   // copies until the pieces lie as in the first one
+    u32 place[TURN];
 #pragma unroll
-        for (int x = 0; x < N; ++x) {
-            const int t = x * (64 / CH) + lane / CH, row = t < u1 - u ? t : u1 - u - 1;
-            lds_copy16<0>(base, (u32)(row * D * 2 + sp_kpiece<D>(t, lane % CH) * 16), to + x * 1024);
+    for (int x = 0; x < TURN; ++x) {
+        const int t = x * (64 / CH) + lane / CH;
+        place[x] = (u32)(t * D * 2 + sp_kpiece<D>(t, lane % CH) * 16);
+    }
+    auto copy = [&](const u16 *from, int u, u32 to) __attribute__((always_inline)) {
+        const u16 *base = from + (int64_t)u * D;
+        if (u1 - u >= 32) {
+#pragma unroll
+            for (int x = 0; x < N; ++x) lds_copy16<0>(base + x / TURN * (TURN * 512), place[x % TURN], to + x * 1024);
+        } else {   // (a group past the run's repeats the last)
+#pragma unroll 1
+            for (int x = 0; x < N; ++x) {
+                const int t = x * (64 / CH) + lane / CH, row = t < u1 - u ? t : u1 - u - 1;
+                lds_copy16<0>(base, (u32)(row * D * 2 + sp_kpiece<D>(t, lane % CH) * 16), to + x * 1024);
+            }
         }
     };
     auto read = [&](const char *from, u32x4 (&x)[KS]) __attribute__((always_inline)) {
@@ -159,17 +171,13 @@ __device__ __forceinline__ float bound_units(const SelectCall &c, int b, int hkv
         for (int off = 32; off > 0; off >>= 1) { const u32 o = __shfl_xor(top, off); top = o > top ? o : top; }
         // 2^(141 - e) with e the largest's exponent field: below 2^15; what is not finite stays so
         const int e = (int)(top >> 7), up = e == 0 || e == 255 ? 0 : 141 - e;
-        const int up1 = up / 2, up2 = up - up1;   // (either factor is a normal number)
-        const float f1 = __uint_as_float((u32)(127 + up1) << 23), f2 = __uint_as_float((u32)(127 + up2) << 23);
-        unscale = __uint_as_float((u32)(127 - up1) << 23);
 #pragma unroll
         for (int k = 0; k < KS; ++k)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float x = __uint_as_float(q[k][i] << 16) * f1 * f2, y = __uint_as_float(q[k][i] & 0xFFFF0000u) * f1 * f2;
-                q[k][i] = __builtin_bit_cast(u32, f16x2{(f16)x, (f16)y});
-            }
-        unscale *= __uint_as_float((u32)(127 - up2) << 23);
+            for (int i = 0; i < 4; ++i)
+                q[k][i] = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_pkrtz(__builtin_amdgcn_ldexpf(__uint_as_float(q[k][i] << 16), up),
+                                                                             __builtin_amdgcn_ldexpf(__uint_as_float(q[k][i] & 0xFFFF0000u), up)));
+        unscale = __builtin_amdgcn_ldexpf(1.f, -up);
     }
     const float levels = (float)a.levels;
     const u32 levels2 = __builtin_bit_cast(u32, f16x2{(f16)levels, (f16)levels});
@@ -178,9 +186,10 @@ __device__ __forceinline__ float bound_units(const SelectCall &c, int b, int hkv
 #pragma unroll 1
     for (int u = u0; u < u1; u += stride) {
         const bool more = u + stride < u1;
-        // (what is formed of the queries is formed anew in every step: held across them it would take the registers of other waves)
+        if constexpr (D == 256) {   // (what is formed of the queries is held across the steps elsewhere)
 #pragma unroll
-        for (int k = 0; k < KS; ++k) asm volatile("" : "+v"(q[k]));
+            for (int k = 0; k < KS; ++k) asm volatile("" : "+v"(q[k]));
+        }
         f32x16 S, W, A;
 #pragma unroll
         for (int r = 0; r < 16; ++r) S[r] = W[r] = A[r] = 0.f;
@@ -204,27 +213,28 @@ __device__ __forceinline__ float bound_units(const SelectCall &c, int b, int hkv
 #pragma unroll
             for (int i = 0; i < 4; i += 2) low = low3(low, x[k][i], x[k][i + 1]);
         const bool negative = __any(low != 0);   // a scale below zero, or NaN
-        // |z| + L |s| as fp16 numbers, off by 2^-11 of themselves
-#pragma unroll
-        for (int k = 0; k < KS; ++k) {
-            u32x4 p;
+        // A over |z| + L |s| as fp16 numbers, off by 2^-11 of themselves
+        auto sum = [&](int k, u32 mask) __attribute__((always_inline)) {
+            u32x4 p, size;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const u32 size = negative ? x[k][i] & 0x7FFF7FFFu : x[k][i];
-                y[k][i] = as_u(__builtin_elementwise_fma(as_h2(size), as_h2(levels2), as_h2(y[k][i])));
+                size[i] = as_u(__builtin_elementwise_fma(as_h2(x[k][i] & mask), as_h2(levels2), as_h2(y[k][i])));
                 p[i] = q[k][i] & 0x7FFF7FFFu;
             }
-            A = SpanMma<f16>::mma(p, y[k], A);
-        }
+            A = SpanMma<f16>::mma(p, size, A);
+        };
         if (!negative) {
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
+                sum(k, ~0u);
                 u32x4 p;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) p[i] = positive(q[k][i]);
                 W = SpanMma<f16>::mma(p, x[k], W);
             }
         } else {
+#pragma unroll
+            for (int k = 0; k < KS; ++k) sum(k, 0x7FFF7FFFu);
 #pragma unroll 1
             for (int m = 0; m < 2; ++m) {
                 const u32 flip = m ? 0x80008000u : 0u;
@@ -261,7 +271,7 @@ __device__ __forceinline__ float bound_units(const SelectCall &c, int b, int hkv
 }
 
 // Items of many rows, and few of many groups: a wave a run of units, scores and bounds to memory.
-template <int D, bool BF16> __global__ __launch_bounds__(256) void block_bound_kernel(SelectCall c) {
+template <int D, bool BF16> __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) void block_bound_kernel(SelectCall c) {
     extern __shared__ __align__(16) char rings[];
     const vq_block_select_args &a = c.a;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -624,7 +634,7 @@ template <bool STORED, int THREADS> __global__ __launch_bounds__(THREADS) void b
 
 // Scores and choice of a tile of up to 32 rows in one block, the scores in LDS.
 template <int D, bool BF16, int THREADS>
-__global__ __launch_bounds__(THREADS) void block_choose_kernel(SelectCall c) {
+__global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) void block_choose_kernel(SelectCall c) {
     constexpr int WAVES = THREADS / 64;
     extern __shared__ __align__(16) char rings[];   // of the waves, then the scores of the blocks and of the groups
     float *const keys = (float *)(rings + WAVES * BoundRing<D>::BYTES);
