@@ -135,6 +135,18 @@ def test_large_and_small_queries(dtype, big):
         _same(q, scale, zero, 9, levels=15, group_size=32, n_packed=2880, query_block=query_block)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+def test_a_large_channel_that_no_key_has(dtype):
+    """The other channels decide, 2^-32 (fp16: 2^-20) of the largest."""
+    require_gpu()
+    q, scale, zero = _inputs(2, 8, 2, 6, 128, 120, dtype=dtype, seed=15)
+    q *= 2.0 ** (-12 if dtype == F16 else -22)
+    q[..., 17] = 2.0 ** (8 if dtype == F16 else 10)
+    zero[..., :120, 17], scale[..., :120, 17] = 0, 0
+    for query_block in (1, 6):
+        _same(q, scale, zero, 11, levels=15, group_size=32, n_packed=3840, query_block=query_block)
+
+
 @pytest.mark.parametrize("bits,group", [(2, 32), (4, 64), (8, 32)])
 def test_scores_bound_the_products(bits, group):
     """What a store's own scales say of its keys, as far as a slot's rounding to fp16 goes; and a block that holds a key along the query

@@ -92,6 +92,10 @@ __device__ __forceinline__ u32 positive(u32 x) { return __builtin_bit_cast(u32, 
 __device__ __forceinline__ u32 max_bits(u32 x, u32 y) {   // of two magnitudes each
     return __builtin_bit_cast(u32, __builtin_elementwise_max(__builtin_bit_cast(u16x2, x), __builtin_bit_cast(u16x2, y)));
 }
+// of two magnitudes each, of the second its bits less one: zeros are the largest
+__device__ __forceinline__ u32 min_bits(u32 x, u32 y) {
+    return __builtin_bit_cast(u32, __builtin_elementwise_min(__builtin_bit_cast(u16x2, x), (u16x2)(__builtin_bit_cast(u16x2, y) - (u16x2){1, 1})));
+}
 // the smallest of three halves each, NaN where one is (none the result of a matrix product)
 __device__ __forceinline__ u32 low3(u32 x, u32 y, u32 z) {
     u32 r;
@@ -105,8 +109,8 @@ __device__ __forceinline__ u32 low3(u32 x, u32 y, u32 z) {
 //
 // products of fp16 numbers with v_mfma_f32_32x32x16 (the last one only where a scale is negative; lane n = lane % 32, h = lane / 32: row or group n,
 // channels 16 ks + 8 h ..).  A wave keeps its rows' queries, walks a run of units of 32 groups and writes each group's largest bound over its rows.
-// bf16 queries become fp16 numbers by a power of two that puts a row tile's largest near 2^15.  Float32 sums of D terms are off by less than
-// (D + 8) 2^-22 A, A = sum |q| (|z| + L |s|), which the wave forms too, by a third product: the choice knows how far to trust the scores (with A
+// bf16 queries become fp16 numbers by a power of two that puts a row tile's largest near 2^15.  A float32 sum of D terms, each cut to 24 bits of the
+// largest, is off by less than D 2^-23 of the magnitudes' sum: the scores by (D + 16) 2^-23 A, A = sum |q| (|z| + L |s|), which the wave forms too, by a third product: the choice knows how far to trust the scores (with A
 // bounded by the largest sum of |q| times the largest |z| + L |s| it asked 64 bits for 3 to 5 blocks a tile).  Bound by the bytes of the scales and zeros for one query a sequence.
 // Zeros and scales come asynchronously, in whole stretches of 1 KB, into the wave's ring, the next unit's ahead (as loads of a lane's own operands they touch a
 // cache line in four instructions: 16 sequences at 32k 27 us, this .. us); pieces of a row lie rotated by the row, so that the lanes that read them
@@ -220,6 +224,8 @@ __device__ __forceinline__ float bound_units(const SelectCall &c, int b, int hkv
             for (int i = 0; i < 4; ++i) {
                 size[i] = as_u(__builtin_elementwise_fma(as_h2(x[k][i] & mask), as_h2(levels2), as_h2(y[k][i])));
                 p[i] = q[k][i] & 0x7FFF7FFFu;
+                // (a bf16 query far below its tile's largest is cut to a multiple of 2^-24: as magnitudes of 2^-7 or more cover that too)
+                if (BF16) p[i] = max_bits(p[i], 0x20002000u);
             }
             A = SpanMma<f16>::mma(p, size, A);
         };
@@ -311,11 +317,12 @@ __device__ __forceinline__ uint64_t exact_key(const SelectCall &c, int b, int hk
     const int parts = 64 / many, part = lane % parts;
     const int64_t at = (((int64_t)b * a.Hkv + hkv) * c.stride + u) * D;
     const u16 *const zero = (const u16 *)a.k_zero + at, *const scale = (const u16 *)a.k_scale + at;
+    const bool bf16 = a.dtype == VQ_BF16;
     uint64_t best = 0;
     for (int r0 = 0; r0 < rows; r0 += many) {
         const int r = r0 + lane / parts, x = r < rows ? r : rows - 1, end = sel_end(a, live, pos0 + x / G);
         const u16 *q = (const u16 *)a.q + (((int64_t)b * a.Hq + hkv * G + x % G) * a.Sq + pos0 + x / G) * D;
-        double s = 0.;
+        double s = 0., w = 0.;
         for (int d0 = part * 8; d0 < D; d0 += AHEAD * parts * 8) {
             u32x4 x4[AHEAD], z4[AHEAD], s4[AHEAD];
 #pragma unroll
@@ -326,18 +333,44 @@ __device__ __forceinline__ uint64_t exact_key(const SelectCall &c, int b, int hk
                 z4[k] = *(const u32x4 *)(zero + d);
                 s4[k] = *(const u32x4 *)(scale + d);
             }
+            // Products are exact in float32 (22 bits), where no bf16 query lies outside 2^-63 .. 2^64
+            u32 top = 0, low = ~0u;   // of the magnitudes' bits, the lower end less one, so that zeros are not it
+            if (bf16) {
 #pragma unroll
-            for (int k = 0; k < AHEAD; ++k) {
-                if (k > 0 && d0 + k * parts * 8 >= D) break;
+                for (int k = 0; k < AHEAD; ++k)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const u16 xb = (u16)(x4[k][i / 2] >> (16 * (i & 1)));
-                    const double y = a.dtype == VQ_BF16 ? (double)bf16_to_f32(xb) : (double)(float)__builtin_bit_cast(f16, xb);
-                    const double z = (double)(float)as_h2(z4[k][i / 2])[i & 1], r1 = y * (double)(float)as_h2(s4[k][i / 2])[i & 1] * a.levels;
-                    s += y * z + (r1 > 0. || r1 != r1 ? r1 : 0.);
-                }
+                    for (int i = 0; i < 4; ++i) {
+                        const u32 size = x4[k][i] & 0x7FFF7FFFu;
+                        top = max_bits(top, size);
+                        low = min_bits(low, size);
+                    }
             }
+            const bool narrow = !bf16 || ((top >> 16) < 0x5F80u && (top & 0xFFFFu) < 0x5F80u && (low >> 16) >= 0x2000u && (low & 0xFFFFu) >= 0x2000u);
+            auto add = [&](auto product) __attribute__((always_inline)) {
+#pragma unroll
+                for (int k = 0; k < AHEAD; ++k) {
+                    if (k > 0 && d0 + k * parts * 8 >= D) break;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const u16 xb = (u16)(x4[k][i / 2] >> (16 * (i & 1)));
+                        product(bf16 ? bf16_to_f32(xb) : (float)__builtin_bit_cast(f16, xb), (float)as_h2(z4[k][i / 2])[i & 1], (float)as_h2(s4[k][i / 2])[i & 1]);
+                    }
+                }
+            };
+            if (__all(narrow))
+                add([&](float y, float z, float t) __attribute__((always_inline)) {
+                    const float p = y * t;
+                    s += (double)(y * z);
+                    w += (double)(p <= 0.f ? 0.f : p);
+                });
+            else
+                add([&](double y, double z, double t) __attribute__((always_inline)) {
+                    const double p = y * t;
+                    s += y * z;
+                    w += p <= 0. ? 0. : p;
+                });
         }
+        s += (double)a.levels * w;
         for (int off = 1; off < parts; off <<= 1) s = shfl_add(s, off);
         if (u * g < end) best = max_key(best, pick_key(s));
     }
@@ -608,7 +641,7 @@ template <int THREADS> __device__ __forceinline__ void pick_blocks(const SelectC
         most = fmaxf(most, x);
     }
 }
-__device__ __forceinline__ float pick_error(const SelectCall &c, float bound) { return bound < INFINITY ? bound * ((float)(c.a.D + 9) * 0x1p-22f) : INFINITY; }
+__device__ __forceinline__ float pick_error(const SelectCall &c, float bound) { return bound < INFINITY ? bound * ((float)(c.a.D + 16) * 0x1p-23f) : INFINITY; }
 
 template <bool STORED, int THREADS> __global__ __launch_bounds__(THREADS) void block_pick_kernel(SelectCall c) {
     extern __shared__ float keys[];
