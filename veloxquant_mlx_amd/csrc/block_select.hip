@@ -769,7 +769,9 @@ SelectCall cut_select(const vq_block_select_args &a) {
         c.runs = (int)cdiv(units, c.run_units);
         // (the products and the grid of a call of this size are left to the vector units)
         if ((double)c.items * c.row_tiles * (double)c.groups >= 67108864.) c.mma = 0;
-        c.one = c.mma && c.row_tiles == 1 && (c.total + c.groups) * 4 <= ONE_SCORES;
+        // One block a tile where its waves walk two units each at most, or tiles fill the chip: one sequence of 8 kv heads over 8k tokens in groups of
+        // 32 11.9 us, in two launches 13.1; over 16k 13.6 and 13.4, 32k 16.1 and 13.2; four sequences of 32k 17.5 and 16.1, eight 17.9 and 19.0.
+        c.one = c.mma && c.row_tiles == 1 && (c.total + c.groups) * 4 <= ONE_SCORES && (c.items >= 64 || units <= (a.D == 256 ? 8 : 16));
     }
     return c;
 }
