@@ -19,7 +19,8 @@ struct SelectCall {
     vq_block_select_args a;
     int64_t tiles, total;   // tiles of queries a sequence, blocks of the store
     int64_t items;          // B Hkv tiles
-    double *scores;         // [items][total], of 64 bits (or room for them)
+    uint64_t *exact;        // [items][total], room for the keys of scores of 64 bits (block_pick_kernel)
+    uint64_t *stored;       // [items][groups], those of every group where the filter does not take the call
     // the filter on the matrix units:
     int mma;                // 1: it takes the call
     int one;                // 1: in one launch, a block an item
@@ -55,33 +56,78 @@ __device__ __forceinline__ int sel_last(const vq_block_select_args &a, int tile)
     return (int)(last < a.Sq ? last : a.Sq) - 1;
 }
 
-// A wave a (tile, block): lanes along the channels.
-__global__ __launch_bounds__(256) void block_score_kernel(SelectCall c) {
+// Scores of 64 bits as whole numbers in their order.
+__device__ __forceinline__ uint64_t pick_key(double s) {   // ascending with the score, NaN above all
+    if (s != s) return ~UINT64_C(0);
+    const uint64_t u = (uint64_t)__double_as_longlong(s + 0.);
+    return u >> 63 ? ~u : u | (UINT64_C(1) << 63);
+}
+__device__ __forceinline__ uint64_t max_key(uint64_t x, uint64_t y) { return x > y ? x : y; }
+__device__ __forceinline__ double key_score(uint64_t k) { return __longlong_as_double((int64_t)(k >> 63 ? k & ~(UINT64_C(1) << 63) : ~k)); }   // (NaN for NaN's)
+
+// Float32 queries, scales or zeros, and head sizes that the matrix units do not take: every group's score in 64 bits, on the vector units.
+//
+// Four lanes a group, each with four channels of every sixteen, and RW rows at a time, whose queries lie in LDS as doubles; the products y z and y s of
+// a channel are formed in double, where they are exact: two conversions a channel and six instructions a row.  WIDE: four channels a load.
+constexpr int SCORE_GROUPS = 64;   // a block of threads
+template <typename T, bool WIDE, int RW> __global__ __launch_bounds__(256) void group_score_kernel(SelectCall c) {
+    extern __shared__ double qs[];   // [RW][D, up to whole sixteens]
     const vq_block_select_args &a = c.a;
-    const int lane = threadIdx.x & 63;
-    const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (id >= a.B * a.Hkv * c.tiles * c.total) return;
-    const int64_t j = id % c.total, tile = id / c.total % c.tiles, bh = id / (c.total * c.tiles), hkv = bh % a.Hkv, b = bh / a.Hkv;
-    const int64_t G = a.Hq / a.Hkv, i1 = sel_last(a, (int)tile), groups = (a.cap_tokens + a.group - 1) / a.group;
-    const int live = sel_live(a, (int)b);
-    double best = -INFINITY;
-    for (int64_t t = j * a.block_tokens; t < (j + 1) * a.block_tokens; t += a.group)
-        for (int64_t i = tile * a.query_block; i <= i1; ++i) {
-            if (t >= sel_end(a, live, (int)i)) continue;
-            for (int64_t g = 0; g < G; ++g) {
-                double s = 0.;
-                for (int64_t d = lane; d < a.D; d += 64) {
-                    const int64_t at = (bh * groups + t / a.group) * a.D + d;
-                    const double q = sel_ld(a.q, a.dtype, ((b * a.Hq + hkv * G + g) * a.Sq + i) * a.D + d);
-                    const double z = sel_ld(a.k_zero, a.meta_dtype, at), r = q * (double)sel_ld(a.k_scale, a.meta_dtype, at) * a.levels;
-                    s += q * z + (r > 0. ? r : r != r ? r : 0.);
-                }
+    const int tid = threadIdx.x, part = tid & 3;
+    const u32 many = (u32)((c.groups + SCORE_GROUPS - 1) / SCORE_GROUPS), item = blockIdx.x / many, bh = item / (u32)c.tiles;
+    const int u0 = (int)(blockIdx.x % many) * SCORE_GROUPS, tile = (int)(item % (u32)c.tiles), hkv = (int)(bh % (u32)a.Hkv), b = (int)(bh / (u32)a.Hkv);
+    const int live = sel_live(a, b), G = (int)a.Hq / (int)a.Hkv, D = (int)a.D, room = (D + 15) / 16 * 16, g = a.group, pos0 = tile * (int)c.query_block,
+              last = sel_last(a, tile), groups = (sel_end(a, live, last) + g - 1) / g;   // that some row sees
+    if (u0 >= groups) return;
+    const int rows = (last - pos0 + 1) * G, u = u0 + (tid >> 2);
+    const int64_t at = ((int64_t)bh * c.stride + (u < groups ? u : groups - 1)) * D;   // (past the last group: it again)
+    const T *const zero = (const T *)a.k_zero + at, *const scale = (const T *)a.k_scale + at;
+    struct alignas(4 * sizeof(T)) Four { T v[4]; };
+    uint64_t best = 0;   // (no score's key)
+    for (int r0 = 0; r0 < rows; r0 += RW) {
+        __syncthreads();
+        for (int i = tid; i < RW * room; i += 256) {
+            const int row = i / room, d = i - row * room, x = r0 + row < rows ? r0 + row : rows - 1;
+            qs[i] = d < D ? sel_ld(a.q, a.dtype, (((int64_t)b * a.Hq + hkv * G + x % G) * a.Sq + pos0 + x / G) * D + d) : 0.f;
+        }
+        __syncthreads();
+        double sum[RW], pos[RW];
 #pragma unroll
-                for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off);
-                best = s > best || s != s ? s : best;
+        for (int r = 0; r < RW; ++r) sum[r] = pos[r] = 0.;
+#pragma unroll 4
+        for (int d = part * 4; d < D; d += 16) {
+            Four z, t;
+            if constexpr (WIDE) {
+                z = *(const Four *)(zero + d);
+                t = *(const Four *)(scale + d);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    z.v[e] = d + e < D ? zero[d + e] : (T)0.f;
+                    t.v[e] = d + e < D ? scale[d + e] : (T)0.f;
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const double zd = (double)(float)z.v[e], td = (double)(float)t.v[e];
+#pragma unroll
+                for (int r = 0; r < RW; ++r) {
+                    const double y = qs[r * room + d + e], p = y * td;
+                    sum[r] = __builtin_fma(y, zd, sum[r]);
+                    pos[r] += p <= 0. ? 0. : p;
+                }
             }
         }
-    if (lane == 0) c.scores[id] = best;
+#pragma unroll
+        for (int r = 0; r < RW; ++r) {
+            double x = __builtin_fma((double)a.levels, pos[r], sum[r]);
+            x += __shfl_xor(x, 1);
+            x += __shfl_xor(x, 2);
+            const int row = r0 + r;
+            if (row < rows && u * g < sel_end(a, live, pos0 + row / G)) best = max_key(best, pick_key(x));
+        }
+    }
+    if (part == 0 && u < groups) c.stored[(int64_t)item * c.groups + u] = best;
 }
 
 // ---- the matrix units as a filter
@@ -297,12 +343,6 @@ template <int D, bool BF16> __global__ __launch_bounds__(256) __attribute__((amd
 
 // ---- the choice
 
-__device__ __forceinline__ uint64_t pick_key(double s) {   // ascending with the score, NaN above all
-    if (s != s) return ~UINT64_C(0);
-    const uint64_t u = (uint64_t)__double_as_longlong(s + 0.);
-    return u >> 63 ? ~u : u | (UINT64_C(1) << 63);
-}
-__device__ __forceinline__ uint64_t max_key(uint64_t x, uint64_t y) { return x > y ? x : y; }
 __device__ __forceinline__ double shfl_add(double s, int off) { return s + __shfl_xor(s, off); }
 
 // The key of group u's score in 64 bits, the largest over the tile's rows, by a wave: 64 / R lanes a row (R the rows, up to the next power of two),
@@ -430,6 +470,37 @@ template <int WAVES> __device__ __forceinline__ int pick_bin(const u32 *hist, u3
     return (int)found[0];
 }
 
+// A tile's place, what it sees, and the choices that need no score: all of at most `count` visible blocks, and else the first and the recent ones.
+// False: nothing is left to choose.
+struct PickTile {
+    int b, hkv, tile, live, lo, n;   // (blocks lo .. lo + n - 1 to choose from)
+    int per, seen;                   // groups of a block, groups that some row sees
+    u32 want;
+};
+__device__ __forceinline__ bool pick_begin(const SelectCall &c, PickTile &t) {
+    const vq_block_select_args &a = c.a;
+    const u32 bh = blockIdx.x / (u32)c.tiles;
+    t.tile = (int)(blockIdx.x % (u32)c.tiles);
+    t.hkv = (int)(bh % (u32)a.Hkv);
+    t.b = (int)(bh / (u32)a.Hkv);
+    t.live = sel_live(a, t.b);
+    const int end = sel_end(a, t.live, sel_last(a, t.tile));
+    t.per = (int)a.block_tokens / a.group;
+    t.seen = (end + a.group - 1) / a.group;
+    const int V = (int)((u32)(end + (int)a.block_tokens - 1) / (u32)a.block_tokens), count = (int)a.count;
+    int32_t *out = a.out + (int64_t)blockIdx.x * count;
+    if (V <= count) {
+        for (int i = threadIdx.x; i < count; i += blockDim.x) out[i] = i < V ? i : -1;
+        return false;
+    }
+    t.lo = (int)a.first;
+    t.n = V - (int)a.recent - t.lo;
+    t.want = (u32)(count - (int)a.first - (int)a.recent);   // of n, which are more
+    for (int i = threadIdx.x; i < t.lo; i += blockDim.x) out[i] = i;
+    for (int i = threadIdx.x; i < (int)a.recent; i += blockDim.x) out[count - (int)a.recent + i] = t.lo + t.n + i;
+    return t.want > 0;
+}
+
 // The choice of a tile, by a block of threads.  keys: the approximate scores of the blocks [lo, hi) from this thread's blocks on, in LDS; `least`, `most`, `e`: of this
 // thread's, the last one how far a score may be off, infinite where something is not finite.
 //
@@ -439,21 +510,20 @@ template <int WAVES> __device__ __forceinline__ int pick_bin(const u32 *hist, u3
 // PICK_LIST (equal scores, values that are not finite, which make e so) they are by a radix select over the bits.
 // STORED: the scores of 64 bits lie in memory; else they are formed here.
 template <bool STORED, int THREADS>
-__device__ __forceinline__ void pick(const SelectCall &c, PickRoom<THREADS> &room, float *keys, int b, int hkv, int tile, int live, int lo, int n, u32 want, float least, float most,
-                                     float e) {
+__device__ __forceinline__ void pick(const SelectCall &c, PickRoom<THREADS> &room, float *keys, const PickTile &t, float least, float most, float e) {
     constexpr int WAVES = THREADS / 64;
     const vq_block_select_args &a = c.a;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int32_t *out = a.out + (int64_t)blockIdx.x * a.count;
-    uint64_t *const score = (uint64_t *)c.scores + (int64_t)blockIdx.x * c.total;   // 64 bits a block
-    const int per = (int)a.block_tokens / a.group;   // groups of a block
-    // the key of a group of block j (group i of it), by a wave; 0 behind the last one
+    uint64_t *const score = c.exact + (int64_t)blockIdx.x * c.total;
+    const int b = t.b, hkv = t.hkv, tile = t.tile, live = t.live, lo = t.lo, n = t.n, per = t.per, seen = t.seen;
+    const u32 want = t.want;
+    // the key of group i of block j, by a wave; 0 behind the last group that some row sees
     auto key_of = [&](int j, int i) __attribute__((always_inline)) -> uint64_t {
-        if (STORED) return pick_key(__longlong_as_double((int64_t)score[lo + j]));
         const int u = (lo + j) * per + i;
-        return u < (int)c.groups ? exact_key(c, b, hkv, tile, live, u) : 0;
+        if (u >= seen) return 0;
+        return STORED ? c.stored[(int64_t)blockIdx.x * c.groups + u] : exact_key(c, b, hkv, tile, live, u);
     };
-    const int parts = STORED ? 1 : per;
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) {
         least = fminf(least, __shfl_xor(least, off));
@@ -528,9 +598,9 @@ __device__ __forceinline__ void pick(const SelectCall &c, PickRoom<THREADS> &roo
         if (wave == 0 && maybe) { room.list[64 + mine] = j; room.exact[mine] = 0; }
         __syncthreads();   // (every wave has read the list's scores, which the first one replaces)
         if (!all) {
-            for (u32 i = wave; i < doubt * parts; i += WAVES) {
-                const uint64_t k = key_of(room.list[64 + i / parts], i % parts);
-                if (lane == 0) atomicMax((unsigned long long *)&room.exact[i / parts], (unsigned long long)k);
+            for (u32 i = wave; i < doubt * per; i += WAVES) {
+                const uint64_t k = key_of(room.list[64 + i / per], i % per);
+                if (lane == 0) atomicMax((unsigned long long *)&room.exact[i / per], (unsigned long long)k);
             }
             __syncthreads();
         }
@@ -547,9 +617,9 @@ __device__ __forceinline__ void pick(const SelectCall &c, PickRoom<THREADS> &roo
     } else if (listed <= PICK_LIST) {
         for (u32 i = tid; i < listed; i += THREADS) room.exact[i] = 0;
         __syncthreads();
-        for (u32 i = wave; i < listed * parts; i += WAVES) {
-            const uint64_t k = key_of(room.list[i / parts], i % parts);
-            if (lane == 0) atomicMax((unsigned long long *)&room.exact[i / parts], (unsigned long long)k);
+        for (u32 i = wave; i < listed * per; i += WAVES) {
+            const uint64_t k = key_of(room.list[i / per], i % per);
+            if (lane == 0) atomicMax((unsigned long long *)&room.exact[i / per], (unsigned long long)k);
         }
         __syncthreads();
         for (u32 i = tid; i < listed; i += THREADS) {
@@ -564,7 +634,7 @@ __device__ __forceinline__ void pick(const SelectCall &c, PickRoom<THREADS> &roo
             const float x = keys[j];
             uint64_t k = x > over ? ~UINT64_C(0) : 0;
             if (!(x > over) && !(x < under))
-                for (int i = 0; i < parts; ++i) k = max_key(k, key_of(j, i));
+                for (int i = 0; i < per; ++i) k = max_key(k, key_of(j, i));
             if (lane == 0) score[lo + j] = k;
         }
         __threadfence_block();
@@ -602,36 +672,10 @@ __device__ __forceinline__ void pick(const SelectCall &c, PickRoom<THREADS> &roo
     }
 }
 
-// A tile's place, what it sees, and the choices that need no score: all of at most `count` visible blocks, and else the first and the recent ones.
-// False: nothing is left to choose.
-struct PickTile { int b, hkv, tile, live, end, lo, n; u32 want; };
-__device__ __forceinline__ bool pick_begin(const SelectCall &c, PickTile &t) {
-    const vq_block_select_args &a = c.a;
-    const u32 bh = blockIdx.x / (u32)c.tiles;
-    t.tile = (int)(blockIdx.x % (u32)c.tiles);
-    t.hkv = (int)(bh % (u32)a.Hkv);
-    t.b = (int)(bh / (u32)a.Hkv);
-    t.live = sel_live(a, t.b);
-    t.end = sel_end(a, t.live, sel_last(a, t.tile));
-    const int V = (int)((u32)(t.end + (int)a.block_tokens - 1) / (u32)a.block_tokens), count = (int)a.count;
-    int32_t *out = a.out + (int64_t)blockIdx.x * count;
-    if (V <= count) {
-        for (int i = threadIdx.x; i < count; i += blockDim.x) out[i] = i < V ? i : -1;
-        return false;
-    }
-    t.lo = (int)a.first;
-    t.n = V - (int)a.recent - t.lo;
-    t.want = (u32)(count - (int)a.first - (int)a.recent);   // of n, which are more
-    for (int i = threadIdx.x; i < t.lo; i += blockDim.x) out[i] = i;
-    for (int i = threadIdx.x; i < (int)a.recent; i += blockDim.x) out[count - (int)a.recent + i] = t.lo + t.n + i;
-    return t.want > 0;
-}
-
 // A thread's blocks' approximate scores from those of their groups (row tile rt's at approx + rt * groups).
 template <int THREADS> __device__ __forceinline__ void pick_blocks(const SelectCall &c, const PickTile &t, const float *approx, int row_tiles, int groups, float *keys, float &least, float &most, float &e) {
-    const int per = (int)c.a.block_tokens / c.a.group, seen = (t.end + c.a.group - 1) / c.a.group;   // groups of a block, groups that some row sees
     for (int j = threadIdx.x; j < t.n; j += THREADS) {
-        const int u0 = (t.lo + j) * per, u1 = u0 + per < seen ? u0 + per : seen;
+        const int u0 = (t.lo + j) * t.per, u1 = u0 + t.per < t.seen ? u0 + t.per : t.seen;
         float x = -INFINITY;
         for (int rt = 0; rt < row_tiles; ++rt)
             for (int u = u0; u < u1; ++u) x = fmaxf(x, approx[(int64_t)rt * groups + u]);
@@ -650,8 +694,11 @@ template <bool STORED, int THREADS> __global__ __launch_bounds__(THREADS) void b
     if (!pick_begin(c, t)) return;
     float least = INFINITY, most = -INFINITY, e = 0.f;
     if (STORED) {
+        const uint64_t *stored = c.stored + (int64_t)blockIdx.x * c.groups;
         for (int j = threadIdx.x; j < t.n; j += THREADS) {
-            const float x = (float)c.scores[blockIdx.x * c.total + t.lo + j];
+            uint64_t k = 0;
+            for (int u = (t.lo + j) * t.per; u < (t.lo + j + 1) * t.per && u < t.seen; ++u) k = max_key(k, stored[u]);
+            const float x = (float)key_score(k);
             keys[j] = x;
             e = __builtin_fabsf(x) < INFINITY ? fmaxf(e, __builtin_fabsf(x) * 0x1p-23f) : INFINITY;
             least = fminf(least, x);
@@ -662,7 +709,7 @@ template <bool STORED, int THREADS> __global__ __launch_bounds__(THREADS) void b
         for (int i = threadIdx.x; i < many; i += THREADS) e = fmaxf(e, pick_error(c, c.bounds[(int64_t)blockIdx.x * many + i]));
         pick_blocks<THREADS>(c, t, c.approx + (int64_t)blockIdx.x * c.row_tiles * c.groups, c.row_tiles, (int)c.groups, keys, least, most, e);
     }
-    pick<STORED, THREADS>(c, room, keys, t.b, t.hkv, t.tile, t.live, t.lo, t.n, t.want, least, most, e);
+    pick<STORED, THREADS>(c, room, keys, t, least, most, e);
 }
 
 // Scores and choice of a tile of up to 32 rows in one block, the scores in LDS.
@@ -674,15 +721,15 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(D == 25
     __shared__ PickRoom<THREADS> room;
     PickTile t;
     if (!pick_begin(c, t)) return;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), per = (int)c.a.block_tokens / c.a.group, seen = (t.end + c.a.group - 1) / c.a.group;
-    const int u0 = t.lo * per, u1 = (t.lo + t.n) * per < seen ? (t.lo + t.n) * per : seen;   // the groups of those to choose from
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), u0 = t.lo * t.per,
+              u1 = (t.lo + t.n) * t.per < t.seen ? (t.lo + t.n) * t.per : t.seen;   // the groups of those to choose from
     float *const approx = keys + c.total;
     float least = INFINITY, most = -INFINITY, e = 0.f;
     if (u0 + wave * 32 < u1) e = pick_error(c, bound_units<D, BF16>(c, t.b, t.hkv, t.tile, 0, t.live, u0 + wave * 32, u1, WAVES * 32, approx,
                                                                        rings + wave * BoundRing<D>::BYTES));
     __syncthreads();
     pick_blocks<THREADS>(c, t, approx, 1, 0, keys, least, most, e);
-    pick<false, THREADS>(c, room, keys, t.b, t.hkv, t.tile, t.live, t.lo, t.n, t.want, least, most, e);
+    pick<false, THREADS>(c, room, keys, t, least, most, e);
 }
 
 // The same over any number of blocks, their scores of 64 bits in memory throughout.
@@ -692,7 +739,12 @@ __global__ __launch_bounds__(256) void block_pick_any_kernel(SelectCall c) {
     PickTile t;
     if (!pick_begin(c, t)) return;
     const int tid = threadIdx.x;
-    const double *score = c.scores + blockIdx.x * c.total + t.lo;
+    const uint64_t *stored = c.stored + (int64_t)blockIdx.x * c.groups;
+    auto key_of = [&](int j) __attribute__((always_inline)) {
+        uint64_t k = 0;
+        for (int u = (t.lo + j) * t.per; u < (t.lo + j + 1) * t.per && u < t.seen; ++u) k = max_key(k, stored[u]);
+        return k;
+    };
     int32_t *out = c.a.out + (int64_t)blockIdx.x * c.a.count + t.lo;
     u32 left = t.want;
     uint64_t key = 0;
@@ -700,7 +752,7 @@ __global__ __launch_bounds__(256) void block_pick_any_kernel(SelectCall c) {
         hist[tid] = 0;
         __syncthreads();
         for (int j = tid; j < t.n; j += THREADS) {
-            const uint64_t k = pick_key(score[j]);
+            const uint64_t k = key_of(j);
             if (shift == 56 || (k ^ key) >> (shift + 8) == 0) atomicAdd(&hist[k >> shift & 255], 1u);
         }
         __syncthreads();
@@ -710,7 +762,7 @@ __global__ __launch_bounds__(256) void block_pick_any_kernel(SelectCall c) {
     u32 done = 0, equal = 0;
     for (int j0 = 0; j0 < t.n; j0 += THREADS) {
         const int j = j0 + tid;
-        const uint64_t k = j < t.n ? pick_key(score[j]) : 0;
+        const uint64_t k = j < t.n ? key_of(j) : 0;
         u32 some;
         const u32 rank = equal + block_before<WAVES>(j < t.n && k == key, false, some, waves);
         equal += some;
@@ -742,7 +794,7 @@ int check_select(const char *fn, const vq_block_select_args *args) {
                (long long)a.Sq, (long long)(a.n_packed + a.n_tail));
     const double tiles = (double)cdiv(a.Sq, a.query_block), rows = (double)a.B * (double)a.Hkv * tiles;
     VQ_REQUIRE((double)a.B * (double)a.Hq * (double)a.Sq < 16777216., VQ_ERR_UNSUPPORTED, "%s: 2^24 or more query rows", fn);
-    VQ_REQUIRE(rows * (double)cdiv(a.n_packed, a.block_tokens) < 67108864., VQ_ERR_UNSUPPORTED, "%s: 2^26 or more scores", fn);
+    VQ_REQUIRE(rows * (double)cdiv(a.n_packed, a.group) < 67108864. && rows < 8388608., VQ_ERR_UNSUPPORTED, "%s: 2^26 or more scores", fn);
     VQ_REQUIRE(a.q != nullptr && a.out != nullptr && (a.n_packed == 0 || (a.k_scale != nullptr && a.k_zero != nullptr)), VQ_ERR_INVALID,
                "%s: null q, out, scale or zero", fn);
     return VQ_OK;
@@ -775,12 +827,13 @@ SelectCall cut_select(const vq_block_select_args &a) {
     }
     return c;
 }
-struct SelectRoom { size_t scores, approx, bounds, all; };
+struct SelectRoom { size_t stored, approx, bounds, all; };
 SelectRoom select_room(const SelectCall &c) {
     SelectRoom r = {};
     if (c.total <= c.a.count) return r;
     auto whole = [](size_t n) { return (n + 15) / 16 * 16; };
-    r.approx = whole((size_t)(c.items * c.total) * 8);
+    r.stored = whole((size_t)(c.items * c.total) * 8);
+    r.approx = r.stored + (c.mma ? 0 : whole((size_t)(c.items * c.groups) * 8));
     r.bounds = r.all = r.approx;
     if (c.mma && !c.one) {
         r.bounds = r.approx + whole((size_t)(c.items * c.row_tiles * c.groups) * 4);
@@ -825,6 +878,17 @@ template <int D, bool BF16> int launch_choice(const char *fn, const SelectCall &
     if (int rc = launch_of(fn, block_bound_kernel<D, BF16>, cdiv(c.items * c.row_tiles * c.runs, 4), 256, rings, rings, allowed, c)) return rc;
     return launch_pick<false>(fn, c, (size_t)c.total * 4);
 }
+template <typename T, bool WIDE, int RW> void launch_scores_of(const SelectCall &c) {
+    group_score_kernel<T, WIDE, RW><<<(unsigned)(c.items * cdiv(c.groups, SCORE_GROUPS)), 256, (size_t)RW * cdiv(c.a.D, 16) * 16 * 8, (hipStream_t)c.a.stream>>>(c);
+}
+template <typename T, bool WIDE> void launch_scores(const SelectCall &c) {
+    const int64_t rows = c.a.Hq / c.a.Hkv * c.query_block;
+    if (rows == 1) launch_scores_of<T, WIDE, 1>(c);
+    else if (rows == 2) launch_scores_of<T, WIDE, 2>(c);
+    else if (rows <= 4) launch_scores_of<T, WIDE, 4>(c);
+    else launch_scores_of<T, WIDE, 8>(c);
+}
+
 template <int D> int launch_choice(const char *fn, const SelectCall &c) { return c.a.dtype == VQ_BF16 ? launch_choice<D, true>(fn, c) : launch_choice<D, false>(fn, c); }
 
 }  // namespace
@@ -848,11 +912,14 @@ extern "C" int vq_block_select(const vq_block_select_args *args) {
                "%s: workspace of %zu bytes required, 16-byte aligned", fn, room.all);
     hipStream_t st = (hipStream_t)a.stream;
     if (room.all > 0) {
-        c.scores = (double *)a.workspace;
+        c.exact = (uint64_t *)a.workspace;
+        c.stored = (uint64_t *)((char *)a.workspace + room.stored);
         c.approx = (float *)((char *)a.workspace + room.approx);
         c.bounds = (float *)((char *)a.workspace + room.bounds);
         if (c.mma) return a.D == 64 ? launch_choice<64>(fn, c) : a.D == 128 ? launch_choice<128>(fn, c) : launch_choice<256>(fn, c);
-        block_score_kernel<<<(unsigned)cdiv(c.items * c.total, 4), 256, 0, st>>>(c);
+        const bool wide = a.D % 4 == 0 && (((uintptr_t)a.k_scale | (uintptr_t)a.k_zero) & 15) == 0;
+        if (a.meta_dtype == VQ_F32) wide ? launch_scores<float, true>(c) : launch_scores<float, false>(c);
+        else wide ? launch_scores<f16, true>(c) : launch_scores<f16, false>(c);
         VQ_HIP_CHECK_LAUNCH(fn);
         if (c.total > PICK_MOST) {
             block_pick_any_kernel<<<(unsigned)c.items, 256, 0, st>>>(c);
