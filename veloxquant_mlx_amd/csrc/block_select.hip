@@ -67,19 +67,19 @@ __device__ __forceinline__ double key_score(uint64_t k) { return __longlong_as_d
 
 // Float32 queries, scales or zeros, and head sizes that the matrix units do not take: every group's score in 64 bits, on the vector units.
 //
-// Four lanes a group, each with four channels of every sixteen, and RW rows at a time, whose queries lie in LDS as doubles; the products y z and y s of
+// Eight lanes a group, each with four channels of every 32, and RW rows at a time, whose queries lie in LDS as doubles; the products y z and y s of
 // a channel are formed in double, where they are exact: two conversions a channel and six instructions a row.  WIDE: four channels a load.
-constexpr int SCORE_GROUPS = 64;   // a block of threads
+constexpr int SCORE_GROUPS = 32;   // a block of threads
 template <typename T, bool WIDE, int RW> __global__ __launch_bounds__(256) void group_score_kernel(SelectCall c) {
-    extern __shared__ double qs[];   // [RW][D, up to whole sixteens]
+    extern __shared__ double qs[];   // [RW][D, up to whole 32s]
     const vq_block_select_args &a = c.a;
-    const int tid = threadIdx.x, part = tid & 3;
+    const int tid = threadIdx.x, part = tid & 7;
     const u32 many = (u32)((c.groups + SCORE_GROUPS - 1) / SCORE_GROUPS), item = blockIdx.x / many, bh = item / (u32)c.tiles;
     const int u0 = (int)(blockIdx.x % many) * SCORE_GROUPS, tile = (int)(item % (u32)c.tiles), hkv = (int)(bh % (u32)a.Hkv), b = (int)(bh / (u32)a.Hkv);
-    const int live = sel_live(a, b), G = (int)a.Hq / (int)a.Hkv, D = (int)a.D, room = (D + 15) / 16 * 16, g = a.group, pos0 = tile * (int)c.query_block,
+    const int live = sel_live(a, b), G = (int)a.Hq / (int)a.Hkv, D = (int)a.D, room = (D + 31) / 32 * 32, g = a.group, pos0 = tile * (int)c.query_block,
               last = sel_last(a, tile), groups = (sel_end(a, live, last) + g - 1) / g;   // that some row sees
     if (u0 >= groups) return;
-    const int rows = (last - pos0 + 1) * G, u = u0 + (tid >> 2);
+    const int rows = (last - pos0 + 1) * G, u = u0 + (tid >> 3);
     const int64_t at = ((int64_t)bh * c.stride + (u < groups ? u : groups - 1)) * D;   // (past the last group: it again)
     const T *const zero = (const T *)a.k_zero + at, *const scale = (const T *)a.k_scale + at;
     struct alignas(4 * sizeof(T)) Four { T v[4]; };
@@ -95,7 +95,7 @@ template <typename T, bool WIDE, int RW> __global__ __launch_bounds__(256) void 
 #pragma unroll
         for (int r = 0; r < RW; ++r) sum[r] = pos[r] = 0.;
 #pragma unroll 4
-        for (int d = part * 4; d < D; d += 16) {
+        for (int d = part * 4; d < D; d += 32) {
             Four z, t;
             if constexpr (WIDE) {
                 z = *(const Four *)(zero + d);
@@ -123,6 +123,7 @@ template <typename T, bool WIDE, int RW> __global__ __launch_bounds__(256) void 
             double x = __builtin_fma((double)a.levels, pos[r], sum[r]);
             x += __shfl_xor(x, 1);
             x += __shfl_xor(x, 2);
+            x += __shfl_xor(x, 4);
             const int row = r0 + r;
             if (row < rows && u * g < sel_end(a, live, pos0 + row / G)) best = max_key(best, pick_key(x));
         }
@@ -879,7 +880,7 @@ template <int D, bool BF16> int launch_choice(const char *fn, const SelectCall &
     return launch_pick<false>(fn, c, (size_t)c.total * 4);
 }
 template <typename T, bool WIDE, int RW> void launch_scores_of(const SelectCall &c) {
-    group_score_kernel<T, WIDE, RW><<<(unsigned)(c.items * cdiv(c.groups, SCORE_GROUPS)), 256, (size_t)RW * cdiv(c.a.D, 16) * 16 * 8, (hipStream_t)c.a.stream>>>(c);
+    group_score_kernel<T, WIDE, RW><<<(unsigned)(c.items * cdiv(c.groups, SCORE_GROUPS)), 256, (size_t)RW * cdiv(c.a.D, 32) * 32 * 8, (hipStream_t)c.a.stream>>>(c);
 }
 template <typename T, bool WIDE> void launch_scores(const SelectCall &c) {
     const int64_t rows = c.a.Hq / c.a.Hkv * c.query_block;
