@@ -633,6 +633,11 @@ typedef struct vq_block_attend_args {
     vq_store_attend_args store;
     const int32_t *blocks;
     int64_t count, block_tokens, query_block;
+    /* Optional: counters_len device integers, zero when the call is enqueued and left zero by it, its own while it runs (calls on one
+     * stream may share them, a captured graph may not with anything else): with B * Hkv * tiles * ceil(Hq / Hkv * query_block / 32) or more of them a call
+     * that is cut in parts adds these up in the same launch. */
+    int32_t *counters;
+    int64_t counters_len;
 } vq_block_attend_args;
 size_t vq_block_attend_workspace(const vq_block_attend_args *a);
 int vq_block_attend(const vq_block_attend_args *a);

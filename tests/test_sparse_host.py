@@ -35,8 +35,8 @@ def test_packed_blocks_are_the_structures():
     head = bytes(_lib.ROTARY_PACK.size)
     a = _lib.NormRotaryArgs.from_buffer_copy(head + _lib.NORM_PACK.pack(1, 2, 3, 4, 5, 0.5))
     assert list(a.weight) == [1, 2] and list(a.weight_stride) == [3, 4] and a.weight_dtype == 5 and a.eps == 0.5
-    b = _lib.BlockAttendArgs.from_buffer_copy(bytes(_lib.STORE_ATTEND_PACK.size) + _lib.BLOCK_LISTS_PACK.pack(1, 2, 3, 4))
-    assert (b.blocks, b.count, b.block_tokens, b.query_block) == (1, 2, 3, 4)
+    b = _lib.BlockAttendArgs.from_buffer_copy(bytes(_lib.STORE_ATTEND_PACK.size) + _lib.BLOCK_LISTS_PACK.pack(1, 2, 3, 4, 5, 6))
+    assert (b.blocks, b.count, b.block_tokens, b.query_block, b.counters, b.counters_len) == (1, 2, 3, 4, 5, 6)
 
 
 def _norm(**kw):

@@ -173,7 +173,8 @@ class BlockSelectArgs(C.Structure):
 class BlockAttendArgs(C.Structure):
     """Mirror of ``vq_block_attend_args``."""
 
-    _fields_ = [("store", StoreAttendArgs), ("blocks", vp), ("count", i64), ("block_tokens", i64), ("query_block", i64)]
+    _fields_ = [("store", StoreAttendArgs), ("blocks", vp), ("count", i64), ("block_tokens", i64), ("query_block", i64), ("counters", vp),
+                ("counters_len", i64)]
 
 
 # Argument blocks packed by ``struct`` in one go, as ATTEND_PACK: x, out, heads, x_strides, out_strides, ...
@@ -186,7 +187,7 @@ NORM_PACK = struct.Struct("@PPqqif")   # behind a ROTARY_PACK
 assert ROTARY_PACK.size + NORM_PACK.size == C.sizeof(NormRotaryArgs)
 BLOCK_SELECT_PACK = struct.Struct("@PPPPqqqqqqqqqqqqqPPNPiiiii0q")
 assert BLOCK_SELECT_PACK.size == C.sizeof(BlockSelectArgs)
-BLOCK_LISTS_PACK = struct.Struct("@Pqqq")   # behind a STORE_ATTEND_PACK
+BLOCK_LISTS_PACK = struct.Struct("@PqqqPq")   # behind a STORE_ATTEND_PACK
 assert STORE_ATTEND_PACK.size + BLOCK_LISTS_PACK.size == C.sizeof(BlockAttendArgs)
 
 

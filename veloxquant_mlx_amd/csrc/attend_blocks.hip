@@ -90,7 +90,7 @@ int check_blocks(const char *fn, const vq_block_attend_args *args) {
 
 // The matrix-unit kernel takes what it takes of attention over spans, where blocks are whole units of 32 slots: tiles of 32 rows of a kv head's
 // query heads at the positions of one list, each over the list's units, in as many runs as fill the chip.
-bool plan_few(BlockCall &c) {
+bool plan_few(BlockCall &c, const vq_block_attend_args &args) {
     const vq_store_attend_args &a = c.s.a;
     if (a.own.n_packed == 0 || c.block_tokens % 32 != 0 || !span_mfma_supported(a)) return false;
     const int64_t all = cdiv(a.own.n_packed, 32), sub = c.block_tokens / 32 < all ? c.block_tokens / 32 : all;
@@ -108,7 +108,7 @@ bool plan_few(BlockCall &c) {
     c.s.owaves = 4;
     c.s.osplits = c.s.nparts = (int)splits;
     c.lists = {c.blocks, (int)c.tiles, (int)c.count, (int)c.block_tokens, (int)qb, (int)cdiv(a.own.n_packed, c.block_tokens), (int)sub, (int)(c.count * sub),
-               (int)units, (int)row_tiles};
+               (int)units, (int)row_tiles, splits > 1 && items <= args.counters_len ? args.counters : nullptr};
     c.few = 1;
     return true;
 }
@@ -123,7 +123,7 @@ BlockCall cut_blocks(const vq_block_attend_args &args) {
     const vq_store_attend_args &a = c.s.a;
     c.tiles = cdiv(a.Sq, c.query_block);
     if (a.own.n_packed == 0) { c.s.a.pack_bits = 8; c.s.a.group = 1; c.count = 0; }   // fields that no packed slot reads
-    if (plan_few(c)) return c;
+    if (plan_few(c, args)) return c;
     // as many waves as fill the chip eight deep, runs of 64 slots or more
     const int64_t rows = a.B * a.Hq * a.Sq;
     double slots = (double)c.count * (double)c.block_tokens;
@@ -174,7 +174,7 @@ extern "C" int vq_block_attend(const vq_block_attend_args *args) {
     }
     if (c.few) {
         if (int rc = a.pack_bits == 4 ? launch_blocks_few4(c.s, c.lists) : launch_blocks_few2(c.s, c.lists)) return rc;
-        return need > 0 ? launch_span_merge1(fn, c.s) : VQ_OK;
+        return need > 0 && c.lists.counters == nullptr ? launch_span_merge1(fn, c.s) : VQ_OK;
     }
     blocks_any_kernel<<<(unsigned)cdiv(a.B * a.Hq * a.Sq * c.s.nparts, 4), 256, 0, (hipStream_t)a.stream>>>(c);
     VQ_HIP_CHECK_LAUNCH(fn);

@@ -35,6 +35,7 @@ struct BlockLists {
     int total;                      // blocks of the store
     int sub, packed_units, units;   // units of an entry, of a list, and with the tail
     int row_tiles;                  // tiles of rows of a tile of queries
+    int32_t *counters;              // zeros, one a tile of rows: the last block of a tile adds up its parts; NULL: another launch does
 };
 constexpr int BLOCK_UNITS = 1024;   // units of a list that a block of threads walks, at most
 

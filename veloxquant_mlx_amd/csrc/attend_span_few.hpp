@@ -131,11 +131,86 @@ __device__ __forceinline__ void span_few_block(const SpanCall &c, int id, const 
         const int end = w1 - bl.packed_units < most ? w1 - bl.packed_units : most;
         tail_units = end > tail_u ? end - tail_u : 0;
     }
+    // ---- lists in parts: the block that comes last to a tile's counter adds the parts up, 32 lanes a row.  What orders its loads behind the others' stores:
+    // every thread waits until its own, which are written through, have been acknowledged, the barrier collects the block, one thread counts it, and the
+    // loads, at device scope too, are issued behind the count's return and a barrier (as in attend_mfma_packed.hpp).
+    auto join = [&]() __attribute__((always_inline)) {
+        if constexpr (LISTS) {
+            if (bl.counters == nullptr) return;
+            int *const ticket = listed + BLOCK_UNITS;
+            int32_t *const counter = bl.counters + (((int64_t)b * Hkv + hkv) * bl.tiles + tile) * bl.row_tiles + j0 / ROWS;
+            wait_copies<0>();
+            __syncthreads();
+            if (tid == 0) *ticket = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __syncthreads();
+            if (*ticket != c.nparts - 1) return;
+            const int ch = tid & 31;
+#pragma unroll 1
+            for (int x = tid >> 5; x < here; x += F::THREADS / 32) {
+                int jb2, pos2;
+                const int64_t row = row_of(x, jb2, pos2), rec = row * c.nparts;
+                auto pair_at = [](const float *p) __attribute__((always_inline)) {
+                    const uint64_t u = __hip_atomic_load((const uint64_t *)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    return make_float2(__uint_as_float((u32)u), __uint_as_float((u32)(u >> 32)));
+                };
+                float m = -INFINITY, den = 0.f, num[DT];
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) num[dt] = 0.f;
+#pragma unroll 1
+                for (int p0 = 0; p0 < c.nparts; p0 += 32) {
+                    const float2 ml = p0 + ch < c.nparts ? pair_at(c.ml + (rec + p0 + ch) * 2) : make_float2(-INFINITY, 0.f);
+                    float top = ml.x;
+#pragma unroll
+                    for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
+                    const float mn = fmaxf(m, top), keep = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn), f = mn == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - mn);
+                    m = mn;
+                    float l = f * ml.y;
+#pragma unroll
+                    for (int off = 16; off > 0; off >>= 1) l += __shfl_xor(l, off);
+                    den = __builtin_fmaf(den, keep, l);
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt) num[dt] *= keep;
+                    const int many = c.nparts - p0 < 32 ? c.nparts - p0 : 32;
+#pragma unroll 1
+                    for (int p = 0; p < many; p += 4) {   // four parts' sums under way; a part without a visible slot has none
+                        float2 y[4][DT / 2];
+                        float by[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const int at = p + k < many ? p + k : p;
+                            by[k] = p + k < many ? __shfl(f, at, 32) : 0.f;
+#pragma unroll
+                            for (int dt = 0; dt < DT; dt += 2) y[k][dt / 2] = pair_at(c.sums + (rec + p0 + at) * D + ch * DT + dt);
+                        }
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+#pragma unroll
+                            for (int dt = 0; dt < DT; dt += 2) {
+                                num[dt] = by[k] != 0.f ? __builtin_fmaf(by[k], y[k][dt / 2].x, num[dt]) : num[dt];
+                                num[dt + 1] = by[k] != 0.f ? __builtin_fmaf(by[k], y[k][dt / 2].y, num[dt + 1]) : num[dt + 1];
+                            }
+                    }
+                }
+                const float by = den > 0.f || den != den ? 1.f / den : 0.f;
+                u16 *dst = (u16 *)a.out + row * D + ch * DT;
+#pragma unroll
+                for (int dt = 0; dt < DT; dt += 2)
+                    *(u32 *)(dst + dt) = a.dtype == VQ_BF16 ? SpanMma<bf16_t>::pack(num[dt] * by, num[dt + 1] * by) : SpanMma<f16>::pack(num[dt] * by, num[dt + 1] * by);
+            }
+            if (tid == 0) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+    };
+    // two floats of a part: written through where another block of the launch reads them
+    auto store2 = [&](float *p, float x, float y) __attribute__((always_inline)) {
+        if constexpr (LISTS) st_partial2(p, x, y);
+        else *(float2 *)p = make_float2(x, y);
+    };
     if ((LISTS ? n_listed + tail_units == 0 : w0 == w1) && c.nparts > 1) {   // (uniform) nothing: sums are not written
         if (tid < here * MAPS) {
             int x, y;
-            *(float2 *)(c.ml + ((row_of(tid / MAPS, x, y) * c.nparts + part) * MAPS + tid % MAPS) * 2) = make_float2(-INFINITY, 0.f);
+            store2(c.ml + ((row_of(tid / MAPS, x, y) * c.nparts + part) * MAPS + tid % MAPS) * 2, -INFINITY, 0.f);
         }
+        join();
         return;
     }
 
@@ -494,10 +569,10 @@ __device__ __forceinline__ void span_few_block(const SpanCall &c, int id, const 
             }
             if (c.nparts > 1) {
                 const int64_t rec = (row * c.nparts + part) * MAPS + w;
-                if (ch == 0) *(float2 *)(c.ml + rec * 2) = make_float2(m, den);
+                if (ch == 0) store2(c.ml + rec * 2, m, den);
                 float *dst = c.sums + rec * D + ch * DT;
 #pragma unroll
-                for (int dt = 0; dt < DT; dt += 2) *(float2 *)(dst + dt) = make_float2(num[dt], num[dt + 1]);
+                for (int dt = 0; dt < DT; dt += 2) store2(dst + dt, num[dt], num[dt + 1]);
             }
             const float by = den > 0.f || den != den ? (w == 0 ? 1.f : -span_lam(a, hkv * G + (shared ? (j0 + x) % r1 : j0 + x) % G)) / den : 0.f;
 #pragma unroll
@@ -522,6 +597,7 @@ __device__ __forceinline__ void span_few_block(const SpanCall &c, int id, const 
         for (int dt = 0; dt < DT; dt += 2)
             *(u32 *)(dst + dt) = a.dtype == VQ_BF16 ? SpanMma<bf16_t>::pack(o[dt], o[dt + 1]) : SpanMma<f16>::pack(o[dt], o[dt + 1]);
     }
+    if (LISTS && c.nparts > 1) join();
 }
 
 template <int BITS, int D, int MAPS, int WAVES>

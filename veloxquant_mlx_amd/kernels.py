@@ -1020,14 +1020,17 @@ def release_tile_scratch() -> int:
 _sync_counters: dict[tuple, torch.Tensor] = {}
 
 
-def _counters(device: torch.device, stream: int | None = None) -> torch.Tensor:
+_block_counters: dict[tuple, torch.Tensor] = {}   # of attention over chosen blocks: no captured graph holds them
+
+
+def _counters(device: torch.device, stream: int | None = None, table: dict = _sync_counters) -> torch.Tensor:
     """Per-(device, stream) int32 counters the single-launch decode path needs: zero when a
     call is enqueued, left zero by it (65536 = the largest B*H_kv the MFMA path takes)."""
     key = (device.type, device.index, _stream_of(device) if stream is None else stream)
-    c = _sync_counters.get(key)
+    c = table.get(key)
     if c is None:
         c = torch.zeros(65536, dtype=torch.int32, device=device)
-        _sync_counters[key] = c
+        table[key] = c
     return c
 
 
@@ -1609,7 +1612,8 @@ def _store_attend(name, maps, q, prefix, own, scale, causal, seq_lens, sliding_w
                 raise ValueError(f"{name}: norm_weight must be a contiguous [{D}] tensor on {device}")
             weight, weight_tag = norm_weight.data_ptr(), _ftag(name, norm_weight)
     bits, group, meta, layout = packed or (8, 1, 0, 0)
-    more = b""
+    stream = _stream_of(device)
+    more = bytes
     if lists is not None:
         blocks, block_size, query_block = lists
         if block_size < 1 or query_block < 1:
@@ -1618,19 +1622,20 @@ def _store_attend(name, maps, q, prefix, own, scale, causal, seq_lens, sliding_w
         if blocks.ndim != 4 or blocks.shape[:3] != want or blocks.dtype != torch.int32 or blocks.device != device or not blocks.is_contiguous():
             raise ValueError(f"{name}: blocks must be a contiguous int32 [{want[0]}, {want[1]}, {want[2]}, n] tensor on {device}, got {tuple(blocks.shape)} "
                              f"in {blocks.dtype} on {blocks.device}")
-        try:
-            more = _lib.BLOCK_LISTS_PACK.pack(blocks.data_ptr(), blocks.shape[3], block_size, query_block)
-        except (_lib.struct.error, OverflowError) as e:
-            raise ValueError(f"{name}: {e}") from None
+
+        def more():
+            # (a graph under capture has no counters that are its own and zero at every replay: its parts are added up by a second launch)
+            counters = None if _capturing() else _counters(device, stream, _block_counters)
+            return _lib.BLOCK_LISTS_PACK.pack(blocks.data_ptr(), blocks.shape[3], block_size, query_block, 0 if counters is None else counters.data_ptr(),
+                                              0 if counters is None else counters.numel())
     lib = _lib.load()
-    stream = _stream_of(device)
     call, room = lib.store_attend_packed[maps], lib.store_attend_packed_workspace[maps]
 
     def block(ws):
         return _lib.STORE_ATTEND_PACK.pack(
             q.data_ptr(), out.data_ptr(), B, Hq, heads, Sq, D, *prefix_f, *own_f, lens, lam_p, lam_stride, weight,
             0 if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), stream, sliding_window or 0, tag,
-            tag if tail is None else _FLOAT_TAG[tail], weight_tag, bits, group, meta, layout, 1 if causal else 0, scale, norm_eps, gain) + more
+            tag if tail is None else _FLOAT_TAG[tail], weight_tag, bits, group, meta, layout, 1 if causal else 0, scale, norm_eps, gain) + more()
 
     try:
         _launch_on(device, lambda: _scratch_call(device, stream, call, room, block))
