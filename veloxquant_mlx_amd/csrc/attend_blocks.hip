@@ -97,18 +97,19 @@ bool plan_few(BlockCall &c, const vq_block_attend_args &args) {
     const int64_t qb = c.query_block < a.Sq ? c.query_block : a.Sq, row_tiles = cdiv(a.Hq / a.Hkv * qb, 32);
     if (c.count * sub >= (1 << 24)) return false;
     const int64_t units = c.count * sub + cdiv(a.own.n_tail, 32), items = a.B * a.Hkv * c.tiles * row_tiles;
-    // One round of blocks of equal runs, two blocks a CU (one with heads of 256 channels), four units a wave or more
+    // One round of blocks of equal runs, two blocks a CU (one with heads of 256 channels), two units a wave or
+    // more, of long lists four (8 kv heads: 69 units 15.1 us in runs of eight, 15.6 of sixteen; 261 units 16.4 and 14.9)
     int64_t run = cdiv(items * units, a.D == 256 ? 256 : 512);
-    if (run < 16) run = 16;
+    if (run < (units > 128 ? 16 : 8)) run = units > 128 ? 16 : 8;
     if (run > BLOCK_UNITS) run = BLOCK_UNITS;
     const int64_t splits = units > 0 ? cdiv(units, run) : 1;
-    if (items * splits >= (1 << 22)) return false;
+    if (items * splits >= (1 << 22) || splits > 65535 || c.tiles * row_tiles > 65535) return false;
     c.s.apart = c.s.pfew = 0;
     c.s.ofew = 1;
     c.s.owaves = 4;
     c.s.osplits = c.s.nparts = (int)splits;
     c.lists = {c.blocks, (int)c.tiles, (int)c.count, (int)c.block_tokens, (int)qb, (int)cdiv(a.own.n_packed, c.block_tokens), (int)sub, (int)(c.count * sub),
-               (int)units, (int)row_tiles, splits > 1 && items <= args.counters_len ? args.counters : nullptr};
+               (int)units, (int)(units / splits), (int)(units % splits), (int)row_tiles, splits > 1 && items <= args.counters_len ? args.counters : nullptr};
     c.few = 1;
     return true;
 }

@@ -34,6 +34,7 @@ struct BlockLists {
     int block_tokens, query_block;
     int total;                      // blocks of the store
     int sub, packed_units, units;   // units of an entry, of a list, and with the tail
+    int run, longer;                // units of a run, and how many runs have one more
     int row_tiles;                  // tiles of rows of a tile of queries
     int32_t *counters;              // zeros, one a tile of rows: the last block of a tile adds up its parts; NULL: another launch does
 };

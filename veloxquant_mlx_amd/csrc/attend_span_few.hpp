@@ -50,14 +50,24 @@ __device__ __forceinline__ void span_few_block(const SpanCall &c, int id, const 
     if (!shared) id -= shared_blocks;
     const int hkv = id % Hkv;
     id /= Hkv;
-    const int b = shared ? 0 : id % (int)a.B;
-    if (!shared) id /= (int)a.B;
-    const int splits = shared ? c.psplits : c.osplits, split = id % splits, part = shared || !c.apart ? split : c.psplits + split;
+    const int b = LISTS ? id : shared ? 0 : id % (int)a.B;   // (lists: a grid of (sequence and kv head, run, tile))
+    if (!LISTS && !shared) id /= (int)a.B;
+    const int splits = shared ? c.psplits : c.osplits, split = LISTS ? (int)blockIdx.y : id % splits, part = shared || !c.apart ? split : c.psplits + split;
+    // ---- lists: the run, its first entries asked for ahead of all else
+    [[maybe_unused]] const int32_t *list = nullptr;
+    [[maybe_unused]] int l0 = 0, l1 = 0, entry = -1;   // units of the list
+    if constexpr (LISTS) {
+        l0 = split * bl.run + (split < bl.longer ? split : bl.longer);
+        l1 = l0 + bl.run + (split < bl.longer ? 1 : 0);
+        list = bl.blocks + (((int64_t)b * Hkv + hkv) * bl.tiles + (int)blockIdx.z / bl.row_tiles) * bl.count;
+        if (l0 + tid < (l1 < bl.packed_units ? l1 : bl.packed_units)) entry = list[(l0 + tid) / bl.sub];
+    }
+
     // ---- this lane's query row: positions outermost
     constexpr int ROWS = 32 / MAPS;
-    const int tile = LISTS ? id / splits / bl.row_tiles : 0, pos0 = LISTS ? tile * bl.query_block : 0;   // the tile of queries, its first
+    const int tile = LISTS ? (int)blockIdx.z / bl.row_tiles : 0, pos0 = LISTS ? tile * bl.query_block : 0;   // the tile of queries, its first
     const int rows = LISTS ? G * (Sq - pos0 < bl.query_block ? Sq - pos0 : bl.query_block) : shared ? (int)a.B * r1 : r1;
-    const int j0 = (LISTS ? id / splits % bl.row_tiles : id / splits) * ROWS, here = rows - j0 < ROWS ? rows - j0 : ROWS;   // the block's tile of rows
+    const int j0 = (LISTS ? (int)blockIdx.z % bl.row_tiles : id / splits) * ROWS, here = rows - j0 < ROWS ? rows - j0 : ROWS;   // the block's tile of rows
     const int map = MAPS == 2 ? n >> 4 : 0, j = n % ROWS, jc = j < here ? j : here - 1;
     auto row_of = [&](int x, int &jb, int &pos) __attribute__((always_inline)) {   // flattened [B, Hq, Sq] row of tile row x
         x += j0;
@@ -93,14 +103,13 @@ __device__ __forceinline__ void span_few_block(const SpanCall &c, int id, const 
     const int np0 = shared || !c.apart ? (int)a.prefix.n_packed : 0, nt0 = shared || !c.apart ? (int)a.prefix.n_tail : 0;
     const int own = shared ? 0 : own_live, np1 = own < (int)a.own.n_packed ? own : (int)a.own.n_packed, nt1 = own - np1;
     const int tail0 = (int)a.prefix.n_packed, tail1 = before + (int)a.own.n_packed;
-    const int total = LISTS ? bl.units : units_seen(0, np0) + units_seen(tail0, nt0) + units_seen(before, np1) + units_seen(tail1, nt1);
+    const int total = LISTS ? 0 : units_seen(0, np0) + units_seen(tail0, nt0) + units_seen(before, np1) + units_seen(tail1, nt1);
     const int run = total / splits, longer = total % splits;   // (the first runs a unit longer)
-    const int w0 = split * run + (split < longer ? split : longer), w1 = w0 + run + (split < longer ? 1 : 0);
+    const int w0 = LISTS ? l0 : split * run + (split < longer ? split : longer), w1 = LISTS ? l1 : w0 + run + (split < longer ? 1 : 0);
     // ---- lists: the run's units of packed slots that some row sees, in order; then its units of the tail, from tail_u on
     int *const listed = (int *)(lds + F::LDS);
     int n_listed = 0, tail_u = 0, tail_units = 0;
     if constexpr (LISTS) {
-        const int32_t *list = bl.blocks + (((int64_t)b * Hkv + hkv) * bl.tiles + tile) * bl.count;
         const int limit = any_hi < np1 ? any_hi : np1, last = w1 < bl.packed_units ? w1 : bl.packed_units;
         int *const taken = listed + BLOCK_UNITS;   // by each wave
 #pragma unroll 1
@@ -108,7 +117,7 @@ __device__ __forceinline__ void span_few_block(const SpanCall &c, int id, const 
             const int v = v0 + tid;
             int t0 = -1;
             if (v < last) {
-                const int e = list[v / bl.sub];
+                const int e = v0 == w0 ? entry : list[v / bl.sub];
                 if (e >= 0 && e < bl.total) t0 = e * bl.block_tokens + v % bl.sub * UNIT;
             }
             const bool take = t0 >= 0 && t0 < limit;
@@ -144,6 +153,7 @@ __device__ __forceinline__ void span_few_block(const SpanCall &c, int id, const 
             if (tid == 0) *ticket = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             __syncthreads();
             if (*ticket != c.nparts - 1) return;
+            constexpr int AT_ONCE = 8;   // parts whose sums are under way
             const int ch = tid & 31;
 #pragma unroll 1
             for (int x = tid >> 5; x < here; x += F::THREADS / 32) {
@@ -156,9 +166,19 @@ __device__ __forceinline__ void span_few_block(const SpanCall &c, int id, const 
                 float m = -INFINITY, den = 0.f, num[DT];
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) num[dt] = 0.f;
+                float2 y[AT_ONCE][DT / 2];
+                auto sums_of = [&](int p) __attribute__((always_inline)) {   // (parts past the last: it again)
+#pragma unroll
+                    for (int k = 0; k < AT_ONCE; ++k) {
+                        const int at = p + k < c.nparts ? p + k : c.nparts - 1;
+#pragma unroll
+                        for (int dt = 0; dt < DT; dt += 2) y[k][dt / 2] = pair_at(c.sums + (rec + at) * D + ch * DT + dt);
+                    }
+                };
 #pragma unroll 1
                 for (int p0 = 0; p0 < c.nparts; p0 += 32) {
                     const float2 ml = p0 + ch < c.nparts ? pair_at(c.ml + (rec + p0 + ch) * 2) : make_float2(-INFINITY, 0.f);
+                    sums_of(p0);   // (asked for with the maxima)
                     float top = ml.x;
 #pragma unroll
                     for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
@@ -172,23 +192,19 @@ __device__ __forceinline__ void span_few_block(const SpanCall &c, int id, const 
                     for (int dt = 0; dt < DT; ++dt) num[dt] *= keep;
                     const int many = c.nparts - p0 < 32 ? c.nparts - p0 : 32;
 #pragma unroll 1
-                    for (int p = 0; p < many; p += 4) {   // four parts' sums under way; a part without a visible slot has none
-                        float2 y[4][DT / 2];
-                        float by[4];
+                    for (int p = 0;; ) {
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const int at = p + k < many ? p + k : p;
-                            by[k] = p + k < many ? __shfl(f, at, 32) : 0.f;
-#pragma unroll
-                            for (int dt = 0; dt < DT; dt += 2) y[k][dt / 2] = pair_at(c.sums + (rec + p0 + at) * D + ch * DT + dt);
-                        }
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
+                        for (int k = 0; k < AT_ONCE; ++k) {
+                            const float by = p + k < many ? __shfl(f, p + k, 32) : 0.f;   // (a part without a visible slot has no sums)
 #pragma unroll
                             for (int dt = 0; dt < DT; dt += 2) {
-                                num[dt] = by[k] != 0.f ? __builtin_fmaf(by[k], y[k][dt / 2].x, num[dt]) : num[dt];
-                                num[dt + 1] = by[k] != 0.f ? __builtin_fmaf(by[k], y[k][dt / 2].y, num[dt + 1]) : num[dt + 1];
+                                num[dt] = by != 0.f ? __builtin_fmaf(by, y[k][dt / 2].x, num[dt]) : num[dt];
+                                num[dt + 1] = by != 0.f ? __builtin_fmaf(by, y[k][dt / 2].y, num[dt + 1]) : num[dt + 1];
                             }
+                        }
+                        p += AT_ONCE;
+                        if (p >= many) break;
+                        sums_of(p0 + p);
                     }
                 }
                 const float by = den > 0.f || den != den ? 1.f / den : 0.f;
@@ -661,7 +677,7 @@ template <int BITS, int D, int WAVES> int launch_blocks_few_of(const SpanCall &c
     const auto kernel = blocks_few_kernel<BITS, D, WAVES>;
     static std::atomic<bool> allowed[64] = {};
     if (int rc = span_allow_lds((const void *)kernel, bytes, allowed)) return rc;
-    kernel<<<(unsigned)(c.a.B * c.a.Hkv * c.osplits * bl.tiles * bl.row_tiles), 64 * WAVES, bytes, (hipStream_t)c.a.stream>>>(c, bl);
+    kernel<<<dim3((unsigned)(c.a.B * c.a.Hkv), (unsigned)c.osplits, (unsigned)(bl.tiles * bl.row_tiles)), 64 * WAVES, bytes, (hipStream_t)c.a.stream>>>(c, bl);
     VQ_HIP_CHECK_LAUNCH("attention over blocks");
     return VQ_OK;
 }
