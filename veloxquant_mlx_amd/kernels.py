@@ -1494,11 +1494,17 @@ def _store_fields(name, which, device, batch, k_packed=None, k_scale=None, k_zer
     fields = [0, 0, 0, 0, 0, 0, 0, 0]
     if n_packed:
         arrays = (k_packed, k_scale, k_zero, v_packed, v_scale, v_zero)
-        for t in arrays:
-            if t is None or t.ndim != 4 or not t.is_contiguous():
-                raise ValueError(f"{name}: packed tensors ({which}) must be given, 4D and contiguous")
-            if t.device != device:
-                raise ValueError(f"{name}: packed tensors ({which}) must live on {device}, got {t.device}")
+        at = device.index   # (six devices compared as numbers: the loop below takes 2 us)
+        if not (k_packed is not None and k_scale is not None and k_zero is not None and v_packed is not None and v_scale is not None
+                and v_zero is not None and k_packed.get_device() == k_scale.get_device() == k_zero.get_device() == v_packed.get_device()
+                == v_scale.get_device() == v_zero.get_device() == at and k_packed.ndim == k_scale.ndim == v_packed.ndim == v_scale.ndim == 4
+                and k_packed.is_contiguous() and k_scale.is_contiguous() and k_zero.is_contiguous() and v_packed.is_contiguous()
+                and v_scale.is_contiguous() and v_zero.is_contiguous()):
+            for t in arrays:
+                if t is None or t.ndim != 4 or not t.is_contiguous():
+                    raise ValueError(f"{name}: packed tensors ({which}) must be given, 4D and contiguous")
+                if t.device != device:
+                    raise ValueError(f"{name}: packed tensors ({which}) must live on {device}, got {t.device}")
         bits, g = int(bits), int(group_size)
         if not 1 <= bits <= 8 or g < 1 or v_layout not in _V_LAYOUT:
             raise ValueError(f"{name}: bits={bits}, group_size={g}, v_layout={v_layout!r} ({which})")
@@ -1551,15 +1557,15 @@ def _store_fields(name, which, device, batch, k_packed=None, k_scale=None, k_zer
 
 
 def _scratch_call(device, stream, call, room, block):
-    """Run ``call(block(workspace))`` with the stream's scratch, or with one of its own that a graph under capture keeps."""
+    """Run ``call(block(workspace, captured))`` with the stream's scratch, or with one of its own that a graph under capture keeps."""
     if _capturing():
         # a graph's scratch is its own: two graphs captured on one stream may run at once, and the scratch kept for the
         # stream is given back when a larger one replaces it
-        need = room(block(None))
-        return call(block(torch.empty(need, dtype=torch.uint8, device=device) if need else None))
-    rc = call(block(_workspace(device, 0, stream)))
+        need = room(block(None, True))
+        return call(block(torch.empty(need, dtype=torch.uint8, device=device) if need else None, True))
+    rc = call(block(_workspace(device, 0, stream), False))
     if rc == _lib.VQ_ERR_WORKSPACE:
-        rc = call(block(_workspace(device, room(block(None)), stream)))
+        rc = call(block(_workspace(device, room(block(None, False)), stream), False))
     return rc
 
 
@@ -1613,7 +1619,7 @@ def _store_attend(name, maps, q, prefix, own, scale, causal, seq_lens, sliding_w
             weight, weight_tag = norm_weight.data_ptr(), _ftag(name, norm_weight)
     bits, group, meta, layout = packed or (8, 1, 0, 0)
     stream = _stream_of(device)
-    more = bytes
+    more = None
     if lists is not None:
         blocks, block_size, query_block = lists
         if block_size < 1 or query_block < 1:
@@ -1623,19 +1629,20 @@ def _store_attend(name, maps, q, prefix, own, scale, causal, seq_lens, sliding_w
             raise ValueError(f"{name}: blocks must be a contiguous int32 [{want[0]}, {want[1]}, {want[2]}, n] tensor on {device}, got {tuple(blocks.shape)} "
                              f"in {blocks.dtype} on {blocks.device}")
 
-        def more():
+        def more(captured):
             # (a graph under capture has no counters that are its own and zero at every replay: its parts are added up by a second launch)
-            counters = None if _capturing() else _counters(device, stream, _block_counters)
+            counters = None if captured else _counters(device, stream, _block_counters)
             return _lib.BLOCK_LISTS_PACK.pack(blocks.data_ptr(), blocks.shape[3], block_size, query_block, 0 if counters is None else counters.data_ptr(),
                                               0 if counters is None else counters.numel())
     lib = _lib.load()
     call, room = lib.store_attend_packed[maps], lib.store_attend_packed_workspace[maps]
 
-    def block(ws):
-        return _lib.STORE_ATTEND_PACK.pack(
+    def block(ws, captured):
+        args = _lib.STORE_ATTEND_PACK.pack(
             q.data_ptr(), out.data_ptr(), B, Hq, heads, Sq, D, *prefix_f, *own_f, lens, lam_p, lam_stride, weight,
             0 if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), stream, sliding_window or 0, tag,
-            tag if tail is None else _FLOAT_TAG[tail], weight_tag, bits, group, meta, layout, 1 if causal else 0, scale, norm_eps, gain) + more()
+            tag if tail is None else _FLOAT_TAG[tail], weight_tag, bits, group, meta, layout, 1 if causal else 0, scale, norm_eps, gain)
+        return args if more is None else args + more(captured)
 
     try:
         _launch_on(device, lambda: _scratch_call(device, stream, call, room, block))
@@ -1754,7 +1761,7 @@ def select_blocks(q: torch.Tensor, k_scale: torch.Tensor, k_zero: torch.Tensor, 
     lib = _lib.load()
     stream = _stream_of(device)
 
-    def block(ws):
+    def block(ws, captured):
         return _lib.BLOCK_SELECT_PACK.pack(
             q.data_ptr(), k_scale.data_ptr(), k_zero.data_ptr(), out.data_ptr(), B, Hq, heads, Sq, D, n_packed, groups * group_size, n_tail, block_size,
             query_block, n_select, first, recent, lens, 0 if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), stream, tag,
@@ -1872,25 +1879,28 @@ def norm_rotary_embed(q: torch.Tensor, k: torch.Tensor | None = None, *, q_weigh
     Squares, their sum, the norm and the turn are float32, with one rounding at the end.  The other arguments, strides and outputs as for
     :func:`rotary_embed`."""
     name = "norm_rotary_embed"
-    eps = float(norm_eps)
-    if not 0 <= eps < float("inf"):
+    if not 0 <= norm_eps < math.inf:
         raise ValueError(f"{name}: norm_eps={norm_eps} must be a number from 0 on")
-    at, strides, tag, keep = [0, 0], [0, 0], 0, []
-    for i, (w, x, what) in enumerate(((q_weight, q, "q"), (k_weight, k, "k"))):
-        if w is None:
-            continue
-        if x is None:
+    q_at = q_step = k_at = k_step = tag = 0
+    if q_weight is not None:
+        q_weight, q_at, q_step, tag = _norm_weight(name, q_weight, q, "q")
+    if k_weight is not None:
+        if k is None:
             raise ValueError(f"{name}: k_weight without k")
-        if x.ndim != 4 or w.device != x.device or (w.shape != x.shape[3:] and w.shape != (x.shape[1], x.shape[3])):
-            raise ValueError(f"{name}: the weight for {what} must be [D] or [H, D] of its {tuple(x.shape)} on {x.device}, got {tuple(w.shape)} on {w.device}")
-        if keep and w.dtype != keep[0].dtype:
-            raise ValueError(f"{name}: q_weight and k_weight must be of one dtype, got {keep[0].dtype} and {w.dtype}")
-        tag = _ftag(name, w)
-        w = w.contiguous()
-        keep.append(w)
-        at[i], strides[i] = w.data_ptr(), x.shape[3] if w.ndim == 2 else 0
+        if q_weight is not None and k_weight.dtype != q_weight.dtype:
+            raise ValueError(f"{name}: q_weight and k_weight must be of one dtype, got {q_weight.dtype} and {k_weight.dtype}")
+        k_weight, k_at, k_step, tag = _norm_weight(name, k_weight, k, "k")
     return _rotary_rows(name, q, k, inv_freq, offset, positions, traditional, attention_factor, False, out, k_out,
-                        _lib.NORM_PACK.pack(*at, *strides, tag, eps), keep)
+                        _lib.NORM_PACK.pack(q_at, k_at, q_step, k_step, tag, norm_eps), (q_weight, k_weight))
+
+
+def _norm_weight(name, w, x, what):
+    """A norm's weight, contiguous; its address, the elements between heads' rows (0: one for all) and its type."""
+    shape, rows = w.shape, x.shape
+    if len(rows) != 4 or w.get_device() != x.get_device() or shape[-1:] != rows[3:] or (len(shape) != 1 and shape != (rows[1], rows[3])):
+        raise ValueError(f"{name}: the weight for {what} must be [D] or [H, D] of its {tuple(rows)} on {x.device}, got {tuple(shape)} on {w.device}")
+    w = w.contiguous()
+    return w, w.data_ptr(), 0 if len(shape) == 1 else rows[3], _ftag(name, w)
 
 
 def _rotary_rows(name, q, k, inv_freq, offset, positions, traditional, attention_factor, inverse, out, k_out, norm=None, keep=()):
