@@ -602,7 +602,7 @@ int vq_differential_attend(const vq_store_attend_args *a);
 
 /* The blocks of block_tokens packed slots (a multiple of the group) that the queries of a tile attend to, by a bound on their scores: a
  * key group's keys lie between zero and zero + levels * scale in every channel, so sum_c max(q_c zero_c, q_c (zero_c + levels
- * scale_c)) bounds its products with a query; a block's score is the largest bound over its groups, the query heads of the kv head
+ * scale_c)) bounds its products with a query (but for a slot's rounding to fp16); a block's score is the largest bound over its groups, the query heads of the kv head
  * and the queries of the tile (query_block consecutive ones choose together, the last tile fewer), of the groups that a query sees.
  * Query i of Sq stands at slot n - Sq + i of the sequence's n live slots (n_packed + n_tail, or seq_lens); causal hides the slots
  * behind it.  Of the blocks that the tile's last query sees all are chosen if they are `count` at most; else the first `first`, the

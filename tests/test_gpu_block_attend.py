@@ -9,7 +9,7 @@ from tests._blocks import attend, choose, times_seen
 from tests._gpu import gpu, require_gpu
 from tests._spans import close, store
 from veloxquant_mlx_amd import kernels as K
-from veloxquant_mlx_amd.cache import KVCacheConfig, KVCacheFactory
+from veloxquant_mlx_amd.cache import KVCacheConfig, KVCacheFactory, LayerStackedKIVICache
 from veloxquant_mlx_amd.rotary import RotaryPositions
 
 pytestmark = gpu
@@ -146,17 +146,17 @@ def test_blocks_that_are_not_listed_are_not_read(D, dtype):
 
 
 def test_far_slots():
-    """Slots whose channels lie past 2^31 elements into their buffers."""
+    """Slots whose words lie past 2^31 bytes into their buffers."""
     require_gpu()
-    B, H, D, n, block = 1, 2, 128, 1 << 20, 128
+    B, H, D, n, block = 1, 3, 128, 1 << 24, 128
     g = torch.Generator(device="cuda").manual_seed(1)
     words = torch.randint(-2 ** 31, 2 ** 31 - 1, (B, H, n, D // 8), generator=g, device="cuda", dtype=torch.int32)
     values = torch.randint(-2 ** 31, 2 ** 31 - 1, (B, H, n // 8, D), generator=g, device="cuda", dtype=torch.int32)
     ks, kz = (torch.rand((B, H, n // 32, D), generator=g, device="cuda").half() * 0.1 for _ in range(2))
     vs, vz = (torch.rand((B, H, D // 32, n), generator=g, device="cuda").half() * 0.1 for _ in range(2))
     s = dict(k_packed=words, k_scale=ks, k_zero=kz, v_packed=values, v_scale=vs, v_zero=vz, bits=4, group_size=32, v_layout="token")
-    q = torch.randn((B, 8, 1, D), generator=g, device="cuda").half()
-    blocks = torch.tensor([0, 1, 4095, 8190, 8191], dtype=torch.int32, device="cuda").expand(B, H, 1, 5).contiguous()
+    q = torch.randn((B, 12, 1, D), generator=g, device="cuda").half()
+    blocks = torch.tensor([0, 1, 4095, n // block - 2, n // block - 1], dtype=torch.int32, device="cuda").expand(B, H, 1, 5).contiguous()
     got = K.block_sparse_attend(q, blocks, **s, n_packed=n, block_size=block, scale=0.1)
     at = torch.cat([torch.arange(int(e) * block, (int(e) + 1) * block, device="cuda") for e in blocks[0, 0, 0]])
     few = dict(s, k_packed=words[:, :, at].contiguous(), v_packed=values.view(B, H, -1, block // 8, D)[:, :, blocks[0, 0, 0].long()].flatten(2, 3).contiguous(),
@@ -165,6 +165,32 @@ def test_far_slots():
                v_scale=vs[..., at].contiguous(), v_zero=vz[..., at].contiguous())
     near = torch.arange(5, dtype=torch.int32, device="cuda").expand(B, H, 1, 5).contiguous()
     assert torch.equal(got, K.block_sparse_attend(q, near, **few, n_packed=5 * block, block_size=block, scale=0.1))
+
+
+def test_lists_longer_than_a_block_walks():
+    """2200 entries of 32 tokens for each of 512 kv heads: more units than one block of threads holds."""
+    require_gpu()
+    entries = (torch.arange(2200, dtype=torch.int32, device="cuda") % 5 - 1)     # each of four blocks 440 times, and none
+    blocks = entries.expand(128, 4, 1, 2200).contiguous()
+    _case(128, 4, 4, 64, (128, 3), 32, 2200, bits=2, blocks=blocks, seed=10)
+
+
+@pytest.mark.parametrize("Sq,query_block", [(1, 1), (40, 4)])
+def test_a_layer_of_a_stack(Sq, query_block):
+    require_gpu()
+    cfg = KVCacheConfig(method="kivi", head_dim=128, bit_width_inlier=4, kivi_group_size=32, residual_length=32, fused_sdpa=True, fused_sdpa_memory_bound=True)
+    stack, alone = LayerStackedKIVICache(cfg, 2), [KVCacheFactory.create(cfg) for _ in range(2)]
+    g = torch.Generator(device="cuda").manual_seed(4)
+    for S in (300, 1, Sq):
+        k, v = (torch.randn((2, 2, 4, S, 128), generator=g, device="cuda").half() for _ in range(2))
+        for layer in range(2):
+            stack[layer].update_and_fetch(k[layer], v[layer])
+            alone[layer].update_and_fetch(k[layer], v[layer])
+        stack.fused_sdpa_all(torch.randn((2, 2, 8, 1, 128), generator=g, device="cuda").half(), 0.1)      # (stacks the layers' buffers)
+    q = torch.randn((2, 8, Sq, 128), generator=g, device="cuda").half()
+    for layer in range(2):
+        args = (q, 0.1, 4)
+        assert torch.equal(stack[layer].fused_sparse_sdpa(*args, query_block=query_block), alone[layer].fused_sparse_sdpa(*args, query_block=query_block))
 
 
 def test_output_stream_graph_and_repeats():

@@ -92,7 +92,7 @@ int check_blocks(const char *fn, const vq_block_attend_args *args) {
 // query heads at the positions of one list, each over the list's units, in as many runs as fill the chip.
 bool plan_few(BlockCall &c, const vq_block_attend_args &args) {
     const vq_store_attend_args &a = c.s.a;
-    if (a.own.n_packed == 0 || c.block_tokens % 32 != 0 || !span_mfma_supported(a)) return false;
+    if (c.block_tokens % 32 != 0 || !span_mfma_supported(a)) return false;
     const int64_t all = cdiv(a.own.n_packed, 32), sub = c.block_tokens / 32 < all ? c.block_tokens / 32 : all;
     const int64_t qb = c.query_block < a.Sq ? c.query_block : a.Sq, row_tiles = cdiv(a.Hq / a.Hkv * qb, 32);
     if (c.count * sub >= (1 << 24)) return false;
@@ -123,7 +123,6 @@ BlockCall cut_blocks(const vq_block_attend_args &args) {
     c.query_block = args.query_block;
     const vq_store_attend_args &a = c.s.a;
     c.tiles = cdiv(a.Sq, c.query_block);
-    if (a.own.n_packed == 0) { c.s.a.pack_bits = 8; c.s.a.group = 1; c.count = 0; }   // fields that no packed slot reads
     if (plan_few(c, args)) return c;
     // as many waves as fill the chip eight deep, runs of 64 slots or more
     const int64_t rows = a.B * a.Hq * a.Sq;
@@ -155,6 +154,7 @@ int64_t block_floats(const BlockCall &c, int64_t &sums) {
 extern "C" size_t vq_block_attend_workspace(const vq_block_attend_args *args) {
     using namespace vq;
     if (check_blocks("vq_block_attend", args) != VQ_OK) return 0;
+    if (args->store.own.n_packed == 0) return vq_shared_prefix_attend_workspace(&args->store);   // (no list names a slot)
     return block_bytes(cut_blocks(*args));
 }
 
@@ -162,6 +162,7 @@ extern "C" int vq_block_attend(const vq_block_attend_args *args) {
     using namespace vq;
     const char *fn = "vq_block_attend";
     if (int rc = check_blocks(fn, args)) return rc;
+    if (args->store.own.n_packed == 0) return vq_shared_prefix_attend(&args->store);
     BlockCall c = cut_blocks(*args);
     const vq_store_attend_args &a = c.s.a;
     const size_t need = block_bytes(c);

@@ -287,6 +287,7 @@ template <typename T> int launch_norm_rotary(const vq_norm_rotary_args &n, hipSt
         return VQ_OK;
     }
     const int64_t rows = tokens * heads;
+    VQ_REQUIRE(rows < (INT64_C(1) << 26), VQ_ERR_UNSUPPORTED, "vq_norm_rotary: too many rows for one launch");
     norm_rotary_any_kernel<T><<<(unsigned)cdiv(rows, 4), 256, 0, st>>>(n);
     VQ_HIP_CHECK_LAUNCH("vq_norm_rotary");
     return VQ_OK;
@@ -311,7 +312,7 @@ extern "C" int vq_norm_rotary(const vq_norm_rotary_args *args, void *stream) {
     }
     const int64_t heads = a.heads[0] + a.heads[1];
     if (a.B == 0 || a.S == 0 || heads == 0) return VQ_OK;
-    VQ_REQUIRE((double)a.B * (double)a.S * (double)heads < 16777216. * 4., VQ_ERR_UNSUPPORTED, "%s: 2^26 or more rows", fn);
+    VQ_REQUIRE((double)a.B * (double)a.S < 4294967296., VQ_ERR_UNSUPPORTED, "%s: too many rows for one launch", fn);
     VQ_DISPATCH_FLOAT(a.dtype, T, return launch_norm_rotary<T>(*args, (hipStream_t)stream));
     return VQ_OK;
 }

@@ -1710,7 +1710,7 @@ def select_blocks(q: torch.Tensor, k_scale: torch.Tensor, k_zero: torch.Tensor, 
 
     A block holds ``block_size`` slots, a multiple of ``group_size`` (default: one group).  Its score bounds what any of its keys can score: a
     group's keys lie between ``zero`` and ``zero + levels * scale`` in every channel (``levels`` the top code), so ``sum_c max(q_c zero_c,
-    q_c (zero_c + levels scale_c))`` is at least every ``q k`` of the group; the block's is the largest over its groups, over the query heads of
+    q_c (zero_c + levels scale_c))`` is at least every ``q k`` of the group (but for the rounding of a slot to fp16); the block's is the largest over its groups, over the query heads of
     the kv head and over the ``query_block`` consecutive queries of the tile, which choose together (the last tile may hold fewer).  ``k_scale``,
     ``k_zero [B,Hkv,cap/group,D]`` (float16 or float32) are the store's own, so choosing reads no key.
 
@@ -1879,7 +1879,7 @@ def norm_rotary_embed(q: torch.Tensor, k: torch.Tensor | None = None, *, q_weigh
     Squares, their sum, the norm and the turn are float32, with one rounding at the end.  The other arguments, strides and outputs as for
     :func:`rotary_embed`."""
     name = "norm_rotary_embed"
-    if not 0 <= norm_eps < math.inf:
+    if not 0 <= norm_eps < 1e38:
         raise ValueError(f"{name}: norm_eps={norm_eps} must be a number from 0 on")
     q_at = q_step = k_at = k_step = tag = 0
     if q_weight is not None:
