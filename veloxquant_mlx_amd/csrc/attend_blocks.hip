@@ -108,8 +108,12 @@ bool plan_few(BlockCall &c, const vq_block_attend_args &args) {
     c.s.ofew = 1;
     c.s.owaves = 4;
     c.s.osplits = c.s.nparts = (int)splits;
+    // Parts are added up in the launch where a tile's are 32 KB at most, which the one block that does it reads past its caches at ~20 GB/s (4 rows of 128
+    // channels in nine parts, 18 KB: 1.9 us; 9 rows of 256 in eleven, 99 KB: 7.5, and a launch of its own 4 to 5)
+    const int64_t rows = a.Hq / a.Hkv * qb < 32 ? a.Hq / a.Hkv * qb : 32;
+    const bool join = splits > 1 && items <= args.counters_len && rows * splits * a.D * 4 <= 32 * 1024;
     c.lists = {c.blocks, (int)c.tiles, (int)c.count, (int)c.block_tokens, (int)qb, (int)cdiv(a.own.n_packed, c.block_tokens), (int)sub, (int)(c.count * sub),
-               (int)units, (int)(units / splits), (int)(units % splits), (int)row_tiles, splits > 1 && items <= args.counters_len ? args.counters : nullptr};
+               (int)units, (int)(units / splits), (int)(units % splits), (int)row_tiles, join ? args.counters : nullptr};
     c.few = 1;
     return true;
 }

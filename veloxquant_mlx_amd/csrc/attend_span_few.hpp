@@ -167,12 +167,12 @@ __device__ __forceinline__ void span_few_block(const SpanCall &c, int id, const 
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) num[dt] = 0.f;
                 float2 y[AT_ONCE][DT / 2];
-                auto sums_of = [&](int p) __attribute__((always_inline)) {   // (parts past the last: it again)
+                auto sums_of = [&](int p) __attribute__((always_inline)) {
 #pragma unroll
                     for (int k = 0; k < AT_ONCE; ++k) {
-                        const int at = p + k < c.nparts ? p + k : c.nparts - 1;
+                        if (p + k >= c.nparts) break;
 #pragma unroll
-                        for (int dt = 0; dt < DT; dt += 2) y[k][dt / 2] = pair_at(c.sums + (rec + at) * D + ch * DT + dt);
+                        for (int dt = 0; dt < DT; dt += 2) y[k][dt / 2] = pair_at(c.sums + (rec + p + k) * D + ch * DT + dt);
                     }
                 };
 #pragma unroll 1
@@ -195,7 +195,8 @@ __device__ __forceinline__ void span_few_block(const SpanCall &c, int id, const 
                     for (int p = 0;; ) {
 #pragma unroll
                         for (int k = 0; k < AT_ONCE; ++k) {
-                            const float by = p + k < many ? __shfl(f, p + k, 32) : 0.f;   // (a part without a visible slot has no sums)
+                            if (p + k >= many) break;
+                            const float by = __shfl(f, p + k, 32);   // (a part without a visible slot has no sums)
 #pragma unroll
                             for (int dt = 0; dt < DT; dt += 2) {
                                 num[dt] = by != 0.f ? __builtin_fmaf(by, y[k][dt / 2].x, num[dt]) : num[dt];
