@@ -1518,13 +1518,11 @@ def _store_fields(name, which, device, batch, k_packed=None, k_scale=None, k_zer
         k_meta, v_meta = k_scale.shape, v_scale.shape
         channels = k_meta[3]
         GV = -(-channels // g)
-        if v_layout == "token":
-            want = ((B, heads, cap // per, channels), (B, heads, GV, cap))
-        else:
-            want = ((B, heads, cap, W), (B, heads, cap, GV))
-        if (B != batch or W != -(-channels // per) or cap < n_packed or (v_layout == "token" and cap % per)
-                or k_meta != (B, heads, -(-cap // g), channels) or k_zero.shape != k_meta or v_packed.shape != want[0]
-                or v_meta != want[1] or v_zero.shape != v_meta):
+        token = v_layout == "token"
+        if (B != batch or W != -(-channels // per) or cap < n_packed or (token and cap % per)
+                or k_meta != (B, heads, -(-cap // g), channels) or k_zero.shape != k_meta
+                or v_packed.shape != ((B, heads, cap // per, channels) if token else (B, heads, cap, W))
+                or v_meta != ((B, heads, GV, cap) if token else (B, heads, cap, GV)) or v_zero.shape != v_meta):
             raise ValueError(f"{name}: packed tensors ({which}) {[tuple(t.shape) for t in arrays]} do not fit a batch of {batch}, {n_packed} tokens, "
                              f"{bits} bits, groups of {g}, values packed by {v_layout}")
         packed = (bits, g, VQ_F16 if meta == torch.float16 else VQ_F32, _V_LAYOUT[v_layout])
@@ -1582,7 +1580,7 @@ def _store_attend(name, maps, q, prefix, own, scale, causal, seq_lens, sliding_w
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != q.shape or out.dtype != dtype or out.device != device or not out.is_contiguous():
         raise ValueError(f"{name}: out must be a contiguous {tuple(q.shape)} tensor in {dtype} on {device}")
-    own_f, heads, channels, packed, tail, keep = _store_fields(name, "own", device, B, **own)
+    own_f, heads, channels, packed, tail, keep = _store_fields(name, "own", device, B, *own)
     prefix_f = _NO_STORE
     if prefix is not None:
         prefix_f, h2, c2, packed2, tail2, keep2 = _store_fields(name, "prefix", device, 1, **prefix)
@@ -1674,8 +1672,7 @@ def shared_prefix_attend(q: torch.Tensor, prefix: dict, *, k_packed=None, k_scal
     token) and up to 64 rows a sequence and kv head (``Sq * Hq / Hkv``) the prefix meets the rows of all sequences together, read once a
     tile of 128 of them (32 where they are few).  Longer chunks walk it a sequence and tile; other stores and types a query row, an
     order of magnitude slower."""
-    own = dict(k_packed=k_packed, k_scale=k_scale, k_zero=k_zero, v_packed=v_packed, v_scale=v_scale, v_zero=v_zero, n_packed=n_packed,
-               bits=bits, group_size=group_size, v_layout=v_layout, k_tail=k_tail, v_tail=v_tail, n_tail=n_tail)
+    own = (k_packed, k_scale, k_zero, v_packed, v_scale, v_zero, n_packed, bits, group_size, v_layout, k_tail, v_tail, n_tail)
     return _store_attend("shared_prefix_attend", 1, q, prefix, own, scale, causal, seq_lens, sliding_window, out)
 
 
@@ -1692,8 +1689,7 @@ def differential_attend(q: torch.Tensor, lam: torch.Tensor | float, *, k_packed=
     ``k_tail`` / ``v_tail``).  ``lam``: float32 ``[Hq]`` or of one value on the device, or a number.  The result is scaled by ``gain``; with
     ``norm_weight`` (``[D]``) every head's output is first divided by ``sqrt(mean(o^2) + norm_eps)`` and multiplied by it, which is the
     layer's head norm (``gain = 1 - lambda_init``).  Both maps' weights and sums are formed in one pass over the slots.  ``out`` may be ``q``."""
-    own = dict(k_packed=k_packed, k_scale=k_scale, k_zero=k_zero, v_packed=v_packed, v_scale=v_scale, v_zero=v_zero, n_packed=n_packed,
-               bits=bits, group_size=group_size, v_layout=v_layout, k_tail=k_tail, v_tail=v_tail, n_tail=n_tail)
+    own = (k_packed, k_scale, k_zero, v_packed, v_scale, v_zero, n_packed, bits, group_size, v_layout, k_tail, v_tail, n_tail)
     return _store_attend("differential_attend", 2, q, None, own, scale, causal, seq_lens, sliding_window, out, lam, norm_weight, norm_eps,
                          gain)
 
@@ -1787,8 +1783,7 @@ def block_sparse_attend(q: torch.Tensor, blocks: torch.Tensor, *, block_size: in
     ``causal``, not behind the query.  Entries may come in any order; one below zero or past the live slots names nothing, one that is
     named twice counts twice.  The plain rows of the tail are all seen, up to the query's own.  Slots that no list names are not read.  A
     row that sees nothing is zero.  Numbers as for :func:`shared_prefix_attend`."""
-    own = dict(k_packed=k_packed, k_scale=k_scale, k_zero=k_zero, v_packed=v_packed, v_scale=v_scale, v_zero=v_zero, n_packed=n_packed,
-               bits=bits, group_size=group_size, v_layout=v_layout, k_tail=k_tail, v_tail=v_tail, n_tail=n_tail)
+    own = (k_packed, k_scale, k_zero, v_packed, v_scale, v_zero, n_packed, bits, group_size, v_layout, k_tail, v_tail, n_tail)
     return _store_attend("block_sparse_attend", 0, q, None, own, scale, causal, seq_lens, 0, out, lists=(blocks, int(block_size), int(query_block)))
 
 
