@@ -668,24 +668,22 @@ int launch_span_both4(const SpanCall &c);
 
 // ---- lists of blocks
 constexpr int BLOCK_LDS = (BLOCK_UNITS + 8) * 4;   // their units, and a number a wave
-template <int BITS, int D, int WAVES>
-__global__ __launch_bounds__((64 * WAVES)) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2, D == 256 ? 1 : 2))) void blocks_few_kernel(SpanCall c, BlockLists bl) {
-    span_few_block<BITS, D, 1, WAVES, true>(c, (int)blockIdx.x, bl);
+template <int BITS, int D>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2, D == 256 ? 1 : 2))) void blocks_few_kernel(SpanCall c, BlockLists bl) {
+    span_few_block<BITS, D, 1, 4, true>(c, (int)blockIdx.x, bl);
 }
-template <int BITS, int D, int WAVES> int launch_blocks_few_of(const SpanCall &c, const BlockLists &bl) {
-    constexpr int bytes = SpanFew<BITS, D, WAVES>::LDS + BLOCK_LDS;
+template <int BITS, int D> int launch_blocks_few_of(const SpanCall &c, const BlockLists &bl) {
+    constexpr int bytes = SpanFew<BITS, D, 4>::LDS + BLOCK_LDS;
     static_assert(bytes <= 160 * 1024, "units beside the rooms");
-    const auto kernel = blocks_few_kernel<BITS, D, WAVES>;
+    const auto kernel = blocks_few_kernel<BITS, D>;
     static std::atomic<bool> allowed[64] = {};
     if (int rc = span_allow_lds((const void *)kernel, bytes, allowed)) return rc;
-    kernel<<<dim3((unsigned)(c.a.B * c.a.Hkv), (unsigned)c.osplits, (unsigned)(bl.tiles * bl.row_tiles)), 64 * WAVES, bytes, (hipStream_t)c.a.stream>>>(c, bl);
+    kernel<<<dim3((unsigned)(c.a.B * c.a.Hkv), (unsigned)c.osplits, (unsigned)(bl.tiles * bl.row_tiles)), 256, bytes, (hipStream_t)c.a.stream>>>(c, bl);
     VQ_HIP_CHECK_LAUNCH("attention over blocks");
     return VQ_OK;
 }
 template <int BITS> int launch_blocks_few_as(const SpanCall &c, const BlockLists &bl) {
-    if (c.a.D == 256) return launch_blocks_few_of<BITS, 256, 4>(c, bl);
-    if (c.a.D == 64) return c.owaves == 8 ? launch_blocks_few_of<BITS, 64, 8>(c, bl) : launch_blocks_few_of<BITS, 64, 4>(c, bl);
-    return c.owaves == 8 ? launch_blocks_few_of<BITS, 128, 8>(c, bl) : launch_blocks_few_of<BITS, 128, 4>(c, bl);
+    return c.a.D == 256 ? launch_blocks_few_of<BITS, 256>(c, bl) : c.a.D == 64 ? launch_blocks_few_of<BITS, 64>(c, bl) : launch_blocks_few_of<BITS, 128>(c, bl);
 }
 
 #define VQ_SPAN_FEW_LAUNCHER(NAME, BITS)                                                                                \

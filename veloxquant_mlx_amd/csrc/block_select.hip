@@ -125,7 +125,7 @@ template <typename T, bool WIDE, int RW> __global__ __launch_bounds__(256) void 
             x += __shfl_xor(x, 2);
             x += __shfl_xor(x, 4);
             const int row = r0 + r;
-            if (row < rows && u * g < sel_end(a, live, pos0 + row / G)) best = max_key(best, pick_key(x));
+            if (row < rows && u < groups && u * g < sel_end(a, live, pos0 + row / G)) best = max_key(best, pick_key(x));
         }
     }
     if (part == 0 && u < groups) c.stored[(int64_t)item * c.groups + u] = best;
@@ -160,7 +160,7 @@ __device__ __forceinline__ u32 low3(u32 x, u32 y, u32 z) {
 // largest, is off by less than D 2^-23 of the magnitudes' sum: the scores by (D + 16) 2^-23 A, A = sum |q| (|z| + L |s|), which the wave forms too, by a third product: the choice knows how far to trust the scores (with A
 // bounded by the largest sum of |q| times the largest |z| + L |s| it asked 64 bits for 3 to 5 blocks a tile).  Bound by the bytes of the scales and zeros for one query a sequence.
 // Zeros and scales come asynchronously, in whole stretches of 1 KB, into the wave's ring, the next unit's ahead (as loads of a lane's own operands they touch a
-// cache line in four instructions: 16 sequences at 32k 27 us, this .. us); pieces of a row lie rotated by the row, so that the lanes that read them
+// cache line in four instructions: 16 sequences at 32k 27 us, and 21.5 so); pieces of a row lie rotated by the row, so that the lanes that read them
 // spread over the banks.
 template <int D> struct BoundRing { static constexpr int HALF = 64 * D, BYTES = 2 * HALF, COPIES = HALF / 1024; };   // a wave's: zeros, scales of 32 groups
 
@@ -423,7 +423,6 @@ __device__ __forceinline__ uint64_t exact_key(const SelectCall &c, int b, int hk
 constexpr int PICK_MOST = 16384;   // blocks whose scores are held in LDS
 constexpr int ONE_SCORES = 20 * 1024;   // bytes of scores beside the rings of eight waves
 constexpr int PICK_LIST = 512;     // blocks that are told apart in 64 bits there
-
 
 template <int THREADS> struct PickRoom {
     static constexpr int WAVES = THREADS / 64;
