@@ -106,6 +106,19 @@ def test_scores_a_hair_apart():
     assert torch.equal(got.flatten().long(), up.sort().values)
 
 
+@pytest.mark.parametrize("D", [128, 80])
+def test_float32_scores_a_hair_apart(D):
+    require_gpu()
+    q, scale, zero = _inputs(1, 4, 1, 1, D, 256, seed=9, spare=0, dtype=F32, meta=F32)
+    scale[:], zero[:] = scale[:, :, :1], zero[:, :, :1]
+    q[..., 5] = 2.0 ** -12
+    scale[..., 5], zero[..., 5] = 2.0 ** -6, 0.25
+    up = torch.randperm(256, generator=torch.Generator().manual_seed(1))[:40].cuda()
+    zero[0, 0, up, 5] = 0.25 + 2.0 ** -24      # 2^-36 of a score
+    got = _same(q, scale, zero, 40, levels=15, group_size=32, n_packed=256 * 32)
+    assert torch.equal(got.flatten().long(), up.sort().values)
+
+
 @pytest.mark.parametrize("Sq,query_block", [(1, 1), (6, 6)])
 def test_values_that_are_not_finite(Sq, query_block):
     require_gpu()

@@ -4,8 +4,8 @@
 // with a query above  sum_c max(q_c zero_c, q_c (zero_c + L scale_c)).  A block's score is the largest such bound over its groups, over
 // the query heads of the kv head and over the queries of a tile, which choose together; the bounds are what the store keeps anyway.
 //
-// Which blocks are chosen must not hang on the order of a sum, so scores are formed in 64 bits: products of two 24-bit numbers and a
-// code are exact there, and the sum of a head's channels is good to 1e-15 of its terms.  Equal scores: the lower block first.
+// Which blocks are chosen must not hang on the order of a sum, so scores are formed in 64 bits: the sum of a head's channels is good to
+// 1e-15 of its terms.  Equal scores: the lower block first.
 //
 // The chosen ones come out in ascending order, -1 behind them where fewer are visible: the first `first` and the last `recent` visible
 // blocks always, the others by score.
@@ -31,12 +31,6 @@ struct SelectCall {
     float *approx;          // [items][row_tiles][groups]
     float *bounds;          // [items][row_tiles][runs]
 };
-
-__device__ __forceinline__ float sel_ld(const void *p, int tag, int64_t i) {
-    if (tag == VQ_F16) return (float)((const f16 *)p)[i];
-    if (tag == VQ_BF16) return bf16_to_f32(((const u16 *)p)[i]);
-    return ((const float *)p)[i];
-}
 
 // Live slots of a sequence, and of the packed ones those [0, end) that its query i sees (slots and queries: below 2^30).
 __device__ __forceinline__ int sel_live(const vq_block_select_args &a, int b) {
@@ -67,15 +61,21 @@ __device__ __forceinline__ double key_score(uint64_t k) { return __longlong_as_d
 
 // Float32 queries, scales or zeros, and head sizes that the matrix units do not take: every group's score in 64 bits, on the vector units.
 //
-// Eight lanes a group, each with four channels of every 32, and RW rows at a time, whose queries lie in LDS as doubles; the products y z and y s of
-// a channel are formed in double, where they are exact: two conversions a channel and six instructions a row.  WIDE: four channels a load.
+// Eight lanes a group, each with four channels of every 32, all of them asked for ahead of the queries, of which RW rows at a time lie in LDS as
+// doubles.  With a group's middle and half width in a channel, m = z + L s / 2 and w = L |s| / 2, the bound is sum y m + |y| w: two
+// multiply-adds a channel and row, where the larger of two products takes six instructions (13.3 us, and 15.1).  What is not finite leaves no finite sum, and is done
+// again by the products.  WIDE: four channels a load.
 constexpr int SCORE_GROUPS = 32;   // a block of threads
 template <typename T, bool WIDE, int RW> __global__ __launch_bounds__(256) void group_score_kernel(SelectCall c) {
+    constexpr int STEPS = 4;   // of 32 channels, at once
     extern __shared__ double qs[];   // [RW][D, up to whole 32s]
     const vq_block_select_args &a = c.a;
     const int tid = threadIdx.x, part = tid & 7;
-    const u32 many = (u32)((c.groups + SCORE_GROUPS - 1) / SCORE_GROUPS), item = blockIdx.x / many, bh = item / (u32)c.tiles;
-    const int u0 = (int)(blockIdx.x % many) * SCORE_GROUPS, tile = (int)(item % (u32)c.tiles), hkv = (int)(bh % (u32)a.Hkv), b = (int)(bh / (u32)a.Hkv);
+    // (tiles outermost, so that those of a head, which read the same groups, share a cache: 5 sequences of 4 kv heads, three queries a tile
+    // of their own, 12 MB of float32 12.4 us; head by head 13.3)
+    const u32 many = (u32)((c.groups + SCORE_GROUPS - 1) / SCORE_GROUPS), heads = (u32)a.B * (u32)a.Hkv, id = blockIdx.x / many, bh = id % heads;
+    const int u0 = (int)(blockIdx.x % many) * SCORE_GROUPS, tile = (int)(id / heads), hkv = (int)(bh % (u32)a.Hkv), b = (int)(bh / (u32)a.Hkv);
+    const int64_t item = (int64_t)bh * c.tiles + tile;
     const int live = sel_live(a, b), G = (int)a.Hq / (int)a.Hkv, D = (int)a.D, room = (D + 31) / 32 * 32, g = a.group, pos0 = tile * (int)c.query_block,
               last = sel_last(a, tile), groups = (sel_end(a, live, last) + g - 1) / g;   // that some row sees
     if (u0 >= groups) return;
@@ -83,52 +83,94 @@ template <typename T, bool WIDE, int RW> __global__ __launch_bounds__(256) void 
     const int64_t at = ((int64_t)bh * c.stride + (u < groups ? u : groups - 1)) * D;   // (past the last group: it again)
     const T *const zero = (const T *)a.k_zero + at, *const scale = (const T *)a.k_scale + at;
     struct alignas(4 * sizeof(T)) Four { T v[4]; };
+    const double levels = (double)a.levels, half = 0.5 * levels;
     uint64_t best = 0;   // (no score's key)
+#pragma unroll 1
     for (int r0 = 0; r0 < rows; r0 += RW) {
-        __syncthreads();
-        for (int i = tid; i < RW * room; i += 256) {
-            const int row = i / room, d = i - row * room, x = r0 + row < rows ? r0 + row : rows - 1;
-            qs[i] = d < D ? sel_ld(a.q, a.dtype, (((int64_t)b * a.Hq + hkv * G + x % G) * a.Sq + pos0 + x / G) * D + d) : 0.f;
-        }
-        __syncthreads();
-        double sum[RW], pos[RW];
+        if (r0 > 0) __syncthreads();
+        Four z[STEPS], t[STEPS];
+        auto load = [&](int from) __attribute__((always_inline)) {
 #pragma unroll
-        for (int r = 0; r < RW; ++r) sum[r] = pos[r] = 0.;
-#pragma unroll 4
-        for (int d = part * 4; d < D; d += 32) {
-            Four z, t;
-            if constexpr (WIDE) {
-                z = *(const Four *)(zero + d);
-                t = *(const Four *)(scale + d);
-            } else {
+            for (int k = 0; k < STEPS; ++k) {
+                const int d = from + part * 4 + 32 * k;
+                if (WIDE && d < D) {
+                    z[k] = *(const Four *)(zero + d);
+                    t[k] = *(const Four *)(scale + d);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        z[k].v[e] = d + e < D ? zero[d + e] : (T)0.f;
+                        t[k].v[e] = d + e < D ? scale[d + e] : (T)0.f;
+                    }
+                }
+            }
+        };
+        load(0);
+        auto fill = [&](auto value) __attribute__((always_inline)) {
+            float y[RW];
+#pragma unroll
+            for (int r = 0; r < RW; ++r) {
+                const int x = r0 + r < rows ? r0 + r : rows - 1;
+                y[r] = tid < D ? value((((int64_t)b * a.Hq + hkv * G + x % G) * a.Sq + pos0 + x / G) * D + tid) : 0.f;
+            }
+            if (tid < room)
+#pragma unroll
+                for (int r = 0; r < RW; ++r) qs[r * room + tid] = (double)y[r];
+        };
+        if (a.dtype == VQ_F16) fill([&](int64_t i) { return (float)((const f16 *)a.q)[i]; });
+        else if (a.dtype == VQ_BF16) fill([&](int64_t i) { return bf16_to_f32(((const u16 *)a.q)[i]); });
+        else fill([&](int64_t i) { return ((const float *)a.q)[i]; });
+        __syncthreads();
+        double sum[RW];
+#pragma unroll
+        for (int r = 0; r < RW; ++r) sum[r] = 0.;
+#pragma unroll 1
+        for (int d0 = 0; d0 < D; d0 += 32 * STEPS) {
+            if (d0 > 0) load(d0);
+#pragma unroll
+            for (int k = 0; k < STEPS; ++k) {
+                const int d = d0 + 32 * k;
+                if (d >= D) break;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    z.v[e] = d + e < D ? zero[d + e] : (T)0.f;
-                    t.v[e] = d + e < D ? scale[d + e] : (T)0.f;
-                }
-            }
+                    const double td = (double)(float)t[k].v[e], m = __builtin_fma(half, td, (double)(float)z[k].v[e]), w = half * __builtin_fabs(td);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const double zd = (double)(float)z.v[e], td = (double)(float)t.v[e];
-#pragma unroll
-                for (int r = 0; r < RW; ++r) {
-                    const double y = qs[r * room + d + e], p = y * td;
-                    sum[r] = __builtin_fma(y, zd, sum[r]);
-                    pos[r] += p <= 0. ? 0. : p;
+                    for (int r = 0; r < RW; ++r) {
+                        const double y = qs[r * room + d + part * 4 + e];
+                        sum[r] = __builtin_fma(y, m, sum[r]);
+                        sum[r] = __builtin_fma(__builtin_fabs(y), w, sum[r]);
+                    }
                 }
             }
         }
-#pragma unroll
-        for (int r = 0; r < RW; ++r) {
-            double x = __builtin_fma((double)a.levels, pos[r], sum[r]);
+        auto take = [&](int r, double x) __attribute__((always_inline)) {
             x += __shfl_xor(x, 1);
             x += __shfl_xor(x, 2);
             x += __shfl_xor(x, 4);
             const int row = r0 + r;
             if (row < rows && u < groups && u * g < sel_end(a, live, pos0 + row / G)) best = max_key(best, pick_key(x));
+        };
+        bool odd = false;
+#pragma unroll
+        for (int r = 0; r < RW; ++r) odd = odd || !(__builtin_fabs(sum[r]) < (double)INFINITY);
+        if (__any(odd)) {
+#pragma unroll 1
+            for (int r = 0; r < RW; ++r) {
+                double s = 0., p = 0.;
+                for (int d0 = part * 4; d0 < D; d0 += 32)
+                    for (int d = d0; d < d0 + 4 && d < D; ++d) {
+                        const double y = qs[r * room + d], x = y * (double)(float)scale[d];
+                        s = __builtin_fma(y, (double)(float)zero[d], s);
+                        p += x <= 0. ? 0. : x;
+                    }
+                take(r, __builtin_fma(levels, p, s));
+            }
+        } else {
+#pragma unroll
+            for (int r = 0; r < RW; ++r) take(r, sum[r]);
         }
     }
-    if (part == 0 && u < groups) c.stored[(int64_t)item * c.groups + u] = best;
+    if (part == 0 && u < groups) c.stored[item * c.groups + u] = best;
 }
 
 // ---- the matrix units as a filter
