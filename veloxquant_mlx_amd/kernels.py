@@ -1892,10 +1892,14 @@ def norm_rotary_embed(q: torch.Tensor, k: torch.Tensor | None = None, *, q_weigh
 def _norm_weight(name, w, x, what):
     """A norm's weight, contiguous; its address, the elements between heads' rows (0: one for all) and its type."""
     shape, rows = w.shape, x.shape
-    if len(rows) != 4 or w.get_device() != x.get_device() or shape[-1:] != rows[3:] or (len(shape) != 1 and shape != (rows[1], rows[3])):
+    one = len(shape) == 1
+    if len(rows) != 4 or (shape[0] != rows[3] if one else shape != (rows[1], rows[3])) or w.get_device() != x.get_device():
         raise ValueError(f"{name}: the weight for {what} must be [D] or [H, D] of its {tuple(rows)} on {x.device}, got {tuple(shape)} on {w.device}")
     w = w.contiguous()
-    return w, w.data_ptr(), 0 if len(shape) == 1 else rows[3], _ftag(name, w)
+    return w, w.data_ptr(), 0 if one else rows[3], _ftag(name, w)
+
+
+_empty_like, _ROWS = torch.empty_like, torch.contiguous_format
 
 
 def _rotary_rows(name, q, k, inv_freq, offset, positions, traditional, attention_factor, inverse, out, k_out, norm=None, keep=()):
@@ -1909,9 +1913,11 @@ def _rotary_rows(name, q, k, inv_freq, offset, positions, traditional, attention
         _need_gpu(name, q, inv_freq, *(() if k is None else (k,)))
     B, Hq, S, D = q.shape
     tag = _ftag(name, q)
-    if k is not None and (k.dtype != dtype or k.device != device or k.shape[0] != B or k.shape[2] != S or k.shape[3] != D):
+    here = q.get_device()
+    if k is not None and (k.dtype != dtype or k.get_device() != here or k.shape != (B, k.shape[1], S, D)):
         raise ValueError(f"{name}: k must be [{B}, H, {S}, {D}] in {dtype} on {device}, got {tuple(k.shape)} in {k.dtype} on {k.device}")
-    if inv_freq.ndim != 1 or inv_freq.dtype not in (torch.float64, torch.float32) or inv_freq.device != device:
+    wide_freq = inv_freq.dtype == torch.float64
+    if inv_freq.ndim != 1 or not (wide_freq or inv_freq.dtype == torch.float32) or inv_freq.get_device() != here:
         raise ValueError(f"{name}: inv_freq must be float64 or float32 [dims / 2] on {device}")
     dims = 2 * inv_freq.shape[0]
     if not 2 <= dims <= D:
@@ -1933,15 +1939,15 @@ def _rotary_rows(name, q, k, inv_freq, offset, positions, traditional, attention
         at_b = at.stride(0) if at.numel() > 1 else 0
     else:
         first = int(offset)
-    if at is not None and (at.dtype not in (torch.int32, torch.int64) or at.device != device):
+    if at is not None and (at.dtype not in (torch.int32, torch.int64) or at.get_device() != here):
         raise ValueError(f"{name}: positions and offsets must be int32 or int64 on {device}, got {at.dtype} on {at.device}")
 
     def rows_of(t, o, what):
         """The rows as the library takes them and their output, new or checked."""
-        if t.stride(3) != 1 and D > 1:
+        if D > 1 and t.stride(3) != 1:
             t = t.contiguous()
         if o is None:
-            o = torch.empty_like(t, memory_format=torch.contiguous_format)
+            o = _empty_like(t, memory_format=_ROWS)
         elif o.shape != t.shape or o.dtype != dtype or o.device != device or (D > 1 and o.stride(3) != 1):
             raise ValueError(f"{name}: the output for {what} must be {tuple(t.shape)} in {dtype} on {device} with adjacent channels")
         elif not _rows_apart(o):
@@ -1975,7 +1981,7 @@ def _rotary_rows(name, q, k, inv_freq, offset, positions, traditional, attention
     try:
         args = _lib.ROTARY_PACK.pack(
             q.data_ptr(), kp, out.data_ptr(), kop, Hq, Hk, qb, qh, qs, kb, kh, ks, pb, ph, ps, ob, oh, os_, B, S, D, dims,
-            inv_freq.data_ptr(), 0 if at is None else at.data_ptr(), at_b, at_s, first, tag, VQ_F64 if inv_freq.dtype == torch.float64 else VQ_F32,
+            inv_freq.data_ptr(), 0 if at is None else at.data_ptr(), at_b, at_s, first, tag, VQ_F64 if wide_freq else VQ_F32,
             VQ_I64 if at is None or at.dtype == torch.int64 else VQ_I32, add_index, 1 if traditional else 0, 1 if inverse else 0,
             attention_factor)
     except (_lib.struct.error, OverflowError) as e:
