@@ -75,6 +75,21 @@ def test_other_stores(kw):
         _case(2, 6, 2, D, own, block, 4, Sq, query_block, group=group, **kw)
 
 
+@pytest.mark.parametrize("Hq,Hkv,Sq,query_block", [(8, 2, 70, 16), (12, 4, 33, 5), (2, 2, 40, 40), (20, 1, 3, 1)])
+@pytest.mark.parametrize("kw", [
+    dict(D=128, bits=8), dict(D=256, bits=8, dtype=BF16), dict(D=80, group=16, block=48, dtype=F32), dict(D=17, group=8, block=8, bits=5, own=(480, 37)),
+    dict(D=200, v_layout="channel", bits=6, own=(480, 45)), dict(D=1, group=1, block=5, meta=F32, bits=8)])
+def test_tiles_over_other_stores(Hq, Hkv, Sq, query_block, kw):
+    require_gpu()
+    kw = dict(dict(own=(512, 75), block=64, group=32), **kw)
+    D, own, block, group = (kw.pop(x) for x in ("D", "own", "block", "group"))
+    if kw.get("v_layout", "token") == "token" and own[0] % (32 // kw.get("bits", 4)):
+        own = (480, own[1])
+    for lens in (None, [0, 90, own[0], 9999]):
+        for causal in (True, False):
+            _case(4, Hq, Hkv, D, own, block, 7, Sq, query_block, group=group, lens=lens, causal=causal, seed=Sq, **kw)
+
+
 @pytest.mark.parametrize("D,bits,dtype", [(128, 4, F16), (128, 2, BF16), (256, 4, F16), (64, 2, F16), (96, 4, F16), (128, 4, F32)])
 @pytest.mark.parametrize("Sq,query_block", [(1, 1), (9, 4)])
 def test_lengths_and_rows_that_see_nothing(D, bits, dtype, Sq, query_block):

@@ -5,74 +5,249 @@
 // the store name nothing, an entry that is named twice counts twice.  Behind them come the plain rows (the tail), up to the query's own
 // place.  o = sum p v / sum p, p = exp(scale q k - max) over what it sees; a row that sees nothing is zero.
 #include "attend_blocks.hpp"
+#include "attend_span_mfma.hpp"
 
 namespace vq {
 
 namespace {
 
-// Any head size up to 256, type, bit width, layout and strides, in float32 on the vector units: a wave takes a query row over a run
-// of its list's entries and a run of its tail, lanes along the channels.
-__global__ __launch_bounds__(256) void blocks_any_kernel(BlockCall c) {
-    constexpr int E = SPAN_MAX_D / 64;
+// Any head size up to 256, type, bit width, layout and strides, in float32: a block of four waves takes 16 RT rows of a kv head's query heads at the
+// positions of one list, over a run of units of 32 slots, the list's slots in one line and then the tail's.  A unit's slots are looked up by one wave,
+// reconstructed by all threads, a channel each, and laid down in LDS as float32 once for all rows; scores and sums are products of float32 numbers
+// (v_mfma_f32_16x16x4: lane i + 16 h holds row or column i of step h, and rows 4 h .. 4 h + 3 of column i of the result; a lane's four channels or
+// slots in a row are those of four steps, any order serving a sum), the softmax has TPR threads a row.
+//
+// Bound by reconstruction and by the waits between a unit's five barriers: 16 sequences of 8 kv heads, 3.2k of 8-bit slots each, 214 us; a chunk of 512 queries
+// in 64 lists of 2k slots 682 (a wave a row, each with its own reconstruction: 1891 and 33827).
+constexpr int ANY_SP = 36;          // floats from row to row of the scores
+constexpr int ANY_INFO = 4 * 32 + 4;   // ints about a unit
+template <int RT> constexpr size_t any_bytes(int D) {
+    const int kp = (D + 15) / 16 * 16 + 4;
+    return (size_t)((16 * RT + 64) * kp + (3 - RT) * 16 * RT * ANY_SP + 16 * RT + 2 * ANY_INFO) * 4;
+}
+template <int RT> __global__ __launch_bounds__(256) void blocks_any_kernel(BlockCall c) {
+    constexpr int ROWS = 16 * RT, TPR = 256 / ROWS, SPT = 32 / TPR, HALVES = 3 - RT;   // (16 rows: two waves share a tile of scores, half of the channels each)
+    extern __shared__ __align__(16) float any_lds[];
     const vq_store_attend_args &a = c.s.a;
-    const int lane = threadIdx.x & 63;
-    const int64_t wid = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (wid >= a.B * a.Hq * a.Sq * c.s.nparts) return;   // whole waves leave together
-    const int64_t row = wid / c.s.nparts, part = wid % c.s.nparts;
-    const int64_t pos = row % a.Sq, h = row / a.Sq % a.Hq, b = row / (a.Sq * a.Hq);
-    const int64_t hkv = h / (a.Hq / a.Hkv), D = a.D, bh = b * a.Hkv + hkv;
-    int64_t lo, hi;
-    span_visible(a, span_own_live(a, b), pos, lo, hi);
-    const float scale = a.scale * LOG2E;
-    const int32_t *list = c.blocks + (bh * c.tiles + pos / c.query_block) * c.count;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i = lane & 15, h = lane >> 4;
+    const int D = (int)a.D, Dp = (D + 15) / 16 * 16, KP = Dp + 4, steps = Dp / 16, G = (int)(a.Hq / a.Hkv), n_packed = (int)a.own.n_packed;
+    float *const Qs = any_lds, *const Ks = Qs + ROWS * KP, *const Vs = Ks + 32 * KP, *const Sb = Vs + 32 * KP, *const keeps = Sb + HALVES * ROWS * ANY_SP;
+    int *const infos = (int *)(keeps + ROWS);
+    u32 id = blockIdx.x;
+    const int part = (int)(id % (u32)c.s.nparts);
+    id /= (u32)c.s.nparts;
+    const int j0 = (int)(id % (u32)c.row_tiles) * ROWS;
+    id /= (u32)c.row_tiles;
+    const int tile = (int)(id % (u32)c.tiles);
+    const int64_t bh = id / (u32)c.tiles, b = bh / a.Hkv, hkv = bh % a.Hkv;
+    const int pos0 = (int)(tile * c.query_block), at_once = (int)(a.Sq - pos0 < c.query_block ? a.Sq - pos0 : c.query_block);
+    const int here = at_once * G - j0 < ROWS ? at_once * G - j0 : ROWS;
+    if (here <= 0) return;   // (the last tile may hold fewer rows)
+    auto row_of = [&](int x) __attribute__((always_inline)) { return (b * a.Hq + hkv * G + (j0 + x) % G) * a.Sq + pos0 + (j0 + x) / G; };
+    const int64_t live = span_own_live(a, b);
+    int64_t lo, hi, any_hi;
+    const int mine = tid / TPR < here ? tid / TPR : here - 1;   // the row of this thread's softmax
+    span_visible(a, live, pos0 + (j0 + mine) / G, lo, hi);
+    span_visible(a, live, pos0 + (j0 + here - 1) / G, lo, any_hi);
+    const int limit = (int)(any_hi < n_packed ? any_hi : n_packed);
 
-    float q[E], acc[E], m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const int64_t d = lane + 64 * e;
-        q[e] = d < D ? span_ld(a.q, a.dtype, row * D + d) : 0.f;
-        acc[e] = 0.f;
-    }
+    // ---- a channel and every step-th row or slot a thread
+    const int step = 256 / Dp, d = tid % Dp, s0 = tid < step * Dp ? tid / Dp : 32, dd = d < D ? d : D - 1;
+    for (int x = s0; x < ROWS; x += step) Qs[x * KP + d] = x < here && d < D ? span_ld(a.q, a.dtype, row_of(x) * D + d) : 0.f;
     const SpanPacked p = SpanPacked::of(a, a.own);
-    auto take = [&](int64_t t) {
-        float v[E], dot = 0.f;
+    const bool token = a.v_layout == VQ_V_TOKEN_PACKED;
+    const int kd = dd / p.per, kshift = dd % p.per * p.bits, vg = dd / p.group;
+    const int64_t kwords = bh * a.own.cap_tokens, kmeta = bh * p.GK, vwords = token ? bh * (a.own.cap_tokens / p.per) : kwords, vmeta = (bh * p.GV + vg) * a.own.cap_tokens;
+    // a unit's packed slots, its places in `info`: slots (or another of the unit where there is none), groups, rows of words, shifts
+    auto packed = [&](const int *info, u32 there, auto meta) __attribute__((always_inline)) {
+        using T = decltype(meta);
+        const T *const ksc = (const T *)a.own.k_scale, *const kz = (const T *)a.own.k_zero, *const vsc = (const T *)a.own.v_scale, *const vz = (const T *)a.own.v_zero;
+        const u32 *const kp = (const u32 *)a.own.k_packed, *const vp = (const u32 *)a.own.v_packed;
+        constexpr int N = 4;   // slots whose words are under way
+#pragma unroll 1
+        for (int s = s0; s < 32; s += N * step) {
+            u32 kw[N], vw[N];
+            T k_s[N], k_z[N], v_s[N], v_z[N];
+            int vshift[N];
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const int64_t d = lane + 64 * e;
-            v[e] = 0.f;
-            if (d >= D) continue;
-            float k;
-            if (t < a.own.n_packed) {
-                k = p.key(bh, t, d);
-                v[e] = p.value(bh, t, d);
-            } else {
-                const int64_t r = t - a.own.n_packed;
-                k = span_ld(a.own.k_tail, a.tail_dtype, b * a.own.k_strides[0] + hkv * a.own.k_strides[1] + r * a.own.k_strides[2] + d);
-                v[e] = span_ld(a.own.v_tail, a.tail_dtype, b * a.own.v_strides[0] + hkv * a.own.v_strides[1] + r * a.own.v_strides[2] + d);
+            for (int j = 0; j < N; ++j) {
+                const int x = s + j * step < 32 ? s + j * step : s, t = info[x];
+                kw[j] = kp[(kwords + t) * p.W + kd];
+                const int64_t km = (kmeta + info[32 + x]) * D + dd;
+                k_s[j] = ksc[km];
+                k_z[j] = kz[km];
+                vw[j] = token ? vp[(vwords + info[64 + x]) * D + dd] : vp[(vwords + t) * p.W + kd];
+                vshift[j] = token ? info[96 + x] : kshift;
+                const int64_t vm = token ? vmeta + t : (kwords + t) * p.GV + vg;
+                v_s[j] = vsc[vm];
+                v_z[j] = vz[vm];
             }
-            dot = __builtin_fmaf(q[e], k, dot);
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const int x = s + j * step;
+                if (x >= 32) break;
+                const bool is = d < D && there >> x & 1;
+                const float k = (float)(f16)__builtin_fmaf((float)(kw[j] >> kshift & p.mask), (float)k_s[j], (float)k_z[j]);
+                const float v = (float)(f16)__builtin_fmaf((float)(vw[j] >> vshift[j] & p.mask), (float)v_s[j], (float)v_z[j]);
+                Ks[x * KP + d] = is ? k : 0.f;
+                Vs[x * KP + d] = is ? v : 0.f;
+            }
         }
-        const float x = span_wave_sum(dot) * scale, mn = fmaxf(m, x);
-        const float keep = mn == -INFINITY ? 1.f : exp2f(m - mn), y = mn == -INFINITY && x == x ? 0.f : exp2f(x - mn);
-        l = l * keep + y;
-        m = mn;
-#pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] = __builtin_fmaf(y, v[e], acc[e] * keep);
     };
-    const int64_t packed = hi < a.own.n_packed ? hi : a.own.n_packed;
-    for (int64_t i = c.count * part / c.s.nparts; i < c.count * (part + 1) / c.s.nparts; ++i) {
-        const int64_t t0 = (int64_t)list[i] * c.block_tokens;
-        if (t0 < 0) continue;
-        const int64_t t1 = t0 + c.block_tokens < packed ? t0 + c.block_tokens : packed;
-        for (int64_t t = t0; t < t1; ++t) take(t);
-    }
-    const int64_t n = hi > a.own.n_packed ? hi - a.own.n_packed : 0;
-    for (int64_t t = n * part / c.s.nparts; t < n * (part + 1) / c.s.nparts; ++t) take(a.own.n_packed + t);
-    const int64_t rec = row * c.s.nparts + part;
-    if (lane == 0) { c.s.ml[rec * 2] = m; c.s.ml[rec * 2 + 1] = l; }
+    auto mixed = [&](const int *info, u32 there) __attribute__((always_inline)) {
+#pragma unroll 2
+        for (int x = s0; x < 32; x += step) {
+            float k = 0.f, v = 0.f;
+            if (d < D && there >> x & 1) {
+                const int t = info[x], r = t - n_packed;
+                if (r < 0) {
+                    k = p.key(bh, t, d);
+                    v = p.value(bh, t, d);
+                } else {
+                    k = span_ld(a.own.k_tail, a.tail_dtype, b * a.own.k_strides[0] + hkv * a.own.k_strides[1] + r * a.own.k_strides[2] + d);
+                    v = span_ld(a.own.v_tail, a.tail_dtype, b * a.own.v_strides[0] + hkv * a.own.v_strides[1] + r * a.own.v_strides[2] + d);
+                }
+            }
+            Ks[x * KP + d] = k;
+            Vs[x * KP + d] = v;
+        }
+    };
+
+    const float scale = a.scale * LOG2E;
+    const int32_t *const list = c.blocks + (bh * c.tiles + tile) * c.count;
+    const u32 sub = (u32)c.sub;
+    float m = -INFINITY, l = 0.f;
+    f32x4 acc[4][RT];   // of 16 channels each, every fourth a wave
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-        if (lane + 64 * e < D) c.s.sums[rec * D + lane + 64 * e] = acc[e];
+    for (int y = 0; y < 4; ++y)
+#pragma unroll
+        for (int r = 0; r < RT; ++r) acc[y][r] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int64_t run = c.units / c.s.nparts, longer = c.units % c.s.nparts, u0 = part * run + (part < longer ? part : longer);   // (the first runs a unit longer)
+    const int64_t u1 = u0 + run + (part < longer ? 1 : 0);
+#pragma unroll 1
+    for (int64_t u = u0; u < u1; ++u) {
+        int *const info = infos + (int)(u & 1) * ANY_INFO;   // (two in turn: a unit that holds nothing is left without another barrier)
+        if (wave == 0) {
+            const int64_t at = u * 32 + (lane & 31);
+            int t = -1;
+            if (at < c.list_slots) {
+                const int64_t e = c.list_slots >> 32 == 0 ? (int64_t)((u32)at / sub) : at / sub;
+                const int64_t slot = (int64_t)list[e] * c.block_tokens + (at - e * sub);
+                if (slot >= 0 && slot < limit) t = (int)slot;
+            } else if (n_packed + (at - c.list_slots) < any_hi) {   // (what the last row sees lies within the store)
+                t = n_packed + (int)(at - c.list_slots);
+            }
+            const u32 there = (u32)__ballot(t >= 0), tail = (u32)__ballot(t >= n_packed);
+            if (there != 0) t = t >= 0 ? t : __shfl(t, __builtin_ctz(there));
+            if (lane < 32 && there != 0) {
+                info[lane] = t;
+                info[32 + lane] = (int)((u32)t / (u32)p.group);
+                info[64 + lane] = (int)((u32)t / (u32)p.per);
+                info[96 + lane] = (int)((u32)t % (u32)p.per) * p.bits;
+            }
+            if (lane == 0) { info[128] = (int)there; info[129] = tail != 0; }
+        }
+        __syncthreads();
+        const u32 there = (u32)__builtin_amdgcn_readfirstlane(info[128]);
+        if (there == 0) continue;
+        if (__builtin_amdgcn_readfirstlane(info[129])) mixed(info, there);
+        else if (a.meta_dtype == VQ_F16) packed(info, there, (f16)0.f);
+        else packed(info, there, 0.f);
+        // (a unit's own slots, for the softmax behind the next barrier)
+        __syncthreads();
+        {
+            const int rt = RT == 2 ? wave & 1 : 0, st = RT == 2 ? wave >> 1 : wave & 1, half = RT == 2 ? 0 : wave >> 1;
+            const int k0 = half ? steps / 2 : 0, k1 = RT == 2 || half ? steps : steps / 2;
+            f32x4 S = {0.f, 0.f, 0.f, 0.f};
+            const float *const x = Qs + (rt * 16 + i) * KP + 4 * h, *const y = Ks + (st * 16 + i) * KP + 4 * h;
+#pragma unroll 2
+            for (int k = k0; k < k1; ++k) {
+                const f32x4 x4 = *(const f32x4 *)(x + 16 * k), y4 = *(const f32x4 *)(y + 16 * k);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) S = __builtin_amdgcn_mfma_f32_16x16x4f32(x4[e], y4[e], S, 0, 0, 0);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) Sb[(half * ROWS + rt * 16 + 4 * h + r) * ANY_SP + st * 16 + i] = S[r];
+        }
+        __syncthreads();
+        {
+            float *const s = Sb + tid / TPR * ANY_SP + tid % TPR * SPT;
+            float x[SPT], top = m;
+#pragma unroll
+            for (int j = 0; j < SPT; ++j) {
+                const int at = tid % TPR * SPT + j;
+                x[j] = (HALVES == 2 ? s[j] + s[ROWS * ANY_SP + j] : s[j]) * scale;
+                if (!(there >> at & 1) || info[at] >= hi) x[j] = -INFINITY;
+                top = fmaxf(top, x[j]);
+            }
+#pragma unroll
+            for (int off = 1; off < TPR; off <<= 1) top = fmaxf(top, __shfl_xor(top, off));
+            const float keep = top == -INFINITY ? 1.f : exp2f(m - top);
+            l *= keep;
+#pragma unroll
+            for (int j = 0; j < SPT; ++j) {
+                const float y = top == -INFINITY && x[j] == x[j] ? 0.f : exp2f(x[j] - top);
+                l += y;
+                s[j] = y;
+            }
+            m = top;
+            if (tid % TPR == 0) keeps[tid / TPR] = keep;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            const f32x4 keep = *(const f32x4 *)(keeps + r * 16 + 4 * h);
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[y][r][e] *= keep[e];
+        }
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            f32x4 w[RT];
+#pragma unroll
+            for (int r = 0; r < RT; ++r) w[r] = *(const f32x4 *)(Sb + (r * 16 + i) * ANY_SP + 16 * g + 4 * h);
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+                const int ct = wave + 4 * y;
+                if (ct >= steps) break;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float v = Vs[(16 * g + 4 * h + e) * KP + ct * 16 + i];
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) acc[y][r] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[r][e], v, acc[y][r], 0, 0, 0);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int off = 1; off < TPR; off <<= 1) l += __shfl_xor(l, off);
+    if (tid % TPR == 0 && tid / TPR < here) {
+        float *const ml = c.s.ml + (row_of(tid / TPR) * c.s.nparts + part) * 2;
+        ml[0] = m;
+        ml[1] = l;
+    }
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int x = r * 16 + 4 * h + e;
+            if (x >= here) continue;
+            float *const sums = c.s.sums + (row_of(x) * c.s.nparts + part) * D;
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+                if ((wave + 4 * y) * 16 + i < D) sums[(wave + 4 * y) * 16 + i] = acc[y][r][e];
+        }
+}
+
+template <int RT> int launch_blocks_any(const char *fn, const BlockCall &c, int64_t blocks) {
+    const size_t bytes = any_bytes<RT>((int)c.s.a.D);
+    static std::atomic<bool> allowed[64] = {};
+    if (bytes > 64 * 1024)
+        if (int rc = span_allow_lds((const void *)blocks_any_kernel<RT>, (int)any_bytes<RT>(SPAN_MAX_D), allowed)) return rc;
+    blocks_any_kernel<RT><<<(unsigned)blocks, 256, bytes, (hipStream_t)c.s.a.stream>>>(c);
+    VQ_HIP_CHECK_LAUNCH(fn);
+    return VQ_OK;
 }
 
 int check_blocks(const char *fn, const vq_block_attend_args *args) {
@@ -128,12 +303,16 @@ BlockCall cut_blocks(const vq_block_attend_args &args) {
     const vq_store_attend_args &a = c.s.a;
     c.tiles = cdiv(a.Sq, c.query_block);
     if (plan_few(c, args)) return c;
-    // as many waves as fill the chip eight deep, runs of 64 slots or more
-    const int64_t rows = a.B * a.Hq * a.Sq;
-    double slots = (double)c.count * (double)c.block_tokens;
-    slots = (slots < (double)a.own.n_packed ? slots : (double)a.own.n_packed) + (double)a.own.n_tail;
-    int64_t parts = 8192 / rows;
-    if ((double)parts > slots / 64.) parts = (int64_t)(slots / 64.);
+    // two blocks a CU, four units or more a run
+    const int64_t G = a.Hq / a.Hkv;
+    if (c.query_block > a.Sq) c.query_block = a.Sq;
+    c.rows16 = G * c.query_block > 16 ? 2 : 1;
+    c.row_tiles = (int)cdiv(G * c.query_block, 16 * c.rows16);
+    c.sub = c.block_tokens < a.own.n_packed ? c.block_tokens : a.own.n_packed;
+    c.list_slots = c.count * c.sub;
+    c.units = cdiv(c.list_slots + a.own.n_tail, 32);
+    int64_t parts = cdiv(512, a.B * a.Hkv * c.tiles * c.row_tiles);
+    if (parts > c.units / 4) parts = c.units / 4;
     c.s.nparts = (int)(parts < 1 ? 1 : parts);
     return c;
 }
@@ -182,7 +361,7 @@ extern "C" int vq_block_attend(const vq_block_attend_args *args) {
         if (int rc = a.pack_bits == 4 ? launch_blocks_few4(c.s, c.lists) : launch_blocks_few2(c.s, c.lists)) return rc;
         return need > 0 && c.lists.counters == nullptr ? launch_span_merge1(fn, c.s) : VQ_OK;
     }
-    blocks_any_kernel<<<(unsigned)cdiv(a.B * a.Hq * a.Sq * c.s.nparts, 4), 256, 0, (hipStream_t)a.stream>>>(c);
-    VQ_HIP_CHECK_LAUNCH(fn);
+    const int64_t blocks = a.B * a.Hkv * c.tiles * c.row_tiles * c.s.nparts;   // (no more than query rows, or 1024)
+    if (int rc = c.rows16 == 2 ? launch_blocks_any<2>(fn, c, blocks) : launch_blocks_any<1>(fn, c, blocks)) return rc;
     return launch_span_merge1(fn, c.s);
 }

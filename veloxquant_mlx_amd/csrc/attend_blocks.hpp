@@ -11,6 +11,10 @@ struct BlockCall {
     int64_t tiles, count, block_tokens, query_block;
     int few;                 // 1: by the matrix-unit kernel for few rows (attend_span_few.hpp), with
     BlockLists lists;
+    // 0: by blocks_any_kernel, with
+    int rows16, row_tiles;   // 16s of rows of a tile, tiles of rows of a tile of queries
+    int64_t sub;             // slots of an entry (at most the store's)
+    int64_t list_slots, units;   // of a list, units of 32 of them and of the tail's
 };
 
 int launch_blocks_few2(const SpanCall &c, const BlockLists &l);
