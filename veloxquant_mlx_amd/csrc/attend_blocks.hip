@@ -17,8 +17,10 @@ namespace {
 // (v_mfma_f32_16x16x4: lane i + 16 h holds row or column i of step h, and rows 4 h .. 4 h + 3 of column i of the result; a lane's four channels or
 // slots in a row are those of four steps, any order serving a sum), the softmax has TPR threads a row.
 //
-// Bound by reconstruction and by the waits between a unit's five barriers: 16 sequences of 8 kv heads, 3.2k of 8-bit slots each, 214 us; a chunk of 512 queries
-// in 64 lists of 2k slots 682 (a wave a row, each with its own reconstruction: 1891 and 33827).
+// Bound by the latencies of a unit, one after another (its entries of the list, then its words in four batches, five barriers), with two blocks a CU to
+// cover each other: 16 sequences of 8 kv heads, 3.2k of 8-bit slots each, 214 us; a chunk of 512 queries in 64 lists of 2k slots 682 (a wave a row,
+// each with its own reconstruction: 1891 and 33827).  Eight slots' words under way in place of four take registers that the second block needs (1080);
+// a third of the loads, keys' scales shared and values' by way of LDS, is no faster (248 and 722).
 constexpr int ANY_SP = 36;          // floats from row to row of the scores
 constexpr int ANY_INFO = 4 * 32 + 4;   // ints about a unit
 template <int RT> constexpr size_t any_bytes(int D) {
@@ -95,7 +97,6 @@ template <int RT> __global__ __launch_bounds__(256) void blocks_any_kernel(Block
         }
     };
     auto mixed = [&](const int *info, u32 there) __attribute__((always_inline)) {
-#pragma unroll 2
         for (int x = s0; x < 32; x += step) {
             float k = 0.f, v = 0.f;
             if (d < D && there >> x & 1) {
@@ -160,7 +161,6 @@ template <int RT> __global__ __launch_bounds__(256) void blocks_any_kernel(Block
             const int k0 = half ? steps / 2 : 0, k1 = RT == 2 || half ? steps : steps / 2;
             f32x4 S = {0.f, 0.f, 0.f, 0.f};
             const float *const x = Qs + (rt * 16 + i) * KP + 4 * h, *const y = Ks + (st * 16 + i) * KP + 4 * h;
-#pragma unroll 2
             for (int k = k0; k < k1; ++k) {
                 const f32x4 x4 = *(const f32x4 *)(x + 16 * k), y4 = *(const f32x4 *)(y + 16 * k);
 #pragma unroll
@@ -303,7 +303,7 @@ BlockCall cut_blocks(const vq_block_attend_args &args) {
     const vq_store_attend_args &a = c.s.a;
     c.tiles = cdiv(a.Sq, c.query_block);
     if (plan_few(c, args)) return c;
-    // two blocks a CU, four units or more a run
+    // two blocks a CU, two units or more a run (8 kv heads, 69 units of 8-bit slots: 35 us, in runs of four 45)
     const int64_t G = a.Hq / a.Hkv;
     if (c.query_block > a.Sq) c.query_block = a.Sq;
     c.rows16 = G * c.query_block > 16 ? 2 : 1;
@@ -312,7 +312,7 @@ BlockCall cut_blocks(const vq_block_attend_args &args) {
     c.list_slots = c.count * c.sub;
     c.units = cdiv(c.list_slots + a.own.n_tail, 32);
     int64_t parts = cdiv(512, a.B * a.Hkv * c.tiles * c.row_tiles);
-    if (parts > c.units / 4) parts = c.units / 4;
+    if (parts > c.units / 2) parts = c.units / 2;
     c.s.nparts = (int)(parts < 1 ? 1 : parts);
     return c;
 }
