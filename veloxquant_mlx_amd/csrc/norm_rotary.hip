@@ -3,6 +3,10 @@
 // y_c = x_c w_c / sqrt(mean(x^2) + eps) over the D channels of a head, w the norm's weight (one row, or one a head; none: ones); then
 // channel pair i of the first `dims` turns by the angle p w_i as in rotary.hip, channels dims .. D - 1 of y pass through.  Squares, their sum
 // and the turn are float32, the angle is formed in double; a value is rounded once, to the element type.
+//
+// Bound by HBM, a read and a write of every row: 40 heads of 128 channels, 8192 tokens of a projection's view in bf16 41 us, 4.1 TB/s (a wave a row, read
+// twice: 223); 16 heads of 256, 7 x 1003 tokens, a weight row a head 25.7 us, 4.5 TB/s; one token 5.5, latency.  Four waves a SIMD by a cap on registers: 58 us in place
+// of 41.
 #include "common.hpp"
 
 namespace vq {

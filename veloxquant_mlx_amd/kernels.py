@@ -1782,7 +1782,9 @@ def block_sparse_attend(q: torch.Tensor, blocks: torch.Tensor, *, block_size: in
     list ``t`` of their kv head (entry ``e``: slots ``e * block_size`` .. ``(e + 1) * block_size - 1``), as far as these are live and, with
     ``causal``, not behind the query.  Entries may come in any order; one below zero or past the live slots names nothing, one that is
     named twice counts twice.  The plain rows of the tail are all seen, up to the query's own.  Slots that no list names are not read.  A
-    row that sees nothing is zero.  Numbers as for :func:`shared_prefix_attend`."""
+    row that sees nothing is zero.  Numbers as for :func:`shared_prefix_attend`.  2- and 4-bit stores with heads of 64, 128 or 256 channels, groups
+    of 32, 64 or 128 and values packed by token run on the matrix units where blocks are whole units of 32 slots; other stores, sizes and float32 rows
+    in float32, some ten times slower."""
     own = (k_packed, k_scale, k_zero, v_packed, v_scale, v_zero, n_packed, bits, group_size, v_layout, k_tail, v_tail, n_tail)
     return _store_attend("block_sparse_attend", 0, q, None, own, scale, causal, seq_lens, 0, out, lists=(blocks, int(block_size), int(query_block)))
 
