@@ -184,7 +184,8 @@ assert STORE_ATTEND_PACK.size == C.sizeof(StoreAttendArgs)
 ROTARY_PACK = struct.Struct("@PPPPqqqqqqqqqqqqqqqqqqPPqqqiiiiiif0q")
 assert ROTARY_PACK.size == C.sizeof(RotaryArgs)
 NORM_PACK = struct.Struct("@PPqqif")   # behind a ROTARY_PACK
-assert ROTARY_PACK.size + NORM_PACK.size == C.sizeof(NormRotaryArgs)
+NORM_ROTARY_PACK = struct.Struct(ROTARY_PACK.format + NORM_PACK.format[1:])
+assert ROTARY_PACK.size + NORM_PACK.size == NORM_ROTARY_PACK.size == C.sizeof(NormRotaryArgs)
 BLOCK_SELECT_PACK = struct.Struct("@PPPPqqqqqqqqqqqqqPPNPiiiii0q")
 assert BLOCK_SELECT_PACK.size == C.sizeof(BlockSelectArgs)
 BLOCK_LISTS_PACK = struct.Struct("@PqqqPq")   # behind a STORE_ATTEND_PACK

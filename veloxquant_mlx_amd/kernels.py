@@ -45,7 +45,8 @@ def _stream(t: torch.Tensor) -> int:
 
 def _stream_of(device: torch.device) -> int:
     if _raw_stream is not None:
-        return _raw_stream(torch.cuda.current_device() if device.index is None else device.index)
+        at = device.index
+        return _raw_stream(torch.cuda.current_device() if at is None else at)
     return torch.cuda.current_stream(device).cuda_stream
 
 
@@ -62,19 +63,22 @@ _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device
 def _launch_on(device: torch.device, call) -> None:
     """Run a library call with ``device`` as the current one (a launch goes to the current device, whose default stream has
     the same handle on every device) and raise what it returns."""
-    if device.index is None or device.index == _current_device():
+    at = device.index
+    if at is None or at == _current_device():
         rc = call()
     else:
         with torch.cuda.device(device):
             rc = call()
-    _lib.check(rc)
+    if rc:
+        _lib.check(rc)
 
 
 def _ftag(name: str, t: torch.Tensor) -> int:
-    if t.dtype not in _FLOAT_TAG:
+    tag = _FLOAT_TAG.get(t.dtype)
+    if tag is None:
         raise ValueError(f"{name}: unsupported dtype {t.dtype}; expected one of "
                          f"{sorted(str(d) for d in _FLOAT_TAG)}")
-    return _FLOAT_TAG[t.dtype]
+    return tag
 
 
 def _bytes_as_words(codes: torch.Tensor) -> torch.Tensor:
@@ -1878,53 +1882,58 @@ def norm_rotary_embed(q: torch.Tensor, k: torch.Tensor | None = None, *, q_weigh
     name = "norm_rotary_embed"
     if not 0 <= norm_eps < 1e38:
         raise ValueError(f"{name}: norm_eps={norm_eps} must be a number from 0 on")
-    q_at = q_step = k_at = k_step = tag = 0
-    if q_weight is not None:
-        q_weight, q_at, q_step, tag = _norm_weight(name, q_weight, q, "q")
-    if k_weight is not None:
-        if k is None:
-            raise ValueError(f"{name}: k_weight without k")
-        if q_weight is not None and k_weight.dtype != q_weight.dtype:
-            raise ValueError(f"{name}: q_weight and k_weight must be of one dtype, got {q_weight.dtype} and {k_weight.dtype}")
-        k_weight, k_at, k_step, tag = _norm_weight(name, k_weight, k, "k")
-    return _rotary_rows(name, q, k, inv_freq, offset, positions, traditional, attention_factor, False, out, k_out,
-                        _lib.NORM_PACK.pack(q_at, k_at, q_step, k_step, tag, norm_eps), (q_weight, k_weight))
+    if k_weight is not None and k is None:
+        raise ValueError(f"{name}: k_weight without k")
+    return _rotary_rows(name, q, k, inv_freq, offset, positions, traditional, attention_factor, False, out, k_out, (q_weight, k_weight, norm_eps))
 
 
-def _norm_weight(name, w, x, what):
+def _norm_weight(name, w, heads, channels, at, what):
     """A norm's weight, contiguous; its address, the elements between heads' rows (0: one for all) and its type."""
-    shape, rows = w.shape, x.shape
+    shape = w.shape
     one = len(shape) == 1
-    if len(rows) != 4 or (shape[0] != rows[3] if one else shape != (rows[1], rows[3])) or w.get_device() != x.get_device():
-        raise ValueError(f"{name}: the weight for {what} must be [D] or [H, D] of its {tuple(rows)} on {x.device}, got {tuple(shape)} on {w.device}")
-    w = w.contiguous()
-    return w, w.data_ptr(), 0 if one else rows[3], _ftag(name, w)
+    if (shape[0] != channels if one else shape != (heads, channels)) or w.get_device() != at:
+        raise ValueError(f"{name}: the weight for {what} must be [{channels}] or [{heads}, {channels}] on device {at}, got {tuple(shape)} on {w.device}")
+    if not w.is_contiguous():
+        w = w.contiguous()
+    return w, w.data_ptr(), 0 if one else channels, _ftag(name, w)
 
 
 _empty_like, _ROWS = torch.empty_like, torch.contiguous_format
 
 
-def _rotary_rows(name, q, k, inv_freq, offset, positions, traditional, attention_factor, inverse, out, k_out, norm=None, keep=()):
-    """``norm``: the packed fields of the norm in front of the turn, or None; ``keep``: tensors that they point into."""
+def _rotary_rows(name, q, k, inv_freq, offset, positions, traditional, attention_factor, inverse, out, k_out, norm=None):
+    """``norm``: weights of queries and keys and the epsilon of the norm in front of the turn, or None."""
     if q.ndim != 4 or (k is not None and k.ndim != 4):
         raise ValueError(f"{name}: q and k must be [B, H, S, D], got {tuple(q.shape)}" + ("" if k is None else f" and {tuple(k.shape)}"))
     if k is None and k_out is not None:
         raise ValueError(f"{name}: k_out without k")
-    device, dtype = q.device, q.dtype
-    if not (q.is_cuda and inv_freq.is_cuda and (k is None or k.is_cuda)):
-        _need_gpu(name, q, inv_freq, *(() if k is None else (k,)))
+    here, dtype = q.get_device(), q.dtype
     B, Hq, S, D = q.shape
+    if norm is not None:
+        q_weight, k_weight, eps = norm
+        q_at = q_step = k_at = k_step = weight_tag = 0
+        if q_weight is not None:
+            q_weight, q_at, q_step, weight_tag = _norm_weight(name, q_weight, Hq, D, here, "q")
+        if k_weight is not None:
+            if q_weight is not None and k_weight.dtype != q_weight.dtype:
+                raise ValueError(f"{name}: q_weight and k_weight must be of one dtype, got {q_weight.dtype} and {k_weight.dtype}")
+            k_weight, k_at, k_step, weight_tag = _norm_weight(name, k_weight, k.shape[1], D, here, "k")
+    if here < 0 or not inv_freq.is_cuda or (k is not None and not k.is_cuda):
+        _need_gpu(name, q, inv_freq, *(() if k is None else (k,)))
     tag = _ftag(name, q)
-    here = q.get_device()
-    if k is not None and (k.dtype != dtype or k.get_device() != here or k.shape != (B, k.shape[1], S, D)):
-        raise ValueError(f"{name}: k must be [{B}, H, {S}, {D}] in {dtype} on {device}, got {tuple(k.shape)} in {k.dtype} on {k.device}")
+    Hk = 0
+    if k is not None:
+        kB, Hk, kS, kD = k.shape
+        if k.dtype != dtype or k.get_device() != here or kB != B or kS != S or kD != D:
+            raise ValueError(f"{name}: k must be [{B}, H, {S}, {D}] in {dtype} on {q.device}, got {tuple(k.shape)} in {k.dtype} on {k.device}")
     wide_freq = inv_freq.dtype == torch.float64
     if inv_freq.ndim != 1 or not (wide_freq or inv_freq.dtype == torch.float32) or inv_freq.get_device() != here:
-        raise ValueError(f"{name}: inv_freq must be float64 or float32 [dims / 2] on {device}")
+        raise ValueError(f"{name}: inv_freq must be float64 or float32 [dims / 2] on {q.device}")
     dims = 2 * inv_freq.shape[0]
     if not 2 <= dims <= D:
         raise ValueError(f"{name}: {dims // 2} frequencies turn {dims} channels of {D}")
-    inv_freq = inv_freq.contiguous()
+    if not inv_freq.is_contiguous():
+        inv_freq = inv_freq.contiguous()
     at, at_b, at_s, first, add_index = None, 0, 0, 0, 1
     if positions is not None:
         if isinstance(offset, torch.Tensor):
@@ -1942,32 +1951,49 @@ def _rotary_rows(name, q, k, inv_freq, offset, positions, traditional, attention
     else:
         first = int(offset)
     if at is not None and (at.dtype not in (torch.int32, torch.int64) or at.get_device() != here):
-        raise ValueError(f"{name}: positions and offsets must be int32 or int64 on {device}, got {at.dtype} on {at.device}")
+        raise ValueError(f"{name}: positions and offsets must be int32 or int64 on {q.device}, got {at.dtype} on {at.device}")
 
-    def rows_of(t, o, what):
-        """The rows as the library takes them and their output, new or checked."""
-        if D > 1 and t.stride(3) != 1:
-            t = t.contiguous()
-        if o is None:
-            o = _empty_like(t, memory_format=_ROWS)
-        elif o.shape != t.shape or o.dtype != dtype or o.device != device or (D > 1 and o.stride(3) != 1):
-            raise ValueError(f"{name}: the output for {what} must be {tuple(t.shape)} in {dtype} on {device} with adjacent channels")
-        elif not _rows_apart(o):
-            raise ValueError(f"{name}: rows of the output for {what} share memory")
-        return t, o
-
-    fresh = out is None and k_out is None
-    q, out = rows_of(q, out, "q")
-    result = out
-    Hk, kb, kh, ks, ob, oh, os_, kp, kop = 0, 0, 0, 0, 0, 0, 0, 0, 0
+    # rows as the library takes them
+    qb, qh, qs, step = q.stride()
+    if step != 1 and D > 1:
+        q = q.contiguous()
+        qb, qh, qs, _ = q.stride()
+    kp = kop = kb = kh = ks = ob = oh = os_ = 0
     if k is not None:
-        k, k_out = rows_of(k, k_out, "k")
-        result = (out, k_out)
-        Hk, kp, kop = k.shape[1], k.data_ptr(), k_out.data_ptr()
-        kb, kh, ks, _ = k.stride()
-        ob, oh, os_, _ = k_out.stride()
+        kb, kh, ks, step = k.stride()
+        if step != 1 and D > 1:
+            k = k.contiguous()
+            kb, kh, ks, _ = k.stride()
+    fresh = out is None and k_out is None
+
+    def output(t, o, what):
+        if o is None:
+            return _empty_like(t, memory_format=_ROWS)
+        if o.shape != t.shape or o.dtype != dtype or o.get_device() != here or (D > 1 and o.stride(3) != 1):
+            raise ValueError(f"{name}: the output for {what} must be {tuple(t.shape)} in {dtype} on {q.device} with adjacent channels")
+        if not _rows_apart(o):
+            raise ValueError(f"{name}: rows of the output for {what} share memory")
+        return o
+
+    if fresh:
+        result = out = _empty_like(q, memory_format=_ROWS)
+        ps, ph = D, S * D
+        pb = Hq * ph
+        if k is not None:
+            k_out = _empty_like(k, memory_format=_ROWS)
+            os_, oh, ob = D, ph, Hk * ph
+            result = (out, k_out)
+    else:
+        result = out = output(q, out, "q")
+        pb, ph, ps, _ = out.stride()
+        if k is not None:
+            k_out = output(k, k_out, "k")
+            ob, oh, os_, _ = k_out.stride()
+            result = (out, k_out)
     if B == 0 or S == 0 or Hq + Hk == 0:
         return result
+    if k is not None:
+        kp, kop = k.data_ptr(), k_out.data_ptr()
     if not fresh:   # (new outputs overlap nothing)
         has_q, has_k = q.numel() > 0, k is not None and k.numel() > 0
         q_still, k_still = has_q and _same_rows(q, out), has_k and _same_rows(k, k_out)
@@ -1978,20 +2004,19 @@ def _rotary_rows(name, q, k, inv_freq, offset, positions, traditional, attention
             if meets and not _apart(o, t):
                 raise ValueError(f"{name}: the output for {what} overlaps other rows of the call (it may only be its input itself)")
     lib = _lib.load()
-    qb, qh, qs, _ = q.stride()
-    pb, ph, ps, _ = out.stride()
     try:
-        args = _lib.ROTARY_PACK.pack(
-            q.data_ptr(), kp, out.data_ptr(), kop, Hq, Hk, qb, qh, qs, kb, kh, ks, pb, ph, ps, ob, oh, os_, B, S, D, dims,
-            inv_freq.data_ptr(), 0 if at is None else at.data_ptr(), at_b, at_s, first, tag, VQ_F64 if wide_freq else VQ_F32,
-            VQ_I64 if at is None or at.dtype == torch.int64 else VQ_I32, add_index, 1 if traditional else 0, 1 if inverse else 0,
-            attention_factor)
+        args = (q.data_ptr(), kp, out.data_ptr(), kop, Hq, Hk, qb, qh, qs, kb, kh, ks, pb, ph, ps, ob, oh, os_, B, S, D, dims,
+                inv_freq.data_ptr(), 0 if at is None else at.data_ptr(), at_b, at_s, first, tag, VQ_F64 if wide_freq else VQ_F32,
+                VQ_I64 if at is None or at.dtype == torch.int64 else VQ_I32, add_index, 1 if traditional else 0, 1 if inverse else 0,
+                attention_factor)
+        if norm is None:
+            call, args = lib.rotary_packed, _lib.ROTARY_PACK.pack(*args)
+        else:
+            call, args = lib.norm_rotary_packed, _lib.NORM_ROTARY_PACK.pack(*args, q_at, k_at, q_step, k_step, weight_tag, eps)
     except (_lib.struct.error, OverflowError) as e:
         raise ValueError(f"{name}: {e}") from None
-    if norm is None:
-        _launch_on(device, lambda: lib.rotary_packed(args, _stream_of(device)))
-    else:
-        _launch_on(device, lambda: lib.norm_rotary_packed(args + norm, _stream_of(device)))
+    device = q.device
+    _launch_on(device, lambda: call(args, _stream_of(device)))
     return result
 
 
