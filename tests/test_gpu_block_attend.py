@@ -289,3 +289,28 @@ def test_an_empty_list_needs_no_store():
     q = torch.zeros((0, 4, 1, 64), dtype=F16, device="cuda")
     t = torch.zeros((0, 2, 3, 64), dtype=F16, device="cuda")
     assert K.block_sparse_attend(q, torch.zeros((0, 2, 1, 2), dtype=torch.int32, device="cuda"), block_size=32, k_tail=t, v_tail=t, n_tail=3).shape == q.shape
+
+
+@pytest.mark.parametrize("D,bits,dtype", [(128, 2, F16), (64, 4, BF16), (128, 8, F16)])
+def test_calls_under_way_on_two_streams(D, bits, dtype):
+    """Choice and attention in parts on two streams at once: each stream has its own scratch and counters."""
+    require_gpu()
+    sets = []
+    for seed in (20, 30):
+        q, s, blocks, _ = _case(1, 8, 2, D, (4096, 60), 32, 60, bits=bits, dtype=dtype, seed=seed)
+        sets.append((q, s, torch.cuda.Stream()))
+
+    def step(q, s):
+        chosen = K.select_blocks(q, s["k_scale"], s["k_zero"], 60, levels=2 ** bits - 1, group_size=32, n_packed=4096, n_tail=60, causal=True)
+        return chosen, K.block_sparse_attend(q, chosen, **s, block_size=32, scale=0.1, causal=True)
+
+    want = [step(q, s) for q, s, _ in sets]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        got = []
+        for q, s, stream in sets:
+            with torch.cuda.stream(stream):
+                got.append(step(q, s))
+        torch.cuda.synchronize()
+        for (a, b), (c, d) in zip(got, want):
+            assert torch.equal(a, c) and torch.equal(b, d)
