@@ -134,6 +134,31 @@ def test_values_that_are_not_finite(Sq, query_block):
     assert got[1, 0, 0].tolist() == [0, 1, 2, 3, 4, 5]
 
 
+@pytest.mark.parametrize("what", ["ordinary", "signed", "close", "small", "past fp16", "odd"])
+@pytest.mark.parametrize("dtype,D,Sq,query_block,groups", [(F16, 128, 48, 16, 2100), (BF16, 256, 24, 3, 2100), (BF16, 64, 100, 50, 2051)])
+def test_many_rows_over_float32_stores(dtype, D, Sq, query_block, groups, what):
+    """Sizes from which float32 scales and zeros are looked through rounded to fp16 first."""
+    require_gpu()
+    q, scale, zero = _inputs(1, 8, 2, Sq, D, groups, dtype=dtype, meta=F32, seed=D, signed=what == "signed")
+    assert 8 * Sq * groups * D > 1e8
+    if what == "close":         # far less apart than fp16 numbers are
+        near = zero[:, :, :1] * (1 + 2.0 ** -16 * torch.rand((1, 2, groups, 1), generator=torch.Generator(device="cuda").manual_seed(3), device="cuda"))
+        zero[:, :, :groups], scale[:, :, :groups] = near, scale[:, :, :1].clone()
+    elif what == "small":
+        zero *= 2.0 ** -30
+        scale *= 2.0 ** -30
+        q = (q.float() * 2.0 ** -12).to(dtype)
+    elif what == "past fp16":
+        zero[:, 0] *= 1e6
+        scale[0, 1, 77, 3] = 3e38
+    elif what == "odd":
+        zero[0, 0, 50, 3] = float("nan")
+        scale[0, 1, 70, 9] = float("inf")
+    lens = torch.tensor([groups * 32 - 100], device="cuda")
+    _same(q, scale, zero, 40, levels=15, group_size=32, n_packed=groups * 32, n_tail=9, block_size=64, query_block=query_block, first=1, recent=1, causal=True,
+          seq_lens=lens if what == "ordinary" else None)
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16, F32])
 @pytest.mark.parametrize("big", [2.0 ** 15, 2.0 ** -20])
 def test_large_and_small_queries(dtype, big):

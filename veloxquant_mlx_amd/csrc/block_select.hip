@@ -30,6 +30,11 @@ struct SelectCall {
     int runs, run_units;    // waves a row tile, units of 32 groups of each
     float *approx;          // [items][row_tiles][groups]
     float *bounds;          // [items][row_tiles][runs]
+    // float32 scales and zeros, which it takes rounded to fp16: a's are the copies
+    int narrow;
+    u16 *copies;            // [zeros, scales][B][Hkv][groups][D]
+    const float *wide_zero, *wide_scale;
+    int64_t wide_stride;
 };
 
 // Live slots of a sequence, and of the packed ones those [0, end) that its query i sees (slots and queries: below 2^30).
@@ -59,7 +64,7 @@ __device__ __forceinline__ uint64_t pick_key(double s) {   // ascending with the
 __device__ __forceinline__ uint64_t max_key(uint64_t x, uint64_t y) { return x > y ? x : y; }
 __device__ __forceinline__ double key_score(uint64_t k) { return __longlong_as_double((int64_t)(k >> 63 ? k & ~(UINT64_C(1) << 63) : ~k)); }   // (NaN for NaN's)
 
-// Float32 queries, scales or zeros, and head sizes that the matrix units do not take: every group's score in 64 bits, on the vector units.
+// Float32 queries, head sizes that the matrix units do not take, few products over float32 scales and zeros: every group's score in 64 bits, on the vector units.
 //
 // Eight lanes a group, each with four channels of every 32, all of them asked for ahead of the queries, of which RW rows at a time lie in LDS as
 // doubles.  With a group's middle and half width in a channel, m = z + L s / 2 and w = L |s| / 2, the bound is sum y m + |y| w: two
@@ -179,6 +184,7 @@ template <typename T, bool WIDE, int RW> __global__ __launch_bounds__(256) void 
 // ---- the matrix units as a filter
 
 typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+typedef u32 u32x2 __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ u32 positive(u32 x) { return __builtin_bit_cast(u32, __builtin_elementwise_max(as_h2(x), f16x2{(f16)0.f, (f16)0.f})); }
 __device__ __forceinline__ u32 max_bits(u32 x, u32 y) {   // of two magnitudes each
@@ -276,6 +282,20 @@ __device__ __forceinline__ float bound_units(const SelectCall &c, int b, int hkv
         unscale = __builtin_amdgcn_ldexpf(1.f, -up);
     }
     const float levels = (float)a.levels;
+    float small = 0.f;   // what rounded zeros and scales below the normal numbers are off by, (1 + L) 2^-25 sum |q|, as a part of A (see pick_error), twice
+    if (c.narrow) {
+        small = 0x1p-6f;   // (queries below the normal numbers, which may count as zero here)
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) small = __builtin_amdgcn_fdot2(as_h2(q[k][i] & 0x7FFF7FFFu), f16x2{(f16)1.f, (f16)1.f}, small, false);
+        small += __shfl_xor(small, 32);
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) small = fmaxf(small, __shfl_xor(small, off));
+        small *= (1.f + levels) * 0x1p-13f;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) asm volatile("" : "+v"(q[k]));   // (the magnitudes are not kept)
+    }
     const u32 levels2 = __builtin_bit_cast(u32, f16x2{(f16)levels, (f16)levels});
     const int seen = sel_end(a, live, pos0);   // by every query
     u32 most = 0;   // bits of the largest sum of |q| (|z| + L |s|), NaN above infinity above all else
@@ -365,7 +385,7 @@ __device__ __forceinline__ float bound_units(const SelectCall &c, int b, int hkv
     }
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) { const u32 o = __shfl_xor(most, off); most = o > most ? o : most; }
-    return __uint_as_float(most) * unscale;
+    return (__uint_as_float(most) + small) * unscale;
 }
 
 // Items of many rows, and few of many groups: a wave a run of units, scores and bounds to memory.
@@ -385,6 +405,26 @@ template <int D, bool BF16> __global__ __launch_bounds__(256) __attribute__((amd
     if (u0 < u1) bound = bound_units<D, BF16>(c, b, hkv, tile, (int)(tile_row % (u32)c.row_tiles), live, u0, u1, 32, c.approx + (int64_t)tile_row * c.groups,
                                                    rings + wave * BoundRing<D>::BYTES);
     if ((threadIdx.x & 63) == 0) c.bounds[id] = bound;
+}
+
+// Float32 zeros and scales of the groups that a sequence sees, rounded to fp16: eight channels a thread.
+__global__ __launch_bounds__(256) void narrow_kernel(SelectCall c) {
+    const vq_block_select_args &a = c.a;
+    const u32 pieces = (u32)(c.groups * a.D / 8), id = blockIdx.x * 256 + threadIdx.x, bh = id / pieces, at = id % pieces;
+    if (bh >= (u32)(a.B * a.Hkv)) return;
+    const int64_t u = at * 8 / (u32)a.D;
+    if (u * a.group >= sel_live(a, (int)(bh / (u32)a.Hkv))) return;
+    const int64_t from = (int64_t)bh * c.wide_stride * a.D + (int64_t)at * 8;
+    u16 *const to = c.copies + (int64_t)id * 8;
+    const f32x4 z0 = *(const f32x4 *)(c.wide_zero + from), z1 = *(const f32x4 *)(c.wide_zero + from + 4), s0 = *(const f32x4 *)(c.wide_scale + from), s1 = *(const f32x4 *)(c.wide_scale + from + 4);
+    f16x8 z, s;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        z[i] = (f16)z0[i]; z[4 + i] = (f16)z1[i];
+        s[i] = (f16)s0[i]; s[4 + i] = (f16)s1[i];
+    }
+    *(f16x8 *)to = z;
+    *(f16x8 *)(to + a.B * a.Hkv * c.groups * a.D) = s;
 }
 
 // ---- the choice
@@ -457,6 +497,53 @@ __device__ __forceinline__ uint64_t exact_key(const SelectCall &c, int b, int hk
                 });
         }
         s += (double)a.levels * w;
+        for (int off = 1; off < parts; off <<= 1) s = shfl_add(s, off);
+        if (u * g < end) best = max_key(best, pick_key(s));
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) best = max_key(best, __shfl_xor((unsigned long long)best, off));
+    return best;
+}
+
+// The same from float32 scales and zeros.
+__device__ __forceinline__ uint64_t exact_key_wide(const SelectCall &c, int b, int hkv, int tile, int live, int u) {
+    constexpr int AHEAD = 4;
+    const vq_block_select_args &a = c.a;
+    const int lane = threadIdx.x & 63, G = (int)a.Hq / (int)a.Hkv, D = (int)a.D, g = a.group;
+    const int pos0 = tile * (int)c.query_block, rows = (sel_last(a, tile) - pos0 + 1) * G;
+    int many = 1;
+    while (many < rows && many < 64) many <<= 1;
+    const int parts = 64 / many, part = lane % parts;
+    const int64_t at = (((int64_t)b * a.Hkv + hkv) * c.wide_stride + u) * D;
+    const float *const zero = c.wide_zero + at, *const scale = c.wide_scale + at;
+    const bool bf16 = a.dtype == VQ_BF16;
+    uint64_t best = 0;
+    for (int r0 = 0; r0 < rows; r0 += many) {
+        const int r = r0 + lane / parts, x = r < rows ? r : rows - 1, end = sel_end(a, live, pos0 + x / G);
+        const u16 *q = (const u16 *)a.q + (((int64_t)b * a.Hq + hkv * G + x % G) * a.Sq + pos0 + x / G) * D;
+        double s = 0., w = 0.;
+        for (int d0 = part * 4; d0 < D; d0 += AHEAD * parts * 4) {
+            u32x2 x2[AHEAD];
+            f32x4 z4[AHEAD], s4[AHEAD];
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k) {
+                const int d = d0 + k * parts * 4;
+                if (k > 0 && d >= D) { x2[k] = u32x2{0, 0}; z4[k] = s4[k] = f32x4{0.f, 0.f, 0.f, 0.f}; continue; }
+                x2[k] = *(const u32x2 *)(q + d);
+                z4[k] = *(const f32x4 *)(zero + d);
+                s4[k] = *(const f32x4 *)(scale + d);
+            }
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const u16 xb = (u16)(x2[k][i / 2] >> (16 * (i & 1)));
+                    const double y = bf16 ? bf16_to_f32(xb) : (float)__builtin_bit_cast(f16, xb), p = y * (double)s4[k][i];
+                    s = __builtin_fma(y, (double)z4[k][i], s);
+                    w += p <= 0. ? 0. : p;
+                }
+        }
+        s = __builtin_fma((double)a.levels, w, s);
         for (int off = 1; off < parts; off <<= 1) s = shfl_add(s, off);
         if (u * g < end) best = max_key(best, pick_key(s));
     }
@@ -567,7 +654,8 @@ __device__ __forceinline__ void pick(const SelectCall &c, PickRoom<THREADS> &roo
     auto key_of = [&](int j, int i) __attribute__((always_inline)) -> uint64_t {
         const int u = (lo + j) * per + i;
         if (u >= seen) return 0;
-        return STORED ? c.stored[(int64_t)blockIdx.x * c.groups + u] : exact_key(c, b, hkv, tile, live, u);
+        if (STORED) return c.stored[(int64_t)blockIdx.x * c.groups + u];
+        return c.narrow ? exact_key_wide(c, b, hkv, tile, live, u) : exact_key(c, b, hkv, tile, live, u);
     };
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) {
@@ -730,7 +818,10 @@ template <int THREADS> __device__ __forceinline__ void pick_blocks(const SelectC
         most = fmaxf(most, x);
     }
 }
-__device__ __forceinline__ float pick_error(const SelectCall &c, float bound) { return bound < INFINITY ? bound * ((float)(c.a.D + 16) * 0x1p-23f) : INFINITY; }
+// How far a score may be off, A the bound's; scales and zeros rounded to fp16 are off by 2^-11 of themselves.
+__device__ __forceinline__ float pick_error(const SelectCall &c, float bound) {
+    return bound < INFINITY ? bound * ((float)(c.a.D + 16) * 0x1p-23f + (c.narrow ? 0x1.02p-11f : 0.f)) : INFINITY;
+}
 
 template <bool STORED, int THREADS> __global__ __launch_bounds__(THREADS) void block_pick_kernel(SelectCall c) {
     extern __shared__ float keys[];
@@ -856,7 +947,10 @@ SelectCall cut_select(const vq_block_select_args &a) {
     c.stride = cdiv(a.cap_tokens, a.group);
     c.row_tiles = (int)cdiv(a.Hq / a.Hkv * c.query_block, 32);
     if (c.total <= a.count) return c;   // every visible block is chosen: no scores
-    c.mma = (a.D == 64 || a.D == 128 || a.D == 256) && a.dtype != VQ_F32 && a.meta_dtype == VQ_F16 && c.total <= PICK_MOST &&
+    // (what it costs to round them and to tell more blocks apart is earned back from some 10^8 products on: 8 kv heads of 128 channels over 524 groups, 128 rows a kv
+    // head 34.5 us and 33.2 in 64 bits throughout, 256 rows 37.4 and 47.8, 2048 rows 74 and 308; 16 sequences at 32k, 4 rows a head 56 and 38, 16 rows 84 and 117)
+    c.narrow = a.meta_dtype == VQ_F32 && (double)a.B * (double)a.Hq * (double)a.Sq * (double)c.groups * (double)a.D >= 1e8;
+    c.mma = (a.D == 64 || a.D == 128 || a.D == 256) && a.dtype != VQ_F32 && (a.meta_dtype == VQ_F16 || c.narrow) && c.total <= PICK_MOST &&
             (((uintptr_t)a.q | (uintptr_t)a.k_scale | (uintptr_t)a.k_zero) & 15) == 0;
     if (c.mma) {
         // a unit a wave until the eight waves that a CU holds have work
@@ -870,20 +964,22 @@ SelectCall cut_select(const vq_block_select_args &a) {
         // 32 11.9 us, in two launches 13.1; over 16k 13.6 and 13.4, 32k 16.1 and 13.2; four sequences of 32k 17.5 and 16.1, eight 17.9 and 19.0.
         c.one = c.mma && c.row_tiles == 1 && (c.total + c.groups) * 4 <= ONE_SCORES && (c.items >= 64 || units <= (a.D == 256 ? 8 : 16));
     }
+    if (!c.mma) c.narrow = 0;
     return c;
 }
-struct SelectRoom { size_t stored, approx, bounds, all; };
+struct SelectRoom { size_t stored, approx, bounds, copies, all; };
 SelectRoom select_room(const SelectCall &c) {
     SelectRoom r = {};
     if (c.total <= c.a.count) return r;
     auto whole = [](size_t n) { return (n + 15) / 16 * 16; };
     r.stored = whole((size_t)(c.items * c.total) * 8);
     r.approx = r.stored + (c.mma ? 0 : whole((size_t)(c.items * c.groups) * 8));
-    r.bounds = r.all = r.approx;
+    r.bounds = r.copies = r.approx;
     if (c.mma && !c.one) {
         r.bounds = r.approx + whole((size_t)(c.items * c.row_tiles * c.groups) * 4);
-        r.all = r.bounds + whole((size_t)(c.items * c.row_tiles * c.runs) * 4);
+        r.copies = r.bounds + whole((size_t)(c.items * c.row_tiles * c.runs) * 4);
     }
+    r.all = r.copies + (c.narrow ? (size_t)(c.a.B * c.a.Hkv * c.groups * c.a.D) * 4 : 0);
     return r;
 }
 
@@ -961,6 +1057,17 @@ extern "C" int vq_block_select(const vq_block_select_args *args) {
         c.stored = (uint64_t *)((char *)a.workspace + room.stored);
         c.approx = (float *)((char *)a.workspace + room.approx);
         c.bounds = (float *)((char *)a.workspace + room.bounds);
+        if (c.narrow) {
+            c.copies = (u16 *)((char *)a.workspace + room.copies);
+            c.wide_zero = (const float *)a.k_zero;
+            c.wide_scale = (const float *)a.k_scale;
+            c.wide_stride = c.stride;
+            c.stride = c.groups;
+            c.a.k_zero = c.copies;
+            c.a.k_scale = c.copies + a.B * a.Hkv * c.groups * a.D;
+            narrow_kernel<<<(unsigned)cdiv(a.B * a.Hkv * c.groups * a.D / 8, 256), 256, 0, st>>>(c);
+            VQ_HIP_CHECK_LAUNCH(fn);
+        }
         if (c.mma) return a.D == 64 ? launch_choice<64>(fn, c) : a.D == 128 ? launch_choice<128>(fn, c) : launch_choice<256>(fn, c);
         const bool wide = a.D % 4 == 0 && (((uintptr_t)a.k_scale | (uintptr_t)a.k_zero) & 15) == 0;
         if (a.meta_dtype == VQ_F32) wide ? launch_scores<float, true>(c) : launch_scores<float, false>(c);
