@@ -1785,8 +1785,8 @@ def block_sparse_attend(q: torch.Tensor, blocks: torch.Tensor, *, block_size: in
     :func:`select_blocks` gives them: queries ``t * query_block`` and the next ``query_block - 1`` see, of the packed slots, those of the blocks of
     list ``t`` of their kv head (entry ``e``: slots ``e * block_size`` .. ``(e + 1) * block_size - 1``), as far as these are live and, with
     ``causal``, not behind the query.  Entries may come in any order; one below zero or past the live slots names nothing, one that is
-    named twice counts twice.  The plain rows of the tail are all seen, up to the query's own.  Slots that no list names are not read.  A
-    row that sees nothing is zero.  Numbers as for :func:`shared_prefix_attend`.  2- and 4-bit stores with heads of 64, 128 or 256 channels, groups
+    named twice counts twice.  The plain rows of the tail are all seen, up to the query's own.  Slots that no list names are not read;
+    live values have to be finite, what lies behind the live slots may be anything.  A row that sees nothing is zero.  Numbers as for :func:`shared_prefix_attend`.  2- and 4-bit stores with heads of 64, 128 or 256 channels, groups
     of 32, 64 or 128 and values packed by token run on the matrix units where blocks are whole units of 32 slots; other stores, sizes and float32 rows
     in float32, some ten times slower."""
     own = (k_packed, k_scale, k_zero, v_packed, v_scale, v_zero, n_packed, bits, group_size, v_layout, k_tail, v_tail, n_tail)
