@@ -181,6 +181,34 @@ template <typename T, bool WIDE, int RW> __global__ __launch_bounds__(256) void 
     if (part == 0 && u < groups) c.stored[item * c.groups + u] = best;
 }
 
+// Over a wave by moves within rows of sixteen lanes and from row to row, not through the LDS unit: the largest (of op's) in every lane; the sum up to and with a lane.
+template <int CTRL, int ROWS> __device__ __forceinline__ u32 moved(u32 old, u32 x) { return (u32)__builtin_amdgcn_update_dpp((int)old, (int)x, CTRL, ROWS, 0xF, false); }
+template <typename Op> __device__ __forceinline__ u32 wave_all(u32 x, Op op) {
+    x = op(x, moved<0x111, 0xF>(x, x));   // row_shr 1, 2, 4, 8: a lane without a source meets itself
+    x = op(x, moved<0x112, 0xF>(x, x));
+    x = op(x, moved<0x114, 0xF>(x, x));
+    x = op(x, moved<0x118, 0xF>(x, x));
+    x = op(x, moved<0x142, 0xA>(x, x));   // row_bcast 15, 31
+    x = op(x, moved<0x143, 0xC>(x, x));
+    return (u32)__builtin_amdgcn_readlane((int)x, 63);
+}
+__device__ __forceinline__ u32 wave_max_bits(u32 x) { return wave_all(x, [](u32 y, u32 z) { return y > z ? y : z; }); }
+__device__ __forceinline__ float wave_max(float x) {
+    return __uint_as_float(wave_all(__float_as_uint(x), [](u32 y, u32 z) { return __float_as_uint(fmaxf(__uint_as_float(y), __uint_as_float(z))); }));
+}
+__device__ __forceinline__ float wave_min(float x) {
+    return __uint_as_float(wave_all(__float_as_uint(x), [](u32 y, u32 z) { return __float_as_uint(fminf(__uint_as_float(y), __uint_as_float(z))); }));
+}
+__device__ __forceinline__ u32 wave_sum_up(u32 x) {
+    x += moved<0x111, 0xF>(0, x);
+    x += moved<0x112, 0xF>(0, x);
+    x += moved<0x114, 0xF>(0, x);
+    x += moved<0x118, 0xF>(0, x);
+    x += moved<0x142, 0xA>(0, x);
+    x += moved<0x143, 0xC>(0, x);
+    return x;
+}
+
 // ---- the matrix units as a filter
 
 typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
@@ -269,8 +297,7 @@ __device__ __forceinline__ float bound_units(const SelectCall &c, int b, int hkv
 #pragma unroll
             for (int i = 0; i < 4; ++i) top = max_bits(top, q[k][i] & 0x7FFF7FFFu);
         top = top >> 16 > (top & 0xFFFFu) ? top >> 16 : top & 0xFFFFu;
-#pragma unroll
-        for (int off = 32; off > 0; off >>= 1) { const u32 o = __shfl_xor(top, off); top = o > top ? o : top; }
+        top = wave_max_bits(top);
         // 2^(141 - e) with e the largest's exponent field: below 2^15; what is not finite stays so
         const int e = (int)(top >> 7), up = e == 0 || e == 255 ? 0 : 141 - e;
 #pragma unroll
@@ -289,9 +316,7 @@ __device__ __forceinline__ float bound_units(const SelectCall &c, int b, int hkv
         for (int k = 0; k < KS; ++k)
 #pragma unroll
             for (int i = 0; i < 4; ++i) small = __builtin_amdgcn_fdot2(as_h2(q[k][i] & 0x7FFF7FFFu), f16x2{(f16)1.f, (f16)1.f}, small, false);
-        small += __shfl_xor(small, 32);
-#pragma unroll
-        for (int off = 16; off > 0; off >>= 1) small = fmaxf(small, __shfl_xor(small, off));
+        small = wave_max(small + __shfl_xor(small, 32));
         small *= (1.f + levels) * 0x1p-13f;
 #pragma unroll
         for (int k = 0; k < KS; ++k) asm volatile("" : "+v"(q[k]));   // (the magnitudes are not kept)
@@ -383,9 +408,7 @@ __device__ __forceinline__ float bound_units(const SelectCall &c, int b, int hkv
         best = fmaxf(best, __shfl_xor(best, 32)) * unscale;
         if (h == 0 && u + n < u1) out[u + n] = best;
     }
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) { const u32 o = __shfl_xor(most, off); most = o > most ? o : most; }
-    return (__uint_as_float(most) + small) * unscale;
+    return (__uint_as_float(wave_max_bits(most)) + small) * unscale;
 }
 
 // Items of many rows, and few of many groups: a wave a run of units, scores and bounds to memory.
@@ -583,20 +606,17 @@ template <int WAVES> __device__ __forceinline__ u32 block_before(bool one, bool 
     return before;
 }
 
-// The bin, a thread each, that holds the `left`-th from the highest bin down; `left` becomes how many of that bin are wanted.  (A barrier
-// lies between the last count and the call.)
+// The bin that holds the `left`-th from the highest bin down (a thread each, the highest bin's first); `left` becomes how many of that bin are
+// wanted.  (A barrier lies between the last count and the call.)
 template <int WAVES> __device__ __forceinline__ int pick_bin(const u32 *hist, u32 &left, u32 *waves, u32 *found) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const u32 mine = hist[tid];
-    u32 sum = mine;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) { const u32 o = __shfl_down(sum, off); sum += lane + off < 64 ? o : 0; }
-    if (lane == 0) waves[wave] = sum;
+    const int tid = threadIdx.x, wave = tid >> 6, bin = WAVES * 64 - 1 - tid;
+    const u32 mine = hist[bin], sum = wave_sum_up(mine);
+    if ((tid & 63) == 63) waves[wave] = sum;
     __syncthreads();
     u32 above = sum - mine;
 #pragma unroll
-    for (int w = 1; w < WAVES; ++w) above += w > wave ? waves[w] : 0;
-    if (above < left && above + mine >= left) { found[0] = (u32)tid; found[1] = left - above; }
+    for (int w = 0; w < WAVES - 1; ++w) above += w < wave ? waves[w] : 0;
+    if (above < left && above + mine >= left) { found[0] = (u32)bin; found[1] = left - above; }
     __syncthreads();
     left = found[1];
     return (int)found[0];
@@ -657,12 +677,9 @@ __device__ __forceinline__ void pick(const SelectCall &c, PickRoom<THREADS> &roo
         if (STORED) return c.stored[(int64_t)blockIdx.x * c.groups + u];
         return c.narrow ? exact_key_wide(c, b, hkv, tile, live, u) : exact_key(c, b, hkv, tile, live, u);
     };
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-        least = fminf(least, __shfl_xor(least, off));
-        most = fmaxf(most, __shfl_xor(most, off));
-        e = fmaxf(e, __shfl_xor(e, off));
-    }
+    least = wave_min(least);
+    most = wave_max(most);
+    e = wave_max(e);
     if (lane == 0) { room.low[wave] = least; room.high[wave] = most; room.off_by[wave] = e; }
     room.hist[tid] = 0;
     __syncthreads();
@@ -693,8 +710,8 @@ __device__ __forceinline__ void pick(const SelectCall &c, PickRoom<THREADS> &roo
                 const float x = keys[j];
                 if (x >= from && x <= to && (u32)((x - from) * by) % THREADS == bin) { l = fminf(l, x); m = fmaxf(m, x); }
             }
-#pragma unroll
-            for (int off = 32; off > 0; off >>= 1) { l = fminf(l, __shfl_xor(l, off)); m = fmaxf(m, __shfl_xor(m, off)); }
+            l = wave_min(l);
+            m = wave_max(m);
             if (lane == 0) { room.low[wave] = l; room.high[wave] = m; }
             __syncthreads();
             from = room.low[0]; to = room.high[0];
@@ -720,9 +737,9 @@ __device__ __forceinline__ void pick(const SelectCall &c, PickRoom<THREADS> &roo
         const int j = room.list[lane < (int)listed ? lane : 0];
         const float x = lane < (int)listed ? keys[j] : -INFINITY;
         u32 rank = 0;   // (equal ones in the list's order)
-        for (int o = 0; o < (int)listed; ++o) { const float y = __shfl(x, o); rank += y > x || (y == x && o < lane) ? 1 : 0; }
+        for (int o = 0; o < (int)listed; ++o) { const float y = __uint_as_float((u32)__builtin_amdgcn_readlane(__float_as_uint(x), o)); rank += y > x || (y == x && o < lane) ? 1 : 0; }
         const uint64_t kth = __ballot(lane < (int)listed && rank == need - 1);
-        const float t = __shfl(x, kth != 0 ? __builtin_ctzll(kth) : 0);   // (none among values that are not finite: e is not either)
+        const float t = __uint_as_float((u32)__builtin_amdgcn_readlane(__float_as_uint(x), kth != 0 ? __builtin_ctzll(kth) : 0));   // (none among values that are not finite: e is not either)
         const bool in = lane < (int)listed && x > t + e, maybe = lane < (int)listed && !in && !(x < t - e);
         const uint64_t m = __ballot(maybe);
         const u32 doubt = (u32)__popcll(m), wanted = need - (u32)__popcll(__ballot(in));
