@@ -405,7 +405,8 @@ __device__ __forceinline__ float bound_units(const SelectCall &c, int b, int hkv
         float best = S[0];
 #pragma unroll
         for (int r = 1; r < 16; ++r) best = fmaxf(best, S[r]);
-        best = fmaxf(best, __shfl_xor(best, 32)) * unscale;
+        const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(best), __float_as_uint(best), false, false);
+        best = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1])) * unscale;
         if (h == 0 && u + n < u1) out[u + n] = best;
     }
     return (__uint_as_float(wave_max_bits(most)) + small) * unscale;
@@ -705,6 +706,12 @@ __device__ __forceinline__ void pick(const SelectCall &c, PickRoom<THREADS> &roo
             __syncthreads();
             const u32 bin = (u32)pick_bin<WAVES>(room.hist, left, room.waves, room.found);
             among = room.hist[bin];
+            if (among <= 32 || pass == 3) {   // (by its edges, and what rounding may put beside them)
+                const float width = (to - from) / (float)(THREADS - 1), edge = from + ((float)bin + 1.001f) * width;
+                from += ((float)bin - 0.001f) * width;
+                to = edge < to ? edge : to;
+                break;
+            }
             float l = INFINITY, m = -INFINITY;
             for (int j = tid; j < n; j += THREADS) {
                 const float x = keys[j];
@@ -722,12 +729,16 @@ __device__ __forceinline__ void pick(const SelectCall &c, PickRoom<THREADS> &roo
     // ---- the list of those that may be the kth best, or are within e of it; t: the kth best's score, where the list is short
     float over = e < INFINITY ? to + e : INFINITY, under = e < INFINITY ? from - e : -INFINITY;
     u32 sure = 0, listed = 0;
-    for (int j0 = 0; j0 < n; j0 += THREADS) {
+    u32 at_of[2] = {0, 0};   // of this thread's first two: how many are listed before it, how many sure ones (upper half)
+    bool sure_of[2] = {false, false}, listed_of[2] = {false, false};
+    for (int j0 = 0, turn = 0; j0 < n; j0 += THREADS, ++turn) {
         const float x = j0 + tid < n ? keys[j0 + tid] : -INFINITY;
         const bool here = j0 + tid < n, in = here && x > over, maybe = here && !in && !(x < under);
         u32 some;
-        const u32 at = listed + (block_before<WAVES>(maybe, in, some, room.waves) & 0xFFFFu);
+        const u32 before = block_before<WAVES>(maybe, in, some, room.waves), at = listed + (before & 0xFFFFu);
         if (maybe && at < PICK_LIST) room.list[at] = j0 + tid;
+        if (turn == 0) { at_of[0] = before; sure_of[0] = in; listed_of[0] = maybe; }
+        if (turn == 1) { at_of[1] = before + (listed | sure << 16); sure_of[1] = in; listed_of[1] = maybe; }
         listed += some & 0xFFFFu;
         sure += some >> 16;
     }
@@ -744,6 +755,15 @@ __device__ __forceinline__ void pick(const SelectCall &c, PickRoom<THREADS> &roo
         const uint64_t m = __ballot(maybe);
         const u32 doubt = (u32)__popcll(m), wanted = need - (u32)__popcll(__ballot(in));
         const bool all = doubt == wanted;
+        if (all && n <= 2 * THREADS) {   // (every wave knows the taken ones of the list: the places of all follow)
+            const uint64_t taken = __ballot(in || maybe);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const u32 at = at_of[k] & 0xFFFFu, before = at < 64 ? (u32)__popcll(taken & ((UINT64_C(1) << at) - 1)) : (u32)__popcll(taken);
+                if (sure_of[k] || (listed_of[k] && (taken >> (at & 63) & 1))) out[lo + (int)(before + (at_of[k] >> 16))] = lo + k * THREADS + tid;
+            }
+            return;
+        }
         const u32 mine = (u32)__popcll(m & ((UINT64_C(1) << lane) - 1));   // this lane's place among the doubtful
         if (wave == 0 && maybe) { room.list[64 + mine] = j; room.exact[mine] = 0; }
         __syncthreads();   // (every wave has read the list's scores, which the first one replaces)
