@@ -64,6 +64,50 @@ __device__ __forceinline__ uint64_t pick_key(double s) {   // ascending with the
 __device__ __forceinline__ uint64_t max_key(uint64_t x, uint64_t y) { return x > y ? x : y; }
 __device__ __forceinline__ double key_score(uint64_t k) { return __longlong_as_double((int64_t)(k >> 63 ? k & ~(UINT64_C(1) << 63) : ~k)); }   // (NaN for NaN's)
 
+// Over a wave by moves within rows of sixteen lanes and from row to row, not through the LDS unit: the largest (of op's) in every lane; the sum up to and with a lane.
+template <int CTRL, int ROWS> __device__ __forceinline__ u32 moved(u32 old, u32 x) { return (u32)__builtin_amdgcn_update_dpp((int)old, (int)x, CTRL, ROWS, 0xF, false); }
+template <typename Op> __device__ __forceinline__ u32 wave_all(u32 x, Op op) {
+    x = op(x, moved<0x111, 0xF>(x, x));   // row_shr 1, 2, 4, 8: a lane without a source meets itself
+    x = op(x, moved<0x112, 0xF>(x, x));
+    x = op(x, moved<0x114, 0xF>(x, x));
+    x = op(x, moved<0x118, 0xF>(x, x));
+    x = op(x, moved<0x142, 0xA>(x, x));   // row_bcast 15, 31
+    x = op(x, moved<0x143, 0xC>(x, x));
+    return (u32)__builtin_amdgcn_readlane((int)x, 63);
+}
+__device__ __forceinline__ u32 wave_max_bits(u32 x) { return wave_all(x, [](u32 y, u32 z) { return y > z ? y : z; }); }
+__device__ __forceinline__ float wave_max(float x) {
+    return __uint_as_float(wave_all(__float_as_uint(x), [](u32 y, u32 z) { return __float_as_uint(fmaxf(__uint_as_float(y), __uint_as_float(z))); }));
+}
+__device__ __forceinline__ float wave_min(float x) {
+    return __uint_as_float(wave_all(__float_as_uint(x), [](u32 y, u32 z) { return __float_as_uint(fminf(__uint_as_float(y), __uint_as_float(z))); }));
+}
+__device__ __forceinline__ u32 wave_sum_up(u32 x) {
+    x += moved<0x111, 0xF>(0, x);
+    x += moved<0x112, 0xF>(0, x);
+    x += moved<0x114, 0xF>(0, x);
+    x += moved<0x118, 0xF>(0, x);
+    x += moved<0x142, 0xA>(0, x);
+    x += moved<0x143, 0xC>(0, x);
+    return x;
+}
+
+// The sum over `parts` neighbouring lanes (a power of two), in each of them: within sixteen by moves (as above), then through the LDS unit.
+template <int CTRL> __device__ __forceinline__ double add_moved(double s) {
+    const uint64_t x = (uint64_t)__double_as_longlong(s);
+    const u32 low = moved<CTRL, 0xF>(0, (u32)x), high = moved<CTRL, 0xF>(0, (u32)(x >> 32));
+    return s + __longlong_as_double((int64_t)((uint64_t)high << 32 | low));
+}
+__device__ __forceinline__ double sum_parts(double s, int parts) {
+    if (parts > 1) s = add_moved<0xB1>(s);    // quad_perm [1,0,3,2]
+    if (parts > 2) s = add_moved<0x4E>(s);    // quad_perm [2,3,0,1]
+    if (parts > 4) s = add_moved<0x141>(s);   // row_half_mirror
+    if (parts > 8) s = add_moved<0x140>(s);   // row_mirror
+    if (parts > 16) s += __shfl_xor(s, 16);
+    if (parts > 32) s += __shfl_xor(s, 32);
+    return s;
+}
+
 // Float32 queries, head sizes that the matrix units do not take, few products over float32 scales and zeros: every group's score in 64 bits, on the vector units.
 //
 // Eight lanes a group, each with four channels of every 32, all of them asked for ahead of the queries, of which RW rows at a time lie in LDS as
@@ -152,9 +196,7 @@ template <typename T, bool WIDE, int RW> __global__ __launch_bounds__(256) void 
             }
         }
         auto take = [&](int r, double x) __attribute__((always_inline)) {
-            x += __shfl_xor(x, 1);
-            x += __shfl_xor(x, 2);
-            x += __shfl_xor(x, 4);
+            x = sum_parts(x, 8);
             const int row = r0 + r;
             if (row < rows && u < groups && u * g < sel_end(a, live, pos0 + row / G)) best = max_key(best, pick_key(x));
         };
@@ -179,34 +221,6 @@ template <typename T, bool WIDE, int RW> __global__ __launch_bounds__(256) void 
         }
     }
     if (part == 0 && u < groups) c.stored[item * c.groups + u] = best;
-}
-
-// Over a wave by moves within rows of sixteen lanes and from row to row, not through the LDS unit: the largest (of op's) in every lane; the sum up to and with a lane.
-template <int CTRL, int ROWS> __device__ __forceinline__ u32 moved(u32 old, u32 x) { return (u32)__builtin_amdgcn_update_dpp((int)old, (int)x, CTRL, ROWS, 0xF, false); }
-template <typename Op> __device__ __forceinline__ u32 wave_all(u32 x, Op op) {
-    x = op(x, moved<0x111, 0xF>(x, x));   // row_shr 1, 2, 4, 8: a lane without a source meets itself
-    x = op(x, moved<0x112, 0xF>(x, x));
-    x = op(x, moved<0x114, 0xF>(x, x));
-    x = op(x, moved<0x118, 0xF>(x, x));
-    x = op(x, moved<0x142, 0xA>(x, x));   // row_bcast 15, 31
-    x = op(x, moved<0x143, 0xC>(x, x));
-    return (u32)__builtin_amdgcn_readlane((int)x, 63);
-}
-__device__ __forceinline__ u32 wave_max_bits(u32 x) { return wave_all(x, [](u32 y, u32 z) { return y > z ? y : z; }); }
-__device__ __forceinline__ float wave_max(float x) {
-    return __uint_as_float(wave_all(__float_as_uint(x), [](u32 y, u32 z) { return __float_as_uint(fmaxf(__uint_as_float(y), __uint_as_float(z))); }));
-}
-__device__ __forceinline__ float wave_min(float x) {
-    return __uint_as_float(wave_all(__float_as_uint(x), [](u32 y, u32 z) { return __float_as_uint(fminf(__uint_as_float(y), __uint_as_float(z))); }));
-}
-__device__ __forceinline__ u32 wave_sum_up(u32 x) {
-    x += moved<0x111, 0xF>(0, x);
-    x += moved<0x112, 0xF>(0, x);
-    x += moved<0x114, 0xF>(0, x);
-    x += moved<0x118, 0xF>(0, x);
-    x += moved<0x142, 0xA>(0, x);
-    x += moved<0x143, 0xC>(0, x);
-    return x;
 }
 
 // ---- the matrix units as a filter
@@ -453,8 +467,6 @@ __global__ __launch_bounds__(256) void narrow_kernel(SelectCall c) {
 
 // ---- the choice
 
-__device__ __forceinline__ double shfl_add(double s, int off) { return s + __shfl_xor(s, off); }
-
 // The key of group u's score in 64 bits, the largest over the tile's rows, by a wave: 64 / R lanes a row (R the rows, up to the next power of two),
 // eight channels at a time.
 __device__ __forceinline__ uint64_t exact_key(const SelectCall &c, int b, int hkv, int tile, int live, int u) {
@@ -521,11 +533,10 @@ __device__ __forceinline__ uint64_t exact_key(const SelectCall &c, int b, int hk
                 });
         }
         s += (double)a.levels * w;
-        for (int off = 1; off < parts; off <<= 1) s = shfl_add(s, off);
+        s = sum_parts(s, parts);
         if (u * g < end) best = max_key(best, pick_key(s));
     }
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) best = max_key(best, __shfl_xor((unsigned long long)best, off));
+    for (int off = 32; off >= parts; off >>= 1) best = max_key(best, __shfl_xor((unsigned long long)best, off));
     return best;
 }
 
@@ -568,11 +579,10 @@ __device__ __forceinline__ uint64_t exact_key_wide(const SelectCall &c, int b, i
                 }
         }
         s = __builtin_fma((double)a.levels, w, s);
-        for (int off = 1; off < parts; off <<= 1) s = shfl_add(s, off);
+        s = sum_parts(s, parts);
         if (u * g < end) best = max_key(best, pick_key(s));
     }
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) best = max_key(best, __shfl_xor((unsigned long long)best, off));
+    for (int off = 32; off >= parts; off >>= 1) best = max_key(best, __shfl_xor((unsigned long long)best, off));
     return best;
 }
 
