@@ -25,6 +25,11 @@ __device__ __forceinline__ float nr_rsqrt(float t) {
     return __builtin_amdgcn_rsqf(small ? t * 0x1p64f : t) * (small ? 0x1p32f : 1.f);
 }
 
+// x of another lane of the same sixteen
+template <int CTRL> __device__ __forceinline__ float nr_moved(float x) {
+    return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), CTRL, 0xF, 0xF, true));
+}
+
 __device__ __forceinline__ int64_t nr_position(const vq_rotary_args &a, int64_t b, int64_t s) {
     int64_t p = a.offset + (a.add_index ? s : 0);
     if (a.positions != nullptr) {
@@ -216,9 +221,17 @@ template <typename T, int N, bool HALF, bool OWN> __global__ __launch_bounds__(N
             }
             sum[k] = (has0 ? p0 : 0.f) + (has1 ? p1 : 0.f);
         }
-        for (int off = 1; off < 1 << c.lanes_log2; off <<= 1)
+        // (within sixteen lanes by moves, not through the LDS unit)
+        auto meet = [&](auto other) __attribute__((always_inline)) {
 #pragma unroll
-            for (int k = 0; k < NR_FLIGHT; ++k) sum[k] += __shfl_xor(sum[k], off);
+            for (int k = 0; k < NR_FLIGHT; ++k) sum[k] += other(sum[k]);
+        };
+        if (c.lanes_log2 > 0) meet([](float x) { return nr_moved<0xB1>(x); });    // quad_perm [1,0,3,2]
+        if (c.lanes_log2 > 1) meet([](float x) { return nr_moved<0x4E>(x); });    // quad_perm [2,3,0,1]
+        if (c.lanes_log2 > 2) meet([](float x) { return nr_moved<0x141>(x); });   // row_half_mirror
+        if (c.lanes_log2 > 3) meet([](float x) { return nr_moved<0x140>(x); });   // row_mirror
+        if (c.lanes_log2 > 4) meet([](float x) { return __shfl_xor(x, 16); });
+        if (c.lanes_log2 > 5) meet([](float x) { return __shfl_xor(x, 32); });
 #pragma unroll
         for (int k = 0; k < NR_FLIGHT; ++k) {
             if (h + k >= to) break;
