@@ -5,7 +5,7 @@
 // and the turn are float32, the angle is formed in double; a value is rounded once, to the element type.
 //
 // Bound by HBM, a read and a write of every row: 40 heads of 128 channels, 8192 tokens of a projection's view in bf16 41 us, 4.1 TB/s (a wave a row, read
-// twice: 223); 16 heads of 256, 7 x 1003 tokens, a weight row a head 25.7 us, 4.5 TB/s; one token 5.5, latency.  Four waves a SIMD by a cap on registers: 58 us in place
+// twice: 223); 16 heads of 256, 7 x 1003 tokens, a weight row a head 24.6 us, 4.7 TB/s; one token 5.3, latency.  Four waves a SIMD by a cap on registers: 58 us in place
 // of 41.
 #include "common.hpp"
 
@@ -105,7 +105,7 @@ __device__ __forceinline__ void nr_st(bf16_t *p, float v) { p->bits = __builtin_
 __device__ __forceinline__ void nr_st(float *p, float v) { *p = v; }
 
 // Rows in whole pieces of 16 bytes.  The lanes of a row hold two pieces each, in the half layout a piece and the one that its channels pair with
-// (else half a row apart, so that a load of the lanes is one stretch), so the row is read once: the squares meet in log2(lanes) shuffles, norm and turn are applied to what the lane holds.  A lane keeps the sines
+// (else half a row apart, so that a load of the lanes is one stretch), so the row is read once: the squares meet in log2(lanes) steps, norm and turn are applied to what the lane holds.  A lane keeps the sines
 // and cosines of its pairs at one position and walks over heads, queries then keys; norm weight and turn are one factor a term
 // (w_0 cos, w_1 sin, w_1 cos, w_0 sin), formed once for all heads that share a weight row, and the first rows are asked for ahead of the angles.
 //
