@@ -236,3 +236,20 @@ def test_empty_batch():
     q = torch.zeros((0, 4, 1, 64), dtype=F16, device="cuda")
     z = torch.zeros((0, 2, 3, 64), dtype=F16, device="cuda")
     assert K.select_blocks(q, z, z, 2, levels=3, group_size=32, n_packed=96).shape == (0, 2, 1, 2)
+
+
+@pytest.mark.parametrize("D", [128, 80, 33])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("Sq,query_block", [(1, 1), (6, 6)])
+def test_equal_scores_beside_values_that_are_not_finite(Sq, query_block, dtype, D):
+    """All blocks alike in float32 but a few that are not finite: those first, then the lowest, wherever the former lie."""
+    require_gpu()
+    q, scale, zero = _inputs(3, 8, 4, Sq, D, 100, seed=16, dtype=dtype, meta=F32, spare=0)
+    scale[:], zero[:] = scale[:, :, :1].clone(), zero[:, :, :1].clone()
+    zero[0, :, 50, 3] = float("nan")
+    scale[1, :, 70, 9] = float("nan")
+    zero[2, :, [20, 99], 0] = float("nan")
+    got = _same(q, scale, zero, 6, levels=15, group_size=32, n_packed=3200, query_block=query_block)
+    for b, odd in enumerate(([50], [70], [20, 99])):
+        want = torch.tensor(list(range(6 - len(odd))) + odd, dtype=torch.int32, device="cuda")
+        assert torch.equal(got[b], want.expand(4, 1, 6))

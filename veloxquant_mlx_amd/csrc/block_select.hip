@@ -195,15 +195,19 @@ template <typename T, bool WIDE, int RW> __global__ __launch_bounds__(256) void 
                 }
             }
         }
-        auto take = [&](int r, double x) __attribute__((always_inline)) {
-            x = sum_parts(x, 8);
+        auto take = [&](int r, double x) __attribute__((always_inline)) {   // (the row's score, in each of the group's lanes)
             const int row = r0 + r;
             if (row < rows && u < groups && u * g < sel_end(a, live, pos0 + row / G)) best = max_key(best, pick_key(x));
         };
-        bool odd = false;
+        // A group's score hangs on its own numbers alone: of equal groups none may be rounded another way because its neighbour in the wave is not finite.
+        u32 odd = 0;   // rows whose score is not finite
 #pragma unroll
-        for (int r = 0; r < RW; ++r) odd = odd || !(__builtin_fabs(sum[r]) < (double)INFINITY);
-        if (__any(odd)) {
+        for (int r = 0; r < RW; ++r) {
+            const double x = sum_parts(sum[r], 8);
+            if (__builtin_fabs(x) < (double)INFINITY) take(r, x);
+            else odd |= 1u << r;
+        }
+        if (__any(odd != 0)) {
 #pragma unroll 1
             for (int r = 0; r < RW; ++r) {
                 double s = 0., p = 0.;
@@ -213,11 +217,9 @@ template <typename T, bool WIDE, int RW> __global__ __launch_bounds__(256) void 
                         s = __builtin_fma(y, (double)(float)zero[d], s);
                         p += x <= 0. ? 0. : x;
                     }
-                take(r, __builtin_fma(levels, p, s));
+                const double x = sum_parts(__builtin_fma(levels, p, s), 8);
+                if (odd >> r & 1) take(r, x);
             }
-        } else {
-#pragma unroll
-            for (int r = 0; r < RW; ++r) take(r, sum[r]);
         }
     }
     if (part == 0 && u < groups) c.stored[item * c.groups + u] = best;
