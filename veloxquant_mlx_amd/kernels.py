@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import threading
 
 import torch
 from torch.autograd import forward_ad as _forward_ad
@@ -1000,6 +1001,18 @@ def _workspace(device: torch.device, nbytes: int, stream: int | None = None) -> 
     return ws
 
 
+_scratch_locks: dict[tuple, threading.RLock] = {}
+
+
+def _scratch_lock(device: torch.device, stream: int) -> threading.RLock:
+    """Held from fetching what is kept for a stream (scratch, tiles, counters) until the last launch that uses it is enqueued. Host threads may
+    share a stream, and library calls run without the interpreter's lock: the launches of two calls would mix over one scratch, or one call
+    would replace the scratch that another is about to hand over."""
+    key = (device.type, device.index, stream)
+    lock = _scratch_locks.get(key)
+    return _scratch_locks.setdefault(key, threading.RLock()) if lock is None else lock
+
+
 _tile_scratches: dict[tuple, torch.Tensor] = {}
 _TILE_SCRATCH_MAX = 2 << 30   # bytes; larger inputs are attended without tiles
 
@@ -1259,16 +1272,17 @@ def kivi_packed_attend(q: torch.Tensor, *, k_packed=None, k_scale=None, k_zero=N
         pth, npt = ctypes.c_int(0), ctypes.c_int(0)
         _lib.check(lib.vq_kivi_attend_plan(a, ctypes.byref(pth), ctypes.byref(npt)))
         _plan_out["path"], _plan_out["nparts"] = pth.value, npt.value
-    a.stream = _stream(q)
+    a.stream = stream = _stream(q)
     if static_scratch:
         _lib.check(lib.vq_kivi_attend_static(a))
         return out
     ext = _lib.AttendExt(pair_heads, None if seq_lens is None else seq_lens.data_ptr()) if pair_heads or seq_lens is not None else None
     need = lib.vq_kivi_attend_workspace_ext(a, ext)   # of the call that runs: lengths change its plan
-    ws = _workspace(q.device, need)
-    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
-    a.sync_counters = _counters(q.device).data_ptr() if _single_launch else None
-    _lib.check(lib.vq_kivi_attend_ext(a, ext))
+    with _scratch_lock(q.device, stream):
+        ws = _workspace(q.device, need, stream)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+        a.sync_counters = _counters(q.device, stream).data_ptr() if _single_launch else None
+        _lib.check(lib.vq_kivi_attend_ext(a, ext))
     return out
 
 
@@ -1315,27 +1329,28 @@ def kivi_decode_attend(q, k_packed, k_scale, k_zero, v_packed, v_scale, v_zero, 
     lib = _lib.load()
     device = q.device
     stream = _stream_of(device)
-    ws = _workspace(device, 0, stream)
     order = 0 if fixed_order is None else 1 if fixed_order is True else 2 if fixed_order is False else None
     if order is None:
         return None
-    for _ in range(2):
-        try:
-            args = _lib.ATTEND_PACK.pack(
-                q.data_ptr(), out.data_ptr(), tag, tag, B, Hq, Hkv, 1, D,
-                k_packed.data_ptr(), k_scale.data_ptr(), k_zero.data_ptr(), v_packed.data_ptr(), v_scale.data_ptr(), v_zero.data_ptr(),
-                bits, group_size, VQ_F16 if meta == torch.float16 else VQ_F32, _V_LAYOUT[v_layout], n_packed, cap,
-                k_tail.data_ptr(), v_tail.data_ptr(), tail_tag, n_tail, k_tail.shape[2], scale, 0, num_splits,
-                ws.data_ptr(), ws.numel(), stream, _counters(device, stream).data_ptr(), 0, 0, new_k, new_v, order, sliding_window,
-                0, 0, 0, 0, 0, 0, 0, 0)
-        except (_lib.struct.error, OverflowError):   # a number that the block's fields do not hold as it is
-            return None
-        rc = lib.attend_packed(args, ext)
-        if rc == 0:
-            return out
-        if rc != _lib.VQ_ERR_WORKSPACE:
-            break
-        ws = _workspace(device, lib.attend_packed_workspace(args, ext), stream)
+    with _scratch_lock(device, stream):
+        ws = _workspace(device, 0, stream)
+        for _ in range(2):
+            try:
+                args = _lib.ATTEND_PACK.pack(
+                    q.data_ptr(), out.data_ptr(), tag, tag, B, Hq, Hkv, 1, D,
+                    k_packed.data_ptr(), k_scale.data_ptr(), k_zero.data_ptr(), v_packed.data_ptr(), v_scale.data_ptr(), v_zero.data_ptr(),
+                    bits, group_size, VQ_F16 if meta == torch.float16 else VQ_F32, _V_LAYOUT[v_layout], n_packed, cap,
+                    k_tail.data_ptr(), v_tail.data_ptr(), tail_tag, n_tail, k_tail.shape[2], scale, 0, num_splits,
+                    ws.data_ptr(), ws.numel(), stream, _counters(device, stream).data_ptr(), 0, 0, new_k, new_v, order, sliding_window,
+                    0, 0, 0, 0, 0, 0, 0, 0)
+            except (_lib.struct.error, OverflowError):   # a number that the block's fields do not hold as it is
+                return None
+            rc = lib.attend_packed(args, ext)
+            if rc == 0:
+                return out
+            if rc != _lib.VQ_ERR_WORKSPACE:
+                break
+            ws = _workspace(device, lib.attend_packed_workspace(args, ext), stream)
     if rc != _lib.VQ_ERR_INVALID and rc != _lib.VQ_ERR_UNSUPPORTED:
         _lib.check(rc)
     return None
@@ -1565,9 +1580,10 @@ def _scratch_call(device, stream, call, room, block):
         # stream is given back when a larger one replaces it
         need = room(block(None, True))
         return call(block(torch.empty(need, dtype=torch.uint8, device=device) if need else None, True))
-    rc = call(block(_workspace(device, 0, stream), False))
-    if rc == _lib.VQ_ERR_WORKSPACE:
-        rc = call(block(_workspace(device, room(block(None, False)), stream), False))
+    with _scratch_lock(device, stream):
+        rc = call(block(_workspace(device, 0, stream), False))
+        if rc == _lib.VQ_ERR_WORKSPACE:
+            rc = call(block(_workspace(device, room(block(None, False)), stream), False))
     return rc
 
 
@@ -2074,9 +2090,12 @@ def vecinfer_attend_indices(q: torch.Tensor, k_indices: torch.Tensor, k_codebook
     if need == 0:
         return None
     out = torch.empty_like(q)
-    ws = _workspace(q.device, need)
-    a.out, a.workspace, a.workspace_bytes, a.stream = out.data_ptr(), ws.data_ptr(), ws.numel(), _stream(q)
-    _lib.check(lib.vq_vecinfer_attend_indices(C.byref(a)))
+    stream = _stream(q)
+    a.out, a.stream = out.data_ptr(), stream
+    with _scratch_lock(q.device, stream):
+        ws = _workspace(q.device, need, stream)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+        _lib.check(lib.vq_vecinfer_attend_indices(C.byref(a)))
     return out
 
 
@@ -2148,10 +2167,11 @@ def metal_fused_sdpa(q_tilde: torch.Tensor, k_indices: torch.Tensor, k_codebook:
     need = lib.vq_vecinfer_attend_workspace(C.byref(a))
     if need == 0:
         _lib.check(lib.vq_vecinfer_attend(C.byref(a)))   # raises with the validation message
-    ws = _workspace(q.device, need)
-    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
-    a.stream = _stream(q)
-    _lib.check(lib.vq_vecinfer_attend(C.byref(a)))
+    a.stream = stream = _stream(q)
+    with _scratch_lock(q.device, stream):
+        ws = _workspace(q.device, need, stream)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+        _lib.check(lib.vq_vecinfer_attend(C.byref(a)))
     return out
 
 
