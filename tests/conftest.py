@@ -14,9 +14,16 @@ def pytest_configure(config):
 
 
 @pytest.fixture(autouse=True)
-def _random_numbers():
-    """What a test draws without a seed of its own is the same in every run (which rows of a sink-protecting cache are protected hangs on it)."""
-    torch.manual_seed(0)
+def _seeded_draw(request):
+    """``test_protected_rows_of_an_emptied_cache_are_forgotten`` draws its keys without a seed and expects side rows, which are there only if one of the two
+    tokens of the largest mean norm lies below the packed boundary (32 of 70): 38 * 37 / (70 * 69), three draws in ten, have none. It draws the
+    same keys in every run; no other test's numbers are touched."""
+    if request.node.name.startswith("test_protected_rows_of_an_emptied_cache_are_forgotten"):
+        with torch.random.fork_rng(devices=[]):
+            torch.random.default_generator.manual_seed(0)
+            yield
+    else:
+        yield
 
 
 @pytest.fixture
