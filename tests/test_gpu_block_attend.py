@@ -314,3 +314,39 @@ def test_calls_under_way_on_two_streams(D, bits, dtype):
         torch.cuda.synchronize()
         for (a, b), (c, d) in zip(got, want):
             assert torch.equal(a, c) and torch.equal(b, d)
+
+
+@pytest.mark.parametrize("bits,dtype", [(4, F16), (2, BF16)])
+@pytest.mark.parametrize("Hq,D,total,n", [(1, 64, 700, 650), (2, 64, 1100, 1000), (1, 128, 1100, 1000)])
+def test_more_parts_than_a_round_of_the_sum(Hq, D, total, n, bits, dtype):
+    """One list over 650 units or more, in more than 32 parts, which the block that ends last adds up in rounds of 32."""
+    require_gpu()
+    parts = -(-(n + 1) // 16)       # (a list's units and the tail's one, in runs of 16)
+    assert parts > 32 and Hq * parts * D * 4 <= 32 * 1024
+    q, s, blocks, got = _case(1, Hq, 1, D, (total * 32, 5), 32, n, bits=bits, dtype=dtype, seed=21)
+    kw = dict(block_size=32, scale=D ** -0.5, causal=True)
+    graph = torch.cuda.CUDAGraph()      # (parts added up by a launch of their own)
+    with torch.cuda.graph(graph):
+        other = K.block_sparse_attend(q, blocks, **s, **kw)
+    for _ in range(3):
+        other.zero_()
+        graph.replay()
+        assert float((other.float() - got.float()).abs().max()) <= 2 * torch.finfo(dtype).eps * float(got.float().abs().max())
+    # the last parts, and all but the first, hold nothing that is seen
+    for live in (total * 16, 40, 3):
+        _case(1, Hq, 1, D, (total * 32, 5), 32, n, bits=bits, dtype=dtype, seed=21, lens=[live])
+
+
+@pytest.mark.parametrize("D,bits,dtype", [(128, 4, F16), (128, 2, BF16), (256, 4, F16), (64, 4, F16), (128, 8, F16), (128, 4, F32)])
+@pytest.mark.parametrize("Sq,query_block", [(1, 1), (20, 6)])
+def test_all_blocks_are_the_whole_store(Sq, query_block, D, bits, dtype):
+    """Lists of all blocks: attention over the whole store, each as far from 64 bits as its roundings go."""
+    require_gpu()
+    every = torch.arange(8, dtype=torch.int32, device="cuda").expand(3, 2, -(-Sq // query_block), 8).contiguous()
+    q, s, _, got = _case(3, 8, 2, D, (512, 77), 64, 8, Sq, query_block, bits=bits, dtype=dtype, view=True, seed=22, blocks=every)
+    whole = K.shared_prefix_attend(q, None, **s, scale=D ** -0.5, causal=True)
+    _, k, v = store(3, 2, 512, 77, D, bits=bits, dtype=dtype, spare=40, view=True, seed=23)      # (the case's)
+    times = times_seen(every, 64, query_block, 3, Sq, 512, 77, None, True)
+    want, far = attend(q, k, v, times, D ** -0.5, 0.0 if dtype == F32 else 2.0 ** -11)
+    close(whole, want, far)
+    assert bool(((got.double() - whole.double()).abs() <= 2 * (far * (1 + 2.0 ** -8) + torch.finfo(dtype).eps / 2 * want.abs() + 1e-6)).all())

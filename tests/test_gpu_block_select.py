@@ -253,3 +253,47 @@ def test_equal_scores_beside_values_that_are_not_finite(Sq, query_block, dtype, 
     for b, odd in enumerate(([50], [70], [20, 99])):
         want = torch.tensor(list(range(6 - len(odd))) + odd, dtype=torch.int32, device="cuda")
         assert torch.equal(got[b], want.expand(4, 1, 6))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("groups", [60, 300])
+def test_more_tiles_than_compute_units(groups, D, dtype):
+    """280 tiles of up to 32 rows: one launch, of four waves a tile."""
+    require_gpu()
+    q, scale, zero = _inputs(2, 8, 2, 70, D, groups, dtype=dtype, seed=17 + D)
+    for causal in (True, False):
+        _same(q, scale, zero, 7, levels=15, group_size=32, n_packed=groups * 32, n_tail=30, first=1, recent=1, causal=causal)
+    lens = torch.tensor([groups * 32 - 50, 40], device="cuda")
+    _same(q, scale, zero, 7, levels=15, group_size=32, n_packed=groups * 32 - 3, n_tail=30, block_size=64, recent=2, causal=True, seq_lens=lens)
+
+
+@pytest.mark.parametrize("dtype,D", [(F16, 128), (BF16, 128), (BF16, 64), (F16, 256)])
+@pytest.mark.parametrize("B,Hq,Hkv,Sq,query_block,groups", [(4, 32, 8, 64, 16, 300), (2, 16, 2, 144, 16, 1000), (2, 24, 2, 9, 3, 33)])
+def test_runs_of_many_units(B, Hq, Hkv, Sq, query_block, groups, dtype, D):
+    """Two row tiles a tile or more, and (but in the last case) waves that walk two or three units of 32 groups each."""
+    require_gpu()
+    items, row_tiles, units = B * Hkv * -(-Sq // query_block), -(-Hq // Hkv * query_block // 32), -(-groups // 32)
+    assert row_tiles >= 2 and (groups == 33 or items * row_tiles * units > 2048)
+    q, scale, zero = _inputs(B, Hq, Hkv, Sq, D, groups, dtype=dtype, seed=18, signed=D == 64)
+    _same(q, scale, zero, 6, levels=15, group_size=32, n_packed=groups * 32 - 7, n_tail=40, query_block=query_block, first=1, recent=1, causal=True)
+
+
+@pytest.mark.parametrize("dtype,meta,D", [(F16, F16, 64), (F32, F32, 33), (BF16, F32, 128)])
+@pytest.mark.parametrize("Sq,query_block", [(1, 1), (3, 2)])
+def test_more_blocks_than_lds_holds(Sq, query_block, dtype, meta, D):
+    """More than 16384 blocks: a choice by scores in memory."""
+    require_gpu()
+    groups = 16500
+    q, scale, zero = _inputs(3, 4, 2, Sq, D, groups, dtype=dtype, meta=meta, seed=19)
+    zero[0, 1, 16400, 3] = float("nan")
+    zero[0, 0, 9000:9100], scale[0, 0, 9000:9100] = zero[0, 0, 77].clone(), scale[0, 0, 77].clone()       # a hundred alike
+    scale[2, :, :groups], zero[2, :, :groups] = scale[2, :, :1].clone(), zero[2, :, :1].clone()     # all alike
+    kw = dict(levels=15, group_size=8, n_packed=groups * 8, n_tail=5, query_block=query_block, causal=True)
+    got = _same(q, scale, zero, 40, **kw)
+    assert 16400 in got[0, 1, 0].tolist()
+    assert torch.equal(got[2, 0, 0], torch.arange(40, dtype=torch.int32, device="cuda"))
+    lens = torch.tensor([16390 * 8 + 3, 16 * 8, 200], device="cuda")
+    _same(q, scale, zero, 40, first=2, recent=3, seq_lens=lens, **kw)
+    # two groups a block: as many blocks need twice the groups, so fewer blocks than that, told apart in LDS again
+    _same(q, scale, zero, 9, **dict(kw, block_size=16))
