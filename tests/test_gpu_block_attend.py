@@ -350,3 +350,28 @@ def test_all_blocks_are_the_whole_store(Sq, query_block, D, bits, dtype):
     want, far = attend(q, k, v, times, D ** -0.5, 0.0 if dtype == F32 else 2.0 ** -11)
     close(whole, want, far)
     assert bool(((got.double() - whole.double()).abs() <= 2 * (far * (1 + 2.0 ** -8) + torch.finfo(dtype).eps / 2 * want.abs() + 1e-6)).all())
+
+
+@pytest.mark.parametrize("S", [20, 200])
+@pytest.mark.parametrize("memory_bound", [True, False])
+def test_a_cache_refuses_the_same_with_and_without_packed_tokens(S, memory_bound):
+    require_gpu()
+    cache = KVCacheFactory.create(KVCacheConfig(method="kivi", head_dim=128, bit_width_inlier=4, kivi_group_size=32, residual_length=64, fused_sdpa=True,
+                                                fused_sdpa_memory_bound=memory_bound))
+    g = torch.Generator(device="cuda").manual_seed(24)
+    k, q = (torch.randn((2, h, S, 128), generator=g, device="cuda").half() for h in (2, 4))
+    cache.update_and_fetch(k, k)
+    assert (cache._n_quantized > 0) == (S == 200)
+    q = q[:, :, :5].contiguous()
+    for bad in (dict(query_block=0), dict(n_select=0), dict(n_select=-1), dict(block_size=48), dict(first=-1), dict(first=3, recent=2), dict(recent=-2)):
+        kw = dict(dict(n_select=4, query_block=2), **bad)
+        with pytest.raises(ValueError, match="select_blocks: "):
+            cache.select_blocks(q, **kw)
+        with pytest.raises(ValueError, match="select_blocks: |fused_sparse_sdpa: "):
+            cache.fused_sparse_sdpa(q, 0.1, **kw)
+    for rows in (q[:1], q[:, :3], q[..., :64].contiguous()):     # another batch, heads over no kv head, other channels
+        with pytest.raises(ValueError, match="select_blocks: "):
+            cache.select_blocks(rows, 4)
+    got = cache.select_blocks(q, 4, query_block=2)
+    assert got.shape == (2, 2, 3, 4) and got.dtype == torch.int32 and (S == 200 or bool((got == -1).all()))
+    assert torch.equal(cache.select_blocks(q, 4, query_block=2, lengths=[S, S]), got)

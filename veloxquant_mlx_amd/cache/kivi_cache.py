@@ -538,12 +538,13 @@ class KIVIKVCache(FP16KVCache):
         name = f"{type(self).__name__}.select_blocks"
         self._sparse_ready(name)
         nq = self._n_quantized
-        if nq == 0:
-            B, H, _ = self._shape_bhd
-            return torch.full((B, H, -(-q.shape[2] // int(query_block)), int(n_select)), -1, dtype=torch.int32, device=q.device)
         if lengths is not None:
             lengths = batch_lengths(name, lengths, q)
-        return K.select_blocks(q, self._ks, self._kz, n_select, levels=self._levels, group_size=self._group_size, n_packed=nq,
+        ks, kz = self._ks, self._kz
+        if nq == 0:   # (no groups yet: nothing is listed)
+            B, H, D = self._shape_bhd
+            ks = kz = q.new_empty((B, H, 0, D), dtype=self._meta_dtype)
+        return K.select_blocks(q, ks, kz, n_select, levels=self._levels, group_size=self._group_size, n_packed=nq,
                                n_tail=self.offset - nq, block_size=block_size, query_block=query_block, first=first, recent=recent,
                                causal=bool(causal), seq_lens=lengths)
 
