@@ -607,7 +607,8 @@ int vq_differential_attend(const vq_store_attend_args *a);
  * Query i of Sq stands at slot n - Sq + i of the sequence's n live slots (n_packed + n_tail, or seq_lens); causal hides the slots
  * behind it.  Of the blocks that the tile's last query sees all are chosen if they are `count` at most; else the first `first`, the
  * last `recent` and the best of the others.  Scores are formed in 64 bits, equal ones go to the lower block, NaN above all.  out:
- * int32 [B, Hkv, tiles, count], ascending, -1 behind the chosen where fewer are visible.  No counterpart in the reference. */
+ * int32 [B, Hkv, tiles, count], ascending, -1 behind the chosen where fewer are visible.  Fewer than 2^24 query rows, 2^23 tiles and 2^26 (tile, group) scores
+ * a call.  No counterpart in the reference. */
 typedef struct vq_block_select_args {
     const void *q;                     /* [B, Hq, Sq, D] contiguous, dtype; D <= 256 */
     const void *k_scale, *k_zero;      /* [B, Hkv, ceil(cap_tokens / group), D], meta_dtype VQ_F16 / VQ_F32 */

@@ -375,3 +375,11 @@ def test_a_cache_refuses_the_same_with_and_without_packed_tokens(S, memory_bound
     got = cache.select_blocks(q, 4, query_block=2)
     assert got.shape == (2, 2, 3, 4) and got.dtype == torch.int32 and (S == 200 or bool((got == -1).all()))
     assert torch.equal(cache.select_blocks(q, 4, query_block=2, lengths=[S, S]), got)
+
+
+def test_more_tiles_of_rows_than_a_grid_holds():
+    """65600 queries that choose singly: taken in float32."""
+    require_gpu()
+    q, s, blocks, got = _case(1, 1, 1, 64, (128, 3), 32, 2, 65600, bits=4, causal=False, seed=25)
+    few = K.block_sparse_attend(q[:, :, :100].contiguous(), blocks[:, :, :100].contiguous(), **s, block_size=32, scale=64 ** -0.5)
+    assert float((few.double() - got[:, :, :100].double()).abs().max()) <= 2.0 ** -9 * float(got.abs().max())

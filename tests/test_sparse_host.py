@@ -192,3 +192,14 @@ def test_caches_that_cannot_choose():
         empty = KVCacheFactory.create(KVCacheConfig(head_dim=128, fused_sdpa=True, **base))
         with pytest.raises(RuntimeError, match="before any tokens"):
             call(empty)
+
+
+def test_sizes_past_one_call_are_refused():
+    """The limits that the documentation names; each refusal comes ahead of any launch."""
+    lib = _lib.load()
+    many = dict(B=1, Hq=8, Hkv=8, n_packed=32768, cap_tokens=32768, block_tokens=32)
+    assert lib.vq_block_select(_select(**many, Sq=8192)) == _lib.VQ_ERR_UNSUPPORTED and "scores" in _lib.last_error()
+    assert lib.vq_block_select_workspace(_select(**many, Sq=8191)) > 0 and lib.vq_block_select_workspace(_select(**many, Sq=8192, query_block=2)) > 0
+    assert lib.vq_block_select(_select(B=1, Hq=1, Hkv=1, Sq=1 << 23, n_packed=32)) == _lib.VQ_ERR_UNSUPPORTED and "scores" in _lib.last_error()
+    assert lib.vq_block_select(_select(B=1, Hq=2, Hkv=1, Sq=1 << 23, n_packed=32)) == _lib.VQ_ERR_UNSUPPORTED and "query rows" in _lib.last_error()
+    assert lib.vq_norm_rotary(_norm(D=7, dims=6, S=1 << 25), None) == _lib.VQ_ERR_UNSUPPORTED and "rows" in _lib.last_error()      # two heads

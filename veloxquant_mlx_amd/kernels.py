@@ -1734,7 +1734,11 @@ def select_blocks(q: torch.Tensor, k_scale: torch.Tensor, k_zero: torch.Tensor, 
     (int64 ``[B]`` on the device) a sequence has only that many live ones of both.  Queries align to the end of a sequence; ``causal`` hides
     the slots behind a query's own position, and a block is visible if its first slot is.  If the tile's last query sees ``n_select``
     blocks or fewer, those are all chosen; else the first ``first``, the last ``recent`` and the best of the others.  Scores are formed in
-    64 bits, so the choice does not depend on the order of a sum; of equal ones the lower block is taken, NaN counts above all."""
+    64 bits, so the choice does not depend on the order of a sum; of equal ones the lower block is taken, NaN counts above all.
+
+    One call takes fewer than 2^24 query rows (``B * Hq * Sq``), 2^23 tiles and 2^26 scores (``B * Hkv * tiles * groups`` of the packed slots: 8192 queries that
+    choose singly over 8 kv heads and 32k slots in groups of 32 are past that); larger ones are refused, and can be made in parts of the queries (with ``seq_lens``) or with a larger
+    ``query_block``."""
     name = "select_blocks"
     if q.ndim != 4 or k_scale.ndim != 4:
         raise ValueError(f"{name}: q must be [B, Hq, Sq, D] and k_scale [B, Hkv, groups, D], got {tuple(q.shape)} and {tuple(k_scale.shape)}")
@@ -1803,8 +1807,9 @@ def block_sparse_attend(q: torch.Tensor, blocks: torch.Tensor, *, block_size: in
     ``causal``, not behind the query.  Entries may come in any order; one below zero or past the live slots names nothing, one that is
     named twice counts twice.  The plain rows of the tail are all seen, up to the query's own.  Slots that no list names are not read;
     live values have to be finite, what lies behind the live slots may be anything.  A row that sees nothing is zero.  Numbers as for :func:`shared_prefix_attend`.  2- and 4-bit stores with heads of 64, 128 or 256 channels, groups
-    of 32, 64 or 128 and values packed by token run on the matrix units where blocks are whole units of 32 slots; other stores, sizes and float32 rows
-    in float32, some ten times slower."""
+    of 32, 64 or 128 and values packed by token run on the matrix units where blocks are whole units of 32 slots: weights are rounded to fp16 there, bf16 queries
+    and tail rows count as fp16 numbers (magnitudes above 65504 as 65504, below 2^-14 in steps of 2^-24). Other stores and sizes, float32 rows, and more than 65535 tiles of rows
+    (32 query rows of a kv head at the positions of one list) run in float32, some ten times slower."""
     own = (k_packed, k_scale, k_zero, v_packed, v_scale, v_zero, n_packed, bits, group_size, v_layout, k_tail, v_tail, n_tail)
     return _store_attend("block_sparse_attend", 0, q, None, own, scale, causal, seq_lens, 0, out, lists=(blocks, int(block_size), int(query_block)))
 
@@ -1894,7 +1899,8 @@ def norm_rotary_embed(q: torch.Tensor, k: torch.Tensor | None = None, *, q_weigh
 
     ``q_weight``, ``k_weight``: ``[D]``, or a row a head (``[Hq, D]``, ``[Hk, D]``), float16, bfloat16 or float32, both of one dtype; None: ones.
     Squares, their sum, the norm and the turn are float32, with one rounding at the end.  The other arguments, strides and outputs as for
-    :func:`rotary_embed`."""
+    :func:`rotary_embed`.  Rows that are not whole pieces of 16 bytes, aligned and uncut by the pairs, or whose weights (a row a head) are of another type or
+    given for one of the two alone, are read twice, at a seventh of the speed, and fewer than 2^26 of them (``B * S`` times all heads) a call."""
     name = "norm_rotary_embed"
     if not 0 <= norm_eps < 1e38:
         raise ValueError(f"{name}: norm_eps={norm_eps} must be a number from 0 on")
