@@ -17,8 +17,8 @@ namespace {
 // (v_mfma_f32_16x16x4: lane i + 16 h holds row or column i of step h, and rows 4 h .. 4 h + 3 of column i of the result; a lane's four channels or
 // slots in a row are those of four steps, any order serving a sum), the softmax has TPR threads a row.
 //
-// Bound by the latencies of a unit, one after another (its entries of the list, then its words in four batches, five barriers), with two blocks a CU to
-// cover each other: 16 sequences of 8 kv heads, 3.2k of 8-bit slots each, 214 us; a chunk of 512 queries in 64 lists of 2k slots 682 (a wave a row,
+// Bound by the latencies of a unit, one after another (its entries of the list, then its words in four batches, five barriers), with two blocks a CU (one
+// past 192 channels with 32 rows, past 224 with 16: LDS) to cover each other: 16 sequences of 8 kv heads, 3.2k of 8-bit slots each, 214 us; a chunk of 512 queries in 64 lists of 2k slots 682 (a wave a row,
 // each with its own reconstruction: 1891 and 33827).  Eight slots' words under way in place of four take registers that the second block needs (1080);
 // a third of the loads, keys' scales shared and values' by way of LDS, is no faster (248 and 722).
 constexpr int ANY_SP = 36;          // floats from row to row of the scores
@@ -283,7 +283,7 @@ bool plan_few(BlockCall &c, const vq_block_attend_args &args) {
     c.s.ofew = 1;
     c.s.owaves = 4;
     c.s.osplits = c.s.nparts = (int)splits;
-    // Parts are added up in the launch where a tile's are 32 KB at most, which the one block that does it reads past its caches at ~20 GB/s (4 rows of 128
+    // Parts are added up in the launch where a tile's are 32 KB at most, which the one block that does it reads past its caches at 9 to 14 GB/s (4 rows of 128
     // channels in nine parts, 18 KB: 1.9 us; 9 rows of 256 in eleven, 99 KB: 7.5, and a launch of its own 4 to 5)
     const int64_t rows = a.Hq / a.Hkv * qb < 32 ? a.Hq / a.Hkv * qb : 32;
     const bool join = splits > 1 && items <= args.counters_len && rows * splits * a.D * 4 <= 32 * 1024;
