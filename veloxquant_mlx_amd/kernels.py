@@ -993,7 +993,7 @@ _workspaces: dict[tuple, torch.Tensor] = {}
 
 
 def _workspace(device: torch.device, nbytes: int, stream: int | None = None) -> torch.Tensor:
-    key = (device.type, device.index, _stream_of(device) if stream is None else stream)
+    key = (device.index, _stream_of(device) if stream is None else stream)
     ws = _workspaces.get(key)
     if ws is None or ws.numel() < nbytes:
         ws = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
@@ -1008,7 +1008,7 @@ def _scratch_lock(device: torch.device, stream: int) -> threading.RLock:
     """Held from fetching what is kept for a stream (scratch, tiles, counters) until the last launch that uses it is enqueued. Host threads may
     share a stream, and library calls run without the interpreter's lock: the launches of two calls would mix over one scratch, or one call
     would replace the scratch that another is about to hand over."""
-    key = (device.type, device.index, stream)
+    key = (device.index, stream)
     lock = _scratch_locks.get(key)
     return _scratch_locks.setdefault(key, threading.RLock()) if lock is None else lock
 
@@ -1043,7 +1043,7 @@ _block_counters: dict[tuple, torch.Tensor] = {}   # of attention over chosen blo
 def _counters(device: torch.device, stream: int | None = None, table: dict = _sync_counters) -> torch.Tensor:
     """Per-(device, stream) int32 counters the single-launch decode path needs: zero when a
     call is enqueued, left zero by it (65536 = the largest B*H_kv the MFMA path takes)."""
-    key = (device.type, device.index, _stream_of(device) if stream is None else stream)
+    key = (device.index, _stream_of(device) if stream is None else stream)
     c = table.get(key)
     if c is None:
         c = torch.zeros(65536, dtype=torch.int32, device=device)
